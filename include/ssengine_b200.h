@@ -191,6 +191,17 @@ int ssb_kda_prefill_ws(const ssb_kda_layer* layer, const void* x, int64_t ldx, c
                        const void* beta, int64_t ldb, int64_t T, const int32_t* seqs, int64_t R, void* out,
                        int64_t ldo, void* workspace, int64_t ws_bytes, int32_t* status, void* stream);
 
+/* The recurrent form of the same layer over short runs of new tokens (a decode step: one token a request; drafts or a
+ * few tokens: any length, one after the other): arguments, sequence table and state blocks as ssb_kda_prefill_ws, so a
+ * request may move between the two forms at any token. q, k, v and everything up to the bf16 output stay in fp32 (the
+ * prefill form rounds the conv outputs to bf16). No workspace; one launch. x, g, conv state 4-byte aligned with even
+ * pitches, recurrent state 16-byte aligned (block stride % 4 == 0). Sequences that reach outside [0, T) or name a
+ * negative block are skipped with status 1, sequences without rows leave their blocks as they are; the blocks named by
+ * one call must be distinct. */
+int ssb_kda_decode(const ssb_kda_layer* layer, const void* x, int64_t ldx, const void* g, int64_t ldg,
+                   const void* beta, int64_t ldb, int64_t T, const int32_t* seqs, int64_t R, void* out, int64_t ldo,
+                   int32_t* status, void* stream);
+
 /* The short conv alone: q, k, v bf16 [T, H * 128] each (contiguous) and the conv state blocks updated; rows outside
  * every sequence are written as 0. Replaces `kda_conv.conv_qkv` (ssengine/model/kda_conv.py:146-164). */
 int ssb_kda_conv(const ssb_kda_layer* layer, const void* x, int64_t ldx, int64_t T, const int32_t* seqs, int64_t R,
@@ -262,6 +273,26 @@ int ssb_indexer_expand(const int32_t* pool_ids, int64_t ldp, int32_t k, const in
 int ssb_sparse_mla(const void* q, int64_t T, const void* kv_cache, const int32_t* indices, int64_t ld_idx,
                    int32_t n_idx, const int32_t* qsl, int32_t R, const int32_t* page_table, int64_t width,
                    float bmm1_scale, float bmm2_scale, void* out, int32_t* status, void* stream);
+
+/* Latent attention of new tokens (a decode step) over the paged FP8 cache, split over each row's tokens and joined:
+ * out bf16 [T, heads, 512] = bmm2_scale * softmax(bmm1_scale * q . kv) kv[:, 0:512] as ssb_sparse_mla, for 1..128 heads.
+ * q [T, heads, 576] bf16 (q_e4m3 = 0: its values enter exactly, up to 2^-22 of the head's largest) or e4m3 (1), row
+ * stride ldq and head_stride in elements (16-byte multiples). Query row t belongs to row reqs[t] of page_table int32
+ * [R, width] (reqs NULL: row t; several rows may share one, e.g. draft tokens) and sees positions 0 .. seq_lens[t] - 1,
+ * or, with indices int32 [T, ld_idx], the first n_idx listed positions (-1 = none; at or past seq_lens[t], when that is
+ * given: none; a position listed twice counts twice). Tokens of a negative page, past the table or past cache_rows are
+ * left out. A row with no token gets zeros and lse -inf; a reqs entry outside [0, R) the same, with status 1. lse (fp32
+ * [T, heads] or NULL) = the natural log of the sum of the row's weights. workspace: 256-byte aligned,
+ * ssb_mla_decode_workspace_bytes(T, heads) or more (returns 3 when smaller), its contents need not be kept. The lengths
+ * are read on the device: the call can be captured in a graph and replayed as they grow. */
+int ssb_mla_decode(const void* q, int32_t q_e4m3, int64_t ldq, int64_t head_stride, int64_t T, int32_t heads,
+                   const void* kv_cache, int64_t cache_rows, const int32_t* page_table, int64_t R, int64_t width,
+                   const int32_t* reqs, const int32_t* seq_lens, const int32_t* indices, int64_t ld_idx,
+                   int32_t n_idx, float bmm1_scale, float bmm2_scale, void* out, float* lse, void* workspace,
+                   int64_t ws_bytes, int32_t* status, void* stream);
+
+/* Device bytes of the workspace of ssb_mla_decode; -1 on bad arguments. */
+int64_t ssb_mla_decode_workspace_bytes(int64_t T, int32_t heads);
 
 /* MLA cache append: row t of src bf16 [T, 576] (row pitch lds elements, % 8 == 0) into kv_cache row slots[t] (int64,
  * skipped when < 0) as e4m3(x / k_scale), round to nearest even, saturating to +-448 (576 bytes a row). Replaces the

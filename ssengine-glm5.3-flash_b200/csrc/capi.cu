@@ -303,6 +303,22 @@ int ssb_kda_prefill(const ssb_kda_layer* layer, const void* x, int64_t ldx, cons
   return ssb_kda_prefill_ws(layer, x, ldx, g, ldg, beta, ldb, T, seqs, R, out, ldo, nullptr, 0, status, stream);
 }
 
+int ssb_kda_decode(const ssb_kda_layer* layer, const void* x, int64_t ldx, const void* g, int64_t ldg,
+                   const void* beta, int64_t ldb, int64_t T, const int32_t* seqs, int64_t R, void* out, int64_t ldo,
+                   int32_t* status, void* stream) {
+  ssb::KdaArgs a;
+  if (T < 0 || !kda_args(layer, x, ldx, seqs, R, a)) return kErrArgs;
+  a.g = static_cast<const __nv_bfloat16*>(g);
+  a.ldg = ldg;
+  a.beta = static_cast<const __nv_bfloat16*>(beta);
+  a.ldb = ldb;
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.ldo = ldo;
+  a.status = status;
+  a.T = T;
+  return ssb::launch_kda_decode(a, static_cast<cudaStream_t>(stream));
+}
+
 int64_t ssb_kda_workspace_bytes(int32_t heads, int64_t T, int64_t R) {
   if (heads <= 0 || T < 0 || R < 0 || R > (1 << 30)) return -1;
   return ssb::kda_workspace_bytes(heads, T, static_cast<int>(R));
@@ -381,6 +397,42 @@ int ssb_sparse_mla(const void* q, int64_t T, const void* kv_cache, const int32_t
   a.T = T;
   a.status = status;
   return ssb::launch_sparse_mla(a, static_cast<cudaStream_t>(stream));
+}
+
+int64_t ssb_mla_decode_workspace_bytes(int64_t T, int32_t heads) {
+  if (T < 0 || T > 0x7fffffff || heads <= 0 || heads > 128) return -1;
+  return ssb::mla_decode_workspace_bytes(T, heads);
+}
+
+int ssb_mla_decode(const void* q, int32_t q_e4m3, int64_t ldq, int64_t head_stride, int64_t T, int32_t heads,
+                   const void* kv_cache, int64_t cache_rows, const int32_t* page_table, int64_t R, int64_t width,
+                   const int32_t* reqs, const int32_t* seq_lens, const int32_t* indices, int64_t ld_idx,
+                   int32_t n_idx, float bmm1_scale, float bmm2_scale, void* out, float* lse, void* workspace,
+                   int64_t ws_bytes, int32_t* status, void* stream) {
+  if (width <= 0 || width > (1 << 24) || R <= 0 || R > (1 << 28) || (q_e4m3 != 0 && q_e4m3 != 1)) return kErrArgs;
+  ssb::MlaDecodeArgs a;
+  a.q = q;
+  a.q_e4m3 = q_e4m3;
+  a.ldq = ldq;
+  a.hsq = head_stride;
+  a.T = T;
+  a.H = heads;
+  a.kv = static_cast<const uint8_t*>(kv_cache);
+  a.cache_rows = cache_rows;
+  a.table = page_table;
+  a.R = static_cast<int32_t>(R);
+  a.width = static_cast<int32_t>(width);
+  a.reqs = reqs;
+  a.seq_lens = seq_lens;
+  a.indices = indices;
+  a.ld_idx = ld_idx;
+  a.n_idx = n_idx;
+  a.bmm1 = bmm1_scale;
+  a.bmm2 = bmm2_scale;
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.lse = lse;
+  a.status = status;
+  return ssb::launch_mla_decode(a, workspace, ws_bytes, static_cast<cudaStream_t>(stream));
 }
 
 int ssb_mla_cache_append(const void* src, int64_t lds, const int64_t* slots, int64_t T, void* cache, float k_scale,

@@ -138,6 +138,8 @@ struct KdaArgs {
   int64_t ws_slots = 0;                // chunk slots the workspace holds (set by the launcher)
 };
 int64_t kda_workspace_bytes(int H, int64_t T, int R);
+// The recurrent form over short runs of new tokens (csrc/kda_decode.cu); the workspace fields are not used.
+int launch_kda_decode(const KdaArgs& a, cudaStream_t stream);
 int launch_kda_prefill(const KdaArgs& a, cudaStream_t stream);
 
 // 2D tensor map (no swizzle) over [rows, width] elements of `dtype` (a CUtensorMapDataType) with row pitch ld_bytes;
@@ -199,6 +201,36 @@ int launch_mla_append(const void* src, int64_t lds, const int64_t* slots, int64_
                       cudaStream_t stream);
 int launch_mla_q_pack(const void* lat, int64_t rows_pad, const void* rope, int64_t ldr, int64_t rope_stride,
                       int64_t T, void* q8, float q_scale, cudaStream_t stream);
+
+// Latent attention of new tokens over the paged cache (csrc/mla_decode.cu).
+struct MlaRowParts {                   // which ranges a row was cut into: CTAs first .. last, the first one's part slot
+  int32_t first, last, first_slot, pad;
+};
+struct MlaDecodeArgs {
+  const void* q = nullptr;             // [T, H, 576] bf16 or e4m3, strides in elements
+  int32_t q_e4m3 = 0;
+  int64_t ldq = 0, hsq = 0;            // row and head stride
+  int64_t T = 0;
+  int32_t H = 0;                       // 1 .. 128
+  const uint8_t* kv = nullptr;         // e4m3 latent cache [cache_rows, 576]
+  int64_t cache_rows = 0;
+  const int32_t* table = nullptr;      // [R, width] KV pages (128 tokens), negative: missing
+  int32_t R = 0, width = 0;
+  const int32_t* reqs = nullptr;       // [T] table row of each query row (null: row t)
+  const int32_t* seq_lens = nullptr;   // [T] visible tokens (null with indices: every listed token)
+  const int32_t* indices = nullptr;    // [T, ld_idx] selected positions, -1 = none (null: all visible tokens)
+  int64_t ld_idx = 0;
+  int32_t n_idx = 0;
+  float bmm1 = 0.0f, bmm2 = 1.0f;
+  __nv_bfloat16* out = nullptr;        // [T, H, 512]
+  float* lse = nullptr;                // [T, H] or null
+  int32_t* status = nullptr;
+  MlaRowParts* rows = nullptr;         // workspace (set by the launcher)
+  float2* part_ml = nullptr;
+  float* part_o = nullptr;
+};
+int64_t mla_decode_workspace_bytes(int64_t T, int H);
+int launch_mla_decode(const MlaDecodeArgs& a, void* ws, int64_t ws_bytes, cudaStream_t stream);
 
 // Indexer key pools (csrc/kpool.cu).
 struct KpoolArgs {

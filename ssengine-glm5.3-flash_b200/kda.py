@@ -85,6 +85,32 @@ class KdaLayer:
                                    None if status is None else status.data_ptr(), lib.stream_ptr(stream))
         lib.check("ssb_kda_prefill_ws", rc)
 
+    def decode(self, qkv: torch.Tensor, g: torch.Tensor, beta: torch.Tensor, out: torch.Tensor, seqs: torch.Tensor,
+               conv_state: torch.Tensor, rec_state: torch.Tensor, stream=None,
+               status: torch.Tensor | None = None) -> torch.Tensor:
+        """The recurrent form for new tokens: the arguments of `prefill`, the same state blocks, any number of rows a
+        sequence (one in a decode step), token after token in one launch without a workspace. Rows outside every
+        sequence are not written. `status` (int32 [1] on the device) receives 1 if a sequence reaches outside the rows
+        or names a negative block (it is skipped). Returns `out`."""
+        so = lib.load()
+        T, P = qkv.shape[0], self.heads * HEAD_DIM
+        for name, t, cols in (("qkv", qkv, 3 * P), ("g", g, P), ("beta", beta, self.heads), ("out", out, P)):
+            if t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape[0] < T or t.shape[1] < cols or t.stride(1) != 1:
+                raise ValueError(f"{name}: bf16 [{T}, >= {cols}] with unit column stride, got {t.dtype} "
+                                 f"{tuple(t.shape)} strides {t.stride()}")
+        if seqs.dtype != torch.int32 or seqs.dim() != 2 or seqs.shape[1] != 4 or not seqs.is_contiguous():
+            raise ValueError(f"seqs: contiguous int32 [R, 4], got {seqs.dtype} {tuple(seqs.shape)}")
+        if len({t.device for t in (qkv, g, beta, out, seqs, conv_state, rec_state, self.conv_weight)}) != 1:
+            raise ValueError("the tensors of one call must be on one device")
+        if not qkv.is_cuda:
+            raise ValueError(f"the tensors are on {qkv.device}, not on a GPU")
+        L = self.c_struct(conv_state, rec_state)
+        rc = so.ssb_kda_decode(ctypes.byref(L), qkv.data_ptr(), qkv.stride(0), g.data_ptr(), g.stride(0),
+                               beta.data_ptr(), beta.stride(0), T, seqs.data_ptr(), seqs.shape[0], out.data_ptr(),
+                               out.stride(0), None if status is None else status.data_ptr(), lib.stream_ptr(stream))
+        lib.check("ssb_kda_decode", rc)
+        return out
+
     def conv_qkv(self, qkv: torch.Tensor, seqs: torch.Tensor, conv_state: torch.Tensor, rec_state: torch.Tensor,
                  stream=None):
         """The short conv alone -> q, k, v bf16 [T, P] each; the conv state blocks of `seqs` updated."""

@@ -24,7 +24,8 @@ EXPORTS = ("ssb_version", "ssb_sf_atom_cols", "ssb_nvfp4_quantize", "ssb_nvfp4_g
            "ssb_kpool_insert", "ssb_gated_rmsnorm", "ssb_gated_rmsnorm_nvfp4", "ssb_hc_expand", "ssb_hc_mean",
            "ssb_nvfp4_gemm_grouped", "ssb_rmsnorm_cols", "ssb_rope", "ssb_transpose_heads", "ssb_concat_cols",
            "ssb_head_tiles", "ssb_moe_route_sigmoid", "ssb_copy_runs", "ssb_indexer_logits_fp8",
-           "ssb_indexer_q_quant", "ssb_kpool_insert_fp8")
+           "ssb_indexer_q_quant", "ssb_kpool_insert_fp8", "ssb_kda_decode", "ssb_mla_decode",
+           "ssb_mla_decode_workspace_bytes")
 
 EPI_F32, EPI_BF16, EPI_SWIGLU = 0, 1, 2
 ROUTE_SOFTMAX, ROUTE_SIGMOID_BIAS = 0, 1
@@ -77,7 +78,7 @@ _LIB = None
 # Kernels each entry point launches (1 unless listed), for the count of this library's launches in a timed region
 KERNELS_PER_CALL = {"ssb_moe_forward": 10, "ssb_moe_forward_profiled": 10, "ssb_mhc_ws": 2,
                     "ssb_kda_prefill": 2, "ssb_kda_prefill_ws": 2, "ssb_kpool_insert": 2, "ssb_kpool_insert_fp8": 2,
-                    "ssb_stage_metadata": 2}
+                    "ssb_stage_metadata": 2, "ssb_mla_decode": 2}
 
 
 class _Counting:
@@ -136,6 +137,11 @@ _SIGS = {
                             _I64, _P, _P], ctypes.c_int),
     "ssb_kda_workspace_bytes": ([ctypes.c_int32, _I64, _I64], ctypes.c_int64),
     "ssb_kda_conv": ([ctypes.POINTER(KdaLayerC), _P, _I64, _I64, _P, _I64, _P, _P, _P, _P], ctypes.c_int),
+    "ssb_kda_decode": ([ctypes.POINTER(KdaLayerC), _P, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _P, _P],
+                       ctypes.c_int),
+    "ssb_mla_decode": ([_P, _I32, _I64, _I64, _I64, _I32, _P, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _I32, _F, _F, _P,
+                        _P, _P, _I64, _P, _P], ctypes.c_int),
+    "ssb_mla_decode_workspace_bytes": ([_I64, _I32], ctypes.c_int64),
     "ssb_ipc_export": ([_P, _P, ctypes.POINTER(ctypes.c_int64)], ctypes.c_int),
     "ssb_ipc_open": ([_P, ctypes.POINTER(ctypes.c_void_p)], ctypes.c_int),
     "ssb_ipc_close": ([_P], ctypes.c_int),
@@ -205,6 +211,23 @@ def scratch(device, nbytes: int):
     t = _SCRATCH.get(key)
     if t is None or t.numel() < nbytes:
         t = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+        _SCRATCH[key] = t
+    return t
+
+
+def stream_scratch(device, nbytes: int, stream=None):
+    """A uint8 workspace of at least `nbytes` for calls on `stream` (default: the current one) alone, grown on demand:
+    calls on different streams get different buffers. It is allocated on that stream, so a buffer that is outgrown is
+    reused only after the stream's earlier calls."""
+    import torch
+
+    dev = torch.device(device)
+    s = torch.cuda.current_stream(dev) if stream is None else stream
+    key = (dev.type, s.device.index, int(s.cuda_stream))
+    t = _SCRATCH.get(key)
+    if t is None or t.numel() < nbytes:
+        with torch.cuda.stream(s):
+            t = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=s.device)
         _SCRATCH[key] = t
     return t
 

@@ -1,5 +1,5 @@
-"""Sparse MLA prefill, the FP8 latent-cache append and the FP8 query pack of one DSA layer through the C ABI
-(`ssb_sparse_mla`, `ssb_mla_cache_append`, `ssb_mla_q_pack`).
+"""Sparse MLA prefill, the attention of new tokens, the FP8 latent-cache append and the FP8 query pack of one DSA layer
+through the C ABI (`ssb_sparse_mla`, `ssb_mla_decode`, `ssb_mla_cache_append`, `ssb_mla_q_pack`).
 
 Mirrors the reference's calls: the TRTLLM sparse MLA with FP8 query and cache (`trtllm_batch_decode_with_kv_cache_mla`
 with the indexer's top-k token lists and bmm1 = scale * q_scale * k_scale, bmm2 = k_scale; split at 32,768 rows:
@@ -32,6 +32,84 @@ def sparse_mla(q8: torch.Tensor, kv_cache: torch.Tensor, indices: torch.Tensor, 
                            qsl.data_ptr(), qsl.shape[0] - 1, page_table.data_ptr(), page_table.shape[1], bmm1, bmm2,
                            out.data_ptr(), None if status is None else status.data_ptr(), lib.stream_ptr(stream))
     lib.check("ssb_sparse_mla", rc)
+    return out
+
+
+def decode_workspace_bytes(T: int, heads: int) -> int:
+    """Device bytes of the workspace of one `decode` / `decode_selected` call (`ssb_mla_decode_workspace_bytes`)."""
+    n = lib.load().ssb_mla_decode_workspace_bytes(T, heads)
+    if n < 0:
+        raise ValueError(f"bad MLA decode workspace query: T={T}, heads={heads} (1..128)")
+    return int(n)
+
+
+def decode(q: torch.Tensor, kv_cache: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, bmm1: float,
+           out: torch.Tensor, bmm2: float = 1.0, reqs: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+           workspace: torch.Tensor | None = None, stream=None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of new tokens over all of their request's cache: row t sees positions 0 .. seq_lens[t] - 1 of the
+    pages in row reqs[t] (default t) of page_table int32 [R, width]. q [T, H, 576], H = 1..128, bf16 or e4m3 bytes
+    (uint8) with unit stride in the last dimension and 16-byte row and head strides; kv_cache e4m3 bytes uint8
+    [slots, 576]; seq_lens, reqs int32 [T]; -> out bf16 [T, H, 512] and, when given, lse fp32 [T, H]. A row without a
+    token gets zeros (lse -inf). bmm1 = softmax scale * q_scale * k_scale, bmm2 = k_scale, as `sparse_mla`. Split over
+    the tokens and joined in `workspace` (uint8, `decode_workspace_bytes(T, H)`; default: one kept per stream); the
+    lengths are read on the device. `status` (int32 [1] on the device) receives 1 for a reqs entry outside the table,
+    4 if a bounded wait gave up."""
+    return _decode(q, kv_cache, None, page_table, seq_lens, bmm1, out, bmm2, None, reqs, lse, workspace, stream, status)
+
+
+def decode_selected(q: torch.Tensor, kv_cache: torch.Tensor, indices: torch.Tensor, page_table: torch.Tensor,
+                    bmm1: float, out: torch.Tensor, bmm2: float = 1.0, n_idx: int | None = None,
+                    seq_lens: torch.Tensor | None = None, reqs: torch.Tensor | None = None,
+                    lse: torch.Tensor | None = None, workspace: torch.Tensor | None = None, stream=None,
+                    status: torch.Tensor | None = None) -> torch.Tensor:
+    """`decode` over the positions listed in the first n_idx columns of indices int32 [T, >= n_idx] (the indexer's
+    expanded selection; -1 = none), those at or past seq_lens[t] left out when seq_lens is given (it also tells how
+    much work a short row holds, which balances the split)."""
+    if indices.dtype != torch.int32 or indices.dim() != 2 or indices.stride(1) != 1 or indices.shape[0] < q.shape[0]:
+        raise ValueError(f"indices: int32 [{q.shape[0]}, n] with unit column stride, got {indices.dtype} "
+                         f"{tuple(indices.shape)}")
+    n = indices.shape[1] if n_idx is None else n_idx
+    if not 0 <= n <= indices.shape[1]:
+        raise ValueError(f"n_idx {n} of {indices.shape[1]} columns")
+    return _decode(q, kv_cache, indices, page_table, seq_lens, bmm1, out, bmm2, n, reqs, lse, workspace, stream, status)
+
+
+def _decode(q, kv_cache, indices, page_table, seq_lens, bmm1, out, bmm2, n_idx, reqs, lse, workspace, stream, status):
+    so = lib.load()
+    if q.dtype not in (torch.bfloat16, torch.uint8) or q.dim() != 3 or q.shape[2] != DQ or q.stride(2) != 1:
+        raise ValueError(f"q: bf16 or e4m3 bytes [T, heads, {DQ}] with unit stride in the last dimension, got {q.dtype} "
+                         f"{tuple(q.shape)} strides {q.stride()}")
+    T, H = q.shape[:2]
+    if kv_cache.dtype != torch.uint8 or kv_cache.dim() != 2 or kv_cache.shape[1] != DQ or not kv_cache.is_contiguous():
+        raise ValueError(f"kv_cache: contiguous uint8 [slots, {DQ}], got {kv_cache.dtype} {tuple(kv_cache.shape)}")
+    if out.dtype != torch.bfloat16 or out.shape != (T, H, DV) or not out.is_contiguous():
+        raise ValueError(f"out: contiguous bf16 {(T, H, DV)}, got {out.dtype} {tuple(out.shape)}")
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous():
+        raise ValueError(f"page_table: contiguous int32 [R, width], got {page_table.dtype} {tuple(page_table.shape)}")
+    for name, t, dt, shape in (("seq_lens", seq_lens, torch.int32, (T,)), ("reqs", reqs, torch.int32, (T,)),
+                               ("lse", lse, torch.float32, (T, H))):
+        if t is not None and (t.dtype != dt or t.shape != shape or not t.is_contiguous()):
+            raise ValueError(f"{name}: contiguous {dt} {shape}, got {t.dtype} {tuple(t.shape)}")
+    if reqs is None and page_table.shape[0] < T:
+        raise ValueError(f"page_table has {page_table.shape[0]} rows for {T} query rows and no reqs")
+    if len({t.device for t in (q, kv_cache, page_table, out, seq_lens, indices, reqs, lse, workspace)
+            if t is not None}) != 1:
+        raise ValueError("the tensors of one call must be on one device")
+    need = decode_workspace_bytes(T, H)
+    if workspace is not None and (workspace.dtype != torch.uint8 or not workspace.is_contiguous() or
+                                  workspace.numel() < need):
+        raise ValueError(f"workspace: contiguous uint8 of {need} bytes or more")
+    if not q.is_cuda:
+        raise ValueError(f"the tensors are on {q.device}, not on a GPU")
+    if workspace is None:
+        workspace = lib.stream_scratch(q.device, need, stream)
+    ptr = lambda t: None if t is None else t.data_ptr()
+    rc = so.ssb_mla_decode(q.data_ptr(), int(q.dtype == torch.uint8), q.stride(0), q.stride(1), T, H,
+                           kv_cache.data_ptr(), kv_cache.shape[0], page_table.data_ptr(), page_table.shape[0],
+                           page_table.shape[1], ptr(reqs), ptr(seq_lens), ptr(indices),
+                           0 if indices is None else indices.stride(0), n_idx or 0, bmm1, bmm2, out.data_ptr(),
+                           ptr(lse), workspace.data_ptr(), workspace.numel(), ptr(status), lib.stream_ptr(stream))
+    lib.check("ssb_mla_decode", rc)
     return out
 
 
