@@ -9,6 +9,8 @@
 // workspace as (running max m, sum l, unnormalised O) in fp32 and are joined by a second kernel:
 //   M = max_i m_i;  O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.
 // No atomics and a fixed order of the sums: the same inputs give the same bits.
+#include <cuda_fp16.h>
+
 #include "common.cuh"
 #include "ops.h"
 
@@ -17,7 +19,6 @@ namespace {
 
 constexpr int kDq = 576, kDv = 512, kUnit = 128, kTileH = 64;
 constexpr int kMaxCtas = 148;                  // ranges a call is cut into at most (the workspace is sized by it)
-constexpr int kThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Plan {                                   // the row of a CTA's first unit
@@ -25,22 +26,28 @@ struct Plan {                                   // the row of a CTA's first unit
   int64_t first;                                // units before that row
 };
 
-// Tokens (selected: list columns) and units of row t.
+// Tokens and units of row t. How many tokens a row's list names is not known before it is read: its share is planned
+// by the list's width or, where that is smaller, the tokens it can name.
 SSB_DEVICE int row_bound(const MlaDecodeArgs& a, int64_t t) {
-  int64_t n = a.indices != nullptr ? a.n_idx : min((int64_t)a.width * kUnit, (int64_t)a.seq_lens[t]);
+  int64_t n = a.indices != nullptr ? a.n_idx : (int64_t)a.width * kUnit;
+  if (a.seq_lens != nullptr) n = min(n, (int64_t)a.seq_lens[t]);
   if (a.reqs != nullptr && (a.reqs[t] < 0 || a.reqs[t] >= a.R)) n = 0;
   return n > 0 ? static_cast<int>(n) : 0;
 }
 SSB_DEVICE int row_units(const MlaDecodeArgs& a, int64_t t) { return (row_bound(a, t) + kUnit - 1) / kUnit; }
 
-// All threads of the CTA: this CTA's range [lo, hi) of units and the row that holds unit lo (row = T: nothing to do).
+// All threads of the CTA (256 or more): this CTA's range [lo, hi) of units and the row that holds unit lo.
+constexpr int kScan = 256;
 SSB_DEVICE void find_range(const MlaDecodeArgs& a, int cta, int ctas, int64_t* sh, int64_t& lo, int64_t& hi, Plan& p) {
   const int tid = threadIdx.x;
-  int64_t sum = 0;
-  for (int64_t t = tid; t < a.T; t += blockDim.x) sum += row_units(a, t);
-  sh[tid] = sum;
+  const bool in = tid < kScan;
+  if (in) {
+    int64_t sum = 0;
+    for (int64_t t = tid; t < a.T; t += kScan) sum += row_units(a, t);
+    sh[tid] = sum;
+  }
   __syncthreads();
-  for (int o = blockDim.x / 2; o > 0; o >>= 1) {
+  for (int o = kScan / 2; o > 0; o >>= 1) {
     if (tid < o) sh[tid] += sh[tid + o];
     __syncthreads();
   }
@@ -49,27 +56,27 @@ SSB_DEVICE void find_range(const MlaDecodeArgs& a, int cta, int ctas, int64_t* s
   const int64_t used = min((int64_t)ctas, total);      // every range in use holds a unit: a row's CTAs are consecutive
   lo = cta < used ? total * cta / used : total;
   hi = cta < used ? total * (cta + 1) / used : total;
-  if (tid == 0) sh[256] = a.T, sh[257] = 0;
+  if (tid == 0) sh[kScan] = a.T, sh[kScan + 1] = 0;
   int64_t base = 0;
-  for (int64_t c = 0; c < a.T; c += blockDim.x) {
+  for (int64_t c = 0; c < a.T; c += kScan) {
     const int64_t t = c + tid;
-    const int64_t n = t < a.T ? row_units(a, t) : 0;
-    sh[tid] = n;
+    const int64_t n = in && t < a.T ? row_units(a, t) : 0;
+    if (in) sh[tid] = n;
     __syncthreads();
-    for (int o = 1; o < blockDim.x; o <<= 1) {
-      const int64_t v = tid >= o ? sh[tid - o] : 0;
+    for (int o = 1; o < kScan; o <<= 1) {
+      const int64_t v = in && tid >= o ? sh[tid - o] : 0;
       __syncthreads();
-      sh[tid] += v;
+      if (in) sh[tid] += v;
       __syncthreads();
     }
-    const int64_t end = base + sh[tid], beg = end - n;
-    if (n > 0 && beg <= lo && lo < end) sh[256] = t, sh[257] = beg;
-    base += sh[blockDim.x - 1];
+    const int64_t end = base + (in ? sh[tid] : 0), beg = end - n;
+    if (n > 0 && beg <= lo && lo < end) sh[kScan] = t, sh[kScan + 1] = beg;
+    base += sh[kScan - 1];
     __syncthreads();
     if (base > lo) break;
   }
-  p.row = static_cast<int>(sh[256]);
-  p.first = sh[257];
+  p.row = static_cast<int>(sh[kScan]);
+  p.first = sh[kScan + 1];
 }
 
 SSB_DEVICE float* part_o(const MlaDecodeArgs& a, int tile, int slot) {
@@ -79,156 +86,596 @@ SSB_DEVICE float2* part_ml(const MlaDecodeArgs& a, int tile, int slot) {
   return a.part_ml + ((int64_t)tile * 2 * kMaxCtas + slot) * kTileH;
 }
 
-// Cache row of the j-th token of row t's list (-1: none).
-SSB_DEVICE int64_t token_slot(const MlaDecodeArgs& a, int64_t t, int64_t j) {
-  const int64_t req = a.reqs != nullptr ? a.reqs[t] : t;
-  int64_t pos = j;
-  if (a.indices != nullptr) {
-    pos = a.indices[t * a.ld_idx + j];
-    if (pos < 0 || (a.seq_lens != nullptr && pos >= a.seq_lens[t])) return -1;
-  }
-  if (pos / kUnit >= a.width) return -1;
-  const int64_t page = a.table[req * a.width + pos / kUnit];
-  const int64_t slot = page * kUnit + pos % kUnit;
-  return page >= 0 && slot < a.cache_rows ? slot : -1;
+// ---- shared memory ------------------------------------------------------------------------------------------------
+constexpr int kSoftmax = 128;                   // warps 0-3
+constexpr int kGatherWarps = 4;                 // warps 5-8
+constexpr int kThreads = kSoftmax + 32 + 32 * kGatherWarps;
+constexpr int kChunk = 16384;                   // [128 rows x 128 B], 128-byte swizzle
+constexpr int kRope = 8192;                     // [128 rows x 64 B], 64-byte swizzle
+constexpr int kRows = 4 * kChunk + kRope;       // 128 rows of 576 bytes: the keys of a unit, or the query tile's parts
+constexpr int kOffQ = 0;
+constexpr int kOffKv = kRows;                   // two units
+constexpr int kOffPlo = 3 * kRows;              // the low parts of P; the high parts take the unit's rope chunk
+constexpr int kOffBar = kOffPlo + kRope;        // mbarriers
+constexpr int kOffMisc = kOffBar + 96;          // tmem address, abort flag, last-unit flags
+constexpr int kOffMask = kOffMisc + 32;         // uint32 [2][4]: tokens present in a unit
+constexpr int kOffScale = kOffMask + 32;        // float [64]: base-2 score scale of each head
+constexpr int kOffExp = kOffScale + 256;        // float [2][4][64]: each warp's exponents of a unit
+constexpr int kOffSum = kOffExp + 2048;         // float [64]: rescale factors, bmm2 / l
+constexpr int kSmem = kOffSum + 256;
+static_assert(kOffScale % 16 == 0 && kOffExp % 16 == 0 && kOffSum % 16 == 0 && kSmem <= 232448, "shared memory");
+// TMEM columns: O^T as 4 tiles of 128 dims x 64 heads, S^T 128 tokens x (64 high | 64 low), block scales
+constexpr uint32_t kColO = 0, kColS = 256, kColOne = 384, kColHi = 388, kColLo = 392;
+constexpr float kPTop = 8.0f;                   // the largest weight of a 32-token block is stored in (2^7, 2^8]
+constexpr float kMaxRise = 64.0f;               // exponents above the reference before the accumulators are rescaled
+
+// Block-scaled instruction descriptor (kind::mxf8f6f4): e4m3 A and B (format 0), ue8m0 scales (bit 23), A and B
+// MN-major (bits 15, 16), N >> 3 in [17,23), M >> 4 in [24,29), B's scale byte in [4,6).
+__host__ __device__ constexpr uint32_t idesc_mx(int M, int N, int b_byte) {
+  return (static_cast<uint32_t>(b_byte) << 4) | (1u << 15) | (1u << 16) | (static_cast<uint32_t>(N >> 3) << 17) |
+         (1u << 23) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+SSB_DEVICE void tc_mma_mx(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t acc, uint32_t sfa,
+                          uint32_t sfb) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),
+      "l"(ad), "l"(bd), "r"(idesc), "r"(acc), "r"(sfa), "r"(sfb)
+      : "memory");
+}
+SSB_DEVICE void tmem_st_x4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(a), "r"(b), "r"(c),
+               "r"(d)
+               : "memory");
+}
+SSB_DEVICE void cp_async16(uint32_t dst, const void* src, bool valid) {
+  const int n = valid ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+SSB_DEVICE void cp_async_arrive_noinc(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+SSB_DEVICE void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// Largest of the 32 lanes' values, NaN ignored (all NaN: NaN).
+SSB_DEVICE float warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+SSB_DEVICE float ex2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two halves -> two e4m3 bytes (round to nearest even, the first in the low byte) and back.
+SSB_DEVICE uint32_t half2_e4m3(__half2 v) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<uint32_t*>(&v)));
+  return r;
+}
+SSB_DEVICE __half2 e4m3_half2(uint32_t b) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(b)));
+  return *reinterpret_cast<__half2*>(&r);
+}
+// v (|v| <= 256) as hi + lo / 16 in e4m3: 8 significant bits, down to a quantum of 2^-13. v enters as two halves (11
+// bits, so that the rounding to 8 is the one that counts).
+SSB_DEVICE void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const __half2 v = __floats2half2_rn(a, b);
+  hi = half2_e4m3(v);
+  lo = half2_e4m3(__hmul2(__hsub2(v, e4m3_half2(hi)), __float2half2_rn(16.0f)));
+}
+// Byte offset of 16-byte granule g of row r: a 128-byte-swizzled chunk, a 64-byte-swizzled one.
+SSB_DEVICE uint32_t sw128(int r, int g) { return r * 128 + ((g ^ (r & 7)) << 4); }
+SSB_DEVICE uint32_t sw64(int r, int g) { return r * 64 + ((g ^ ((r >> 1) & 3)) << 4); }
+constexpr uint32_t kSw128 = 2, kSw64 = 4;       // descriptor layout types
+// Granule g (0-35) of row r of 576 bytes.
+SSB_DEVICE uint32_t row_off(int r, int g) {
+  return g < 32 ? (g >> 3) * kChunk + sw128(r, g & 7) : 4 * kChunk + sw64(r, g - 32);
 }
 
-constexpr int kTok = 32;                        // tokens a tile
-constexpr int kQLd = 578, kKLd = 578;           // bf16 row pitches in shared memory
-constexpr int kOffK = kTileH * kQLd * 2;
-constexpr int kOffS = kOffK + kTok * kKLd * 2;
-constexpr int kOffStat = kOffS + kTileH * kTok * 4;
-constexpr int kOffPlan = kOffStat + 3 * kTileH * 4;
-constexpr int kOffSlot = kOffPlan + 260 * 8;
-constexpr int kSmem = kOffSlot + kTok * 8;
-
-__global__ void __launch_bounds__(kThreads, 1) mla_decode_kernel(const MlaDecodeArgs a) {
-  extern __shared__ __align__(16) uint8_t smem[];
-  __nv_bfloat16* Q = reinterpret_cast<__nv_bfloat16*>(smem);
-  __nv_bfloat16* K = reinterpret_cast<__nv_bfloat16*>(smem + kOffK);
-  float* Sc = reinterpret_cast<float*>(smem + kOffS);
-  float* M = reinterpret_cast<float*>(smem + kOffStat);
-  float* L = M + kTileH;
-  float* Al = L + kTileH;
-  int64_t* sh = reinterpret_cast<int64_t*>(smem + kOffPlan);
-  int64_t* slots = reinterpret_cast<int64_t*>(smem + kOffSlot);
-  const int tid = threadIdx.x, cta = blockIdx.x, tile = blockIdx.y;
-  const int h0 = tile * kTileH, nh = min(kTileH, a.H - h0);
-  int64_t lo, hi;
-  Plan p;
-  find_range(a, cta, gridDim.x, sh, lo, hi, p);
-  int64_t at = lo, first = p.first;
-  bool head_part = true;                        // the CTA's first segment: partial slot 0, a later one slot 1
-  for (int64_t t = p.row; t < a.T && at < hi; ++t) {
-    const int nb = row_units(a, t);
-    if (nb == 0) continue;
-    const int64_t end = min(hi, first + nb);
-    const int b0 = static_cast<int>(at - first), b1 = static_cast<int>(end - first), n = row_bound(a, t);
-    __syncthreads();
-    for (int i = tid; i < kTileH * kDq; i += kThreads) {
-      const int h = i / kDq, c = i - h * kDq;
-      float v = 0.0f;
-      if (h < nh) {
-        const int64_t off = t * a.ldq + (h0 + h) * a.hsq + c;
-        v = a.q_e4m3 ? e4m3_value(static_cast<const uint8_t*>(a.q)[off])
-                     : __bfloat162float(static_cast<const __nv_bfloat16*>(a.q)[off]);
-      }
-      Q[h * kQLd + c] = __float2bfloat16(v);
+// Sums over the 32 lanes of 32 values a lane, transposed: lane l receives the total of value l.
+SSB_DEVICE float warp_sum_transposed(float* v, int lane) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const float keep = up ? v[i + o] : v[i], send = up ? v[i] : v[i + o];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
     }
-    if (tid < kTileH) M[tid] = -INFINITY, L[tid] = 0.0f;
-    float o[2][kTileH];
+  }
+  return v[0];
+}
+
+struct Bars {
+  uint32_t kv_full, kv_empty, q_full, s_full, s_empty, p_full, pv_done, o_full, drain;   // kv_*: two each
+};
+
+// One query row's heads h0 .. h0 + 63 into the query tile: rows 0-63 the high parts, 64-127 the low parts of
+// q 2^-k (k per head, its largest value in [2^7, 2^8)), zero rows past nh. bf16 has 8 significant bits, so the two e4m3
+// parts hold a value exactly unless it is below 2^-14 of the head's largest. Also each head's score scale. Warps 0-3.
+SSB_DEVICE void stage_q(const MlaDecodeArgs& a, uint8_t* smem, int64_t t, int h0, int nh, int warp, int lane) {
+  uint8_t* Q = smem + kOffQ;
+  float* scale = reinterpret_cast<float*>(smem + kOffScale);
+  const float unit = a.bmm1 * kLog2e;
+  if (a.q_e4m3) {
+    const uint8_t* q = static_cast<const uint8_t*>(a.q) + t * a.ldq;
+#pragma unroll 6
+    for (int i = warp * 32 + lane; i < kTileH * 36; i += kSoftmax) {
+      const int h = i / 36, g = i - h * 36;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (h < nh) v = *reinterpret_cast<const uint4*>(q + (h0 + h) * a.hsq + g * 16);
+      *reinterpret_cast<uint4*>(Q + row_off(h, g)) = v;
+    }
+    if (warp < 2) scale[warp * 32 + lane] = unit;
+    return;
+  }
+  const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + t * a.ldq;
+#pragma unroll 2
+  for (int i = 0; i < kTileH / 4; ++i) {
+    const int h = 16 * warp + i;
+    uint4 v[3];
 #pragma unroll
-    for (int h = 0; h < kTileH; ++h) o[0][h] = o[1][h] = 0.0f;
-    for (int64_t j0 = (int64_t)b0 * kUnit; j0 < min((int64_t)b1 * kUnit, (int64_t)n); j0 += kTok) {
-      __syncthreads();
-      if (tid < kTok) slots[tid] = j0 + tid < n ? token_slot(a, t, j0 + tid) : -1;
-      __syncthreads();
-      for (int i = tid; i < kTok * (kDq / 2); i += kThreads) {
-        const int r = i / (kDq / 2), c = i - r * (kDq / 2);
-        const int64_t sl = slots[r];
-        float2 v = make_float2(0.0f, 0.0f);
-        if (sl >= 0) {
-          const uint16_t w = reinterpret_cast<const uint16_t*>(a.kv + sl * kDq)[c];
-          v = make_float2(e4m3_value(w & 0xFF), e4m3_value(w >> 8));
-        }
-        *reinterpret_cast<__nv_bfloat162*>(K + r * kKLd + 2 * c) = __floats2bfloat162_rn(v.x, v.y);
+    for (int j = 0; j < 3; ++j) {
+      const int g = lane + 32 * j;                                    // 72 granules of 8 values
+      v[j] = h < nh && g < 72 ? *reinterpret_cast<const uint4*>(q + (h0 + h) * a.hsq + 8 * g) : make_uint4(0, 0, 0, 0);
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 3; ++j) {
+      const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = max(top, max(w[e] & 0x7FFFu, (w[e] >> 16) & 0x7FFFu));   // bf16 magnitudes
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    const int ex = static_cast<int>(top >> 7);                        // the largest value's biased exponent
+    const int k = ex == 0 || ex == 255 ? 0 : max(min(ex - 134, 120), -120);
+    const float down = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+    if (lane == 0) scale[h] = h < nh ? unit * __uint_as_float(static_cast<uint32_t>(127 + k) << 23) : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 3; ++j) {
+      const int g = lane + 32 * j;
+      if (g >= 72) continue;
+      const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        // an infinite query value leaves no finite weight: NaN, which e4m3 can carry (it has no infinity)
+        const float x = __uint_as_float(w[e] << 16) * down, y = __uint_as_float(w[e] & 0xFFFF0000u) * down;
+        split2(isinf(x) ? NAN : x, isinf(y) ? NAN : y, hi[e], lo[e]);
       }
-      __syncthreads();
-      {
-        const int h = tid >> 2, g = tid & 3;
-        float s[8] = {};
-        for (int c = 0; c < kDq; c += 2) {
-          const float2 qv = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(Q + h * kQLd + c));
+      const uint32_t sub = 8 * (g & 1);                               // 8 values: half a 16-byte granule
+      *reinterpret_cast<uint2*>(Q + row_off(h, g >> 1) + sub) = make_uint2(hi[0] | (hi[1] << 16), hi[2] | (hi[3] << 16));
+      *reinterpret_cast<uint2*>(Q + row_off(64 + h, g >> 1) + sub) =
+          make_uint2(lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16));
+    }
+  }
+}
+
+// A CTA's share of one row: units [b0, b1) of the row's nb planned ones; every role walks the same segments.
+struct Segment {
+  int64_t t;
+  int b0, b1, nb;
+};
+struct Walk {
+  int64_t t, at, hi, first;
+  SSB_DEVICE bool next(const MlaDecodeArgs& a, Segment& s) {
+    for (; t < a.T && at < hi; ++t) {
+      const int nb = row_units(a, t);
+      if (nb == 0) continue;
+      const int64_t end = min(hi, first + nb);
+      s.t = t, s.b0 = static_cast<int>(at - first), s.b1 = static_cast<int>(end - first), s.nb = nb;
+      at = end;
+      first += nb;
+      ++t;
+      return true;
+    }
+    return false;
+  }
+};
+
+template <bool Q8>
+__global__ void __launch_bounds__(kThreads, 1) mla_decode_kernel(const MlaDecodeArgs a) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cta = blockIdx.x, tile = blockIdx.y;
+  const int h0 = tile * kTileH, nh = min(kTileH, a.H - h0);
+  const uint32_t sbase = smem_u32(smem), bar = sbase + kOffBar;
+  const Bars B = {bar, bar + 16, bar + 32, bar + 40, bar + 48, bar + 56, bar + 64, bar + 72, bar + 80};
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kOffMisc);
+  volatile int32_t* abort_flag = reinterpret_cast<volatile int32_t*>(smem + kOffMisc + 4);
+  volatile int32_t* last_unit = reinterpret_cast<volatile int32_t*>(smem + kOffMisc + 8);     // [2]
+  volatile uint32_t* mask = reinterpret_cast<volatile uint32_t*>(smem + kOffMask);
+  if (sbase & 1023) {                                    // the swizzled tiles need it; no static shared memory precedes
+    if (tid == 0) raise_status(a.status, kErrCuda);
+    return;
+  }
+
+  Walk walk;
+  {
+    int64_t lo, hi;
+    Plan p;
+    find_range(a, cta, gridDim.x, reinterpret_cast<int64_t*>(smem + kOffKv), lo, hi, p);
+    if (lo >= hi) return;                                // fewer units than CTAs
+    walk = {p.row, lo, hi, p.first};
+  }
+  if (tid == 0) {
+    mbar_init(B.kv_full, 33 * kGatherWarps);             // every lane's copies, one arrive a warp for the mask
+    mbar_init(B.kv_full + 8, 33 * kGatherWarps);
+    mbar_init(B.kv_empty, 1);
+    mbar_init(B.kv_empty + 8, 1);
+    mbar_init(B.q_full, kSoftmax);
+    mbar_init(B.s_full, 1);
+    mbar_init(B.s_empty, kSoftmax);
+    mbar_init(B.p_full, kSoftmax);
+    mbar_init(B.pv_done, 1);
+    mbar_init(B.o_full, 1);
+    mbar_init(B.drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();                                       // also: every thread has read the plan's words
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp > 4) {
+    // ---------------------------------------------------------------- gather: warp w brings tokens 32 w .. 32 w + 31
+    const int w = warp - 5;
+    const int cols = a.indices != nullptr ? (a.n_idx + kUnit - 1) / kUnit : 0;
+    int u = 0;
+    Segment s;
+    bool ok = true;
+    while (ok && walk.next(a, s)) {
+      const int64_t req = a.reqs != nullptr ? a.reqs[s.t] : s.t;
+      const int32_t* pages = a.table + req * a.width;
+      const int len = a.seq_lens != nullptr ? a.seq_lens[s.t] : 0x7fffffff;
+      const int32_t* idx = a.indices != nullptr ? a.indices + s.t * a.ld_idx : nullptr;
+      int c0 = s.b0, c1 = s.b1;
+      unsigned long long live = ~0ull;                   // bit i: unit c0 + i holds a selected token
+      if (idx != nullptr) {                              // the row's planned share as units of list columns
+        c0 = static_cast<int>((int64_t)s.b0 * cols / s.nb);
+        c1 = static_cast<int>((int64_t)s.b1 * cols / s.nb);
+        if (c1 - c0 <= 64) {
+          live = 0;
+          for (int c = c0; c < c1; ++c) {
+            bool any = false;
 #pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            const float2 kv = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(K + (g + 4 * u) * kKLd + c));
-            s[u] = fmaf(qv.y, kv.y, fmaf(qv.x, kv.x, s[u]));
+            for (int j = 0; j < 4; ++j) {
+              const int col = c * kUnit + 32 * j + lane;
+              const int pos = col < a.n_idx ? idx[col] : -1;
+              any |= pos >= 0 && pos < len;
+            }
+            if (__any_sync(0xffffffffu, any)) live |= 1ull << (c - c0);
+          }
+          if (live == 0) live = 1;                       // nothing selected: one empty unit gives the zeros
+        }
+      }
+      auto slot_at = [&](int c) -> int64_t {             // cache row of this lane's token of unit c (-1: none)
+        int pos = c * kUnit + 32 * w + lane;
+        if (idx != nullptr) pos = pos < a.n_idx ? idx[pos] : -1;
+        if (pos < 0 || pos >= len || pos / kUnit >= a.width) return -1;
+        const int64_t slot = (int64_t)pages[pos / kUnit] * kUnit + pos % kUnit;
+        return slot >= 0 && slot < a.cache_rows ? slot : -1;
+      };
+      auto next_live = [&](int c) {
+        while (c < c1 && c - c0 < 64 && !((live >> (c - c0)) & 1)) ++c;
+        return c;
+      };
+      int c = next_live(c0);
+      int64_t slot = slot_at(c);
+      while (c < c1) {
+        const int buf = u & 1, cn = next_live(c + 1);
+        const int64_t slot_n = cn < c1 ? slot_at(cn) : -1;
+        if (u >= 2) ok = mbar_wait(B.kv_empty + 8 * buf, ((u >> 1) - 1) & 1, abort_flag, a.status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint32_t dst = sbase + kOffKv + buf * kRows;
+        const uint32_t present = __ballot_sync(0xffffffffu, slot >= 0);
+        const uint32_t lat = dst + (lane >> 3) * kChunk;
+#pragma unroll 8
+        for (int r = 0; r < 32; ++r) {                   // a warp instruction a token: its 512 latent bytes
+          const int64_t sl = __shfl_sync(0xffffffffu, slot, r);
+          cp_async16(lat + sw128(32 * w + r, lane & 7), a.kv + (sl < 0 ? 0 : sl) * kDq + 16 * lane, sl >= 0);
+        }
+#pragma unroll
+        for (int r = 0; r < 32; r += 8) {                // 8 tokens: their 64 rope bytes
+          const int64_t sl = __shfl_sync(0xffffffffu, slot, r + (lane >> 2));
+          cp_async16(dst + 4 * kChunk + sw64(32 * w + r + (lane >> 2), lane & 3),
+                     a.kv + (sl < 0 ? 0 : sl) * kDq + kDv + 16 * (lane & 3), sl >= 0);
+        }
+        cp_async_arrive_noinc(B.kv_full + 8 * buf);      // fires when this thread's copies have landed
+        if (lane == 0) {
+          mask[4 * buf + w] = present;
+          if (w == 0) last_unit[buf] = cn >= c1;
+          mbar_arrive(B.kv_full + 8 * buf);
+        }
+        ++u;
+        c = cn;
+        slot = slot_n;
+      }
+    }
+    cp_async_wait_all();
+  } else if (warp == 4) {
+    // ---------------------------------------------------------------- MMA issue (one thread)
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = idesc_e4m3(128, Q8 ? 64 : 128);
+      int u = 0, seg = 0;
+      Segment s;
+      bool ok = true;
+      auto scores = [&](int v) {                         // S^T [tokens, heads] = K Q^T of unit v
+        const uint32_t kv = sbase + kOffKv + (v & 1) * kRows;
+#pragma unroll
+        for (int c = 0; c < 5; ++c) {
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) {
+            if (c == 4 && ks >= 2) break;                // the rope chunk: 64 bytes a row
+            const uint32_t sbo = c < 4 ? 1024 : 512, sw = c < 4 ? kSw128 : kSw64;
+            tc_mma_f8(tmem + kColS, smem_desc(kv + c * kChunk + ks * 32, 0, sbo, sw),
+                      smem_desc(sbase + kOffQ + c * kChunk + ks * 32, 0, sbo, sw), idesc_s, (c | ks) != 0 ? 1u : 0u);
           }
         }
-        float mb = -INFINITY;
+        tc_commit(B.s_full);
+      };
+      auto values = [&](int v, bool fresh) {             // O^T [dims, heads] (+)= V^T P^T of unit v, high then low parts
+        const uint32_t kv = sbase + kOffKv + (v & 1) * kRows;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          s[u] = slots[g + 4 * u] >= 0 ? s[u] * (a.bmm1 * kLog2e) : -INFINITY;
-          mb = fmaxf(mb, s[u]);
-        }
-        mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, 1));
-        mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, 2));
-        const float m0 = M[h], m1 = fmaxf(m0, mb);
-        float ls = 0.0f;
+        for (int d = 0; d < 4; ++d) {
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const float pv = slots[g + 4 * u] >= 0 ? exp2f(s[u] - (m1 == -INFINITY ? 0.0f : m1)) : 0.0f;
-          Sc[h * kTok + g + 4 * u] = pv;
-          ls += pv;
+          for (int ks = 0; ks < 4; ++ks) {               // 32 tokens a step: one block of scales
+            const uint64_t ad = smem_desc(kv + d * kChunk + ks * 4096, kChunk, 1024, kSw128);
+            tc_mma_mx(tmem + kColO + 64 * d, ad, smem_desc(kv + 4 * kChunk + ks * 2048, kRope, 512, kSw64),
+                      idesc_mx(128, 64, ks), fresh && ks == 0 ? 0u : 1u, tmem + kColOne, tmem + kColHi);
+            tc_mma_mx(tmem + kColO + 64 * d, ad, smem_desc(sbase + kOffPlo + ks * 2048, kRope, 512, kSw64),
+                      idesc_mx(128, 64, ks), 1u, tmem + kColOne, tmem + kColLo);
+          }
         }
-        ls += __shfl_xor_sync(0xffffffffu, ls, 1);
-        ls += __shfl_xor_sync(0xffffffffu, ls, 2);
+        tc_commit(B.kv_empty + 8 * (v & 1));
+        tc_commit(B.pv_done);
+      };
+      while (ok && walk.next(a, s)) {
+        ok = mbar_wait(B.q_full, seg & 1, abort_flag, a.status);
+        bool fresh = true, last = false;
+        const int u0 = u;
+        while (ok && !last) {
+          ok = mbar_wait(B.kv_full + 8 * (u & 1), (u >> 1) & 1, abort_flag, a.status);
+          if (ok && u > 0) ok = mbar_wait(B.s_empty, (u - 1) & 1, abort_flag, a.status);
+          if (!ok) break;
+          last = last_unit[u & 1] != 0;
+          fence_proxy_async_smem();                      // rows brought by other threads' copies -> the tensor core
+          tc_fence_after();
+          scores(u);
+          ++u;
+          // the value product runs one unit behind the scores, the last one of a row right after its weights
+          for (int v = u - 2; v < (last ? u : u - 1); ++v) {
+            if (v < u0) continue;
+            ok = mbar_wait(B.p_full, v & 1, abort_flag, a.status);
+            if (!ok) break;
+            tc_fence_after();
+            values(v, fresh);
+            fresh = false;
+          }
+        }
+        if (ok) tc_commit(B.o_full);
+        ++seg;
+      }
+      tc_commit(B.drain);                                // everything issued has completed when this arrives
+      const unsigned long long t0 = globaltimer();
+      while (!mbar_try_wait(B.drain, 0) && globaltimer() - t0 <= kWaitNs) {}
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax (warps 0-3): a token a thread
+    const uint32_t tq = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    const float* scale = reinterpret_cast<const float*>(smem + kOffScale);
+    float* ebuf = reinterpret_cast<float*>(smem + kOffExp);
+    float* sums = reinterpret_cast<float*>(smem + kOffSum);
+    const int row = 32 * warp + lane;
+    tmem_st_x4(tq + kColOne, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu);    // V enters with scale 1
+    tmem_st_wait();
+    int u = 0, seg = 0;
+    Segment s, s_next;
+    bool more = walk.next(a, s);
+    stage_q(a, smem, s.t, h0, nh, warp, lane);
+    fence_proxy_async_smem();
+    tc_fence_before();
+    mbar_arrive(B.q_full);
+    bool ok = true;
+    named_bar(1, kSoftmax);                              // every head's scale is written
+    while (more) {
+      float l[kTileH];
+#pragma unroll
+      for (int h = 0; h < kTileH; ++h) l[h] = 0.0f;
+      float ref0 = -INFINITY, ref1 = -INFINITY;          // reference exponents of heads lane and lane + 32
+      bool last = false;
+      while (!last) {
+        const int buf = u & 1;
+        float* eb = ebuf + (u & 1) * 256;                // exponents of this unit
+        float* fac = ebuf + ((u + 1) & 1) * 256 + 64 * warp;   // this warp's row of the other half: free after the barrier
+        ok = mbar_wait(B.s_full, u & 1, abort_flag, a.status);
+        if (ok) ok = mbar_wait(B.kv_full + 8 * buf, (u >> 1) & 1, abort_flag, a.status);   // the mask's writes
+        tc_fence_after();
+        last = last_unit[buf] != 0;
+        const bool valid = (mask[4 * buf + warp] >> lane) & 1;
+        float p[kTileH];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float x[32], y[32];
+          tmem_ld_32x32b_x32(tq + kColS + 32 * j, x);
+          if (!Q8) tmem_ld_32x32b_x32(tq + kColS + 64 + 32 * j, y);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) p[32 * j + i] = Q8 ? x[i] : fmaf(y[i], 0.0625f, x[i]);
+        }
+        tc_fence_before();
+        mbar_arrive(B.s_empty);
+        // weights against the warp's own exponent: e = ceil of the largest base-2 score of its 32 tokens, weight
+        // 2^(x - e + 8); a head without a token here has e = -inf
+#pragma unroll
+        for (int h = 0; h < kTileH; h += 4) {
+          const float4 sc = *reinterpret_cast<const float4*>(scale + h);
+          const float c[4] = {sc.x, sc.y, sc.z, sc.w};
+          float e[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float x = valid ? p[h + k] * c[k] : -INFINITY;
+            const float m = warp_max(x);
+            e[k] = ceilf(m);
+            p[h + k] = ex2_fast(x + (m == -INFINITY ? 0.0f : kPTop - e[k]));
+          }
+          if (lane == 0) *reinterpret_cast<float4*>(eb + 64 * warp + h) = make_float4(e[0], e[1], e[2], e[3]);
+        }
+        if (named_bar_or(1, kSoftmax, !ok)) {
+          ok = false;
+          break;
+        }
+        float e0[4], e1[4], m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          e0[k] = eb[64 * k + lane], e1[k] = eb[64 * k + 32 + lane];
+          m0 = fmaxf(m0, e0[k]), m1 = fmaxf(m1, e1[k]);
+        }
+        if (ref0 == -INFINITY) ref0 = m0;
+        if (ref1 == -INFINITY) ref1 = m1;
+        // the value product of the unit before has read its weights and scales; the accumulators are at rest
+        if (u > 0) ok = mbar_wait(B.pv_done, (u - 1) & 1, abort_flag, a.status);
+        tc_fence_after();
+        // fp32 accumulators take exponents up to kMaxRise above the reference; beyond that they are rescaled
+        const bool up0 = m0 - ref0 > kMaxRise, up1 = m1 - ref1 > kMaxRise;
+        if (__any_sync(0xffffffffu, up0 || up1)) {
+          fac[lane] = up0 ? exp2f(ref0 - m0) : 1.0f;
+          fac[32 + lane] = up1 ? exp2f(ref1 - m1) : 1.0f;
+          if (up0) ref0 = m0;
+          if (up1) ref1 = m1;
+          __syncwarp();
+#pragma unroll
+          for (int h = 0; h < kTileH; ++h) l[h] *= fac[h];
+#pragma unroll 1
+          for (int d = 0; d < 8; ++d) {
+            float o[32];
+            tmem_ld_32x32b_x32(tq + kColO + 32 * d, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] *= fac[32 * (d & 1) + i];
+            tmem_st_32x32b_x32(tq + kColO + 32 * d, o);
+          }
+          tmem_st_wait();
+          __syncwarp();
+        }
+        // block scales 2^(e - ref) of the four warps (32 tokens each) as ue8m0 bytes, the low parts' 2^-4 of them
+        uint32_t hi0 = 0, hi1 = 0, lo0 = 0, lo1 = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int b0 = 127 + static_cast<int>(fminf(fmaxf(e0[k] - ref0, -126.0f), kMaxRise));
+          const int b1 = 127 + static_cast<int>(fminf(fmaxf(e1[k] - ref1, -126.0f), kMaxRise));
+          hi0 |= static_cast<uint32_t>(b0) << (8 * k);
+          hi1 |= static_cast<uint32_t>(b1) << (8 * k);
+          lo0 |= static_cast<uint32_t>(max(b0 - 4, 0)) << (8 * k);
+          lo1 |= static_cast<uint32_t>(max(b1 - 4, 0)) << (8 * k);
+        }
+        const float ew0 = eb[64 * warp + lane], ew1 = eb[64 * warp + 32 + lane];
+        fac[lane] = exp2f(fminf(fmaxf(ew0 - ref0, -126.0f), kMaxRise));
+        fac[32 + lane] = exp2f(fminf(fmaxf(ew1 - ref1, -126.0f), kMaxRise));
         __syncwarp();
-        if (g == 0) {
-          Al[h] = m0 == -INFINITY ? 0.0f : exp2f(m0 - m1);
-          L[h] = L[h] * Al[h] + ls;
-          M[h] = m1;
+        tmem_st_x4(tq + kColHi, hi0, hi1, 0u, 0u);
+        tmem_st_x4(tq + kColLo, lo0, lo1, 0u, 0u);
+        uint8_t* ph = smem + kOffKv + buf * kRows + 4 * kChunk;
+        uint8_t* pl = smem + kOffPlo;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {                    // 16 heads a 16-byte granule
+          uint32_t wh[4], wl[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int h = 16 * g + 4 * q;
+            const float4 f = *reinterpret_cast<const float4*>(fac + h);
+            l[h] = fmaf(p[h], f.x, l[h]), l[h + 1] = fmaf(p[h + 1], f.y, l[h + 1]);
+            l[h + 2] = fmaf(p[h + 2], f.z, l[h + 2]), l[h + 3] = fmaf(p[h + 3], f.w, l[h + 3]);
+            uint32_t ha, la, hb, lb;
+            split2(p[h], p[h + 1], ha, la);
+            split2(p[h + 2], p[h + 3], hb, lb);
+            wh[q] = ha | (hb << 16);
+            wl[q] = la | (lb << 16);
+          }
+          *reinterpret_cast<uint4*>(ph + sw64(row, g)) = make_uint4(wh[0], wh[1], wh[2], wh[3]);
+          *reinterpret_cast<uint4*>(pl + sw64(row, g)) = make_uint4(wl[0], wl[1], wl[2], wl[3]);
+        }
+        tmem_st_wait();
+        fence_proxy_async_smem();
+        tc_fence_before();
+        mbar_arrive(B.p_full);
+        ++u;
+      }
+      // ---- the row's sums, the next row's query, then the accumulators ----
+      const float l0 = warp_sum_transposed(l, lane), l1 = warp_sum_transposed(l + 32, lane);
+      if (named_bar_or(1, kSoftmax, !ok)) break;         // (also: the last unit's exponents are read)
+      ebuf[64 * warp + lane] = l0;
+      ebuf[64 * warp + 32 + lane] = l1;
+      named_bar(1, kSoftmax);
+      float t0 = 0.0f, t1 = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) t0 += ebuf[64 * k + lane], t1 += ebuf[64 * k + 32 + lane];
+      if (warp == 0) {                                   // a NaN sum stays one
+        sums[lane] = t0 == 0.0f ? 0.0f : a.bmm2 / t0;
+        sums[32 + lane] = t1 == 0.0f ? 0.0f : a.bmm2 / t1;
+      }
+      named_bar(1, kSoftmax);
+      more = walk.next(a, s_next);
+      if (more) {
+        stage_q(a, smem, s_next.t, h0, nh, warp, lane);
+        fence_proxy_async_smem();
+        mbar_arrive(B.q_full);
+      }
+      ok = mbar_wait(B.o_full, seg & 1, abort_flag, a.status);
+      if (named_bar_or(1, kSoftmax, !ok)) break;
+      tc_fence_after();
+      const bool whole = s.b0 == 0 && s.b1 == s.nb;
+      const int slot = 2 * cta + (seg == 0 ? 0 : 1);
+      if (warp == 0) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int h = lane + 32 * k;
+          const float lt = k ? t1 : t0, m = (k ? ref1 : ref0) - kPTop;
+          if (!whole) part_ml(a, tile, slot)[h] = make_float2(m, lt);
+          else if (a.lse != nullptr && h < nh)
+            a.lse[s.t * a.H + h0 + h] = lt == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m) + log2f(lt)) / kLog2e;
+        }
+        if (lane == 0 && tile == 0) {
+          if (s.b0 == 0) a.rows[s.t].first = cta, a.rows[s.t].first_slot = slot;
+          if (s.b1 == s.nb) a.rows[s.t].last = cta;
         }
       }
-      __syncthreads();
+#pragma unroll 1
+      for (int d = 0; d < 8; ++d) {                      // 128 dims x 32 heads; a lane holds one dim
+        float o[32];
+        tmem_ld_32x32b_x32(tq + kColO + 32 * d, o);
+        tmem_ld_wait();
+        const int dim = 128 * (d >> 1) + row, hb = 32 * (d & 1);
+        if (whole) {
+          __nv_bfloat16* out = a.out + (s.t * a.H + h0 + hb) * kDv + dim;
 #pragma unroll
-      for (int h = 0; h < kTileH; ++h) o[0][h] *= Al[h], o[1][h] *= Al[h];
-      for (int j = 0; j < kTok; ++j) {
-        const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(K + j * kKLd + 2 * tid));
+          for (int i = 0; i < 32; ++i)
+            if (hb + i < nh) out[i * kDv] = __float2bfloat16(o[i] * sums[hb + i]);
+        } else {
+          float* po = part_o(a, tile, slot) + hb * kDv + dim;
 #pragma unroll
-        for (int h = 0; h < kTileH; ++h) {
-          const float pv = Sc[h * kTok + j];
-          o[0][h] = fmaf(pv, v.x, o[0][h]);
-          o[1][h] = fmaf(pv, v.y, o[1][h]);
+          for (int i = 0; i < 32; ++i) po[i * kDv] = o[i];
         }
       }
+      tc_fence_before();
+      s = s_next;
+      ++seg;
     }
-    __syncthreads();
-    const bool whole = b0 == 0 && b1 == nb;
-    const int slot = 2 * cta + (head_part ? 0 : 1);
-    if (whole) {
-#pragma unroll
-      for (int h = 0; h < kTileH; ++h) {
-        if (h >= nh) break;
-        const float inv = L[h] == 0.0f ? 0.0f : a.bmm2 / L[h];         // a NaN sum stays one
-        reinterpret_cast<__nv_bfloat162*>(a.out + (t * a.H + h0 + h) * kDv)[tid] =
-            __floats2bfloat162_rn(o[0][h] * inv, o[1][h] * inv);
-      }
-      if (a.lse != nullptr && tid < nh)
-        a.lse[t * a.H + h0 + tid] = L[tid] == 0.0f ? -INFINITY : (M[tid] + log2f(L[tid])) / kLog2e;
-    } else {
-      float* po = part_o(a, tile, slot);
-#pragma unroll
-      for (int h = 0; h < kTileH; ++h) reinterpret_cast<float2*>(po + h * kDv)[tid] = make_float2(o[0][h], o[1][h]);
-      if (tid < kTileH) part_ml(a, tile, slot)[tid] = make_float2(M[tid], L[tid]);
-    }
-    if (tid == 0 && tile == 0) {
-      if (b0 == 0) a.rows[t].first = cta, a.rows[t].first_slot = slot;
-      if (b1 == nb) a.rows[t].last = cta;
-    }
-    head_part = false;
-    at = end;
-    first += nb;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
   }
 }
 
@@ -316,13 +763,13 @@ int launch_mla_decode(const MlaDecodeArgs& a_in, void* ws, int64_t ws_bytes, cud
   a.part_ml = reinterpret_cast<float2*>(p);
   p += up256(slots * kTileH * 8);
   a.part_o = reinterpret_cast<float*>(p);
-  static bool attr = false;
-  if (!attr) {
-    if (cudaFuncSetAttribute(mla_decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
-      return kErrCuda;
-    attr = true;
+  auto* kernel = a.q_e4m3 ? mla_decode_kernel<true> : mla_decode_kernel<false>;
+  static bool attr[2] = {false, false};
+  if (!attr[a.q_e4m3]) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return kErrCuda;
+    attr[a.q_e4m3] = true;
   }
-  mla_decode_kernel<<<dim3((unsigned)(kMaxCtas / tiles), (unsigned)tiles), kThreads, kSmem, stream>>>(a);
+  kernel<<<dim3((unsigned)(kMaxCtas / tiles), (unsigned)tiles), kThreads, kSmem, stream>>>(a);
   if (cudaGetLastError() != cudaSuccess) return kErrCuda;
   mla_join_kernel<<<dim3((unsigned)a.T, (unsigned)a.H, 4), 128, 0, stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
