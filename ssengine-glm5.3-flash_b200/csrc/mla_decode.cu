@@ -87,8 +87,11 @@ SSB_DEVICE float2* part_ml(const MlaDecodeArgs& a, int tile, int slot) {
 }
 
 // ---- shared memory ------------------------------------------------------------------------------------------------
-constexpr int kSoftmax = 128;                   // warps 0-3
-constexpr int kGatherWarps = 4;                 // warps 5-8
+constexpr int kSoftWarps = 8;                   // warps 0-7: token quarter warp & 3, heads 32 (warp >> 2) .. + 31
+constexpr int kSoftmax = 32 * kSoftWarps;
+constexpr int kHalf = 128;                      // threads of one head half
+constexpr int kMmaWarp = kSoftWarps;            // warp 8; warps 9-12 gather
+constexpr int kGatherWarps = 4;
 constexpr int kThreads = kSoftmax + 32 + 32 * kGatherWarps;
 constexpr int kChunk = 16384;                   // [128 rows x 128 B], 128-byte swizzle
 constexpr int kRope = 8192;                     // [128 rows x 64 B], 64-byte swizzle
@@ -96,18 +99,19 @@ constexpr int kRows = 4 * kChunk + kRope;       // 128 rows of 576 bytes: the ke
 constexpr int kOffQ = 0;
 constexpr int kOffKv = kRows;                   // two units
 constexpr int kOffPlo = 3 * kRows;              // the low parts of P; the high parts take the unit's rope chunk
-constexpr int kOffBar = kOffPlo + kRope;        // mbarriers
+constexpr int kOffSf = kOffPlo + kRope;         // block scales of P: byte (h % 32) 16 + (h / 32) 4 + token quarter
+constexpr int kOffBar = kOffSf + 512;           // mbarriers
 constexpr int kOffMisc = kOffBar + 96;          // tmem address, abort flag, last-unit flags
 constexpr int kOffMask = kOffMisc + 32;         // uint32 [2][4]: tokens present in a unit
-constexpr int kOffScale = kOffMask + 32;        // float [64]: base-2 score scale of each head
-constexpr int kOffExp = kOffScale + 256;        // float [2][4][64]: each warp's exponents of a unit
-constexpr int kOffSum = kOffExp + 2048;         // float [64]: rescale factors, bmm2 / l
+constexpr int kOffScale = kOffMask + 32;        // float2 [64]: base-2 score scale and minus the reference of each head
+constexpr int kOffExp = kOffScale + 512;        // float [4][64]: maxima of the token quarters, or their sums
+constexpr int kOffSum = kOffExp + 1024;         // float [64]: rescale factors, bmm2 / l
 constexpr int kSmem = kOffSum + 256;
-static_assert(kOffScale % 16 == 0 && kOffExp % 16 == 0 && kOffSum % 16 == 0 && kSmem <= 232448, "shared memory");
-// TMEM columns: O^T as 4 tiles of 128 dims x 64 heads, S^T 128 tokens x (64 high | 64 low), block scales
-constexpr uint32_t kColO = 0, kColS = 256, kColOne = 384, kColHi = 388, kColLo = 392;
-constexpr float kPTop = 8.0f;                   // the largest weight of a 32-token block is stored in (2^7, 2^8]
-constexpr float kMaxRise = 64.0f;               // exponents above the reference before the accumulators are rescaled
+static_assert(kOffScale % 16 == 0 && kOffExp % 16 == 0 && kOffSf % 128 == 0 && kSmem <= 232448, "shared memory");
+// TMEM columns: O^T as 4 tiles of 128 dims x 64 heads, S^T 128 tokens x (64 high | 64 low), block scales of V (1 against
+// the high parts of P, 2^-4 against the low ones) and of P
+constexpr uint32_t kColO = 0, kColS = 256, kColOne = 384, kColLow = 388, kColP = 392;
+constexpr float kMaxRise = 64.0f;               // base-2 scores above the reference before the accumulators are rescaled
 
 // Block-scaled instruction descriptor (kind::mxf8f6f4): e4m3 A and B (format 0), ue8m0 scales (bit 23), A and B
 // MN-major (bits 15, 16), N >> 3 in [17,23), M >> 4 in [24,29), B's scale byte in [4,6).
@@ -128,6 +132,17 @@ SSB_DEVICE void tmem_st_x4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, u
   asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(a), "r"(b), "r"(c),
                "r"(d)
                : "memory");
+}
+SSB_DEVICE void tmem_ld_x16(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 SSB_DEVICE void cp_async16(uint32_t dst, const void* src, bool valid) {
   const int n = valid ? 16 : 0;
@@ -195,61 +210,76 @@ struct Bars {
 
 // One query row's heads h0 .. h0 + 63 into the query tile: rows 0-63 the high parts, 64-127 the low parts of
 // q 2^-k (k per head, its largest value in [2^7, 2^8)), zero rows past nh. bf16 has 8 significant bits, so the two e4m3
-// parts hold a value exactly unless it is below 2^-14 of the head's largest. Also each head's score scale. Warps 0-3.
+// parts hold a value exactly unless it is below 2^-14 of the head's largest. Also each head's score scale (its reference
+// cleared). Warps 0-7, 8 heads each.
+template <bool Q8>
 SSB_DEVICE void stage_q(const MlaDecodeArgs& a, uint8_t* smem, int64_t t, int h0, int nh, int warp, int lane) {
   uint8_t* Q = smem + kOffQ;
-  float* scale = reinterpret_cast<float*>(smem + kOffScale);
+  float2* scale = reinterpret_cast<float2*>(smem + kOffScale);
   const float unit = a.bmm1 * kLog2e;
-  if (a.q_e4m3) {
+  if (Q8) {
     const uint8_t* q = static_cast<const uint8_t*>(a.q) + t * a.ldq;
-#pragma unroll 6
-    for (int i = warp * 32 + lane; i < kTileH * 36; i += kSoftmax) {
-      const int h = i / 36, g = i - h * 36;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (h < nh) v = *reinterpret_cast<const uint4*>(q + (h0 + h) * a.hsq + g * 16);
-      *reinterpret_cast<uint4*>(Q + row_off(h, g)) = v;
+    uint4 v[9];
+#pragma unroll
+    for (int j = 0; j < 9; ++j) {
+      const int i = warp * 32 + lane + kSoftmax * j, h = i / 36, g = i - h * 36;
+      v[j] = h < nh ? *reinterpret_cast<const uint4*>(q + (h0 + h) * a.hsq + g * 16) : make_uint4(0, 0, 0, 0);
     }
-    if (warp < 2) scale[warp * 32 + lane] = unit;
+#pragma unroll
+    for (int j = 0; j < 9; ++j) {
+      const int i = warp * 32 + lane + kSoftmax * j, h = i / 36, g = i - h * 36;
+      *reinterpret_cast<uint4*>(Q + row_off(h, g)) = v[j];
+    }
+    if (warp < 2) scale[warp * 32 + lane] = make_float2(unit, 0.0f);
     return;
   }
   const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + t * a.ldq;
-#pragma unroll 2
-  for (int i = 0; i < kTileH / 4; ++i) {
-    const int h = 16 * warp + i;
-    uint4 v[3];
+#pragma unroll 1
+  for (int i0 = 0; i0 < 8; i0 += 4) {
+    uint4 v[4][3];
 #pragma unroll
-    for (int j = 0; j < 3; ++j) {
-      const int g = lane + 32 * j;                                    // 72 granules of 8 values
-      v[j] = h < nh && g < 72 ? *reinterpret_cast<const uint4*>(q + (h0 + h) * a.hsq + 8 * g) : make_uint4(0, 0, 0, 0);
-    }
-    uint32_t top = 0;
+    for (int i = 0; i < 4; ++i) {
+      const int h = 8 * warp + i0 + i;
 #pragma unroll
-    for (int j = 0; j < 3; ++j) {
-      const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) top = max(top, max(w[e] & 0x7FFFu, (w[e] >> 16) & 0x7FFFu));   // bf16 magnitudes
-    }
-    top = __reduce_max_sync(0xffffffffu, top);
-    const int ex = static_cast<int>(top >> 7);                        // the largest value's biased exponent
-    const int k = ex == 0 || ex == 255 ? 0 : max(min(ex - 134, 120), -120);
-    const float down = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
-    if (lane == 0) scale[h] = h < nh ? unit * __uint_as_float(static_cast<uint32_t>(127 + k) << 23) : 0.0f;
-#pragma unroll
-    for (int j = 0; j < 3; ++j) {
-      const int g = lane + 32 * j;
-      if (g >= 72) continue;
-      const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-      uint32_t hi[4], lo[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        // an infinite query value leaves no finite weight: NaN, which e4m3 can carry (it has no infinity)
-        const float x = __uint_as_float(w[e] << 16) * down, y = __uint_as_float(w[e] & 0xFFFF0000u) * down;
-        split2(isinf(x) ? NAN : x, isinf(y) ? NAN : y, hi[e], lo[e]);
+      for (int j = 0; j < 3; ++j) {
+        const int g = lane + 32 * j;                                  // 72 granules of 8 values
+        v[i][j] = h < nh && g < 72 ? *reinterpret_cast<const uint4*>(q + (h0 + h) * a.hsq + 8 * g)
+                                   : make_uint4(0, 0, 0, 0);
       }
-      const uint32_t sub = 8 * (g & 1);                               // 8 values: half a 16-byte granule
-      *reinterpret_cast<uint2*>(Q + row_off(h, g >> 1) + sub) = make_uint2(hi[0] | (hi[1] << 16), hi[2] | (hi[3] << 16));
-      *reinterpret_cast<uint2*>(Q + row_off(64 + h, g >> 1) + sub) =
-          make_uint2(lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int h = 8 * warp + i0 + i;
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < 3; ++j) {
+        const uint32_t w[4] = {v[i][j].x, v[i][j].y, v[i][j].z, v[i][j].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = max(top, max(w[e] & 0x7FFFu, (w[e] >> 16) & 0x7FFFu));   // bf16 magnitudes
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+      const int ex = static_cast<int>(top >> 7);                      // the largest value's biased exponent
+      const int k = ex == 0 || ex == 255 ? 0 : max(min(ex - 134, 120), -120);
+      const float down = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+      if (lane == 0)
+        scale[h] = make_float2(h < nh ? unit * __uint_as_float(static_cast<uint32_t>(127 + k) << 23) : 0.0f, 0.0f);
+#pragma unroll
+      for (int j = 0; j < 3; ++j) {
+        const int g = lane + 32 * j;
+        if (g >= 72) continue;
+        const uint32_t w[4] = {v[i][j].x, v[i][j].y, v[i][j].z, v[i][j].w};
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          // an infinite query value leaves no finite weight: NaN, which e4m3 can carry (it has no infinity)
+          const float x = __uint_as_float(w[e] << 16) * down, y = __uint_as_float(w[e] & 0xFFFF0000u) * down;
+          split2(isinf(x) ? NAN : x, isinf(y) ? NAN : y, hi[e], lo[e]);
+        }
+        const uint32_t sub = 8 * (g & 1);                             // 8 values: half a 16-byte granule
+        *reinterpret_cast<uint2*>(Q + row_off(h, g >> 1) + sub) = make_uint2(hi[0] | (hi[1] << 16), hi[2] | (hi[3] << 16));
+        *reinterpret_cast<uint2*>(Q + row_off(64 + h, g >> 1) + sub) =
+            make_uint2(lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16));
+      }
     }
   }
 }
@@ -277,7 +307,9 @@ struct Walk {
 };
 
 template <bool Q8>
-__global__ void __launch_bounds__(kThreads, 1) mla_decode_kernel(const MlaDecodeArgs a) {
+__global__ void __launch_bounds__(kThreads, 1)
+    mla_decode_kernel(const __grid_constant__ CUtensorMap mlat, const __grid_constant__ CUtensorMap mrope,
+                      const MlaDecodeArgs a) {
   extern __shared__ __align__(1024) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = blockIdx.x, tile = blockIdx.y;
@@ -297,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1) mla_decode_kernel(const MlaDecode
   {
     int64_t lo, hi;
     Plan p;
-    find_range(a, cta, gridDim.x, reinterpret_cast<int64_t*>(smem + kOffKv), lo, hi, p);
+    find_range(a, cta, gridDim.x, reinterpret_cast<int64_t*>(smem + kOffPlo), lo, hi, p);
     if (lo >= hi) return;                                // fewer units than CTAs
     walk = {p.row, lo, hi, p.first};
   }
@@ -325,9 +357,13 @@ __global__ void __launch_bounds__(kThreads, 1) mla_decode_kernel(const MlaDecode
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp > 4) {
+  if (warp > kMmaWarp) {
     // ---------------------------------------------------------------- gather: warp w brings tokens 32 w .. 32 w + 31
-    const int w = warp - 5;
+    const int w = warp - kMmaWarp - 1;
+    if (w == 0 && lane == 0) {
+      tma_prefetch_desc(&mlat);
+      tma_prefetch_desc(&mrope);
+    }
     const int cols = a.indices != nullptr ? (a.n_idx + kUnit - 1) / kUnit : 0;
     int u = 0;
     Segment s;
@@ -357,44 +393,61 @@ __global__ void __launch_bounds__(kThreads, 1) mla_decode_kernel(const MlaDecode
           if (live == 0) live = 1;                       // nothing selected: one empty unit gives the zeros
         }
       }
-      auto slot_at = [&](int c) -> int64_t {             // cache row of this lane's token of unit c (-1: none)
+      auto slot_at = [&](int c) -> int {                 // cache row of this lane's token of unit c (-1: none)
         int pos = c * kUnit + 32 * w + lane;
         if (idx != nullptr) pos = pos < a.n_idx ? idx[pos] : -1;
         if (pos < 0 || pos >= len || pos / kUnit >= a.width) return -1;
         const int64_t slot = (int64_t)pages[pos / kUnit] * kUnit + pos % kUnit;
-        return slot >= 0 && slot < a.cache_rows ? slot : -1;
+        return slot >= 0 && slot < a.cache_rows ? static_cast<int>(slot) : -1;
       };
       auto next_live = [&](int c) {
         while (c < c1 && c - c0 < 64 && !((live >> (c - c0)) & 1)) ++c;
         return c;
       };
       int c = next_live(c0);
-      int64_t slot = slot_at(c);
+      int slot = slot_at(c);
       while (c < c1) {
         const int buf = u & 1, cn = next_live(c + 1);
-        const int64_t slot_n = cn < c1 ? slot_at(cn) : -1;
+        const int slot_n = cn < c1 ? slot_at(cn) : -1;
         if (u >= 2) ok = mbar_wait(B.kv_empty + 8 * buf, ((u >> 1) - 1) & 1, abort_flag, a.status);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        const uint32_t dst = sbase + kOffKv + buf * kRows;
+        const uint32_t dst = sbase + kOffKv + buf * kRows, full = B.kv_full + 8 * buf;
         const uint32_t present = __ballot_sync(0xffffffffu, slot >= 0);
-        const uint32_t lat = dst + (lane >> 3) * kChunk;
-#pragma unroll 8
-        for (int r = 0; r < 32; ++r) {                   // a warp instruction a token: its 512 latent bytes
-          const int64_t sl = __shfl_sync(0xffffffffu, slot, r);
-          cp_async16(lat + sw128(32 * w + r, lane & 7), a.kv + (sl < 0 ? 0 : sl) * kDq + 16 * lane, sl >= 0);
-        }
+        // a whole page comes as tiles; a row's last page, and selected tokens, row by row: rows that are not there have
+        // to be zeros (whatever the cache holds there, NaN too, would meet weight 0 in the value product)
+        const bool page = idx == nullptr && (c + 1) * kUnit <= len && slot >= 0 &&
+                          slot - (32 * w + lane) + kUnit <= a.cache_rows;     // the same in every lane and warp
+        if (page) {
+          if (w == 0 && lane == 0) {
+            mbar_arrive_expect_tx(full, kRows);
+            const int y = slot;                          // this lane's token is the page's first
 #pragma unroll
-        for (int r = 0; r < 32; r += 8) {                // 8 tokens: their 64 rope bytes
-          const int64_t sl = __shfl_sync(0xffffffffu, slot, r + (lane >> 2));
-          cp_async16(dst + 4 * kChunk + sw64(32 * w + r + (lane >> 2), lane & 3),
-                     a.kv + (sl < 0 ? 0 : sl) * kDq + kDv + 16 * (lane & 3), sl >= 0);
+            for (int j = 0; j < 4; ++j) tma_load_2d(dst + j * kChunk, &mlat, 128 * j, y, full);
+            tma_load_2d(dst + 4 * kChunk, &mrope, kDv, y, full);
+          } else {
+            mbar_arrive(full);
+          }
+        } else {
+          const uint32_t lat = dst + (lane >> 3) * kChunk + 4096 * w;
+          const uint8_t* src = a.kv + 16 * lane;
+#pragma unroll 16
+          for (int r = 0; r < 32; ++r) {                 // a warp instruction a token: its 512 latent bytes
+            const int sl = __shfl_sync(0xffffffffu, slot, r);
+            cp_async16(lat + sw128(r, lane & 7), src + (int64_t)max(sl, 0) * kDq, sl >= 0);
+          }
+#pragma unroll
+          for (int r = 0; r < 32; r += 8) {              // 8 tokens: their 64 rope bytes
+            const int sl = __shfl_sync(0xffffffffu, slot, r + (lane >> 2));
+            cp_async16(dst + 4 * kChunk + sw64(32 * w + r + (lane >> 2), lane & 3),
+                       a.kv + (int64_t)max(sl, 0) * kDq + kDv + 16 * (lane & 3), sl >= 0);
+          }
+          cp_async_arrive_noinc(full);                   // fires when this thread's copies have landed
         }
-        cp_async_arrive_noinc(B.kv_full + 8 * buf);      // fires when this thread's copies have landed
         if (lane == 0) {
           mask[4 * buf + w] = present;
           if (w == 0) last_unit[buf] = cn >= c1;
-          mbar_arrive(B.kv_full + 8 * buf);
+          mbar_arrive(full);
         }
         ++u;
         c = cn;
@@ -402,38 +455,48 @@ __global__ void __launch_bounds__(kThreads, 1) mla_decode_kernel(const MlaDecode
       }
     }
     cp_async_wait_all();
-  } else if (warp == 4) {
+  } else if (warp == kMmaWarp) {
     // ---------------------------------------------------------------- MMA issue (one thread)
     if (lane == 0) {
       constexpr uint32_t idesc_s = idesc_e4m3(128, Q8 ? 64 : 128);
+      // descriptors of the operands' first tiles; a tile further on is an addition to the address field
+      const uint64_t dq = smem_desc(sbase + kOffQ, 0, 1024, kSw128);
+      const uint64_t dqr = smem_desc(sbase + kOffQ + 4 * kChunk, 0, 512, kSw64);
+      const uint64_t dk = smem_desc(sbase + kOffKv, 0, 1024, kSw128);
+      const uint64_t dkr = smem_desc(sbase + kOffKv + 4 * kChunk, 0, 512, kSw64);
+      const uint64_t dv = smem_desc(sbase + kOffKv, kChunk, 1024, kSw128);
+      const uint64_t dph = smem_desc(sbase + kOffKv + 4 * kChunk, kRope, 512, kSw64);
+      const uint64_t dpl = smem_desc(sbase + kOffPlo, kRope, 512, kSw64);
+      const uint64_t dsf = smem_desc(sbase + kOffSf, 0, 128, 0);
       int u = 0, seg = 0;
       Segment s;
       bool ok = true;
       auto scores = [&](int v) {                         // S^T [tokens, heads] = K Q^T of unit v
-        const uint32_t kv = sbase + kOffKv + (v & 1) * kRows;
+        const uint64_t k = dk + (v & 1) * (kRows >> 4), kr = dkr + (v & 1) * (kRows >> 4);
 #pragma unroll
-        for (int c = 0; c < 5; ++c) {
+        for (int c = 0; c < 4; ++c) {
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks) {
-            if (c == 4 && ks >= 2) break;                // the rope chunk: 64 bytes a row
-            const uint32_t sbo = c < 4 ? 1024 : 512, sw = c < 4 ? kSw128 : kSw64;
-            tc_mma_f8(tmem + kColS, smem_desc(kv + c * kChunk + ks * 32, 0, sbo, sw),
-                      smem_desc(sbase + kOffQ + c * kChunk + ks * 32, 0, sbo, sw), idesc_s, (c | ks) != 0 ? 1u : 0u);
-          }
+          for (int ks = 0; ks < 4; ++ks)
+            tc_mma_f8(tmem + kColS, k + ((c * kChunk + ks * 32) >> 4), dq + ((c * kChunk + ks * 32) >> 4), idesc_s,
+                      (c | ks) != 0 ? 1u : 0u);
         }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)                   // the rope chunk: 64 bytes a row
+          tc_mma_f8(tmem + kColS, kr + ((ks * 32) >> 4), dqr + ((ks * 32) >> 4), idesc_s, 1u);
         tc_commit(B.s_full);
       };
       auto values = [&](int v, bool fresh) {             // O^T [dims, heads] (+)= V^T P^T of unit v, high then low parts
-        const uint32_t kv = sbase + kOffKv + (v & 1) * kRows;
+        const uint64_t kv = dv + (v & 1) * (kRows >> 4), ph = dph + (v & 1) * (kRows >> 4);
+        tc_cp_sf(tmem + kColP, dsf);
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks) {               // 32 tokens a step: one block of scales
-            const uint64_t ad = smem_desc(kv + d * kChunk + ks * 4096, kChunk, 1024, kSw128);
-            tc_mma_mx(tmem + kColO + 64 * d, ad, smem_desc(kv + 4 * kChunk + ks * 2048, kRope, 512, kSw64),
-                      idesc_mx(128, 64, ks), fresh && ks == 0 ? 0u : 1u, tmem + kColOne, tmem + kColHi);
-            tc_mma_mx(tmem + kColO + 64 * d, ad, smem_desc(sbase + kOffPlo + ks * 2048, kRope, 512, kSw64),
-                      idesc_mx(128, 64, ks), 1u, tmem + kColOne, tmem + kColLo);
+            const uint64_t ad = kv + ((d * kChunk + ks * 4096) >> 4);
+            tc_mma_mx(tmem + kColO + 64 * d, ad, ph + ((ks * 2048) >> 4), idesc_mx(128, 64, ks),
+                      fresh && ks == 0 ? 0u : 1u, tmem + kColOne, tmem + kColP);
+            tc_mma_mx(tmem + kColO + 64 * d, ad, dpl + ((ks * 2048) >> 4), idesc_mx(128, 64, ks), 1u, tmem + kColLow,
+                      tmem + kColP);
           }
         }
         tc_commit(B.kv_empty + 8 * (v & 1));
@@ -470,198 +533,190 @@ __global__ void __launch_bounds__(kThreads, 1) mla_decode_kernel(const MlaDecode
       while (!mbar_try_wait(B.drain, 0) && globaltimer() - t0 <= kWaitNs) {}
     }
   } else {
-    // ---------------------------------------------------------------- softmax (warps 0-3): a token a thread
-    const uint32_t tq = tmem + (static_cast<uint32_t>(warp * 32) << 16);
-    const float* scale = reinterpret_cast<const float*>(smem + kOffScale);
-    float* ebuf = reinterpret_cast<float*>(smem + kOffExp);
+    // ---------------------------------------------------------------- softmax (warps 0-7): a token and 32 heads a thread
+    const int quarter = warp & 3, half = warp >> 2, hb = 32 * half, bid = 1 + half;
+    const int row = 32 * quarter + lane;
+    const uint32_t tq = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
+    float2* scale = reinterpret_cast<float2*>(smem + kOffScale);
+    float* part = reinterpret_cast<float*>(smem + kOffExp);
     float* sums = reinterpret_cast<float*>(smem + kOffSum);
-    const int row = 32 * warp + lane;
-    tmem_st_x4(tq + kColOne, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu);    // V enters with scale 1
+    uint8_t* sf = smem + kOffSf;
+    if (half == 0) tmem_st_x4(tq + kColOne, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu);   // 1
+    else tmem_st_x4(tq + kColLow, 0x7B7B7B7Bu, 0x7B7B7B7Bu, 0x7B7B7B7Bu, 0x7B7B7B7Bu);            // 2^-4
     tmem_st_wait();
     int u = 0, seg = 0;
     Segment s, s_next;
-    bool more = walk.next(a, s);
-    stage_q(a, smem, s.t, h0, nh, warp, lane);
+    bool more = walk.next(a, s), ok = true;
+    stage_q<Q8>(a, smem, s.t, h0, nh, warp, lane);
     fence_proxy_async_smem();
     tc_fence_before();
     mbar_arrive(B.q_full);
-    bool ok = true;
-    named_bar(1, kSoftmax);                              // every head's scale is written
+    named_bar(3, kSoftmax);                              // every head's scale is written
     while (more) {
-      float l[kTileH];
+      float l[32];
 #pragma unroll
-      for (int h = 0; h < kTileH; ++h) l[h] = 0.0f;
-      float ref0 = -INFINITY, ref1 = -INFINITY;          // reference exponents of heads lane and lane + 32
-      bool last = false;
+      for (int h = 0; h < 32; ++h) l[h] = 0.0f;
+      float ref = -INFINITY;                             // reference of head hb + lane (the same in the 4 quarters)
+      bool last = false, fresh = true, unset = true;
       while (!last) {
         const int buf = u & 1;
-        float* eb = ebuf + (u & 1) * 256;                // exponents of this unit
-        float* fac = ebuf + ((u + 1) & 1) * 256 + 64 * warp;   // this warp's row of the other half: free after the barrier
         ok = mbar_wait(B.s_full, u & 1, abort_flag, a.status);
         if (ok) ok = mbar_wait(B.kv_full + 8 * buf, (u >> 1) & 1, abort_flag, a.status);   // the mask's writes
         tc_fence_after();
         last = last_unit[buf] != 0;
-        const bool valid = (mask[4 * buf + warp] >> lane) & 1;
-        float p[kTileH];
+        const uint32_t present = mask[4 * buf + quarter];
+        const bool valid = (present >> lane) & 1;
+        float p[32];
+        auto load_scores = [&]() {                       // base-2 scores less the reference; tokens not there: -inf
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float x[32], y[32];
-          tmem_ld_32x32b_x32(tq + kColS + 32 * j, x);
-          if (!Q8) tmem_ld_32x32b_x32(tq + kColS + 64 + 32 * j, y);
-          tmem_ld_wait();
+          for (int j = 0; j < 32; j += 16) {
+            float x[16], y[16];
+            tmem_ld_x16(tq + kColS + hb + j, x);
+            if (!Q8) tmem_ld_x16(tq + kColS + 64 + hb + j, y);
+            tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) p[32 * j + i] = Q8 ? x[i] : fmaf(y[i], 0.0625f, x[i]);
+            for (int i = 0; i < 16; i += 2) {
+              const float4 c = *reinterpret_cast<const float4*>(scale + hb + j + i);
+              p[j + i] = fmaf(Q8 ? x[i] : fmaf(y[i], 0.0625f, x[i]), c.x, c.y);
+              p[j + i + 1] = fmaf(Q8 ? x[i + 1] : fmaf(y[i + 1], 0.0625f, x[i + 1]), c.z, c.w);
+            }
+          }
+          if (present != 0xffffffffu) {
+#pragma unroll
+            for (int h = 0; h < 32; ++h) p[h] = valid ? p[h] : -INFINITY;
+          }
+        };
+        load_scores();
+        float top = p[0];
+#pragma unroll
+        for (int h = 1; h < 32; ++h) top = fmaxf(top, p[h]);
+        // the four quarters agree on the rare path; a failed wait travels the same way
+        const bool rise = named_bar_or(bid, kHalf, unset || top > kMaxRise || !ok);
+        if (rise) {
+          if (named_bar_or(bid, kHalf, !ok)) {
+            ok = false;
+            break;
+          }
+          // new references: a head without one, or with scores more than kMaxRise above it, takes the ceiling of this
+          // unit's largest score; what it has accumulated is rescaled
+          const float old = ref == -INFINITY ? 0.0f : ref;
+#pragma unroll
+          for (int h = 0; h < 32; ++h) {
+            const float m = warp_max(p[h]);
+            if (lane == 0) part[64 * quarter + hb + h] = m;
+          }
+          named_bar(bid, kHalf);
+          float m = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) m = fmaxf(m, part[64 * k + hb + lane]);
+          const bool move = m > -INFINITY && (ref == -INFINITY || m > kMaxRise);
+          const float now = move ? ceilf(m + old) : old;
+          const float f = move && ref != -INFINITY ? exp2f(old - now) : 1.0f;
+          if (move) ref = now;
+          unset = __any_sync(0xffffffffu, ref == -INFINITY);
+          if (quarter == 0) {
+            sums[hb + lane] = f;
+            scale[hb + lane].y = -now;
+          }
+          const bool scaled = __any_sync(0xffffffffu, f != 1.0f);
+          named_bar(bid, kHalf);
+          if (scaled && !fresh) {
+#pragma unroll
+            for (int h = 0; h < 32; ++h) l[h] *= sums[hb + h];
+            ok = mbar_wait(B.pv_done, (u - 1) & 1, abort_flag, a.status);
+            tc_fence_after();
+#pragma unroll 1
+            for (int d = 0; d < 4; ++d) {
+              tmem_ld_32x32b_x32(tq + kColO + 64 * d + hb, p);
+              tmem_ld_wait();
+#pragma unroll
+              for (int h = 0; h < 32; ++h) p[h] *= sums[hb + h];
+              tmem_st_32x32b_x32(tq + kColO + 64 * d + hb, p);
+            }
+            tmem_st_wait();
+          }
+          load_scores();
         }
         tc_fence_before();
         mbar_arrive(B.s_empty);
-        // weights against the warp's own exponent: e = ceil of the largest base-2 score of its 32 tokens, weight
-        // 2^(x - e + 8); a head without a token here has e = -inf
+        // weights 2^score; then each head's largest over the warp's 32 tokens gives their block scale: its exponent E
+        // moves the weights to [2^7, 2^8) at most, the scale 2^(E - 134) moves them back in the product
+        uint32_t wh[8], wl[8];
 #pragma unroll
-        for (int h = 0; h < kTileH; h += 4) {
-          const float4 sc = *reinterpret_cast<const float4*>(scale + h);
-          const float c[4] = {sc.x, sc.y, sc.z, sc.w};
-          float e[4];
+        for (int h = 0; h < 32; ++h) {
+          p[h] = ex2_fast(p[h]);
+          l[h] += p[h];
+        }
+        if (u > 0 && !mbar_wait(B.pv_done, (u - 1) & 1, abort_flag, a.status)) ok = false;   // its P and scales are read
+#pragma unroll
+        for (int h = 0; h < 32; h += 4) {
+          uint32_t part_hi[2], part_lo[2];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const float x = valid ? p[h + k] * c[k] : -INFINITY;
-            const float m = warp_max(x);
-            e[k] = ceilf(m);
-            p[h + k] = ex2_fast(x + (m == -INFINITY ? 0.0f : kPTop - e[k]));
+            const uint32_t e = max(__reduce_max_sync(0xffffffffu, __float_as_uint(p[h + k])) & 0x7F800000u, 12u << 23);
+            p[h + k] *= __uint_as_float((261u << 23) - e);
+            if (lane == 0) sf[(h + k) * 16 + 4 * half + quarter] = static_cast<uint8_t>((e >> 23) - 7);
           }
-          if (lane == 0) *reinterpret_cast<float4*>(eb + 64 * warp + h) = make_float4(e[0], e[1], e[2], e[3]);
+          split2(p[h], p[h + 1], part_hi[0], part_lo[0]);
+          split2(p[h + 2], p[h + 3], part_hi[1], part_lo[1]);
+          wh[h / 4] = part_hi[0] | (part_hi[1] << 16);
+          wl[h / 4] = part_lo[0] | (part_lo[1] << 16);
         }
-        if (named_bar_or(1, kSoftmax, !ok)) {
-          ok = false;
-          break;
-        }
-        float e0[4], e1[4], m0 = -INFINITY, m1 = -INFINITY;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          e0[k] = eb[64 * k + lane], e1[k] = eb[64 * k + 32 + lane];
-          m0 = fmaxf(m0, e0[k]), m1 = fmaxf(m1, e1[k]);
-        }
-        if (ref0 == -INFINITY) ref0 = m0;
-        if (ref1 == -INFINITY) ref1 = m1;
-        // the value product of the unit before has read its weights and scales; the accumulators are at rest
-        if (u > 0) ok = mbar_wait(B.pv_done, (u - 1) & 1, abort_flag, a.status);
-        tc_fence_after();
-        // fp32 accumulators take exponents up to kMaxRise above the reference; beyond that they are rescaled
-        const bool up0 = m0 - ref0 > kMaxRise, up1 = m1 - ref1 > kMaxRise;
-        if (__any_sync(0xffffffffu, up0 || up1)) {
-          fac[lane] = up0 ? exp2f(ref0 - m0) : 1.0f;
-          fac[32 + lane] = up1 ? exp2f(ref1 - m1) : 1.0f;
-          if (up0) ref0 = m0;
-          if (up1) ref1 = m1;
-          __syncwarp();
-#pragma unroll
-          for (int h = 0; h < kTileH; ++h) l[h] *= fac[h];
-#pragma unroll 1
-          for (int d = 0; d < 8; ++d) {
-            float o[32];
-            tmem_ld_32x32b_x32(tq + kColO + 32 * d, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] *= fac[32 * (d & 1) + i];
-            tmem_st_32x32b_x32(tq + kColO + 32 * d, o);
-          }
-          tmem_st_wait();
-          __syncwarp();
-        }
-        // block scales 2^(e - ref) of the four warps (32 tokens each) as ue8m0 bytes, the low parts' 2^-4 of them
-        uint32_t hi0 = 0, hi1 = 0, lo0 = 0, lo1 = 0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int b0 = 127 + static_cast<int>(fminf(fmaxf(e0[k] - ref0, -126.0f), kMaxRise));
-          const int b1 = 127 + static_cast<int>(fminf(fmaxf(e1[k] - ref1, -126.0f), kMaxRise));
-          hi0 |= static_cast<uint32_t>(b0) << (8 * k);
-          hi1 |= static_cast<uint32_t>(b1) << (8 * k);
-          lo0 |= static_cast<uint32_t>(max(b0 - 4, 0)) << (8 * k);
-          lo1 |= static_cast<uint32_t>(max(b1 - 4, 0)) << (8 * k);
-        }
-        const float ew0 = eb[64 * warp + lane], ew1 = eb[64 * warp + 32 + lane];
-        fac[lane] = exp2f(fminf(fmaxf(ew0 - ref0, -126.0f), kMaxRise));
-        fac[32 + lane] = exp2f(fminf(fmaxf(ew1 - ref1, -126.0f), kMaxRise));
-        __syncwarp();
-        tmem_st_x4(tq + kColHi, hi0, hi1, 0u, 0u);
-        tmem_st_x4(tq + kColLo, lo0, lo1, 0u, 0u);
         uint8_t* ph = smem + kOffKv + buf * kRows + 4 * kChunk;
         uint8_t* pl = smem + kOffPlo;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {                    // 16 heads a 16-byte granule
-          uint32_t wh[4], wl[4];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int h = 16 * g + 4 * q;
-            const float4 f = *reinterpret_cast<const float4*>(fac + h);
-            l[h] = fmaf(p[h], f.x, l[h]), l[h + 1] = fmaf(p[h + 1], f.y, l[h + 1]);
-            l[h + 2] = fmaf(p[h + 2], f.z, l[h + 2]), l[h + 3] = fmaf(p[h + 3], f.w, l[h + 3]);
-            uint32_t ha, la, hb, lb;
-            split2(p[h], p[h + 1], ha, la);
-            split2(p[h + 2], p[h + 3], hb, lb);
-            wh[q] = ha | (hb << 16);
-            wl[q] = la | (lb << 16);
-          }
-          *reinterpret_cast<uint4*>(ph + sw64(row, g)) = make_uint4(wh[0], wh[1], wh[2], wh[3]);
-          *reinterpret_cast<uint4*>(pl + sw64(row, g)) = make_uint4(wl[0], wl[1], wl[2], wl[3]);
+        for (int g = 0; g < 2; ++g) {                    // 16 heads a 16-byte granule
+          *reinterpret_cast<uint4*>(ph + sw64(row, 2 * half + g)) = make_uint4(wh[4 * g], wh[4 * g + 1], wh[4 * g + 2], wh[4 * g + 3]);
+          *reinterpret_cast<uint4*>(pl + sw64(row, 2 * half + g)) = make_uint4(wl[4 * g], wl[4 * g + 1], wl[4 * g + 2], wl[4 * g + 3]);
         }
-        tmem_st_wait();
         fence_proxy_async_smem();
         tc_fence_before();
         mbar_arrive(B.p_full);
+        fresh = false;
         ++u;
       }
       // ---- the row's sums, the next row's query, then the accumulators ----
-      const float l0 = warp_sum_transposed(l, lane), l1 = warp_sum_transposed(l + 32, lane);
-      if (named_bar_or(1, kSoftmax, !ok)) break;         // (also: the last unit's exponents are read)
-      ebuf[64 * warp + lane] = l0;
-      ebuf[64 * warp + 32 + lane] = l1;
-      named_bar(1, kSoftmax);
-      float t0 = 0.0f, t1 = 0.0f;
+      const float ls = warp_sum_transposed(l, lane);
+      if (named_bar_or(3, kSoftmax, !ok)) break;
+      part[64 * quarter + hb + lane] = ls;
+      named_bar(3, kSoftmax);
+      float total = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) t0 += ebuf[64 * k + lane], t1 += ebuf[64 * k + 32 + lane];
-      if (warp == 0) {                                   // a NaN sum stays one
-        sums[lane] = t0 == 0.0f ? 0.0f : a.bmm2 / t0;
-        sums[32 + lane] = t1 == 0.0f ? 0.0f : a.bmm2 / t1;
-      }
-      named_bar(1, kSoftmax);
+      for (int k = 0; k < 4; ++k) total += part[64 * k + hb + lane];
+      if (quarter == 0) sums[hb + lane] = total == 0.0f ? 0.0f : a.bmm2 / total;     // a NaN sum stays one
       more = walk.next(a, s_next);
       if (more) {
-        stage_q(a, smem, s_next.t, h0, nh, warp, lane);
+        stage_q<Q8>(a, smem, s_next.t, h0, nh, warp, lane);
         fence_proxy_async_smem();
         mbar_arrive(B.q_full);
       }
       ok = mbar_wait(B.o_full, seg & 1, abort_flag, a.status);
-      if (named_bar_or(1, kSoftmax, !ok)) break;
+      if (named_bar_or(3, kSoftmax, !ok)) break;
       tc_fence_after();
       const bool whole = s.b0 == 0 && s.b1 == s.nb;
       const int slot = 2 * cta + (seg == 0 ? 0 : 1);
-      if (warp == 0) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int h = lane + 32 * k;
-          const float lt = k ? t1 : t0, m = (k ? ref1 : ref0) - kPTop;
-          if (!whole) part_ml(a, tile, slot)[h] = make_float2(m, lt);
-          else if (a.lse != nullptr && h < nh)
-            a.lse[s.t * a.H + h0 + h] = lt == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m) + log2f(lt)) / kLog2e;
-        }
-        if (lane == 0 && tile == 0) {
+      if (quarter == 0) {
+        const int h = hb + lane;
+        if (!whole) part_ml(a, tile, slot)[h] = make_float2(ref, total);
+        else if (a.lse != nullptr && h < nh)
+          a.lse[s.t * a.H + h0 + h] = total == 0.0f ? -INFINITY : ((ref == -INFINITY ? 0.0f : ref) + log2f(total)) / kLog2e;
+        if (half == 0 && lane == 0 && tile == 0) {
           if (s.b0 == 0) a.rows[s.t].first = cta, a.rows[s.t].first_slot = slot;
           if (s.b1 == s.nb) a.rows[s.t].last = cta;
         }
       }
 #pragma unroll 1
-      for (int d = 0; d < 8; ++d) {                      // 128 dims x 32 heads; a lane holds one dim
+      for (int d = 0; d < 4; ++d) {                      // 128 dims x 32 heads; a lane holds one dim
         float o[32];
-        tmem_ld_32x32b_x32(tq + kColO + 32 * d, o);
+        tmem_ld_32x32b_x32(tq + kColO + 64 * d + hb, o);
         tmem_ld_wait();
-        const int dim = 128 * (d >> 1) + row, hb = 32 * (d & 1);
         if (whole) {
-          __nv_bfloat16* out = a.out + (s.t * a.H + h0 + hb) * kDv + dim;
+          __nv_bfloat16* out = a.out + (s.t * a.H + h0 + hb) * kDv + 128 * d + row;
 #pragma unroll
           for (int i = 0; i < 32; ++i)
             if (hb + i < nh) out[i * kDv] = __float2bfloat16(o[i] * sums[hb + i]);
         } else {
-          float* po = part_o(a, tile, slot) + hb * kDv + dim;
+          float* po = part_o(a, tile, slot) + hb * kDv + 128 * d + row;
 #pragma unroll
           for (int i = 0; i < 32; ++i) po[i * kDv] = o[i];
         }
@@ -746,7 +801,7 @@ int64_t mla_decode_workspace_bytes(int64_t T, int H) {
 int launch_mla_decode(const MlaDecodeArgs& a_in, void* ws, int64_t ws_bytes, cudaStream_t stream) {
   MlaDecodeArgs a = a_in;
   const int eb = a.q_e4m3 ? 1 : 2;
-  if (a.T < 0 || a.T > 0x7fffffff || a.H <= 0 || a.H > 128 || a.R <= 0 || a.width <= 0 || a.cache_rows < 0 ||
+  if (a.T < 0 || a.T > 0x7fffffff || a.H <= 0 || a.H > 128 || a.R <= 0 || a.width <= 0 || a.cache_rows <= 0 || a.cache_rows > 0x7fffffff ||
       (a.indices == nullptr && a.seq_lens == nullptr) ||
       (a.indices != nullptr && (a.n_idx < 0 || a.ld_idx < a.n_idx)) || (a.reqs == nullptr && a.T > a.R))
     return kErrArgs;
@@ -769,7 +824,12 @@ int launch_mla_decode(const MlaDecodeArgs& a_in, void* ws, int64_t ws_bytes, cud
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return kErrCuda;
     attr[a.q_e4m3] = true;
   }
-  kernel<<<dim3((unsigned)(kMaxCtas / tiles), (unsigned)tiles), kThreads, kSmem, stream>>>(a);
+  CUtensorMap mlat, mrope;
+  const int u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  int rc = make_map_2d_ex(&mlat, u8, a.kv, a.cache_rows, kDq, kDq, 128, kUnit, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc == kOk) rc = make_map_2d_ex(&mrope, u8, a.kv, a.cache_rows, kDq, kDq, 64, kUnit, CU_TENSOR_MAP_SWIZZLE_64B);
+  if (rc != kOk) return rc;
+  kernel<<<dim3((unsigned)(kMaxCtas / tiles), (unsigned)tiles), kThreads, kSmem, stream>>>(mlat, mrope, a);
   if (cudaGetLastError() != cudaSuccess) return kErrCuda;
   mla_join_kernel<<<dim3((unsigned)a.T, (unsigned)a.H, 4), 128, 0, stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
