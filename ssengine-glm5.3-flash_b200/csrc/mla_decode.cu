@@ -101,7 +101,7 @@ constexpr int kOffKv = kRows;                   // two units
 constexpr int kOffPlo = 3 * kRows;              // the low parts of P; the high parts take the unit's rope chunk
 constexpr int kOffSf = kOffPlo + kRope;         // block scales of P: byte (h % 32) 16 + (h / 32) 4 + token quarter
 constexpr int kOffBar = kOffSf + 512;           // mbarriers
-constexpr int kOffMisc = kOffBar + 96;          // tmem address, abort flag, last-unit flags
+constexpr int kOffMisc = kOffBar + 128;         // tmem address, abort flag, last-unit flags
 constexpr int kOffMask = kOffMisc + 32;         // uint32 [2][4]: tokens present in a unit
 constexpr int kOffScale = kOffMask + 32;        // float2 [64]: base-2 score scale and minus the reference of each head
 constexpr int kOffExp = kOffScale + 512;        // float [4][64]: maxima of the token quarters, or their sums
@@ -111,6 +111,7 @@ static_assert(kOffScale % 16 == 0 && kOffExp % 16 == 0 && kOffSf % 128 == 0 && k
 // TMEM columns: O^T as 4 tiles of 128 dims x 64 heads, S^T 128 tokens x (64 high | 64 low), block scales of V (1 against
 // the high parts of P, 2^-4 against the low ones) and of P
 constexpr uint32_t kColO = 0, kColS = 256, kColOne = 384, kColLow = 388, kColP = 392;
+constexpr int kAhead = 4;                       // pages prefetched into L2 beyond the two in shared memory
 constexpr float kMaxRise = 64.0f;               // base-2 scores above the reference before the accumulators are rescaled
 
 // Block-scaled instruction descriptor (kind::mxf8f6f4): e4m3 A and B (format 0), ue8m0 scales (bit 23), A and B
@@ -132,17 +133,6 @@ SSB_DEVICE void tmem_st_x4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, u
   asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(a), "r"(b), "r"(c),
                "r"(d)
                : "memory");
-}
-SSB_DEVICE void tmem_ld_x16(uint32_t taddr, float (&v)[16]) {
-  uint32_t r[16];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
-      "[%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 SSB_DEVICE void cp_async16(uint32_t dst, const void* src, bool valid) {
   const int n = valid ? 16 : 0;
@@ -204,9 +194,25 @@ SSB_DEVICE float warp_sum_transposed(float* v, int lane) {
   return v[0];
 }
 
-struct Bars {
-  uint32_t kv_full, kv_empty, q_full, s_full, s_empty, p_full, pv_done, o_full, drain;   // kv_*: two each
+struct Bars {                                    // kv_full: one a buffer, kv_empty: one a half buffer (64 tokens)
+  uint32_t kv_full, kv_empty, q_full, s_full, s_empty, p_full, pv_done, o_full, drain;
 };
+SSB_DEVICE bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+SSB_DEVICE void tma_prefetch_2d(const CUtensorMap* m, int32_t x, int32_t y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(m)), "r"(x),
+               "r"(y)
+               : "memory");
+}
 
 // One query row's heads h0 .. h0 + 63 into the query tile: rows 0-63 the high parts, 64-127 the low parts of
 // q 2^-k (k per head, its largest value in [2^7, 2^8)), zero rows past nh. bf16 has 8 significant bits, so the two e4m3
@@ -315,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int cta = blockIdx.x, tile = blockIdx.y;
   const int h0 = tile * kTileH, nh = min(kTileH, a.H - h0);
   const uint32_t sbase = smem_u32(smem), bar = sbase + kOffBar;
-  const Bars B = {bar, bar + 16, bar + 32, bar + 40, bar + 48, bar + 56, bar + 64, bar + 72, bar + 80};
+  const Bars B = {bar, bar + 16, bar + 48, bar + 56, bar + 64, bar + 72, bar + 80, bar + 88, bar + 96};
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kOffMisc);
   volatile int32_t* abort_flag = reinterpret_cast<volatile int32_t*>(smem + kOffMisc + 4);
   volatile int32_t* last_unit = reinterpret_cast<volatile int32_t*>(smem + kOffMisc + 8);     // [2]
@@ -336,8 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     mbar_init(B.kv_full, 33 * kGatherWarps);             // every lane's copies, one arrive a warp for the mask
     mbar_init(B.kv_full + 8, 33 * kGatherWarps);
-    mbar_init(B.kv_empty, 1);
-    mbar_init(B.kv_empty + 8, 1);
+    for (int i = 0; i < 4; ++i) mbar_init(B.kv_empty + 8 * i, 1);
     mbar_init(B.q_full, kSoftmax);
     mbar_init(B.s_full, 1);
     mbar_init(B.s_empty, kSoftmax);
@@ -406,25 +411,40 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       int c = next_live(c0);
       int slot = slot_at(c);
+      // the tiles of this warp's lane 0: its half of the unit's tokens (w >> 1), latent chunks 0, 1 and the rope, or 2, 3
+      const int ch = 2 * (w & 1);
+      auto whole_page = [&](int c, int slot) {           // the same in every lane and warp
+        return idx == nullptr && (c + 1) * kUnit <= len && slot >= 0 && slot - (32 * w + lane) + kUnit <= a.cache_rows;
+      };
+      auto prefetch = [&](int c) {                       // a page some units ahead into L2
+        if (lane != 0 || idx != nullptr || c >= c1) return;
+        const int sl = slot_at(c);                       // the first token of the warp's quarter
+        if (!whole_page(c, sl)) return;
+        const int y = sl - 32 * w + 64 * (w >> 1);
+        tma_prefetch_2d(&mlat, 128 * ch, y);
+        tma_prefetch_2d(&mlat, 128 * ch + 128, y);
+        if (ch == 0) tma_prefetch_2d(&mrope, kDv, y);
+      };
+      for (int i = 0; i < kAhead; ++i) prefetch(c0 + 2 + i);
       while (c < c1) {
         const int buf = u & 1, cn = next_live(c + 1);
         const int slot_n = cn < c1 ? slot_at(cn) : -1;
-        if (u >= 2) ok = mbar_wait(B.kv_empty + 8 * buf, ((u >> 1) - 1) & 1, abort_flag, a.status);
+        prefetch(c + 2 + kAhead);
+        if (u >= 2) ok = mbar_wait(B.kv_empty + 16 * buf + 8 * (w >> 1), ((u >> 1) - 1) & 1, abort_flag, a.status);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const uint32_t dst = sbase + kOffKv + buf * kRows, full = B.kv_full + 8 * buf;
         const uint32_t present = __ballot_sync(0xffffffffu, slot >= 0);
         // a whole page comes as tiles; a row's last page, and selected tokens, row by row: rows that are not there have
         // to be zeros (whatever the cache holds there, NaN too, would meet weight 0 in the value product)
-        const bool page = idx == nullptr && (c + 1) * kUnit <= len && slot >= 0 &&
-                          slot - (32 * w + lane) + kUnit <= a.cache_rows;     // the same in every lane and warp
-        if (page) {
-          if (w == 0 && lane == 0) {
-            mbar_arrive_expect_tx(full, kRows);
-            const int y = slot;                          // this lane's token is the page's first
-#pragma unroll
-            for (int j = 0; j < 4; ++j) tma_load_2d(dst + j * kChunk, &mlat, 128 * j, y, full);
-            tma_load_2d(dst + 4 * kChunk, &mrope, kDv, y, full);
+        if (whole_page(c, slot)) {
+          if (lane == 0) {
+            const int hf = w >> 1, y = slot - 32 * w + 64 * hf;
+            const uint32_t d0 = dst + ch * kChunk + hf * (kChunk / 2);
+            mbar_arrive_expect_tx(full, kChunk + (ch == 0 ? kRope / 2 : 0));
+            tma_load_2d(d0, &mlat, 128 * ch, y, full);
+            tma_load_2d(d0 + kChunk, &mlat, 128 * ch + 128, y, full);
+            if (ch == 0) tma_load_2d(dst + 4 * kChunk + hf * (kRope / 2), &mrope, kDv, y, full);
           } else {
             mbar_arrive(full);
           }
@@ -468,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t dph = smem_desc(sbase + kOffKv + 4 * kChunk, kRope, 512, kSw64);
       const uint64_t dpl = smem_desc(sbase + kOffPlo, kRope, 512, kSw64);
       const uint64_t dsf = smem_desc(sbase + kOffSf, 0, 128, 0);
-      int u = 0, seg = 0;
+      int uq = 0, up = 0, seg = 0;                       // units whose scores, whose values have been issued
       Segment s;
       bool ok = true;
       auto scores = [&](int v) {                         // S^T [tokens, heads] = K Q^T of unit v
@@ -489,41 +509,45 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t kv = dv + (v & 1) * (kRows >> 4), ph = dph + (v & 1) * (kRows >> 4);
         tc_cp_sf(tmem + kColP, dsf);
 #pragma unroll
-        for (int d = 0; d < 4; ++d) {
+        for (int ks = 0; ks < 4; ++ks) {                 // 32 tokens a step: one block of scales
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks) {               // 32 tokens a step: one block of scales
+          for (int d = 0; d < 4; ++d) {
             const uint64_t ad = kv + ((d * kChunk + ks * 4096) >> 4);
             tc_mma_mx(tmem + kColO + 64 * d, ad, ph + ((ks * 2048) >> 4), idesc_mx(128, 64, ks),
                       fresh && ks == 0 ? 0u : 1u, tmem + kColOne, tmem + kColP);
             tc_mma_mx(tmem + kColO + 64 * d, ad, dpl + ((ks * 2048) >> 4), idesc_mx(128, 64, ks), 1u, tmem + kColLow,
                       tmem + kColP);
           }
+          if (ks & 1) tc_commit(B.kv_empty + 16 * (v & 1) + 8 * (ks >> 1));     // 64 tokens' rows are free
         }
-        tc_commit(B.kv_empty + 8 * (v & 1));
         tc_commit(B.pv_done);
       };
       while (ok && walk.next(a, s)) {
         ok = mbar_wait(B.q_full, seg & 1, abort_flag, a.status);
         bool fresh = true, last = false;
-        const int u0 = u;
-        while (ok && !last) {
-          ok = mbar_wait(B.kv_full + 8 * (u & 1), (u >> 1) & 1, abort_flag, a.status);
-          if (ok && u > 0) ok = mbar_wait(B.s_empty, (u - 1) & 1, abort_flag, a.status);
-          if (!ok) break;
-          last = last_unit[u & 1] != 0;
-          fence_proxy_async_smem();                      // rows brought by other threads' copies -> the tensor core
-          tc_fence_after();
-          scores(u);
-          ++u;
-          // the value product runs one unit behind the scores, the last one of a row right after its weights
-          for (int v = u - 2; v < (last ? u : u - 1); ++v) {
-            if (v < u0) continue;
-            ok = mbar_wait(B.p_full, v & 1, abort_flag, a.status);
-            if (!ok) break;
+        unsigned long long t0 = globaltimer();
+        while (ok && !(last && up == uq)) {
+          // whichever is ready: the next unit's scores first, else the values of the one whose weights are there
+          if (!last && mbar_test(B.kv_full + 8 * (uq & 1), (uq >> 1) & 1) &&
+              (uq == 0 || mbar_test(B.s_empty, (uq - 1) & 1))) {
+            last = last_unit[uq & 1] != 0;
+            fence_proxy_async_smem();                    // rows brought by other threads' copies -> the tensor core
             tc_fence_after();
-            values(v, fresh);
+            scores(uq++);
+          } else if (up < uq && mbar_test(B.p_full, up & 1)) {
+            tc_fence_after();
+            values(up++, fresh);
             fresh = false;
+          } else {
+            if (*abort_flag) ok = false;
+            if (globaltimer() - t0 > kWaitNs) {
+              *abort_flag = 1;
+              raise_status(a.status, kErrTimeout);
+              ok = false;
+            }
+            continue;
           }
+          t0 = globaltimer();
         }
         if (ok) tc_commit(B.o_full);
         ++seg;
@@ -568,18 +592,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool valid = (present >> lane) & 1;
         float p[32];
         auto load_scores = [&]() {                       // base-2 scores less the reference; tokens not there: -inf
+          float y[32];
+          tmem_ld_32x32b_x32(tq + kColS + hb, p);
+          if (!Q8) tmem_ld_32x32b_x32(tq + kColS + 64 + hb, y);
+          tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 32; j += 16) {
-            float x[16], y[16];
-            tmem_ld_x16(tq + kColS + hb + j, x);
-            if (!Q8) tmem_ld_x16(tq + kColS + 64 + hb + j, y);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              const float4 c = *reinterpret_cast<const float4*>(scale + hb + j + i);
-              p[j + i] = fmaf(Q8 ? x[i] : fmaf(y[i], 0.0625f, x[i]), c.x, c.y);
-              p[j + i + 1] = fmaf(Q8 ? x[i + 1] : fmaf(y[i + 1], 0.0625f, x[i + 1]), c.z, c.w);
-            }
+          for (int i = 0; i < 32; i += 2) {
+            const float4 c = *reinterpret_cast<const float4*>(scale + hb + i);
+            p[i] = fmaf(Q8 ? p[i] : fmaf(y[i], 0.0625f, p[i]), c.x, c.y);
+            p[i + 1] = fmaf(Q8 ? p[i + 1] : fmaf(y[i + 1], 0.0625f, p[i + 1]), c.z, c.w);
           }
           if (present != 0xffffffffu) {
 #pragma unroll
@@ -641,13 +662,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(B.s_empty);
         // weights 2^score; then each head's largest over the warp's 32 tokens gives their block scale: its exponent E
         // moves the weights to [2^7, 2^8) at most, the scale 2^(E - 134) moves them back in the product
-        uint32_t wh[8], wl[8];
+        uint32_t wh[8], wl[8], mine = 0;
 #pragma unroll
         for (int h = 0; h < 32; ++h) {
           p[h] = ex2_fast(p[h]);
           l[h] += p[h];
         }
-        if (u > 0 && !mbar_wait(B.pv_done, (u - 1) & 1, abort_flag, a.status)) ok = false;   // its P and scales are read
 #pragma unroll
         for (int h = 0; h < 32; h += 4) {
           uint32_t part_hi[2], part_lo[2];
@@ -655,13 +675,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int k = 0; k < 4; ++k) {
             const uint32_t e = max(__reduce_max_sync(0xffffffffu, __float_as_uint(p[h + k])) & 0x7F800000u, 12u << 23);
             p[h + k] *= __uint_as_float((261u << 23) - e);
-            if (lane == 0) sf[(h + k) * 16 + 4 * half + quarter] = static_cast<uint8_t>((e >> 23) - 7);
+            mine = lane == h + k ? e : mine;
           }
           split2(p[h], p[h + 1], part_hi[0], part_lo[0]);
           split2(p[h + 2], p[h + 3], part_hi[1], part_lo[1]);
           wh[h / 4] = part_hi[0] | (part_hi[1] << 16);
           wl[h / 4] = part_lo[0] | (part_lo[1] << 16);
         }
+        if (u > 0 && !mbar_wait(B.pv_done, (u - 1) & 1, abort_flag, a.status)) ok = false;   // its P and scales are read
+        sf[16 * lane + 4 * half + quarter] = static_cast<uint8_t>((mine >> 23) - 7);
         uint8_t* ph = smem + kOffKv + buf * kRows + 4 * kChunk;
         uint8_t* pl = smem + kOffPlo;
 #pragma unroll
@@ -826,8 +848,8 @@ int launch_mla_decode(const MlaDecodeArgs& a_in, void* ws, int64_t ws_bytes, cud
   }
   CUtensorMap mlat, mrope;
   const int u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
-  int rc = make_map_2d_ex(&mlat, u8, a.kv, a.cache_rows, kDq, kDq, 128, kUnit, CU_TENSOR_MAP_SWIZZLE_128B);
-  if (rc == kOk) rc = make_map_2d_ex(&mrope, u8, a.kv, a.cache_rows, kDq, kDq, 64, kUnit, CU_TENSOR_MAP_SWIZZLE_64B);
+  int rc = make_map_2d_ex(&mlat, u8, a.kv, a.cache_rows, kDq, kDq, 128, kUnit / 2, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc == kOk) rc = make_map_2d_ex(&mrope, u8, a.kv, a.cache_rows, kDq, kDq, 64, kUnit / 2, CU_TENSOR_MAP_SWIZZLE_64B);
   if (rc != kOk) return rc;
   kernel<<<dim3((unsigned)(kMaxCtas / tiles), (unsigned)tiles), kThreads, kSmem, stream>>>(mlat, mrope, a);
   if (cudaGetLastError() != cudaSuccess) return kErrCuda;
