@@ -89,30 +89,38 @@ SSB_DEVICE float2* part_ml(const MlaDecodeArgs& a, int tile, int slot) {
 // ---- shared memory ------------------------------------------------------------------------------------------------
 constexpr int kSoftWarps = 8;                   // warps 0-7: token quarter warp & 3, heads 32 (warp >> 2) .. + 31
 constexpr int kSoftmax = 32 * kSoftWarps;
-constexpr int kHalf = 128;                      // threads of one head half
-constexpr int kMmaWarp = kSoftWarps;            // warp 8; warps 9-12 gather
+constexpr int kGroup = 128;                     // threads of one half of the heads
+constexpr int kScoreWarp = kSoftWarps;          // warp 8 issues the score products
+constexpr int kValueWarp = kScoreWarp + 1;      // warp 9 the value products
+constexpr int kGatherWarp = kValueWarp + 1;     // warps 10-13 bring the cache rows
 constexpr int kGatherWarps = 4;
-constexpr int kThreads = kSoftmax + 32 + 32 * kGatherWarps;
+constexpr int kThreads = 32 * (kGatherWarp + kGatherWarps);
 constexpr int kChunk = 16384;                   // [128 rows x 128 B], 128-byte swizzle
 constexpr int kRope = 8192;                     // [128 rows x 64 B], 64-byte swizzle
-constexpr int kRows = 4 * kChunk + kRope;       // 128 rows of 576 bytes: the keys of a unit, or the query tile's parts
+constexpr int kRows = 4 * kChunk + kRope;       // 128 rows of 576 bytes: the query tile's parts
+constexpr int kLat = 4 * kChunk;                // a unit's latent rows
+constexpr uint32_t kBase = 1024;                // bytes of a block's shared memory that the system reserves
 constexpr int kOffQ = 0;
-constexpr int kOffKv = kRows;                   // two units
-constexpr int kOffPlo = 3 * kRows;              // the low parts of P; the high parts take the unit's rope chunk
-constexpr int kOffSf = kOffPlo + kRope;         // block scales of P: byte (h % 32) 16 + (h / 32) 4 + token quarter
+constexpr int kOffKv = kRows;                   // the latent rows of two units
+constexpr int kOffRope = kOffKv + 2 * kLat;     // the rope keys of one: free again once its scores are done
+constexpr int kOffPhi = kOffRope + kRope;       // the parts of P
+constexpr int kOffPlo = kOffPhi + kRope;
+constexpr int kOffSf = kOffPlo + kRope;         // block scales of P, two units: byte (h % 32) 16 + unit 8 + (h / 32) 4 + quarter
 constexpr int kOffBar = kOffSf + 512;           // mbarriers
-constexpr int kOffMisc = kOffBar + 128;         // tmem address, abort flag, last-unit flags
-constexpr int kOffMask = kOffMisc + 32;         // uint32 [2][4]: tokens present in a unit
-constexpr int kOffScale = kOffMask + 32;        // float2 [64]: base-2 score scale and minus the reference of each head
+constexpr int kOffMisc = kOffBar + 256;         // tmem address, abort flag, last-unit flags
+constexpr int kOffRise = kOffMisc + 32;         // int32 [2][2]: a unit with scores far above a half's references
+constexpr int kOffMask = kOffRise + 32;         // uint32 [2][4]: tokens present in a unit
+constexpr int kOffScale = kOffMask + 32;        // float [2][64]: base-2 score scale, minus the reference of each head
 constexpr int kOffExp = kOffScale + 512;        // float [4][64]: maxima of the token quarters, or their sums
 constexpr int kOffSum = kOffExp + 1024;         // float [64]: rescale factors, bmm2 / l
 constexpr int kSmem = kOffSum + 256;
 static_assert(kOffScale % 16 == 0 && kOffExp % 16 == 0 && kOffSf % 128 == 0 && kSmem <= 232448, "shared memory");
-// TMEM columns: O^T as 4 tiles of 128 dims x 64 heads, S^T 128 tokens x (64 high | 64 low), block scales of V (1 against
-// the high parts of P, 2^-4 against the low ones) and of P
-constexpr uint32_t kColO = 0, kColS = 256, kColOne = 384, kColLow = 388, kColP = 392;
+// TMEM columns: O^T as 4 tiles of 128 dims x 64 heads, S^T 128 tokens x (64 high | 64 low), block scales of V
+// (2^-7 against the high parts of P, 2^-11 against the low ones) and of P (2 columns a unit)
+constexpr uint32_t kColO = 0, kColS = 256, kColV = 384, kColLow = 388, kColP = 392;
 constexpr int kAhead = 4;                       // pages prefetched into L2 beyond the two in shared memory
-constexpr float kMaxRise = 64.0f;               // base-2 scores above the reference before the accumulators are rescaled
+constexpr float kMaxRise = 4.0f;                // base-2 scores above a head's reference before it moves and O is rescaled
+constexpr float kNoHead = -1000.0f;             // base-2 score of the heads that the tile does not have: weight 0
 
 // Block-scaled instruction descriptor (kind::mxf8f6f4): e4m3 A and B (format 0), ue8m0 scales (bit 23), A and B
 // MN-major (bits 15, 16), N >> 3 in [17,23), M >> 4 in [24,29), B's scale byte in [4,6).
@@ -120,6 +128,7 @@ __host__ __device__ constexpr uint32_t idesc_mx(int M, int N, int b_byte) {
   return (static_cast<uint32_t>(b_byte) << 4) | (1u << 15) | (1u << 16) | (static_cast<uint32_t>(N >> 3) << 17) |
          (1u << 23) | (static_cast<uint32_t>(M >> 4) << 24);
 }
+// D[tmem] (+)= A B, e4m3 operands with ue8m0 scales for blocks of 32 along the reduction.
 SSB_DEVICE void tc_mma_mx(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t acc, uint32_t sfa,
                           uint32_t sfb) {
   asm volatile(
@@ -164,8 +173,8 @@ SSB_DEVICE __half2 e4m3_half2(uint32_t b) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(b)));
   return *reinterpret_cast<__half2*>(&r);
 }
-// v (|v| <= 256) as hi + lo / 16 in e4m3: 8 significant bits, down to a quantum of 2^-13. v enters as two halves (11
-// bits, so that the rounding to 8 is the one that counts).
+// v (|v| <= 256) as hi + lo / 16 in e4m3: 8 significant bits down to 2^-6, a quantum of 2^-13 below. v enters as two
+// halves (11 bits, so that the rounding to 8 is the one that counts).
 SSB_DEVICE void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
   const __half2 v = __floats2half2_rn(a, b);
   hi = half2_e4m3(v);
@@ -181,7 +190,7 @@ SSB_DEVICE uint32_t row_off(int r, int g) {
 }
 
 // Sums over the 32 lanes of 32 values a lane, transposed: lane l receives the total of value l.
-SSB_DEVICE float warp_sum_transposed(float* v, int lane) {
+SSB_DEVICE float warp_sum_transposed(float (&v)[32], int lane) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const bool up = lane & o;
@@ -193,25 +202,147 @@ SSB_DEVICE float warp_sum_transposed(float* v, int lane) {
   }
   return v[0];
 }
-
-struct Bars {                                    // kv_full: one a buffer, kv_empty: one a half buffer (64 tokens)
-  uint32_t kv_full, kv_empty, q_full, s_full, s_empty, p_full, pv_done, o_full, drain;
-};
-SSB_DEVICE bool mbar_test(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
+SSB_DEVICE void tmem_ld_x16(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+SSB_DEVICE uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+SSB_DEVICE bool elect_lane() {                   // true in one lane of a converged warp
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, e;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+struct Bars {                                    // lat_*: 2 buffers x 4 chunks; agree: one a half of the heads
+  uint32_t lat_full, lat_empty, rope_full, rope_empty, q_full, s_full, s_empty, p_full, pv_done, o_full, drain, agree;
+};
+// One arrival for a warp, after all its lanes got here (512 arrivals a unit on one word kept shared memory from the MMAs).
+SSB_DEVICE void warp_arrive(uint32_t bar, int lane) {
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
+}
+SSB_DEVICE void mbar_arrive_n(uint32_t bar, uint32_t n) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n) : "memory");
+}
+// mbar_wait with a suspended wait: up to kNapNs a try, so that a role that waits leaves the issue slots to the others
+// (the plain form polls). Bounded in the same way.
+constexpr uint32_t kNapNs = 50000;
+SSB_DEVICE bool mbar_nap(uint32_t bar, uint32_t parity, volatile int32_t* abort_flag, int32_t* status) {
+  unsigned long long t0 = 0;
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(kNapNs)
+        : "memory");
+    if (ok) return true;
+    if (*abort_flag) return false;
+    const unsigned long long t = globaltimer();
+    if (t0 == 0) t0 = t;
+    if (t - t0 > kWaitNs) {
+      *abort_flag = 1;
+      raise_status(status, kErrTimeout);
+      return false;
+    }
+  }
 }
 SSB_DEVICE void tma_prefetch_2d(const CUtensorMap* m, int32_t x, int32_t y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(m)), "r"(x),
                "r"(y)
                : "memory");
+}
+
+// A CTA's share of one row: units [b0, b1) of the row's nb planned ones; every role walks the same segments.
+struct Segment {
+  int64_t t;
+  int b0, b1, nb;
+};
+struct Walk {
+  int64_t t, at, hi, first;
+  SSB_DEVICE bool next(const MlaDecodeArgs& a, Segment& s) {
+    for (; t < a.T && at < hi; ++t) {
+      const int nb = row_units(a, t);
+      if (nb == 0) continue;
+      const int64_t end = min(hi, first + nb);
+      s.t = t, s.b0 = static_cast<int>(at - first), s.b1 = static_cast<int>(end - first), s.nb = nb;
+      at = end;
+      first += nb;
+      ++t;
+      return true;
+    }
+    return false;
+  }
+};
+
+// The two products of a unit in buffer buf, by a whole warp of which one lane issues: the addresses are the same in every
+// lane, so they stay in uniform registers, and the loops stay small. (By one thread, with everything unrolled, the roles'
+// code together outgrew the instruction cache and every warp waited for instructions.)
+template <bool Q8>
+SSB_DEVICE bool issue_scores(const Bars& B, uint32_t sbase, int buf, uint32_t parity, bool leader,
+                             volatile int32_t* abort_flag, int32_t* status) {
+  constexpr uint32_t idesc = idesc_e4m3(128, Q8 ? 64 : 128);         // S^T [tokens, heads] = K Q^T
+  uint64_t ad = smem_desc(sbase + kOffRope, 0, 512, kSw64), bd = smem_desc(sbase + kOffQ + 4 * kChunk, 0, 512, kSw64);
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks)                                     // the rope keys: 64 bytes a row
+    if (leader) tc_mma_f8(kColS, ad + 2 * ks, bd + 2 * ks, idesc, ks != 0 ? 1u : 0u);
+  ad = smem_desc(sbase + kOffKv + buf * kLat, 0, 1024, kSw128);
+  bd = smem_desc(sbase + kOffQ, 0, 1024, kSw128);
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    if (!mbar_nap(B.lat_full + 32 * buf + 8 * c, parity, abort_flag, status)) return false;
+    fence_proxy_async_smem();                                        // rows that threads copied -> the tensor core
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks)
+      if (leader) tc_mma_f8(kColS, ad + 2 * ks, bd + 2 * ks, idesc, 1u);
+    ad += kChunk >> 4;
+    bd += kChunk >> 4;
+  }
+  if (leader) {
+    tc_commit(B.rope_empty);
+    tc_commit(B.s_full);
+  }
+  return true;
+}
+SSB_DEVICE void issue_values(const Bars& B, uint32_t sbase, int buf, bool fresh, bool leader) {
+  uint64_t ad = smem_desc(sbase + kOffKv + buf * kLat, kChunk, 1024, kSw128);     // O^T [dims, heads] (+)= V^T P^T
+  const uint64_t hi = smem_desc(sbase + kOffPhi, kRope, 512, kSw64), lo = smem_desc(sbase + kOffPlo, kRope, 512, kSw64);
+  uint32_t o = kColO, empty = B.lat_empty + 32 * buf;
+  const uint32_t sfp = kColP + 2 * buf;
+  if (leader) tc_cp_sf(kColP, smem_desc(sbase + kOffSf, 0, 128, 0));
+#pragma unroll 1
+  for (int d = 0; d < 4; ++d) {                                      // 128 dims
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {                                 // 32 tokens a step: one block of scales
+      if (leader) {
+        tc_mma_mx(o, ad + ks * (4096 >> 4), hi + ks * (2048 >> 4), idesc_mx(128, 64, ks), ks == 0 && fresh ? 0u : 1u, kColV,
+                  sfp);
+        tc_mma_mx(o, ad + ks * (4096 >> 4), lo + ks * (2048 >> 4), idesc_mx(128, 64, ks), 1u, kColLow, sfp);
+      }
+    }
+    if (leader) tc_commit(empty);                                    // the chunk is free for the unit after the next
+    ad += kChunk >> 4;
+    o += 64;
+    empty += 8;
+  }
+  if (leader) tc_commit(B.pv_done);
 }
 
 // One query row's heads h0 .. h0 + 63 into the query tile: rows 0-63 the high parts, 64-127 the low parts of
@@ -221,11 +352,11 @@ SSB_DEVICE void tma_prefetch_2d(const CUtensorMap* m, int32_t x, int32_t y) {
 template <bool Q8>
 SSB_DEVICE void stage_q(const MlaDecodeArgs& a, uint8_t* smem, int64_t t, int h0, int nh, int warp, int lane) {
   uint8_t* Q = smem + kOffQ;
-  float2* scale = reinterpret_cast<float2*>(smem + kOffScale);
+  float* scale = reinterpret_cast<float*>(smem + kOffScale);
   const float unit = a.bmm1 * kLog2e;
   if (Q8) {
     const uint8_t* q = static_cast<const uint8_t*>(a.q) + t * a.ldq;
-    uint4 v[9];
+    uint4 v[9];                                                       // 64 x 36 granules
 #pragma unroll
     for (int j = 0; j < 9; ++j) {
       const int i = warp * 32 + lane + kSoftmax * j, h = i / 36, g = i - h * 36;
@@ -236,7 +367,11 @@ SSB_DEVICE void stage_q(const MlaDecodeArgs& a, uint8_t* smem, int64_t t, int h0
       const int i = warp * 32 + lane + kSoftmax * j, h = i / 36, g = i - h * 36;
       *reinterpret_cast<uint4*>(Q + row_off(h, g)) = v[j];
     }
-    if (warp < 2) scale[warp * 32 + lane] = make_float2(unit, 0.0f);
+    if (warp < 2) {
+      const int h = warp * 32 + lane;
+      scale[h] = h < nh ? unit : 0.0f;
+      scale[64 + h] = h < nh ? 0.0f : kNoHead;
+    }
     return;
   }
   const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + t * a.ldq;
@@ -267,8 +402,10 @@ SSB_DEVICE void stage_q(const MlaDecodeArgs& a, uint8_t* smem, int64_t t, int h0
       const int ex = static_cast<int>(top >> 7);                      // the largest value's biased exponent
       const int k = ex == 0 || ex == 255 ? 0 : max(min(ex - 134, 120), -120);
       const float down = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
-      if (lane == 0)
-        scale[h] = make_float2(h < nh ? unit * __uint_as_float(static_cast<uint32_t>(127 + k) << 23) : 0.0f, 0.0f);
+      if (lane == 0) {
+        scale[h] = h < nh ? unit * __uint_as_float(static_cast<uint32_t>(127 + k) << 23) : 0.0f;
+        scale[64 + h] = h < nh ? 0.0f : kNoHead;
+      }
 #pragma unroll
       for (int j = 0; j < 3; ++j) {
         const int g = lane + 32 * j;
@@ -290,28 +427,6 @@ SSB_DEVICE void stage_q(const MlaDecodeArgs& a, uint8_t* smem, int64_t t, int h0
   }
 }
 
-// A CTA's share of one row: units [b0, b1) of the row's nb planned ones; every role walks the same segments.
-struct Segment {
-  int64_t t;
-  int b0, b1, nb;
-};
-struct Walk {
-  int64_t t, at, hi, first;
-  SSB_DEVICE bool next(const MlaDecodeArgs& a, Segment& s) {
-    for (; t < a.T && at < hi; ++t) {
-      const int nb = row_units(a, t);
-      if (nb == 0) continue;
-      const int64_t end = min(hi, first + nb);
-      s.t = t, s.b0 = static_cast<int>(at - first), s.b1 = static_cast<int>(end - first), s.nb = nb;
-      at = end;
-      first += nb;
-      ++t;
-      return true;
-    }
-    return false;
-  }
-};
-
 template <bool Q8>
 __global__ void __launch_bounds__(kThreads, 1)
     mla_decode_kernel(const __grid_constant__ CUtensorMap mlat, const __grid_constant__ CUtensorMap mrope,
@@ -321,12 +436,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int cta = blockIdx.x, tile = blockIdx.y;
   const int h0 = tile * kTileH, nh = min(kTileH, a.H - h0);
   const uint32_t sbase = smem_u32(smem), bar = sbase + kOffBar;
-  const Bars B = {bar, bar + 16, bar + 48, bar + 56, bar + 64, bar + 72, bar + 80, bar + 88, bar + 96};
+  const Bars B = {bar,       bar + 64,  bar + 128, bar + 136, bar + 144, bar + 152,
+                  bar + 160, bar + 168, bar + 176, bar + 184, bar + 192, bar + 200};
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kOffMisc);
   volatile int32_t* abort_flag = reinterpret_cast<volatile int32_t*>(smem + kOffMisc + 4);
   volatile int32_t* last_unit = reinterpret_cast<volatile int32_t*>(smem + kOffMisc + 8);     // [2]
   volatile uint32_t* mask = reinterpret_cast<volatile uint32_t*>(smem + kOffMask);
-  if (sbase & 1023) {                                    // the swizzled tiles need it; no static shared memory precedes
+  if (sbase != kBase) {                                  // no static shared memory precedes
     if (tid == 0) raise_status(a.status, kErrCuda);
     return;
   }
@@ -340,16 +456,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     walk = {p.row, lo, hi, p.first};
   }
   if (tid == 0) {
-    mbar_init(B.kv_full, 33 * kGatherWarps);             // every lane's copies, one arrive a warp for the mask
-    mbar_init(B.kv_full + 8, 33 * kGatherWarps);
-    for (int i = 0; i < 4; ++i) mbar_init(B.kv_empty + 8 * i, 1);
-    mbar_init(B.q_full, kSoftmax);
+    for (int i = 0; i < 8; ++i) {                        // every gather lane's copies; for the last chunk also an
+      mbar_init(B.lat_full + 8 * i, 128 + ((i & 3) == 3 ? kGatherWarps : 0));      // arrival a warp for its mask word
+      mbar_init(B.lat_empty + 8 * i, 1);
+    }
+    mbar_init(B.rope_full, 128);
+    mbar_init(B.rope_empty, 1);
+    mbar_init(B.q_full, kSoftWarps);
     mbar_init(B.s_full, 1);
-    mbar_init(B.s_empty, kSoftmax);
-    mbar_init(B.p_full, kSoftmax);
+    mbar_init(B.s_empty, kSoftWarps);
+    mbar_init(B.p_full, kSoftWarps);
     mbar_init(B.pv_done, 1);
     mbar_init(B.o_full, 1);
-    mbar_init(B.drain, 1);
+    mbar_init(B.drain, 2);
+    for (int i = 0; i < 2; ++i) mbar_init(B.agree + 8 * i, 4);
+    for (int i = 0; i < 4; ++i) reinterpret_cast<int32_t*>(smem + kOffRise)[i] = 0;
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -360,11 +481,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();                                       // also: every thread has read the plan's words
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  constexpr uint32_t tmem = 0;                           // the whole of TMEM: its first lane and column
+  if (*tmem_slot != tmem && tid == 0) {
+    *abort_flag = 1;
+    raise_status(a.status, kErrCuda);
+  }
 
-  if (warp > kMmaWarp) {
+  if (warp >= kGatherWarp) {
     // ---------------------------------------------------------------- gather: warp w brings tokens 32 w .. 32 w + 31
-    const int w = warp - kMmaWarp - 1;
+    const int w = warp - kGatherWarp;
     if (w == 0 && lane == 0) {
       tma_prefetch_desc(&mlat);
       tma_prefetch_desc(&mrope);
@@ -411,8 +536,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       int c = next_live(c0);
       int slot = slot_at(c);
-      // the tiles of this warp's lane 0: its half of the unit's tokens (w >> 1), latent chunks 0, 1 and the rope, or 2, 3
-      const int ch = 2 * (w & 1);
       auto whole_page = [&](int c, int slot) {           // the same in every lane and warp
         return idx == nullptr && (c + 1) * kUnit <= len && slot >= 0 && slot - (32 * w + lane) + kUnit <= a.cache_rows;
       };
@@ -420,54 +543,78 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane != 0 || idx != nullptr || c >= c1) return;
         const int sl = slot_at(c);                       // the first token of the warp's quarter
         if (!whole_page(c, sl)) return;
-        const int y = sl - 32 * w + 64 * (w >> 1);
-        tma_prefetch_2d(&mlat, 128 * ch, y);
-        tma_prefetch_2d(&mlat, 128 * ch + 128, y);
-        if (ch == 0) tma_prefetch_2d(&mrope, kDv, y);
+        tma_prefetch_2d(&mlat, 128 * w, sl - 32 * w);
+        if (w == 0) tma_prefetch_2d(&mrope, kDv, sl);
       };
       for (int i = 0; i < kAhead; ++i) prefetch(c0 + 2 + i);
       while (c < c1) {
         const int buf = u & 1, cn = next_live(c + 1);
         const int slot_n = cn < c1 ? slot_at(cn) : -1;
         prefetch(c + 2 + kAhead);
-        if (u >= 2) ok = mbar_wait(B.kv_empty + 16 * buf + 8 * (w >> 1), ((u >> 1) - 1) & 1, abort_flag, a.status);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const uint32_t dst = sbase + kOffKv + buf * kRows, full = B.kv_full + 8 * buf;
+        const uint32_t full = B.lat_full + 32 * buf, empty = B.lat_empty + 32 * buf, parity = ((u >> 1) - 1) & 1;
+        const uint32_t dst = sbase + kOffKv + buf * kLat;
         const uint32_t present = __ballot_sync(0xffffffffu, slot >= 0);
-        // a whole page comes as tiles; a row's last page, and selected tokens, row by row: rows that are not there have
-        // to be zeros (whatever the cache holds there, NaN too, would meet weight 0 in the value product)
+        // a whole page comes as tiles, a chunk a warp; a row's last page, and selected tokens, row by row: rows that are
+        // not there have to be zeros (whatever the cache holds there, NaN too, would meet weight 0 in the value product)
         if (whole_page(c, slot)) {
           if (lane == 0) {
-            const int hf = w >> 1, y = slot - 32 * w + 64 * hf;
-            const uint32_t d0 = dst + ch * kChunk + hf * (kChunk / 2);
-            mbar_arrive_expect_tx(full, kChunk + (ch == 0 ? kRope / 2 : 0));
-            tma_load_2d(d0, &mlat, 128 * ch, y, full);
-            tma_load_2d(d0 + kChunk, &mlat, 128 * ch + 128, y, full);
-            if (ch == 0) tma_load_2d(dst + 4 * kChunk + hf * (kRope / 2), &mrope, kDv, y, full);
-          } else {
-            mbar_arrive(full);
-          }
-        } else {
-          const uint32_t lat = dst + (lane >> 3) * kChunk + 4096 * w;
-          const uint8_t* src = a.kv + 16 * lane;
-#pragma unroll 16
-          for (int r = 0; r < 32; ++r) {                 // a warp instruction a token: its 512 latent bytes
-            const int sl = __shfl_sync(0xffffffffu, slot, r);
-            cp_async16(lat + sw128(r, lane & 7), src + (int64_t)max(sl, 0) * kDq, sl >= 0);
-          }
+            const int y = slot - 32 * w;
+            // (a warp arrives for a unit only after the phase before is complete: its keys have been used)
+            if (u >= 1) ok = mbar_nap(B.rope_empty, (u - 1) & 1, abort_flag, a.status);
+            if (ok && w == 0) {
+              mbar_arrive_expect_tx(B.rope_full, kRope);
+              mbar_arrive_n(B.rope_full, 31);
+              tma_load_2d(sbase + kOffRope, &mrope, kDv, y, B.rope_full);
+            } else if (ok) {
+              mbar_arrive_n(B.rope_full, 32);
+            }
+            if (ok && u >= 2) ok = mbar_nap(empty + 8 * w, parity, abort_flag, a.status);
+            if (ok) {
+              mbar_arrive_expect_tx(full + 8 * w, kChunk);
+              mbar_arrive_n(full + 8 * w, 31);
+              tma_load_2d(dst + w * kChunk, &mlat, 128 * w, y, full + 8 * w);
+            }
 #pragma unroll
-          for (int r = 0; r < 32; r += 8) {              // 8 tokens: their 64 rope bytes
+            for (int j = 0; j < 3; ++j)
+              if (j != w) mbar_arrive_n(full + 8 * j, 32);
+            // the mask words and flag of the unit two before are read by now: its last chunk's values are done
+            if (w != 3 && ok && u >= 2) ok = mbar_nap(empty + 24, parity, abort_flag, a.status);
+            if (w != 3) mbar_arrive_n(full + 24, 32);
+          }
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+        } else {
+          if (u >= 1) ok = mbar_nap(B.rope_empty, (u - 1) & 1, abort_flag, a.status);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+#pragma unroll
+          for (int r = 0; r < 32; r += 8) {              // 8 tokens a warp instruction: their 64 rope bytes
             const int sl = __shfl_sync(0xffffffffu, slot, r + (lane >> 2));
-            cp_async16(dst + 4 * kChunk + sw64(32 * w + r + (lane >> 2), lane & 3),
+            cp_async16(sbase + kOffRope + sw64(32 * w + r + (lane >> 2), lane & 3),
                        a.kv + (int64_t)max(sl, 0) * kDq + kDv + 16 * (lane & 3), sl >= 0);
           }
-          cp_async_arrive_noinc(full);                   // fires when this thread's copies have landed
+          cp_async_arrive_noinc(B.rope_full);            // fires when this thread's copies have landed
+          int sl[8];
+#pragma unroll
+          for (int r = 0; r < 8; ++r) sl[r] = __shfl_sync(0xffffffffu, slot, 4 * r + (lane >> 3));
+#pragma unroll 1
+          for (int j = 0; j < 4; ++j) {
+            if (u >= 2) ok = mbar_nap(empty + 8 * j, parity, abort_flag, a.status);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const uint8_t* src = a.kv + 128 * j + 16 * (lane & 7);
+#pragma unroll
+            for (int r = 0; r < 8; ++r)                  // 4 tokens a warp instruction: 128 of their latent bytes
+              cp_async16(dst + j * kChunk + sw128(32 * w + 4 * r + (lane >> 3), lane & 7),
+                         src + (int64_t)max(sl[r], 0) * kDq, sl[r] >= 0);
+            cp_async_arrive_noinc(full + 8 * j);
+          }
+          if (!ok) break;
         }
         if (lane == 0) {
           mask[4 * buf + w] = present;
           if (w == 0) last_unit[buf] = cn >= c1;
-          mbar_arrive(full);
+          mbar_arrive(full + 24);
         }
         ++u;
         c = cn;
@@ -475,98 +622,66 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     cp_async_wait_all();
-  } else if (warp == kMmaWarp) {
-    // ---------------------------------------------------------------- MMA issue (one thread)
-    if (lane == 0) {
-      constexpr uint32_t idesc_s = idesc_e4m3(128, Q8 ? 64 : 128);
-      // descriptors of the operands' first tiles; a tile further on is an addition to the address field
-      const uint64_t dq = smem_desc(sbase + kOffQ, 0, 1024, kSw128);
-      const uint64_t dqr = smem_desc(sbase + kOffQ + 4 * kChunk, 0, 512, kSw64);
-      const uint64_t dk = smem_desc(sbase + kOffKv, 0, 1024, kSw128);
-      const uint64_t dkr = smem_desc(sbase + kOffKv + 4 * kChunk, 0, 512, kSw64);
-      const uint64_t dv = smem_desc(sbase + kOffKv, kChunk, 1024, kSw128);
-      const uint64_t dph = smem_desc(sbase + kOffKv + 4 * kChunk, kRope, 512, kSw64);
-      const uint64_t dpl = smem_desc(sbase + kOffPlo, kRope, 512, kSw64);
-      const uint64_t dsf = smem_desc(sbase + kOffSf, 0, 128, 0);
-      int uq = 0, up = 0, seg = 0;                       // units whose scores, whose values have been issued
-      Segment s;
-      bool ok = true;
-      auto scores = [&](int v) {                         // S^T [tokens, heads] = K Q^T of unit v
-        const uint64_t k = dk + (v & 1) * (kRows >> 4), kr = dkr + (v & 1) * (kRows >> 4);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-#pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            tc_mma_f8(tmem + kColS, k + ((c * kChunk + ks * 32) >> 4), dq + ((c * kChunk + ks * 32) >> 4), idesc_s,
-                      (c | ks) != 0 ? 1u : 0u);
-        }
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)                   // the rope chunk: 64 bytes a row
-          tc_mma_f8(tmem + kColS, kr + ((ks * 32) >> 4), dqr + ((ks * 32) >> 4), idesc_s, 1u);
-        tc_commit(B.s_full);
-      };
-      auto values = [&](int v, bool fresh) {             // O^T [dims, heads] (+)= V^T P^T of unit v, high then low parts
-        const uint64_t kv = dv + (v & 1) * (kRows >> 4), ph = dph + (v & 1) * (kRows >> 4);
-        tc_cp_sf(tmem + kColP, dsf);
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {                 // 32 tokens a step: one block of scales
-#pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            const uint64_t ad = kv + ((d * kChunk + ks * 4096) >> 4);
-            tc_mma_mx(tmem + kColO + 64 * d, ad, ph + ((ks * 2048) >> 4), idesc_mx(128, 64, ks),
-                      fresh && ks == 0 ? 0u : 1u, tmem + kColOne, tmem + kColP);
-            tc_mma_mx(tmem + kColO + 64 * d, ad, dpl + ((ks * 2048) >> 4), idesc_mx(128, 64, ks), 1u, tmem + kColLow,
-                      tmem + kColP);
-          }
-          if (ks & 1) tc_commit(B.kv_empty + 16 * (v & 1) + 8 * (ks >> 1));     // 64 tokens' rows are free
-        }
-        tc_commit(B.pv_done);
-      };
-      while (ok && walk.next(a, s)) {
-        ok = mbar_wait(B.q_full, seg & 1, abort_flag, a.status);
-        bool fresh = true, last = false;
-        unsigned long long t0 = globaltimer();
-        while (ok && !(last && up == uq)) {
-          // whichever is ready: the next unit's scores first, else the values of the one whose weights are there
-          if (!last && mbar_test(B.kv_full + 8 * (uq & 1), (uq >> 1) & 1) &&
-              (uq == 0 || mbar_test(B.s_empty, (uq - 1) & 1))) {
-            last = last_unit[uq & 1] != 0;
-            fence_proxy_async_smem();                    // rows brought by other threads' copies -> the tensor core
-            tc_fence_after();
-            scores(uq++);
-          } else if (up < uq && mbar_test(B.p_full, up & 1)) {
-            tc_fence_after();
-            values(up++, fresh);
-            fresh = false;
-          } else {
-            if (*abort_flag) ok = false;
-            if (globaltimer() - t0 > kWaitNs) {
-              *abort_flag = 1;
-              raise_status(a.status, kErrTimeout);
-              ok = false;
-            }
-            continue;
-          }
-          t0 = globaltimer();
-        }
-        if (ok) tc_commit(B.o_full);
-        ++seg;
+  } else if (warp == kValueWarp) {
+    // ---------------------------------------------------------------- value products
+    const bool leader = elect_lane();
+    int u = 0;
+    Segment s;
+    bool ok = true;
+    while (ok && walk.next(a, s)) {
+      bool last = false, fresh = true;
+      while (!last) {
+        ok = mbar_nap(B.p_full, u & 1, abort_flag, a.status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        last = last_unit[u & 1] != 0;
+        tc_fence_after();
+        issue_values(B, sbase, u & 1, fresh, leader);
+        fresh = false;
+        ++u;
       }
-      tc_commit(B.drain);                                // everything issued has completed when this arrives
-      const unsigned long long t0 = globaltimer();
-      while (!mbar_try_wait(B.drain, 0) && globaltimer() - t0 <= kWaitNs) {}
+      if (ok && leader) tc_commit(B.o_full);
     }
+    if (leader) tc_commit(B.drain);                      // everything issued here has completed when this arrives
+  } else if (warp == kScoreWarp) {
+    // ---------------------------------------------------------------- score products
+    const bool leader = elect_lane();
+    int u = 0, seg = 0;
+    Segment s;
+    bool ok = true;
+    while (ok && walk.next(a, s)) {
+      ok = mbar_nap(B.q_full, seg & 1, abort_flag, a.status);
+      bool last = false;
+      while (!last) {
+        if (ok) ok = mbar_nap(B.rope_full, u & 1, abort_flag, a.status);
+        if (ok && u > 0) ok = mbar_nap(B.s_empty, (u - 1) & 1, abort_flag, a.status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        fence_proxy_async_smem();                        // rows that threads copied -> the tensor core
+        tc_fence_after();
+        ok = issue_scores<Q8>(B, sbase, u & 1, (u >> 1) & 1, leader, abort_flag, a.status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        last = last_unit[u & 1] != 0;
+        ++u;
+      }
+      ++seg;
+    }
+    if (leader) tc_commit(B.drain);
+    const unsigned long long t0 = globaltimer();
+    while (!mbar_try_wait(B.drain, 0) && globaltimer() - t0 <= 2 * kWaitNs) {}
+    __syncwarp();
   } else {
     // ---------------------------------------------------------------- softmax (warps 0-7): a token and 32 heads a thread
     const int quarter = warp & 3, half = warp >> 2, hb = 32 * half, bid = 1 + half;
     const int row = 32 * quarter + lane;
     const uint32_t tq = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
-    float2* scale = reinterpret_cast<float2*>(smem + kOffScale);
+    float* scale = reinterpret_cast<float*>(smem + kOffScale);
     float* part = reinterpret_cast<float*>(smem + kOffExp);
     float* sums = reinterpret_cast<float*>(smem + kOffSum);
-    uint8_t* sf = smem + kOffSf;
-    if (half == 0) tmem_st_x4(tq + kColOne, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu);   // 1
-    else tmem_st_x4(tq + kColLow, 0x7B7B7B7Bu, 0x7B7B7B7Bu, 0x7B7B7B7Bu, 0x7B7B7B7Bu);            // 2^-4
+    volatile int32_t* far = reinterpret_cast<volatile int32_t*>(smem + kOffRise);
+    if (half == 0) tmem_st_x4(tq + kColV, 0x78787878u, 0x78787878u, 0x78787878u, 0x78787878u);   // 2^-7
+    else tmem_st_x4(tq + kColLow, 0x74747474u, 0x74747474u, 0x74747474u, 0x74747474u);          // 2^-11
     tmem_st_wait();
     int u = 0, seg = 0;
     Segment s, s_next;
@@ -574,47 +689,69 @@ __global__ void __launch_bounds__(kThreads, 1)
     stage_q<Q8>(a, smem, s.t, h0, nh, warp, lane);
     fence_proxy_async_smem();
     tc_fence_before();
-    mbar_arrive(B.q_full);
+    warp_arrive(B.q_full, lane);
     named_bar(3, kSoftmax);                              // every head's scale is written
     while (more) {
-      float l[32];
+      uint64_t l[16];                                    // the thread's sums of heads hb + 2 i, hb + 2 i + 1
 #pragma unroll
-      for (int h = 0; h < 32; ++h) l[h] = 0.0f;
-      float ref = -INFINITY;                             // reference of head hb + lane (the same in the 4 quarters)
+      for (int i = 0; i < 16; ++i) l[i] = 0;
+      float ref = hb + lane < nh ? -INFINITY : -kNoHead; // reference of head hb + lane (the same in the 4 quarters)
       bool last = false, fresh = true, unset = true;
       while (!last) {
         const int buf = u & 1;
-        ok = mbar_wait(B.s_full, u & 1, abort_flag, a.status);
-        if (ok) ok = mbar_wait(B.kv_full + 8 * buf, (u >> 1) & 1, abort_flag, a.status);   // the mask's writes
+        ok = mbar_nap(B.s_full, u & 1, abort_flag, a.status);
+        if (ok) ok = mbar_nap(B.lat_full + 32 * buf + 24, (u >> 1) & 1, abort_flag, a.status);   // the mask's writes
         tc_fence_after();
         last = last_unit[buf] != 0;
         const uint32_t present = mask[4 * buf + quarter];
-        const bool valid = (present >> lane) & 1;
-        float p[32];
+        uint64_t p[16];
+        float top[8];                                    // of 4 heads each: the warp's largest
         auto load_scores = [&]() {                       // base-2 scores less the reference; tokens not there: -inf
-          float y[32];
-          tmem_ld_32x32b_x32(tq + kColS + hb, p);
-          if (!Q8) tmem_ld_32x32b_x32(tq + kColS + 64 + hb, y);
-          tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float4 c = *reinterpret_cast<const float4*>(scale + hb + i);
-            p[i] = fmaf(Q8 ? p[i] : fmaf(y[i], 0.0625f, p[i]), c.x, c.y);
-            p[i + 1] = fmaf(Q8 ? p[i + 1] : fmaf(y[i + 1], 0.0625f, p[i + 1]), c.z, c.w);
+          for (int j = 0; j < 32; j += 16) {
+            float x[16], y[16];
+            tmem_ld_x16(tq + kColS + hb + j, x);
+            if (!Q8) tmem_ld_x16(tq + kColS + 64 + hb + j, y);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+              const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(scale + hb + j + i);
+              const ulonglong2 r = *reinterpret_cast<const ulonglong2*>(scale + 64 + hb + j + i);
+              uint64_t v = f2pack(x[i], x[i + 1]), w = f2pack(x[i + 2], x[i + 3]);
+              if (!Q8) {
+                v = fma2(f2pack(y[i], y[i + 1]), f2pack(0.0625f, 0.0625f), v);
+                w = fma2(f2pack(y[i + 2], y[i + 3]), f2pack(0.0625f, 0.0625f), w);
+              }
+              p[(j + i) / 2] = fma2(v, c.x, r.x);
+              p[(j + i) / 2 + 1] = fma2(w, c.y, r.y);
+            }
           }
-          if (present != 0xffffffffu) {
+          if (present != 0xffffffffu && !((present >> lane) & 1)) {
 #pragma unroll
-            for (int h = 0; h < 32; ++h) p[h] = valid ? p[h] : -INFINITY;
+            for (int i = 0; i < 16; ++i) p[i] = f2pack(-INFINITY, -INFINITY);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float v0, v1, v2, v3;
+            f2unpack(p[2 * i], v0, v1);
+            f2unpack(p[2 * i + 1], v2, v3);
+            top[i] = warp_max(fmaxf(fmaxf(v0, v1), fmaxf(v2, v3)));
           }
         };
         load_scores();
-        float top = p[0];
+        float most = top[0];
 #pragma unroll
-        for (int h = 1; h < 32; ++h) top = fmaxf(top, p[h]);
-        // the four quarters agree on the rare path; a failed wait travels the same way
-        const bool rise = named_bar_or(bid, kHalf, unset || top > kMaxRise || !ok);
-        if (rise) {
-          if (named_bar_or(bid, kHalf, !ok)) {
+        for (int i = 1; i < 8; ++i) most = fmaxf(most, top[i]);
+        // the four quarters of a half agree on the rare path (a failed wait travels the same way)
+        if (lane == 0) {
+          if (unset || most > kMaxRise || !ok) far[2 * buf + half] = 1;
+          mbar_arrive(B.agree + 8 * half);
+        }
+        if (!mbar_nap(B.agree + 8 * half, u & 1, abort_flag, a.status)) ok = false;
+        // (a quarter sets the next unit's flag at the earliest after this one is agreed on, and this buffer's next flag
+        // after the next agreement: cleared here, it is not lost)
+        if (far[2 * buf + half]) {
+          if (named_bar_or(bid, kGroup, !ok)) {
             ok = false;
             break;
           }
@@ -622,11 +759,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           // unit's largest score; what it has accumulated is rescaled
           const float old = ref == -INFINITY ? 0.0f : ref;
 #pragma unroll
-          for (int h = 0; h < 32; ++h) {
-            const float m = warp_max(p[h]);
-            if (lane == 0) part[64 * quarter + hb + h] = m;
+          for (int i = 0; i < 16; ++i) {
+            float v0, v1;
+            f2unpack(p[i], v0, v1);
+            v0 = warp_max(v0), v1 = warp_max(v1);
+            if (lane == 0) *reinterpret_cast<float2*>(part + 64 * quarter + hb + 2 * i) = make_float2(v0, v1);
           }
-          named_bar(bid, kHalf);
+          named_bar(bid, kGroup);
           float m = -INFINITY;
 #pragma unroll
           for (int k = 0; k < 4; ++k) m = fmaxf(m, part[64 * k + hb + lane]);
@@ -637,82 +776,89 @@ __global__ void __launch_bounds__(kThreads, 1)
           unset = __any_sync(0xffffffffu, ref == -INFINITY);
           if (quarter == 0) {
             sums[hb + lane] = f;
-            scale[hb + lane].y = -now;
+            scale[64 + hb + lane] = -now;
+            if (lane == 0) far[2 * buf + half] = 0;
           }
           const bool scaled = __any_sync(0xffffffffu, f != 1.0f);
-          named_bar(bid, kHalf);
+          named_bar(bid, kGroup);
           if (scaled && !fresh) {
 #pragma unroll
-            for (int h = 0; h < 32; ++h) l[h] *= sums[hb + h];
-            ok = mbar_wait(B.pv_done, (u - 1) & 1, abort_flag, a.status);
+            for (int i = 0; i < 16; ++i) l[i] = mul2(l[i], *reinterpret_cast<const uint64_t*>(sums + hb + 2 * i));
+            if (!mbar_nap(B.pv_done, (u - 1) & 1, abort_flag, a.status)) ok = false;
             tc_fence_after();
 #pragma unroll 1
             for (int d = 0; d < 4; ++d) {
-              tmem_ld_32x32b_x32(tq + kColO + 64 * d + hb, p);
+              float o[32];
+              tmem_ld_32x32b_x32(tq + kColO + 64 * d + hb, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int h = 0; h < 32; ++h) p[h] *= sums[hb + h];
-              tmem_st_32x32b_x32(tq + kColO + 64 * d + hb, p);
+              for (int h = 0; h < 32; ++h) o[h] *= sums[hb + h];
+              tmem_st_32x32b_x32(tq + kColO + 64 * d + hb, o);
             }
             tmem_st_wait();
           }
           load_scores();
         }
         tc_fence_before();
-        mbar_arrive(B.s_empty);
-        // weights 2^score; then each head's largest over the warp's 32 tokens gives their block scale: its exponent E
-        // moves the weights to [2^7, 2^8) at most, the scale 2^(E - 134) moves them back in the product
-        uint32_t wh[8], wl[8], mine = 0;
+        warp_arrive(B.s_empty, lane);
+        // weights 2^(score - E + 8) with an exponent E for the warp's 32 tokens and 4 heads: the ceiling of the largest of
+        // their scores above the heads' references. 2^(E - 8) is their block scale in the product and their weight in the
+        // sums; the e4m3 pairs keep 8 bits down to 2^-14 of that largest.
+        uint32_t wh[8], wl[8];
+        uint8_t* sf = smem + kOffSf + 8 * buf + 4 * half + quarter;
 #pragma unroll
-        for (int h = 0; h < 32; ++h) {
-          p[h] = ex2_fast(p[h]);
-          l[h] += p[h];
-        }
+        for (int i = 0; i < 8; ++i) {
+          const float e = fminf(fmaxf(ceilf(top[i]), -100.0f), kMaxRise);
+          const uint32_t eb = static_cast<uint32_t>(static_cast<int>(e) + 119);        // biased exponent of 2^(E - 8)
+          const uint64_t off = f2pack(8.0f - e, 8.0f - e);
+          const uint64_t unit = f2pack(__uint_as_float(eb << 23), __uint_as_float(eb << 23));
+          if (lane < 4) sf[16 * (4 * i + lane)] = static_cast<uint8_t>(eb + 7);         // V's scale is 2^-7
+          uint32_t ph[2], pl[2];
 #pragma unroll
-        for (int h = 0; h < 32; h += 4) {
-          uint32_t part_hi[2], part_lo[2];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t e = max(__reduce_max_sync(0xffffffffu, __float_as_uint(p[h + k])) & 0x7F800000u, 12u << 23);
-            p[h + k] *= __uint_as_float((261u << 23) - e);
-            mine = lane == h + k ? e : mine;
+          for (int k = 0; k < 2; ++k) {
+            float w0, w1;
+            f2unpack(add2(p[2 * i + k], off), w0, w1);
+            w0 = ex2_fast(w0), w1 = ex2_fast(w1);
+            l[2 * i + k] = fma2(f2pack(w0, w1), unit, l[2 * i + k]);
+            split2(w0, w1, ph[k], pl[k]);
           }
-          split2(p[h], p[h + 1], part_hi[0], part_lo[0]);
-          split2(p[h + 2], p[h + 3], part_hi[1], part_lo[1]);
-          wh[h / 4] = part_hi[0] | (part_hi[1] << 16);
-          wl[h / 4] = part_lo[0] | (part_lo[1] << 16);
+          wh[i] = ph[0] | (ph[1] << 16);
+          wl[i] = pl[0] | (pl[1] << 16);
         }
-        if (u > 0 && !mbar_wait(B.pv_done, (u - 1) & 1, abort_flag, a.status)) ok = false;   // its P and scales are read
-        sf[16 * lane + 4 * half + quarter] = static_cast<uint8_t>((mine >> 23) - 7);
-        uint8_t* ph = smem + kOffKv + buf * kRows + 4 * kChunk;
-        uint8_t* pl = smem + kOffPlo;
+        if (u > 0 && !mbar_nap(B.pv_done, (u - 1) & 1, abort_flag, a.status)) ok = false;   // its P has been read
 #pragma unroll
         for (int g = 0; g < 2; ++g) {                    // 16 heads a 16-byte granule
-          *reinterpret_cast<uint4*>(ph + sw64(row, 2 * half + g)) = make_uint4(wh[4 * g], wh[4 * g + 1], wh[4 * g + 2], wh[4 * g + 3]);
-          *reinterpret_cast<uint4*>(pl + sw64(row, 2 * half + g)) = make_uint4(wl[4 * g], wl[4 * g + 1], wl[4 * g + 2], wl[4 * g + 3]);
+          *reinterpret_cast<uint4*>(smem + kOffPhi + sw64(row, 2 * half + g)) =
+              make_uint4(wh[4 * g], wh[4 * g + 1], wh[4 * g + 2], wh[4 * g + 3]);
+          *reinterpret_cast<uint4*>(smem + kOffPlo + sw64(row, 2 * half + g)) =
+              make_uint4(wl[4 * g], wl[4 * g + 1], wl[4 * g + 2], wl[4 * g + 3]);
         }
         fence_proxy_async_smem();
         tc_fence_before();
-        mbar_arrive(B.p_full);
+        warp_arrive(B.p_full, lane);
         fresh = false;
         ++u;
       }
       // ---- the row's sums, the next row's query, then the accumulators ----
-      const float ls = warp_sum_transposed(l, lane);
+      float lf[32];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) f2unpack(l[i], lf[2 * i], lf[2 * i + 1]);
+      const float ls = warp_sum_transposed(lf, lane);
       if (named_bar_or(3, kSoftmax, !ok)) break;
       part[64 * quarter + hb + lane] = ls;
       named_bar(3, kSoftmax);
       float total = 0.0f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) total += part[64 * k + hb + lane];
+      if (ref == -INFINITY && total == total) total = 0.0f;                          // no token
       if (quarter == 0) sums[hb + lane] = total == 0.0f ? 0.0f : a.bmm2 / total;     // a NaN sum stays one
       more = walk.next(a, s_next);
       if (more) {
         stage_q<Q8>(a, smem, s_next.t, h0, nh, warp, lane);
         fence_proxy_async_smem();
-        mbar_arrive(B.q_full);
+        warp_arrive(B.q_full, lane);
       }
-      ok = mbar_wait(B.o_full, seg & 1, abort_flag, a.status);
+      ok = mbar_nap(B.o_full, seg & 1, abort_flag, a.status);
       if (named_bar_or(3, kSoftmax, !ok)) break;
       tc_fence_after();
       const bool whole = s.b0 == 0 && s.b1 == s.nb;
@@ -843,13 +989,18 @@ int launch_mla_decode(const MlaDecodeArgs& a_in, void* ws, int64_t ws_bytes, cud
   auto* kernel = a.q_e4m3 ? mla_decode_kernel<true> : mla_decode_kernel<false>;
   static bool attr[2] = {false, false};
   if (!attr[a.q_e4m3]) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return kErrCuda;
+    int dev = 0, reserved = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&reserved, cudaDevAttrReservedSharedMemoryPerBlock, dev) != cudaSuccess ||
+        reserved != (int)kBase ||
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
+      return kErrCuda;
     attr[a.q_e4m3] = true;
   }
   CUtensorMap mlat, mrope;
   const int u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
-  int rc = make_map_2d_ex(&mlat, u8, a.kv, a.cache_rows, kDq, kDq, 128, kUnit / 2, CU_TENSOR_MAP_SWIZZLE_128B);
-  if (rc == kOk) rc = make_map_2d_ex(&mrope, u8, a.kv, a.cache_rows, kDq, kDq, 64, kUnit / 2, CU_TENSOR_MAP_SWIZZLE_64B);
+  int rc = make_map_2d_ex(&mlat, u8, a.kv, a.cache_rows, kDq, kDq, 128, kUnit, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc == kOk) rc = make_map_2d_ex(&mrope, u8, a.kv, a.cache_rows, kDq, kDq, 64, kUnit, CU_TENSOR_MAP_SWIZZLE_64B);
   if (rc != kOk) return rc;
   kernel<<<dim3((unsigned)(kMaxCtas / tiles), (unsigned)tiles), kThreads, kSmem, stream>>>(mlat, mrope, a);
   if (cudaGetLastError() != cudaSuccess) return kErrCuda;
