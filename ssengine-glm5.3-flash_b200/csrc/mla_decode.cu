@@ -6,9 +6,27 @@
 // Split: a row of n tokens is ceil(n / 128) units of work; the units of all rows, in row order, are cut into equal
 // contiguous ranges, one per CTA (two rows or more may share a CTA, one row may span many). A CTA works through its
 // range row by row; a row that lies in one range is finished there, the parts of a row cut between ranges go to the
-// workspace as (running max m, sum l, unnormalised O) in fp32 and are joined by a second kernel:
+// workspace as (reference m, sum l, unnormalised O) in fp32 and are joined by a second kernel:
 //   M = max_i m_i;  O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.
 // No atomics and a fixed order of the sums: the same inputs give the same bits.
+//
+// One CTA of 22 warps an SM, over units of 128 tokens and a tile of 64 heads:
+//   gather (4 warps): a whole page as TMA tiles (4 chunks [128 tokens x 128 B] and the rope keys), a row's last page and
+//       selected tokens by cp.async row by row, what is not there zero-filled; pages ahead prefetched into L2;
+//   scores (1 warp issues): S^T [128 tokens x 64 heads] = K Q^T, tcgen05 kind::f8f6f4, M = 128. bf16 queries enter
+//       exactly, as two e4m3 parts (64 high rows, 64 low ones, N = 128): the half of the tensor core that 64 heads alone
+//       would leave idle;
+//   softmax (16 warps, a token and 16 heads a thread): weights 2^(s - E), E one exponent for 32 tokens x 4 heads, again
+//       as two e4m3 parts (8 bits), with 2^E as the ue8m0 block scale of the second product. The accumulators stand
+//       against a reference per head that moves only when scores rise 2^4 above it;
+//   values (1 warp issues): O^T [512 dims x 64 heads] += V^T P^T, kind::mxf8f6f4, 4 tiles of M = 128, N = 64, from the same
+//       rows read the other way round.
+// TMEM: O^T 256 columns, S^T 128, block scales. Shared memory: query parts 72 KB, latent rows 2 x 64 KB, rope keys 8 KB
+// (needed for the scores only), P 16 KB.
+// Bounds: 576 bytes a token from HBM against 64 x 2,176 products of 8 bits: 2,700 cycles a unit at the measured copy
+// rate, and as many for the two products, which read shared memory at its full rate (18 instructions of 64 cycles, 32 of
+// 48). One thread's instruction stream matters as much: the roles' loops are kept small because they share 28 KB of
+// instruction cache.
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -18,115 +36,51 @@ namespace ssb {
 namespace {
 
 constexpr int kDq = 576, kDv = 512, kUnit = 128, kTileH = 64;
-constexpr int kMaxCtas = 148;                  // ranges a call is cut into at most (the workspace is sized by it)
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMaxCtas = 148;                   // ranges a call is cut into at most (the workspace is sized by it)
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kNone = -INFINITY;
 
-struct Plan {                                   // the row of a CTA's first unit
-  int row;
-  int64_t first;                                // units before that row
-};
-
-// Tokens and units of row t. How many tokens a row's list names is not known before it is read: its share is planned
-// by the list's width or, where that is smaller, the tokens it can name.
-SSB_DEVICE int row_bound(const MlaDecodeArgs& a, int64_t t) {
-  int64_t n = a.indices != nullptr ? a.n_idx : (int64_t)a.width * kUnit;
-  if (a.seq_lens != nullptr) n = min(n, (int64_t)a.seq_lens[t]);
-  if (a.reqs != nullptr && (a.reqs[t] < 0 || a.reqs[t] >= a.R)) n = 0;
-  return n > 0 ? static_cast<int>(n) : 0;
-}
-SSB_DEVICE int row_units(const MlaDecodeArgs& a, int64_t t) { return (row_bound(a, t) + kUnit - 1) / kUnit; }
-
-// All threads of the CTA (256 or more): this CTA's range [lo, hi) of units and the row that holds unit lo.
-constexpr int kScan = 256;
-SSB_DEVICE void find_range(const MlaDecodeArgs& a, int cta, int ctas, int64_t* sh, int64_t& lo, int64_t& hi, Plan& p) {
-  const int tid = threadIdx.x;
-  const bool in = tid < kScan;
-  if (in) {
-    int64_t sum = 0;
-    for (int64_t t = tid; t < a.T; t += kScan) sum += row_units(a, t);
-    sh[tid] = sum;
-  }
-  __syncthreads();
-  for (int o = kScan / 2; o > 0; o >>= 1) {
-    if (tid < o) sh[tid] += sh[tid + o];
-    __syncthreads();
-  }
-  const int64_t total = sh[0];
-  __syncthreads();
-  const int64_t used = min((int64_t)ctas, total);      // every range in use holds a unit: a row's CTAs are consecutive
-  lo = cta < used ? total * cta / used : total;
-  hi = cta < used ? total * (cta + 1) / used : total;
-  if (tid == 0) sh[kScan] = a.T, sh[kScan + 1] = 0;
-  int64_t base = 0;
-  for (int64_t c = 0; c < a.T; c += kScan) {
-    const int64_t t = c + tid;
-    const int64_t n = in && t < a.T ? row_units(a, t) : 0;
-    if (in) sh[tid] = n;
-    __syncthreads();
-    for (int o = 1; o < kScan; o <<= 1) {
-      const int64_t v = in && tid >= o ? sh[tid - o] : 0;
-      __syncthreads();
-      if (in) sh[tid] += v;
-      __syncthreads();
-    }
-    const int64_t end = base + (in ? sh[tid] : 0), beg = end - n;
-    if (n > 0 && beg <= lo && lo < end) sh[kScan] = t, sh[kScan + 1] = beg;
-    base += sh[kScan - 1];
-    __syncthreads();
-    if (base > lo) break;
-  }
-  p.row = static_cast<int>(sh[kScan]);
-  p.first = sh[kScan + 1];
-}
-
-SSB_DEVICE float* part_o(const MlaDecodeArgs& a, int tile, int slot) {
-  return a.part_o + ((int64_t)tile * 2 * kMaxCtas + slot) * kTileH * kDv;
-}
-SSB_DEVICE float2* part_ml(const MlaDecodeArgs& a, int tile, int slot) {
-  return a.part_ml + ((int64_t)tile * 2 * kMaxCtas + slot) * kTileH;
-}
-
-// ---- shared memory ------------------------------------------------------------------------------------------------
-constexpr int kSoftWarps = 8;                   // warps 0-7: token quarter warp & 3, heads 32 (warp >> 2) .. + 31
+constexpr int kSoftWarps = 16;                  // warps 0-15: token quarter warp & 3, heads 16 (warp >> 2) .. + 15
 constexpr int kSoftmax = 32 * kSoftWarps;
-constexpr int kGroup = 128;                     // threads of one half of the heads
-constexpr int kScoreWarp = kSoftWarps;          // warp 8 issues the score products
-constexpr int kValueWarp = kScoreWarp + 1;      // warp 9 the value products
-constexpr int kGatherWarp = kValueWarp + 1;     // warps 10-13 bring the cache rows
+constexpr int kGroup = 128;                     // threads of one group of 16 heads
+constexpr int kScoreWarp = kSoftWarps;          // warp 16 issues the score products
+constexpr int kValueWarp = kScoreWarp + 1;      // warp 17 the value products
+constexpr int kGatherWarp = kValueWarp + 1;     // warps 18-21 bring the cache rows
 constexpr int kGatherWarps = 4;
 constexpr int kThreads = 32 * (kGatherWarp + kGatherWarps);
+
+// ---- shared memory ------------------------------------------------------------------------------------------------
 constexpr int kChunk = 16384;                   // [128 rows x 128 B], 128-byte swizzle
 constexpr int kRope = 8192;                     // [128 rows x 64 B], 64-byte swizzle
-constexpr int kRows = 4 * kChunk + kRope;       // 128 rows of 576 bytes: the query tile's parts
 constexpr int kLat = 4 * kChunk;                // a unit's latent rows
-constexpr uint32_t kBase = 1024;                // bytes of a block's shared memory that the system reserves
-constexpr int kOffQ = 0;
-constexpr int kOffKv = kRows;                   // the latent rows of two units
+constexpr int kOffQ = 0;                        // the query tile's parts: 4 chunks and the rope
+constexpr int kOffKv = kLat + kRope;            // the latent rows of two units
 constexpr int kOffRope = kOffKv + 2 * kLat;     // the rope keys of one: free again once its scores are done
 constexpr int kOffPhi = kOffRope + kRope;       // the parts of P
 constexpr int kOffPlo = kOffPhi + kRope;
 constexpr int kOffSf = kOffPlo + kRope;         // block scales of P, two units: byte (h % 32) 16 + unit 8 + (h / 32) 4 + quarter
 constexpr int kOffBar = kOffSf + 512;           // mbarriers
-constexpr int kOffMisc = kOffBar + 256;         // tmem address, abort flag, last-unit flags
-constexpr int kOffRise = kOffMisc + 32;         // int32 [2][2]: a unit with scores far above a half's references
+constexpr int kOffMisc = kOffBar + 256;         // tmem address, abort flag, last-unit flags, plan
+constexpr int kOffRise = kOffMisc + 64;         // int32 [2][4]: a unit with scores far above a group's references
 constexpr int kOffMask = kOffRise + 32;         // uint32 [2][4]: tokens present in a unit
 constexpr int kOffScale = kOffMask + 32;        // float [2][64]: base-2 score scale, minus the reference of each head
 constexpr int kOffExp = kOffScale + 512;        // float [4][64]: maxima of the token quarters, or their sums
 constexpr int kOffSum = kOffExp + 1024;         // float [64]: rescale factors, bmm2 / l
 constexpr int kSmem = kOffSum + 256;
 static_assert(kOffScale % 16 == 0 && kOffExp % 16 == 0 && kOffSf % 128 == 0 && kSmem <= 232448, "shared memory");
-// TMEM columns: O^T as 4 tiles of 128 dims x 64 heads, S^T 128 tokens x (64 high | 64 low), block scales of V
-// (2^-7 against the high parts of P, 2^-11 against the low ones) and of P (2 columns a unit)
+// TMEM columns: O^T as 4 tiles of 128 dims x 64 heads, S^T 128 tokens x (64 high | 64 low), block scales of V (2^-7 against
+// the high parts of P, 2^-11 against the low ones) and of P (2 columns a unit)
 constexpr uint32_t kColO = 0, kColS = 256, kColV = 384, kColLow = 388, kColP = 392;
 constexpr int kAhead = 4;                       // pages prefetched into L2 beyond the two in shared memory
 constexpr float kMaxRise = 4.0f;                // base-2 scores above a head's reference before it moves and O is rescaled
 constexpr float kNoHead = -1000.0f;             // base-2 score of the heads that the tile does not have: weight 0
+constexpr uint32_t kSw128 = 2, kSw64 = 4;       // descriptor layout types
 
 // Block-scaled instruction descriptor (kind::mxf8f6f4): e4m3 A and B (format 0), ue8m0 scales (bit 23), A and B
 // MN-major (bits 15, 16), N >> 3 in [17,23), M >> 4 in [24,29), B's scale byte in [4,6).
-__host__ __device__ constexpr uint32_t idesc_mx(int M, int N, int b_byte) {
-  return (static_cast<uint32_t>(b_byte) << 4) | (1u << 15) | (1u << 16) | (static_cast<uint32_t>(N >> 3) << 17) |
-         (1u << 23) | (static_cast<uint32_t>(M >> 4) << 24);
+__host__ __device__ constexpr uint32_t idesc_mx(int M, int N) {
+  return (1u << 15) | (1u << 16) | (static_cast<uint32_t>(N >> 3) << 17) | (1u << 23) |
+         (static_cast<uint32_t>(M >> 4) << 24);
 }
 // D[tmem] (+)= A B, e4m3 operands with ue8m0 scales for blocks of 32 along the reduction.
 SSB_DEVICE void tc_mma_mx(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t acc, uint32_t sfa,
@@ -138,11 +92,49 @@ SSB_DEVICE void tc_mma_mx(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, 
       "l"(ad), "l"(bd), "r"(idesc), "r"(acc), "r"(sfa), "r"(sfb)
       : "memory");
 }
-SSB_DEVICE void tmem_st_x4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(a), "r"(b), "r"(c),
-               "r"(d)
-               : "memory");
+SSB_DEVICE void tmem_ld_x16(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
+// Two columns of each of the 4 tiles of O^T (64 columns apart).
+SSB_DEVICE void tmem_ld_2x4(uint32_t taddr, float (&v)[8]) {
+  uint32_t r[8];
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];"
+                 : "=r"(r[2 * d]), "=r"(r[2 * d + 1])
+                 : "r"(taddr + 64 * d));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+}
+SSB_DEVICE void tmem_st_x16(uint32_t taddr, const float (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
+      "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
+      : "memory");
+}
+SSB_DEVICE void tmem_st_x4(uint32_t taddr, uint32_t v) {               // one word in 4 columns
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %1, %1, %1};" ::"r"(taddr), "r"(v) : "memory");
+}
+SSB_DEVICE bool elect_lane() {                   // true in one lane of a converged warp
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, e;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
 SSB_DEVICE void cp_async16(uint32_t dst, const void* src, bool valid) {
   const int n = valid ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
@@ -151,6 +143,27 @@ SSB_DEVICE void cp_async_arrive_noinc(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 SSB_DEVICE void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+SSB_DEVICE void tma_prefetch_2d(const CUtensorMap* m, int32_t x, int32_t y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(m)), "r"(x),
+               "r"(y)
+               : "memory");
+}
+
+// Sums over the 32 lanes of 16 values a lane, transposed: lane l receives the total of value l & 15.
+SSB_DEVICE float warp_sum_transposed(float (&v)[16], int lane) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 16);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const float keep = up ? v[i + o] : v[i], send = up ? v[i] : v[i + o];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+    }
+  }
+  return v[0];
+}
 // Largest of the 32 lanes' values, NaN ignored (all NaN: NaN).
 SSB_DEVICE float warp_max(float v) {
   float r;
@@ -161,6 +174,11 @@ SSB_DEVICE float ex2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+SSB_DEVICE uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 // Two halves -> two e4m3 bytes (round to nearest even, the first in the low byte) and back.
 SSB_DEVICE uint32_t half2_e4m3(__half2 v) {
@@ -183,55 +201,31 @@ SSB_DEVICE void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
 // Byte offset of 16-byte granule g of row r: a 128-byte-swizzled chunk, a 64-byte-swizzled one.
 SSB_DEVICE uint32_t sw128(int r, int g) { return r * 128 + ((g ^ (r & 7)) << 4); }
 SSB_DEVICE uint32_t sw64(int r, int g) { return r * 64 + ((g ^ ((r >> 1) & 3)) << 4); }
-constexpr uint32_t kSw128 = 2, kSw64 = 4;       // descriptor layout types
 // Granule g (0-35) of row r of 576 bytes.
-SSB_DEVICE uint32_t row_off(int r, int g) {
-  return g < 32 ? (g >> 3) * kChunk + sw128(r, g & 7) : 4 * kChunk + sw64(r, g - 32);
-}
+SSB_DEVICE uint32_t row_off(int r, int g) { return g < 32 ? (g >> 3) * kChunk + sw128(r, g & 7) : kLat + sw64(r, g - 32); }
 
-// Sums over the 32 lanes of 32 values a lane, transposed: lane l receives the total of value l.
-SSB_DEVICE float warp_sum_transposed(float (&v)[32], int lane) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const bool up = lane & o;
-#pragma unroll
-    for (int i = 0; i < o; ++i) {
-      const float keep = up ? v[i + o] : v[i], send = up ? v[i] : v[i + o];
-      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-    }
-  }
-  return v[0];
-}
-SSB_DEVICE void tmem_ld_x16(uint32_t taddr, float (&v)[16]) {
-  uint32_t r[16];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
-      "[%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-}
-SSB_DEVICE uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
-SSB_DEVICE bool elect_lane() {                   // true in one lane of a converged warp
-  uint32_t p;
-  asm volatile(
-      "{\n\t.reg .pred e;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "selp.u32 %0, 1, 0, e;\n\t}"
-      : "=r"(p));
-  return p != 0;
-}
-struct Bars {                                    // lat_*: 2 buffers x 4 chunks; agree: one a half of the heads
+// ---- barriers -----------------------------------------------------------------------------------------------------
+struct Bars {                                    // lat_*: 2 buffers x 4 chunks; agree: one a group of heads
   uint32_t lat_full, lat_empty, rope_full, rope_empty, q_full, s_full, s_empty, p_full, pv_done, o_full, drain, agree;
 };
-// One arrival for a warp, after all its lanes got here (512 arrivals a unit on one word kept shared memory from the MMAs).
+// mbar_wait whose second and later tries are out of line: the many waits stay short in the instruction cache.
+__device__ __noinline__ bool mbar_wait_more(uint32_t bar, uint32_t parity, volatile int32_t* abort_flag,
+                                            int32_t* status) {
+  const unsigned long long t0 = globaltimer();
+  while (true) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*abort_flag) return false;
+    if (globaltimer() - t0 > kWaitNs) {
+      *abort_flag = 1;
+      raise_status(status, kErrTimeout);
+      return false;
+    }
+  }
+}
+SSB_DEVICE bool mbar_nap(uint32_t bar, uint32_t parity, volatile int32_t* abort_flag, int32_t* status) {
+  return mbar_try_wait(bar, parity) || mbar_wait_more(bar, parity, abort_flag, status);
+}
+// One arrival for a warp, after all its lanes got here.
 SSB_DEVICE void warp_arrive(uint32_t bar, int lane) {
   __syncwarp();
   if (lane == 0) mbar_arrive(bar);
@@ -239,35 +233,15 @@ SSB_DEVICE void warp_arrive(uint32_t bar, int lane) {
 SSB_DEVICE void mbar_arrive_n(uint32_t bar, uint32_t n) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n) : "memory");
 }
-// mbar_wait with a suspended wait: up to kNapNs a try, so that a role that waits leaves the issue slots to the others
-// (the plain form polls). Bounded in the same way.
-constexpr uint32_t kNapNs = 50000;
-SSB_DEVICE bool mbar_nap(uint32_t bar, uint32_t parity, volatile int32_t* abort_flag, int32_t* status) {
-  unsigned long long t0 = 0;
-  while (true) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity), "r"(kNapNs)
-        : "memory");
-    if (ok) return true;
-    if (*abort_flag) return false;
-    const unsigned long long t = globaltimer();
-    if (t0 == 0) t0 = t;
-    if (t - t0 > kWaitNs) {
-      *abort_flag = 1;
-      raise_status(status, kErrTimeout);
-      return false;
-    }
-  }
-}
-SSB_DEVICE void tma_prefetch_2d(const CUtensorMap* m, int32_t x, int32_t y) {
-  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(m)), "r"(x),
-               "r"(y)
-               : "memory");
+
+// ---- the plan -----------------------------------------------------------------------------------------------------
+// Tokens and units of row t. How many tokens a row's list names is not known before it is read: its share is planned
+// by the list's width or, where that is smaller, the tokens it can name.
+SSB_DEVICE int row_units(const MlaDecodeArgs& a, int64_t t) {
+  int64_t n = a.indices != nullptr ? a.n_idx : (int64_t)a.width * kUnit;
+  if (a.seq_lens != nullptr) n = min(n, (int64_t)a.seq_lens[t]);
+  if (a.reqs != nullptr && (a.reqs[t] < 0 || a.reqs[t] >= a.R)) n = 0;
+  return n > 0 ? static_cast<int>((n + kUnit - 1) / kUnit) : 0;
 }
 
 // A CTA's share of one row: units [b0, b1) of the row's nb planned ones; every role walks the same segments.
@@ -276,30 +250,85 @@ struct Segment {
   int b0, b1, nb;
 };
 struct Walk {
-  int64_t t, at, hi, first;
-  SSB_DEVICE bool next(const MlaDecodeArgs& a, Segment& s) {
-    for (; t < a.T && at < hi; ++t) {
-      const int nb = row_units(a, t);
-      if (nb == 0) continue;
-      const int64_t end = min(hi, first + nb);
-      s.t = t, s.b0 = static_cast<int>(at - first), s.b1 = static_cast<int>(end - first), s.nb = nb;
-      at = end;
-      first += nb;
-      ++t;
-      return true;
-    }
-    return false;
-  }
+  int64_t t, at, hi, first;                     // next row, next unit, end of the range, units before row t
 };
+__device__ __noinline__ bool walk_next(const MlaDecodeArgs& a, Walk& w, Segment& s) {
+  for (; w.t < a.T && w.at < w.hi; ++w.t) {
+    const int nb = row_units(a, w.t);
+    if (nb == 0) continue;
+    const int64_t end = min(w.hi, w.first + nb);
+    s.t = w.t, s.b0 = static_cast<int>(w.at - w.first), s.b1 = static_cast<int>(end - w.first), s.nb = nb;
+    w.at = end;
+    w.first += nb;
+    ++w.t;
+    return true;
+  }
+  return false;
+}
 
-// The two products of a unit in buffer buf, by a whole warp of which one lane issues: the addresses are the same in every
-// lane, so they stay in uniform registers, and the loops stay small. (By one thread, with everything unrolled, the roles'
-// code together outgrew the instruction cache and every warp waited for instructions.)
+// All threads of the CTA: its range of units and the row that holds the first of them. sh: 16 int64 words for the warps'
+// sums, 2 for the row. False: more CTAs than units, nothing to do here.
+SSB_DEVICE bool find_range(const MlaDecodeArgs& a, int cta, int ctas, int64_t* sh, Walk& out) {
+  constexpr int kScan = kSoftmax;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const bool in = tid < kScan;
+  int64_t n = 0, total = 0;
+#pragma unroll 1
+  for (int64_t t = tid; in && t < a.T; t += kScan) n += row_units(a, t);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  if (in && lane == 0) sh[warp] = n;
+  if (tid == 0) sh[16] = a.T, sh[17] = 0;
+  __syncthreads();
+#pragma unroll 1
+  for (int w = 0; w < kSoftWarps; ++w) total += sh[w];
+  const int64_t used = min((int64_t)ctas, total);      // every range in use holds a unit: a row's CTAs are consecutive
+  const int64_t lo = cta < used ? total * cta / used : total;
+  out.at = lo;
+  out.hi = cta < used ? total * (cta + 1) / used : total;
+  int64_t base = 0;
+#pragma unroll 1
+  for (int64_t c = 0; c < a.T && base <= lo; c += kScan) {
+    const int64_t t = c + tid;
+    n = in && t < a.T ? row_units(a, t) : 0;
+    int64_t end = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, end, o);
+      if (lane >= o) end += v;
+    }
+    __syncthreads();
+    if (in && lane == 31) sh[warp] = end;
+    __syncthreads();
+    int64_t before = base;
+#pragma unroll 1
+    for (int w = 0; w < kSoftWarps; ++w) {
+      if (w < warp) before += sh[w];
+      base += sh[w];
+    }
+    end += before;
+    if (n > 0 && end - n <= lo && lo < end) sh[16] = t, sh[17] = end - n;
+  }
+  __syncthreads();
+  out.t = sh[16];
+  out.first = sh[17];
+  return out.at < out.hi;
+}
+
+SSB_DEVICE float* part_o(const MlaDecodeArgs& a, int tile, int slot) {
+  return a.part_o + ((int64_t)tile * 2 * kMaxCtas + slot) * kTileH * kDv;
+}
+SSB_DEVICE float2* part_ml(const MlaDecodeArgs& a, int tile, int slot) {
+  return a.part_ml + ((int64_t)tile * 2 * kMaxCtas + slot) * kTileH;
+}
+
+// ---- the two products ---------------------------------------------------------------------------------------------
+// By a whole warp of which one lane issues: the addresses are the same in every lane, so they stay in uniform registers.
 template <bool Q8>
 SSB_DEVICE bool issue_scores(const Bars& B, uint32_t sbase, int buf, uint32_t parity, bool leader,
                              volatile int32_t* abort_flag, int32_t* status) {
   constexpr uint32_t idesc = idesc_e4m3(128, Q8 ? 64 : 128);         // S^T [tokens, heads] = K Q^T
-  uint64_t ad = smem_desc(sbase + kOffRope, 0, 512, kSw64), bd = smem_desc(sbase + kOffQ + 4 * kChunk, 0, 512, kSw64);
+  uint64_t ad = smem_desc(sbase + kOffRope, 0, 512, kSw64), bd = smem_desc(sbase + kOffQ + kLat, 0, 512, kSw64);
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks)                                     // the rope keys: 64 bytes a row
     if (leader) tc_mma_f8(kColS, ad + 2 * ks, bd + 2 * ks, idesc, ks != 0 ? 1u : 0u);
@@ -323,19 +352,25 @@ SSB_DEVICE bool issue_scores(const Bars& B, uint32_t sbase, int buf, uint32_t pa
 }
 SSB_DEVICE void issue_values(const Bars& B, uint32_t sbase, int buf, bool fresh, bool leader) {
   uint64_t ad = smem_desc(sbase + kOffKv + buf * kLat, kChunk, 1024, kSw128);     // O^T [dims, heads] (+)= V^T P^T
-  const uint64_t hi = smem_desc(sbase + kOffPhi, kRope, 512, kSw64), lo = smem_desc(sbase + kOffPlo, kRope, 512, kSw64);
+  const uint64_t hi0 = smem_desc(sbase + kOffPhi, kRope, 512, kSw64), lo0 = smem_desc(sbase + kOffPlo, kRope, 512, kSw64);
   uint32_t o = kColO, empty = B.lat_empty + 32 * buf;
   const uint32_t sfp = kColP + 2 * buf;
   if (leader) tc_cp_sf(kColP, smem_desc(sbase + kOffSf, 0, 128, 0));
 #pragma unroll 1
   for (int d = 0; d < 4; ++d) {                                      // 128 dims
-#pragma unroll
+    uint64_t v = ad, hi = hi0, lo = lo0;
+    uint32_t id = idesc_mx(128, 64), acc = fresh ? 0u : 1u;
+#pragma unroll 1
     for (int ks = 0; ks < 4; ++ks) {                                 // 32 tokens a step: one block of scales
       if (leader) {
-        tc_mma_mx(o, ad + ks * (4096 >> 4), hi + ks * (2048 >> 4), idesc_mx(128, 64, ks), ks == 0 && fresh ? 0u : 1u, kColV,
-                  sfp);
-        tc_mma_mx(o, ad + ks * (4096 >> 4), lo + ks * (2048 >> 4), idesc_mx(128, 64, ks), 1u, kColLow, sfp);
+        tc_mma_mx(o, v, hi, id, acc, kColV, sfp);
+        tc_mma_mx(o, v, lo, id, 1u, kColLow, sfp);
       }
+      v += 4096 >> 4;
+      hi += 2048 >> 4;
+      lo += 2048 >> 4;
+      id += 1u << 4;
+      acc = 1;
     }
     if (leader) tc_commit(empty);                                    // the chunk is free for the unit after the next
     ad += kChunk >> 4;
@@ -348,89 +383,64 @@ SSB_DEVICE void issue_values(const Bars& B, uint32_t sbase, int buf, bool fresh,
 // One query row's heads h0 .. h0 + 63 into the query tile: rows 0-63 the high parts, 64-127 the low parts of
 // q 2^-k (k per head, its largest value in [2^7, 2^8)), zero rows past nh. bf16 has 8 significant bits, so the two e4m3
 // parts hold a value exactly unless it is below 2^-14 of the head's largest. Also each head's score scale (its reference
-// cleared). Warps 0-7, 8 heads each.
+// cleared). 8 threads a head, 9 granules each (twice: for the largest value, then from the L1 cache for the parts).
 template <bool Q8>
-SSB_DEVICE void stage_q(const MlaDecodeArgs& a, uint8_t* smem, int64_t t, int h0, int nh, int warp, int lane) {
+__device__ __noinline__ void stage_q(const MlaDecodeArgs& a, uint8_t* smem, int64_t t, int h0, int nh) {
   uint8_t* Q = smem + kOffQ;
   float* scale = reinterpret_cast<float*>(smem + kOffScale);
-  const float unit = a.bmm1 * kLog2e;
+  const int h = threadIdx.x >> 3, sub = threadIdx.x & 7;
+  const bool have = h < nh;
+  const int64_t off = t * a.ldq + (int64_t)(h0 + min(h, nh - 1)) * a.hsq;
+  int k = 0;
   if (Q8) {
-    const uint8_t* q = static_cast<const uint8_t*>(a.q) + t * a.ldq;
-    uint4 v[9];                                                       // 64 x 36 granules
+    const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.q) + off);
 #pragma unroll
-    for (int j = 0; j < 9; ++j) {
-      const int i = warp * 32 + lane + kSoftmax * j, h = i / 36, g = i - h * 36;
-      v[j] = h < nh ? *reinterpret_cast<const uint4*>(q + (h0 + h) * a.hsq + g * 16) : make_uint4(0, 0, 0, 0);
+    for (int j = 0; j < 5; ++j) {                                     // 36 granules of 16 values
+      const int g = sub + 8 * j;
+      if (g < 36) *reinterpret_cast<uint4*>(Q + row_off(h, g)) = have ? __ldg(q + g) : make_uint4(0, 0, 0, 0);
     }
+  } else {
+    const uint4* q = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + off);
+    uint4 v[9];
 #pragma unroll
-    for (int j = 0; j < 9; ++j) {
-      const int i = warp * 32 + lane + kSoftmax * j, h = i / 36, g = i - h * 36;
-      *reinterpret_cast<uint4*>(Q + row_off(h, g)) = v[j];
-    }
-    if (warp < 2) {
-      const int h = warp * 32 + lane;
-      scale[h] = h < nh ? unit : 0.0f;
-      scale[64 + h] = h < nh ? 0.0f : kNoHead;
-    }
-    return;
-  }
-  const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + t * a.ldq;
+    for (int j = 0; j < 9; ++j) v[j] = __ldg(q + sub + 8 * j);        // 72 granules of 8 values
+    uint32_t top = 0;                                                 // bf16 magnitudes, two at a time
+#pragma unroll
+    for (int j = 0; j < 9; ++j)
+      top = __vmaxu2(top, __vmaxu2(__vmaxu2(v[j].x & 0x7FFF7FFFu, v[j].y & 0x7FFF7FFFu),
+                                   __vmaxu2(v[j].z & 0x7FFF7FFFu, v[j].w & 0x7FFF7FFFu)));
+    top = max(top & 0xFFFFu, top >> 16);
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const int ex = static_cast<int>(top >> 7);                        // the largest value's biased exponent
+    if (ex != 0) k = max(min(ex - 134, 120), -120);
+    // an infinite or NaN query value leaves its head no finite score: NaN, which e4m3 can carry (it has no infinity)
+    const float down = !have ? 0.0f : ex == 255 ? NAN : __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
 #pragma unroll 1
-  for (int i0 = 0; i0 < 8; i0 += 4) {
-    uint4 v[4][3];
+    for (int j = 0; j < 9; ++j) {
+      const int g = sub + 8 * j;
+      const uint4 w4 = __ldg(q + g);
+      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+      uint32_t hi[4], lo[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int h = 8 * warp + i0 + i;
-#pragma unroll
-      for (int j = 0; j < 3; ++j) {
-        const int g = lane + 32 * j;                                  // 72 granules of 8 values
-        v[i][j] = h < nh && g < 72 ? *reinterpret_cast<const uint4*>(q + (h0 + h) * a.hsq + 8 * g)
-                                   : make_uint4(0, 0, 0, 0);
-      }
+      for (int e = 0; e < 4; ++e)
+        split2(__uint_as_float(w[e] << 16) * down, __uint_as_float(w[e] & 0xFFFF0000u) * down, hi[e], lo[e]);
+      const uint32_t at = row_off(h, g >> 1) + 8 * (g & 1);           // 8 values: half a 16-byte granule
+      const uint32_t low = g < 64 ? 64 * 128 : 64 * 64;               // 64 rows further on, where the swizzle repeats
+      *reinterpret_cast<uint2*>(Q + at) = make_uint2(hi[0] | (hi[1] << 16), hi[2] | (hi[3] << 16));
+      *reinterpret_cast<uint2*>(Q + at + low) = make_uint2(lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16));
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int h = 8 * warp + i0 + i;
-      uint32_t top = 0;
-#pragma unroll
-      for (int j = 0; j < 3; ++j) {
-        const uint32_t w[4] = {v[i][j].x, v[i][j].y, v[i][j].z, v[i][j].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) top = max(top, max(w[e] & 0x7FFFu, (w[e] >> 16) & 0x7FFFu));   // bf16 magnitudes
-      }
-      top = __reduce_max_sync(0xffffffffu, top);
-      const int ex = static_cast<int>(top >> 7);                      // the largest value's biased exponent
-      const int k = ex == 0 || ex == 255 ? 0 : max(min(ex - 134, 120), -120);
-      const float down = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
-      if (lane == 0) {
-        scale[h] = h < nh ? unit * __uint_as_float(static_cast<uint32_t>(127 + k) << 23) : 0.0f;
-        scale[64 + h] = h < nh ? 0.0f : kNoHead;
-      }
-#pragma unroll
-      for (int j = 0; j < 3; ++j) {
-        const int g = lane + 32 * j;
-        if (g >= 72) continue;
-        const uint32_t w[4] = {v[i][j].x, v[i][j].y, v[i][j].z, v[i][j].w};
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          // an infinite query value leaves no finite weight: NaN, which e4m3 can carry (it has no infinity)
-          const float x = __uint_as_float(w[e] << 16) * down, y = __uint_as_float(w[e] & 0xFFFF0000u) * down;
-          split2(isinf(x) ? NAN : x, isinf(y) ? NAN : y, hi[e], lo[e]);
-        }
-        const uint32_t sub = 8 * (g & 1);                             // 8 values: half a 16-byte granule
-        *reinterpret_cast<uint2*>(Q + row_off(h, g >> 1) + sub) = make_uint2(hi[0] | (hi[1] << 16), hi[2] | (hi[3] << 16));
-        *reinterpret_cast<uint2*>(Q + row_off(64 + h, g >> 1) + sub) =
-            make_uint2(lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16));
-      }
-    }
+  }
+  if (sub == 0) {
+    scale[h] = have ? a.bmm1 * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + k) << 23) : 0.0f;
+    scale[64 + h] = have ? 0.0f : kNoHead;
   }
 }
 
 template <bool Q8>
 __global__ void __launch_bounds__(kThreads, 1)
     mla_decode_kernel(const __grid_constant__ CUtensorMap mlat, const __grid_constant__ CUtensorMap mrope,
-                      const MlaDecodeArgs a) {
+                      const __grid_constant__ MlaDecodeArgs a) {
   extern __shared__ __align__(1024) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = blockIdx.x, tile = blockIdx.y;
@@ -442,20 +452,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int32_t* abort_flag = reinterpret_cast<volatile int32_t*>(smem + kOffMisc + 4);
   volatile int32_t* last_unit = reinterpret_cast<volatile int32_t*>(smem + kOffMisc + 8);     // [2]
   volatile uint32_t* mask = reinterpret_cast<volatile uint32_t*>(smem + kOffMask);
-  if (sbase != kBase) {                                  // no static shared memory precedes
+  if (sbase & 1023) {                                    // the swizzled tiles need it; no static shared memory precedes
     if (tid == 0) raise_status(a.status, kErrCuda);
     return;
   }
 
-  Walk walk;
-  {
-    int64_t lo, hi;
-    Plan p;
-    find_range(a, cta, gridDim.x, reinterpret_cast<int64_t*>(smem + kOffPlo), lo, hi, p);
-    if (lo >= hi) return;                                // fewer units than CTAs
-    walk = {p.row, lo, hi, p.first};
+  // rows without a token: zeros
+#pragma unroll 1
+  for (int64_t t = cta; t < a.T; t += gridDim.x) {
+    if (row_units(a, t) != 0) continue;
+    if (tid == 0 && a.reqs != nullptr && (a.reqs[t] < 0 || a.reqs[t] >= a.R)) raise_status(a.status, kErrArgs);
+    uint4* o = reinterpret_cast<uint4*>(a.out + (t * a.H + h0) * kDv);
+    for (int i = tid; i < nh * kDv / 8; i += kThreads) o[i] = make_uint4(0, 0, 0, 0);
+    if (a.lse != nullptr && tid < nh) a.lse[t * a.H + h0 + tid] = kNone;
   }
+  Walk walk;
+  const bool work = find_range(a, cta, gridDim.x, reinterpret_cast<int64_t*>(smem + kOffPlo), walk);
+  if (!work) return;
   if (tid == 0) {
+#pragma unroll 1
     for (int i = 0; i < 8; ++i) {                        // every gather lane's copies; for the last chunk also an
       mbar_init(B.lat_full + 8 * i, 128 + ((i & 3) == 3 ? kGatherWarps : 0));      // arrival a warp for its mask word
       mbar_init(B.lat_empty + 8 * i, 1);
@@ -469,8 +484,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(B.pv_done, 1);
     mbar_init(B.o_full, 1);
     mbar_init(B.drain, 2);
-    for (int i = 0; i < 2; ++i) mbar_init(B.agree + 8 * i, 4);
-    for (int i = 0; i < 4; ++i) reinterpret_cast<int32_t*>(smem + kOffRise)[i] = 0;
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) mbar_init(B.agree + 8 * i, 4);
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) reinterpret_cast<int32_t*>(smem + kOffRise)[i] = 0;
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -488,19 +505,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 
   if (warp >= kGatherWarp) {
-    // ---------------------------------------------------------------- gather: warp w brings tokens 32 w .. 32 w + 31
-    const int w = warp - kGatherWarp;
-    if (w == 0 && lane == 0) {
-      tma_prefetch_desc(&mlat);
-      tma_prefetch_desc(&mrope);
-    }
+    // ---------------------------------------------------------------- gather: warp w brings tokens 32 w .. 32 w + 31, or
+    const int w = warp - kGatherWarp;                    // of a whole page the latent chunk w (warp 0 also the rope keys)
     const int cols = a.indices != nullptr ? (a.n_idx + kUnit - 1) / kUnit : 0;
     int u = 0;
     Segment s;
     bool ok = true;
-    while (ok && walk.next(a, s)) {
-      const int64_t req = a.reqs != nullptr ? a.reqs[s.t] : s.t;
-      const int32_t* pages = a.table + req * a.width;
+    while (ok && walk_next(a, walk, s)) {
+      const int32_t* pages = a.table + (a.reqs != nullptr ? (int64_t)a.reqs[s.t] : s.t) * a.width;
       const int len = a.seq_lens != nullptr ? a.seq_lens[s.t] : 0x7fffffff;
       const int32_t* idx = a.indices != nullptr ? a.indices + s.t * a.ld_idx : nullptr;
       int c0 = s.b0, c1 = s.b1;
@@ -510,6 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         c1 = static_cast<int>((int64_t)s.b1 * cols / s.nb);
         if (c1 - c0 <= 64) {
           live = 0;
+#pragma unroll 2
           for (int c = c0; c < c1; ++c) {
             bool any = false;
 #pragma unroll
@@ -523,82 +536,77 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (live == 0) live = 1;                       // nothing selected: one empty unit gives the zeros
         }
       }
-      auto slot_at = [&](int c) -> int {                 // cache row of this lane's token of unit c (-1: none)
-        int pos = c * kUnit + 32 * w + lane;
-        if (idx != nullptr) pos = pos < a.n_idx ? idx[pos] : -1;
-        if (pos < 0 || pos >= len || pos / kUnit >= a.width) return -1;
-        const int64_t slot = (int64_t)pages[pos / kUnit] * kUnit + pos % kUnit;
-        return slot >= 0 && slot < a.cache_rows ? static_cast<int>(slot) : -1;
+      // first cache row of the page of position p (-1: none)
+      auto page_row = [&](int p) -> int64_t { return p / kUnit < a.width ? (int64_t)pages[p / kUnit] * kUnit : -1; };
+      auto token = [&](int c) {                          // position of this lane's token of unit c (-1: none)
+        int p = c * kUnit + 32 * w + lane;
+        if (idx != nullptr) p = p < a.n_idx ? idx[p] : -1;
+        return p < len ? p : -1;
       };
       auto next_live = [&](int c) {
         while (c < c1 && c - c0 < 64 && !((live >> (c - c0)) & 1)) ++c;
         return c;
       };
       int c = next_live(c0);
-      int slot = slot_at(c);
-      auto whole_page = [&](int c, int slot) {           // the same in every lane and warp
-        return idx == nullptr && (c + 1) * kUnit <= len && slot >= 0 && slot - (32 * w + lane) + kUnit <= a.cache_rows;
-      };
-      auto prefetch = [&](int c) {                       // a page some units ahead into L2
-        if (lane != 0 || idx != nullptr || c >= c1) return;
-        const int sl = slot_at(c);                       // the first token of the warp's quarter
-        if (!whole_page(c, sl)) return;
-        tma_prefetch_2d(&mlat, 128 * w, sl - 32 * w);
-        if (w == 0) tma_prefetch_2d(&mrope, kDv, sl);
-      };
-      for (int i = 0; i < kAhead; ++i) prefetch(c0 + 2 + i);
+      int p = token(c);
+      int64_t page = p >= 0 ? page_row(p) : -1;
+      int ahead = idx == nullptr ? c0 + 2 : c1;          // next page to prefetch: whole pages only
       while (c < c1) {
         const int buf = u & 1, cn = next_live(c + 1);
-        const int slot_n = cn < c1 ? slot_at(cn) : -1;
-        prefetch(c + 2 + kAhead);
+        for (; ahead < c1 && ahead <= c + 2 + kAhead; ++ahead) {
+          const int64_t y = page_row(ahead * kUnit);
+          if (lane == 0 && y >= 0 && y + kUnit <= a.cache_rows && (ahead + 1) * kUnit <= len) {
+            tma_prefetch_2d(&mlat, 128 * w, static_cast<int>(y));
+            if (w == 0) tma_prefetch_2d(&mrope, kDv, static_cast<int>(y));
+          }
+        }
+        int pn = -1;
+        int64_t page_n = -1;
+        if (cn < c1) {
+          pn = token(cn);
+          page_n = pn >= 0 ? page_row(pn) : -1;
+        }
         const uint32_t full = B.lat_full + 32 * buf, empty = B.lat_empty + 32 * buf, parity = ((u >> 1) - 1) & 1;
         const uint32_t dst = sbase + kOffKv + buf * kLat;
+        const int64_t row = page + (p & (kUnit - 1));
+        const int slot = p >= 0 && page >= 0 && row < a.cache_rows ? static_cast<int>(row) : -1;
         const uint32_t present = __ballot_sync(0xffffffffu, slot >= 0);
-        // a whole page comes as tiles, a chunk a warp; a row's last page, and selected tokens, row by row: rows that are
-        // not there have to be zeros (whatever the cache holds there, NaN too, would meet weight 0 in the value product)
-        if (whole_page(c, slot)) {
-          if (lane == 0) {
-            const int y = slot - 32 * w;
-            // (a warp arrives for a unit only after the phase before is complete: its keys have been used)
-            if (u >= 1) ok = mbar_nap(B.rope_empty, (u - 1) & 1, abort_flag, a.status);
-            if (ok && w == 0) {
+        // (a warp arrives for a unit only after the phase before is complete: its keys have been used)
+        if (u >= 1) ok = mbar_nap(B.rope_empty, (u - 1) & 1, abort_flag, a.status);
+        // a whole page (the same in every lane and warp) comes as tiles; a row's last page, and selected tokens, row by
+        // row: rows that are not there have to be zeros (whatever the cache holds there, NaN too, would meet weight 0 in
+        // the value product)
+        if (idx == nullptr && (c + 1) * kUnit <= len && page >= 0 && page + kUnit <= a.cache_rows) {
+          const int y = static_cast<int>(page);
+          if (ok && lane == 0) {
+            if (w == 0) {
               mbar_arrive_expect_tx(B.rope_full, kRope);
-              mbar_arrive_n(B.rope_full, 31);
               tma_load_2d(sbase + kOffRope, &mrope, kDv, y, B.rope_full);
-            } else if (ok) {
-              mbar_arrive_n(B.rope_full, 32);
             }
-            if (ok && u >= 2) ok = mbar_nap(empty + 8 * w, parity, abort_flag, a.status);
+            mbar_arrive_n(B.rope_full, w == 0 ? 31 : 32);
+            if (u >= 2) ok = mbar_nap(empty + 8 * w, parity, abort_flag, a.status);
             if (ok) {
               mbar_arrive_expect_tx(full + 8 * w, kChunk);
-              mbar_arrive_n(full + 8 * w, 31);
               tma_load_2d(dst + w * kChunk, &mlat, 128 * w, y, full + 8 * w);
+              // the mask words and flag of the unit two before are read by now: its last chunk's values are done
+              if (u >= 2) ok = mbar_nap(empty + 24, parity, abort_flag, a.status);
+#pragma unroll 1
+              for (int j = 0; j < 4; ++j) mbar_arrive_n(full + 8 * j, j == w ? 31 : 32);
             }
-#pragma unroll
-            for (int j = 0; j < 3; ++j)
-              if (j != w) mbar_arrive_n(full + 8 * j, 32);
-            // the mask words and flag of the unit two before are read by now: its last chunk's values are done
-            if (w != 3 && ok && u >= 2) ok = mbar_nap(empty + 24, parity, abort_flag, a.status);
-            if (w != 3) mbar_arrive_n(full + 24, 32);
           }
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-        } else {
-          if (u >= 1) ok = mbar_nap(B.rope_empty, (u - 1) & 1, abort_flag, a.status);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-#pragma unroll
-          for (int r = 0; r < 32; r += 8) {              // 8 tokens a warp instruction: their 64 rope bytes
-            const int sl = __shfl_sync(0xffffffffu, slot, r + (lane >> 2));
-            cp_async16(sbase + kOffRope + sw64(32 * w + r + (lane >> 2), lane & 3),
-                       a.kv + (int64_t)max(sl, 0) * kDq + kDv + 16 * (lane & 3), sl >= 0);
-          }
-          cp_async_arrive_noinc(B.rope_full);            // fires when this thread's copies have landed
+        } else if (ok) {
           int sl[8];
 #pragma unroll
           for (int r = 0; r < 8; ++r) sl[r] = __shfl_sync(0xffffffffu, slot, 4 * r + (lane >> 3));
+#pragma unroll
+          for (int r = 0; r < 32; r += 8) {              // 8 tokens a warp instruction: their 64 rope bytes
+            const int rs = __shfl_sync(0xffffffffu, slot, r + (lane >> 2));
+            cp_async16(sbase + kOffRope + sw64(32 * w + r + (lane >> 2), lane & 3),
+                       a.kv + (int64_t)max(rs, 0) * kDq + kDv + 16 * (lane & 3), rs >= 0);
+          }
+          cp_async_arrive_noinc(B.rope_full);            // fires when this thread's copies have landed
 #pragma unroll 1
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < 4 && ok; ++j) {
             if (u >= 2) ok = mbar_nap(empty + 8 * j, parity, abort_flag, a.status);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
@@ -609,8 +617,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                          src + (int64_t)max(sl[r], 0) * kDq, sl[r] >= 0);
             cp_async_arrive_noinc(full + 8 * j);
           }
-          if (!ok) break;
         }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
         if (lane == 0) {
           mask[4 * buf + w] = present;
           if (w == 0) last_unit[buf] = cn >= c1;
@@ -618,7 +627,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         ++u;
         c = cn;
-        slot = slot_n;
+        p = pn;
+        page = page_n;
       }
     }
     cp_async_wait_all();
@@ -628,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int u = 0;
     Segment s;
     bool ok = true;
-    while (ok && walk.next(a, s)) {
+    while (ok && walk_next(a, walk, s)) {
       bool last = false, fresh = true;
       while (!last) {
         ok = mbar_nap(B.p_full, u & 1, abort_flag, a.status);
@@ -649,7 +659,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int u = 0, seg = 0;
     Segment s;
     bool ok = true;
-    while (ok && walk.next(a, s)) {
+    while (ok && walk_next(a, walk, s)) {
       ok = mbar_nap(B.q_full, seg & 1, abort_flag, a.status);
       bool last = false;
       while (!last) {
@@ -672,30 +682,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     while (!mbar_try_wait(B.drain, 0) && globaltimer() - t0 <= 2 * kWaitNs) {}
     __syncwarp();
   } else {
-    // ---------------------------------------------------------------- softmax (warps 0-7): a token and 32 heads a thread
-    const int quarter = warp & 3, half = warp >> 2, hb = 32 * half, bid = 1 + half;
-    const int row = 32 * quarter + lane;
+    // ---------------------------------------------------------------- softmax (warps 0-15): a token and 16 heads a thread
+    const int quarter = warp & 3, group = warp >> 2, hb = 16 * group, bid = 1 + group;
+    const int row = 32 * quarter + lane, mine = hb + (lane & 15);
     const uint32_t tq = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
     float* scale = reinterpret_cast<float*>(smem + kOffScale);
     float* part = reinterpret_cast<float*>(smem + kOffExp);
     float* sums = reinterpret_cast<float*>(smem + kOffSum);
     volatile int32_t* far = reinterpret_cast<volatile int32_t*>(smem + kOffRise);
-    if (half == 0) tmem_st_x4(tq + kColV, 0x78787878u, 0x78787878u, 0x78787878u, 0x78787878u);   // 2^-7
-    else tmem_st_x4(tq + kColLow, 0x74747474u, 0x74747474u, 0x74747474u, 0x74747474u);          // 2^-11
+    if (group < 2) tmem_st_x4(tq + (group == 0 ? kColV : kColLow), group == 0 ? 0x78787878u : 0x74747474u);
     tmem_st_wait();
     int u = 0, seg = 0;
-    Segment s, s_next;
-    bool more = walk.next(a, s), ok = true;
-    stage_q<Q8>(a, smem, s.t, h0, nh, warp, lane);
+    Segment s;
+    bool more = walk_next(a, walk, s), ok = true;
+    stage_q<Q8>(a, smem, s.t, h0, nh);
     fence_proxy_async_smem();
     tc_fence_before();
     warp_arrive(B.q_full, lane);
-    named_bar(3, kSoftmax);                              // every head's scale is written
+    named_bar(5, kSoftmax);                              // every head's scale is written
     while (more) {
-      uint64_t l[16];                                    // the thread's sums of heads hb + 2 i, hb + 2 i + 1
+      uint64_t l[8];                                     // the thread's sums of heads hb + 2 i, hb + 2 i + 1
 #pragma unroll
-      for (int i = 0; i < 16; ++i) l[i] = 0;
-      float ref = hb + lane < nh ? -INFINITY : -kNoHead; // reference of head hb + lane (the same in the 4 quarters)
+      for (int i = 0; i < 8; ++i) l[i] = 0;
+      float ref = mine < nh ? kNone : -kNoHead;          // reference of head mine (the same in the 4 quarters)
       bool last = false, fresh = true, unset = true;
       while (!last) {
         const int buf = u & 1;
@@ -704,110 +713,107 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         last = last_unit[buf] != 0;
         const uint32_t present = mask[4 * buf + quarter];
-        uint64_t p[16];
-        float top[8];                                    // of 4 heads each: the warp's largest
-        auto load_scores = [&]() {                       // base-2 scores less the reference; tokens not there: -inf
-#pragma unroll
-          for (int j = 0; j < 32; j += 16) {
+        uint64_t p[8];
+        float top[4];                                    // of 4 heads each: the warp's largest
+        bool moved = false;
+#pragma unroll 1
+        while (true) {
+          // base-2 scores less the reference; tokens not there: -inf
+          {
             float x[16], y[16];
-            tmem_ld_x16(tq + kColS + hb + j, x);
-            if (!Q8) tmem_ld_x16(tq + kColS + 64 + hb + j, y);
+            tmem_ld_x16(tq + kColS + hb, x);
+            if (!Q8) tmem_ld_x16(tq + kColS + 64 + hb, y);
             tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
-              const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(scale + hb + j + i);
-              const ulonglong2 r = *reinterpret_cast<const ulonglong2*>(scale + 64 + hb + j + i);
+              const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(scale + hb + i);
+              const ulonglong2 r = *reinterpret_cast<const ulonglong2*>(scale + 64 + hb + i);
               uint64_t v = f2pack(x[i], x[i + 1]), w = f2pack(x[i + 2], x[i + 3]);
               if (!Q8) {
                 v = fma2(f2pack(y[i], y[i + 1]), f2pack(0.0625f, 0.0625f), v);
                 w = fma2(f2pack(y[i + 2], y[i + 3]), f2pack(0.0625f, 0.0625f), w);
               }
-              p[(j + i) / 2] = fma2(v, c.x, r.x);
-              p[(j + i) / 2 + 1] = fma2(w, c.y, r.y);
+              p[i / 2] = fma2(v, c.x, r.x);
+              p[i / 2 + 1] = fma2(w, c.y, r.y);
             }
           }
           if (present != 0xffffffffu && !((present >> lane) & 1)) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) p[i] = f2pack(-INFINITY, -INFINITY);
+            for (int i = 0; i < 8; ++i) p[i] = f2pack(kNone, kNone);
           }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
+          for (int i = 0; i < 4; ++i) {
             float v0, v1, v2, v3;
             f2unpack(p[2 * i], v0, v1);
             f2unpack(p[2 * i + 1], v2, v3);
             top[i] = warp_max(fmaxf(fmaxf(v0, v1), fmaxf(v2, v3)));
           }
-        };
-        load_scores();
-        float most = top[0];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) most = fmaxf(most, top[i]);
-        // the four quarters of a half agree on the rare path (a failed wait travels the same way)
-        if (lane == 0) {
-          if (unset || most > kMaxRise || !ok) far[2 * buf + half] = 1;
-          mbar_arrive(B.agree + 8 * half);
-        }
-        if (!mbar_nap(B.agree + 8 * half, u & 1, abort_flag, a.status)) ok = false;
-        // (a quarter sets the next unit's flag at the earliest after this one is agreed on, and this buffer's next flag
-        // after the next agreement: cleared here, it is not lost)
-        if (far[2 * buf + half]) {
+          if (moved) break;
+          // the four quarters of a group agree on the rare path (a failed wait travels the same way)
+          if (lane == 0) {
+            if (unset || fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > kMaxRise || !ok) far[4 * buf + group] = 1;
+            mbar_arrive(B.agree + 8 * group);
+          }
+          if (!mbar_nap(B.agree + 8 * group, u & 1, abort_flag, a.status)) ok = false;
+          // (a quarter sets the next unit's flag at the earliest after this one is agreed on, and this buffer's next flag
+          // after the next agreement: cleared below, it is not lost)
+          if (far[4 * buf + group] == 0) break;
           if (named_bar_or(bid, kGroup, !ok)) {
             ok = false;
             break;
           }
           // new references: a head without one, or with scores more than kMaxRise above it, takes the ceiling of this
           // unit's largest score; what it has accumulated is rescaled
-          const float old = ref == -INFINITY ? 0.0f : ref;
+          const float old = ref == kNone ? 0.0f : ref;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
+          for (int i = 0; i < 8; ++i) {
             float v0, v1;
             f2unpack(p[i], v0, v1);
             v0 = warp_max(v0), v1 = warp_max(v1);
             if (lane == 0) *reinterpret_cast<float2*>(part + 64 * quarter + hb + 2 * i) = make_float2(v0, v1);
           }
           named_bar(bid, kGroup);
-          float m = -INFINITY;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) m = fmaxf(m, part[64 * k + hb + lane]);
-          const bool move = m > -INFINITY && (ref == -INFINITY || m > kMaxRise);
+          const float m = fmaxf(fmaxf(part[mine], part[64 + mine]), fmaxf(part[128 + mine], part[192 + mine]));
+          const bool move = m > kNone && (ref == kNone || m > kMaxRise);
           const float now = move ? ceilf(m + old) : old;
-          const float f = move && ref != -INFINITY ? exp2f(old - now) : 1.0f;
+          const float f = move && ref != kNone ? exp2f(old - now) : 1.0f;
           if (move) ref = now;
-          unset = __any_sync(0xffffffffu, ref == -INFINITY);
+          unset = __any_sync(0xffffffffu, ref == kNone);
           if (quarter == 0) {
-            sums[hb + lane] = f;
-            scale[64 + hb + lane] = -now;
-            if (lane == 0) far[2 * buf + half] = 0;
+            sums[mine] = f;
+            scale[64 + mine] = -now;
+            if (lane == 0) far[4 * buf + group] = 0;
           }
           const bool scaled = __any_sync(0xffffffffu, f != 1.0f);
           named_bar(bid, kGroup);
           if (scaled && !fresh) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) l[i] = mul2(l[i], *reinterpret_cast<const uint64_t*>(sums + hb + 2 * i));
+            for (int i = 0; i < 8; ++i) l[i] = mul2(l[i], *reinterpret_cast<const uint64_t*>(sums + hb + 2 * i));
             if (!mbar_nap(B.pv_done, (u - 1) & 1, abort_flag, a.status)) ok = false;
             tc_fence_after();
 #pragma unroll 1
             for (int d = 0; d < 4; ++d) {
-              float o[32];
-              tmem_ld_32x32b_x32(tq + kColO + 64 * d + hb, o);
+              float o[16];
+              tmem_ld_x16(tq + kColO + 64 * d + hb, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int h = 0; h < 32; ++h) o[h] *= sums[hb + h];
-              tmem_st_32x32b_x32(tq + kColO + 64 * d + hb, o);
+              for (int h = 0; h < 16; ++h) o[h] *= sums[hb + h];
+              tmem_st_x16(tq + kColO + 64 * d + hb, o);
             }
             tmem_st_wait();
           }
-          load_scores();
+          moved = true;
         }
+        if (!moved && far[4 * buf + group] != 0) break;  // a wait gave up (in all four quarters)
         tc_fence_before();
         warp_arrive(B.s_empty, lane);
         // weights 2^(score - E + 8) with an exponent E for the warp's 32 tokens and 4 heads: the ceiling of the largest of
         // their scores above the heads' references. 2^(E - 8) is their block scale in the product and their weight in the
         // sums; the e4m3 pairs keep 8 bits down to 2^-14 of that largest.
-        uint32_t wh[8], wl[8];
-        uint8_t* sf = smem + kOffSf + 8 * buf + 4 * half + quarter;
+        uint32_t wh[4], wl[4];
+        uint8_t* sf = smem + kOffSf + 16 * (hb & 31) + 8 * buf + 4 * (group >> 1) + quarter;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4; ++i) {
           const float e = fminf(fmaxf(ceilf(top[i]), -100.0f), kMaxRise);
           const uint32_t eb = static_cast<uint32_t>(static_cast<int>(e) + 119);        // biased exponent of 2^(E - 8)
           const uint64_t off = f2pack(8.0f - e, 8.0f - e);
@@ -826,13 +832,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           wl[i] = pl[0] | (pl[1] << 16);
         }
         if (u > 0 && !mbar_nap(B.pv_done, (u - 1) & 1, abort_flag, a.status)) ok = false;   // its P has been read
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {                    // 16 heads a 16-byte granule
-          *reinterpret_cast<uint4*>(smem + kOffPhi + sw64(row, 2 * half + g)) =
-              make_uint4(wh[4 * g], wh[4 * g + 1], wh[4 * g + 2], wh[4 * g + 3]);
-          *reinterpret_cast<uint4*>(smem + kOffPlo + sw64(row, 2 * half + g)) =
-              make_uint4(wl[4 * g], wl[4 * g + 1], wl[4 * g + 2], wl[4 * g + 3]);
-        }
+        *reinterpret_cast<uint4*>(smem + kOffPhi + sw64(row, group)) = make_uint4(wh[0], wh[1], wh[2], wh[3]);
+        *reinterpret_cast<uint4*>(smem + kOffPlo + sw64(row, group)) = make_uint4(wl[0], wl[1], wl[2], wl[3]);
         fence_proxy_async_smem();
         tc_fence_before();
         warp_arrive(B.p_full, lane);
@@ -840,57 +841,62 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++u;
       }
       // ---- the row's sums, the next row's query, then the accumulators ----
-      float lf[32];
+      float lf[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) f2unpack(l[i], lf[2 * i], lf[2 * i + 1]);
+      for (int i = 0; i < 8; ++i) f2unpack(l[i], lf[2 * i], lf[2 * i + 1]);
       const float ls = warp_sum_transposed(lf, lane);
-      if (named_bar_or(3, kSoftmax, !ok)) break;
-      part[64 * quarter + hb + lane] = ls;
-      named_bar(3, kSoftmax);
-      float total = 0.0f;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) total += part[64 * k + hb + lane];
-      if (ref == -INFINITY && total == total) total = 0.0f;                          // no token
-      if (quarter == 0) sums[hb + lane] = total == 0.0f ? 0.0f : a.bmm2 / total;     // a NaN sum stays one
-      more = walk.next(a, s_next);
+      if (named_bar_or(5, kSoftmax, !ok)) break;
+      if (lane < 16) part[64 * quarter + mine] = ls;
+      named_bar(5, kSoftmax);
+      float total = part[mine] + part[64 + mine] + part[128 + mine] + part[192 + mine];
+      if (ref == kNone && total == total) total = 0.0f;                              // no token
+      if (quarter == 0) sums[mine] = total == 0.0f ? 0.0f : a.bmm2 / total;          // a NaN sum stays one
+      const Segment done = s;
+      more = walk_next(a, walk, s);
       if (more) {
-        stage_q<Q8>(a, smem, s_next.t, h0, nh, warp, lane);
+        stage_q<Q8>(a, smem, s.t, h0, nh);
         fence_proxy_async_smem();
         warp_arrive(B.q_full, lane);
       }
       ok = mbar_nap(B.o_full, seg & 1, abort_flag, a.status);
-      if (named_bar_or(3, kSoftmax, !ok)) break;
+      if (named_bar_or(5, kSoftmax, !ok)) break;
       tc_fence_after();
-      const bool whole = s.b0 == 0 && s.b1 == s.nb;
+      const bool whole = done.b0 == 0 && done.b1 == done.nb;
       const int slot = 2 * cta + (seg == 0 ? 0 : 1);
-      if (quarter == 0) {
-        const int h = hb + lane;
-        if (!whole) part_ml(a, tile, slot)[h] = make_float2(ref, total);
-        else if (a.lse != nullptr && h < nh)
-          a.lse[s.t * a.H + h0 + h] = total == 0.0f ? -INFINITY : ((ref == -INFINITY ? 0.0f : ref) + log2f(total)) / kLog2e;
-        if (half == 0 && lane == 0 && tile == 0) {
-          if (s.b0 == 0) a.rows[s.t].first = cta, a.rows[s.t].first_slot = slot;
-          if (s.b1 == s.nb) a.rows[s.t].last = cta;
+      if (quarter == 0 && lane < 16) {
+        if (!whole) part_ml(a, tile, slot)[mine] = make_float2(ref, total);
+        else if (a.lse != nullptr && mine < nh)
+          a.lse[done.t * a.H + h0 + mine] = total == 0.0f ? kNone : ((ref == kNone ? 0.0f : ref) + log2f(total)) * kLn2;
+        if (group == 0 && lane == 0 && tile == 0) {
+          if (done.b0 == 0) a.rows[done.t].first = cta, a.rows[done.t].first_slot = slot;
+          if (done.b1 == done.nb) a.rows[done.t].last = cta;
         }
       }
+      __nv_bfloat16* out = a.out + (done.t * a.H + h0 + hb) * kDv + row;
+      float* po = part_o(a, tile, slot) + hb * kDv + row;
 #pragma unroll 1
-      for (int d = 0; d < 4; ++d) {                      // 128 dims x 32 heads; a lane holds one dim
-        float o[32];
-        tmem_ld_32x32b_x32(tq + kColO + 64 * d + hb, o);
+      for (int i = 0; i < 16; i += 2) {                  // 2 heads x 4 tiles of 128 dims; a lane holds one dim of each
+        float o[8];
+        tmem_ld_2x4(tq + kColO + hb + i, o);
         tmem_ld_wait();
         if (whole) {
-          __nv_bfloat16* out = a.out + (s.t * a.H + h0 + hb) * kDv + 128 * d + row;
+          const float inv0 = sums[hb + i], inv1 = sums[hb + i + 1];
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (hb + i < nh) out[i * kDv] = __float2bfloat16(o[i] * sums[hb + i]);
+          for (int d = 0; d < 4; ++d) {
+            if (hb + i < nh) out[128 * d] = __float2bfloat16(o[2 * d] * inv0);
+            if (hb + i + 1 < nh) out[kDv + 128 * d] = __float2bfloat16(o[2 * d + 1] * inv1);
+          }
         } else {
-          float* po = part_o(a, tile, slot) + hb * kDv + 128 * d + row;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) po[i * kDv] = o[i];
+          for (int d = 0; d < 4; ++d) {
+            po[128 * d] = o[2 * d];
+            po[kDv + 128 * d] = o[2 * d + 1];
+          }
         }
+        out += 2 * kDv;
+        po += 2 * kDv;
       }
       tc_fence_before();
-      s = s_next;
       ++seg;
     }
   }
@@ -902,57 +908,54 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins a row's parts: one CTA per (row, head, 128 output values), warp w taking parts w, w + 4, ...; rows without a
-// token get zeros (lse -inf), rows that one CTA finished are left alone.
-__global__ void __launch_bounds__(128) mla_join_kernel(const MlaDecodeArgs a) {
+// Joins a row's parts. gridDim.z == 4: one CTA per (row, head, 128 output values), warp w taking parts w, w + 4, ...;
+// gridDim.z == 1: one per (row, head), a warp 128 values and all the parts (chosen by the number of CTAs, below). Rows
+// that one CTA finished, or that have no token, are left alone.
+__global__ void __launch_bounds__(128) mla_join_kernel(const __grid_constant__ MlaDecodeArgs a) {
   __shared__ float4 so[4][32];
   __shared__ float sl[4];
   const int64_t t = blockIdx.x;
   const int h = blockIdx.y, tile = h / kTileH, hh = h - tile * kTileH;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  __nv_bfloat16* out = a.out + (t * a.H + h) * kDv + blockIdx.z * 128;
-  const int nb = row_units(a, t);
-  if (nb == 0) {
-    if (a.reqs != nullptr && threadIdx.x == 0 && (a.reqs[t] < 0 || a.reqs[t] >= a.R)) raise_status(a.status, kErrArgs);
-    out[threadIdx.x] = __float2bfloat16(0.0f);
-    if (a.lse != nullptr && blockIdx.z == 0 && threadIdx.x == 0) a.lse[t * a.H + h] = -INFINITY;
-    return;
-  }
+  if (row_units(a, t) == 0) return;
   const MlaRowParts rp = a.rows[t];
   if (rp.first == rp.last) return;
-  const int parts = rp.last - rp.first + 1;
+  const bool spread = gridDim.z == 4;
+  const int parts = rp.last - rp.first + 1, step = spread ? 4 : 1, dim = 128 * (spread ? blockIdx.z : warp);
   auto slot_of = [&](int i) { return i == 0 ? rp.first_slot : 2 * (rp.first + i); };
-  float m = -INFINITY;
+  float m = kNone;
   for (int i = lane; i < parts; i += 32) m = fmaxf(m, part_ml(a, tile, slot_of(i))[hh].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float l = 0.0f;
-  const float mz = m == -INFINITY ? 0.0f : m;            // a part without a token (or all NaN) has m = -inf, f = 0
-  for (int i = warp; i < parts; i += 4) {
+  const float mz = m == kNone ? 0.0f : m;                // a part without a token (or all NaN) has m = -inf, f = 0
+#pragma unroll 4
+  for (int i = spread ? warp : 0; i < parts; i += step) {
     const float2 ml = part_ml(a, tile, slot_of(i))[hh];
     const float f = exp2f(ml.x - mz);
-    const float4 v = reinterpret_cast<const float4*>(part_o(a, tile, slot_of(i)) + hh * kDv + blockIdx.z * 128)[lane];
-    acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y);
-    acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
+    const float4 v = reinterpret_cast<const float4*>(part_o(a, tile, slot_of(i)) + hh * kDv + dim)[lane];
+    s.x = fmaf(f, v.x, s.x), s.y = fmaf(f, v.y, s.y);
+    s.z = fmaf(f, v.z, s.z), s.w = fmaf(f, v.w, s.w);
     l = fmaf(f, ml.y, l);
   }
-  so[warp][lane] = acc;
-  if (lane == 0) sl[warp] = l;
-  __syncthreads();
-  if (warp != 0) return;
-  l = sl[0] + sl[1] + sl[2] + sl[3];
-  float4 s = so[0][lane];
+  if (spread) {
+    so[warp][lane] = s;
+    if (lane == 0) sl[warp] = l;
+    __syncthreads();
+    if (warp != 0) return;
+    l = sl[0] + sl[1] + sl[2] + sl[3];
 #pragma unroll
-  for (int w = 1; w < 4; ++w) {
-    const float4 v = so[w][lane];
-    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    for (int w = 1; w < 4; ++w) {
+      const float4 v = so[w][lane];
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
   }
-  const float inv = l == 0.0f ? 0.0f : a.bmm2 / l;
-  __nv_bfloat162 lo = __floats2bfloat162_rn(s.x * inv, s.y * inv), hi = __floats2bfloat162_rn(s.z * inv, s.w * inv);
-  reinterpret_cast<uint2*>(out)[lane] = make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
-  if (a.lse != nullptr && blockIdx.z == 0 && lane == 0)
-    a.lse[t * a.H + h] = l == 0.0f ? -INFINITY : (mz + log2f(l)) / kLog2e;
+  const float inv = l == 0.0f ? 0.0f : a.bmm2 / l;       // a NaN sum stays one
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(s.x * inv, s.y * inv), hi = __floats2bfloat162_rn(s.z * inv, s.w * inv);
+  reinterpret_cast<uint2*>(a.out + (t * a.H + h) * kDv + dim)[lane] =
+      make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+  if (a.lse != nullptr && dim == 0 && lane == 0) a.lse[t * a.H + h] = l == 0.0f ? kNone : (mz + log2f(l)) * kLn2;
 }
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -969,8 +972,8 @@ int64_t mla_decode_workspace_bytes(int64_t T, int H) {
 int launch_mla_decode(const MlaDecodeArgs& a_in, void* ws, int64_t ws_bytes, cudaStream_t stream) {
   MlaDecodeArgs a = a_in;
   const int eb = a.q_e4m3 ? 1 : 2;
-  if (a.T < 0 || a.T > 0x7fffffff || a.H <= 0 || a.H > 128 || a.R <= 0 || a.width <= 0 || a.cache_rows <= 0 || a.cache_rows > 0x7fffffff ||
-      (a.indices == nullptr && a.seq_lens == nullptr) ||
+  if (a.T < 0 || a.T > 0x7fffffff || a.H <= 0 || a.H > 128 || a.R <= 0 || a.width <= 0 || a.cache_rows <= 0 ||
+      a.cache_rows > 0x7fffffff || (a.indices == nullptr && a.seq_lens == nullptr) ||
       (a.indices != nullptr && (a.n_idx < 0 || a.ld_idx < a.n_idx)) || (a.reqs == nullptr && a.T > a.R))
     return kErrArgs;
   if (a.T == 0) return kOk;
@@ -989,12 +992,7 @@ int launch_mla_decode(const MlaDecodeArgs& a_in, void* ws, int64_t ws_bytes, cud
   auto* kernel = a.q_e4m3 ? mla_decode_kernel<true> : mla_decode_kernel<false>;
   static bool attr[2] = {false, false};
   if (!attr[a.q_e4m3]) {
-    int dev = 0, reserved = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&reserved, cudaDevAttrReservedSharedMemoryPerBlock, dev) != cudaSuccess ||
-        reserved != (int)kBase ||
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
-      return kErrCuda;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return kErrCuda;
     attr[a.q_e4m3] = true;
   }
   CUtensorMap mlat, mrope;
@@ -1004,7 +1002,9 @@ int launch_mla_decode(const MlaDecodeArgs& a_in, void* ws, int64_t ws_bytes, cud
   if (rc != kOk) return rc;
   kernel<<<dim3((unsigned)(kMaxCtas / tiles), (unsigned)tiles), kThreads, kSmem, stream>>>(mlat, mrope, a);
   if (cudaGetLastError() != cudaSuccess) return kErrCuda;
-  mla_join_kernel<<<dim3((unsigned)a.T, (unsigned)a.H, 4), 128, 0, stream>>>(a);
+  // few rows are cut into many parts each: their CTAs are spread over the parts and the output values
+  const unsigned z = a.T * a.H <= 8 * kMaxCtas ? 4 : 1;
+  mla_join_kernel<<<dim3((unsigned)a.T, (unsigned)a.H, z), 128, 0, stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
 }
 
