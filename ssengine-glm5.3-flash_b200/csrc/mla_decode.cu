@@ -21,8 +21,8 @@
 //       against a reference per head that moves only when scores rise 2^4 above it;
 //   values (1 warp issues): O^T [512 dims x 64 heads] += V^T P^T, kind::mxf8f6f4, 4 tiles of M = 128, N = 64, from the same
 //       rows read the other way round.
-// TMEM: O^T 256 columns, S^T 128, block scales. Shared memory: query parts 72 KB, latent rows 2 x 64 KB, rope keys 8 KB
-// (needed for the scores only), P 16 KB.
+// TMEM: O^T 256 columns, S^T 128, block scales. Shared memory: query parts 72 KB, two units' rows 2 x 72 KB (the high parts
+// of P take the place of the rope keys, which only the scores need), the low parts of P 8 KB.
 // Bounds: 576 bytes a token from HBM against 64 x 2,176 products of 8 bits: 2,700 cycles a unit at the measured copy
 // rate, and as many for the two products, which read shared memory at its full rate (18 instructions of 64 cycles, 32 of
 // 48). One thread's instruction stream matters as much: the roles' loops are kept small because they share 28 KB of
@@ -55,9 +55,8 @@ constexpr int kRope = 8192;                     // [128 rows x 64 B], 64-byte sw
 constexpr int kLat = 4 * kChunk;                // a unit's latent rows
 constexpr int kOffQ = 0;                        // the query tile's parts: 4 chunks and the rope
 constexpr int kOffKv = kLat + kRope;            // the latent rows of two units
-constexpr int kOffRope = kOffKv + 2 * kLat;     // the rope keys of one: free again once its scores are done
-constexpr int kOffPhi = kOffRope + kRope;       // the parts of P
-constexpr int kOffPlo = kOffPhi + kRope;
+constexpr int kOffRope = kOffKv + 2 * kLat;     // their rope keys; once its scores are done, a unit's high parts of P
+constexpr int kOffPlo = kOffRope + 2 * kRope;   // the low parts of P
 constexpr int kOffSf = kOffPlo + kRope;         // block scales of P, two units: byte (h % 32) 16 + unit 8 + (h / 32) 4 + quarter
 constexpr int kOffBar = kOffSf + 512;           // mbarriers
 constexpr int kOffMisc = kOffBar + 256;         // tmem address, abort flag, last-unit flags, plan
@@ -71,7 +70,7 @@ static_assert(kOffScale % 16 == 0 && kOffExp % 16 == 0 && kOffSf % 128 == 0 && k
 // TMEM columns: O^T as 4 tiles of 128 dims x 64 heads, S^T 128 tokens x (64 high | 64 low), block scales of V (2^-7 against
 // the high parts of P, 2^-11 against the low ones) and of P (2 columns a unit)
 constexpr uint32_t kColO = 0, kColS = 256, kColV = 384, kColLow = 388, kColP = 392;
-constexpr int kAhead = 4;                       // pages prefetched into L2 beyond the two in shared memory
+constexpr int kAhead = 1;                       // pages prefetched into L2 beyond the two in shared memory
 constexpr float kMaxRise = 4.0f;                // base-2 scores above a head's reference before it moves and O is rescaled
 constexpr float kNoHead = -1000.0f;             // base-2 score of the heads that the tile does not have: weight 0
 constexpr uint32_t kSw128 = 2, kSw64 = 4;       // descriptor layout types
@@ -205,8 +204,9 @@ SSB_DEVICE uint32_t sw64(int r, int g) { return r * 64 + ((g ^ ((r >> 1) & 3)) <
 SSB_DEVICE uint32_t row_off(int r, int g) { return g < 32 ? (g >> 3) * kChunk + sw128(r, g & 7) : kLat + sw64(r, g - 32); }
 
 // ---- barriers -----------------------------------------------------------------------------------------------------
-struct Bars {                                    // lat_*: 2 buffers x 4 chunks; agree: one a group of heads
-  uint32_t lat_full, lat_empty, rope_full, rope_empty, q_full, s_full, s_empty, p_full, pv_done, o_full, drain, agree;
+struct Bars {                                    // lat_*: 2 buffers x 4 chunks (the rope keys with the last); agree: one a
+                                                 // group of heads
+  uint32_t lat_full, lat_empty, q_full, s_full, s_empty, p_full, pv_done, o_full, drain, agree;
 };
 // mbar_wait whose second and later tries are out of line: the many waits stay short in the instruction cache.
 __device__ __noinline__ bool mbar_wait_more(uint32_t bar, uint32_t parity, volatile int32_t* abort_flag,
@@ -328,31 +328,31 @@ template <bool Q8>
 SSB_DEVICE bool issue_scores(const Bars& B, uint32_t sbase, int buf, uint32_t parity, bool leader,
                              volatile int32_t* abort_flag, int32_t* status) {
   constexpr uint32_t idesc = idesc_e4m3(128, Q8 ? 64 : 128);         // S^T [tokens, heads] = K Q^T
-  uint64_t ad = smem_desc(sbase + kOffRope, 0, 512, kSw64), bd = smem_desc(sbase + kOffQ + kLat, 0, 512, kSw64);
-#pragma unroll
-  for (int ks = 0; ks < 2; ++ks)                                     // the rope keys: 64 bytes a row
-    if (leader) tc_mma_f8(kColS, ad + 2 * ks, bd + 2 * ks, idesc, ks != 0 ? 1u : 0u);
-  ad = smem_desc(sbase + kOffKv + buf * kLat, 0, 1024, kSw128);
-  bd = smem_desc(sbase + kOffQ, 0, 1024, kSw128);
+  uint64_t ad = smem_desc(sbase + kOffKv + buf * kLat, 0, 1024, kSw128), bd = smem_desc(sbase + kOffQ, 0, 1024, kSw128);
+  uint32_t acc = 0;
 #pragma unroll 1
   for (int c = 0; c < 4; ++c) {
     if (!mbar_nap(B.lat_full + 32 * buf + 8 * c, parity, abort_flag, status)) return false;
     fence_proxy_async_smem();                                        // rows that threads copied -> the tensor core
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks)
-      if (leader) tc_mma_f8(kColS, ad + 2 * ks, bd + 2 * ks, idesc, 1u);
+    for (int ks = 0; ks < 4; ++ks) {
+      if (leader) tc_mma_f8(kColS, ad + 2 * ks, bd + 2 * ks, idesc, acc);
+      acc = 1;
+    }
     ad += kChunk >> 4;
     bd += kChunk >> 4;
   }
-  if (leader) {
-    tc_commit(B.rope_empty);
-    tc_commit(B.s_full);
-  }
+  ad = smem_desc(sbase + kOffRope + buf * kRope, 0, 512, kSw64);
+  bd = smem_desc(sbase + kOffQ + kLat, 0, 512, kSw64);
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks)                                     // the rope keys: 64 bytes a row
+    if (leader) tc_mma_f8(kColS, ad + 2 * ks, bd + 2 * ks, idesc, 1u);
+  if (leader) tc_commit(B.s_full);
   return true;
 }
 SSB_DEVICE void issue_values(const Bars& B, uint32_t sbase, int buf, bool fresh, bool leader) {
   uint64_t ad = smem_desc(sbase + kOffKv + buf * kLat, kChunk, 1024, kSw128);     // O^T [dims, heads] (+)= V^T P^T
-  const uint64_t hi0 = smem_desc(sbase + kOffPhi, kRope, 512, kSw64), lo0 = smem_desc(sbase + kOffPlo, kRope, 512, kSw64);
+  const uint64_t hi0 = smem_desc(sbase + kOffRope + buf * kRope, kRope, 512, kSw64), lo0 = smem_desc(sbase + kOffPlo, kRope, 512, kSw64);
   uint32_t o = kColO, empty = B.lat_empty + 32 * buf;
   const uint32_t sfp = kColP + 2 * buf;
   if (leader) tc_cp_sf(kColP, smem_desc(sbase + kOffSf, 0, 128, 0));
@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int h0 = tile * kTileH, nh = min(kTileH, a.H - h0);
   const uint32_t sbase = smem_u32(smem), bar = sbase + kOffBar;
   const Bars B = {bar,       bar + 64,  bar + 128, bar + 136, bar + 144, bar + 152,
-                  bar + 160, bar + 168, bar + 176, bar + 184, bar + 192, bar + 200};
+                  bar + 160, bar + 168, bar + 176, bar + 184};
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kOffMisc);
   volatile int32_t* abort_flag = reinterpret_cast<volatile int32_t*>(smem + kOffMisc + 4);
   volatile int32_t* last_unit = reinterpret_cast<volatile int32_t*>(smem + kOffMisc + 8);     // [2]
@@ -475,8 +475,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(B.lat_full + 8 * i, 128 + ((i & 3) == 3 ? kGatherWarps : 0));      // arrival a warp for its mask word
       mbar_init(B.lat_empty + 8 * i, 1);
     }
-    mbar_init(B.rope_full, 128);
-    mbar_init(B.rope_empty, 1);
     mbar_init(B.q_full, kSoftWarps);
     mbar_init(B.s_full, 1);
     mbar_init(B.s_empty, kSoftWarps);
@@ -506,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp >= kGatherWarp) {
     // ---------------------------------------------------------------- gather: warp w brings tokens 32 w .. 32 w + 31, or
-    const int w = warp - kGatherWarp;                    // of a whole page the latent chunk w (warp 0 also the rope keys)
+    const int w = warp - kGatherWarp;                    // of a whole page the latent chunk w (warp 3 also the rope keys)
     const int cols = a.indices != nullptr ? (a.n_idx + kUnit - 1) / kUnit : 0;
     int u = 0;
     Segment s;
@@ -557,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int64_t y = page_row(ahead * kUnit);
           if (lane == 0 && y >= 0 && y + kUnit <= a.cache_rows && (ahead + 1) * kUnit <= len) {
             tma_prefetch_2d(&mlat, 128 * w, static_cast<int>(y));
-            if (w == 0) tma_prefetch_2d(&mrope, kDv, static_cast<int>(y));
+            if (w == 3) tma_prefetch_2d(&mrope, kDv, static_cast<int>(y));
           }
         }
         int pn = -1;
@@ -571,40 +569,27 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int64_t row = page + (p & (kUnit - 1));
         const int slot = p >= 0 && page >= 0 && row < a.cache_rows ? static_cast<int>(row) : -1;
         const uint32_t present = __ballot_sync(0xffffffffu, slot >= 0);
-        // (a warp arrives for a unit only after the phase before is complete: its keys have been used)
-        if (u >= 1) ok = mbar_nap(B.rope_empty, (u - 1) & 1, abort_flag, a.status);
-        // a whole page (the same in every lane and warp) comes as tiles; a row's last page, and selected tokens, row by
+        // A chunk is free when the values of the unit two before have used it; by then that unit's scores are done and its
+        // mask word and flag are read, so a warp may also arrive on the other chunks' barriers for this unit.
+        // A whole page (the same in every lane and warp) comes as tiles; a row's last page, and selected tokens, row by
         // row: rows that are not there have to be zeros (whatever the cache holds there, NaN too, would meet weight 0 in
-        // the value product)
+        // the value product).
         if (idx == nullptr && (c + 1) * kUnit <= len && page >= 0 && page + kUnit <= a.cache_rows) {
           const int y = static_cast<int>(page);
-          if (ok && lane == 0) {
-            if (w == 0) {
-              mbar_arrive_expect_tx(B.rope_full, kRope);
-              tma_load_2d(sbase + kOffRope, &mrope, kDv, y, B.rope_full);
-            }
-            mbar_arrive_n(B.rope_full, w == 0 ? 31 : 32);
+          if (lane == 0) {
             if (u >= 2) ok = mbar_nap(empty + 8 * w, parity, abort_flag, a.status);
             if (ok) {
-              mbar_arrive_expect_tx(full + 8 * w, kChunk);
+              mbar_arrive_expect_tx(full + 8 * w, w == 3 ? kChunk + kRope : kChunk);
               tma_load_2d(dst + w * kChunk, &mlat, 128 * w, y, full + 8 * w);
-              // the mask words and flag of the unit two before are read by now: its last chunk's values are done
-              if (u >= 2) ok = mbar_nap(empty + 24, parity, abort_flag, a.status);
+              if (w == 3) tma_load_2d(sbase + kOffRope + buf * kRope, &mrope, kDv, y, full + 24);
 #pragma unroll 1
               for (int j = 0; j < 4; ++j) mbar_arrive_n(full + 8 * j, j == w ? 31 : 32);
             }
           }
-        } else if (ok) {
+        } else {
           int sl[8];
 #pragma unroll
           for (int r = 0; r < 8; ++r) sl[r] = __shfl_sync(0xffffffffu, slot, 4 * r + (lane >> 3));
-#pragma unroll
-          for (int r = 0; r < 32; r += 8) {              // 8 tokens a warp instruction: their 64 rope bytes
-            const int rs = __shfl_sync(0xffffffffu, slot, r + (lane >> 2));
-            cp_async16(sbase + kOffRope + sw64(32 * w + r + (lane >> 2), lane & 3),
-                       a.kv + (int64_t)max(rs, 0) * kDq + kDv + 16 * (lane & 3), rs >= 0);
-          }
-          cp_async_arrive_noinc(B.rope_full);            // fires when this thread's copies have landed
 #pragma unroll 1
           for (int j = 0; j < 4 && ok; ++j) {
             if (u >= 2) ok = mbar_nap(empty + 8 * j, parity, abort_flag, a.status);
@@ -615,7 +600,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int r = 0; r < 8; ++r)                  // 4 tokens a warp instruction: 128 of their latent bytes
               cp_async16(dst + j * kChunk + sw128(32 * w + 4 * r + (lane >> 3), lane & 7),
                          src + (int64_t)max(sl[r], 0) * kDq, sl[r] >= 0);
-            cp_async_arrive_noinc(full + 8 * j);
+            if (j == 3) {
+#pragma unroll
+              for (int r = 0; r < 32; r += 8) {          // 8 tokens a warp instruction: their 64 rope bytes
+                const int rs = __shfl_sync(0xffffffffu, slot, r + (lane >> 2));
+                cp_async16(sbase + kOffRope + buf * kRope + sw64(32 * w + r + (lane >> 2), lane & 3),
+                           a.kv + (int64_t)max(rs, 0) * kDq + kDv + 16 * (lane & 3), rs >= 0);
+              }
+            }
+            cp_async_arrive_noinc(full + 8 * j);         // fires when this thread's copies have landed
           }
         }
         ok = __all_sync(0xffffffffu, ok);
@@ -663,11 +656,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = mbar_nap(B.q_full, seg & 1, abort_flag, a.status);
       bool last = false;
       while (!last) {
-        if (ok) ok = mbar_nap(B.rope_full, u & 1, abort_flag, a.status);
         if (ok && u > 0) ok = mbar_nap(B.s_empty, (u - 1) & 1, abort_flag, a.status);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        fence_proxy_async_smem();                        // rows that threads copied -> the tensor core
         tc_fence_after();
         ok = issue_scores<Q8>(B, sbase, u & 1, (u >> 1) & 1, leader, abort_flag, a.status);
         ok = __all_sync(0xffffffffu, ok);
@@ -715,32 +706,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t present = mask[4 * buf + quarter];
         uint64_t p[8];
         float top[4];                                    // of 4 heads each: the warp's largest
-        bool moved = false;
-#pragma unroll 1
-        while (true) {
-          // base-2 scores less the reference; tokens not there: -inf
-          {
-            float x[16], y[16];
-            tmem_ld_x16(tq + kColS + hb, x);
-            if (!Q8) tmem_ld_x16(tq + kColS + 64 + hb, y);
-            tmem_ld_wait();
+        {                                                // base-2 scores less the reference; tokens not there: -inf
+          float x[16], y[16];
+          tmem_ld_x16(tq + kColS + hb, x);
+          if (!Q8) tmem_ld_x16(tq + kColS + 64 + hb, y);
+          tmem_ld_wait();
+          tc_fence_before();
+          warp_arrive(B.s_empty, lane);
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-              const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(scale + hb + i);
-              const ulonglong2 r = *reinterpret_cast<const ulonglong2*>(scale + 64 + hb + i);
-              uint64_t v = f2pack(x[i], x[i + 1]), w = f2pack(x[i + 2], x[i + 3]);
-              if (!Q8) {
-                v = fma2(f2pack(y[i], y[i + 1]), f2pack(0.0625f, 0.0625f), v);
-                w = fma2(f2pack(y[i + 2], y[i + 3]), f2pack(0.0625f, 0.0625f), w);
-              }
-              p[i / 2] = fma2(v, c.x, r.x);
-              p[i / 2 + 1] = fma2(w, c.y, r.y);
+          for (int i = 0; i < 16; i += 4) {
+            const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(scale + hb + i);
+            const ulonglong2 r = *reinterpret_cast<const ulonglong2*>(scale + 64 + hb + i);
+            uint64_t v = f2pack(x[i], x[i + 1]), w = f2pack(x[i + 2], x[i + 3]);
+            if (!Q8) {
+              v = fma2(f2pack(y[i], y[i + 1]), f2pack(0.0625f, 0.0625f), v);
+              w = fma2(f2pack(y[i + 2], y[i + 3]), f2pack(0.0625f, 0.0625f), w);
             }
+            p[i / 2] = fma2(v, c.x, r.x);
+            p[i / 2 + 1] = fma2(w, c.y, r.y);
           }
-          if (present != 0xffffffffu && !((present >> lane) & 1)) {
+        }
+        if (present != 0xffffffffu && !((present >> lane) & 1)) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) p[i] = f2pack(kNone, kNone);
-          }
+          for (int i = 0; i < 8; ++i) p[i] = f2pack(kNone, kNone);
+        }
+        auto tops = [&]() {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             float v0, v1, v2, v3;
@@ -748,16 +738,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             f2unpack(p[2 * i + 1], v2, v3);
             top[i] = warp_max(fmaxf(fmaxf(v0, v1), fmaxf(v2, v3)));
           }
-          if (moved) break;
-          // the four quarters of a group agree on the rare path (a failed wait travels the same way)
-          if (lane == 0) {
-            if (unset || fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > kMaxRise || !ok) far[4 * buf + group] = 1;
-            mbar_arrive(B.agree + 8 * group);
-          }
-          if (!mbar_nap(B.agree + 8 * group, u & 1, abort_flag, a.status)) ok = false;
-          // (a quarter sets the next unit's flag at the earliest after this one is agreed on, and this buffer's next flag
-          // after the next agreement: cleared below, it is not lost)
-          if (far[4 * buf + group] == 0) break;
+        };
+        tops();
+        // the four quarters of a group agree on the rare path (a failed wait travels the same way)
+        if (lane == 0) {
+          if (unset || fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > kMaxRise || !ok) far[4 * buf + group] = 1;
+          mbar_arrive(B.agree + 8 * group);
+        }
+        if (!mbar_nap(B.agree + 8 * group, u & 1, abort_flag, a.status)) ok = false;
+        // (a quarter sets the next unit's flag at the earliest after this one is agreed on, and this buffer's next flag
+        // after the next agreement: cleared below, it is not lost)
+        if (far[4 * buf + group] != 0) {
           if (named_bar_or(bid, kGroup, !ok)) {
             ok = false;
             break;
@@ -779,13 +770,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float f = move && ref != kNone ? exp2f(old - now) : 1.0f;
           if (move) ref = now;
           unset = __any_sync(0xffffffffu, ref == kNone);
+          named_bar(bid, kGroup);                        // the maxima are read: their place takes the moves
           if (quarter == 0) {
             sums[mine] = f;
+            part[mine] = old - now;
             scale[64 + mine] = -now;
             if (lane == 0) far[4 * buf + group] = 0;
           }
           const bool scaled = __any_sync(0xffffffffu, f != 1.0f);
           named_bar(bid, kGroup);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) p[i] = add2(p[i], *reinterpret_cast<const uint64_t*>(part + hb + 2 * i));
+          tops();
           if (scaled && !fresh) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) l[i] = mul2(l[i], *reinterpret_cast<const uint64_t*>(sums + hb + 2 * i));
@@ -802,11 +798,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tmem_st_wait();
           }
-          moved = true;
         }
-        if (!moved && far[4 * buf + group] != 0) break;  // a wait gave up (in all four quarters)
-        tc_fence_before();
-        warp_arrive(B.s_empty, lane);
         // weights 2^(score - E + 8) with an exponent E for the warp's 32 tokens and 4 heads: the ceiling of the largest of
         // their scores above the heads' references. 2^(E - 8) is their block scale in the product and their weight in the
         // sums; the e4m3 pairs keep 8 bits down to 2^-14 of that largest.
@@ -832,7 +824,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           wl[i] = pl[0] | (pl[1] << 16);
         }
         if (u > 0 && !mbar_nap(B.pv_done, (u - 1) & 1, abort_flag, a.status)) ok = false;   // its P has been read
-        *reinterpret_cast<uint4*>(smem + kOffPhi + sw64(row, group)) = make_uint4(wh[0], wh[1], wh[2], wh[3]);
+        *reinterpret_cast<uint4*>(smem + kOffRope + buf * kRope + sw64(row, group)) = make_uint4(wh[0], wh[1], wh[2], wh[3]);
         *reinterpret_cast<uint4*>(smem + kOffPlo + sw64(row, group)) = make_uint4(wl[0], wl[1], wl[2], wl[3]);
         fence_proxy_async_smem();
         tc_fence_before();
