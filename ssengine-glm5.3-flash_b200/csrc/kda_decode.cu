@@ -11,9 +11,12 @@
 // fp32 (the chunked prefill rounds the conv outputs to bf16 for its tensor-core operands; nothing here needs that).
 //
 // Bound: HBM. A head's 64 KB of state are read and written once a call, 7 D^2 FLOP a token over them; a call moves
-// 128 KB a head and request whatever the run's length. One CTA per (request, head), 8 warps; warp w keeps value rows
-// 16 w .. 16 w + 15 in registers, a lane 4 key columns of each (one 512-byte row a warp load, 16 loads in flight a lane
-// before the conv and the gates are computed, so these hide behind the reads).
+// 128 KB a head and request whatever the run's length. One CTA per (request, head), 8 warps, two CTAs an SM; warp w keeps
+// value rows 16 w .. 16 w + 15 in registers, a lane 4 key columns of each (one 512-byte row a warp load, 16 loads in
+// flight a lane while the conv and the gates are computed). Products and updates as packed fp32 pairs, short
+// exponentials and quotients: with the library forms the code outgrew the instruction cache (406 us at 256 requests x 64
+// heads, now 347: the copy rate). Measured against that: 8 lanes a row, which saves 24 of the 31 shuffles of the row sums
+// (357 us); the states through three 64 KB buffers by bulk copies with two groups of warps on every other one (614 us).
 #include "common.cuh"
 #include "ops.h"
 
@@ -24,9 +27,30 @@ constexpr int kDim = 128;
 constexpr int kDecThreads = 256;
 constexpr int kRowsW = 16;             // value rows a warp
 
-SSB_DEVICE float sigmoid_exact(float z) { return 1.0f / (1.0f + expf(-z)); }
-SSB_DEVICE float silu_exact(float y) { return y / (1.0f + expf(-y)); }
+// e^x as 2^(x log2 e) with the product's rounding error carried to first order: ex2.approx's own error (2^-22) remains.
+SSB_DEVICE float exp_fast(float x) {
+  constexpr float kHi = 1.44269502162933349609375f, kLo = 1.925963033500928e-8f;        // log2 e in two parts
+  const float t = x * kHi;
+  const float r = fmaf(x, kLo, fmaf(x, kHi, -t));
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t));
+  return fmaf(y, fminf(fmaxf(r, -1.0f), 1.0f) * 0.6931471805599453f, y);
+}
+SSB_DEVICE float sigmoid_fast(float z) { return __fdividef(1.0f, 1.0f + exp_fast(-z)); }
+SSB_DEVICE float silu_fast(float y) { return __fdividef(y, 1.0f + exp_fast(-y)); }
 SSB_DEVICE float2 bf2(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
+// The state is not read again by this call: its stores leave the caches first.
+SSB_DEVICE void store_stream(float* p, ulonglong2 v) {
+  float4 f;
+  f2unpack(v.x, f.x, f.y);
+  f2unpack(v.y, f.z, f.w);
+  __stcs(reinterpret_cast<float4*>(p), f);
+}
+SSB_DEVICE float sum2(uint64_t v) {
+  float a, b;
+  f2unpack(v, a, b);
+  return a + b;
+}
 
 // Sums over the 32 lanes of 32 values a lane, transposed: lane l receives the total of value l (31 shuffles).
 SSB_DEVICE float warp_sum_transposed(float (&v)[32], int lane) {
@@ -42,9 +66,8 @@ SSB_DEVICE float warp_sum_transposed(float (&v)[32], int lane) {
   return v[0];
 }
 
-__global__ void __launch_bounds__(kDecThreads, 2) kda_decode_kernel(const KdaArgs a) {
-  __shared__ __align__(16) float sy[2][3][kDim];       // conv outputs q | k | v, double-buffered over tokens
-  __shared__ __align__(16) float sa[2][kDim];          // the key channels' decays
+__global__ void __launch_bounds__(kDecThreads, 2) kda_decode_kernel(const __grid_constant__ KdaArgs a) {
+  __shared__ __align__(16) float sy[2][4][kDim];       // q | k | v | decay of a token, double-buffered
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int r = blockIdx.x / a.H, h = blockIdx.x - r * a.H;
   const int4 sq = __ldg(reinterpret_cast<const int4*>(a.seqs) + r);   // {first row, end row, state block, has state}
@@ -56,94 +79,87 @@ __global__ void __launch_bounds__(kDecThreads, 2) kda_decode_kernel(const KdaArg
   if (e == s) return;
   const bool init = sq.w != 0;
   float* S = a.rec_state + (int64_t)sq.z * a.rs_stride + ((int64_t)h * kDim + kRowsW * warp) * kDim + 4 * lane;
-  float4 st[kRowsW];
+  ulonglong2 st[kRowsW];                               // row i of the warp: columns 4 lane .. 4 lane + 3
 #pragma unroll
   for (int i = 0; i < kRowsW; ++i)
-    st[i] = init ? *reinterpret_cast<const float4*>(S + i * kDim) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    st[i] = init ? *reinterpret_cast<const ulonglong2*>(S + i * kDim) : make_ulonglong2(0, 0);
 
   // threads 0-191: a pair of conv channels each (q 0-63, k 64-127, v 128-191); threads 192-255: a pair of gates
   const bool conv = tid < 192;
-  const int pair = tid & 63;
-  const int64_t col = (int64_t)(tid >> 6) * a.P + h * kDim + 2 * pair;
-  float2 w0 = {}, w1 = {}, w2 = {}, w3 = {}, x0 = {}, x1 = {}, x2 = {};
-  uint32_t raw0 = 0, raw1 = 0, raw2 = 0;
+  const int pair = tid & 63, part = tid >> 6;
+  const int64_t col = (int64_t)part * a.P + h * kDim + 2 * pair;
   __nv_bfloat16* cs = a.conv_state + (int64_t)sq.z * a.cs_stride + col;
-  float rate = 0.0f;
-  float2 dt = {};
-  if (conv) {
-    const uint4 wv = __ldg(reinterpret_cast<const uint4*>(a.conv_w + col * 4));   // 2 channels x 4 taps
-    const float2 p0 = bf2(wv.x), p1 = bf2(wv.y), p2 = bf2(wv.z), p3 = bf2(wv.w);
-    w0 = make_float2(p0.x, p2.x);
-    w1 = make_float2(p0.y, p2.y);
-    w2 = make_float2(p1.x, p3.x);
-    w3 = make_float2(p1.y, p3.y);
-    if (init) {
-      raw0 = *reinterpret_cast<const uint32_t*>(cs);
-      raw1 = *reinterpret_cast<const uint32_t*>(cs + 3 * a.P);
-      raw2 = *reinterpret_cast<const uint32_t*>(cs + 6 * a.P);
-    }
-  } else {
-    rate = expf(__ldg(a.a_log + h));
-    dt = __ldg(reinterpret_cast<const float2*>(a.dt_bias + h * kDim) + pair);
+  const uint32_t* in = reinterpret_cast<const uint32_t*>(conv ? a.x + col : a.g + h * kDim + 2 * pair);
+  const int64_t pitch = (conv ? a.ldx : a.ldg) / 2;
+  uint32_t raw0 = 0, raw1 = 0, raw2 = 0;
+  if (conv && init) {
+    raw0 = *reinterpret_cast<const uint32_t*>(cs);
+    raw1 = *reinterpret_cast<const uint32_t*>(cs + 3 * a.P);
+    raw2 = *reinterpret_cast<const uint32_t*>(cs + 6 * a.P);
   }
-
+  uint32_t raw = __ldg(in + s * pitch);
+  float beta = __bfloat162float(a.beta[(int64_t)s * a.ldb + h]);
+#pragma unroll 1
   for (int t = s; t < e; ++t) {
-    const int buf = (t - s) & 1;
+    float* y = &sy[(t - s) & 1][0][0];
+    float2 o;
     if (conv) {
-      const uint32_t raw = __ldg(reinterpret_cast<const uint32_t*>(a.x + (int64_t)t * a.ldx + col));
-      x0 = bf2(raw0), x1 = bf2(raw1), x2 = bf2(raw2);
-      const float2 x3 = bf2(raw);
-      float2 y;
-      y.x = fmaf(w3.x, x3.x, fmaf(w2.x, x2.x, fmaf(w1.x, x1.x, w0.x * x0.x)));
-      y.y = fmaf(w3.y, x3.y, fmaf(w2.y, x2.y, fmaf(w1.y, x1.y, w0.y * x0.y)));
-      *reinterpret_cast<float2*>(&sy[buf][tid >> 6][2 * pair]) = make_float2(silu_exact(y.x), silu_exact(y.y));
+      const uint4 wv = __ldg(reinterpret_cast<const uint4*>(a.conv_w + col * 4));   // 2 channels x 4 taps
+      const float2 x0 = bf2(raw0), x1 = bf2(raw1), x2 = bf2(raw2), x3 = bf2(raw);
+      const float2 p0 = bf2(wv.x), p1 = bf2(wv.y), p2 = bf2(wv.z), p3 = bf2(wv.w);
+      o.x = silu_fast(fmaf(p1.y, x3.x, fmaf(p1.x, x2.x, fmaf(p0.y, x1.x, p0.x * x0.x))));
+      o.y = silu_fast(fmaf(p3.y, x3.y, fmaf(p3.x, x2.y, fmaf(p2.y, x1.y, p2.x * x0.y))));
       raw0 = raw1, raw1 = raw2, raw2 = raw;
     } else {
-      const float2 g = bf2(__ldg(reinterpret_cast<const uint32_t*>(a.g + (int64_t)t * a.ldg + h * kDim) + pair));
-      *reinterpret_cast<float2*>(&sa[buf][2 * pair]) =
-          make_float2(expf(a.lower_bound * sigmoid_exact(rate * (g.x + dt.x))),
-                      expf(a.lower_bound * sigmoid_exact(rate * (g.y + dt.y))));
+      const float2 g = bf2(raw), dt = __ldg(reinterpret_cast<const float2*>(a.dt_bias + h * kDim) + pair);
+      const float rate = exp_fast(__ldg(a.a_log + h));
+      o.x = exp_fast(a.lower_bound * sigmoid_fast(rate * (g.x + dt.x)));
+      o.y = exp_fast(a.lower_bound * sigmoid_fast(rate * (g.y + dt.y)));
     }
-    const float b = sigmoid_exact(__bfloat162float(a.beta[(int64_t)t * a.ldb + h]));
+    *reinterpret_cast<float2*>(y + part * kDim + 2 * pair) = o;
+    const float b = sigmoid_fast(beta);
+    if (t + 1 < e) {                                     // the next token's inputs, behind this one's arithmetic
+      raw = __ldg(in + (t + 1) * pitch);
+      beta = __bfloat162float(a.beta[(int64_t)(t + 1) * a.ldb + h]);
+    }
     __syncthreads();
-    float4 q = *reinterpret_cast<const float4*>(&sy[buf][0][4 * lane]);
-    float4 k = *reinterpret_cast<const float4*>(&sy[buf][1][4 * lane]);
-    const float4 dec = *reinterpret_cast<const float4*>(&sa[buf][4 * lane]);
-    const float v = sy[buf][2][kRowsW * warp + (lane & 15)];
-    float qq = q.x * q.x + q.y * q.y + q.z * q.z + q.w * q.w;
-    float kk = k.x * k.x + k.y * k.y + k.z * k.z + k.w * k.w;
-    float qk = q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w;
+    const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(y + 4 * lane);
+    const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(y + kDim + 4 * lane);
+    const ulonglong2 dec = *reinterpret_cast<const ulonglong2*>(y + 3 * kDim + 4 * lane);
+    float nq = sum2(fma2(q.y, q.y, mul2(q.x, q.x))), nk = sum2(fma2(k.y, k.y, mul2(k.x, k.x)));
+    float nd = sum2(fma2(q.y, k.y, mul2(q.x, k.x)));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      qq += __shfl_xor_sync(0xffffffffu, qq, o);
-      kk += __shfl_xor_sync(0xffffffffu, kk, o);
-      qk += __shfl_xor_sync(0xffffffffu, qk, o);
+    for (int o2 = 16; o2 > 0; o2 >>= 1) {
+      nq += __shfl_xor_sync(0xffffffffu, nq, o2);
+      nk += __shfl_xor_sync(0xffffffffu, nk, o2);
+      nd += __shfl_xor_sync(0xffffffffu, nd, o2);
     }
-    const float rq = a.scale / sqrtf(qq + 1e-6f), rk = 1.0f / sqrtf(kk + 1e-6f);
-    q = make_float4(q.x * rq, q.y * rq, q.z * rq, q.w * rq);
-    k = make_float4(k.x * rk, k.y * rk, k.z * rk, k.w * rk);
-    float d[32];                                       // S k of row i at i, scale S q at 16 + i
+    const float rq = a.scale * rsqrtf(nq + 1e-6f), rk = rsqrtf(nk + 1e-6f);
+    float d[2 * kRowsW];                                 // of row i: S k at i, S q at 16 + i (k, q not yet normalised)
 #pragma unroll
     for (int i = 0; i < kRowsW; ++i) {
-      float4& m = st[i];
-      m.x *= dec.x, m.y *= dec.y, m.z *= dec.z, m.w *= dec.w;
-      d[i] = m.x * k.x + m.y * k.y + m.z * k.z + m.w * k.w;
-      d[16 + i] = m.x * q.x + m.y * q.y + m.z * q.z + m.w * q.w;
+      ulonglong2& m = st[i];
+      m.x = mul2(m.x, dec.x);
+      m.y = mul2(m.y, dec.y);
+      d[i] = sum2(fma2(m.y, k.y, mul2(m.x, k.x)));
+      d[kRowsW + i] = sum2(fma2(m.y, q.y, mul2(m.x, q.x)));
     }
     const float tot = warp_sum_transposed(d, lane);
-    const float sqv = __shfl_xor_sync(0xffffffffu, tot, 16);      // lanes 0-15: S q of their row
-    const float u = b * (v - tot);                                // lanes 0-15: u of their row
-    if (lane < 16)
-      a.out[(int64_t)t * a.ldo + h * kDim + kRowsW * warp + lane] = __float2bfloat16(sqv + u * (qk * rq * rk));
+    const float sqv = __shfl_xor_sync(0xffffffffu, tot, kRowsW);       // lanes 0-15: S q of their row
+    const int row = kRowsW * warp + (lane & 15);
+    const float u = b * (y[2 * kDim + row] - tot * rk);                // lanes 0-15: u of their row
+    if (lane < kRowsW) a.out[(int64_t)t * a.ldo + h * kDim + row] = __float2bfloat16(sqv * rq + u * (nd * rq * rk));
+    const float ur = u * rk;
 #pragma unroll
     for (int i = 0; i < kRowsW; ++i) {
-      const float ui = __shfl_sync(0xffffffffu, u, i);
-      float4& m = st[i];
-      m.x = fmaf(ui, k.x, m.x), m.y = fmaf(ui, k.y, m.y), m.z = fmaf(ui, k.z, m.z), m.w = fmaf(ui, k.w, m.w);
+      const float ui = __shfl_sync(0xffffffffu, ur, i);
+      const uint64_t u2 = f2pack(ui, ui);
+      st[i].x = fma2(u2, k.x, st[i].x);
+      st[i].y = fma2(u2, k.y, st[i].y);
     }
   }
 #pragma unroll
-  for (int i = 0; i < kRowsW; ++i) *reinterpret_cast<float4*>(S + i * kDim) = st[i];
+  for (int i = 0; i < kRowsW; ++i) store_stream(S + i * kDim, st[i]);
   if (conv) {                                          // this head's channels of the block: no other CTA touches them
     *reinterpret_cast<uint32_t*>(cs) = raw0;
     *reinterpret_cast<uint32_t*>(cs + 3 * a.P) = raw1;

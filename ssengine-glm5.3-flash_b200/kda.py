@@ -37,6 +37,14 @@ def seq_table(seqs, device) -> torch.Tensor:
     return t.to(device)
 
 
+def _row_pitch(name: str, t: torch.Tensor, rows: int, cols: int) -> int:
+    """The row pitch of a bf16 matrix of at least rows x cols with unit column stride; ValueError otherwise."""
+    if t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape[0] < rows or t.shape[1] < cols or t.stride(1) != 1:
+        raise ValueError(f"{name}: bf16 [{rows}, >= {cols}] with unit column stride, got {t.dtype} {tuple(t.shape)} "
+                         f"strides {t.stride()}")
+    return t.stride(0)
+
+
 @dataclass
 class KdaLayer:
     """One KDA layer's parameters on the device."""
@@ -54,13 +62,14 @@ class KdaLayer:
         assert self.conv_weight.dtype == torch.bfloat16 and self.conv_weight.shape == (3 * H * HEAD_DIM, 4)
         assert self.conv_weight.is_contiguous() and self.a_log.dtype == torch.float32
         assert self.dt_bias.dtype == torch.float32 and self.dt_bias.numel() == H * HEAD_DIM
+        cs, rs = conv_state.stride(), rec_state.stride()
         assert conv_state.dtype == torch.bfloat16 and conv_state.shape[1:] == (3, 3 * H * HEAD_DIM)
-        assert conv_state[0].is_contiguous()
+        assert cs[1:] == (3 * H * HEAD_DIM, 1)
         assert rec_state.dtype == torch.float32 and rec_state.shape[1:] == (H, HEAD_DIM, HEAD_DIM)
-        assert rec_state[0].is_contiguous()
+        assert rs[1:] == (HEAD_DIM * HEAD_DIM, HEAD_DIM, 1) or (H == 1 and rs[2:] == (HEAD_DIM, 1))
         return lib.KdaLayerC(H, HEAD_DIM, self.conv_weight.data_ptr(), self.a_log.data_ptr(), self.dt_bias.data_ptr(),
-                             self.lower_bound, HEAD_DIM ** -0.5, conv_state.data_ptr(), conv_state.stride(0),
-                             rec_state.data_ptr(), rec_state.stride(0))
+                             self.lower_bound, HEAD_DIM ** -0.5, conv_state.data_ptr(), cs[0], rec_state.data_ptr(),
+                             rs[0])
 
     def prefill(self, qkv: torch.Tensor, g: torch.Tensor, beta: torch.Tensor, out: torch.Tensor, seqs: torch.Tensor,
                 conv_state: torch.Tensor, rec_state: torch.Tensor, stream=None, status: torch.Tensor | None = None,
@@ -93,21 +102,21 @@ class KdaLayer:
         sequence are not written. `status` (int32 [1] on the device) receives 1 if a sequence reaches outside the rows
         or names a negative block (it is skipped). Returns `out`."""
         so = lib.load()
-        T, P = qkv.shape[0], self.heads * HEAD_DIM
-        for name, t, cols in (("qkv", qkv, 3 * P), ("g", g, P), ("beta", beta, self.heads), ("out", out, P)):
-            if t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape[0] < T or t.shape[1] < cols or t.stride(1) != 1:
-                raise ValueError(f"{name}: bf16 [{T}, >= {cols}] with unit column stride, got {t.dtype} "
-                                 f"{tuple(t.shape)} strides {t.stride()}")
+        H = self.heads
+        P, T = H * HEAD_DIM, qkv.shape[0]
+        pitch = [_row_pitch(n, t, T, c) for n, t, c in (("qkv", qkv, 3 * P), ("g", g, P), ("beta", beta, H), ("out", out, P))]
         if seqs.dtype != torch.int32 or seqs.dim() != 2 or seqs.shape[1] != 4 or not seqs.is_contiguous():
             raise ValueError(f"seqs: contiguous int32 [R, 4], got {seqs.dtype} {tuple(seqs.shape)}")
-        if len({t.device for t in (qkv, g, beta, out, seqs, conv_state, rec_state, self.conv_weight)}) != 1:
-            raise ValueError("the tensors of one call must be on one device")
-        if not qkv.is_cuda:
+        dev = qkv.get_device()
+        for t in (g, beta, out, seqs, conv_state, rec_state, self.conv_weight):
+            if t.get_device() != dev:
+                raise ValueError("the tensors of one call must be on one device")
+        if dev < 0:
             raise ValueError(f"the tensors are on {qkv.device}, not on a GPU")
         L = self.c_struct(conv_state, rec_state)
-        rc = so.ssb_kda_decode(ctypes.byref(L), qkv.data_ptr(), qkv.stride(0), g.data_ptr(), g.stride(0),
-                               beta.data_ptr(), beta.stride(0), T, seqs.data_ptr(), seqs.shape[0], out.data_ptr(),
-                               out.stride(0), None if status is None else status.data_ptr(), lib.stream_ptr(stream))
+        rc = so.ssb_kda_decode(ctypes.byref(L), qkv.data_ptr(), pitch[0], g.data_ptr(), pitch[1], beta.data_ptr(),
+                               pitch[2], T, seqs.data_ptr(), seqs.shape[0], out.data_ptr(), pitch[3],
+                               None if status is None else status.data_ptr(), lib.stream_ptr(stream))
         lib.check("ssb_kda_decode", rc)
         return out
 

@@ -106,6 +106,7 @@ class _Counting:
                 return _fn(*args)
 
             self._wrapped[name] = w
+            self.__dict__[name] = w                        # later calls find it without __getattr__
         return w
 
 _P, _I32, _I64, _F = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
@@ -222,12 +223,13 @@ def stream_scratch(device, nbytes: int, stream=None):
     import torch
 
     dev = torch.device(device)
-    s = torch.cuda.current_stream(dev) if stream is None else stream
-    key = (dev.type, s.device.index, int(s.cuda_stream))
+    index = torch.cuda.current_device() if dev.index is None else dev.index
+    handle = torch._C._cuda_getCurrentRawStream(index) if stream is None else int(stream.cuda_stream)
+    key = (dev.type, index, handle)
     t = _SCRATCH.get(key)
     if t is None or t.numel() < nbytes:
-        with torch.cuda.stream(s):
-            t = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=s.device)
+        with torch.cuda.stream(torch.cuda.current_stream(dev) if stream is None else stream):
+            t = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
         _SCRATCH[key] = t
     return t
 
@@ -240,5 +242,7 @@ def check(name: str, rc: int) -> None:
 def stream_ptr(stream=None) -> int:
     import torch
 
-    s = torch.cuda.current_stream() if stream is None else stream
-    return int(s.cuda_stream)
+    if stream is None:
+        # the current stream's handle itself: building the Stream object costs 4 us a call
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return int(stream.cuda_stream)

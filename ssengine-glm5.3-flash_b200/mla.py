@@ -10,6 +10,8 @@ ssengine/model/pp_patch.py:643-672; ssengine/kernels.py config 25), the fork's F
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import lib
@@ -35,6 +37,7 @@ def sparse_mla(q8: torch.Tensor, kv_cache: torch.Tensor, indices: torch.Tensor, 
     return out
 
 
+@functools.cache
 def decode_workspace_bytes(T: int, heads: int) -> int:
     """Device bytes of the workspace of one `decode` / `decode_selected` call (`ssb_mla_decode_workspace_bytes`)."""
     n = lib.load().ssb_mla_decode_workspace_bytes(T, heads)
@@ -92,23 +95,26 @@ def _decode(q, kv_cache, indices, page_table, seq_lens, bmm1, out, bmm2, n_idx, 
             raise ValueError(f"{name}: contiguous {dt} {shape}, got {t.dtype} {tuple(t.shape)}")
     if reqs is None and page_table.shape[0] < T:
         raise ValueError(f"page_table has {page_table.shape[0]} rows for {T} query rows and no reqs")
-    if len({t.device for t in (q, kv_cache, page_table, out, seq_lens, indices, reqs, lse, workspace)
-            if t is not None}) != 1:
-        raise ValueError("the tensors of one call must be on one device")
     need = decode_workspace_bytes(T, H)
     if workspace is not None and (workspace.dtype != torch.uint8 or not workspace.is_contiguous() or
                                   workspace.numel() < need):
         raise ValueError(f"workspace: contiguous uint8 of {need} bytes or more")
-    if not q.is_cuda:
+    dev = q.get_device()
+    for t in (kv_cache, page_table, out, seq_lens, indices, reqs, lse, workspace):
+        if t is not None and t.get_device() != dev:
+            raise ValueError("the tensors of one call must be on one device")
+    if dev < 0:
         raise ValueError(f"the tensors are on {q.device}, not on a GPU")
     if workspace is None:
         workspace = lib.stream_scratch(q.device, need, stream)
     ptr = lambda t: None if t is None else t.data_ptr()
-    rc = so.ssb_mla_decode(q.data_ptr(), int(q.dtype == torch.uint8), q.stride(0), q.stride(1), T, H,
-                           kv_cache.data_ptr(), kv_cache.shape[0], page_table.data_ptr(), page_table.shape[0],
-                           page_table.shape[1], ptr(reqs), ptr(seq_lens), ptr(indices),
-                           0 if indices is None else indices.stride(0), n_idx or 0, bmm1, bmm2, out.data_ptr(),
-                           ptr(lse), workspace.data_ptr(), workspace.numel(), ptr(status), lib.stream_ptr(stream))
+    ldq, head_stride, _ = q.stride()
+    rows, width = page_table.shape
+    rc = so.ssb_mla_decode(q.data_ptr(), int(q.dtype == torch.uint8), ldq, head_stride, T, H, kv_cache.data_ptr(),
+                           kv_cache.shape[0], page_table.data_ptr(), rows, width, ptr(reqs), ptr(seq_lens),
+                           ptr(indices), 0 if indices is None else indices.stride(0), n_idx or 0, bmm1, bmm2,
+                           out.data_ptr(), ptr(lse), workspace.data_ptr(), workspace.numel(), ptr(status),
+                           lib.stream_ptr(stream))
     lib.check("ssb_mla_decode", rc)
     return out
 
