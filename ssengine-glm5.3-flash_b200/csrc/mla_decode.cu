@@ -12,7 +12,7 @@
 //
 // One CTA of 22 warps an SM, over units of 128 tokens and a tile of 64 heads:
 //   gather (4 warps): a whole page as TMA tiles (4 chunks [128 tokens x 128 B] and the rope keys), a row's last page and
-//       selected tokens by cp.async row by row, what is not there zero-filled; pages ahead prefetched into L2;
+//       selected tokens by cp.async row by row, what is not there zero-filled;
 //   scores (1 warp issues): S^T [128 tokens x 64 heads] = K Q^T, tcgen05 kind::f8f6f4, M = 128. bf16 queries enter
 //       exactly, as two e4m3 parts (64 high rows, 64 low ones, N = 128): the half of the tensor core that 64 heads alone
 //       would leave idle;
@@ -65,12 +65,12 @@ constexpr int kOffMask = kOffRise + 32;         // uint32 [2][4]: tokens present
 constexpr int kOffScale = kOffMask + 32;        // float [2][64]: base-2 score scale, minus the reference of each head
 constexpr int kOffExp = kOffScale + 512;        // float [4][64]: maxima of the token quarters, or their sums
 constexpr int kOffSum = kOffExp + 1024;         // float [64]: rescale factors, bmm2 / l
-constexpr int kSmem = kOffSum + 256;
+constexpr int kOffPlan = kOffSum + 256;         // int32 [52]: the plan's sums and first row
+constexpr int kSmem = kOffPlan + 208;
 static_assert(kOffScale % 16 == 0 && kOffExp % 16 == 0 && kOffSf % 128 == 0 && kSmem <= 232448, "shared memory");
 // TMEM columns: O^T as 4 tiles of 128 dims x 64 heads, S^T 128 tokens x (64 high | 64 low), block scales of V (2^-7 against
 // the high parts of P, 2^-11 against the low ones) and of P (2 columns a unit)
 constexpr uint32_t kColO = 0, kColS = 256, kColV = 384, kColLow = 388, kColP = 392;
-constexpr int kAhead = 1;                       // pages prefetched into L2 beyond the two in shared memory
 constexpr float kMaxRise = 4.0f;                // base-2 scores above a head's reference before it moves and O is rescaled
 constexpr float kNoHead = -1000.0f;             // base-2 score of the heads that the tile does not have: weight 0
 constexpr uint32_t kSw128 = 2, kSw64 = 4;       // descriptor layout types
@@ -102,16 +102,10 @@ SSB_DEVICE void tmem_ld_x16(uint32_t taddr, float (&v)[16]) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
-// Two columns of each of the 4 tiles of O^T (64 columns apart).
-SSB_DEVICE void tmem_ld_2x4(uint32_t taddr, float (&v)[8]) {
-  uint32_t r[8];
-#pragma unroll
-  for (int d = 0; d < 4; ++d)
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];"
-                 : "=r"(r[2 * d]), "=r"(r[2 * d + 1])
-                 : "r"(taddr + 64 * d));
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+SSB_DEVICE void tmem_ld_x4(uint32_t taddr, float (&v)[4]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
+               : "r"(taddr));
 }
 SSB_DEVICE void tmem_st_x16(uint32_t taddr, const float (&v)[16]) {
   asm volatile(
@@ -142,12 +136,6 @@ SSB_DEVICE void cp_async_arrive_noinc(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 SSB_DEVICE void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-SSB_DEVICE void tma_prefetch_2d(const CUtensorMap* m, int32_t x, int32_t y) {
-  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(m)), "r"(x),
-               "r"(y)
-               : "memory");
-}
-
 // Sums over the 32 lanes of 16 values a lane, transposed: lane l receives the total of value l & 15.
 SSB_DEVICE float warp_sum_transposed(float (&v)[16], int lane) {
 #pragma unroll
@@ -237,82 +225,97 @@ SSB_DEVICE void mbar_arrive_n(uint32_t bar, uint32_t n) {
 // ---- the plan -----------------------------------------------------------------------------------------------------
 // Tokens and units of row t. How many tokens a row's list names is not known before it is read: its share is planned
 // by the list's width or, where that is smaller, the tokens it can name.
-SSB_DEVICE int row_units(const MlaDecodeArgs& a, int64_t t) {
-  int64_t n = a.indices != nullptr ? a.n_idx : (int64_t)a.width * kUnit;
-  if (a.seq_lens != nullptr) n = min(n, (int64_t)a.seq_lens[t]);
-  if (a.reqs != nullptr && (a.reqs[t] < 0 || a.reqs[t] >= a.R)) n = 0;
-  return n > 0 ? static_cast<int>((n + kUnit - 1) / kUnit) : 0;
+SSB_DEVICE int row_units(const MlaDecodeArgs& a, int t) {
+  int n = a.indices != nullptr ? a.n_idx : 0x7fffff00;
+  if (a.seq_lens != nullptr) n = min(n, a.seq_lens[t]);
+  if (a.reqs != nullptr && static_cast<uint32_t>(a.reqs[t]) >= static_cast<uint32_t>(a.R)) n = 0;
+  n = n > 0 ? (n + kUnit - 1) / kUnit : 0;
+  return a.indices != nullptr ? n : min(n, a.width);
 }
 
 // A CTA's share of one row: units [b0, b1) of the row's nb planned ones; every role walks the same segments.
 struct Segment {
-  int64_t t;
-  int b0, b1, nb;
+  int t, b0, b1, nb;
 };
+// Ranges are cut in units plus `cost` for every row that has any (a row's staging, drain and epilogue take a CTA about as
+// long as two units; none where a range is a few units and every cut row would lose more).
 struct Walk {
-  int64_t t, at, hi, first;                     // next row, next unit, end of the range, units before row t
+  int t, nb, first, lo, hi, cost;               // next row, its units, the units and costs before it, the range, the cost
 };
 __device__ __noinline__ bool walk_next(const MlaDecodeArgs& a, Walk& w, Segment& s) {
-  for (; w.t < a.T && w.at < w.hi; ++w.t) {
-    const int nb = row_units(a, w.t);
-    if (nb == 0) continue;
-    const int64_t end = min(w.hi, w.first + nb);
-    s.t = w.t, s.b0 = static_cast<int>(w.at - w.first), s.b1 = static_cast<int>(end - w.first), s.nb = nb;
-    w.at = end;
-    w.first += nb;
-    ++w.t;
-    return true;
+  bool found = false;
+  while (!found && w.first < w.hi) {
+    s.t = w.t, s.nb = w.nb;
+    s.b0 = max(w.lo - w.first, 0), s.b1 = min(w.hi - w.first, w.nb);
+    found = s.b0 < s.b1;
+    if (w.nb > 0) w.first += w.nb + w.cost;
+    if (++w.t >= a.T) {
+      w.first = w.hi;
+    } else {
+      w.nb = row_units(a, w.t);
+    }
   }
-  return false;
+  return found;
+}
+constexpr int kRowCost = 2, kCostFrom = 6;      // units; ranges of so many units or more bear it
+
+// All threads of the CTA: its range and the row that holds its beginning. sh: 48 words for the warps' sums, 4 for the row.
+// False: more CTAs than units, nothing to do here.
+SSB_DEVICE bool find_range(const MlaDecodeArgs& a, int cta, int ctas, int32_t* sh, Walk& w) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int units = 0, rows = 0;
+#pragma unroll 1
+  for (int t = tid; t < a.T; t += kThreads) {
+    const int n = row_units(a, t);
+    units += n;
+    rows += n > 0;
+  }
+  units = __reduce_add_sync(0xffffffffu, units);
+  rows = __reduce_add_sync(0xffffffffu, rows);
+  if (lane == 0) sh[warp] = units, sh[24 + warp] = rows;
+  __syncthreads();
+  units = __reduce_add_sync(0xffffffffu, lane < kThreads / 32 ? sh[lane] : 0);
+  rows = __reduce_add_sync(0xffffffffu, lane < kThreads / 32 ? sh[24 + lane] : 0);
+  const int used = min(ctas, units);            // every range in use holds a unit: a row's CTAs are consecutive
+  if (cta >= used) return false;
+  w.cost = units >= kCostFrom * ctas ? kRowCost : 0;
+  const int total = units + rows * w.cost, per = total / used, rem = total - per * used;
+  w.lo = cta * per + min(cta, rem);
+  w.hi = w.lo + per + (cta < rem);
+  if (warp == 0) {
+    int base = 0;
+#pragma unroll 1
+    for (int c = 0;; c += 32) {
+      const int t = c + lane, nb = t < a.T ? row_units(a, t) : 0, v = nb > 0 ? nb + w.cost : 0;
+      int end = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, end, o);
+        if (lane >= o) end += x;
+      }
+      end += base;
+      const bool hit = end - v <= w.lo && w.lo < end;
+      if (hit) sh[48] = t, sh[49] = nb, sh[50] = end - v;
+      base = __shfl_sync(0xffffffffu, end, 31);
+      if (__any_sync(0xffffffffu, hit)) break;
+    }
+  }
+  __syncthreads();
+  w.t = sh[48], w.nb = sh[49], w.first = sh[50];
+  return true;
 }
 
-// All threads of the CTA: its range of units and the row that holds the first of them. sh: 16 int64 words for the warps'
-// sums, 2 for the row. False: more CTAs than units, nothing to do here.
-SSB_DEVICE bool find_range(const MlaDecodeArgs& a, int cta, int ctas, int64_t* sh, Walk& out) {
-  constexpr int kScan = kSoftmax;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const bool in = tid < kScan;
-  int64_t n = 0, total = 0;
+// Rows without a token: zeros. One warp.
+__device__ __noinline__ void zero_rows(const MlaDecodeArgs& a, int cta, int h0, int nh, int lane) {
 #pragma unroll 1
-  for (int64_t t = tid; in && t < a.T; t += kScan) n += row_units(a, t);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-  if (in && lane == 0) sh[warp] = n;
-  if (tid == 0) sh[16] = a.T, sh[17] = 0;
-  __syncthreads();
-#pragma unroll 1
-  for (int w = 0; w < kSoftWarps; ++w) total += sh[w];
-  const int64_t used = min((int64_t)ctas, total);      // every range in use holds a unit: a row's CTAs are consecutive
-  const int64_t lo = cta < used ? total * cta / used : total;
-  out.at = lo;
-  out.hi = cta < used ? total * (cta + 1) / used : total;
-  int64_t base = 0;
-#pragma unroll 1
-  for (int64_t c = 0; c < a.T && base <= lo; c += kScan) {
-    const int64_t t = c + tid;
-    n = in && t < a.T ? row_units(a, t) : 0;
-    int64_t end = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, end, o);
-      if (lane >= o) end += v;
-    }
-    __syncthreads();
-    if (in && lane == 31) sh[warp] = end;
-    __syncthreads();
-    int64_t before = base;
-#pragma unroll 1
-    for (int w = 0; w < kSoftWarps; ++w) {
-      if (w < warp) before += sh[w];
-      base += sh[w];
-    }
-    end += before;
-    if (n > 0 && end - n <= lo && lo < end) sh[16] = t, sh[17] = end - n;
+  for (int t = cta; t < a.T; t += gridDim.x) {
+    if (row_units(a, t) != 0) continue;
+    if (lane == 0 && a.reqs != nullptr && static_cast<uint32_t>(a.reqs[t]) >= static_cast<uint32_t>(a.R))
+      raise_status(a.status, kErrArgs);
+    uint4* o = reinterpret_cast<uint4*>(a.out + ((int64_t)t * a.H + h0) * kDv);
+    for (int i = lane; i < nh * kDv / 8; i += 32) o[i] = make_uint4(0, 0, 0, 0);
+    for (int i = lane; a.lse != nullptr && i < nh; i += 32) a.lse[(int64_t)t * a.H + h0 + i] = kNone;
   }
-  __syncthreads();
-  out.t = sh[16];
-  out.first = sh[17];
-  return out.at < out.hi;
 }
 
 SSB_DEVICE float* part_o(const MlaDecodeArgs& a, int tile, int slot) {
@@ -385,12 +388,12 @@ SSB_DEVICE void issue_values(const Bars& B, uint32_t sbase, int buf, bool fresh,
 // parts hold a value exactly unless it is below 2^-14 of the head's largest. Also each head's score scale (its reference
 // cleared). 8 threads a head, 9 granules each (twice: for the largest value, then from the L1 cache for the parts).
 template <bool Q8>
-__device__ __noinline__ void stage_q(const MlaDecodeArgs& a, uint8_t* smem, int64_t t, int h0, int nh) {
+__device__ __noinline__ void stage_q(const MlaDecodeArgs& a, uint8_t* smem, int t, int h0, int nh) {
   uint8_t* Q = smem + kOffQ;
   float* scale = reinterpret_cast<float*>(smem + kOffScale);
   const int h = threadIdx.x >> 3, sub = threadIdx.x & 7;
   const bool have = h < nh;
-  const int64_t off = t * a.ldq + (int64_t)(h0 + min(h, nh - 1)) * a.hsq;
+  const int64_t off = (int64_t)t * a.ldq + (int64_t)(h0 + min(h, nh - 1)) * a.hsq;
   int k = 0;
   if (Q8) {
     const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.q) + off);
@@ -404,11 +407,14 @@ __device__ __noinline__ void stage_q(const MlaDecodeArgs& a, uint8_t* smem, int6
     uint4 v[9];
 #pragma unroll
     for (int j = 0; j < 9; ++j) v[j] = __ldg(q + sub + 8 * j);        // 72 granules of 8 values
-    uint32_t top = 0;                                                 // bf16 magnitudes, two at a time
+    __nv_bfloat162 most = __floats2bfloat162_rn(0.0f, 0.0f);          // magnitudes, NaN kept
 #pragma unroll
-    for (int j = 0; j < 9; ++j)
-      top = __vmaxu2(top, __vmaxu2(__vmaxu2(v[j].x & 0x7FFF7FFFu, v[j].y & 0x7FFF7FFFu),
-                                   __vmaxu2(v[j].z & 0x7FFF7FFFu, v[j].w & 0x7FFF7FFFu)));
+    for (int j = 0; j < 9; ++j) {
+      const __nv_bfloat162* w = reinterpret_cast<const __nv_bfloat162*>(&v[j]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) most = __hmax2_nan(most, __habs2(w[e]));
+    }
+    uint32_t top = *reinterpret_cast<uint32_t*>(&most) & 0x7FFF7FFFu;
     top = max(top & 0xFFFFu, top >> 16);
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -457,44 +463,36 @@ __global__ void __launch_bounds__(kThreads, 1)
     return;
   }
 
-  // rows without a token: zeros
-#pragma unroll 1
-  for (int64_t t = cta; t < a.T; t += gridDim.x) {
-    if (row_units(a, t) != 0) continue;
-    if (tid == 0 && a.reqs != nullptr && (a.reqs[t] < 0 || a.reqs[t] >= a.R)) raise_status(a.status, kErrArgs);
-    uint4* o = reinterpret_cast<uint4*>(a.out + (t * a.H + h0) * kDv);
-    for (int i = tid; i < nh * kDv / 8; i += kThreads) o[i] = make_uint4(0, 0, 0, 0);
-    if (a.lse != nullptr && tid < nh) a.lse[t * a.H + h0 + tid] = kNone;
-  }
-  Walk walk;
-  const bool work = find_range(a, cta, gridDim.x, reinterpret_cast<int64_t*>(smem + kOffPlo), walk);
-  if (!work) return;
-  if (tid == 0) {
-#pragma unroll 1
-    for (int i = 0; i < 8; ++i) {                        // every gather lane's copies; for the last chunk also an
-      mbar_init(B.lat_full + 8 * i, 128 + ((i & 3) == 3 ? kGatherWarps : 0));      // arrival a warp for its mask word
-      mbar_init(B.lat_empty + 8 * i, 1);
+  asm volatile("griddepcontrol.launch_dependents;");     // the join may be set up meanwhile (it waits for this grid's end)
+  if (warp == kScoreWarp) {
+    if (lane < 24) {                                     // the barriers, one a lane
+      const int i = lane;
+      // lat_full: every gather lane's copies, for the last chunk also an arrival a warp for its mask word
+      const uint32_t n = i < 8 ? 128 + ((i & 3) == 3 ? kGatherWarps : 0) : i < 16 ? 1
+                         : i == 16 || i == 18 || i == 19 ? kSoftWarps : i < 22 ? 1 : i == 22 ? 2 : 4;
+      mbar_init(bar + 8 * i, n);
+      if (i == 23) {
+        mbar_init(bar + 8 * 24, 4);
+        mbar_init(bar + 8 * 25, 4);
+        mbar_init(bar + 8 * 26, 4);
+      }
     }
-    mbar_init(B.q_full, kSoftWarps);
-    mbar_init(B.s_full, 1);
-    mbar_init(B.s_empty, kSoftWarps);
-    mbar_init(B.p_full, kSoftWarps);
-    mbar_init(B.pv_done, 1);
-    mbar_init(B.o_full, 1);
-    mbar_init(B.drain, 2);
-#pragma unroll 1
-    for (int i = 0; i < 4; ++i) mbar_init(B.agree + 8 * i, 4);
-#pragma unroll 1
-    for (int i = 0; i < 8; ++i) reinterpret_cast<int32_t*>(smem + kOffRise)[i] = 0;
-    *abort_flag = 0;
+    if (lane < 8) reinterpret_cast<int32_t*>(smem + kOffRise)[lane] = 0;
+    if (lane == 8) *abort_flag = 0;
     fence_barrier_init();
-  }
-  if (warp == 0) {
+  } else if (warp == kValueWarp) {
     tmem_alloc(smem_u32(tmem_slot), 512);
     tmem_relinquish();
   }
   tc_fence_before();
-  __syncthreads();                                       // also: every thread has read the plan's words
+  Walk walk;
+  if (!find_range(a, cta, gridDim.x, reinterpret_cast<int32_t*>(smem + kOffPlan), walk)) {
+    if (warp == kValueWarp) {
+      zero_rows(a, cta, h0, nh, lane);
+      tmem_dealloc(0, 512);
+    }
+    return;
+  }
   tc_fence_after();
   constexpr uint32_t tmem = 0;                           // the whole of TMEM: its first lane and column
   if (*tmem_slot != tmem && tid == 0) {
@@ -510,9 +508,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     Segment s;
     bool ok = true;
     while (ok && walk_next(a, walk, s)) {
-      const int32_t* pages = a.table + (a.reqs != nullptr ? (int64_t)a.reqs[s.t] : s.t) * a.width;
+      const int32_t* pages = a.table + (int64_t)(a.reqs != nullptr ? a.reqs[s.t] : s.t) * a.width;
       const int len = a.seq_lens != nullptr ? a.seq_lens[s.t] : 0x7fffffff;
-      const int32_t* idx = a.indices != nullptr ? a.indices + s.t * a.ld_idx : nullptr;
+      const int32_t* idx = a.indices != nullptr ? a.indices + (int64_t)s.t * a.ld_idx : nullptr;
       int c0 = s.b0, c1 = s.b1;
       unsigned long long live = ~0ull;                   // bit i: unit c0 + i holds a selected token
       if (idx != nullptr) {                              // the row's planned share as units of list columns
@@ -548,16 +546,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       int c = next_live(c0);
       int p = token(c);
       int64_t page = p >= 0 ? page_row(p) : -1;
-      int ahead = idx == nullptr ? c0 + 2 : c1;          // next page to prefetch: whole pages only
       while (c < c1) {
         const int buf = u & 1, cn = next_live(c + 1);
-        for (; ahead < c1 && ahead <= c + 2 + kAhead; ++ahead) {
-          const int64_t y = page_row(ahead * kUnit);
-          if (lane == 0 && y >= 0 && y + kUnit <= a.cache_rows && (ahead + 1) * kUnit <= len) {
-            tma_prefetch_2d(&mlat, 128 * w, static_cast<int>(y));
-            if (w == 3) tma_prefetch_2d(&mrope, kDv, static_cast<int>(y));
-          }
-        }
         int pn = -1;
         int64_t page_n = -1;
         if (cn < c1) {
@@ -627,6 +617,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     cp_async_wait_all();
   } else if (warp == kValueWarp) {
     // ---------------------------------------------------------------- value products
+    zero_rows(a, cta, h0, nh, lane);
+    __syncwarp();
     const bool leader = elect_lane();
     int u = 0;
     Segment s;
@@ -858,35 +850,37 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (quarter == 0 && lane < 16) {
         if (!whole) part_ml(a, tile, slot)[mine] = make_float2(ref, total);
         else if (a.lse != nullptr && mine < nh)
-          a.lse[done.t * a.H + h0 + mine] = total == 0.0f ? kNone : ((ref == kNone ? 0.0f : ref) + log2f(total)) * kLn2;
+          a.lse[(int64_t)done.t * a.H + h0 + mine] = total == 0.0f ? kNone : ((ref == kNone ? 0.0f : ref) + log2f(total)) * kLn2;
         if (group == 0 && lane == 0 && tile == 0) {
           if (done.b0 == 0) a.rows[done.t].first = cta, a.rows[done.t].first_slot = slot;
           if (done.b1 == done.nb) a.rows[done.t].last = cta;
         }
       }
-      __nv_bfloat16* out = a.out + (done.t * a.H + h0 + hb) * kDv + row;
+      __nv_bfloat16* out = a.out + ((int64_t)done.t * a.H + h0 + hb) * kDv + row;
       float* po = part_o(a, tile, slot) + hb * kDv + row;
 #pragma unroll 1
-      for (int i = 0; i < 16; i += 2) {                  // 2 heads x 4 tiles of 128 dims; a lane holds one dim of each
-        float o[8];
-        tmem_ld_2x4(tq + kColO + hb + i, o);
+      for (int i = 0; i < 16; i += 4) {                  // 4 heads x 4 tiles of 128 dims; a lane holds one dim of each
+        float o[4][4];
+#pragma unroll
+        for (int d = 0; d < 4; ++d) tmem_ld_x4(tq + kColO + 64 * d + hb + i, o[d]);
         tmem_ld_wait();
         if (whole) {
-          const float inv0 = sums[hb + i], inv1 = sums[hb + i + 1];
 #pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            if (hb + i < nh) out[128 * d] = __float2bfloat16(o[2 * d] * inv0);
-            if (hb + i + 1 < nh) out[kDv + 128 * d] = __float2bfloat16(o[2 * d + 1] * inv1);
+          for (int e = 0; e < 4; ++e) {
+            const float inv = sums[hb + i + e];
+            if (hb + i + e < nh) {
+#pragma unroll
+              for (int d = 0; d < 4; ++d) out[e * kDv + 128 * d] = __float2bfloat16(o[d][e] * inv);
+            }
           }
         } else {
 #pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            po[128 * d] = o[2 * d];
-            po[kDv + 128 * d] = o[2 * d + 1];
-          }
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) po[e * kDv + 128 * d] = o[d][e];
         }
-        out += 2 * kDv;
-        po += 2 * kDv;
+        out += 4 * kDv;
+        po += 4 * kDv;
       }
       tc_fence_before();
       ++seg;
@@ -894,7 +888,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 0) {
+  if (warp == kValueWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -909,7 +903,8 @@ __global__ void __launch_bounds__(128) mla_join_kernel(const __grid_constant__ M
   const int64_t t = blockIdx.x;
   const int h = blockIdx.y, tile = h / kTileH, hh = h - tile * kTileH;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (row_units(a, t) == 0) return;
+  asm volatile("griddepcontrol.wait;" ::: "memory");       // the parts are written
+  if (row_units(a, static_cast<int>(t)) == 0) return;
   const MlaRowParts rp = a.rows[t];
   if (rp.first == rp.last) return;
   const bool spread = gridDim.z == 4;
@@ -969,6 +964,8 @@ int launch_mla_decode(const MlaDecodeArgs& a_in, void* ws, int64_t ws_bytes, cud
       (a.indices != nullptr && (a.n_idx < 0 || a.ld_idx < a.n_idx)) || (a.reqs == nullptr && a.T > a.R))
     return kErrArgs;
   if (a.T == 0) return kOk;
+  const int64_t most = a.indices != nullptr ? (a.n_idx + kUnit - 1) / kUnit : a.width;      // units of a row
+  if (a.T * (most + kRowCost) > 0x7fffffff) return kErrArgs;
   if (a.q == nullptr || a.kv == nullptr || a.table == nullptr || a.out == nullptr || ws == nullptr ||
       !aligned(a.q, 16) || !aligned(a.kv, 16) || !aligned(a.out, 16) || !aligned(ws, 256) || (a.ldq * eb) % 16 ||
       (a.hsq * eb) % 16 || a.hsq < kDq || (a.T > 1 && a.ldq < kDq))
@@ -996,8 +993,16 @@ int launch_mla_decode(const MlaDecodeArgs& a_in, void* ws, int64_t ws_bytes, cud
   if (cudaGetLastError() != cudaSuccess) return kErrCuda;
   // few rows are cut into many parts each: their CTAs are spread over the parts and the output values
   const unsigned z = a.T * a.H <= 8 * kMaxCtas ? 4 : 1;
-  mla_join_kernel<<<dim3((unsigned)a.T, (unsigned)a.H, z), 128, 0, stream>>>(a);
-  return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)a.T, (unsigned)a.H, z);
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, mla_join_kernel, a) == cudaSuccess ? kOk : kErrCuda;
 }
 
 }  // namespace ssb
