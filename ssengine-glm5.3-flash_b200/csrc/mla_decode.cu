@@ -151,6 +151,19 @@ SSB_DEVICE float warp_sum_transposed(float (&v)[16], int lane) {
   }
   return v[0];
 }
+// Transposes 4 x 4 values over 4 neighbouring lanes: v[i] of lane l becomes v[l] of lane i (of the four).
+SSB_DEVICE void cross4(float (&v)[4], int lane) {
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i & o) continue;
+      const float got = __shfl_xor_sync(0xffffffffu, up ? v[i] : v[i + o], o);
+      if (up) v[i] = got; else v[i + o] = got;
+    }
+  }
+}
 // Largest of the 32 lanes' values, NaN ignored (all NaN: NaN).
 SSB_DEVICE float warp_max(float v) {
   float r;
@@ -422,19 +435,25 @@ __device__ __noinline__ void stage_q(const MlaDecodeArgs& a, uint8_t* smem, int 
     if (ex != 0) k = max(min(ex - 134, 120), -120);
     // an infinite or NaN query value leaves its head no finite score: NaN, which e4m3 can carry (it has no infinity)
     const float down = !have ? 0.0f : ex == 255 ? NAN : __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+    // granule j of 8 values: half of 16-byte granule 4 j + (sub >> 1) of the row, in chunk j >> 1; the last in the rope
+    uint8_t* even = Q + sw128(h, sub >> 1) + 8 * (sub & 1);
+    uint8_t* odd = Q + sw128(h, 4 + (sub >> 1)) + 8 * (sub & 1);
 #pragma unroll 1
     for (int j = 0; j < 9; ++j) {
-      const int g = sub + 8 * j;
-      const uint4 w4 = __ldg(q + g);
+      const uint4 w4 = __ldg(q + sub + 8 * j);
       const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
       uint32_t hi[4], lo[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         split2(__uint_as_float(w[e] << 16) * down, __uint_as_float(w[e] & 0xFFFF0000u) * down, hi[e], lo[e]);
-      const uint32_t at = row_off(h, g >> 1) + 8 * (g & 1);           // 8 values: half a 16-byte granule
-      const uint32_t low = g < 64 ? 64 * 128 : 64 * 64;               // 64 rows further on, where the swizzle repeats
-      *reinterpret_cast<uint2*>(Q + at) = make_uint2(hi[0] | (hi[1] << 16), hi[2] | (hi[3] << 16));
-      *reinterpret_cast<uint2*>(Q + at + low) = make_uint2(lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16));
+      uint8_t* at = even;
+      if (j == 8) at = Q + kLat + sw64(h, sub >> 1) + 8 * (sub & 1);
+      *reinterpret_cast<uint2*>(at) = make_uint2(hi[0] | (hi[1] << 16), hi[2] | (hi[3] << 16));
+      at += j < 8 ? 64 * 128 : 64 * 64;                               // 64 rows further on, where the swizzle repeats
+      *reinterpret_cast<uint2*>(at) = make_uint2(lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16));
+      at = even + kChunk;
+      even = odd;
+      odd = at;
     }
   }
   if (sub == 0) {
@@ -856,28 +875,30 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (done.b1 == done.nb) a.rows[done.t].last = cta;
         }
       }
-      __nv_bfloat16* out = a.out + ((int64_t)done.t * a.H + h0 + hb) * kDv + row;
-      float* po = part_o(a, tile, slot) + hb * kDv + row;
+      // a lane has one dim of 4 heads; crossed with its 3 neighbours, 4 dims of head (lane & 3)
+      const int e = lane & 3, dim = 32 * quarter + (lane & 28);
+      __nv_bfloat16* out = a.out + ((int64_t)done.t * a.H + h0 + hb + e) * kDv + dim;
+      float* po = part_o(a, tile, slot) + (hb + e) * kDv + dim;
 #pragma unroll 1
-      for (int i = 0; i < 16; i += 4) {                  // 4 heads x 4 tiles of 128 dims; a lane holds one dim of each
+      for (int i = 0; i < 16 && hb + i < nh; i += 4) {   // 4 heads x 4 tiles of 128 dims
         float o[4][4];
 #pragma unroll
         for (int d = 0; d < 4; ++d) tmem_ld_x4(tq + kColO + 64 * d + hb + i, o[d]);
         tmem_ld_wait();
-        if (whole) {
+        const float inv = whole ? sums[hb + i + e] : 1.0f;
+        const bool have = hb + i + e < nh;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float inv = sums[hb + i + e];
-            if (hb + i + e < nh) {
-#pragma unroll
-              for (int d = 0; d < 4; ++d) out[e * kDv + 128 * d] = __float2bfloat16(o[d][e] * inv);
-            }
+        for (int d = 0; d < 4; ++d) {
+          cross4(o[d], lane);
+          if (whole) {
+            const __nv_bfloat162 v0 = __floats2bfloat162_rn(o[d][0] * inv, o[d][1] * inv);
+            const __nv_bfloat162 v1 = __floats2bfloat162_rn(o[d][2] * inv, o[d][3] * inv);
+            if (have)
+              *reinterpret_cast<uint2*>(out + 128 * d) =
+                  make_uint2(*reinterpret_cast<const uint32_t*>(&v0), *reinterpret_cast<const uint32_t*>(&v1));
+          } else {
+            *reinterpret_cast<float4*>(po + 128 * d) = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
           }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int d = 0; d < 4; ++d) po[e * kDv + 128 * d] = o[d][e];
         }
         out += 4 * kDv;
         po += 4 * kDv;
