@@ -168,10 +168,12 @@ class KdaAttention:
         self._lib = lib.load()
 
     def forward(self, y: torch.Tensor, seqs: torch.Tensor, conv_state: torch.Tensor, rec_state: torch.Tensor,
-                status: torch.Tensor, out: torch.Tensor | None = None, stream=None, keep: bool = False) -> torch.Tensor:
+                status: torch.Tensor, out: torch.Tensor | None = None, stream=None, keep: bool = False,
+                decode: bool = False) -> torch.Tensor:
         """y bf16 [T, H] (the layer input after the boundary's RMSNorm) -> attention output bf16 [T, H]; the KDA state
         blocks of `seqs` (int32 [R, 4] on the device) are updated in place. keep: the intermediates stay in
-        `self.parts` (for checks)."""
+        `self.parts` (for checks). decode: the recurrence token by token (`KdaLayer.decode`), for a step's few new
+        rows a request, in place of the chunked scan."""
         T, P, dev = y.shape[0], self.P, self.device
         s = lib.stream_ptr(stream)
         proj = torch.empty(T, self.in_proj.N_pad, dtype=torch.bfloat16, device=dev)
@@ -184,7 +186,8 @@ class KdaAttention:
         ogate = torch.empty(T, P, dtype=torch.bfloat16, device=dev)
         self.g_b(g_a, ogate, status, stream)
         o = torch.empty(T, P, dtype=torch.bfloat16, device=dev)
-        self.kda.prefill(proj, gate, beta, o, seqs, conv_state, rec_state, stream=stream, status=status)
+        scan = self.kda.decode if decode else self.kda.prefill
+        scan(proj, gate, beta, o, seqs, conv_state, rec_state, stream=stream, status=status)
         if keep:
             self.parts = dict(proj=proj, gate=gate, ogate=ogate, o=o.clone())
         if out is None:
@@ -264,10 +267,11 @@ class KdaDecoderLayer:
         self.moe = self.ffn                  # the FFN sub-block (MoELayer or DenseFfn)
         self.device = dev
 
-    def forward(self, res, x_prev, post_prev, comb_prev, seqs, conv_state, rec_state, status, stream=None):
+    def forward(self, res, x_prev, post_prev, comb_prev, seqs, conv_state, rec_state, status, stream=None,
+                decode: bool = False):
         """res bf16 [T, 4, H]; x_prev bf16 [T, H] with post_prev fp32 [T, 4] / comb_prev [T, 4, 4] (x_prev None: the
-        first layer of the stage, pre only). Returns (res after attention, MoE rows, post, comb) for the next
-        boundary."""
+        first layer of the stage, pre only); decode: `KdaAttention.forward`'s. Returns (res after attention, MoE
+        rows, post, comb) for the next boundary."""
         T, H, dev = res.shape[0], self.H, self.device
         f32 = dict(dtype=torch.float32, device=dev)
         res_a = torch.empty_like(res) if x_prev is not None else res
@@ -275,7 +279,7 @@ class KdaDecoderLayer:
         y = torch.empty(T, H, dtype=torch.bfloat16, device=dev)
         self.bound_a(x_prev, res, post_prev, comb_prev, res_a if x_prev is not None else None, post_a, comb_a, y,
                      stream, status=status)
-        x_a = self.attn.forward(y, seqs, conv_state, rec_state, status, stream=stream)
+        x_a = self.attn.forward(y, seqs, conv_state, rec_state, status, stream=stream, decode=decode)
         res_b = torch.empty_like(res)
         post_b, comb_b = torch.empty(T, 4, **f32), torch.empty(T, 4, 4, **f32)
         self.bound_b(x_a, res_a, post_a, comb_a, res_b, post_b, comb_b, y, stream, status=status)
@@ -454,13 +458,22 @@ class DsaAttention:
         return self._side
 
     def forward(self, y, positions, slots, qsl, page_table, kpool_reqs, max_rows, groups, kv_cache, pool_cache,
-                tail_ring, status, stream=None, keep: bool = False):
+                tail_ring, status, stream=None, keep: bool = False, decode: tuple | None = None):
         """y bf16 [T, H]; positions / slots int64 [T]; qsl int32 [R + 1]; page_table int32 [R, width] (KV pages);
         kpool_reqs int32 [R, 4] {first row, rows, start position, tail block}; groups: the indexer's work groups
         (int32 [G, 4]); kv_cache e4m3 bytes uint8 [pages * 128, 576], pool_cache bf16 [pages * 32, 128], tail_ring bf16
-        [blocks, 2, 4, 128] updated in place -> bf16 [T, H]."""
+        [blocks, 2, 4, 128] updated in place -> bf16 [T, H].
+
+        decode (form, reqs int32 [T], seq_lens int32 [T]): the attention of a step's few new rows a request (row t's
+        request and the tokens that it sees, positions[t] + 1), split over the cache: form "selected" over the
+        indexer's tokens as in the prefill (`mla.decode_selected`), "dense" over the whole context (`mla.decode`;
+        the pool keys are inserted, the logits and the top-k are left out)."""
         from . import indexer, mla
 
+        form, reqs, seq_lens = decode if decode is not None else (None, None, None)
+        if form not in (None, "selected", "dense"):
+            raise ValueError(f"decode form {form!r}")
+        select = form != "dense"
         T, dev, s = y.shape[0], self.device, lib.stream_ptr(stream)
         so, QL, L, RP, NH = self._lib, self.q_lora, self.LATENT, self.ROPE, self.HEADS
         bf = dict(dtype=torch.bfloat16, device=dev)
@@ -485,17 +498,19 @@ class DsaAttention:
         q = torch.empty(T, NH * self.qh, **bf)
         q_lat = torch.empty(NH * T, L, **bf)
         q8 = torch.empty(T, NH, L + RP, dtype=torch.uint8, device=dev)
-        q_idx = torch.empty(T, self.IDX_HEADS * self.IDX_DIM, **bf)
         idx = torch.empty(T, self.idx_proj.N_pad, **bf)
-        ldl = _round(int(page_table.shape[1]) * self.POOLS_PER_PAGE, 128)
-        ws = self.logits_ws
-        if ws is not None and ws.numel() >= T * ldl:
-            logits = ws[:T * ldl].view(T, ldl)
-        else:
-            logits = torch.empty(T, ldl, dtype=torch.float32, device=dev)
-        ids = torch.empty(T, self.TOPK, dtype=torch.int32, device=dev)
-        tok = torch.empty(T, 4 * self.TOPK + 3 + 5, dtype=torch.int32, device=dev)
-        if self.indexer_fp8:
+        q_idx = logits = ids = tok = None
+        if select:
+            q_idx = torch.empty(T, self.IDX_HEADS * self.IDX_DIM, **bf)
+            ldl = _round(int(page_table.shape[1]) * self.POOLS_PER_PAGE, 128)
+            ws = self.logits_ws
+            if ws is not None and ws.numel() >= T * ldl:
+                logits = ws[:T * ldl].view(T, ldl)
+            else:
+                logits = torch.empty(T, ldl, dtype=torch.float32, device=dev)
+            ids = torch.empty(T, self.TOPK, dtype=torch.int32, device=dev)
+            tok = torch.empty(T, 4 * self.TOPK + 3 + 5, dtype=torch.int32, device=dev)
+        if self.indexer_fp8 and select:
             q8_idx = torch.empty(T, self.IDX_HEADS, self.IDX_DIM, dtype=torch.uint8, device=dev)
             qs_idx = torch.empty(T, self.IDX_HEADS, dtype=torch.float32, device=dev)
         qa_q = self.q_b.quantize(qa, stream)
@@ -504,29 +519,35 @@ class DsaAttention:
         # on the side stream allocates or runs a torch op: its inputs and outputs are made here, on the layer's
         # stream, and live until the join (the top-k's key ranges included)
         main = stream if stream is not None else torch.cuda.current_stream(dev)
-        with torch.cuda.stream(main):
-            ranges = indexer.key_ranges(positions)
+        if select:
+            with torch.cuda.stream(main):
+                ranges = indexer.key_ranges(positions)
         side = self._side_stream()
         fork = torch.cuda.Event()
         fork.record(main)
         side.wait_event(fork)
-        self.wq_idx.gemm(*qa_q, T, q_idx, status, side)
+        if select:
+            self.wq_idx.gemm(*qa_q, T, q_idx, status, side)
         self.idx_proj.gemm(*y_q, T, idx, status, side)
         k_idx, gate = idx[:, :self.IDX_DIM], idx[:, self.IDX_DIM + self.IDX_HEADS:2 * self.IDX_DIM + self.IDX_HEADS]
         w = idx[:, self.IDX_DIM:self.IDX_DIM + self.IDX_HEADS]          # bf16 head weights, read in place
         if self.indexer_fp8:
             # the logits' common factor (softmax scale x heads^-1/2 = 2^-6) is left out: a power of two, it changes
             # neither the top-k set nor its ties
-            indexer.q_quant(q_idx.view(T, self.IDX_HEADS, self.IDX_DIM), q8_idx, qs_idx, side)
+            if select:
+                indexer.q_quant(q_idx.view(T, self.IDX_HEADS, self.IDX_DIM), q8_idx, qs_idx, side)
             indexer.kpool_insert_fp8(k_idx, gate, self.ape, kpool_reqs, max_rows, page_table, pool_cache, tail_ring,
                                      side)
-            indexer.logits_fp8(q8_idx, qs_idx, w, pool_cache, page_table, groups, logits, status, side)
+            if select:
+                indexer.logits_fp8(q8_idx, qs_idx, w, pool_cache, page_table, groups, logits, status, side)
         else:
             indexer.kpool_insert(k_idx, gate, self.ape, kpool_reqs, max_rows, page_table, pool_cache, tail_ring, side)
-            indexer.logits(q_idx.view(T, self.IDX_HEADS, self.IDX_DIM), w, pool_cache, page_table, groups, logits,
-                           status, side)
-        indexer.topk(logits, positions, self.TOPK, ids, side, ranges=ranges)
-        indexer.expand(ids, positions, tok, side)
+            if select:
+                indexer.logits(q_idx.view(T, self.IDX_HEADS, self.IDX_DIM), w, pool_cache, page_table, groups, logits,
+                               status, side)
+        if select:
+            indexer.topk(logits, positions, self.TOPK, ids, side, ranges=ranges)
+            indexer.expand(ids, positions, tok, side)
         join = torch.cuda.Event()
         join.record(side)
         # queries: q_b, rope on each head's rope slice, absorb of each head's nope part into the latent
@@ -537,10 +558,18 @@ class DsaAttention:
         self.w_uk.bmm(q.view(T, NH, self.qh)[:, :, :self.nope].permute(1, 0, 2), q_lat.view(NH, T, L), stream)
         mla.q_pack(q_lat, T, q[:, self.nope:], self.qh, T, q8, self.q_scale, stream)
         main.wait_event(join)
-        # sparse MLA over the selected tokens, then v_up and o_proj
+        # sparse MLA over the selected tokens (or the decode form), then v_up and o_proj
         o_lat = torch.empty(T, NH, L, **bf)
-        mla.sparse_mla(q8, kv_cache, tok, qsl, page_table, self.scale * self.q_scale * self.k_scale, o_lat,
-                       bmm2=self.k_scale, n_idx=4 * self.TOPK + 3, stream=stream, status=status)
+        bmm1 = self.scale * self.q_scale * self.k_scale
+        if form is None:
+            mla.sparse_mla(q8, kv_cache, tok, qsl, page_table, bmm1, o_lat, bmm2=self.k_scale,
+                           n_idx=4 * self.TOPK + 3, stream=stream, status=status)
+        elif select:
+            mla.decode_selected(q8, kv_cache, tok, page_table, bmm1, o_lat, bmm2=self.k_scale,
+                                n_idx=4 * self.TOPK + 3, seq_lens=seq_lens, reqs=reqs, stream=stream, status=status)
+        else:
+            mla.decode(q8, kv_cache, page_table, seq_lens, bmm1, o_lat, bmm2=self.k_scale, reqs=reqs, stream=stream,
+                       status=status)
         # v_up: each head's latent rows read in place from the token-major attention output, written straight into
         # the token-major o_proj input
         o_in = torch.empty(T, NH * self.v_dim, **bf)
@@ -573,9 +602,11 @@ class DsaDecoderLayer:
         self.moe = self.ffn                  # the FFN sub-block (MoELayer or DenseFfn)
         self.device = dev
 
-    def forward(self, res, x_prev, post_prev, comb_prev, meta: dict, caches: tuple, status, stream=None):
+    def forward(self, res, x_prev, post_prev, comb_prev, meta: dict, caches: tuple, status, stream=None,
+                decode: tuple | None = None):
         """meta: positions, slots, qsl, page_table, kpool_reqs, max_rows, groups (device tensors / ints); caches:
-        (latent cache, pool-key cache, tail ring). Returns (res after attention, MoE rows, post, comb)."""
+        (latent cache, pool-key cache, tail ring); decode: `DsaAttention.forward`'s. Returns (res after attention, MoE
+        rows, post, comb)."""
         T, H, dev = res.shape[0], self.H, self.device
         f32 = dict(dtype=torch.float32, device=dev)
         res_a = torch.empty_like(res) if x_prev is not None else res
@@ -584,7 +615,8 @@ class DsaDecoderLayer:
         self.bound_a(x_prev, res, post_prev, comb_prev, res_a if x_prev is not None else None, post_a, comb_a, y,
                      stream, status=status)
         x_a = self.attn.forward(y, meta["positions"], meta["slots"], meta["qsl"], meta["page_table"],
-                                meta["kpool_reqs"], meta["max_rows"], meta["groups"], *caches, status, stream=stream)
+                                meta["kpool_reqs"], meta["max_rows"], meta["groups"], *caches, status, stream=stream,
+                                decode=decode)
         res_b = torch.empty_like(res)
         post_b, comb_b = torch.empty(T, 4, **f32), torch.empty(T, 4, 4, **f32)
         self.bound_b(x_a, res_a, post_a, comb_a, res_b, post_b, comb_b, y, stream, status=status)

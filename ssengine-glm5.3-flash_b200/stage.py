@@ -11,7 +11,9 @@ Mirrors ssengine/model/stage.py:216-762 of the reference and its contract in sse
 - `run(batch, hidden_in)`: stage 0 embeds the token ids; the stage's layers run in order; stages 0..n-2 return
   [T, hidden_width] bf16 on the device, the last stage returns int64 greedy tokens, one per `is_last` chunk in plan
   chunk order; enqueues GPU work only, a fresh output per call;
-- `forward(plan, hidden_in) = run(prepare(plan), hidden_in)`; `tier_ranges()`.
+- `forward(plan, hidden_in) = run(prepare(plan), hidden_in)`; `tier_ranges()`;
+- `decode(plan, hidden_in)`: the same forward for a step of few new tokens a request (one, or a draft of several),
+  through the layers' decode forms: the KDA recurrence token by token, the DSA attention split over the cache.
 
 Layer kinds (`StageConfig.layer_kind`):
 - "hybrid": the Glm5Next split, decoder layers on the 4-stream mHC residual, DSA + MoE at layers 3, 7, ..., KDA + MoE
@@ -428,13 +430,17 @@ class StageModel:
                      v.get("tok"), v["last"], bucket, keep=[host, dev], kda_seqs=v.get("kda"), dsa=dsa,
                      tier_ops=list(getattr(plan, "tier_ops", None) or []))
 
-    def run(self, batch: Batch, hidden_in: torch.Tensor | None, edge_out=None) -> torch.Tensor | None:
+    def run(self, batch: Batch, hidden_in: torch.Tensor | None, edge_out=None,
+            decode: str | None = None) -> torch.Tensor | None:
         """edge_out: a device address, or a callable returning one when called right before the last kernel (the
         next stage's receive slot, a peer pointer), into which a non-last hybrid stage's final boundary kernel stores
         its [T, 4H] rows directly (the fused stage edge); the call then returns None. Without it the rows come back as
-        a fresh tensor (the reference's contract)."""
+        a fresh tensor (the reference's contract). decode: None, or the layers' decode form ("selected" or "dense",
+        `decode` below)."""
+        if decode not in (None, "selected", "dense"):
+            raise ValueError(f"decode form {decode!r}")
         if self.kda:
-            return self._run_kda(batch, hidden_in, edge_out)
+            return self._run_kda(batch, hidden_in, edge_out, decode)
         T, H = batch.num_tokens, self.hidden_width
         s = lib.stream_ptr()
         if self.first:
@@ -451,7 +457,7 @@ class StageModel:
             return x
         return self._head(x, batch.last_rows)
 
-    def _run_kda(self, batch: Batch, hidden_in: torch.Tensor | None, edge_out=None):
+    def _run_kda(self, batch: Batch, hidden_in: torch.Tensor | None, edge_out=None, decode: str | None = None):
         """KDA + MoE decoder layers on the 4-stream residual: stage 0 expands its embeddings (hc_expand), a later stage
         starts from the received residual with a pre-only boundary (edge_recv); a stage that is not the last ends with
         a post-only boundary into the [T, 4H] rows it sends (edge_send, ssengine/model/pp_patch.py:156-163); the last
@@ -469,14 +475,21 @@ class StageModel:
                 raise ValueError(f"stage {self.stage} needs hidden_in bf16 [{T}, {4 * H}]")
             res = hidden_in.view(T, 4, H)
         x_prev = post = comb = None
+        step = None
+        if decode is not None and batch.dsa is not None:
+            # each row's request and the tokens that it sees, once for the stage's DSA layers
+            rows = torch.arange(T, dtype=torch.int32, device=self.device)
+            reqs = torch.searchsorted(batch.dsa["qsl"], rows, right=True, out_int32=True) - 1
+            step = (decode, reqs, (batch.dsa["positions"] + 1).to(torch.int32))
         for layer in self.layers:
             layer.moe_profile = self.moe_profile
         for layer, state, dsa, grp in zip(self.layers, self.kda_states, self.is_dsa, self.kda_group):
             if dsa:
-                res, x_prev, post, comb = layer.forward(res, x_prev, post, comb, batch.dsa, state, self.status)
+                res, x_prev, post, comb = layer.forward(res, x_prev, post, comb, batch.dsa, state, self.status,
+                                                        decode=step)
             else:
                 res, x_prev, post, comb = layer.forward(res, x_prev, post, comb, batch.kda_seqs[grp], *state,
-                                                        self.status)
+                                                        self.status, decode=decode is not None)
             if self.layer_hook is not None:
                 self.layer_hook(layer, res, x_prev, post, comb)
         if edge_out is not None and not self.last and x_prev is not None:
@@ -506,6 +519,14 @@ class StageModel:
 
     def forward(self, plan, hidden_in: torch.Tensor | None = None) -> torch.Tensor:
         return self.run(self.prepare(plan), hidden_in)
+
+    def decode(self, plan, hidden_in: torch.Tensor | None = None, attention: str = "selected") -> torch.Tensor:
+        """One step of new tokens: a plan whose chunks continue their requests by one token (or a draft of several,
+        each seeing those before it), with the pages and states that `forward` left, -> what `forward` returns, through
+        `KdaLayer.decode` in the KDA layers and in the DSA layers `mla.decode_selected` over the indexer's tokens
+        (attention "selected") or `mla.decode` over the whole context ("dense", the indexer's pool keys kept up to
+        date). Chunks of any length are right; the chunked forms of `forward` are faster for long ones."""
+        return self.run(self.prepare(plan), hidden_in, decode=attention)
 
     def tier_ranges(self) -> list:
         """Byte ranges (device pointer, bytes) of the stage's KV and state tensors for the capacity tiers: every

@@ -145,3 +145,13 @@ def test_c_kda_refuses(over, rc):
     L = lib.KdaLayerC(2, a["dim"], a["w"], 1 << 12, 1 << 12, -5.0, 128 ** -0.5, a["conv"], a["cs"], a["rec"], a["rs"])
     assert lib.load().ssb_kda_decode(ctypes.byref(L), a["x"], a["ldx"], a["g"], a["ldg"], a["beta"], a["ldb"], a["T"],
                                      a["seqs"], a["R"], a["out"], a["ldo"], None, None) == rc
+
+
+def test_stage_and_block_refuse_unknown_forms():
+    from ssengine_b200.layers import DsaAttention
+    from ssengine_b200.stage import StageModel
+
+    with pytest.raises(ValueError):
+        object.__new__(StageModel).run(None, None, decode="sparse")
+    with pytest.raises(ValueError):
+        DsaAttention.forward(object.__new__(DsaAttention), *[None] * 12, decode=("sparse", None, None))
