@@ -35,14 +35,14 @@
 namespace ssb {
 namespace {
 
-constexpr int kDq = 576, kDv = 512, kUnit = 128, kTileH = 64;
+constexpr int kDq = 576, kDv = 512, kPage = 128, kUnit = 64, kTileH = 64;
 constexpr int kMaxCtas = 148;                   // ranges a call is cut into at most (the workspace is sized by it)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kNone = -INFINITY;
 
-constexpr int kSoftWarps = 16;                  // warps 0-15: token quarter warp & 3, heads 16 (warp >> 2) .. + 15
-constexpr int kSoftmax = 32 * kSoftWarps;
-constexpr int kGroup = 128;                     // threads of one group of 16 heads
+constexpr int kSoftWarps = 16;                  // warps 0-15: TMEM lanes 32 (warp & 3) .. (16 heads), tokens 32 (warp >> 2 & 1)
+constexpr int kSoftmax = 32 * kSoftWarps;       // .. + 31 of every second unit, those of parity warp >> 3 (a set)
+constexpr int kSetWarps = 8;
 constexpr int kScoreWarp = kSoftWarps;          // warp 16 issues the score products
 constexpr int kValueWarp = kScoreWarp + 1;      // warp 17 the value products
 constexpr int kGatherWarp = kValueWarp + 1;     // warps 18-21 bring the cache rows
@@ -50,35 +50,38 @@ constexpr int kGatherWarps = 4;
 constexpr int kThreads = 32 * (kGatherWarp + kGatherWarps);
 
 // ---- shared memory ------------------------------------------------------------------------------------------------
-constexpr int kChunk = 16384;                   // [128 rows x 128 B], 128-byte swizzle
-constexpr int kRope = 8192;                     // [128 rows x 64 B], 64-byte swizzle
+constexpr int kSlots = 6;                       // units in shared memory
+constexpr int kChunk = 8192;                    // [64 rows x 128 B], 128-byte swizzle
+constexpr int kRope = 4096;                     // [64 rows x 64 B], 64-byte swizzle
 constexpr int kLat = 4 * kChunk;                // a unit's latent rows
-constexpr int kOffQ = 0;                        // the query tile's parts: 4 chunks and the rope
-constexpr int kOffKv = kLat + kRope;            // the latent rows of two units
-constexpr int kOffRope = kOffKv + 2 * kLat;     // their rope keys; once its scores are done, a unit's high parts of P
-constexpr int kOffPlo = kOffRope + 2 * kRope;   // the low parts of P
-constexpr int kOffSf = kOffPlo + kRope;         // block scales of P, two units: byte (h % 32) 16 + unit 8 + (h / 32) 4 + quarter
+constexpr int kOffKv = 0;                       // the latent rows of the units
+constexpr int kOffRope = kSlots * kLat;         // their rope keys; once its scores are done, a unit's high parts of P
+constexpr int kOffPlo = kOffRope + kSlots * kRope;    // the low parts of P, two units
+constexpr int kOffSf = kOffPlo + 2 * kRope;     // block scales of P, two units: byte (h % 32) 16 + unit 8 + (h / 32) 4 + half
 constexpr int kOffBar = kOffSf + 512;           // mbarriers
-constexpr int kOffMisc = kOffBar + 256;         // tmem address, abort flag, last-unit flags, plan
-constexpr int kOffRise = kOffMisc + 64;         // int32 [2][4]: a unit with scores far above a group's references
-constexpr int kOffMask = kOffRise + 32;         // uint32 [2][4]: tokens present in a unit
-constexpr int kOffScale = kOffMask + 32;        // float [2][64]: base-2 score scale, minus the reference of each head
-constexpr int kOffExp = kOffScale + 512;        // float [4][64]: maxima of the token quarters, or their sums
-constexpr int kOffSum = kOffExp + 1024;         // float [64]: rescale factors, bmm2 / l
+constexpr int kOffMisc = kOffBar + 256;         // tmem address, abort flag, a set's unit with scores far above its references
+constexpr int kOffSlot = kOffMisc + 16;         // int4 [6] (8 places): of a slot's unit the tokens present (2 words), last of its row
+constexpr int kOffRing = kOffSlot + 128;        // int4 [8]: the same by unit, as the softmax and the values read it
+constexpr int kOffK = kOffRing + 128;           // int32 [64]: the query scale's exponent of each head
+constexpr int kOffRef = kOffK + 256;            // float [64]: the heads' references
+constexpr int kOffRow = kOffRef + 256;          // float [4][64]: maxima and rescale factors, or the sums
+constexpr int kOffSum = kOffRow + 1024;         // float [64]: bmm2 / l
 constexpr int kOffPlan = kOffSum + 256;         // int32 [52]: the plan's sums and first row
 constexpr int kSmem = kOffPlan + 208;
-static_assert(kOffScale % 16 == 0 && kOffExp % 16 == 0 && kOffSf % 128 == 0 && kSmem <= 232448, "shared memory");
-// TMEM columns: O^T as 4 tiles of 128 dims x 64 heads, S^T 128 tokens x (64 high | 64 low), block scales of V (2^-7 against
-// the high parts of P, 2^-11 against the low ones) and of P (2 columns a unit)
-constexpr uint32_t kColO = 0, kColS = 256, kColV = 384, kColLow = 388, kColP = 392;
-constexpr float kMaxRise = 4.0f;                // base-2 scores above a head's reference before it moves and O is rescaled
-constexpr float kNoHead = -1000.0f;             // base-2 score of the heads that the tile does not have: weight 0
+static_assert(kOffSlot % 16 == 0 && kOffRow % 16 == 0 && kOffSf % 128 == 0 && kSmem <= 232448, "shared memory");
+// TMEM columns: O^T as 4 tiles of 128 dims x 64 heads; S, 64 tokens; the query parts, 576 bytes a lane; block scales of V
+// (2^-7 against the high parts of P, 2^-11 against the low ones) and of P (2 columns a unit). Lanes 32 i + l of S and the
+// query parts: the high part of head 16 i + l, l < 16, the low part of head 16 i + l - 16 above
+constexpr uint32_t kColO = 0, kColS = 256, kColQ = 320, kColV = 464, kColLow = 468, kColP = 472;
+constexpr float kMaxRise = 64.0f;               // base-2 scores above a head's reference before it moves and O is rescaled
+constexpr float kMinE = -100.0f;                // the least exponent of a block
+enum : int32_t { kMore = 0, kLast = 1, kEnd = 2 };     // a unit, the last unit of its row, no unit: the row has ended
 constexpr uint32_t kSw128 = 2, kSw64 = 4;       // descriptor layout types
 
-// Block-scaled instruction descriptor (kind::mxf8f6f4): e4m3 A and B (format 0), ue8m0 scales (bit 23), A and B
-// MN-major (bits 15, 16), N >> 3 in [17,23), M >> 4 in [24,29), B's scale byte in [4,6).
+// Block-scaled instruction descriptor (kind::mxf8f6f4): e4m3 A and B (format 0), ue8m0 scales (bit 23), A
+// MN-major (bit 15), B K-major, N >> 3 in [17,23), M >> 4 in [24,29), B's scale byte in [4,6).
 __host__ __device__ constexpr uint32_t idesc_mx(int M, int N) {
-  return (1u << 15) | (1u << 16) | (static_cast<uint32_t>(N >> 3) << 17) | (1u << 23) |
+  return (1u << 15) | (static_cast<uint32_t>(N >> 3) << 17) | (1u << 23) |
          (static_cast<uint32_t>(M >> 4) << 24);
 }
 // D[tmem] (+)= A B, e4m3 operands with ue8m0 scales for blocks of 32 along the reduction.
@@ -102,6 +105,15 @@ SSB_DEVICE void tmem_ld_x16(uint32_t taddr, float (&v)[16]) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
+// D[tmem] (+)= A B with e4m3 A in TMEM (a row a lane, 4 values a column) and B in shared memory.
+SSB_DEVICE void tc_mma_f8_ta(uint32_t d, uint32_t a, uint64_t bd, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(bd), "r"(idesc), "r"(acc)
+      : "memory");
+}
 SSB_DEVICE void tmem_ld_x4(uint32_t taddr, float (&v)[4]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
                : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
@@ -117,6 +129,11 @@ SSB_DEVICE void tmem_st_x16(uint32_t taddr, const float (&v)[16]) {
 }
 SSB_DEVICE void tmem_st_x4(uint32_t taddr, uint32_t v) {               // one word in 4 columns
   asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %1, %1, %1};" ::"r"(taddr), "r"(v) : "memory");
+}
+SSB_DEVICE void tmem_st_4(uint32_t taddr, const uint32_t (&v)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3])
+               : "memory");
 }
 SSB_DEVICE bool elect_lane() {                   // true in one lane of a converged warp
   uint32_t p;
@@ -136,21 +153,6 @@ SSB_DEVICE void cp_async_arrive_noinc(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 SSB_DEVICE void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-// Sums over the 32 lanes of 16 values a lane, transposed: lane l receives the total of value l & 15.
-SSB_DEVICE float warp_sum_transposed(float (&v)[16], int lane) {
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 16);
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) {
-    const bool up = lane & o;
-#pragma unroll
-    for (int i = 0; i < o; ++i) {
-      const float keep = up ? v[i + o] : v[i], send = up ? v[i] : v[i + o];
-      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-    }
-  }
-  return v[0];
-}
 // Transposes 4 x 4 values over 4 neighbouring lanes: v[i] of lane l becomes v[l] of lane i (of the four).
 SSB_DEVICE void cross4(float (&v)[4], int lane) {
 #pragma unroll
@@ -163,12 +165,6 @@ SSB_DEVICE void cross4(float (&v)[4], int lane) {
       if (up) v[i] = got; else v[i + o] = got;
     }
   }
-}
-// Largest of the 32 lanes' values, NaN ignored (all NaN: NaN).
-SSB_DEVICE float warp_max(float v) {
-  float r;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-  return r;
 }
 SSB_DEVICE float ex2_fast(float x) {
   float y;
@@ -201,13 +197,9 @@ SSB_DEVICE void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
 // Byte offset of 16-byte granule g of row r: a 128-byte-swizzled chunk, a 64-byte-swizzled one.
 SSB_DEVICE uint32_t sw128(int r, int g) { return r * 128 + ((g ^ (r & 7)) << 4); }
 SSB_DEVICE uint32_t sw64(int r, int g) { return r * 64 + ((g ^ ((r >> 1) & 3)) << 4); }
-// Granule g (0-35) of row r of 576 bytes.
-SSB_DEVICE uint32_t row_off(int r, int g) { return g < 32 ? (g >> 3) * kChunk + sw128(r, g & 7) : kLat + sw64(r, g - 32); }
-
 // ---- barriers -----------------------------------------------------------------------------------------------------
-struct Bars {                                    // lat_*: 2 buffers x 4 chunks (the rope keys with the last); agree: one a
-                                                 // group of heads
-  uint32_t lat_full, lat_empty, q_full, s_full, s_empty, p_full, pv_done, o_full, drain, agree;
+struct Bars {                                    // slots: full, empty; sets: s_full, p_full, pv_done, agree, ref_ok, slow
+  uint32_t full, empty, q_full, s_full, s_empty, p_full, pv_done, o_full, o_free, drain, agree, ref_ok, slow;
 };
 // mbar_wait whose second and later tries are out of line: the many waits stay short in the instruction cache.
 __device__ __noinline__ bool mbar_wait_more(uint32_t bar, uint32_t parity, volatile int32_t* abort_flag,
@@ -243,7 +235,7 @@ SSB_DEVICE int row_units(const MlaDecodeArgs& a, int t) {
   if (a.seq_lens != nullptr) n = min(n, a.seq_lens[t]);
   if (a.reqs != nullptr && static_cast<uint32_t>(a.reqs[t]) >= static_cast<uint32_t>(a.R)) n = 0;
   n = n > 0 ? (n + kUnit - 1) / kUnit : 0;
-  return a.indices != nullptr ? n : min(n, a.width);
+  return a.indices != nullptr ? n : min(n, kPage / kUnit * a.width);
 }
 
 // A CTA's share of one row: units [b0, b1) of the row's nb planned ones; every role walks the same segments.
@@ -251,7 +243,7 @@ struct Segment {
   int t, b0, b1, nb;
 };
 // Ranges are cut in units plus `cost` for every row that has any (a row's staging, drain and epilogue take a CTA about as
-// long as two units; none where a range is a few units and every cut row would lose more).
+// long as four units; none where a range is a few units and every cut row would lose more).
 struct Walk {
   int t, nb, first, lo, hi, cost;               // next row, its units, the units and costs before it, the range, the cost
 };
@@ -270,7 +262,7 @@ __device__ __noinline__ bool walk_next(const MlaDecodeArgs& a, Walk& w, Segment&
   }
   return found;
 }
-constexpr int kRowCost = 2, kCostFrom = 6;      // units; ranges of so many units or more bear it
+constexpr int kRowCost = 4, kCostFrom = 12;      // units; ranges of so many units or more bear it
 
 // All threads of the CTA: its range and the row that holds its beginning. sh: 48 words for the warps' sums, 4 for the row.
 // False: more CTAs than units, nothing to do here.
@@ -340,83 +332,67 @@ SSB_DEVICE float2* part_ml(const MlaDecodeArgs& a, int tile, int slot) {
 
 // ---- the two products ---------------------------------------------------------------------------------------------
 // By a whole warp of which one lane issues: the addresses are the same in every lane, so they stay in uniform registers.
-template <bool Q8>
-SSB_DEVICE bool issue_scores(const Bars& B, uint32_t sbase, int buf, uint32_t parity, bool leader,
-                             volatile int32_t* abort_flag, int32_t* status) {
-  constexpr uint32_t idesc = idesc_e4m3(128, Q8 ? 64 : 128);         // S^T [tokens, heads] = K Q^T
-  uint64_t ad = smem_desc(sbase + kOffKv + buf * kLat, 0, 1024, kSw128), bd = smem_desc(sbase + kOffQ, 0, 1024, kSw128);
-  uint32_t acc = 0;
+SSB_DEVICE void issue_scores(const Bars& B, uint32_t sbase, int slot, int set, bool leader) {
+  constexpr uint32_t idesc = idesc_e4m3(128, kUnit);                 // S [query parts, tokens] = Q K^T
+  uint64_t bd = smem_desc(sbase + kOffKv + slot * kLat, 0, 1024, kSw128);
+  uint32_t q = kColQ, acc = 0;
 #pragma unroll 1
   for (int c = 0; c < 4; ++c) {
-    if (!mbar_nap(B.lat_full + 32 * buf + 8 * c, parity, abort_flag, status)) return false;
-    fence_proxy_async_smem();                                        // rows that threads copied -> the tensor core
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-      if (leader) tc_mma_f8(kColS, ad + 2 * ks, bd + 2 * ks, idesc, acc);
+      if (leader) tc_mma_f8_ta(kColS, q + 8 * ks, bd + 2 * ks, idesc, acc);
       acc = 1;
     }
-    ad += kChunk >> 4;
+    q += 32;
     bd += kChunk >> 4;
   }
-  ad = smem_desc(sbase + kOffRope + buf * kRope, 0, 512, kSw64);
-  bd = smem_desc(sbase + kOffQ + kLat, 0, 512, kSw64);
+  bd = smem_desc(sbase + kOffRope + slot * kRope, 0, 512, kSw64);
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks)                                     // the rope keys: 64 bytes a row
-    if (leader) tc_mma_f8(kColS, ad + 2 * ks, bd + 2 * ks, idesc, 1u);
-  if (leader) tc_commit(B.s_full);
-  return true;
+    if (leader) tc_mma_f8_ta(kColS, q + 8 * ks, bd + 2 * ks, idesc, 1u);
+  if (leader) tc_commit(B.s_full + 8 * set);
 }
-SSB_DEVICE void issue_values(const Bars& B, uint32_t sbase, int buf, bool fresh, bool leader) {
-  uint64_t ad = smem_desc(sbase + kOffKv + buf * kLat, kChunk, 1024, kSw128);     // O^T [dims, heads] (+)= V^T P^T
-  const uint64_t hi0 = smem_desc(sbase + kOffRope + buf * kRope, kRope, 512, kSw64), lo0 = smem_desc(sbase + kOffPlo, kRope, 512, kSw64);
-  uint32_t o = kColO, empty = B.lat_empty + 32 * buf;
-  const uint32_t sfp = kColP + 2 * buf;
+SSB_DEVICE void issue_values(const Bars& B, uint32_t sbase, int slot, int set, bool fresh, bool leader) {
+  uint64_t ad = smem_desc(sbase + kOffKv + slot * kLat, kChunk, 1024, kSw128);    // O^T [dims, heads] (+)= V^T P^T
+  const uint64_t hi0 = smem_desc(sbase + kOffRope + slot * kRope, 0, 512, kSw64);
+  const uint64_t lo0 = smem_desc(sbase + kOffPlo + set * kRope, 0, 512, kSw64);
+  uint32_t o = kColO;
+  const uint32_t sfp = kColP + 2 * set;
   if (leader) tc_cp_sf(kColP, smem_desc(sbase + kOffSf, 0, 128, 0));
 #pragma unroll 1
   for (int d = 0; d < 4; ++d) {                                      // 128 dims
-    uint64_t v = ad, hi = hi0, lo = lo0;
-    uint32_t id = idesc_mx(128, 64), acc = fresh ? 0u : 1u;
-#pragma unroll 1
-    for (int ks = 0; ks < 4; ++ks) {                                 // 32 tokens a step: one block of scales
+    uint32_t acc = fresh ? 0u : 1u;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {                                 // 32 tokens a step: one block of scales
+      const uint32_t id = idesc_mx(128, 64) | (ks << 4);
       if (leader) {
-        tc_mma_mx(o, v, hi, id, acc, kColV, sfp);
-        tc_mma_mx(o, v, lo, id, 1u, kColLow, sfp);
+        tc_mma_mx(o, ad + ks * (4096 >> 4), hi0 + 2 * ks, id, acc, kColV, sfp);
+        tc_mma_mx(o, ad + ks * (4096 >> 4), lo0 + 2 * ks, id, 1u, kColLow, sfp);
       }
-      v += 4096 >> 4;
-      hi += 2048 >> 4;
-      lo += 2048 >> 4;
-      id += 1u << 4;
       acc = 1;
     }
-    if (leader) tc_commit(empty);                                    // the chunk is free for the unit after the next
     ad += kChunk >> 4;
     o += 64;
-    empty += 8;
   }
-  if (leader) tc_commit(B.pv_done);
+  if (leader) {
+    tc_commit(B.empty + 8 * slot);
+    tc_commit(B.pv_done + 8 * set);
+  }
 }
 
-// One query row's heads h0 .. h0 + 63 into the query tile: rows 0-63 the high parts, 64-127 the low parts of
-// q 2^-k (k per head, its largest value in [2^7, 2^8)), zero rows past nh. bf16 has 8 significant bits, so the two e4m3
-// parts hold a value exactly unless it is below 2^-14 of the head's largest. Also each head's score scale (its reference
-// cleared). 8 threads a head, 9 granules each (twice: for the largest value, then from the L1 cache for the parts).
+// One query row's heads h0 .. h0 + 63 as the parts of q 2^-k (k per head, its largest value in [2^7, 2^8)) into TMEM, zero
+// rows past nh. bf16 has 8 significant bits, so the two e4m3 parts hold a value exactly unless it is below 2^-14 of the
+// head's largest. First the exponents, 8 threads a head; then a thread has one part of its head's lane and a quarter of
+// the row, which the first pass left in the L1 cache. e4m3 queries have no low part.
 template <bool Q8>
-__device__ __noinline__ void stage_q(const MlaDecodeArgs& a, uint8_t* smem, int t, int h0, int nh) {
-  uint8_t* Q = smem + kOffQ;
-  float* scale = reinterpret_cast<float*>(smem + kOffScale);
-  const int h = threadIdx.x >> 3, sub = threadIdx.x & 7;
-  const bool have = h < nh;
-  const int64_t off = (int64_t)t * a.ldq + (int64_t)(h0 + min(h, nh - 1)) * a.hsq;
-  int k = 0;
-  if (Q8) {
-    const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.q) + off);
-#pragma unroll
-    for (int j = 0; j < 5; ++j) {                                     // 36 granules of 16 values
-      const int g = sub + 8 * j;
-      if (g < 36) *reinterpret_cast<uint4*>(Q + row_off(h, g)) = have ? __ldg(q + g) : make_uint4(0, 0, 0, 0);
-    }
-  } else {
-    const uint4* q = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + off);
+__device__ __noinline__ void stage_q(const MlaDecodeArgs& a, uint8_t* smem, uint32_t tmem, int t, int h0, int nh) {
+  int32_t* exps = reinterpret_cast<int32_t*>(smem + kOffK);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)t * a.ldq;
+  if (!Q8) {
+    const int h = threadIdx.x >> 3, sub = threadIdx.x & 7;
+    const uint4* q =
+        reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + row + (int64_t)(h0 + min(h, nh - 1)) * a.hsq);
     uint4 v[9];
 #pragma unroll
     for (int j = 0; j < 9; ++j) v[j] = __ldg(q + sub + 8 * j);        // 72 granules of 8 values
@@ -432,34 +408,39 @@ __device__ __noinline__ void stage_q(const MlaDecodeArgs& a, uint8_t* smem, int 
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
     const int ex = static_cast<int>(top >> 7);                        // the largest value's biased exponent
-    if (ex != 0) k = max(min(ex - 134, 120), -120);
     // an infinite or NaN query value leaves its head no finite score: NaN, which e4m3 can carry (it has no infinity)
-    const float down = !have ? 0.0f : ex == 255 ? NAN : __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
-    // granule j of 8 values: half of 16-byte granule 4 j + (sub >> 1) of the row, in chunk j >> 1; the last in the rope
-    uint8_t* even = Q + sw128(h, sub >> 1) + 8 * (sub & 1);
-    uint8_t* odd = Q + sw128(h, 4 + (sub >> 1)) + 8 * (sub & 1);
+    if (sub == 0) exps[h] = ex == 255 ? 255 : ex != 0 ? max(min(ex - 134, 120), -120) : 0;
+    named_bar(5, kSoftmax);
+  }
+  const int h = 16 * (warp & 3) + (lane & 15), part = warp >> 2;      // 144 values
+  const bool high = lane < 16, have = h < nh;
+  const int64_t off = row + (int64_t)(h0 + min(h, nh - 1)) * a.hsq + 144 * part;
+  uint32_t to = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + kColQ + 36 * part;
+  const int k = Q8 ? 0 : exps[h];
+  const float down = !have ? 0.0f : k == 255 ? NAN : __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
 #pragma unroll 1
-    for (int j = 0; j < 9; ++j) {
-      const uint4 w4 = __ldg(q + sub + 8 * j);
-      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-      uint32_t hi[4], lo[4];
+  for (int j = 0; j < 9; ++j, to += 4) {                              // 16 values
+    uint32_t w[4];
+    if (Q8) {
+      const uint4 g = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.q) + off) + j);
+      const bool keep = have && high;
+      w[0] = keep ? g.x : 0, w[1] = keep ? g.y : 0, w[2] = keep ? g.z : 0, w[3] = keep ? g.w : 0;
+    } else {
+      const uint4* q = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + off) + 2 * j;
+      const uint4 g0 = __ldg(q), g1 = __ldg(q + 1);
+      const uint32_t v[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        split2(__uint_as_float(w[e] << 16) * down, __uint_as_float(w[e] & 0xFFFF0000u) * down, hi[e], lo[e]);
-      uint8_t* at = even;
-      if (j == 8) at = Q + kLat + sw64(h, sub >> 1) + 8 * (sub & 1);
-      *reinterpret_cast<uint2*>(at) = make_uint2(hi[0] | (hi[1] << 16), hi[2] | (hi[3] << 16));
-      at += j < 8 ? 64 * 128 : 64 * 64;                               // 64 rows further on, where the swizzle repeats
-      *reinterpret_cast<uint2*>(at) = make_uint2(lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16));
-      at = even + kChunk;
-      even = odd;
-      odd = at;
+      for (int e = 0; e < 4; ++e) {
+        uint32_t hi[2], lo[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          split2(__uint_as_float(v[2 * e + i] << 16) * down, __uint_as_float(v[2 * e + i] & 0xFFFF0000u) * down, hi[i], lo[i]);
+        w[e] = high ? hi[0] | (hi[1] << 16) : lo[0] | (lo[1] << 16);
+      }
     }
+    tmem_st_4(to, w);
   }
-  if (sub == 0) {
-    scale[h] = have ? a.bmm1 * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + k) << 23) : 0.0f;
-    scale[64 + h] = have ? 0.0f : kNoHead;
-  }
+  tmem_st_wait();
 }
 
 template <bool Q8>
@@ -471,12 +452,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int cta = blockIdx.x, tile = blockIdx.y;
   const int h0 = tile * kTileH, nh = min(kTileH, a.H - h0);
   const uint32_t sbase = smem_u32(smem), bar = sbase + kOffBar;
-  const Bars B = {bar,       bar + 64,  bar + 128, bar + 136, bar + 144, bar + 152,
-                  bar + 160, bar + 168, bar + 176, bar + 184};
+  const Bars B = {bar,       bar + 48,  bar + 96,  bar + 104, bar + 120, bar + 128, bar + 144,
+                  bar + 160, bar + 168, bar + 176, bar + 184, bar + 200, bar + 216};
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kOffMisc);
   volatile int32_t* abort_flag = reinterpret_cast<volatile int32_t*>(smem + kOffMisc + 4);
-  volatile int32_t* last_unit = reinterpret_cast<volatile int32_t*>(smem + kOffMisc + 8);     // [2]
-  volatile uint32_t* mask = reinterpret_cast<volatile uint32_t*>(smem + kOffMask);
+  volatile int32_t* far = reinterpret_cast<volatile int32_t*>(smem + kOffMisc + 8);           // [2]
+  int4* slots = reinterpret_cast<int4*>(smem + kOffSlot);
+  int4* ring = reinterpret_cast<int4*>(smem + kOffRing);
   if (sbase & 1023) {                                    // the swizzled tiles need it; no static shared memory precedes
     if (tid == 0) raise_status(a.status, kErrCuda);
     return;
@@ -484,20 +466,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   asm volatile("griddepcontrol.launch_dependents;");     // the join may be set up meanwhile (it waits for this grid's end)
   if (warp == kScoreWarp) {
-    if (lane < 24) {                                     // the barriers, one a lane
-      const int i = lane;
-      // lat_full: every gather lane's copies, for the last chunk also an arrival a warp for its mask word
-      const uint32_t n = i < 8 ? 128 + ((i & 3) == 3 ? kGatherWarps : 0) : i < 16 ? 1
-                         : i == 16 || i == 18 || i == 19 ? kSoftWarps : i < 22 ? 1 : i == 22 ? 2 : 4;
-      mbar_init(bar + 8 * i, n);
-      if (i == 23) {
-        mbar_init(bar + 8 * 24, 4);
-        mbar_init(bar + 8 * 25, 4);
-        mbar_init(bar + 8 * 26, 4);
-      }
+    if (lane < 29) {                                     // the barriers, one a lane
+      // full: every gather lane's copies and a warp's word
+      const uint32_t n = lane < 6 ? 132 : lane < 12 ? 1 : lane == 12 || lane == 21 ? kSoftWarps : lane < 15 ? 2
+                         : lane < 18 ? kSetWarps : lane < 21 ? 1 : lane == 22 ? 2 : kSetWarps;
+      mbar_init(bar + 8 * lane, n);
     }
-    if (lane < 8) reinterpret_cast<int32_t*>(smem + kOffRise)[lane] = 0;
-    if (lane == 8) *abort_flag = 0;
+    if (lane < 2) far[lane] = 0;
+    if (lane == 2) *abort_flag = 0;
     fence_barrier_init();
   } else if (warp == kValueWarp) {
     tmem_alloc(smem_u32(tmem_slot), 512);
@@ -520,10 +496,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 
   if (warp >= kGatherWarp) {
-    // ---------------------------------------------------------------- gather: warp w brings tokens 32 w .. 32 w + 31, or
-    const int w = warp - kGatherWarp;                    // of a whole page the latent chunk w (warp 3 also the rope keys)
+    // ---------------------------------------------------------------- gather: warp w brings of a whole unit the latent
+    // chunk w (warp 3 also the rope keys); otherwise of tokens 32 (w & 1) .. + 31 the chunks 2 (w >> 1), + 1 and half the rope
+    const int w = warp - kGatherWarp, half = w & 1, pair = w >> 1;
     const int cols = a.indices != nullptr ? (a.n_idx + kUnit - 1) / kUnit : 0;
-    int u = 0;
+    int slot = 0, round = 0;                             // unit u's slot u % 6, and u / 6
     Segment s;
     bool ok = true;
     while (ok && walk_next(a, walk, s)) {
@@ -541,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int c = c0; c < c1; ++c) {
             bool any = false;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < kUnit / 32; ++j) {
               const int col = c * kUnit + 32 * j + lane;
               const int pos = col < a.n_idx ? idx[col] : -1;
               any |= pos >= 0 && pos < len;
@@ -552,9 +529,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       // first cache row of the page of position p (-1: none)
-      auto page_row = [&](int p) -> int64_t { return p / kUnit < a.width ? (int64_t)pages[p / kUnit] * kUnit : -1; };
+      auto page_row = [&](int p) -> int64_t { return p / kPage < a.width ? (int64_t)pages[p / kPage] * kPage : -1; };
       auto token = [&](int c) {                          // position of this lane's token of unit c (-1: none)
-        int p = c * kUnit + 32 * w + lane;
+        int p = c * kUnit + 32 * half + lane;
         if (idx != nullptr) p = p < a.n_idx ? idx[p] : -1;
         return p < len ? p : -1;
       };
@@ -566,68 +543,59 @@ __global__ void __launch_bounds__(kThreads, 1)
       int p = token(c);
       int64_t page = p >= 0 ? page_row(p) : -1;
       while (c < c1) {
-        const int buf = u & 1, cn = next_live(c + 1);
+        const int cn = next_live(c + 1);
         int pn = -1;
         int64_t page_n = -1;
         if (cn < c1) {
           pn = token(cn);
           page_n = pn >= 0 ? page_row(pn) : -1;
         }
-        const uint32_t full = B.lat_full + 32 * buf, empty = B.lat_empty + 32 * buf, parity = ((u >> 1) - 1) & 1;
-        const uint32_t dst = sbase + kOffKv + buf * kLat;
-        const int64_t row = page + (p & (kUnit - 1));
-        const int slot = p >= 0 && page >= 0 && row < a.cache_rows ? static_cast<int>(row) : -1;
-        const uint32_t present = __ballot_sync(0xffffffffu, slot >= 0);
-        // A chunk is free when the values of the unit two before have used it; by then that unit's scores are done and its
-        // mask word and flag are read, so a warp may also arrive on the other chunks' barriers for this unit.
-        // A whole page (the same in every lane and warp) comes as tiles; a row's last page, and selected tokens, row by
-        // row: rows that are not there have to be zeros (whatever the cache holds there, NaN too, would meet weight 0 in
-        // the value product).
-        if (idx == nullptr && (c + 1) * kUnit <= len && page >= 0 && page + kUnit <= a.cache_rows) {
-          const int y = static_cast<int>(page);
+        const uint32_t full = B.full + 8 * slot;
+        const uint32_t dst = sbase + kOffKv + slot * kLat, rope = sbase + kOffRope + slot * kRope;
+        const int64_t row = page + (p & (kPage - 1));
+        const int from = p >= 0 && page >= 0 && row < a.cache_rows ? static_cast<int>(row) : -1;
+        const uint32_t present = __ballot_sync(0xffffffffu, from >= 0);
+        // the slot is free when the values of the unit six before have used it (its words were read before its scores)
+        if (round > 0) ok = mbar_nap(B.empty + 8 * slot, (round - 1) & 1, abort_flag, a.status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        // A whole unit of a page (the same in every lane and warp) comes as tiles; a row's last units, and selected tokens,
+        // row by row: rows that are not there have to be zeros (whatever the cache holds there, NaN too, would meet weight 0
+        // in the value product).
+        const int64_t y = page + ((c * kUnit) & (kPage - 1));
+        const bool whole = idx == nullptr && (c + 1) * kUnit <= len && page >= 0 && y + kUnit <= a.cache_rows;
+        if (whole) {
           if (lane == 0) {
-            if (u >= 2) ok = mbar_nap(empty + 8 * w, parity, abort_flag, a.status);
-            if (ok) {
-              mbar_arrive_expect_tx(full + 8 * w, w == 3 ? kChunk + kRope : kChunk);
-              tma_load_2d(dst + w * kChunk, &mlat, 128 * w, y, full + 8 * w);
-              if (w == 3) tma_load_2d(sbase + kOffRope + buf * kRope, &mrope, kDv, y, full + 24);
-#pragma unroll 1
-              for (int j = 0; j < 4; ++j) mbar_arrive_n(full + 8 * j, j == w ? 31 : 32);
-            }
+            mbar_arrive_expect_tx(full, w == 3 ? kChunk + kRope : kChunk);
+            tma_load_2d(dst + w * kChunk, &mlat, 128 * w, static_cast<int>(y), full);
+            if (w == 3) tma_load_2d(rope, &mrope, kDv, static_cast<int>(y), full);
           }
         } else {
           int sl[8];
 #pragma unroll
-          for (int r = 0; r < 8; ++r) sl[r] = __shfl_sync(0xffffffffu, slot, 4 * r + (lane >> 3));
+          for (int r = 0; r < 8; ++r) sl[r] = __shfl_sync(0xffffffffu, from, 4 * r + (lane >> 3));
 #pragma unroll 1
-          for (int j = 0; j < 4 && ok; ++j) {
-            if (u >= 2) ok = mbar_nap(empty + 8 * j, parity, abort_flag, a.status);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
+          for (int j = 2 * pair; j < 2 * pair + 2; ++j) {
             const uint8_t* src = a.kv + 128 * j + 16 * (lane & 7);
 #pragma unroll
             for (int r = 0; r < 8; ++r)                  // 4 tokens a warp instruction: 128 of their latent bytes
-              cp_async16(dst + j * kChunk + sw128(32 * w + 4 * r + (lane >> 3), lane & 7),
+              cp_async16(dst + j * kChunk + sw128(32 * half + 4 * r + (lane >> 3), lane & 7),
                          src + (int64_t)max(sl[r], 0) * kDq, sl[r] >= 0);
-            if (j == 3) {
-#pragma unroll
-              for (int r = 0; r < 32; r += 8) {          // 8 tokens a warp instruction: their 64 rope bytes
-                const int rs = __shfl_sync(0xffffffffu, slot, r + (lane >> 2));
-                cp_async16(sbase + kOffRope + buf * kRope + sw64(32 * w + r + (lane >> 2), lane & 3),
-                           a.kv + (int64_t)max(rs, 0) * kDq + kDv + 16 * (lane & 3), rs >= 0);
-              }
-            }
-            cp_async_arrive_noinc(full + 8 * j);         // fires when this thread's copies have landed
           }
+#pragma unroll
+          for (int r = 0; r < 32; r += 16) {             // 16 tokens a warp instruction: half of their 64 rope bytes
+            const int rs = __shfl_sync(0xffffffffu, from, r + (lane >> 1)), g = 2 * pair + (lane & 1);
+            cp_async16(rope + sw64(32 * half + r + (lane >> 1), g), a.kv + (int64_t)max(rs, 0) * kDq + kDv + 16 * g, rs >= 0);
+          }
+          cp_async_arrive_noinc(full);                   // fires when this thread's copies have landed
         }
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
         if (lane == 0) {
-          mask[4 * buf + w] = present;
-          if (w == 0) last_unit[buf] = cn >= c1;
-          mbar_arrive(full + 24);
+          int32_t* word = reinterpret_cast<int32_t*>(slots + slot);
+          if (pair == 0) word[half] = static_cast<int32_t>(present);
+          if (w == 0) word[2] = cn >= c1 ? kLast : kMore;
+          mbar_arrive_n(full, whole ? 32 : 1);           // of a whole unit also for the lanes that copied nothing
         }
-        ++u;
+        if (++slot == kSlots) slot = 0, ++round;
         c = cn;
         p = pn;
         page = page_n;
@@ -639,43 +607,60 @@ __global__ void __launch_bounds__(kThreads, 1)
     zero_rows(a, cta, h0, nh, lane);
     __syncwarp();
     const bool leader = elect_lane();
-    int u = 0;
+    int u = 0, slot = 0, seg = 0;
     Segment s;
     bool ok = true;
     while (ok && walk_next(a, walk, s)) {
       bool last = false, fresh = true;
+      if (seg > 0) ok = mbar_nap(B.o_free, (seg - 1) & 1, abort_flag, a.status);      // the row before has been read
       while (!last) {
-        ok = mbar_nap(B.p_full, u & 1, abort_flag, a.status);
+        const int set = u & 1;
+        if (ok) ok = mbar_nap(B.p_full + 8 * set, (u >> 1) & 1, abort_flag, a.status);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        last = last_unit[u & 1] != 0;
+        last = ring[u & 7].z != kMore;
         tc_fence_after();
-        issue_values(B, sbase, u & 1, fresh, leader);
+        issue_values(B, sbase, slot, set, fresh, leader);
         fresh = false;
         ++u;
+        if (++slot == kSlots) slot = 0;
       }
       if (ok && leader) tc_commit(B.o_full);
+      ++seg;
     }
     if (leader) tc_commit(B.drain);                      // everything issued here has completed when this arrives
   } else if (warp == kScoreWarp) {
     // ---------------------------------------------------------------- score products
     const bool leader = elect_lane();
-    int u = 0, seg = 0;
+    int u = 0, slot = 0, round = 0, seg = 0;
     Segment s;
     bool ok = true;
     while (ok && walk_next(a, walk, s)) {
-      ok = mbar_nap(B.q_full, seg & 1, abort_flag, a.status);
-      bool last = false;
+      bool last = false, started = false;
       while (!last) {
+        ok = mbar_nap(B.full + 8 * slot, round & 1, abort_flag, a.status);
         if (ok && u > 0) ok = mbar_nap(B.s_empty, (u - 1) & 1, abort_flag, a.status);
+        if (ok && !started) ok = mbar_nap(B.q_full, seg & 1, abort_flag, a.status);
+        started = true;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
+        fence_proxy_async_smem();                        // rows that threads copied -> the tensor core
         tc_fence_after();
-        ok = issue_scores<Q8>(B, sbase, u & 1, (u >> 1) & 1, leader, abort_flag, a.status);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        last = last_unit[u & 1] != 0;
+        // the unit's words, by unit: entry u & 7 was last read for the values of unit u - 8, which are done (the set of unit
+        // u - 3 waited for those of u - 5 before it gave its weights)
+        const int4 word = slots[slot];
+        last = word.z != kMore;
+        if (leader) {
+          ring[u & 7] = word;
+          mbar_arrive(B.s_full + 8 * (u & 1));
+        }
+        issue_scores(B, sbase, slot, u & 1, leader);
         ++u;
+        if (++slot == kSlots) slot = 0, ++round;
+      }
+      if (ok && leader) {                                // the set that has no further unit of the row is told so
+        ring[u & 7] = make_int4(0, 0, kEnd, 0);
+        mbar_arrive_n(B.s_full + 8 * (u & 1), 2);
       }
       ++seg;
     }
@@ -684,181 +669,184 @@ __global__ void __launch_bounds__(kThreads, 1)
     while (!mbar_try_wait(B.drain, 0) && globaltimer() - t0 <= 2 * kWaitNs) {}
     __syncwarp();
   } else {
-    // ---------------------------------------------------------------- softmax (warps 0-15): a token and 16 heads a thread
-    const int quarter = warp & 3, group = warp >> 2, hb = 16 * group, bid = 1 + group;
-    const int row = 32 * quarter + lane, mine = hb + (lane & 15);
+    // ---------------------------------------------------------------- softmax (warps 0-15): 16 tokens of a head a thread
+    const int quarter = warp & 3, half = (warp >> 2) & 1, set = warp >> 3, part = lane >> 4;
+    const int mine = 16 * quarter + (lane & 15);
     const uint32_t tq = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
-    float* scale = reinterpret_cast<float*>(smem + kOffScale);
-    float* part = reinterpret_cast<float*>(smem + kOffExp);
+    const int32_t* exps = reinterpret_cast<const int32_t*>(smem + kOffK);
+    float* refs = reinterpret_cast<float*>(smem + kOffRef);
+    float* rows = reinterpret_cast<float*>(smem + kOffRow);
     float* sums = reinterpret_cast<float*>(smem + kOffSum);
-    volatile int32_t* far = reinterpret_cast<volatile int32_t*>(smem + kOffRise);
-    if (group < 2) tmem_st_x4(tq + (group == 0 ? kColV : kColLow), group == 0 ? 0x78787878u : 0x74747474u);
-    tmem_st_wait();
-    int u = 0, seg = 0;
+    const uint32_t other = 8 * (set ^ 1), own = 8 * set;
+    const bool teller = warp < 4 && lane < 16;           // one thread a head
+    if (warp < 8) tmem_st_x4(tq + (warp < 4 ? kColV : kColLow), warp < 4 ? 0x78787878u : 0x74747474u);
+    int u0 = 0, seg = 0, events = 0;                     // the row's first unit
     Segment s;
     bool more = walk_next(a, walk, s), ok = true;
-    stage_q<Q8>(a, smem, s.t, h0, nh);
-    fence_proxy_async_smem();
+    if (teller) refs[mine] = mine < nh ? kNone : 0.0f;
+    stage_q<Q8>(a, smem, tmem, s.t, h0, nh);             // (also waits for the scales' stores)
     tc_fence_before();
     warp_arrive(B.q_full, lane);
-    named_bar(5, kSoftmax);                              // every head's scale is written
+    named_bar(5, kSoftmax);                              // every head's reference is written
     while (more) {
-      uint64_t l[8];                                     // the thread's sums of heads hb + 2 i, hb + 2 i + 1
-#pragma unroll
-      for (int i = 0; i < 8; ++i) l[i] = 0;
-      float ref = mine < nh ? kNone : -kNoHead;          // reference of head mine (the same in the 4 quarters)
-      bool last = false, fresh = true, unset = true;
-      while (!last) {
-        const int buf = u & 1;
-        ok = mbar_nap(B.s_full, u & 1, abort_flag, a.status);
-        if (ok) ok = mbar_nap(B.lat_full + 32 * buf + 24, (u >> 1) & 1, abort_flag, a.status);   // the mask's writes
+      const int k = Q8 ? 0 : exps[mine];
+      const float c = mine < nh ? a.bmm1 * kLog2e * (k == 255 ? 1.0f : __uint_as_float(static_cast<uint32_t>(127 + k) << 23)) : 0.0f;
+      const float c_own = part ? 0.0625f * c : c, c_got = part ? c : 0.0625f * c;
+      float l = 0.0f, ref = mine < nh ? kNone : 0.0f;    // the sum of the thread's weights, the reference it stands against
+      int u = u0 + ((set ^ u0) & 1);
+      while (true) {
+        ok = mbar_nap(B.s_full + own, events & 1, abort_flag, a.status);
+        ++events;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const int4 word = ring[u & 7];
+        if (word.z == kEnd) {
+          u0 = u;
+          break;
+        }
         tc_fence_after();
-        last = last_unit[buf] != 0;
-        const uint32_t present = mask[4 * buf + quarter];
-        uint64_t p[8];
-        float top[4];                                    // of 4 heads each: the warp's largest
-        {                                                // base-2 scores less the reference; tokens not there: -inf
-          float x[16], y[16];
-          tmem_ld_x16(tq + kColS + hb, x);
-          if (!Q8) tmem_ld_x16(tq + kColS + 64 + hb, y);
+        float v[16];                                     // base-2 scores; tokens not there: -inf
+        {
+          float x[32];
+          tmem_ld_32x32b_x32(tq + kColS + 32 * half, x);
           tmem_ld_wait();
           tc_fence_before();
           warp_arrive(B.s_empty, lane);
+          // lanes l and l + 16 have the high and the low part of 32 tokens: each gives the other the half that it does not keep
 #pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(scale + hb + i);
-            const ulonglong2 r = *reinterpret_cast<const ulonglong2*>(scale + 64 + hb + i);
-            uint64_t v = f2pack(x[i], x[i + 1]), w = f2pack(x[i + 2], x[i + 3]);
-            if (!Q8) {
-              v = fma2(f2pack(y[i], y[i + 1]), f2pack(0.0625f, 0.0625f), v);
-              w = fma2(f2pack(y[i + 2], y[i + 3]), f2pack(0.0625f, 0.0625f), w);
-            }
-            p[i / 2] = fma2(v, c.x, r.x);
-            p[i / 2 + 1] = fma2(w, c.y, r.y);
+          for (int i = 0; i < 16; ++i) {
+            const float got = __shfl_xor_sync(0xffffffffu, part ? x[i] : x[16 + i], 16);
+            v[i] = fmaf(part ? x[16 + i] : x[i], c_own, got * c_got);
           }
         }
-        if (present != 0xffffffffu && !((present >> lane) & 1)) {
+        const uint32_t present = static_cast<uint32_t>(half ? word.y : word.x);
+        if (present != 0xffffffffu) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) p[i] = f2pack(kNone, kNone);
+          for (int i = 0; i < 16; ++i)
+            if (!((present >> (16 * part + i)) & 1)) v[i] = kNone;
         }
-        auto tops = [&]() {
+        float m = kNone;                                 // the largest of the head's 32 tokens, NaN ignored
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m = fmaxf(m, v[i]);
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+        // the references after the unit before (the other set's)
+        if (u != u0) {
+          if (!mbar_nap(B.ref_ok + other, ((u - 1) >> 1) & 1, abort_flag, a.status)) ok = false;
+          const float now = refs[mine];
+          if (now != ref) {
+            if (ref != kNone) l *= exp2f(ref - now);
+            ref = now;
+          }
+        }
+        // the set agrees on the rare path (a failed wait travels the same way): a head without a reference, or with scores
+        // more than kMaxRise above it
+        if (__any_sync(0xffffffffu, (ref == kNone ? m > kNone : m - ref > kMaxRise) || !ok) && lane == 0) far[set] = 1;
+        warp_arrive(B.agree + own, lane);
+        uint32_t wh[4], wl[4];
+        float sum, unit;
+        int eb;
+        bool asked = false;
+#pragma unroll 1
+        while (true) {
+          // weights 2^(score - E + 8) with an exponent E for 32 tokens of a head: the ceiling of the largest of their scores
+          // above the head's reference. 2^(E - 8) is their block scale in the product and their weight in the sums; the
+          // e4m3 pairs keep 8 bits down to 2^-14 of that largest.
+          const float base = ref == kNone ? 0.0f : ref;
+          const float e = fminf(fmaxf(ceilf(m - base), kMinE), kMaxRise);
+          eb = static_cast<int>(e) + 119;                // biased exponent of 2^(E - 8)
+          unit = __uint_as_float(static_cast<uint32_t>(eb) << 23);
+          const float off = 8.0f - e;
+          uint64_t total = f2pack(0.0f, 0.0f);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float v0, v1, v2, v3;
-            f2unpack(p[2 * i], v0, v1);
-            f2unpack(p[2 * i + 1], v2, v3);
-            top[i] = warp_max(fmaxf(fmaxf(v0, v1), fmaxf(v2, v3)));
-          }
-        };
-        tops();
-        // the four quarters of a group agree on the rare path (a failed wait travels the same way)
-        if (lane == 0) {
-          if (unset || fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > kMaxRise || !ok) far[4 * buf + group] = 1;
-          mbar_arrive(B.agree + 8 * group);
-        }
-        if (!mbar_nap(B.agree + 8 * group, u & 1, abort_flag, a.status)) ok = false;
-        // (a quarter sets the next unit's flag at the earliest after this one is agreed on, and this buffer's next flag
-        // after the next agreement: cleared below, it is not lost)
-        if (far[4 * buf + group] != 0) {
-          if (named_bar_or(bid, kGroup, !ok)) {
-            ok = false;
-            break;
-          }
-          // new references: a head without one, or with scores more than kMaxRise above it, takes the ceiling of this
-          // unit's largest score; what it has accumulated is rescaled
-          const float old = ref == kNone ? 0.0f : ref;
+            uint32_t ph[2], pl[2];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float v0, v1;
-            f2unpack(p[i], v0, v1);
-            v0 = warp_max(v0), v1 = warp_max(v1);
-            if (lane == 0) *reinterpret_cast<float2*>(part + 64 * quarter + hb + 2 * i) = make_float2(v0, v1);
+            for (int j = 0; j < 2; ++j) {
+              const float w0 = ex2_fast(v[4 * i + 2 * j] - base + off), w1 = ex2_fast(v[4 * i + 2 * j + 1] - base + off);
+              total = add2(total, f2pack(w0, w1));
+              split2(w0, w1, ph[j], pl[j]);
+            }
+            wh[i] = ph[0] | (ph[1] << 16);
+            wl[i] = pl[0] | (pl[1] << 16);
           }
-          named_bar(bid, kGroup);
-          const float m = fmaxf(fmaxf(part[mine], part[64 + mine]), fmaxf(part[128 + mine], part[192 + mine]));
-          const bool move = m > kNone && (ref == kNone || m > kMaxRise);
-          const float now = move ? ceilf(m + old) : old;
-          const float f = move && ref != kNone ? exp2f(old - now) : 1.0f;
-          if (move) ref = now;
-          unset = __any_sync(0xffffffffu, ref == kNone);
-          named_bar(bid, kGroup);                        // the maxima are read: their place takes the moves
-          if (quarter == 0) {
-            sums[mine] = f;
-            part[mine] = old - now;
-            scale[64 + mine] = -now;
-            if (lane == 0) far[4 * buf + group] = 0;
+          float t0, t1;
+          f2unpack(total, t0, t1);
+          sum = t0 + t1;
+          if (asked) break;
+          asked = true;
+          if (!mbar_nap(B.agree + own, (u >> 1) & 1, abort_flag, a.status)) ok = false;
+          if (!__any_sync(0xffffffffu, far[set] != 0)) break;
+          // new references: the ceiling of this unit's largest score; what has been accumulated is rescaled
+          if (lane < 16) rows[64 * half + mine] = m;
+          warp_arrive(B.slow + own, lane);
+          if (!mbar_nap(B.slow + own, 0, abort_flag, a.status)) ok = false;
+          const float most = fmaxf(rows[mine], rows[64 + mine]);
+          const bool move = ref == kNone ? most > kNone : most - ref > kMaxRise;
+          const float now = move ? ceilf(most) : ref;
+          const float f = move && ref != kNone ? exp2f(ref - now) : 1.0f;
+          if (half == 0 && lane < 16) {
+            refs[mine] = now;
+            rows[128 + mine] = f;
           }
-          const bool scaled = __any_sync(0xffffffffu, f != 1.0f);
-          named_bar(bid, kGroup);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) p[i] = add2(p[i], *reinterpret_cast<const uint64_t*>(part + hb + 2 * i));
-          tops();
-          if (scaled && !fresh) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) l[i] = mul2(l[i], *reinterpret_cast<const uint64_t*>(sums + hb + 2 * i));
-            if (!mbar_nap(B.pv_done, (u - 1) & 1, abort_flag, a.status)) ok = false;
+          if (half == 0 && quarter == 0 && lane == 0) far[set] = 0;
+          warp_arrive(B.slow + own, lane);
+          if (!mbar_nap(B.slow + own, 1, abort_flag, a.status)) ok = false;
+          ref = now;
+          l *= f;
+          if (u != u0) {
+            if (!mbar_nap(B.pv_done + other, ((u - 1) >> 1) & 1, abort_flag, a.status)) ok = false;
             tc_fence_after();
 #pragma unroll 1
-            for (int d = 0; d < 4; ++d) {
+            for (int d = 0; d < 8; ++d) {                // 4 tiles of 128 dims, 16 of the warp's 32 heads at a time
+              const int h = 32 * half + 16 * (d & 1);
+              const uint32_t at = tq + kColO + 64 * (d >> 1) + h;
               float o[16];
-              tmem_ld_x16(tq + kColO + 64 * d + hb, o);
+              tmem_ld_x16(at, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int h = 0; h < 16; ++h) o[h] *= sums[hb + h];
-              tmem_st_x16(tq + kColO + 64 * d + hb, o);
+              for (int i = 0; i < 16; ++i) o[i] *= rows[128 + h + i];
+              tmem_st_x16(at, o);
             }
             tmem_st_wait();
           }
         }
-        // weights 2^(score - E + 8) with an exponent E for the warp's 32 tokens and 4 heads: the ceiling of the largest of
-        // their scores above the heads' references. 2^(E - 8) is their block scale in the product and their weight in the
-        // sums; the e4m3 pairs keep 8 bits down to 2^-14 of that largest.
-        uint32_t wh[4], wl[4];
-        uint8_t* sf = smem + kOffSf + 16 * (hb & 31) + 8 * buf + 4 * (group >> 1) + quarter;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float e = fminf(fmaxf(ceilf(top[i]), -100.0f), kMaxRise);
-          const uint32_t eb = static_cast<uint32_t>(static_cast<int>(e) + 119);        // biased exponent of 2^(E - 8)
-          const uint64_t off = f2pack(8.0f - e, 8.0f - e);
-          const uint64_t unit = f2pack(__uint_as_float(eb << 23), __uint_as_float(eb << 23));
-          if (lane < 4) sf[16 * (4 * i + lane)] = static_cast<uint8_t>(eb + 7);         // V's scale is 2^-7
-          uint32_t ph[2], pl[2];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            float w0, w1;
-            f2unpack(add2(p[2 * i + k], off), w0, w1);
-            w0 = ex2_fast(w0), w1 = ex2_fast(w1);
-            l[2 * i + k] = fma2(f2pack(w0, w1), unit, l[2 * i + k]);
-            split2(w0, w1, ph[k], pl[k]);
-          }
-          wh[i] = ph[0] | (ph[1] << 16);
-          wl[i] = pl[0] | (pl[1] << 16);
-        }
-        if (u > 0 && !mbar_nap(B.pv_done, (u - 1) & 1, abort_flag, a.status)) ok = false;   // its P has been read
-        *reinterpret_cast<uint4*>(smem + kOffRope + buf * kRope + sw64(row, group)) = make_uint4(wh[0], wh[1], wh[2], wh[3]);
-        *reinterpret_cast<uint4*>(smem + kOffPlo + sw64(row, group)) = make_uint4(wl[0], wl[1], wl[2], wl[3]);
+        warp_arrive(B.ref_ok + own, lane);
+        l = fmaf(sum, unit, l);
+        // the values of the set's unit before have read its P
+        if (u >= 2 && !mbar_nap(B.pv_done + own, ((u >> 1) - 1) & 1, abort_flag, a.status)) ok = false;
+        if (lane < 16)                                   // V's scale is 2^-7
+          smem[kOffSf + 16 * (mine & 31) + 8 * set + 4 * (mine >> 5) + half] = static_cast<uint8_t>(eb + 7);
+        const int at = sw64(mine, 2 * half + part);
+        *reinterpret_cast<uint4*>(smem + kOffRope + (u % kSlots) * kRope + at) = make_uint4(wh[0], wh[1], wh[2], wh[3]);
+        *reinterpret_cast<uint4*>(smem + kOffPlo + set * kRope + at) = make_uint4(wl[0], wl[1], wl[2], wl[3]);
         fence_proxy_async_smem();
         tc_fence_before();
-        warp_arrive(B.p_full, lane);
-        fresh = false;
-        ++u;
+        warp_arrive(B.p_full + own, lane);
+        if (word.z == kLast) {
+          u0 = u + 1;
+          break;
+        }
+        u += 2;
       }
       // ---- the row's sums, the next row's query, then the accumulators ----
-      float lf[16];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f2unpack(l[i], lf[2 * i], lf[2 * i + 1]);
-      const float ls = warp_sum_transposed(lf, lane);
       if (named_bar_or(5, kSoftmax, !ok)) break;
-      if (lane < 16) part[64 * quarter + mine] = ls;
+      const float last_ref = refs[mine];
+      if (ref != last_ref && ref != kNone) l *= exp2f(ref - last_ref);
+      ref = last_ref;
+      l += __shfl_xor_sync(0xffffffffu, l, 16);
+      if (lane < 16) rows[64 * (2 * set + half) + mine] = l;
       named_bar(5, kSoftmax);
-      float total = part[mine] + part[64 + mine] + part[128 + mine] + part[192 + mine];
+      float total = rows[mine] + rows[64 + mine] + rows[128 + mine] + rows[192 + mine];
       if (ref == kNone && total == total) total = 0.0f;                              // no token
-      if (quarter == 0) sums[mine] = total == 0.0f ? 0.0f : a.bmm2 / total;          // a NaN sum stays one
+      if (teller) {
+        sums[mine] = total == 0.0f ? 0.0f : a.bmm2 / total;                          // a NaN sum stays one
+        refs[mine] = mine < nh ? kNone : 0.0f;
+      }
       const Segment done = s;
       more = walk_next(a, walk, s);
       if (more) {
-        stage_q<Q8>(a, smem, s.t, h0, nh);
-        fence_proxy_async_smem();
+        stage_q<Q8>(a, smem, tmem, s.t, h0, nh);
+        tc_fence_before();
         warp_arrive(B.q_full, lane);
       }
       ok = mbar_nap(B.o_full, seg & 1, abort_flag, a.status);
@@ -866,15 +854,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const bool whole = done.b0 == 0 && done.b1 == done.nb;
       const int slot = 2 * cta + (seg == 0 ? 0 : 1);
-      if (quarter == 0 && lane < 16) {
+      if (teller) {
         if (!whole) part_ml(a, tile, slot)[mine] = make_float2(ref, total);
         else if (a.lse != nullptr && mine < nh)
           a.lse[(int64_t)done.t * a.H + h0 + mine] = total == 0.0f ? kNone : ((ref == kNone ? 0.0f : ref) + log2f(total)) * kLn2;
-        if (group == 0 && lane == 0 && tile == 0) {
+        if (mine == 0 && tile == 0) {
           if (done.b0 == 0) a.rows[done.t].first = cta, a.rows[done.t].first_slot = slot;
           if (done.b1 == done.nb) a.rows[done.t].last = cta;
         }
       }
+      const int hb = 16 * (warp >> 2);
       // a lane has one dim of 4 heads; crossed with its 3 neighbours, 4 dims of head (lane & 3)
       const int e = lane & 3, dim = 32 * quarter + (lane & 28);
       __nv_bfloat16* out = a.out + ((int64_t)done.t * a.H + h0 + hb + e) * kDv + dim;
@@ -904,6 +893,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         po += 4 * kDv;
       }
       tc_fence_before();
+      warp_arrive(B.o_free, lane);
       ++seg;
     }
   }
@@ -985,7 +975,7 @@ int launch_mla_decode(const MlaDecodeArgs& a_in, void* ws, int64_t ws_bytes, cud
       (a.indices != nullptr && (a.n_idx < 0 || a.ld_idx < a.n_idx)) || (a.reqs == nullptr && a.T > a.R))
     return kErrArgs;
   if (a.T == 0) return kOk;
-  const int64_t most = a.indices != nullptr ? (a.n_idx + kUnit - 1) / kUnit : a.width;      // units of a row
+  const int64_t most = a.indices != nullptr ? (a.n_idx + kUnit - 1) / kUnit : (int64_t)(kPage / kUnit) * a.width;   // units of a row
   if (a.T * (most + kRowCost) > 0x7fffffff) return kErrArgs;
   if (a.q == nullptr || a.kv == nullptr || a.table == nullptr || a.out == nullptr || ws == nullptr ||
       !aligned(a.q, 16) || !aligned(a.kv, 16) || !aligned(a.out, 16) || !aligned(ws, 256) || (a.ldq * eb) % 16 ||
