@@ -62,9 +62,8 @@ constexpr int kOffBar = kOffSf + 512;           // mbarriers
 constexpr int kOffMisc = kOffBar + 256;         // tmem address, abort flag, a set's unit with scores far above its references
 constexpr int kOffSlot = kOffMisc + 16;         // int4 [6] (8 places): of a slot's unit the tokens present (2 words), last of its row
 constexpr int kOffRing = kOffSlot + 128;        // int4 [8]: the same by unit, as the softmax and the values read it
-constexpr int kOffK = kOffRing + 128;           // int32 [64]: the query scale's exponent of each head
-constexpr int kOffRef = kOffK + 256;            // float [64]: the heads' references
-constexpr int kOffRow = kOffRef + 256;          // float [4][64]: maxima and rescale factors, or the sums
+constexpr int kOffRef = kOffRing + 128;         // float [64]: the heads' references
+constexpr int kOffRow = kOffRef + 256;          // float [4][64]: maxima and rescale factors, the sums, or maxima of the query
 constexpr int kOffSum = kOffRow + 1024;         // float [64]: bmm2 / l
 constexpr int kOffPlan = kOffSum + 256;         // int32 [52]: the plan's sums and first row
 constexpr int kSmem = kOffPlan + 208;
@@ -75,6 +74,7 @@ static_assert(kOffSlot % 16 == 0 && kOffRow % 16 == 0 && kOffSf % 128 == 0 && kS
 constexpr uint32_t kColO = 0, kColS = 256, kColQ = 320, kColV = 464, kColLow = 468, kColP = 472;
 constexpr float kMaxRise = 64.0f;               // base-2 scores above a head's reference before it moves and O is rescaled
 constexpr float kMinE = -100.0f;                // the least exponent of a block
+constexpr int kYield = 40;                      // looks at the score warp before the values go ahead (about 30 cycles each)
 enum : int32_t { kMore = 0, kLast = 1, kEnd = 2 };     // a unit, the last unit of its row, no unit: the row has ended
 constexpr uint32_t kSw128 = 2, kSw64 = 4;       // descriptor layout types
 
@@ -281,7 +281,8 @@ SSB_DEVICE bool find_range(const MlaDecodeArgs& a, int cta, int ctas, int32_t* s
   __syncthreads();
   units = __reduce_add_sync(0xffffffffu, lane < kThreads / 32 ? sh[lane] : 0);
   rows = __reduce_add_sync(0xffffffffu, lane < kThreads / 32 ? sh[24 + lane] : 0);
-  const int used = min(ctas, units);            // every range in use holds a unit: a row's CTAs are consecutive
+  // every range in use holds a unit: a row's CTAs are consecutive. A few short rows are not cut finer than two units
+  const int used = min(ctas, max(rows, (units + 1) / 2));
   if (cta >= used) return false;
   w.cost = units >= kCostFrom * ctas ? kRowCost : 0;
   const int total = units + rows * w.cost, per = total / used, rem = total - per * used;
@@ -382,65 +383,72 @@ SSB_DEVICE void issue_values(const Bars& B, uint32_t sbase, int slot, int set, b
 
 // One query row's heads h0 .. h0 + 63 as the parts of q 2^-k (k per head, its largest value in [2^7, 2^8)) into TMEM, zero
 // rows past nh. bf16 has 8 significant bits, so the two e4m3 parts hold a value exactly unless it is below 2^-14 of the
-// head's largest. First the exponents, 8 threads a head; then a thread has one part of its head's lane and a quarter of
-// the row, which the first pass left in the L1 cache. e4m3 queries have no low part.
+// head's largest. A thread has half of its head's quarter of the row (lanes l and l + 16 share a head): first for the
+// largest value, which goes round through rows, then again, four loads ahead, for the parts. Lane l keeps the high ones, lane
+// l + 16 the low ones, and they exchange the others. e4m3 queries have no low part.
 template <bool Q8>
-__device__ __noinline__ void stage_q(const MlaDecodeArgs& a, uint8_t* smem, uint32_t tmem, int t, int h0, int nh) {
-  int32_t* exps = reinterpret_cast<int32_t*>(smem + kOffK);
+__device__ __noinline__ int stage_q(const MlaDecodeArgs& a, uint8_t* smem, uint32_t tmem, int t, int h0, int nh) {
+  int32_t* tops = reinterpret_cast<int32_t*>(smem + kOffRow);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)t * a.ldq;
-  if (!Q8) {
-    const int h = threadIdx.x >> 3, sub = threadIdx.x & 7;
-    const uint4* q =
-        reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + row + (int64_t)(h0 + min(h, nh - 1)) * a.hsq);
-    uint4 v[9];
-#pragma unroll
-    for (int j = 0; j < 9; ++j) v[j] = __ldg(q + sub + 8 * j);        // 72 granules of 8 values
-    __nv_bfloat162 most = __floats2bfloat162_rn(0.0f, 0.0f);          // magnitudes, NaN kept
-#pragma unroll
-    for (int j = 0; j < 9; ++j) {
-      const __nv_bfloat162* w = reinterpret_cast<const __nv_bfloat162*>(&v[j]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) most = __hmax2_nan(most, __habs2(w[e]));
-    }
-    uint32_t top = *reinterpret_cast<uint32_t*>(&most) & 0x7FFF7FFFu;
-    top = max(top & 0xFFFFu, top >> 16);
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const int ex = static_cast<int>(top >> 7);                        // the largest value's biased exponent
-    // an infinite or NaN query value leaves its head no finite score: NaN, which e4m3 can carry (it has no infinity)
-    if (sub == 0) exps[h] = ex == 255 ? 255 : ex != 0 ? max(min(ex - 134, 120), -120) : 0;
-    named_bar(5, kSoftmax);
-  }
   const int h = 16 * (warp & 3) + (lane & 15), part = warp >> 2;      // 144 values
   const bool high = lane < 16, have = h < nh;
-  const int64_t off = row + (int64_t)(h0 + min(h, nh - 1)) * a.hsq + 144 * part;
+  const int64_t off = (int64_t)t * a.ldq + (int64_t)(h0 + min(h, nh - 1)) * a.hsq + 144 * part;
   uint32_t to = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + kColQ + 36 * part;
-  const int k = Q8 ? 0 : exps[h];
-  const float down = !have ? 0.0f : k == 255 ? NAN : __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
-#pragma unroll 1
-  for (int j = 0; j < 9; ++j, to += 4) {                              // 16 values
-    uint32_t w[4];
-    if (Q8) {
-      const uint4 g = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.q) + off) + j);
-      const bool keep = have && high;
-      w[0] = keep ? g.x : 0, w[1] = keep ? g.y : 0, w[2] = keep ? g.z : 0, w[3] = keep ? g.w : 0;
-    } else {
-      const uint4* q = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + off) + 2 * j;
-      const uint4 g0 = __ldg(q), g1 = __ldg(q + 1);
-      const uint32_t v[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
+  int k = 0;
+  if (Q8) {
+    const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.q) + off);
+    const bool keep = have && high;
+#pragma unroll 3
+    for (int j = 0; j < 9; ++j, to += 4) {                            // 16 values
+      const uint4 g = __ldg(q + j);
+      const uint32_t w[4] = {keep ? g.x : 0, keep ? g.y : 0, keep ? g.z : 0, keep ? g.w : 0};
+      tmem_st_4(to, w);
+    }
+  } else {
+    const uint4* q = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + off) + (high ? 0 : 1);
+    __nv_bfloat162 most = __floats2bfloat162_rn(0.0f, 0.0f);          // magnitudes, NaN kept
+    {
+      uint4 v[9];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t hi[2], lo[2];
+      for (int j = 0; j < 9; ++j) v[j] = __ldg(q + 2 * j);            // 8 values
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          split2(__uint_as_float(v[2 * e + i] << 16) * down, __uint_as_float(v[2 * e + i] & 0xFFFF0000u) * down, hi[i], lo[i]);
-        w[e] = high ? hi[0] | (hi[1] << 16) : lo[0] | (lo[1] << 16);
+      for (int j = 0; j < 9; ++j) {
+        const __nv_bfloat162* w = reinterpret_cast<const __nv_bfloat162*>(&v[j]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = __hmax2_nan(most, __habs2(w[e]));
       }
     }
-    tmem_st_4(to, w);
+    int top = *reinterpret_cast<int32_t*>(&most) & 0x7FFF7FFF;
+    top = max(top & 0xFFFF, top >> 16);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 16));
+    if (high) tops[64 * part + h] = top;
+    named_bar(5, kSoftmax);
+    top = max(max(tops[h], tops[64 + h]), max(tops[128 + h], tops[192 + h]));
+    const int ex = top >> 7;                                          // the largest value's biased exponent
+    if (ex != 0) k = max(min(ex - 134, 120), -120);
+    // an infinite or NaN query value leaves its head no finite score: NaN, which e4m3 can carry (it has no infinity)
+    const float down = !have ? 0.0f : ex == 255 ? NAN : __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+    uint4 next[4] = {__ldg(q), __ldg(q + 2), __ldg(q + 4), __ldg(q + 6)};
+#pragma unroll 1
+    for (int j = 0; j < 9; ++j, to += 4) {                            // 16 values, of which this thread has 8
+      const uint4 g = next[0];
+      next[0] = next[1], next[1] = next[2], next[2] = next[3];
+      if (j < 5) next[3] = __ldg(q + 2 * j + 8);
+      const uint32_t v[4] = {g.x, g.y, g.z, g.w};
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        split2(__uint_as_float(v[i] << 16) * down, __uint_as_float(v[i] & 0xFFFF0000u) * down, hi[i], lo[i]);
+      const uint32_t h01 = hi[0] | (hi[1] << 16), h23 = hi[2] | (hi[3] << 16);
+      const uint32_t l01 = lo[0] | (lo[1] << 16), l23 = lo[2] | (lo[3] << 16);
+      const uint32_t r01 = __shfl_xor_sync(0xffffffffu, high ? l01 : h01, 16);
+      const uint32_t r23 = __shfl_xor_sync(0xffffffffu, high ? l23 : h23, 16);
+      const uint32_t w[4] = {high ? h01 : r01, high ? h23 : r23, high ? r01 : l01, high ? r23 : l23};
+      tmem_st_4(to, w);
+    }
   }
   tmem_st_wait();
+  return k;
 }
 
 template <bool Q8>
@@ -459,6 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int32_t* far = reinterpret_cast<volatile int32_t*>(smem + kOffMisc + 8);           // [2]
   int4* slots = reinterpret_cast<int4*>(smem + kOffSlot);
   int4* ring = reinterpret_cast<int4*>(smem + kOffRing);
+  volatile int32_t* scoring = reinterpret_cast<volatile int32_t*>(smem + kOffSlot + 96);    // the score warp has rows to issue
   if (sbase & 1023) {                                    // the swizzled tiles need it; no static shared memory precedes
     if (tid == 0) raise_status(a.status, kErrCuda);
     return;
@@ -474,6 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (lane < 2) far[lane] = 0;
     if (lane == 2) *abort_flag = 0;
+    if (lane == 3) *scoring = 0;
     fence_barrier_init();
   } else if (warp == kValueWarp) {
     tmem_alloc(smem_u32(tmem_slot), 512);
@@ -544,12 +554,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       int64_t page = p >= 0 ? page_row(p) : -1;
       while (c < c1) {
         const int cn = next_live(c + 1);
-        int pn = -1;
-        int64_t page_n = -1;
-        if (cn < c1) {
-          pn = token(cn);
-          page_n = pn >= 0 ? page_row(pn) : -1;
-        }
         const uint32_t full = B.full + 8 * slot;
         const uint32_t dst = sbase + kOffKv + slot * kLat, rope = sbase + kOffRope + slot * kRope;
         const int64_t row = page + (p & (kPage - 1));
@@ -596,9 +600,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive_n(full, whole ? 32 : 1);           // of a whole unit also for the lanes that copied nothing
         }
         if (++slot == kSlots) slot = 0, ++round;
-        c = cn;
-        p = pn;
-        page = page_n;
+        c = cn;                                          // the next unit's tokens, after this one is on its way
+        p = cn < c1 ? token(cn) : -1;
+        page = p >= 0 ? page_row(p) : -1;
       }
     }
     cp_async_wait_all();
@@ -619,6 +623,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         last = ring[u & 7].z != kMore;
+        // scores first, where their rows are there: the values then run while S is read and handed back
+        for (int i = 0; i < kYield && *scoring != 0; ++i) {}
         tc_fence_after();
         issue_values(B, sbase, slot, set, fresh, leader);
         fresh = false;
@@ -639,6 +645,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool last = false, started = false;
       while (!last) {
         ok = mbar_nap(B.full + 8 * slot, round & 1, abort_flag, a.status);
+        if (leader) *scoring = 1;
         if (ok && u > 0) ok = mbar_nap(B.s_empty, (u - 1) & 1, abort_flag, a.status);
         if (ok && !started) ok = mbar_nap(B.q_full, seg & 1, abort_flag, a.status);
         started = true;
@@ -655,6 +662,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive(B.s_full + 8 * (u & 1));
         }
         issue_scores(B, sbase, slot, u & 1, leader);
+        if (leader) *scoring = 0;
         ++u;
         if (++slot == kSlots) slot = 0, ++round;
       }
@@ -673,7 +681,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int quarter = warp & 3, half = (warp >> 2) & 1, set = warp >> 3, part = lane >> 4;
     const int mine = 16 * quarter + (lane & 15);
     const uint32_t tq = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
-    const int32_t* exps = reinterpret_cast<const int32_t*>(smem + kOffK);
     float* refs = reinterpret_cast<float*>(smem + kOffRef);
     float* rows = reinterpret_cast<float*>(smem + kOffRow);
     float* sums = reinterpret_cast<float*>(smem + kOffSum);
@@ -684,13 +691,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     Segment s;
     bool more = walk_next(a, walk, s), ok = true;
     if (teller) refs[mine] = mine < nh ? kNone : 0.0f;
-    stage_q<Q8>(a, smem, tmem, s.t, h0, nh);             // (also waits for the scales' stores)
+    int k = stage_q<Q8>(a, smem, tmem, s.t, h0, nh);     // the query scale's exponent of head mine (also waits for the scales' stores)
     tc_fence_before();
     warp_arrive(B.q_full, lane);
     named_bar(5, kSoftmax);                              // every head's reference is written
     while (more) {
-      const int k = Q8 ? 0 : exps[mine];
-      const float c = mine < nh ? a.bmm1 * kLog2e * (k == 255 ? 1.0f : __uint_as_float(static_cast<uint32_t>(127 + k) << 23)) : 0.0f;
+      const float c = mine < nh ? a.bmm1 * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + k) << 23) : 0.0f;
       const float c_own = part ? 0.0625f * c : c, c_got = part ? c : 0.0625f * c;
       float l = 0.0f, ref = mine < nh ? kNone : 0.0f;    // the sum of the thread's weights, the reference it stands against
       int u = u0 + ((set ^ u0) & 1);
@@ -845,7 +851,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Segment done = s;
       more = walk_next(a, walk, s);
       if (more) {
-        stage_q<Q8>(a, smem, tmem, s.t, h0, nh);
+        if (!Q8) named_bar(5, kSoftmax);                 // the sums are read: their place takes the query's maxima
+        k = stage_q<Q8>(a, smem, tmem, s.t, h0, nh);
         tc_fence_before();
         warp_arrive(B.q_full, lane);
       }
