@@ -194,6 +194,14 @@ SSB_DEVICE void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
   hi = half2_e4m3(v);
   lo = half2_e4m3(__hmul2(__hsub2(v, e4m3_half2(hi)), __float2half2_rn(16.0f)));
 }
+// The same of two halves with 8 significant bits: hi has the leading 4, lo exactly the others (a value below 2^-6, where hi
+// loses bits, is off by 2^-10 at most). Half the conversions of `split2`, which run at a sixteenth of the arithmetic's rate.
+SSB_DEVICE void split2_bf16(uint32_t v, uint32_t& hi, uint32_t& lo) {
+  const uint32_t h = v & 0xFF80FF80u;
+  const __half2 a = *reinterpret_cast<const __half2*>(&v), b = *reinterpret_cast<const __half2*>(&h);
+  hi = half2_e4m3(b);
+  lo = half2_e4m3(__hmul2(__hsub2(a, b), __float2half2_rn(16.0f)));
+}
 // Byte offset of 16-byte granule g of row r: a 128-byte-swizzled chunk, a 64-byte-swizzled one.
 SSB_DEVICE uint32_t sw128(int r, int g) { return r * 128 + ((g ^ (r & 7)) << 4); }
 SSB_DEVICE uint32_t sw64(int r, int g) { return r * 64 + ((g ^ ((r >> 1) & 3)) << 4); }
@@ -383,9 +391,9 @@ SSB_DEVICE void issue_values(const Bars& B, uint32_t sbase, int slot, int set, b
 
 // One query row's heads h0 .. h0 + 63 as the parts of q 2^-k (k per head, its largest value in [2^7, 2^8)) into TMEM, zero
 // rows past nh. bf16 has 8 significant bits, so the two e4m3 parts hold a value exactly unless it is below 2^-14 of the
-// head's largest. A thread has half of its head's quarter of the row (lanes l and l + 16 share a head): first for the
-// largest value, which goes round through rows, then again, four loads ahead, for the parts. Lane l keeps the high ones, lane
-// l + 16 the low ones, and they exchange the others. e4m3 queries have no low part.
+// head's largest (then to 2^-18 of that). First the largest values, 8 threads a head (whole
+// lines); then a thread has half of its lane's head's quarter of the row (lanes l and l + 16 share a head), loaded four
+// ahead: lane l keeps the high parts, lane l + 16 the low ones, and they exchange the others. e4m3 queries have no low part.
 template <bool Q8>
 __device__ __noinline__ int stage_q(const MlaDecodeArgs& a, uint8_t* smem, uint32_t tmem, int t, int h0, int nh) {
   int32_t* tops = reinterpret_cast<int32_t*>(smem + kOffRow);
@@ -405,30 +413,37 @@ __device__ __noinline__ int stage_q(const MlaDecodeArgs& a, uint8_t* smem, uint3
       tmem_st_4(to, w);
     }
   } else {
-    const uint4* q = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + off) + (high ? 0 : 1);
-    __nv_bfloat162 most = __floats2bfloat162_rn(0.0f, 0.0f);          // magnitudes, NaN kept
+    const __nv_bfloat16* base = static_cast<const __nv_bfloat16*>(a.q) + (int64_t)t * a.ldq + (int64_t)h0 * a.hsq;
     {
+      const int th = threadIdx.x >> 3, sub = threadIdx.x & 7;
+      const uint4* q = reinterpret_cast<const uint4*>(base + (int64_t)min(th, nh - 1) * a.hsq) + sub;
       uint4 v[9];
 #pragma unroll
-      for (int j = 0; j < 9; ++j) v[j] = __ldg(q + 2 * j);            // 8 values
+      for (int j = 0; j < 9; ++j) v[j] = __ldg(q + 8 * j);            // 8 values
+      __nv_bfloat162 most = __floats2bfloat162_rn(0.0f, 0.0f);        // magnitudes, NaN kept
 #pragma unroll
       for (int j = 0; j < 9; ++j) {
         const __nv_bfloat162* w = reinterpret_cast<const __nv_bfloat162*>(&v[j]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) most = __hmax2_nan(most, __habs2(w[e]));
       }
+      int top = *reinterpret_cast<int32_t*>(&most) & 0x7FFF7FFF;
+      top = max(top & 0xFFFF, top >> 16);
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (sub == 0) tops[th] = top;
     }
-    int top = *reinterpret_cast<int32_t*>(&most) & 0x7FFF7FFF;
-    top = max(top & 0xFFFF, top >> 16);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 16));
-    if (high) tops[64 * part + h] = top;
+    const uint4* q = reinterpret_cast<const uint4*>(base + (int64_t)min(h, nh - 1) * a.hsq + 144 * part) + (high ? 0 : 1);
+    uint4 next[4] = {__ldg(q), __ldg(q + 2), __ldg(q + 4), __ldg(q + 6)};
     named_bar(5, kSoftmax);
-    top = max(max(tops[h], tops[64 + h]), max(tops[128 + h], tops[192 + h]));
+    const int top = tops[h];
     const int ex = top >> 7;                                          // the largest value's biased exponent
     if (ex != 0) k = max(min(ex - 134, 120), -120);
-    // an infinite or NaN query value leaves its head no finite score: NaN, which e4m3 can carry (it has no infinity)
-    const float down = !have ? 0.0f : ex == 255 ? NAN : __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
-    uint4 next[4] = {__ldg(q), __ldg(q + 2), __ldg(q + 4), __ldg(q + 6)};
+    // q 2^-k as halves by integer arithmetic on two magnitudes at a time: the exponent's bias changes by 112 + k, what is
+    // below 2^-14 becomes 0. An infinite or NaN query value leaves its head no finite score: NaN, which e4m3 can carry (it
+    // has no infinity)
+    const uint32_t bias = static_cast<uint32_t>(-((112 + k) << 7)) & 0xFFFFu, down = bias | (bias << 16);
+    const uint32_t keep = have ? 0xFFFFFFFFu : 0u, bad = have && ex == 255 ? 0x7E007E00u : 0u;
 #pragma unroll 1
     for (int j = 0; j < 9; ++j, to += 4) {                            // 16 values, of which this thread has 8
       const uint4 g = next[0];
@@ -438,7 +453,7 @@ __device__ __noinline__ int stage_q(const MlaDecodeArgs& a, uint8_t* smem, uint3
       uint32_t hi[4], lo[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        split2(__uint_as_float(v[i] << 16) * down, __uint_as_float(v[i] & 0xFFFF0000u) * down, hi[i], lo[i]);
+        split2_bf16((__viaddmax_s16x2_relu(v[i] & 0x7FFF7FFFu, down, 0u) << 3 | (v[i] & 0x80008000u) | bad) & keep, hi[i], lo[i]);
       const uint32_t h01 = hi[0] | (hi[1] << 16), h23 = hi[2] | (hi[3] << 16);
       const uint32_t l01 = lo[0] | (lo[1] << 16), l23 = lo[2] | (lo[3] << 16);
       const uint32_t r01 = __shfl_xor_sync(0xffffffffu, high ? l01 : h01, 16);
@@ -871,33 +886,38 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       const int hb = 16 * (warp >> 2);
+      if (!whole) {                                      // a lane has one dim of 16 heads: 128 bytes a warp and head
+        float* po = part_o(a, tile, slot) + hb * kDv + 32 * quarter + lane;
+#pragma unroll 1
+        for (int d = 0; d < 4 && hb < nh; ++d, po += 128) {
+          float o[16];
+          tmem_ld_x16(tq + kColO + 64 * d + hb, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int h = 0; h < 16; ++h) po[h * kDv] = o[h];
+        }
+      }
       // a lane has one dim of 4 heads; crossed with its 3 neighbours, 4 dims of head (lane & 3)
       const int e = lane & 3, dim = 32 * quarter + (lane & 28);
       __nv_bfloat16* out = a.out + ((int64_t)done.t * a.H + h0 + hb + e) * kDv + dim;
-      float* po = part_o(a, tile, slot) + (hb + e) * kDv + dim;
 #pragma unroll 1
-      for (int i = 0; i < 16 && hb + i < nh; i += 4) {   // 4 heads x 4 tiles of 128 dims
+      for (int i = 0; i < 16 && hb + i < nh && whole; i += 4) {      // 4 heads x 4 tiles of 128 dims
         float o[4][4];
 #pragma unroll
         for (int d = 0; d < 4; ++d) tmem_ld_x4(tq + kColO + 64 * d + hb + i, o[d]);
         tmem_ld_wait();
-        const float inv = whole ? sums[hb + i + e] : 1.0f;
+        const float inv = sums[hb + i + e];
         const bool have = hb + i + e < nh;
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
           cross4(o[d], lane);
-          if (whole) {
-            const __nv_bfloat162 v0 = __floats2bfloat162_rn(o[d][0] * inv, o[d][1] * inv);
-            const __nv_bfloat162 v1 = __floats2bfloat162_rn(o[d][2] * inv, o[d][3] * inv);
-            if (have)
-              *reinterpret_cast<uint2*>(out + 128 * d) =
-                  make_uint2(*reinterpret_cast<const uint32_t*>(&v0), *reinterpret_cast<const uint32_t*>(&v1));
-          } else {
-            *reinterpret_cast<float4*>(po + 128 * d) = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
-          }
+          const __nv_bfloat162 v0 = __floats2bfloat162_rn(o[d][0] * inv, o[d][1] * inv);
+          const __nv_bfloat162 v1 = __floats2bfloat162_rn(o[d][2] * inv, o[d][3] * inv);
+          if (have)
+            *reinterpret_cast<uint2*>(out + 128 * d) =
+                make_uint2(*reinterpret_cast<const uint32_t*>(&v0), *reinterpret_cast<const uint32_t*>(&v1));
         }
         out += 4 * kDv;
-        po += 4 * kDv;
       }
       tc_fence_before();
       warp_arrive(B.o_free, lane);
@@ -921,8 +941,9 @@ __global__ void __launch_bounds__(128) mla_join_kernel(const __grid_constant__ M
   const int64_t t = blockIdx.x;
   const int h = blockIdx.y, tile = h / kTileH, hh = h - tile * kTileH;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int units = row_units(a, static_cast<int>(t));     // of the inputs alone
   asm volatile("griddepcontrol.wait;" ::: "memory");       // the parts are written
-  if (row_units(a, static_cast<int>(t)) == 0) return;
+  if (units == 0) return;
   const MlaRowParts rp = a.rows[t];
   if (rp.first == rp.last) return;
   const bool spread = gridDim.z == 4;
