@@ -270,7 +270,7 @@ __device__ __noinline__ bool walk_next(const MlaDecodeArgs& a, Walk& w, Segment&
   }
   return found;
 }
-constexpr int kRowCost = 4, kCostFrom = 12;      // units; ranges of so many units or more bear it
+constexpr int kRowCost = 10, kCostFrom = 24;      // units; ranges of so many units or more bear it
 
 // All threads of the CTA: its range and the row that holds its beginning. sh: 48 words for the warps' sums, 4 for the row.
 // False: more CTAs than units, nothing to do here.
@@ -533,42 +533,40 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int len = a.seq_lens != nullptr ? a.seq_lens[s.t] : 0x7fffffff;
       const int32_t* idx = a.indices != nullptr ? a.indices + (int64_t)s.t * a.ld_idx : nullptr;
       int c0 = s.b0, c1 = s.b1;
-      unsigned long long live = ~0ull;                   // bit i: unit c0 + i holds a selected token
       if (idx != nullptr) {                              // the row's planned share as units of list columns
         c0 = static_cast<int>((int64_t)s.b0 * cols / s.nb);
         c1 = static_cast<int>((int64_t)s.b1 * cols / s.nb);
-        if (c1 - c0 <= 64) {
-          live = 0;
-#pragma unroll 2
-          for (int c = c0; c < c1; ++c) {
-            bool any = false;
-#pragma unroll
-            for (int j = 0; j < kUnit / 32; ++j) {
-              const int col = c * kUnit + 32 * j + lane;
-              const int pos = col < a.n_idx ? idx[col] : -1;
-              any |= pos >= 0 && pos < len;
-            }
-            if (__any_sync(0xffffffffu, any)) live |= 1ull << (c - c0);
-          }
-          if (live == 0) live = 1;                       // nothing selected: one empty unit gives the zeros
-        }
       }
       // first cache row of the page of position p (-1: none)
-      auto page_row = [&](int p) -> int64_t { return p / kPage < a.width ? (int64_t)pages[p / kPage] * kPage : -1; };
-      auto token = [&](int c) {                          // position of this lane's token of unit c (-1: none)
-        int p = c * kUnit + 32 * half + lane;
-        if (idx != nullptr) p = p < a.n_idx ? idx[p] : -1;
-        return p < len ? p : -1;
+      auto page_row = [&](int p) -> int64_t {
+        return p >= 0 && p / kPage < a.width ? (int64_t)pages[p / kPage] * kPage : -1;
       };
-      auto next_live = [&](int c) {
-        while (c < c1 && c - c0 < 64 && !((live >> (c - c0)) & 1)) ++c;
+      // the first unit from c on that holds a token (c1: none), and the position of this lane's token of it (-1: none)
+      auto find = [&](int c, int& p) {
+        p = -1;
+        if (idx == nullptr) {
+          if (c < c1) p = c * kUnit + 32 * half + lane;
+          if (p >= len) p = -1;
+          return c;
+        }
+#pragma unroll 1
+        for (; c < c1; ++c) {
+          const int col = c * kUnit + lane;
+          const int p0 = col < a.n_idx ? idx[col] : -1, p1 = col + 32 < a.n_idx ? idx[col + 32] : -1;
+          const bool live0 = p0 >= 0 && p0 < len, live1 = p1 >= 0 && p1 < len;
+          if (__any_sync(0xffffffffu, live0 || live1)) {
+            p = half ? (live1 ? p1 : -1) : (live0 ? p0 : -1);
+            break;
+          }
+        }
         return c;
       };
-      int c = next_live(c0);
-      int p = token(c);
-      int64_t page = p >= 0 ? page_row(p) : -1;
+      int p, pn;
+      int c = find(c0, p);
+      if (c >= c1) c = c0;                               // nothing selected: one empty unit gives the zeros
+      int cn = find(c + 1, pn);
+      int64_t page = page_row(p);
       while (c < c1) {
-        const int cn = next_live(c + 1);
         const uint32_t full = B.full + 8 * slot;
         const uint32_t dst = sbase + kOffKv + slot * kLat, rope = sbase + kOffRope + slot * kRope;
         const int64_t row = page + (p & (kPage - 1));
@@ -615,9 +613,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive_n(full, whole ? 32 : 1);           // of a whole unit also for the lanes that copied nothing
         }
         if (++slot == kSlots) slot = 0, ++round;
-        c = cn;                                          // the next unit's tokens, after this one is on its way
-        p = cn < c1 ? token(cn) : -1;
-        page = p >= 0 ? page_row(p) : -1;
+        c = cn;                                          // the next unit's pages and the tokens of the one after it, while
+        p = pn;                                          // this one is on its way
+        page = page_row(p);
+        cn = find(c + 1, pn);
       }
     }
     cp_async_wait_all();
