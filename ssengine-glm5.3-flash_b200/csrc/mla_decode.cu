@@ -537,40 +537,45 @@ __global__ void __launch_bounds__(kThreads, 1)
         c0 = static_cast<int>((int64_t)s.b0 * cols / s.nb);
         c1 = static_cast<int>((int64_t)s.b1 * cols / s.nb);
       }
-      // first cache row of the page of position p (-1: none)
-      auto page_row = [&](int p) -> int64_t {
-        return p >= 0 && p / kPage < a.width ? (int64_t)pages[p / kPage] * kPage : -1;
+      // the page of position p (-1: none); the two list entries of a column at this lane (-1: none)
+      auto page_of = [&](int p) { return p >= 0 && p / kPage < a.width ? pages[p / kPage] : -1; };
+      auto entry = [&](int c, int i) {
+        const int col = c * kUnit + 32 * i + lane;
+        return idx != nullptr && c < c1 && col < a.n_idx ? idx[col] : -1;
       };
-      // the first unit from c on that holds a token (c1: none), and the position of this lane's token of it (-1: none)
-      auto find = [&](int c, int& p) {
+      // the first unit from c on that holds a token (c1: none), e0 and e1 the list entries of unit c; p: the position of
+      // this lane's token of it (-1: none)
+      auto find = [&](int c, int e0, int e1, int& p) {
         p = -1;
         if (idx == nullptr) {
           if (c < c1) p = c * kUnit + 32 * half + lane;
           if (p >= len) p = -1;
-          return c;
+          return min(c, c1);
         }
-#pragma unroll 1
-        for (; c < c1; ++c) {
-          const int col = c * kUnit + lane;
-          const int p0 = col < a.n_idx ? idx[col] : -1, p1 = col + 32 < a.n_idx ? idx[col + 32] : -1;
-          const bool live0 = p0 >= 0 && p0 < len, live1 = p1 >= 0 && p1 < len;
-          if (__any_sync(0xffffffffu, live0 || live1)) {
-            p = half ? (live1 ? p1 : -1) : (live0 ? p0 : -1);
+        while (c < c1) {
+          e0 = e0 < len ? e0 : -1, e1 = e1 < len ? e1 : -1;
+          if (__any_sync(0xffffffffu, e0 >= 0 || e1 >= 0)) {
+            p = half ? e1 : e0;
             break;
           }
+          ++c;
+          e0 = entry(c, 0), e1 = entry(c, 1);
         }
         return c;
       };
       int p, pn;
-      int c = find(c0, p);
+      int c = find(c0, entry(c0, 0), entry(c0, 1), p);
       if (c >= c1) c = c0;                               // nothing selected: one empty unit gives the zeros
-      int cn = find(c + 1, pn);
-      int64_t page = page_row(p);
+      int cn = find(c + 1, entry(c + 1, 0), entry(c + 1, 1), pn);
+      int page = page_of(p);
       while (c < c1) {
+        // the next unit's pages and the list entries of the one after it are on their way while this one is copied (of a
+        // dense unit, which is a few instructions, the pages come after it)
+        const int page_n = idx != nullptr ? page_of(pn) : -1, e0 = entry(cn + 1, 0), e1 = entry(cn + 1, 1);
         const uint32_t full = B.full + 8 * slot;
         const uint32_t dst = sbase + kOffKv + slot * kLat, rope = sbase + kOffRope + slot * kRope;
-        const int64_t row = page + (p & (kPage - 1));
-        const int from = p >= 0 && page >= 0 && row < a.cache_rows ? static_cast<int>(row) : -1;
+        const int64_t row = (int64_t)page * kPage + (p & (kPage - 1));
+        const int from = page >= 0 && row < a.cache_rows ? static_cast<int>(row) : -1;
         const uint32_t present = __ballot_sync(0xffffffffu, from >= 0);
         // the slot is free when the values of the unit six before have used it (its words were read before its scores)
         if (round > 0) ok = mbar_nap(B.empty + 8 * slot, (round - 1) & 1, abort_flag, a.status);
@@ -579,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // A whole unit of a page (the same in every lane and warp) comes as tiles; a row's last units, and selected tokens,
         // row by row: rows that are not there have to be zeros (whatever the cache holds there, NaN too, would meet weight 0
         // in the value product).
-        const int64_t y = page + ((c * kUnit) & (kPage - 1));
+        const int64_t y = (int64_t)page * kPage + ((c * kUnit) & (kPage - 1));
         const bool whole = idx == nullptr && (c + 1) * kUnit <= len && page >= 0 && y + kUnit <= a.cache_rows;
         if (whole) {
           if (lane == 0) {
@@ -588,16 +593,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (w == 3) tma_load_2d(rope, &mrope, kDv, static_cast<int>(y), full);
           }
         } else {
-          int sl[8];
+          // 4 tokens a warp instruction, 128 of their latent bytes; rows 8 apart swizzle alike
+          const uint32_t to[2] = {dst + 2 * pair * kChunk + sw128(32 * half + (lane >> 3), lane & 7),
+                                  dst + 2 * pair * kChunk + sw128(32 * half + 4 + (lane >> 3), lane & 7)};
+          const uint8_t* src = a.kv + 256 * pair + 16 * (lane & 7);
 #pragma unroll
-          for (int r = 0; r < 8; ++r) sl[r] = __shfl_sync(0xffffffffu, from, 4 * r + (lane >> 3));
-#pragma unroll 1
-          for (int j = 2 * pair; j < 2 * pair + 2; ++j) {
-            const uint8_t* src = a.kv + 128 * j + 16 * (lane & 7);
-#pragma unroll
-            for (int r = 0; r < 8; ++r)                  // 4 tokens a warp instruction: 128 of their latent bytes
-              cp_async16(dst + j * kChunk + sw128(32 * half + 4 * r + (lane >> 3), lane & 7),
-                         src + (int64_t)max(sl[r], 0) * kDq, sl[r] >= 0);
+          for (int r = 0; r < 8; ++r) {
+            const int rs = __shfl_sync(0xffffffffu, from, 4 * r + (lane >> 3));
+            const uint8_t* at = src + (int64_t)max(rs, 0) * kDq;
+            cp_async16(to[r & 1] + (r >> 1) * 1024, at, rs >= 0);
+            cp_async16(to[r & 1] + (r >> 1) * 1024 + kChunk, at + 128, rs >= 0);
           }
 #pragma unroll
           for (int r = 0; r < 32; r += 16) {             // 16 tokens a warp instruction: half of their 64 rope bytes
@@ -613,10 +618,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive_n(full, whole ? 32 : 1);           // of a whole unit also for the lanes that copied nothing
         }
         if (++slot == kSlots) slot = 0, ++round;
-        c = cn;                                          // the next unit's pages and the tokens of the one after it, while
-        p = pn;                                          // this one is on its way
-        page = page_row(p);
-        cn = find(c + 1, pn);
+        c = cn;
+        p = pn;
+        page = idx != nullptr ? page_n : page_of(p);
+        cn = find(cn + 1, e0, e1, pn);
       }
     }
     cp_async_wait_all();
