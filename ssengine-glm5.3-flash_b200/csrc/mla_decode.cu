@@ -50,17 +50,19 @@ constexpr int kGatherWarps = 4;
 constexpr int kThreads = 32 * (kGatherWarp + kGatherWarps);
 
 // ---- shared memory ------------------------------------------------------------------------------------------------
-constexpr int kSlots = 6;                       // units in shared memory
+constexpr int kSlots = 5;                       // units in shared memory
 constexpr int kChunk = 8192;                    // [64 rows x 128 B], 128-byte swizzle
 constexpr int kRope = 4096;                     // [64 rows x 64 B], 64-byte swizzle
 constexpr int kLat = 4 * kChunk;                // a unit's latent rows
 constexpr int kOffKv = 0;                       // the latent rows of the units
 constexpr int kOffRope = kSlots * kLat;         // their rope keys; once its scores are done, a unit's high parts of P
 constexpr int kOffPlo = kOffRope + kSlots * kRope;    // the low parts of P, two units
-constexpr int kOffSf = kOffPlo + 2 * kRope;     // block scales of P, two units: byte (h % 32) 16 + unit 8 + (h / 32) 4 + half
+constexpr int kOffQ = kOffPlo + 2 * kRope;      // the query parts' last 96 bytes: [128 rows x 32 B], 32-byte swizzle, then
+constexpr int kOffQRope = kOffQ + 4096;         // [128 rows x 64 B], 64-byte swizzle
+constexpr int kOffSf = kOffQRope + 8192;     // block scales of P, two units: byte (h % 32) 16 + unit 8 + (h / 32) 4 + half
 constexpr int kOffBar = kOffSf + 512;           // mbarriers
 constexpr int kOffMisc = kOffBar + 256;         // tmem address, abort flag, a set's unit with scores far above its references
-constexpr int kOffSlot = kOffMisc + 16;         // int4 [6] (8 places): of a slot's unit the tokens present (2 words), last of its row
+constexpr int kOffSlot = kOffMisc + 16;         // int4 [5] (8 places): of a slot's unit the tokens present (2 words), last of its row
 constexpr int kOffRing = kOffSlot + 128;        // int4 [8]: the same by unit, as the softmax and the values read it
 constexpr int kOffRef = kOffRing + 128;         // float [64]: the heads' references
 constexpr int kOffRow = kOffRef + 256;          // float [4][64]: maxima and rescale factors, the sums, or maxima of the query
@@ -68,18 +70,18 @@ constexpr int kOffSum = kOffRow + 1024;         // float [64]: bmm2 / l
 constexpr int kOffPlan = kOffSum + 256;         // int32 [52]: the plan's sums and first row
 constexpr int kSmem = kOffPlan + 208;
 static_assert(kOffSlot % 16 == 0 && kOffRow % 16 == 0 && kOffSf % 128 == 0 && kSmem <= 232448, "shared memory");
-// TMEM columns: O^T as 4 tiles of 128 dims x 64 heads; S, 64 tokens; the query parts, 576 bytes a lane; block scales of V
-// (2^-7 against the high parts of P, 2^-11 against the low ones) and of P (2 columns a unit). Lanes 32 i + l of S and the
+// TMEM columns: O^T as 4 tiles of 128 dims x 64 heads; S of two units, 64 tokens each; the first 480 bytes of the query
+// parts; block scales of V (byte 0, 2^-7, against the high parts of P, byte 1, 2^-11, against the low ones) and of P (2
+// columns a unit): all 512. Lanes 32 i + l of S and the
 // query parts: the high part of head 16 i + l, l < 16, the low part of head 16 i + l - 16 above
-constexpr uint32_t kColO = 0, kColS = 256, kColQ = 320, kColV = 464, kColLow = 468, kColP = 472;
+constexpr uint32_t kColO = 0, kColS = 256, kColQ = 384, kColV = 504, kColP = 508;
 constexpr float kMaxRise = 64.0f;               // base-2 scores above a head's reference before it moves and O is rescaled
 constexpr float kMinE = -100.0f;                // the least exponent of a block
-constexpr int kYield = 40;                      // looks at the score warp before the values go ahead (about 30 cycles each)
 enum : int32_t { kMore = 0, kLast = 1, kEnd = 2 };     // a unit, the last unit of its row, no unit: the row has ended
-constexpr uint32_t kSw128 = 2, kSw64 = 4;       // descriptor layout types
+constexpr uint32_t kSw128 = 2, kSw64 = 4, kSw32 = 6;       // descriptor layout types
 
 // Block-scaled instruction descriptor (kind::mxf8f6f4): e4m3 A and B (format 0), ue8m0 scales (bit 23), A
-// MN-major (bit 15), B K-major, N >> 3 in [17,23), M >> 4 in [24,29), B's scale byte in [4,6).
+// MN-major (bit 15), B K-major, N >> 3 in [17,23), M >> 4 in [24,29), B's scale byte in [4,6), A's in [29,31).
 __host__ __device__ constexpr uint32_t idesc_mx(int M, int N) {
   return (1u << 15) | (static_cast<uint32_t>(N >> 3) << 17) | (1u << 23) |
          (static_cast<uint32_t>(M >> 4) << 24);
@@ -204,9 +206,10 @@ SSB_DEVICE void split2_bf16(uint32_t v, uint32_t& hi, uint32_t& lo) {
 }
 // Byte offset of 16-byte granule g of row r: a 128-byte-swizzled chunk, a 64-byte-swizzled one.
 SSB_DEVICE uint32_t sw128(int r, int g) { return r * 128 + ((g ^ (r & 7)) << 4); }
+SSB_DEVICE uint32_t sw32(int r, int g) { return r * 32 + ((g ^ ((r >> 2) & 1)) << 4); }
 SSB_DEVICE uint32_t sw64(int r, int g) { return r * 64 + ((g ^ ((r >> 1) & 3)) << 4); }
 // ---- barriers -----------------------------------------------------------------------------------------------------
-struct Bars {                                    // slots: full, empty; sets: s_full, p_full, pv_done, agree, ref_ok, slow
+struct Bars {                                    // slots: full, empty; sets: s_full, s_empty, p_full, pv_done, agree, ref_ok, slow
   uint32_t full, empty, q_full, s_full, s_empty, p_full, pv_done, o_full, o_free, drain, agree, ref_ok, slow;
 };
 // mbar_wait whose second and later tries are out of line: the many waits stay short in the instruction cache.
@@ -344,21 +347,27 @@ SSB_DEVICE float2* part_ml(const MlaDecodeArgs& a, int tile, int slot) {
 SSB_DEVICE void issue_scores(const Bars& B, uint32_t sbase, int slot, int set, bool leader) {
   constexpr uint32_t idesc = idesc_e4m3(128, kUnit);                 // S [query parts, tokens] = Q K^T
   uint64_t bd = smem_desc(sbase + kOffKv + slot * kLat, 0, 1024, kSw128);
+  const uint32_t S = kColS + kUnit * set;
   uint32_t q = kColQ, acc = 0;
 #pragma unroll 1
-  for (int c = 0; c < 4; ++c) {
+  for (int c = 0; c < 3; ++c) {
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-      if (leader) tc_mma_f8_ta(kColS, q + 8 * ks, bd + 2 * ks, idesc, acc);
+      if (leader) tc_mma_f8_ta(S, q + 8 * ks, bd + 2 * ks, idesc, acc);
       acc = 1;
     }
     q += 32;
     bd += kChunk >> 4;
   }
+#pragma unroll
+  for (int ks = 0; ks < 3; ++ks)
+    if (leader) tc_mma_f8_ta(S, q + 8 * ks, bd + 2 * ks, idesc, 1u);
+  if (leader) tc_mma_f8(S, smem_desc(sbase + kOffQ, 0, 256, kSw32), bd + 6, idesc, 1u);
+  const uint64_t ar = smem_desc(sbase + kOffQRope, 0, 512, kSw64);
   bd = smem_desc(sbase + kOffRope + slot * kRope, 0, 512, kSw64);
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks)                                     // the rope keys: 64 bytes a row
-    if (leader) tc_mma_f8_ta(kColS, q + 8 * ks, bd + 2 * ks, idesc, 1u);
+    if (leader) tc_mma_f8(S, ar + 2 * ks, bd + 2 * ks, idesc, 1u);
   if (leader) tc_commit(B.s_full + 8 * set);
 }
 SSB_DEVICE void issue_values(const Bars& B, uint32_t sbase, int slot, int set, bool fresh, bool leader) {
@@ -376,7 +385,7 @@ SSB_DEVICE void issue_values(const Bars& B, uint32_t sbase, int slot, int set, b
       const uint32_t id = idesc_mx(128, 64) | (ks << 4);
       if (leader) {
         tc_mma_mx(o, ad + ks * (4096 >> 4), hi0 + 2 * ks, id, acc, kColV, sfp);
-        tc_mma_mx(o, ad + ks * (4096 >> 4), lo0 + 2 * ks, id, 1u, kColLow, sfp);
+        tc_mma_mx(o, ad + ks * (4096 >> 4), lo0 + 2 * ks, id | (1u << 29), 1u, kColV, sfp);
       }
       acc = 1;
     }
@@ -389,7 +398,19 @@ SSB_DEVICE void issue_values(const Bars& B, uint32_t sbase, int slot, int set, b
   }
 }
 
-// One query row's heads h0 .. h0 + 63 as the parts of q 2^-k (k per head, its largest value in [2^7, 2^8)) into TMEM, zero
+// Values 144 part + 16 j .. + 15 of this thread's row of query parts to their place.
+SSB_DEVICE void keep_q(uint8_t* smem, uint32_t to, const uint32_t (&w)[4], int part, int j) {
+  if (part < 3 || j < 3) {
+    tmem_st_4(to, w);
+  } else {
+    const int row = 32 * ((threadIdx.x >> 5) & 3) + (threadIdx.x & 31);
+    uint8_t* at = j < 5 ? smem + kOffQ + sw32(row, j - 3) : smem + kOffQRope + sw64(row, j - 5);
+    *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// One query row's heads h0 .. h0 + 63 as the parts of q 2^-k (k per head, its largest value in [2^7, 2^8)) into TMEM (the
+// last 96 values: shared memory), zero
 // rows past nh. bf16 has 8 significant bits, so the two e4m3 parts hold a value exactly unless it is below 2^-14 of the
 // head's largest (then to 2^-18 of that). First the largest values, 8 threads a head (whole
 // lines); then a thread has half of its lane's head's quarter of the row (lanes l and l + 16 share a head), loaded four
@@ -410,7 +431,7 @@ __device__ __noinline__ int stage_q(const MlaDecodeArgs& a, uint8_t* smem, uint3
     for (int j = 0; j < 9; ++j, to += 4) {                            // 16 values
       const uint4 g = __ldg(q + j);
       const uint32_t w[4] = {keep ? g.x : 0, keep ? g.y : 0, keep ? g.z : 0, keep ? g.w : 0};
-      tmem_st_4(to, w);
+      keep_q(smem, to, w, part, j);
     }
   } else {
     const __nv_bfloat16* base = static_cast<const __nv_bfloat16*>(a.q) + (int64_t)t * a.ldq + (int64_t)h0 * a.hsq;
@@ -459,9 +480,10 @@ __device__ __noinline__ int stage_q(const MlaDecodeArgs& a, uint8_t* smem, uint3
       const uint32_t r01 = __shfl_xor_sync(0xffffffffu, high ? l01 : h01, 16);
       const uint32_t r23 = __shfl_xor_sync(0xffffffffu, high ? l23 : h23, 16);
       const uint32_t w[4] = {high ? h01 : r01, high ? h23 : r23, high ? r01 : l01, high ? r23 : l23};
-      tmem_st_4(to, w);
+      keep_q(smem, to, w, part, j);
     }
   }
+  fence_proxy_async_smem();
   tmem_st_wait();
   return k;
 }
@@ -475,14 +497,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int cta = blockIdx.x, tile = blockIdx.y;
   const int h0 = tile * kTileH, nh = min(kTileH, a.H - h0);
   const uint32_t sbase = smem_u32(smem), bar = sbase + kOffBar;
-  const Bars B = {bar,       bar + 48,  bar + 96,  bar + 104, bar + 120, bar + 128, bar + 144,
-                  bar + 160, bar + 168, bar + 176, bar + 184, bar + 200, bar + 216};
+  const Bars B = {bar,       bar + 40,  bar + 80,  bar + 88,  bar + 104, bar + 120, bar + 136,
+                  bar + 152, bar + 160, bar + 168, bar + 176, bar + 192, bar + 208};
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kOffMisc);
   volatile int32_t* abort_flag = reinterpret_cast<volatile int32_t*>(smem + kOffMisc + 4);
   volatile int32_t* far = reinterpret_cast<volatile int32_t*>(smem + kOffMisc + 8);           // [2]
   int4* slots = reinterpret_cast<int4*>(smem + kOffSlot);
   int4* ring = reinterpret_cast<int4*>(smem + kOffRing);
-  volatile int32_t* scoring = reinterpret_cast<volatile int32_t*>(smem + kOffSlot + 96);    // the score warp has rows to issue
   if (sbase & 1023) {                                    // the swizzled tiles need it; no static shared memory precedes
     if (tid == 0) raise_status(a.status, kErrCuda);
     return;
@@ -490,15 +511,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   asm volatile("griddepcontrol.launch_dependents;");     // the join may be set up meanwhile (it waits for this grid's end)
   if (warp == kScoreWarp) {
-    if (lane < 29) {                                     // the barriers, one a lane
+    if (lane < 28) {                                     // the barriers, one a lane
       // full: every gather lane's copies and a warp's word
-      const uint32_t n = lane < 6 ? 132 : lane < 12 ? 1 : lane == 12 || lane == 21 ? kSoftWarps : lane < 15 ? 2
-                         : lane < 18 ? kSetWarps : lane < 21 ? 1 : lane == 22 ? 2 : kSetWarps;
+      const uint32_t n = lane < 5 ? 132 : lane < 10 ? 1 : lane == 10 || lane == 20 ? kSoftWarps : lane < 13 ? 2
+                         : lane < 17 ? kSetWarps : lane < 20 ? 1 : lane == 21 ? 2 : kSetWarps;
       mbar_init(bar + 8 * lane, n);
     }
     if (lane < 2) far[lane] = 0;
     if (lane == 2) *abort_flag = 0;
-    if (lane == 3) *scoring = 0;
     fence_barrier_init();
   } else if (warp == kValueWarp) {
     tmem_alloc(smem_u32(tmem_slot), 512);
@@ -525,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // chunk w (warp 3 also the rope keys); otherwise of tokens 32 (w & 1) .. + 31 the chunks 2 (w >> 1), + 1 and half the rope
     const int w = warp - kGatherWarp, half = w & 1, pair = w >> 1;
     const int cols = a.indices != nullptr ? (a.n_idx + kUnit - 1) / kUnit : 0;
-    int slot = 0, round = 0;                             // unit u's slot u % 6, and u / 6
+    int slot = 0, round = 0;                             // unit u's slot u % kSlots, and u / kSlots
     Segment s;
     bool ok = true;
     while (ok && walk_next(a, walk, s)) {
@@ -577,7 +597,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int64_t row = (int64_t)page * kPage + (p & (kPage - 1));
         const int from = page >= 0 && row < a.cache_rows ? static_cast<int>(row) : -1;
         const uint32_t present = __ballot_sync(0xffffffffu, from >= 0);
-        // the slot is free when the values of the unit six before have used it (its words were read before its scores)
+        // the slot is free when the values of the unit kSlots before have used it (its words were read before its scores)
         if (round > 0) ok = mbar_nap(B.empty + 8 * slot, (round - 1) & 1, abort_flag, a.status);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -642,8 +662,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         last = ring[u & 7].z != kMore;
-        // scores first, where their rows are there: the values then run while S is read and handed back
-        for (int i = 0; i < kYield && *scoring != 0; ++i) {}
         tc_fence_after();
         issue_values(B, sbase, slot, set, fresh, leader);
         fresh = false;
@@ -661,19 +679,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     Segment s;
     bool ok = true;
     while (ok && walk_next(a, walk, s)) {
-      bool last = false, started = false;
+      bool last = false;
+      const int first = u;
       while (!last) {
         ok = mbar_nap(B.full + 8 * slot, round & 1, abort_flag, a.status);
-        if (leader) *scoring = 1;
-        if (ok && u > 0) ok = mbar_nap(B.s_empty, (u - 1) & 1, abort_flag, a.status);
-        if (ok && !started) ok = mbar_nap(B.q_full, seg & 1, abort_flag, a.status);
-        started = true;
+        if (ok && u > 1) ok = mbar_nap(B.s_empty + 8 * (u & 1), ((u >> 1) - 1) & 1, abort_flag, a.status);
+        if (ok && u == first) ok = mbar_nap(B.q_full, seg & 1, abort_flag, a.status);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         fence_proxy_async_smem();                        // rows that threads copied -> the tensor core
         tc_fence_after();
-        // the unit's words, by unit: entry u & 7 was last read for the values of unit u - 8, which are done (the set of unit
-        // u - 3 waited for those of u - 5 before it gave its weights)
+        // the unit's words, by unit: entry u & 7 was last read for the values of unit u - 8, which are done (the set that
+        // has read S of u - 2 waited for those of u - 6 before it gave the weights of u - 4)
         const int4 word = slots[slot];
         last = word.z != kMore;
         if (leader) {
@@ -681,11 +698,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive(B.s_full + 8 * (u & 1));
         }
         issue_scores(B, sbase, slot, u & 1, leader);
-        if (leader) *scoring = 0;
         ++u;
         if (++slot == kSlots) slot = 0, ++round;
       }
-      if (ok && leader) {                                // the set that has no further unit of the row is told so
+      // the set that has no further unit of the row is told so, once it has read its last one
+      if (ok && u > first + 1) ok = mbar_nap(B.s_empty + 8 * (u & 1), ((u >> 1) - 1) & 1, abort_flag, a.status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok && leader) {
         ring[u & 7] = make_int4(0, 0, kEnd, 0);
         mbar_arrive_n(B.s_full + 8 * (u & 1), 2);
       }
@@ -705,7 +724,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     float* sums = reinterpret_cast<float*>(smem + kOffSum);
     const uint32_t other = 8 * (set ^ 1), own = 8 * set;
     const bool teller = warp < 4 && lane < 16;           // one thread a head
-    if (warp < 8) tmem_st_x4(tq + (warp < 4 ? kColV : kColLow), warp < 4 ? 0x78787878u : 0x74747474u);
+    if (warp < 4) tmem_st_x4(tq + kColV, 0x7478u);
     int u0 = 0, seg = 0, events = 0;                     // the row's first unit
     Segment s;
     bool more = walk_next(a, walk, s), ok = true;
@@ -733,10 +752,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         float v[16];                                     // base-2 scores; tokens not there: -inf
         {
           float x[32];
-          tmem_ld_32x32b_x32(tq + kColS + 32 * half, x);
+          tmem_ld_32x32b_x32(tq + kColS + kUnit * set + 32 * half, x);
           tmem_ld_wait();
           tc_fence_before();
-          warp_arrive(B.s_empty, lane);
+          warp_arrive(B.s_empty + own, lane);
           // lanes l and l + 16 have the high and the low part of 32 tokens: each gives the other the half that it does not keep
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
