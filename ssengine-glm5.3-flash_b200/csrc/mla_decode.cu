@@ -3,30 +3,38 @@
 //
 //   s_j = bmm1 q[t, h, :] . kv[slot_j, :]   (576 values);   out[t, h, :] = bmm2 sum_j softmax(s)_j kv[slot_j, 0:512]
 //
-// Split: a row of n tokens is ceil(n / 128) units of work; the units of all rows, in row order, are cut into equal
+// Split: a row of n tokens is ceil(n / 64) units of work; the units of all rows, in row order, are cut into equal
 // contiguous ranges, one per CTA (two rows or more may share a CTA, one row may span many). A CTA works through its
 // range row by row; a row that lies in one range is finished there, the parts of a row cut between ranges go to the
 // workspace as (reference m, sum l, unnormalised O) in fp32 and are joined by a second kernel:
 //   M = max_i m_i;  O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.
 // No atomics and a fixed order of the sums: the same inputs give the same bits.
 //
-// One CTA of 22 warps an SM, over units of 128 tokens and a tile of 64 heads:
-//   gather (4 warps): a whole page as TMA tiles (4 chunks [128 tokens x 128 B] and the rope keys), a row's last page and
-//       selected tokens by cp.async row by row, what is not there zero-filled;
-//   scores (1 warp issues): S^T [128 tokens x 64 heads] = K Q^T, tcgen05 kind::f8f6f4, M = 128. bf16 queries enter
-//       exactly, as two e4m3 parts (64 high rows, 64 low ones, N = 128): the half of the tensor core that 64 heads alone
-//       would leave idle;
-//   softmax (16 warps, a token and 16 heads a thread): weights 2^(s - E), E one exponent for 32 tokens x 4 heads, again
+// One CTA of 22 warps an SM, over units of 64 tokens and a tile of 64 heads:
+//   gather (4 warps): a whole unit of a page as TMA tiles (4 chunks [64 tokens x 128 B] and the rope keys), a row's last
+//       units and selected tokens by cp.async row by row, what is not there zero-filled; five units in flight;
+//   scores (1 warp issues): S [128 query parts x 64 tokens] = Q K^T, tcgen05 kind::f8f6f4. bf16 queries enter exactly, as
+//       two e4m3 parts (64 high rows, 64 low ones): the half of the tensor core that 64 heads alone would leave idle.
+//       Q stands in TMEM, which has room for all but 96 bytes a row;
+//   softmax (2 sets of 8 warps, every second unit each; 16 tokens of one head a thread): the high and low parts of a head
+//       are 16 lanes apart and change places by shuffles. Weights 2^(s - E), E one exponent for a head's 32 tokens, again
 //       as two e4m3 parts (8 bits), with 2^E as the ue8m0 block scale of the second product. The accumulators stand
-//       against a reference per head that moves only when scores rise 2^4 above it;
+//       against a reference per head, which the sets hand on from unit to unit and which moves only when scores rise 2^64
+//       above it;
 //   values (1 warp issues): O^T [512 dims x 64 heads] += V^T P^T, kind::mxf8f6f4, 4 tiles of M = 128, N = 64, from the same
 //       rows read the other way round.
-// TMEM: O^T 256 columns, S^T 128, block scales. Shared memory: query parts 72 KB, two units' rows 2 x 72 KB (the high parts
-// of P take the place of the rope keys, which only the scores need), the low parts of P 8 KB.
-// Bounds: 576 bytes a token from HBM against 64 x 2,176 products of 8 bits: 2,700 cycles a unit at the measured copy
-// rate, and as many for the two products, which read shared memory at its full rate (18 instructions of 64 cycles, 32 of
-// 48). One thread's instruction stream matters as much: the roles' loops are kept small because they share 28 KB of
-// instruction cache.
+// TMEM: O^T 256 columns, S of two units 128, Q 120, block scales 8. Shared memory: five units' rows 5 x 36 KB (the high
+// parts of P take the place of the rope keys, which only the scores need), the low parts of P 2 x 4 KB, the end of Q 12 KB.
+// Bounds: 576 bytes a token from HBM against 128 x 576 + 2 x 64 x 512 products of 8 bits: 1,350 cycles a unit at the
+// measured copy rate, and as many for the two products (18 instructions of 32 cycles, 16 of 48, which read shared memory at
+// its full rate). A unit takes about 1,700 cycles. Measured, bf16 queries, 64 heads: 64 rows x 32,768 tokens in 300 us
+// (4.1 TB/s of cache), where the card is at its power limit (the clock falls to 1.4 GHz and the time to 378 us when the call is
+// repeated for seconds); 32 rows of 128 to 32,768 tokens 80 us; 1 x 131,072 tokens 41 us; 1 x 1,000 tokens 18 us, of which
+// the plan is 1.3, the query's staging 5.5, the unit and its products 4.5, the parts' stores 2.3 and the join 4.
+// Measured against it: units of 128 tokens in two slots with a token and 16 heads a thread, whose block maxima need warp
+// reductions, 380 us at 64 x 32,768; one warp issuing both products 356 (one thread issues an instruction every 50 cycles,
+// two threads one every 39); S of one unit 312. The roles' loops are kept small because they share 28 KB of instruction
+// cache: unrolled in full they took 511 us where rolled ones took 485.
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -62,7 +70,7 @@ constexpr int kOffQRope = kOffQ + 4096;         // [128 rows x 64 B], 64-byte sw
 constexpr int kOffSf = kOffQRope + 8192;     // block scales of P, two units: byte (h % 32) 16 + unit 8 + (h / 32) 4 + half
 constexpr int kOffBar = kOffSf + 512;           // mbarriers
 constexpr int kOffMisc = kOffBar + 256;         // tmem address, abort flag, a set's unit with scores far above its references
-constexpr int kOffSlot = kOffMisc + 16;         // int4 [5] (8 places): of a slot's unit the tokens present (2 words), last of its row
+constexpr int kOffSlot = kOffMisc + 16;         // int4 [5] (8 places): a unit's tokens present (2 words), kLast or not
 constexpr int kOffRing = kOffSlot + 128;        // int4 [8]: the same by unit, as the softmax and the values read it
 constexpr int kOffRef = kOffRing + 128;         // float [64]: the heads' references
 constexpr int kOffRow = kOffRef + 256;          // float [4][64]: maxima and rescale factors, the sums, or maxima of the query
@@ -197,7 +205,8 @@ SSB_DEVICE void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
   lo = half2_e4m3(__hmul2(__hsub2(v, e4m3_half2(hi)), __float2half2_rn(16.0f)));
 }
 // The same of two halves with 8 significant bits: hi has the leading 4, lo exactly the others (a value below 2^-6, where hi
-// loses bits, is off by 2^-10 at most). Half the conversions of `split2`, which run at a sixteenth of the arithmetic's rate.
+// loses bits, is off by 2^-10 at most). Half the conversions
+// of `split2`.
 SSB_DEVICE void split2_bf16(uint32_t v, uint32_t& hi, uint32_t& lo) {
   const uint32_t h = v & 0xFF80FF80u;
   const __half2 a = *reinterpret_cast<const __half2*>(&v), b = *reinterpret_cast<const __half2*>(&h);
@@ -209,7 +218,7 @@ SSB_DEVICE uint32_t sw128(int r, int g) { return r * 128 + ((g ^ (r & 7)) << 4);
 SSB_DEVICE uint32_t sw32(int r, int g) { return r * 32 + ((g ^ ((r >> 2) & 1)) << 4); }
 SSB_DEVICE uint32_t sw64(int r, int g) { return r * 64 + ((g ^ ((r >> 1) & 3)) << 4); }
 // ---- barriers -----------------------------------------------------------------------------------------------------
-struct Bars {                                    // slots: full, empty; sets: s_full, s_empty, p_full, pv_done, agree, ref_ok, slow
+struct Bars {                                    // full, empty: a slot each; s_*, p_full, pv_done, agree, ref_ok, slow: a set
   uint32_t full, empty, q_full, s_full, s_empty, p_full, pv_done, o_full, o_free, drain, agree, ref_ok, slow;
 };
 // mbar_wait whose second and later tries are out of line: the many waits stay short in the instruction cache.
@@ -253,8 +262,9 @@ SSB_DEVICE int row_units(const MlaDecodeArgs& a, int t) {
 struct Segment {
   int t, b0, b1, nb;
 };
-// Ranges are cut in units plus `cost` for every row that has any (a row's staging, drain and epilogue take a CTA about as
-// long as four units; none where a range is a few units and every cut row would lose more).
+// Ranges are cut in units plus `cost` for every row that has any: a row's staging, drain and epilogue take a CTA about as
+// long as ten units (32 ragged rows: 85 us at a cost of 4, 80 at 10), none where a range is few units and every cut row
+// would lose more (96 selected rows, 21 units a range: 75 us with the cost, 72 without).
 struct Walk {
   int t, nb, first, lo, hi, cost;               // next row, its units, the units and costs before it, the range, the cost
 };
@@ -293,6 +303,7 @@ SSB_DEVICE bool find_range(const MlaDecodeArgs& a, int cta, int ctas, int32_t* s
   units = __reduce_add_sync(0xffffffffu, lane < kThreads / 32 ? sh[lane] : 0);
   rows = __reduce_add_sync(0xffffffffu, lane < kThreads / 32 ? sh[24 + lane] : 0);
   // every range in use holds a unit: a row's CTAs are consecutive. A few short rows are not cut finer than two units
+  // (a selected row of 2,051 tokens: 19.8 us in single units, 19.0 in pairs)
   const int used = min(ctas, max(rows, (units + 1) / 2));
   if (cta >= used) return false;
   w.cost = units >= kCostFrom * ctas ? kRowCost : 0;
@@ -474,7 +485,8 @@ __device__ __noinline__ int stage_q(const MlaDecodeArgs& a, uint8_t* smem, uint3
       uint32_t hi[4], lo[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        split2_bf16((__viaddmax_s16x2_relu(v[i] & 0x7FFF7FFFu, down, 0u) << 3 | (v[i] & 0x80008000u) | bad) & keep, hi[i], lo[i]);
+        split2_bf16((__viaddmax_s16x2_relu(v[i] & 0x7FFF7FFFu, down, 0u) << 3 | (v[i] & 0x80008000u) | bad) & keep,
+                    hi[i], lo[i]);
       const uint32_t h01 = hi[0] | (hi[1] << 16), h23 = hi[2] | (hi[3] << 16);
       const uint32_t l01 = lo[0] | (lo[1] << 16), l23 = lo[2] | (lo[3] << 16);
       const uint32_t r01 = __shfl_xor_sync(0xffffffffu, high ? l01 : h01, 16);
@@ -729,7 +741,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     Segment s;
     bool more = walk_next(a, walk, s), ok = true;
     if (teller) refs[mine] = mine < nh ? kNone : 0.0f;
-    int k = stage_q<Q8>(a, smem, tmem, s.t, h0, nh);     // the query scale's exponent of head mine (also waits for the scales' stores)
+    int k = stage_q<Q8>(a, smem, tmem, s.t, h0, nh);     // exponent of head mine's query scale
     tc_fence_before();
     warp_arrive(B.q_full, lane);
     named_bar(5, kSoftmax);                              // every head's reference is written
@@ -902,7 +914,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (teller) {
         if (!whole) part_ml(a, tile, slot)[mine] = make_float2(ref, total);
         else if (a.lse != nullptr && mine < nh)
-          a.lse[(int64_t)done.t * a.H + h0 + mine] = total == 0.0f ? kNone : ((ref == kNone ? 0.0f : ref) + log2f(total)) * kLn2;
+          a.lse[(int64_t)done.t * a.H + h0 + mine] =
+              total == 0.0f ? kNone : ((ref == kNone ? 0.0f : ref) + log2f(total)) * kLn2;
         if (mine == 0 && tile == 0) {
           if (done.b0 == 0) a.rows[done.t].first = cta, a.rows[done.t].first_slot = slot;
           if (done.b1 == done.nb) a.rows[done.t].last = cta;
@@ -955,12 +968,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins a row's parts. gridDim.z == 4: one CTA per (row, head, 128 output values), warp w taking parts w, w + 4, ...;
-// gridDim.z == 1: one per (row, head), a warp 128 values and all the parts (chosen by the number of CTAs, below). Rows
-// that one CTA finished, or that have no token, are left alone.
-__global__ void __launch_bounds__(128) mla_join_kernel(const __grid_constant__ MlaDecodeArgs a) {
-  __shared__ float4 so[4][32];
-  __shared__ float sl[4];
+// Joins a row's parts. gridDim.z == 4: one CTA of W = 4 or 16 warps per (row, head, 128 output values), warp w taking parts
+// w, w + W, ...; gridDim.z == 1: one of 4 warps per (row, head), a warp 128 values and all the parts (chosen by the
+// number of CTAs, below). Rows that one CTA finished, or that have no token, are left alone.
+constexpr int kJoinWarps = 16;
+__global__ void __launch_bounds__(32 * kJoinWarps) mla_join_kernel(const __grid_constant__ MlaDecodeArgs a) {
+  __shared__ float4 so[kJoinWarps][32];
+  __shared__ float sl[kJoinWarps];
   const int64_t t = blockIdx.x;
   const int h = blockIdx.y, tile = h / kTileH, hh = h - tile * kTileH;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -970,7 +984,8 @@ __global__ void __launch_bounds__(128) mla_join_kernel(const __grid_constant__ M
   const MlaRowParts rp = a.rows[t];
   if (rp.first == rp.last) return;
   const bool spread = gridDim.z == 4;
-  const int parts = rp.last - rp.first + 1, step = spread ? 4 : 1, dim = 128 * (spread ? blockIdx.z : warp);
+  const int parts = rp.last - rp.first + 1, dim = 128 * (spread ? blockIdx.z : warp);
+  const int step = spread ? static_cast<int>(blockDim.x) / 32 : 1;
   auto slot_of = [&](int i) { return i == 0 ? rp.first_slot : 2 * (rp.first + i); };
   float m = kNone;
   for (int i = lane; i < parts; i += 32) m = fmaxf(m, part_ml(a, tile, slot_of(i))[hh].x);
@@ -993,9 +1008,10 @@ __global__ void __launch_bounds__(128) mla_join_kernel(const __grid_constant__ M
     if (lane == 0) sl[warp] = l;
     __syncthreads();
     if (warp != 0) return;
-    l = sl[0] + sl[1] + sl[2] + sl[3];
-#pragma unroll
-    for (int w = 1; w < 4; ++w) {
+    const int warps = min(parts, step);
+#pragma unroll 4
+    for (int w = 1; w < warps; ++w) {
+      l += sl[w];
       const float4 v = so[w][lane];
       s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
     }
@@ -1026,7 +1042,8 @@ int launch_mla_decode(const MlaDecodeArgs& a_in, void* ws, int64_t ws_bytes, cud
       (a.indices != nullptr && (a.n_idx < 0 || a.ld_idx < a.n_idx)) || (a.reqs == nullptr && a.T > a.R))
     return kErrArgs;
   if (a.T == 0) return kOk;
-  const int64_t most = a.indices != nullptr ? (a.n_idx + kUnit - 1) / kUnit : (int64_t)(kPage / kUnit) * a.width;   // units of a row
+  const int64_t most =                                   // units of a row
+      a.indices != nullptr ? (a.n_idx + kUnit - 1) / kUnit : (int64_t)(kPage / kUnit) * a.width;
   if (a.T * (most + kRowCost) > 0x7fffffff) return kErrArgs;
   if (a.q == nullptr || a.kv == nullptr || a.table == nullptr || a.out == nullptr || ws == nullptr ||
       !aligned(a.q, 16) || !aligned(a.kv, 16) || !aligned(a.out, 16) || !aligned(ws, 256) || (a.ldq * eb) % 16 ||
@@ -1053,11 +1070,13 @@ int launch_mla_decode(const MlaDecodeArgs& a_in, void* ws, int64_t ws_bytes, cud
   if (rc != kOk) return rc;
   kernel<<<dim3((unsigned)(kMaxCtas / tiles), (unsigned)tiles), kThreads, kSmem, stream>>>(mlat, mrope, a);
   if (cudaGetLastError() != cudaSuccess) return kErrCuda;
-  // few rows are cut into many parts each: their CTAs are spread over the parts and the output values
+  // few rows are cut into many parts each: their CTAs are spread over the parts and the output values. 64 heads, 1 x 131,072
+  // tokens: 82 us in all with one CTA a head, 49 with four, 41 with four of 16 warps; 48 rows of 16 heads: 52, 51 and 60;
+  // 96 rows of 64: 64 with one, 80 with four
   const unsigned z = a.T * a.H <= 8 * kMaxCtas ? 4 : 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.T, (unsigned)a.H, z);
-  cfg.blockDim = dim3(128);
+  cfg.blockDim = dim3(a.T * a.H <= kMaxCtas ? 32 * kJoinWarps : 128);
   cfg.stream = stream;
   cudaLaunchAttribute early;
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
