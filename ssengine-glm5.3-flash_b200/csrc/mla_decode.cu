@@ -4,8 +4,8 @@
 //   s_j = bmm1 q[t, h, :] . kv[slot_j, :]   (576 values);   out[t, h, :] = bmm2 sum_j softmax(s)_j kv[slot_j, 0:512]
 //
 // Split: a row of n tokens is ceil(n / 64) units of work; the units of all rows, in row order, are cut into equal
-// contiguous ranges, one per CTA (two rows or more may share a CTA, one row may span many). A CTA works through its
-// range row by row; a row that lies in one range is finished there, the parts of a row cut between ranges go to the
+// contiguous ranges, one per CTA (two rows or more may share a CTA, one row may span many), or, where rows are few or
+// short, each row into parts of its own. A CTA works through its range row by row; a row that lies in one range is finished there, the parts of a row cut between ranges go to the
 // workspace as (reference m, sum l, unnormalised O) in fp32 and are joined by a second kernel:
 //   M = max_i m_i;  O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.
 // No atomics and a fixed order of the sums: the same inputs give the same bits.
@@ -286,7 +286,12 @@ __device__ __noinline__ bool walk_next(const MlaDecodeArgs& a, Walk& w, Segment&
 constexpr int kRowCost = 10, kCostFrom = 24;      // units; ranges of so many units or more bear it
 
 // All threads of the CTA: its range and the row that holds its beginning. sh: 48 words for the warps' sums, 4 for the row.
-// False: more CTAs than units, nothing to do here.
+// False: more CTAs than work, nothing to do here. Where rows are few or short, every row is cut by itself into parts of at
+// most `per` units, one a CTA: sum_r ceil(u_r / per) <= units / per + rows CTAs suffice, which fixes `per`. That leaves some
+// CTAs out, but each begins one row, where a CTA of equal ranges begins 1 + rows / ctas on average and two or more at
+// worst; it is taken where `per` exceeds the equal share by less than those beginnings cost. 34 rows x 1,853 tokens: 38 us
+// in equal ranges, 28 in parts; 62 rows of 2,051 selected tokens: 39 and 35; on the other side 41 rows (median 6,427
+// tokens, 32 heads): 69 and 77; 48 rows (median 4,096, 16 heads): 50 and 59.
 SSB_DEVICE bool find_range(const MlaDecodeArgs& a, int cta, int ctas, int32_t* sh, Walk& w) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int units = 0, rows = 0;
@@ -299,22 +304,28 @@ SSB_DEVICE bool find_range(const MlaDecodeArgs& a, int cta, int ctas, int32_t* s
   units = __reduce_add_sync(0xffffffffu, units);
   rows = __reduce_add_sync(0xffffffffu, rows);
   if (lane == 0) sh[warp] = units, sh[24 + warp] = rows;
+  if (tid == 0) sh[48] = -1;
   __syncthreads();
   units = __reduce_add_sync(0xffffffffu, lane < kThreads / 32 ? sh[lane] : 0);
   rows = __reduce_add_sync(0xffffffffu, lane < kThreads / 32 ? sh[24 + lane] : 0);
-  // every range in use holds a unit: a row's CTAs are consecutive. A few short rows are not cut finer than two units
-  // (a selected row of 2,051 tokens: 19.8 us in single units, 19.0 in pairs)
-  const int used = min(ctas, max(rows, (units + 1) / 2));
-  if (cta >= used) return false;
-  w.cost = units >= kCostFrom * ctas ? kRowCost : 0;
-  const int total = units + rows * w.cost, per = total / used, rem = total - per * used;
-  w.lo = cta * per + min(cta, rem);
-  w.hi = w.lo + per + (cta < rem);
+  const int spare = max(ctas - rows, 1), per = max((units + spare - 1) / spare, 2);
+  const bool parts = rows < ctas && per <= units / ctas + kRowCost + kRowCost * rows / ctas;
+  w.cost = units < kCostFrom * ctas ? 0 : kRowCost;
+  if (parts) {
+    w.lo = cta;
+  } else {
+    // every range in use holds a unit: a row's CTAs are consecutive
+    const int used = min(ctas, units);
+    if (cta >= used) return false;
+    const int total = units + rows * w.cost, share = total / used, rem = total - share * used;
+    w.lo = cta * share + min(cta, rem);
+    w.hi = w.lo + share + (cta < rem);
+  }
   if (warp == 0) {
     int base = 0;
 #pragma unroll 1
-    for (int c = 0;; c += 32) {
-      const int t = c + lane, nb = t < a.T ? row_units(a, t) : 0, v = nb > 0 ? nb + w.cost : 0;
+    for (int c = 0; c < a.T; c += 32) {
+      const int t = c + lane, nb = t < a.T ? row_units(a, t) : 0, v = nb == 0 ? 0 : parts ? (nb + per - 1) / per : nb + w.cost;
       int end = v;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -323,13 +334,18 @@ SSB_DEVICE bool find_range(const MlaDecodeArgs& a, int cta, int ctas, int32_t* s
       }
       end += base;
       const bool hit = end - v <= w.lo && w.lo < end;
-      if (hit) sh[48] = t, sh[49] = nb, sh[50] = end - v;
+      if (hit) sh[48] = t, sh[49] = nb, sh[50] = end - v, sh[51] = v;
       base = __shfl_sync(0xffffffffu, end, 31);
       if (__any_sync(0xffffffffu, hit)) break;
     }
   }
   __syncthreads();
   w.t = sh[48], w.nb = sh[49], w.first = sh[50];
+  if (w.t < 0) return false;
+  if (parts) {                                  // one segment, written as a range of the row's own units
+    const int64_t i = cta - w.first, n = sh[51];
+    w.lo = static_cast<int>(w.nb * i / n), w.hi = static_cast<int>(w.nb * (i + 1) / n), w.first = 0;
+  }
   return true;
 }
 
