@@ -397,7 +397,7 @@ SSB_DEVICE void issue_scores(const Bars& B, uint32_t sbase, int slot, int set, b
     if (leader) tc_mma_f8(S, ar + 2 * ks, bd + 2 * ks, idesc, 1u);
   if (leader) tc_commit(B.s_full + 8 * set);
 }
-SSB_DEVICE void issue_values(const Bars& B, uint32_t sbase, int slot, int set, bool fresh, bool leader) {
+SSB_DEVICE void issue_values(const Bars& B, uint32_t sbase, int slot, int set, int heads, bool fresh, bool leader) {
   uint64_t ad = smem_desc(sbase + kOffKv + slot * kLat, kChunk, 1024, kSw128);    // O^T [dims, heads] (+)= V^T P^T
   const uint64_t hi0 = smem_desc(sbase + kOffRope + slot * kRope, 0, 512, kSw64);
   const uint64_t lo0 = smem_desc(sbase + kOffPlo + set * kRope, 0, 512, kSw64);
@@ -409,7 +409,7 @@ SSB_DEVICE void issue_values(const Bars& B, uint32_t sbase, int slot, int set, b
     uint32_t acc = fresh ? 0u : 1u;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {                                 // 32 tokens a step: one block of scales
-      const uint32_t id = idesc_mx(128, 64) | (ks << 4);
+      const uint32_t id = idesc_mx(128, 0) | (static_cast<uint32_t>(heads >> 3) << 17) | (ks << 4);
       if (leader) {
         tc_mma_mx(o, ad + ks * (4096 >> 4), hi0 + 2 * ks, id, acc, kColV, sfp);
         tc_mma_mx(o, ad + ks * (4096 >> 4), lo0 + 2 * ks, id | (1u << 29), 1u, kColV, sfp);
@@ -691,7 +691,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         last = ring[u & 7].z != kMore;
         tc_fence_after();
-        issue_values(B, sbase, slot, set, fresh, leader);
+        issue_values(B, sbase, slot, set, (nh + 15) & ~15, fresh, leader);
         fresh = false;
         ++u;
         if (++slot == kSlots) slot = 0;
