@@ -39,10 +39,12 @@ def seq_table(seqs, device) -> torch.Tensor:
 
 def _row_pitch(name: str, t: torch.Tensor, rows: int, cols: int) -> int:
     """The row pitch of a bf16 matrix of at least rows x cols with unit column stride; ValueError otherwise."""
-    if t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape[0] < rows or t.shape[1] < cols or t.stride(1) != 1:
-        raise ValueError(f"{name}: bf16 [{rows}, >= {cols}] with unit column stride, got {t.dtype} {tuple(t.shape)} "
-                         f"strides {t.stride()}")
-    return t.stride(0)
+    if t.dtype is torch.bfloat16 and t.dim() == 2:
+        (n, m), (pitch, unit) = t.shape, t.stride()
+        if n >= rows and m >= cols and unit == 1:
+            return pitch
+    raise ValueError(f"{name}: bf16 [{rows}, >= {cols}] with unit column stride, got {t.dtype} {tuple(t.shape)} strides "
+                     f"{t.stride()}")
 
 
 @dataclass
@@ -58,18 +60,18 @@ class KdaLayer:
         return self.a_log.numel()
 
     def c_struct(self, conv_state: torch.Tensor, rec_state: torch.Tensor) -> lib.KdaLayerC:
-        H = self.heads
-        assert self.conv_weight.dtype == torch.bfloat16 and self.conv_weight.shape == (3 * H * HEAD_DIM, 4)
-        assert self.conv_weight.is_contiguous() and self.a_log.dtype == torch.float32
-        assert self.dt_bias.dtype == torch.float32 and self.dt_bias.numel() == H * HEAD_DIM
+        w, a_log, dt_bias = self.conv_weight, self.a_log, self.dt_bias
+        H = a_log.numel()
+        C = 3 * H * HEAD_DIM
+        assert w.dtype is torch.bfloat16 and w.shape == (C, 4) and w.is_contiguous() and a_log.dtype is torch.float32
+        assert dt_bias.dtype is torch.float32 and dt_bias.numel() == H * HEAD_DIM
         cs, rs = conv_state.stride(), rec_state.stride()
-        assert conv_state.dtype == torch.bfloat16 and conv_state.shape[1:] == (3, 3 * H * HEAD_DIM)
-        assert cs[1:] == (3 * H * HEAD_DIM, 1)
-        assert rec_state.dtype == torch.float32 and rec_state.shape[1:] == (H, HEAD_DIM, HEAD_DIM)
+        (_, taps, cols), (_, heads, dv, dk) = conv_state.shape, rec_state.shape
+        assert conv_state.dtype is torch.bfloat16 and taps == 3 and cols == C and cs[1:] == (C, 1)
+        assert rec_state.dtype is torch.float32 and heads == H and dv == HEAD_DIM and dk == HEAD_DIM
         assert rs[1:] == (HEAD_DIM * HEAD_DIM, HEAD_DIM, 1) or (H == 1 and rs[2:] == (HEAD_DIM, 1))
-        return lib.KdaLayerC(H, HEAD_DIM, self.conv_weight.data_ptr(), self.a_log.data_ptr(), self.dt_bias.data_ptr(),
-                             self.lower_bound, HEAD_DIM ** -0.5, conv_state.data_ptr(), cs[0], rec_state.data_ptr(),
-                             rs[0])
+        return lib.KdaLayerC(H, HEAD_DIM, w.data_ptr(), a_log.data_ptr(), dt_bias.data_ptr(), self.lower_bound,
+                             HEAD_DIM ** -0.5, conv_state.data_ptr(), cs[0], rec_state.data_ptr(), rs[0])
 
     def prefill(self, qkv: torch.Tensor, g: torch.Tensor, beta: torch.Tensor, out: torch.Tensor, seqs: torch.Tensor,
                 conv_state: torch.Tensor, rec_state: torch.Tensor, stream=None, status: torch.Tensor | None = None,
@@ -102,10 +104,11 @@ class KdaLayer:
         sequence are not written. `status` (int32 [1] on the device) receives 1 if a sequence reaches outside the rows
         or names a negative block (it is skipped). Returns `out`."""
         so = lib.load()
-        H = self.heads
-        P, T = H * HEAD_DIM, qkv.shape[0]
-        pitch = [_row_pitch(n, t, T, c) for n, t, c in (("qkv", qkv, 3 * P), ("g", g, P), ("beta", beta, H), ("out", out, P))]
-        if seqs.dtype != torch.int32 or seqs.dim() != 2 or seqs.shape[1] != 4 or not seqs.is_contiguous():
+        H, T = self.a_log.numel(), qkv.shape[0]
+        P = H * HEAD_DIM
+        ldx, ldg = _row_pitch("qkv", qkv, T, 3 * P), _row_pitch("g", g, T, P)
+        ldb, ldo = _row_pitch("beta", beta, T, H), _row_pitch("out", out, T, P)
+        if seqs.dtype is not torch.int32 or seqs.dim() != 2 or seqs.shape[1] != 4 or not seqs.is_contiguous():
             raise ValueError(f"seqs: contiguous int32 [R, 4], got {seqs.dtype} {tuple(seqs.shape)}")
         dev = qkv.get_device()
         for t in (g, beta, out, seqs, conv_state, rec_state, self.conv_weight):
@@ -114,8 +117,8 @@ class KdaLayer:
         if dev < 0:
             raise ValueError(f"the tensors are on {qkv.device}, not on a GPU")
         L = self.c_struct(conv_state, rec_state)
-        rc = so.ssb_kda_decode(ctypes.byref(L), qkv.data_ptr(), pitch[0], g.data_ptr(), pitch[1], beta.data_ptr(),
-                               pitch[2], T, seqs.data_ptr(), seqs.shape[0], out.data_ptr(), pitch[3],
+        rc = so.ssb_kda_decode(ctypes.byref(L), qkv.data_ptr(), ldx, g.data_ptr(), ldg, beta.data_ptr(), ldb, T,
+                               seqs.data_ptr(), seqs.shape[0], out.data_ptr(), ldo,
                                None if status is None else status.data_ptr(), lib.stream_ptr(stream))
         lib.check("ssb_kda_decode", rc)
         return out

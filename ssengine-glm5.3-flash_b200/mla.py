@@ -80,22 +80,27 @@ def decode_selected(q: torch.Tensor, kv_cache: torch.Tensor, indices: torch.Tens
 
 def _decode(q, kv_cache, indices, page_table, seq_lens, bmm1, out, bmm2, n_idx, reqs, lse, workspace, stream, status):
     so = lib.load()
-    if q.dtype not in (torch.bfloat16, torch.uint8) or q.dim() != 3 or q.shape[2] != DQ or q.stride(2) != 1:
+    e4m3 = q.dtype is torch.uint8
+    if not (e4m3 or q.dtype is torch.bfloat16) or q.dim() != 3 or q.shape[2] != DQ or q.stride(2) != 1:
         raise ValueError(f"q: bf16 or e4m3 bytes [T, heads, {DQ}] with unit stride in the last dimension, got {q.dtype} "
                          f"{tuple(q.shape)} strides {q.stride()}")
-    T, H = q.shape[:2]
+    T, H, _ = q.shape
     if kv_cache.dtype != torch.uint8 or kv_cache.dim() != 2 or kv_cache.shape[1] != DQ or not kv_cache.is_contiguous():
         raise ValueError(f"kv_cache: contiguous uint8 [slots, {DQ}], got {kv_cache.dtype} {tuple(kv_cache.shape)}")
     if out.dtype != torch.bfloat16 or out.shape != (T, H, DV) or not out.is_contiguous():
         raise ValueError(f"out: contiguous bf16 {(T, H, DV)}, got {out.dtype} {tuple(out.shape)}")
     if page_table.dtype != torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous():
         raise ValueError(f"page_table: contiguous int32 [R, width], got {page_table.dtype} {tuple(page_table.shape)}")
-    for name, t, dt, shape in (("seq_lens", seq_lens, torch.int32, (T,)), ("reqs", reqs, torch.int32, (T,)),
-                               ("lse", lse, torch.float32, (T, H))):
-        if t is not None and (t.dtype != dt or t.shape != shape or not t.is_contiguous()):
-            raise ValueError(f"{name}: contiguous {dt} {shape}, got {t.dtype} {tuple(t.shape)}")
-    if reqs is None and page_table.shape[0] < T:
-        raise ValueError(f"page_table has {page_table.shape[0]} rows for {T} query rows and no reqs")
+    if seq_lens is not None and (seq_lens.dtype is not torch.int32 or seq_lens.shape != (T,) or
+                                 not seq_lens.is_contiguous()):
+        raise ValueError(f"seq_lens: contiguous int32 {(T,)}, got {seq_lens.dtype} {tuple(seq_lens.shape)}")
+    if reqs is not None and (reqs.dtype is not torch.int32 or reqs.shape != (T,) or not reqs.is_contiguous()):
+        raise ValueError(f"reqs: contiguous int32 {(T,)}, got {reqs.dtype} {tuple(reqs.shape)}")
+    if lse is not None and (lse.dtype is not torch.float32 or lse.shape != (T, H) or not lse.is_contiguous()):
+        raise ValueError(f"lse: contiguous float32 {(T, H)}, got {lse.dtype} {tuple(lse.shape)}")
+    rows, width = page_table.shape
+    if reqs is None and rows < T:
+        raise ValueError(f"page_table has {rows} rows for {T} query rows and no reqs")
     need = decode_workspace_bytes(T, H)
     if workspace is not None and (workspace.dtype != torch.uint8 or not workspace.is_contiguous() or
                                   workspace.numel() < need):
@@ -110,8 +115,7 @@ def _decode(q, kv_cache, indices, page_table, seq_lens, bmm1, out, bmm2, n_idx, 
         workspace = lib.stream_scratch(q.device, need, stream)
     ptr = lambda t: None if t is None else t.data_ptr()
     ldq, head_stride, _ = q.stride()
-    rows, width = page_table.shape
-    rc = so.ssb_mla_decode(q.data_ptr(), int(q.dtype == torch.uint8), ldq, head_stride, T, H, kv_cache.data_ptr(),
+    rc = so.ssb_mla_decode(q.data_ptr(), int(e4m3), ldq, head_stride, T, H, kv_cache.data_ptr(),
                            kv_cache.shape[0], page_table.data_ptr(), rows, width, ptr(reqs), ptr(seq_lens),
                            ptr(indices), 0 if indices is None else indices.stride(0), n_idx or 0, bmm1, bmm2,
                            out.data_ptr(), ptr(lse), workspace.data_ptr(), workspace.numel(), ptr(status),
