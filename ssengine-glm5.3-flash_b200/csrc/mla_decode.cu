@@ -1079,11 +1079,13 @@ int launch_mla_decode(const MlaDecodeArgs& a_in, void* ws, int64_t ws_bytes, cud
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return kErrCuda;
     attr[a.q_e4m3] = true;
   }
-  CUtensorMap mlat, mrope;
-  const int u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
-  int rc = make_map_2d_ex(&mlat, u8, a.kv, a.cache_rows, kDq, kDq, 128, kUnit, CU_TENSOR_MAP_SWIZZLE_128B);
-  if (rc == kOk) rc = make_map_2d_ex(&mrope, u8, a.kv, a.cache_rows, kDq, kDq, 64, kUnit, CU_TENSOR_MAP_SWIZZLE_64B);
-  if (rc != kOk) return rc;
+  CUtensorMap mlat = {}, mrope = {};
+  if (a.indices == nullptr) {                            // selected tokens are copied row by row
+    const int u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    int rc = make_map_2d_ex(&mlat, u8, a.kv, a.cache_rows, kDq, kDq, 128, kUnit, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc == kOk) rc = make_map_2d_ex(&mrope, u8, a.kv, a.cache_rows, kDq, kDq, 64, kUnit, CU_TENSOR_MAP_SWIZZLE_64B);
+    if (rc != kOk) return rc;
+  }
   kernel<<<dim3((unsigned)(kMaxCtas / tiles), (unsigned)tiles), kThreads, kSmem, stream>>>(mlat, mrope, a);
   if (cudaGetLastError() != cudaSuccess) return kErrCuda;
   // few rows are cut into many parts each: their CTAs are spread over the parts and the output values. 64 heads, 1 x 131,072
