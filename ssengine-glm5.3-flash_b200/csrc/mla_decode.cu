@@ -27,14 +27,14 @@
 // parts of P take the place of the rope keys, which only the scores need), the low parts of P 2 x 4 KB, the end of Q 12 KB.
 // Bounds: 576 bytes a token from HBM against 128 x 576 + 2 x 64 x 512 products of 8 bits: 1,350 cycles a unit at the
 // measured copy rate, and as many for the two products (18 instructions of 32 cycles, 16 of 48, which read shared memory at
-// its full rate). A unit takes about 1,700 cycles. Measured, bf16 queries, 64 heads: 64 rows x 32,768 tokens in 300 us
+// its full rate). A unit takes about 1,700 cycles. Measured, bf16 queries, 64 heads: 64 rows x 32,768 tokens in 300 to 320 us
 // (4.1 TB/s of cache), where the card is at its power limit (the clock falls to 1.4 GHz and the time to 378 us when the call is
 // repeated for seconds); 32 rows of 128 to 32,768 tokens 80 us; 1 x 131,072 tokens 41 us; 1 x 1,000 tokens 18 us, of which
 // the plan is 1.3, the query's staging 5.5, the unit and its products 4.5, the parts' stores 2.3 and the join 4.
 // Measured against it: units of 128 tokens in two slots with a token and 16 heads a thread, whose block maxima need warp
-// reductions, 380 us at 64 x 32,768; one warp issuing both products 356 (one thread issues an instruction every 50 cycles,
-// two threads one every 39); S of one unit 312. The roles' loops are kept small because they share 28 KB of instruction
-// cache: unrolled in full they took 511 us where rolled ones took 485.
+// reductions, 380 us at 64 x 32,768; one warp issuing both products 356 (its waits for scores and for weights then
+// follow one another); S of one unit 312. The roles' loops are kept small because they share 28 KB of instruction cache:
+// unrolled in full they took 511 us where rolled ones took 485.
 #include <cuda_fp16.h>
 
 #include "common.cuh"
