@@ -28,7 +28,10 @@ constexpr int kDecThreads = 256;
 constexpr int kRowsW = 16;             // value rows a warp
 
 // e^x as 2^(x log2 e) with the product's rounding error carried to first order: ex2.approx's own error (2^-22) remains.
+// x above 88 counts as 88 (e^x must stay finite, or its correction is inf - inf): as a divisor e^88 makes the quotients
+// below 0, as they are there to 2^-126. NaN stays NaN.
 SSB_DEVICE float exp_fast(float x) {
+  x = x > 88.0f ? 88.0f : x;
   constexpr float kHi = 1.44269502162933349609375f, kLo = 1.925963033500928e-8f;        // log2 e in two parts
   const float t = x * kHi;
   const float r = fmaf(x, kLo, fmaf(x, kHi, -t));
