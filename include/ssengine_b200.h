@@ -279,8 +279,8 @@ int ssb_sparse_mla(const void* q, int64_t T, const void* kv_cache, const int32_t
  * q [T, heads, 576] bf16 (q_e4m3 = 0: its values enter exactly, up to 2^-22 of the head's largest) or e4m3 (1), row
  * stride ldq and head_stride in elements (16-byte multiples). Query row t belongs to row reqs[t] of page_table int32
  * [R, width] (reqs NULL: row t; several rows may share one, e.g. draft tokens) and sees positions 0 .. seq_lens[t] - 1,
- * or, with indices int32 [T, ld_idx], the first n_idx listed positions (-1 = none; at or past seq_lens[t], when that is
- * given: none; a position listed twice counts twice). Tokens of a negative page, past the table or past cache_rows are
+ * or, with indices int32 [T, ld_idx] (not NULL, also where n_idx is 0), the first n_idx listed positions (-1 = none; at or
+ * past seq_lens[t], when that is given: none; a position listed twice counts twice). Tokens of a negative page, past the table or past cache_rows are
  * left out. A row with no token gets zeros and lse -inf; a reqs entry outside [0, R) the same, with status 1. lse (fp32
  * [T, heads] or NULL) = the natural log of the sum of the row's weights. workspace: 256-byte aligned,
  * ssb_mla_decode_workspace_bytes(T, heads) or more (returns 3 when smaller), its contents need not be kept. The lengths

@@ -68,7 +68,8 @@ def decode_selected(q: torch.Tensor, kv_cache: torch.Tensor, indices: torch.Tens
                     status: torch.Tensor | None = None) -> torch.Tensor:
     """`decode` over the positions listed in the first n_idx columns of indices int32 [T, >= n_idx] (the indexer's
     expanded selection; -1 = none), those at or past seq_lens[t] left out when seq_lens is given (it also tells how
-    much work a short row holds, which balances the split)."""
+    much work a short row holds, which balances the split). No column (n_idx 0 or indices [T, 0]): no token, as for
+    any row that has none."""
     if indices.dtype != torch.int32 or indices.dim() != 2 or indices.stride(1) != 1 or indices.shape[0] < q.shape[0]:
         raise ValueError(f"indices: int32 [{q.shape[0]}, n] with unit column stride, got {indices.dtype} "
                          f"{tuple(indices.shape)}")
@@ -115,9 +116,11 @@ def _decode(q, kv_cache, indices, page_table, seq_lens, bmm1, out, bmm2, n_idx, 
         workspace = lib.stream_scratch(q.device, need, stream)
     ptr = lambda t: None if t is None else t.data_ptr()
     ldq, head_stride, _ = q.stride()
+    # a selection without columns has no address of its own (NULL means every visible token): any other one, never read
+    listed = None if indices is None else indices.data_ptr() or page_table.data_ptr()
     rc = so.ssb_mla_decode(q.data_ptr(), int(e4m3), ldq, head_stride, T, H, kv_cache.data_ptr(),
                            kv_cache.shape[0], page_table.data_ptr(), rows, width, ptr(reqs), ptr(seq_lens),
-                           ptr(indices), 0 if indices is None else indices.stride(0), n_idx or 0, bmm1, bmm2,
+                           listed, 0 if indices is None else indices.stride(0), n_idx or 0, bmm1, bmm2,
                            out.data_ptr(), ptr(lse), workspace.data_ptr(), workspace.numel(), ptr(status),
                            lib.stream_ptr(stream))
     lib.check("ssb_mla_decode", rc)
