@@ -274,17 +274,17 @@ int ssb_sparse_mla(const void* q, int64_t T, const void* kv_cache, const int32_t
                    int32_t n_idx, const int32_t* qsl, int32_t R, const int32_t* page_table, int64_t width,
                    float bmm1_scale, float bmm2_scale, void* out, int32_t* status, void* stream);
 
-/* Latent attention of new tokens (a decode step) over the paged FP8 cache, split over each row's tokens and joined:
- * out bf16 [T, heads, 512] = bmm2_scale * softmax(bmm1_scale * q . kv) kv[:, 0:512] as ssb_sparse_mla, for 1..128 heads.
- * q [T, heads, 576] bf16 (q_e4m3 = 0: its values enter exactly, up to 2^-22 of the head's largest) or e4m3 (1), row
- * stride ldq and head_stride in elements (16-byte multiples). Query row t belongs to row reqs[t] of page_table int32
- * [R, width] (reqs NULL: row t; several rows may share one, e.g. draft tokens) and sees positions 0 .. seq_lens[t] - 1,
- * or, with indices int32 [T, ld_idx] (not NULL, also where n_idx is 0), the first n_idx listed positions (-1 = none; at or
- * past seq_lens[t], when that is given: none; a position listed twice counts twice). Tokens of a negative page, past the table or past cache_rows are
- * left out. A row with no token gets zeros and lse -inf; a reqs entry outside [0, R) the same, with status 1. lse (fp32
- * [T, heads] or NULL) = the natural log of the sum of the row's weights. workspace: 256-byte aligned,
- * ssb_mla_decode_workspace_bytes(T, heads) or more (returns 3 when smaller), its contents need not be kept. The lengths
- * are read on the device: the call can be captured in a graph and replayed as they grow. */
+/* Latent attention of new tokens (a decode step) over the paged FP8 cache, split over each row's tokens and joined: out
+ * bf16 [T, heads, 512] = bmm2_scale * softmax(bmm1_scale * q . kv) kv[:, 0:512] as ssb_sparse_mla, for 1..128 heads. q
+ * [T, heads, 576] bf16 (q_e4m3 = 0: its values enter to 2^-21 of the head's largest) or e4m3 (1), row stride ldq and
+ * head_stride in elements (16-byte multiples). Query row t belongs to row reqs[t] of page_table int32 [R, width] (reqs
+ * NULL: row t; several rows may share one, e.g. draft tokens) and sees positions 0 .. seq_lens[t] - 1, or, with indices
+ * int32 [T, ld_idx] (not NULL, also where n_idx is 0), the first n_idx listed positions (-1 = none; at or past
+ * seq_lens[t], when that is given: none; a position listed twice counts twice). Tokens of a negative page, past the
+ * table or past cache_rows are left out. A row with no token gets zeros and lse -inf; a reqs entry outside [0, R) the
+ * same, with status 1. lse (fp32 [T, heads] or NULL) = the natural log of the sum of the row's weights. workspace:
+ * 256-byte aligned, ssb_mla_decode_workspace_bytes(T, heads) or more (returns 3 when smaller), its contents need not be
+ * kept. The lengths are read on the device: the call can be captured in a graph and replayed as they grow. */
 int ssb_mla_decode(const void* q, int32_t q_e4m3, int64_t ldq, int64_t head_stride, int64_t T, int32_t heads,
                    const void* kv_cache, int64_t cache_rows, const int32_t* page_table, int64_t R, int64_t width,
                    const int32_t* reqs, const int32_t* seq_lens, const int32_t* indices, int64_t ld_idx,

@@ -204,12 +204,14 @@ SSB_DEVICE void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
   hi = half2_e4m3(v);
   lo = half2_e4m3(__hmul2(__hsub2(v, e4m3_half2(hi)), __float2half2_rn(16.0f)));
 }
-// The same of two halves with 8 significant bits: hi has the leading 4, lo exactly the others (a value below 2^-6, where hi
-// loses bits, is off by 2^-10 at most). Half the conversions
-// of `split2`.
+// The same of two halves with 8 significant bits: hi has the leading 4, lo exactly the others. Below 2^-6, where e4m3 has a
+// quantum of 2^-9, (h + 3) - 3 rounds h to it (3 + h lies where halves have that quantum; a larger h has no finer bits and
+// comes back unchanged), so that lo has all that hi lost: off by 2^-14 at most, lo's own quantum. Half the conversions of
+// `split2`.
 SSB_DEVICE void split2_bf16(uint32_t v, uint32_t& hi, uint32_t& lo) {
   const uint32_t h = v & 0xFF80FF80u;
-  const __half2 a = *reinterpret_cast<const __half2*>(&v), b = *reinterpret_cast<const __half2*>(&h);
+  const __half2 a = *reinterpret_cast<const __half2*>(&v), three = __float2half2_rn(3.0f);
+  const __half2 b = __hsub2_rn(__hadd2_rn(*reinterpret_cast<const __half2*>(&h), three), three);
   hi = half2_e4m3(b);
   lo = half2_e4m3(__hmul2(__hsub2(a, b), __float2half2_rn(16.0f)));
 }
@@ -437,9 +439,8 @@ SSB_DEVICE void keep_q(uint8_t* smem, uint32_t to, const uint32_t (&w)[4], int p
 }
 
 // One query row's heads h0 .. h0 + 63 as the parts of q 2^-k (k per head, its largest value in [2^7, 2^8)) into TMEM (the
-// last 96 values: shared memory), zero
-// rows past nh. bf16 has 8 significant bits, so the two e4m3 parts hold a value exactly unless it is below 2^-14 of the
-// head's largest (then to 2^-18 of that). First the largest values, 8 threads a head (whole
+// last 96 values: shared memory), zero rows past nh. bf16 has 8 significant bits, so the two e4m3 parts hold a value exactly
+// unless it is below 2^-13 of the head's largest (then to 2^-21 of that). First the largest values, 8 threads a head (whole
 // lines); then a thread has half of its lane's head's quarter of the row (lanes l and l + 16 share a head), loaded four
 // ahead: lane l keeps the high parts, lane l + 16 the low ones, and they exchange the others. e4m3 queries have no low part.
 template <bool Q8>

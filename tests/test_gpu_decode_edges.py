@@ -5,7 +5,8 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_decode import BMM1, Cache, queries
+from oracle import mla as omla
+from test_gpu_decode import BMM1, TOL, Cache, attention64, call, queries
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +31,27 @@ def test_a_selection_without_columns(cuda, form, lengths):
                         torch.from_numpy(cache.table).to(cuda), BMM1, out, n_idx=n, seq_lens=seq, lse=lse)
     torch.cuda.synchronize()
     assert not out.any() and bool((lse == float("-inf")).all())
+
+
+def test_query_values_far_below_their_heads_largest(cuda):
+    """One value of 2^7 a head that meets keys of 0, all others 2^-8 .. 2^-7 (2^-15 of it): the scores are theirs alone.
+    The two parts of such a value are off by at most 2^-14 (2^-21 of the largest), 2^-14 / sqrt(3) on average; over 575
+    keys of variance 1 that is 24 x 3.5e-5 a score. bmm1 makes the scores' spread 1, so that a score is off by
+    24 x 3.5e-5 / (24 x 0.0059) = 0.6 %; the bar is twice that beside the usual one."""
+    rng = np.random.default_rng(67)
+    n, H = 900, 64
+    cache = Cache(rng, [n])
+    kv = omla.e4m3_decode(omla.quantize(rng.standard_normal((n, 576)).astype(np.float32), 1.0))
+    kv[:, 0] = 0.0
+    cache.bytes[cache.slots(0, np.arange(n))] = omla.quantize(kv.astype(np.float32), 1.0)
+    q = rng.uniform(2.0 ** -8, 2.0 ** -7, (1, H, 576)) * rng.choice([-1.0, 1.0], (1, H, 576))
+    q[:, :, 0] = 128.0
+    q = torch.from_numpy(q.astype(np.float32)).to(torch.bfloat16)
+    q64 = q.double().numpy()
+    spread = 24.0 * np.sqrt((q64[0, :, 1:] ** 2).mean())
+    out, _, _ = call(cuda, q, cache, seq_lens=np.array([n], np.int32), bmm1=1.0 / spread)
+    want, _ = attention64(q64[0], kv, 1.0 / spread, 1.0)
+    tol = TOL + 2 * 24.0 * 2.0 ** -14 / np.sqrt(3.0) / spread
+    for h in range(H):
+        err = np.linalg.norm(out[0, h] - want[h]) / np.linalg.norm(want[h])
+        assert err < tol, (h, err, tol)
