@@ -44,7 +44,7 @@ namespace ssb {
 namespace {
 
 constexpr int kDq = 576, kDv = 512, kPage = 128, kUnit = 64, kTileH = 64;
-constexpr int kMaxCtas = 148;                   // ranges a call is cut into at most (the workspace is sized by it)
+constexpr int kMaxCtas = kMlaRanges;            // the workspace is sized by it
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kNone = -INFINITY;
 
@@ -987,7 +987,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // Joins a row's parts. gridDim.z == 4: one CTA of W = 4 or 16 warps per (row, head, 128 output values), warp w taking parts
 // w, w + W, ...; gridDim.z == 1: one of 4 warps per (row, head), a warp 128 values and all the parts (chosen by the
-// number of CTAs, below). Rows that one CTA finished, or that have no token, are left alone.
+// number of CTAs, below). Rows that one CTA finished, or that have no token, are left alone, and those without a valid
+// record: the status tells of them.
 constexpr int kJoinWarps = 16;
 __global__ void __launch_bounds__(32 * kJoinWarps) mla_join_kernel(const __grid_constant__ MlaDecodeArgs a) {
   __shared__ float4 so[kJoinWarps][32];
@@ -999,13 +1000,16 @@ __global__ void __launch_bounds__(32 * kJoinWarps) mla_join_kernel(const __grid_
   asm volatile("griddepcontrol.wait;" ::: "memory");       // the parts are written
   if (units == 0) return;
   const MlaRowParts rp = a.rows[t];
+  if (!rp.valid()) {
+    if (threadIdx.x == 0) raise_status(a.status, kErrTimeout);
+    return;
+  }
   if (rp.first == rp.last) return;
   const bool spread = gridDim.z == 4;
   const int parts = rp.last - rp.first + 1, dim = 128 * (spread ? blockIdx.z : warp);
   const int step = spread ? static_cast<int>(blockDim.x) / 32 : 1;
-  auto slot_of = [&](int i) { return i == 0 ? rp.first_slot : 2 * (rp.first + i); };
   float m = kNone;
-  for (int i = lane; i < parts; i += 32) m = fmaxf(m, part_ml(a, tile, slot_of(i))[hh].x);
+  for (int i = lane; i < parts; i += 32) m = fmaxf(m, part_ml(a, tile, rp.slot(i))[hh].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -1013,9 +1017,9 @@ __global__ void __launch_bounds__(32 * kJoinWarps) mla_join_kernel(const __grid_
   const float mz = m == kNone ? 0.0f : m;                // a part without a token (or all NaN) has m = -inf, f = 0
 #pragma unroll 4
   for (int i = spread ? warp : 0; i < parts; i += step) {
-    const float2 ml = part_ml(a, tile, slot_of(i))[hh];
+    const float2 ml = part_ml(a, tile, rp.slot(i))[hh];
     const float f = exp2f(ml.x - mz);
-    const float4 v = reinterpret_cast<const float4*>(part_o(a, tile, slot_of(i)) + hh * kDv + dim)[lane];
+    const float4 v = reinterpret_cast<const float4*>(part_o(a, tile, rp.slot(i)) + hh * kDv + dim)[lane];
     s.x = fmaf(f, v.x, s.x), s.y = fmaf(f, v.y, s.y);
     s.z = fmaf(f, v.z, s.z), s.w = fmaf(f, v.w, s.w);
     l = fmaf(f, ml.y, l);

@@ -203,8 +203,16 @@ int launch_mla_q_pack(const void* lat, int64_t rows_pad, const void* rope, int64
                       int64_t T, void* q8, float q_scale, cudaStream_t stream);
 
 // Latent attention of new tokens over the paged cache (csrc/mla_decode.cu).
+constexpr int kMlaRanges = 148;         // ranges a call is cut into at most; each may hold two parts of rows
 struct MlaRowParts {                   // which ranges a row was cut into: CTAs first .. last, the first one's part slot
   int32_t first, last, first_slot, pad;
+  // False: no record of this call's plan (a CTA gave up before it wrote its part; the workspace may hold anything).
+  __host__ __device__ bool valid() const {
+    return 0 <= first && first <= last && last < kMlaRanges && (first_slot >> 1) == first;
+  }
+  // The slot, 0 .. 2 kMlaRanges - 1, of part i = 0 .. last - first of a valid record: a row that goes on is the first one
+  // of its next CTA.
+  __host__ __device__ int slot(int i) const { return i == 0 ? first_slot : 2 * (first + i); }
 };
 struct MlaDecodeArgs {
   const void* q = nullptr;             // [T, H, 576] bf16 or e4m3, strides in elements
