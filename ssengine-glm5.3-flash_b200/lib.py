@@ -7,6 +7,7 @@ return code.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from pathlib import Path
 
@@ -219,19 +220,23 @@ def scratch(device, nbytes: int):
 def stream_scratch(device, nbytes: int, stream=None):
     """A uint8 workspace of at least `nbytes` for calls on `stream` (default: the current one) alone, grown on demand:
     calls on different streams get different buffers. It is allocated on that stream, so a buffer that is outgrown is
-    reused only after the stream's earlier calls."""
+    reused only after the stream's earlier calls.
+
+    A graph keeps the address that its capture saw, past any growth: while the stream is being captured the buffer is a
+    new one each time, from the graph's own memory, which later work of the same graph may reuse and nothing else."""
     import torch
 
     dev = torch.device(device)
     index = torch.cuda.current_device() if dev.index is None else dev.index
-    handle = torch._C._cuda_getCurrentRawStream(index) if stream is None else int(stream.cuda_stream)
-    key = (dev.type, index, handle)
-    t = _SCRATCH.get(key)
-    if t is None or t.numel() < nbytes:
-        with torch.cuda.stream(torch.cuda.current_stream(dev) if stream is None else stream):
-            t = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
-        _SCRATCH[key] = t
-    return t
+    with contextlib.nullcontext() if stream is None else torch.cuda.stream(stream):
+        if torch.cuda.is_current_stream_capturing():
+            return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+        handle = torch._C._cuda_getCurrentRawStream(index) if stream is None else int(stream.cuda_stream)
+        key = (dev.type, index, handle)
+        t = _SCRATCH.get(key)
+        if t is None or t.numel() < nbytes:
+            t = _SCRATCH[key] = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+        return t
 
 
 def check(name: str, rc: int) -> None:

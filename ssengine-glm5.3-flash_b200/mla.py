@@ -54,10 +54,9 @@ def decode(q: torch.Tensor, kv_cache: torch.Tensor, page_table: torch.Tensor, se
     (uint8) with unit stride in the last dimension and 16-byte row and head strides; kv_cache e4m3 bytes uint8
     [slots, 576]; seq_lens, reqs int32 [T]; -> out bf16 [T, H, 512] and, when given, lse fp32 [T, H]. A row without a
     token gets zeros (lse -inf). bmm1 = softmax scale * q_scale * k_scale, bmm2 = k_scale, as `sparse_mla`. Split over
-    the tokens and joined in `workspace` (uint8, `decode_workspace_bytes(T, H)`; default: one kept per stream, so that
-    captured calls whose graphs replay at the same time need workspaces of their own); the lengths are read on the
-    device. `status` (int32 [1] on the device) receives 1 for a reqs entry outside the table, 4 if a bounded wait gave up
-    (the call's outputs are then undefined)."""
+    the tokens and joined in `workspace` (uint8, `decode_workspace_bytes(T, H)`; default: one kept per stream, or in a
+    capture one of the graph's own); the lengths are read on the device. `status` (int32 [1] on the device) receives 1
+    for a reqs entry outside the table, 4 if a bounded wait gave up (the call's outputs are then undefined)."""
     return _decode(q, kv_cache, None, page_table, seq_lens, bmm1, out, bmm2, None, reqs, lse, workspace, stream, status)
 
 

@@ -1,6 +1,11 @@
 """The decode-step operators' host side and what their kernels share with it, without a GPU."""
 
+import contextlib
 import subprocess
+import weakref
+from types import SimpleNamespace
+
+import pytest
 
 
 ROW_PARTS = r"""
@@ -60,3 +65,56 @@ def test_a_rows_record_stays_within_the_parts_whatever_memory_holds(tmp_path):
                    check=True)
     run = subprocess.run([str(exe)], capture_output=True, text=True)
     assert run.returncode == 0 and run.stdout.strip() == "ok", run.stdout
+
+
+class FakeCuda:
+    """torch.cuda as `lib.stream_scratch` uses it: streams by handle, buffers on the CPU, a capture that can be on."""
+
+    def __init__(self, monkeypatch):
+        import torch
+
+        self.current, self.capturing, self.buffers = 1, set(), []
+        empty = torch.empty
+
+        def alloc(n, dtype, device):
+            t = empty(n, dtype=dtype)
+            self.buffers.append((self.current, weakref.ref(t)))
+            return t
+
+        @contextlib.contextmanager
+        def stream(s):
+            self.current, before = s.cuda_stream, self.current
+            yield
+            self.current = before
+
+        monkeypatch.setattr(torch, "empty", alloc)
+        monkeypatch.setattr(torch.cuda, "stream", stream)
+        monkeypatch.setattr(torch.cuda, "current_stream", lambda dev=None: SimpleNamespace(cuda_stream=self.current))
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: self.current in self.capturing)
+        monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: self.current, raising=False)
+
+
+@pytest.mark.parametrize("explicit", [False, True])
+def test_a_captured_call_keeps_no_buffer_that_can_be_outgrown(monkeypatch, explicit):
+    """Buffers per stream that grow; in a capture a new one each time, not the stream's kept one nor kept as one: what the
+    stream's calls drop later was never the graph's."""
+    from ssengine_b200 import lib
+
+    monkeypatch.setattr(lib, "_SCRATCH", {})
+    cuda = FakeCuda(monkeypatch)
+    get = lambda n: lib.stream_scratch("cuda:0", n, SimpleNamespace(cuda_stream=5) if explicit else None)
+    handle = 5 if explicit else 1
+    eager = get(1000)
+    assert get(600) is eager and cuda.buffers[-1][0] == handle
+    cuda.capturing.add(handle)
+    captured = get(600)
+    again = get(600)
+    assert captured is not eager and again is not captured and captured.numel() >= 600
+    assert cuda.buffers[-1][0] == handle                    # allocated on the capturing stream, so from the graph's pool
+    cuda.capturing.clear()
+    assert get(600) is eager
+    assert all(t is not captured and t is not again for t in lib._SCRATCH.values())
+    larger = get(2000)
+    assert larger.numel() >= 2000 and get(600) is larger
+    cuda.current = 9
+    assert explicit or get(600) is not larger               # another stream, another buffer

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import mla as omla
-from test_gpu_decode import BMM1, TOL, Cache, attention64, call, queries
+from test_gpu_decode import BMM1, TOL, Cache, attention64, call, check, queries
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +55,42 @@ def test_query_values_far_below_their_heads_largest(cuda):
     for h in range(H):
         err = np.linalg.norm(out[0, h] - want[h]) / np.linalg.norm(want[h])
         assert err < tol, (h, err, tol)
+
+
+def test_graphs_outlive_larger_calls_on_their_stream(cuda):
+    """Graphs of growing sizes captured on one stream with the default workspace, larger calls on that stream after them,
+    and the memory that these gave back in other hands: every graph still gives its own results, and touches nothing."""
+    from ssengine_b200 import mla
+
+    rng = np.random.default_rng(83)
+    lens = [int(n) for n in rng.integers(1, 900, 80)]
+    cache = Cache(rng, lens)
+    kv, tb = torch.from_numpy(cache.bytes).to(cuda), torch.from_numpy(cache.table).to(cuda)
+    q, q64 = queries(rng, 80, 80, "bf16")
+    q, seq = q.to(cuda), torch.tensor(lens, dtype=torch.int32, device=cuda)
+    side = torch.cuda.Stream()
+    graphs = []
+    for T, H in ((1, 64), (4, 64), (40, 64), (20, 80)):
+        out = torch.empty(T, H, 512, dtype=torch.bfloat16, device=cuda)
+        args = (q[:T, :H], kv, tb, seq[:T], BMM1, out)
+        with torch.cuda.stream(side):
+            mla.decode(*args)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            mla.decode(*args)
+        graphs.append((graph, out, T, H))
+    big = torch.empty(80, 80, 512, dtype=torch.bfloat16, device=cuda)
+    with torch.cuda.stream(side):
+        mla.decode(q, kv, tb, seq, BMM1, big)
+    torch.cuda.synchronize()
+    others = [torch.full((1 << 20,), 3.0, device=cuda) for _ in range(64)]
+    for graph, out, T, H in graphs:
+        out.fill_(float("nan"))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.double().cpu().numpy()
+        for t in range(T):
+            check(got[t], None, *attention64(q64[t, :H], cache.kv[t], BMM1, 1.0))
+    assert all(bool((o == 3.0).all()) for o in others)
