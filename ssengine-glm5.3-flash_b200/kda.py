@@ -110,12 +110,8 @@ class KdaLayer:
         ldb, ldo = _row_pitch("beta", beta, T, H), _row_pitch("out", out, T, P)
         if seqs.dtype is not torch.int32 or seqs.dim() != 2 or seqs.shape[1] != 4 or not seqs.is_contiguous():
             raise ValueError(f"seqs: contiguous int32 [R, 4], got {seqs.dtype} {tuple(seqs.shape)}")
-        dev = qkv.get_device()
-        for t in (g, beta, out, seqs, conv_state, rec_state, self.conv_weight):
-            if t.get_device() != dev:
-                raise ValueError("the tensors of one call must be on one device")
-        if dev < 0:
-            raise ValueError(f"the tensors are on {qkv.device}, not on a GPU")
+        lib.check_device((qkv, g, beta, out, seqs, conv_state, rec_state, self.conv_weight, self.a_log, self.dt_bias),
+                         status, stream)
         L = self.c_struct(conv_state, rec_state)
         rc = so.ssb_kda_decode(ctypes.byref(L), qkv.data_ptr(), ldx, g.data_ptr(), ldg, beta.data_ptr(), ldb, T,
                                seqs.data_ptr(), seqs.shape[0], out.data_ptr(), ldo,

@@ -239,6 +239,26 @@ def stream_scratch(device, nbytes: int, stream=None):
         return t
 
 
+def check_device(tensors, status=None, stream=None) -> None:
+    """ValueError unless the tensors of one call (None: absent), its status word (int32 on the device) and its stream are
+    all on one GPU, the current one: a launch takes their addresses as they are."""
+    import torch
+
+    dev = tensors[0].get_device()
+    if status is not None and (status.dtype is not torch.int32 or status.numel() < 1):
+        raise ValueError(f"status: int32 [1] on the device, got {status.dtype} {tuple(status.shape)}")
+    for t in (*tensors, status):
+        if t is not None and t.get_device() != dev:
+            raise ValueError("the tensors of one call must be on one device")
+    if dev < 0:
+        raise ValueError(f"the tensors are on {tensors[0].device}, not on a GPU")
+    current = torch.cuda.current_device()
+    stream_dev = dev if stream is None else getattr(stream, "device_index", dev)
+    if dev != current or stream_dev != dev:
+        raise ValueError(f"the tensors are on cuda:{dev}, the current device is cuda:{current}" +
+                         ("" if stream is None else f", the stream's cuda:{stream_dev}"))
+
+
 def check(name: str, rc: int) -> None:
     if rc != 0:
         raise SsbError(name, rc)

@@ -105,12 +105,7 @@ def _decode(q, kv_cache, indices, page_table, seq_lens, bmm1, out, bmm2, n_idx, 
     if workspace is not None and (workspace.dtype != torch.uint8 or not workspace.is_contiguous() or
                                   workspace.numel() < need):
         raise ValueError(f"workspace: contiguous uint8 of {need} bytes or more")
-    dev = q.get_device()
-    for t in (kv_cache, page_table, out, seq_lens, indices, reqs, lse, workspace):
-        if t is not None and t.get_device() != dev:
-            raise ValueError("the tensors of one call must be on one device")
-    if dev < 0:
-        raise ValueError(f"the tensors are on {q.device}, not on a GPU")
+    lib.check_device((q, kv_cache, page_table, out, seq_lens, indices, reqs, lse, workspace), status, stream)
     if workspace is None:
         workspace = lib.stream_scratch(q.device, need, stream)
     ptr = lambda t: None if t is None else t.data_ptr()

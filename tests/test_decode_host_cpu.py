@@ -118,3 +118,52 @@ def test_a_captured_call_keeps_no_buffer_that_can_be_outgrown(monkeypatch, expli
     assert larger.numel() >= 2000 and get(600) is larger
     cuda.current = 9
     assert explicit or get(600) is not larger               # another stream, another buffer
+
+
+class OnDevice:
+    """A tensor as the device check sees it."""
+
+    def __init__(self, index, dtype=None, numel=1):
+        self.index, self.dtype, self.device, self.shape = index, dtype, f"device {index}", (numel,)
+        self.numel = lambda: numel
+        self.get_device = lambda: index
+
+
+def test_calls_refuse_tensors_away_from_the_current_device(monkeypatch):
+    import torch
+
+    from ssengine_b200 import lib
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    on = lambda i: [OnDevice(i), OnDevice(i), None, OnDevice(i)]
+    word = lambda i, dtype=torch.int32, n=1: OnDevice(i, dtype, n)
+    stream = lambda i: SimpleNamespace(cuda_stream=3, device_index=i)
+    lib.check_device(on(1))
+    lib.check_device(on(1), word(1), stream(1))
+    for args in ((on(0),), (on(-1),), (on(1) + [OnDevice(0)],), (on(1) + [OnDevice(-1)],), (on(1), word(-1)),
+                 (on(1), word(0)), (on(1), word(1, torch.int64)), (on(1), word(1, n=0)), (on(1), None, stream(0)),
+                 (on(0), word(0), stream(0))):
+        with pytest.raises(ValueError):
+            lib.check_device(*args)
+
+
+@pytest.mark.parametrize("what", ["a_log", "dt_bias", "status", "conv_weight"])
+def test_the_recurrence_checks_every_tensor_it_reads(monkeypatch, what):
+    """Each tensor that the kernel reads goes through the device check."""
+    import torch
+
+    from ssengine_b200 import lib
+    from ssengine_b200.kda import KdaLayer
+
+    seen = []
+    monkeypatch.setattr(lib, "check_device", lambda ts, status=None, stream=None: seen.extend([*ts, status]) or 1 / 0)
+    H, bf = 2, dict(dtype=torch.bfloat16)
+    P = H * 128
+    L = KdaLayer(torch.zeros(3 * P, 4, **bf), torch.zeros(H), torch.zeros(P))
+    status = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ZeroDivisionError):
+        L.decode(torch.zeros(3, 3 * P, **bf), torch.zeros(3, P, **bf), torch.zeros(3, H, **bf),
+                 torch.zeros(3, P, **bf), torch.zeros(1, 4, dtype=torch.int32), torch.zeros(2, 3, 3 * P, **bf),
+                 torch.zeros(2, H, 128, 128), status=status)
+    want = status if what == "status" else getattr(L, what)
+    assert any(t is want for t in seen)

@@ -94,3 +94,38 @@ def test_graphs_outlive_larger_calls_on_their_stream(cuda):
         for t in range(T):
             check(got[t], None, *attention64(q64[t, :H], cache.kv[t], BMM1, 1.0))
     assert all(bool((o == 3.0).all()) for o in others)
+
+
+@pytest.mark.parametrize("what", ["a_log", "dt_bias", "status", "conv_state", "seqs"])
+def test_kda_refuses_host_tensors(cuda, what):
+    """A tensor left on the host is refused before the launch."""
+    from test_gpu_decode import kda_dev, kda_make
+
+    rng = np.random.default_rng(89)
+    H = 2
+    L, dev = kda_dev(cuda, kda_make(rng, 1, H, 2))
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    a = dict(a_log=L.a_log, dt_bias=L.dt_bias, status=status, conv_state=dev["cst"],
+             seqs=torch.tensor([[0, 1, 1, 1]], dtype=torch.int32, device=cuda))
+    a[what] = a[what].cpu()
+    L.a_log, L.dt_bias = a["a_log"], a["dt_bias"]
+    out = torch.full((1, H * 128), 7.0, dtype=torch.bfloat16, device=cuda)
+    with pytest.raises(ValueError):
+        L.decode(dev["x"], dev["g"], dev["beta"], out, a["seqs"], a["conv_state"], dev["rst"], status=a["status"])
+    torch.cuda.synchronize()
+    assert bool((out == 7.0).all())
+
+
+def test_attention_refuses_a_host_status(cuda):
+    from ssengine_b200 import mla
+
+    i32 = dict(dtype=torch.int32, device=cuda)
+    out = torch.full((1, 4, 512), 7.0, dtype=torch.bfloat16, device=cuda)
+    for status in (torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.uint8, device=cuda),
+                   torch.zeros(0, **i32)):
+        with pytest.raises(ValueError):
+            mla.decode(torch.zeros(1, 4, 576, dtype=torch.bfloat16, device=cuda),
+                       torch.zeros(256, 576, dtype=torch.uint8, device=cuda), torch.zeros(1, 2, **i32),
+                       torch.ones(1, **i32), BMM1, out, status=status)
+    torch.cuda.synchronize()
+    assert bool((out == 7.0).all())
