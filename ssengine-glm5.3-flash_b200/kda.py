@@ -65,6 +65,7 @@ class KdaLayer:
         C = 3 * H * HEAD_DIM
         assert w.dtype is torch.bfloat16 and w.shape == (C, 4) and w.is_contiguous() and a_log.dtype is torch.float32
         assert dt_bias.dtype is torch.float32 and dt_bias.numel() == H * HEAD_DIM
+        assert a_log.is_contiguous() and dt_bias.is_contiguous()
         cs, rs = conv_state.stride(), rec_state.stride()
         (_, taps, cols), (_, heads, dv, dk) = conv_state.shape, rec_state.shape
         assert conv_state.dtype is torch.bfloat16 and taps == 3 and cols == C and cs[1:] == (C, 1)

@@ -167,3 +167,21 @@ def test_the_recurrence_checks_every_tensor_it_reads(monkeypatch, what):
                  torch.zeros(2, H, 128, 128), status=status)
     want = status if what == "status" else getattr(L, what)
     assert any(t is want for t in seen)
+
+
+@pytest.mark.parametrize("what", ["a_log", "dt_bias"])
+def test_gate_parameters_with_strides_are_refused(what):
+    """The kernels read heads (and heads x 128) values in a row: a broadcast parameter has one, a strided one others."""
+    import torch
+
+    from ssengine_b200.kda import KdaLayer
+
+    H = 2
+    P = H * 128
+    n = {"a_log": H, "dt_bias": P}
+    conv, rec = torch.zeros(2, 3, 3 * P, dtype=torch.bfloat16), torch.zeros(2, H, 128, 128)
+    for bad in (lambda k: torch.zeros(1).expand(k), lambda k: torch.zeros(2 * k)[::2]):
+        p = {k: bad(v) if k == what else torch.zeros(v) for k, v in n.items()}
+        with pytest.raises(AssertionError):
+            KdaLayer(torch.zeros(3 * P, 4, dtype=torch.bfloat16), p["a_log"], p["dt_bias"]).c_struct(conv, rec)
+    KdaLayer(torch.zeros(3 * P, 4, dtype=torch.bfloat16), torch.zeros(H), torch.zeros(H, 128)).c_struct(conv, rec)
