@@ -1079,11 +1079,12 @@ int launch_mla_decode(const MlaDecodeArgs& a_in, void* ws, int64_t ws_bytes, cud
   p += up256(slots * kTileH * 8);
   a.part_o = reinterpret_cast<float*>(p);
   auto* kernel = a.q_e4m3 ? mla_decode_kernel<true> : mla_decode_kernel<false>;
-  static bool attr[2] = {false, false};
-  if (!attr[a.q_e4m3]) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return kErrCuda;
-    attr[a.q_e4m3] = true;
-  }
+  static OncePerDevice attr[2];
+  int device = 0;
+  const auto set = [&] {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) == cudaSuccess;
+  };
+  if (cudaGetDevice(&device) != cudaSuccess || !attr[a.q_e4m3].done(device, set)) return kErrCuda;
   CUtensorMap mlat = {}, mrope = {};
   if (a.indices == nullptr) {                            // selected tokens are copied row by row
     const int u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;

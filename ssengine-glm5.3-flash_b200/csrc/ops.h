@@ -202,6 +202,23 @@ int launch_mla_append(const void* src, int64_t lds, const int64_t* slots, int64_
 int launch_mla_q_pack(const void* lat, int64_t rows_pad, const void* rope, int64_t ldr, int64_t rope_stride,
                       int64_t T, void* q8, float q_scale, cudaStream_t stream);
 
+// What a launcher sets once on each device (a kernel's attributes): done(f) calls f where it has not yet succeeded.
+class OncePerDevice {
+ public:
+  template <class F>
+  bool done(int device, F f) {
+    const bool kept = 0 <= device && device < kDevices;
+    if (kept && set_[device]) return true;
+    if (!f()) return false;
+    if (kept) set_[device] = true;
+    return true;
+  }
+
+ private:
+  static constexpr int kDevices = 64;
+  bool set_[kDevices] = {};
+};
+
 // Latent attention of new tokens over the paged cache (csrc/mla_decode.cu).
 constexpr int kMlaRanges = 148;         // ranges a call is cut into at most; each may hold two parts of rows
 struct MlaRowParts {                   // which ranges a row was cut into: CTAs first .. last, the first one's part slot

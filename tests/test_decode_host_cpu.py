@@ -8,6 +8,18 @@ from types import SimpleNamespace
 import pytest
 
 
+def run_host_program(tmp_path, text):
+    """Compiles a program over the library's internal header and runs it on the CPU; it has to print "ok"."""
+    from ssengine_b200 import _build
+
+    src, exe = tmp_path / "host.cu", tmp_path / "host"
+    src.write_text(text)
+    subprocess.run([_build.nvcc(), *_build.ARCH, "-std=c++17", "-O1", f"-I{_build.CSRC}", "-o", str(exe), str(src)],
+                   check=True)
+    run = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert run.returncode == 0 and run.stdout.strip() == "ok", run.stdout
+
+
 ROW_PARTS = r"""
 #include <cstdio>
 #include <cstdint>
@@ -57,14 +69,31 @@ int main() {
 
 def test_a_rows_record_stays_within_the_parts_whatever_memory_holds(tmp_path):
     """The join reads parts by a row's record; a CTA that gave up leaves there what the workspace held before."""
-    from ssengine_b200 import _build
+    run_host_program(tmp_path, ROW_PARTS)
 
-    src, exe = tmp_path / "row_parts.cu", tmp_path / "row_parts"
-    src.write_text(ROW_PARTS)
-    subprocess.run([_build.nvcc(), *_build.ARCH, "-std=c++17", "-O1", f"-I{_build.CSRC}", "-o", str(exe), str(src)],
-                   check=True)
-    run = subprocess.run([str(exe)], capture_output=True, text=True)
-    assert run.returncode == 0 and run.stdout.strip() == "ok", run.stdout
+
+ONCE = r"""
+#include <cstdio>
+#include "ops.h"
+int main() {
+  ssb::OncePerDevice once;
+  int calls = 0;
+  bool works = false;
+  const auto set = [&] { return ++calls, works; };
+  if (once.done(0, set) || calls != 1) return std::puts("a failure passed"), 1;
+  works = true;
+  for (int device : {0, 1, 0, 63, 1, 0, 63})
+    if (!once.done(device, set)) return std::puts("refused"), 1;
+  if (calls != 4) return std::printf("%d calls for three devices and a failure\n", calls), 1;
+  if (!once.done(64, set) || !once.done(64, set) || !once.done(-1, set) || calls != 7) return std::puts("outside"), 1;
+  std::puts("ok");
+}
+"""
+
+
+def test_kernel_attributes_are_set_on_every_device(tmp_path):
+    """Once on each device of the process, again after a failure, and each time for a device beyond the table."""
+    run_host_program(tmp_path, ONCE)
 
 
 class FakeCuda:
