@@ -195,9 +195,9 @@ int ssb_kda_prefill_ws(const ssb_kda_layer* layer, const void* x, int64_t ldx, c
  * few tokens: any length, one after the other): arguments, sequence table and state blocks as ssb_kda_prefill_ws, so a
  * request may move between the two forms at any token. q, k, v and everything up to the bf16 output stay in fp32 (the
  * prefill form rounds the conv outputs to bf16). No workspace; one launch. x, g, conv state 4-byte aligned with even
- * pitches, recurrent state 16-byte aligned (block stride % 4 == 0). Sequences that reach outside [0, T) or name a
- * negative block are skipped with status 1, sequences without rows leave their blocks as they are; the blocks named by
- * one call must be distinct. */
+ * pitches (with one row, T = 1, its pitches are not used), recurrent state 16-byte aligned (block stride % 4 == 0).
+ * Sequences that reach outside [0, T) or name a negative block are skipped with status 1, sequences without rows leave
+ * their blocks as they are; the blocks named by one call must be distinct. */
 int ssb_kda_decode(const ssb_kda_layer* layer, const void* x, int64_t ldx, const void* g, int64_t ldg,
                    const void* beta, int64_t ldb, int64_t T, const int32_t* seqs, int64_t R, void* out, int64_t ldo,
                    int32_t* status, void* stream);
@@ -277,14 +277,15 @@ int ssb_sparse_mla(const void* q, int64_t T, const void* kv_cache, const int32_t
 /* Latent attention of new tokens (a decode step) over the paged FP8 cache, split over each row's tokens and joined: out
  * bf16 [T, heads, 512] = bmm2_scale * softmax(bmm1_scale * q . kv) kv[:, 0:512] as ssb_sparse_mla, for 1..128 heads. q
  * [T, heads, 576] bf16 (q_e4m3 = 0: its values enter to 2^-21 of the head's largest) or e4m3 (1), row stride ldq and
- * head_stride in elements (16-byte multiples). Query row t belongs to row reqs[t] of page_table int32 [R, width] (reqs
- * NULL: row t; several rows may share one, e.g. draft tokens) and sees positions 0 .. seq_lens[t] - 1, or, with indices
- * int32 [T, ld_idx] (not NULL, also where n_idx is 0), the first n_idx listed positions (-1 = none; at or past
- * seq_lens[t], when that is given: none; a position listed twice counts twice). Tokens of a negative page, past the
- * table or past cache_rows are left out. A row with no token gets zeros and lse -inf; a reqs entry outside [0, R) the
- * same, with status 1. lse (fp32 [T, heads] or NULL) = the natural log of the sum of the row's weights. workspace:
- * 256-byte aligned, ssb_mla_decode_workspace_bytes(T, heads) or more (returns 3 when smaller), its contents need not be
- * kept. The lengths are read on the device: the call can be captured in a graph and replayed as they grow. */
+ * head_stride in elements (16-byte multiples; not used with one row, one head). Query row t belongs to row reqs[t] of
+ * page_table int32 [R, width] (reqs NULL: row t; several rows may share one, e.g. draft tokens) and sees positions 0 ..
+ * seq_lens[t] - 1, or, with indices int32 [T, ld_idx] (not NULL, also where n_idx is 0), the first n_idx listed
+ * positions (-1 = none; at or past seq_lens[t], when that is given: none; a position listed twice counts twice). Tokens
+ * of a negative page, past the table or past cache_rows are left out. A row with no token gets zeros and lse -inf; a
+ * reqs entry outside [0, R) the same, with status 1. lse (fp32 [T, heads] or NULL) = the natural log of the sum of the
+ * row's weights. workspace: 256-byte aligned, ssb_mla_decode_workspace_bytes(T, heads) or more (returns 3 when
+ * smaller), its contents need not be kept. The lengths are read on the device: the call can be captured in a graph and
+ * replayed as they grow. */
 int ssb_mla_decode(const void* q, int32_t q_e4m3, int64_t ldq, int64_t head_stride, int64_t T, int32_t heads,
                    const void* kv_cache, int64_t cache_rows, const int32_t* page_table, int64_t R, int64_t width,
                    const int32_t* reqs, const int32_t* seq_lens, const int32_t* indices, int64_t ld_idx,

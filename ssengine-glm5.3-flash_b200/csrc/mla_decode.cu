@@ -1060,16 +1060,18 @@ int launch_mla_decode(const MlaDecodeArgs& a_in, void* ws, int64_t ws_bytes, cud
   const int eb = a.q_e4m3 ? 1 : 2;
   if (a.T < 0 || a.T > 0x7fffffff || a.H <= 0 || a.H > 128 || a.R <= 0 || a.width <= 0 || a.cache_rows <= 0 ||
       a.cache_rows > 0x7fffffff || (a.indices == nullptr && a.seq_lens == nullptr) ||
-      (a.indices != nullptr && (a.n_idx < 0 || a.ld_idx < a.n_idx)) || (a.reqs == nullptr && a.T > a.R))
+      (a.indices != nullptr && (a.n_idx < 0 || (a.T > 1 && a.ld_idx < a.n_idx))) || (a.reqs == nullptr && a.T > a.R))
     return kErrArgs;
   if (a.T == 0) return kOk;
   const int64_t most =                                   // units of a row
       a.indices != nullptr ? (a.n_idx + kUnit - 1) / kUnit : (int64_t)(kPage / kUnit) * a.width;
   if (a.T * (most + kRowCost) > 0x7fffffff) return kErrArgs;
   if (a.q == nullptr || a.kv == nullptr || a.table == nullptr || a.out == nullptr || ws == nullptr ||
-      !aligned(a.q, 16) || !aligned(a.kv, 16) || !aligned(a.out, 16) || !aligned(ws, 256) || (a.ldq * eb) % 16 ||
-      (a.hsq * eb) % 16 || a.hsq < kDq || (a.T > 1 && a.ldq < kDq))
+      !aligned(a.q, 16) || !aligned(a.kv, 16) || !aligned(a.out, 16) || !aligned(ws, 256))
     return kErrArgs;
+  // one row has no row stride, one head no head stride: what the caller's tensor states there is not used
+  if (a.T > 1 && ((a.ldq * eb) % 16 != 0 || a.ldq < kDq)) return kErrArgs;
+  if (a.H > 1 && ((a.hsq * eb) % 16 != 0 || a.hsq < kDq)) return kErrArgs;
   if (ws_bytes < mla_decode_workspace_bytes(a.T, a.H)) return kErrWorkspace;
   const int64_t tiles = tiles_of(a.H), slots = tiles * 2 * kMaxCtas;
   uint8_t* p = static_cast<uint8_t*>(ws);

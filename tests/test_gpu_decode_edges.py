@@ -57,6 +57,62 @@ def test_query_values_far_below_their_heads_largest(cuda):
         assert err < tol, (h, err, tol)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_one_row_or_one_head_with_any_stride(cuda, kind):
+    """A single row has no row stride and a single head no head stride: whatever the tensor states there is not used."""
+    rng = np.random.default_rng(71)
+    cache = Cache(rng, [333, 100])
+    q, q64 = queries(rng, 2, 3, kind)
+    q = q.to(cuda)
+    for rows, heads in (([0], [0, 1, 2]), ([0, 1], [1]), ([1], [2])):
+        part = q[rows][:, heads].contiguous()
+        st = list(part.stride())
+        if len(rows) == 1:
+            st[0] = 7
+        if len(heads) == 1:
+            st[1] = 1
+        lens = [cache.lens[r] for r in rows]
+        out, lse, status = call(cuda, part.as_strided(part.shape, st), cache, seq_lens=np.array(lens, np.int32),
+                                reqs=np.array(rows, np.int32))
+        assert status == 0
+        for i, r in enumerate(rows):
+            check(out[i], lse[i], *attention64(q64[r][heads], cache.kv[r], BMM1, 1.0))
+
+
+def test_one_selected_row_with_any_pitch(cuda):
+    rng = np.random.default_rng(72)
+    cache = Cache(rng, [500])
+    q, q64 = queries(rng, 1, 64, "bf16")
+    idx = np.sort(rng.choice(500, 100, replace=False)).astype(np.int32)
+    from ssengine_b200 import mla
+
+    out = torch.empty(1, 64, 512, dtype=torch.bfloat16, device=cuda)
+    mla.decode_selected(q.to(cuda), torch.from_numpy(cache.bytes).to(cuda),
+                        torch.from_numpy(idx).to(cuda).as_strided((1, 100), (1, 1)),
+                        torch.from_numpy(cache.table).to(cuda), BMM1, out)
+    torch.cuda.synchronize()
+    check(out[0].double().cpu().numpy(), None, *attention64(q64[0], cache.kv[0][idx], BMM1, 1.0))
+
+
+def test_kda_one_row_with_any_stride(cuda):
+    """A single row of projections, gates, betas and outputs has no pitch."""
+    from ssengine_b200.kda import seq_table
+    from test_gpu_decode import kda_check, kda_dev, kda_make, recurrence64
+
+    rng = np.random.default_rng(73)
+    H = 2
+    d = kda_make(rng, 1, H, 3)
+    want = recurrence64(d, [(0, 1, 2, 1)], H)
+    L, dev = kda_dev(cuda, d)
+    one = lambda t: t.as_strided(t.shape, (1, 1))
+    out = torch.zeros(1, H * 128, dtype=torch.bfloat16, device=cuda)
+    L.decode(one(dev["x"]), one(dev["g"]), one(dev["beta"]), one(out), seq_table([(0, 1, 2, 1)], cuda), dev["cst"],
+             dev["rst"])
+    torch.cuda.synchronize()
+    kda_check(out.double().cpu().numpy(), dev["cst"].double().cpu().numpy(), dev["rst"].double().cpu().numpy(), want,
+              [(0, 1, 2, 1)])
+
+
 def test_graphs_outlive_larger_calls_on_their_stream(cuda):
     """Graphs of growing sizes captured on one stream with the default workspace, larger calls on that stream after them,
     and the memory that these gave back in other hands: every graph still gives its own results, and touches nothing."""
