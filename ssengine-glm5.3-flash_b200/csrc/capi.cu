@@ -409,7 +409,7 @@ int ssb_mla_decode(const void* q, int32_t q_e4m3, int64_t ldq, int64_t head_stri
                    const int32_t* reqs, const int32_t* seq_lens, const int32_t* indices, int64_t ld_idx,
                    int32_t n_idx, float bmm1_scale, float bmm2_scale, void* out, float* lse, void* workspace,
                    int64_t ws_bytes, int32_t* status, void* stream) {
-  if (width <= 0 || width > (1 << 24) || R <= 0 || R > (1 << 28) || (q_e4m3 != 0 && q_e4m3 != 1)) return kErrArgs;
+  if (width < 0 || width > (1 << 24) || R < 0 || R > (1 << 28) || (q_e4m3 != 0 && q_e4m3 != 1)) return kErrArgs;
   ssb::MlaDecodeArgs a;
   a.q = q;
   a.q_e4m3 = q_e4m3;

@@ -175,12 +175,14 @@ bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p
 }  // namespace
 
 int launch_kda_decode(const KdaArgs& a, cudaStream_t stream) {
-  if (a.g == nullptr || a.beta == nullptr || a.a_log == nullptr || a.dt_bias == nullptr || a.conv_w == nullptr ||
-      a.conv_state == nullptr || a.rec_state == nullptr || a.out == nullptr || a.x == nullptr || a.seqs == nullptr ||
-      a.T < 0 || a.T > 0x7fffffff || (a.cs_stride % 2) || (a.rs_stride % 4) || a.cs_stride < 9 * (int64_t)a.P ||
-      a.rs_stride < (int64_t)a.H * kDim * kDim || !aligned(a.x, 4) || !aligned(a.g, 4) || !aligned(a.conv_w, 16) ||
-      !aligned(a.dt_bias, 8) || !aligned(a.conv_state, 4) || !aligned(a.rec_state, 16) || !aligned(a.seqs, 16) ||
-      !aligned(a.beta, 2) || !aligned(a.out, 2))
+  // empty tensors (no rows, no sequences) have no address
+  if ((a.T > 0 && (a.x == nullptr || a.g == nullptr || a.beta == nullptr || a.out == nullptr)) ||
+      (a.R > 0 && a.seqs == nullptr) || a.a_log == nullptr || a.dt_bias == nullptr || a.conv_w == nullptr ||
+      a.conv_state == nullptr || a.rec_state == nullptr || a.T < 0 || a.T > 0x7fffffff || (a.cs_stride % 2) ||
+      (a.rs_stride % 4) || a.cs_stride < 9 * (int64_t)a.P || a.rs_stride < (int64_t)a.H * kDim * kDim ||
+      !aligned(a.x, 4) || !aligned(a.g, 4) || !aligned(a.conv_w, 16) || !aligned(a.dt_bias, 8) ||
+      !aligned(a.conv_state, 4) || !aligned(a.rec_state, 16) || !aligned(a.seqs, 16) || !aligned(a.beta, 2) ||
+      !aligned(a.out, 2))
     return kErrArgs;
   // one row has no pitch: what the caller's tensors state there is not used
   if (a.T > 1 && ((a.ldx % 2) || (a.ldg % 2) || a.ldx < 3 * (int64_t)a.P || a.ldg < a.P || a.ldb < a.H || a.ldo < a.P))

@@ -1058,11 +1058,12 @@ int64_t mla_decode_workspace_bytes(int64_t T, int H) {
 int launch_mla_decode(const MlaDecodeArgs& a_in, void* ws, int64_t ws_bytes, cudaStream_t stream) {
   MlaDecodeArgs a = a_in;
   const int eb = a.q_e4m3 ? 1 : 2;
-  if (a.T < 0 || a.T > 0x7fffffff || a.H <= 0 || a.H > 128 || a.R <= 0 || a.width <= 0 || a.cache_rows <= 0 ||
-      a.cache_rows > 0x7fffffff || (a.indices == nullptr && a.seq_lens == nullptr) ||
+  if (a.T < 0 || a.T > 0x7fffffff || a.H <= 0 || a.H > 128) return kErrArgs;
+  if (a.T == 0) return kOk;                              // empty tensors have no address: the others are not looked at
+  if (a.R <= 0 || a.width <= 0 || a.cache_rows <= 0 || a.cache_rows > 0x7fffffff ||
+      (a.indices == nullptr && a.seq_lens == nullptr) ||
       (a.indices != nullptr && (a.n_idx < 0 || (a.T > 1 && a.ld_idx < a.n_idx))) || (a.reqs == nullptr && a.T > a.R))
     return kErrArgs;
-  if (a.T == 0) return kOk;
   const int64_t most =                                   // units of a row
       a.indices != nullptr ? (a.n_idx + kUnit - 1) / kUnit : (int64_t)(kPage / kUnit) * a.width;
   if (a.T * (most + kRowCost) > 0x7fffffff) return kErrArgs;

@@ -113,6 +113,32 @@ def test_kda_one_row_with_any_stride(cuda):
               [(0, 1, 2, 1)])
 
 
+def test_no_rows(cuda):
+    """A step without rows (empty tensors have no address) writes nothing and is no error."""
+    from ssengine_b200 import mla
+    from ssengine_b200.kda import KdaLayer
+
+    cache = torch.zeros(256, 576, dtype=torch.uint8, device=cuda)
+    i32 = dict(dtype=torch.int32, device=cuda)
+    bf = dict(dtype=torch.bfloat16, device=cuda)
+    for R in (0, 2):
+        table = torch.zeros(R, 2, **i32)
+        q, out = torch.empty(0, 64, 576, **bf), torch.empty(0, 64, 512, **bf)
+        assert mla.decode(q, cache, table, torch.empty(0, **i32), BMM1, out) is out
+        assert mla.decode_selected(q, cache, torch.empty(0, 2051, **i32), table, BMM1, out) is out
+    H = 2
+    P = H * 128
+    L = KdaLayer(torch.zeros(3 * P, 4, **bf), torch.zeros(H, device=cuda), torch.zeros(P, device=cuda))
+    conv, rec = torch.ones(3, 3, 3 * P, **bf), torch.ones(3, H, 128, 128, device=cuda)
+    for seqs in (torch.empty(0, 4, **i32), torch.tensor([[0, 0, 1, 1]], **i32)):
+        status = torch.zeros(1, **i32)
+        out = torch.empty(0, P, **bf)
+        assert L.decode(torch.empty(0, 3 * P, **bf), torch.empty(0, P, **bf), torch.empty(0, H, **bf), out, seqs, conv,
+                        rec, status=status) is out
+        torch.cuda.synchronize()
+        assert int(status[0]) == 0 and bool((conv == 1).all()) and bool((rec == 1).all())
+
+
 def test_graphs_outlive_larger_calls_on_their_stream(cuda):
     """Graphs of growing sizes captured on one stream with the default workspace, larger calls on that stream after them,
     and the memory that these gave back in other hands: every graph still gives its own results, and touches nothing."""
