@@ -139,6 +139,18 @@ def test_no_rows(cuda):
         assert int(status[0]) == 0 and bool((conv == 1).all()) and bool((rec == 1).all())
 
 
+def test_lengths_around_a_unit_of_64_tokens(cuda):
+    rng = np.random.default_rng(79)
+    lens = [63, 64, 65, 191, 192, 193, 0, 255, 256, 320, 321]
+    cache = Cache(rng, lens)
+    for kind in ("bf16", "e4m3"):
+        q, q64 = queries(rng, len(lens), 64, kind)
+        out, lse, status = call(cuda, q, cache, seq_lens=np.array(lens, np.int32))
+        assert status == 0
+        for t in range(len(lens)):
+            check(out[t], lse[t], *attention64(q64[t], cache.kv[t], BMM1, 1.0))
+
+
 def test_graphs_outlive_larger_calls_on_their_stream(cuda):
     """Graphs of growing sizes captured on one stream with the default workspace, larger calls on that stream after them,
     and the memory that these gave back in other hands: every graph still gives its own results, and touches nothing."""
