@@ -448,6 +448,7 @@ class DsaAttention:
         self.scale = self.qh ** -0.5
         self.q_scale, self.k_scale = 1.0, 1.0          # per-tensor FP8 scales of the query and the latent cache
         self.logits_ws = None          # optional fp32 buffer the logits rows are cut from (a stage's shared one)
+        self.decode_ws = None          # optional workspace of the decode forms (a stage's shared one)
         self._side = None              # the indexer branch's stream (created on first use)
         self.device = dev
         self._lib = lib.load()
@@ -564,12 +565,16 @@ class DsaAttention:
         if form is None:
             mla.sparse_mla(q8, kv_cache, tok, qsl, page_table, bmm1, o_lat, bmm2=self.k_scale,
                            n_idx=4 * self.TOPK + 3, stream=stream, status=status)
-        elif select:
-            mla.decode_selected(q8, kv_cache, tok, page_table, bmm1, o_lat, bmm2=self.k_scale,
-                                n_idx=4 * self.TOPK + 3, seq_lens=seq_lens, reqs=reqs, stream=stream, status=status)
         else:
-            mla.decode(q8, kv_cache, page_table, seq_lens, bmm1, o_lat, bmm2=self.k_scale, reqs=reqs, stream=stream,
-                       status=status)
+            ws = self.decode_ws
+            if ws is not None and ws.numel() < mla.decode_workspace_bytes(T, NH):
+                ws = None
+            common = dict(bmm2=self.k_scale, reqs=reqs, workspace=ws, stream=stream, status=status)
+            if select:
+                mla.decode_selected(q8, kv_cache, tok, page_table, bmm1, o_lat, n_idx=4 * self.TOPK + 3,
+                                    seq_lens=seq_lens, **common)
+            else:
+                mla.decode(q8, kv_cache, page_table, seq_lens, bmm1, o_lat, **common)
         # v_up: each head's latent rows read in place from the token-major attention output, written straight into
         # the token-major o_proj input
         o_in = torch.empty(T, NH * self.v_dim, **bf)

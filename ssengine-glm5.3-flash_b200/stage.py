@@ -316,21 +316,25 @@ class StageModel:
     def _warm(self) -> None:
         """Reserves the device memory a microbatch needs, so that no forward maps new memory (a cudaMalloc inside a
         forward stalls the host for up to tens of milliseconds while the GPU drains its queue): the indexer's logits
-        rows at `max_context` (one buffer the stage's DSA layers share; they run in order on one stream), the KDA /
-        mHC chunk workspace for `reserve_reqs` requests, and one forward of a dummy request of a full microbatch
-        (written into the null block's pages and state) that loads every kernel and leaves its temporaries in the
-        caching allocator for the next microbatches; then the MoE layers' shared workspace."""
+        rows at `max_context` and the decode forms' workspace for `mb_tokens` rows (buffers that the stage's DSA layers
+        share; they run in order on one stream), the KDA / mHC chunk workspace for `reserve_reqs` requests, one forward
+        of a dummy request of a full microbatch and one step of a token in each decode form (written into the null
+        block's pages and state) that load every kernel and leave their temporaries in the caching allocator for the
+        next microbatches; then the MoE layers' shared workspace."""
         from .messages import Chunk, Plan
 
         cfg = self.cfg
         if any(self.is_dsa):
+            from . import mla
             from .layers import DsaAttention
 
             width = -(-(-(-cfg.max_context // PAGE_TOKENS) * DsaAttention.POOLS_PER_PAGE) // 128) * 128
             logits_ws = torch.empty(cfg.mb_tokens * width, dtype=torch.float32, device=self.device)
+            decode_ws = torch.empty(mla.decode_workspace_bytes(cfg.mb_tokens, DsaAttention.HEADS), dtype=torch.uint8,
+                                    device=self.device)
             for layer, dsa in zip(self.layers, self.is_dsa):
                 if dsa:
-                    layer.attn.logits_ws = logits_ws
+                    layer.attn.logits_ws, layer.attn.decode_ws = logits_ws, decode_ws
         if self.kda:
             from . import kda
 
@@ -341,6 +345,10 @@ class StageModel:
         plan = Plan(-1, [Chunk("warmup", 0, n, pages, [0] * 6, True, [0] * n if self.first else None)])
         hidden = None if self.first else torch.zeros(n, self.hidden_width, dtype=torch.bfloat16, device=self.device)
         self.forward(plan, hidden)
+        if self.kda:
+            token = Plan(-1, [Chunk("warmup", n - 1, 1, pages, [0] * 6, True, [0] if self.first else None)])
+            for form in ("selected", "dense") if any(self.is_dsa) else ("selected",):
+                self.decode(token, None if self.first else hidden[:1], form)
         moes = [layer.moe if self.kda else layer for layer in self.layers]
         moes = [m for m in moes if isinstance(m, moe.MoELayer)]
         ws = max(m.workspace_bytes(self.cfg.mb_tokens) for m in moes) if moes else 0

@@ -223,3 +223,33 @@ def test_attention_refuses_a_host_status(cuda):
                        torch.ones(1, **i32), BMM1, out, status=status)
     torch.cuda.synchronize()
     assert bool((out == 7.0).all())
+
+
+@pytest.mark.parametrize("attention", ["selected", "dense"])
+def test_a_stages_step_uses_what_its_build_reserved(cuda, monkeypatch, attention):
+    """Neither the first step nor one of a full microbatch's rows asks for a workspace of its own, and none maps memory."""
+    from ssengine_b200 import lib
+    from ssengine_b200.messages import Chunk, Plan
+    from ssengine_b200.stage import StageConfig, StageModel
+
+    rows = 128
+    st = StageModel(StageConfig(layer_split=(4,), hidden=512, inter=256, experts=16, top_k=4, vocab=1000, num_blocks=14,
+                                mb_tokens=rows, seed=6, layer_kind="hybrid", kda_heads=2, q_lora=256, mla_nope=64), 0,
+                    cuda)
+    a, b = ([67, 68], [2, 3, 4, 5, 6, 7]), ([69], [8, 9, 10, 11, 12, 13])
+    rng = np.random.default_rng(3)
+    tok = lambda n: rng.integers(0, 1000, n).tolist()
+    st.forward(Plan(0, [Chunk("a", 0, 100, *a, True, tok(100)), Chunk("b", 0, 20, *b, True, tok(20))]))
+
+    def none(*_):
+        raise AssertionError("a step asked for a workspace")
+
+    monkeypatch.setattr(lib, "stream_scratch", none)
+    torch.cuda.synchronize()
+    mapped = torch.cuda.memory_reserved(cuda)
+    st.decode(Plan(1, [Chunk("a", 100, 1, *a, True, tok(1)), Chunk("b", 20, 1, *b, True, tok(1))]), attention=attention)
+    st.decode(Plan(2, [Chunk("a", 101, rows - 50, *a, True, tok(rows - 50)), Chunk("b", 21, 50, *b, True, tok(50))]),
+              attention=attention)
+    torch.cuda.synchronize()
+    assert int(st.status[0]) == 0 and torch.cuda.memory_reserved(cuda) == mapped
+    assert torch.isfinite(st.last_logits).all()
