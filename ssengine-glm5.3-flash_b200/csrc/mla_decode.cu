@@ -240,6 +240,18 @@ __device__ __noinline__ bool mbar_wait_more(uint32_t bar, uint32_t parity, volat
 SSB_DEVICE bool mbar_nap(uint32_t bar, uint32_t parity, volatile int32_t* abort_flag, int32_t* status) {
   return mbar_try_wait(bar, parity) || mbar_wait_more(bar, parity, abort_flag, status);
 }
+// A gather warp that gave up: the tiles it asked for may be on their way into this CTA's shared memory, which is another's
+// once the CTA has ended. It waits for the units it has issued; one that another warp left out stays incomplete, but the
+// own tiles (microseconds) have landed long before the limit.
+__device__ __noinline__ void drain_tiles(uint32_t full, int slot, int round) {
+  const unsigned long long t0 = globaltimer();
+#pragma unroll 1
+  for (int j = 0; j < kSlots; ++j) {
+    const int phase = ring_phase(j, slot, round);
+    while (phase >= 0 && !mbar_try_wait(full + 8 * j, phase) && globaltimer() - t0 <= kWaitNs / 1000) {}
+  }
+  __syncwarp();
+}
 // One arrival for a warp, after all its lanes got here.
 SSB_DEVICE void warp_arrive(uint32_t bar, int lane) {
   __syncwarp();
@@ -674,6 +686,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     cp_async_wait_all();
+    if (!ok) drain_tiles(B.full, slot, round);
   } else if (warp == kValueWarp) {
     // ---------------------------------------------------------------- value products
     zero_rows(a, cta, h0, nh, lane);

@@ -220,6 +220,13 @@ class OncePerDevice {
 };
 
 // Latent attention of new tokens over the paged cache (csrc/mla_decode.cu).
+// A ring of buffers that a producer fills in turn, `slot` the next one, `round` the times it has gone round: the parity of
+// the last phase of buffer j's barrier that it has begun (-1: none yet).
+__host__ __device__ constexpr int ring_phase(int j, int slot, int round) {
+  const int fills = round + (j < slot ? 1 : 0);
+  return fills > 0 ? (fills - 1) & 1 : -1;
+}
+
 constexpr int kMlaRanges = 148;         // ranges a call is cut into at most; each may hold two parts of rows
 struct MlaRowParts {                   // which ranges a row was cut into: CTAs first .. last, the first one's part slot
   int32_t first, last, first_slot, pad;

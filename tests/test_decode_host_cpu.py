@@ -214,3 +214,27 @@ def test_gate_parameters_with_strides_are_refused(what):
         with pytest.raises(AssertionError):
             KdaLayer(torch.zeros(3 * P, 4, dtype=torch.bfloat16), p["a_log"], p["dt_bias"]).c_struct(conv, rec)
     KdaLayer(torch.zeros(3 * P, 4, dtype=torch.bfloat16), torch.zeros(H), torch.zeros(H, 128)).c_struct(conv, rec)
+
+
+PHASES = r"""
+#include <cstdio>
+#include "ops.h"
+int main() {
+  for (int slots = 1; slots <= 8; ++slots) {
+    int begun[8] = {}, slot = 0, round = 0;                 // fills of each buffer so far
+    for (int unit = 0; unit < 100; ++unit) {
+      for (int j = 0; j < slots; ++j)
+        if (ssb::ring_phase(j, slot, round) != (begun[j] == 0 ? -1 : (begun[j] - 1) % 2))
+          return std::printf("buffer %d of %d after %d units\n", j, slots, unit), 1;
+      ++begun[slot];
+      if (++slot == slots) slot = 0, ++round;
+    }
+  }
+  std::puts("ok");
+}
+"""
+
+
+def test_a_producer_that_gives_up_waits_for_the_copies_it_began(tmp_path):
+    """The barrier phase of each buffer's last fill, after any number of units."""
+    run_host_program(tmp_path, PHASES)
