@@ -15,8 +15,10 @@
 // value rows 16 w .. 16 w + 15 in registers, a lane 4 key columns of each (one 512-byte row a warp load, 16 loads in
 // flight a lane while the conv and the gates are computed). Products and updates as packed fp32 pairs, short
 // exponentials and quotients: with the library forms the code outgrew the instruction cache (406 us at 256 requests x 64
-// heads, now 347: the copy rate). Measured against that: 8 lanes a row, which saves 24 of the 31 shuffles of the row sums
-// (357 us); the states through three 64 KB buffers by bulk copies with two groups of warps on every other one (614 us).
+// heads, now 351 to 356, the copy rate). Measured against that: 8 lanes a row, which saves 24 of the 31 shuffles of the
+// row sums (357 us, then against 347); the states through three 64 KB buffers by bulk copies with two groups of warps on
+// every other one (614 us). Runs: each further token costs its arithmetic, little of it beside other CTAs' copies: 24
+// requests x 64 heads 39 us with one token each, 45, 60 and 96 with 2, 4 and 8.
 #include "common.cuh"
 #include "ops.h"
 

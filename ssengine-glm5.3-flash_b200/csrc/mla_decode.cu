@@ -5,16 +5,17 @@
 //
 // Split: a row of n tokens is ceil(n / 64) units of work; the units of all rows, in row order, are cut into equal
 // contiguous ranges, one per CTA (two rows or more may share a CTA, one row may span many), or, where rows are few or
-// short, each row into parts of its own. A CTA works through its range row by row; a row that lies in one range is finished there, the parts of a row cut between ranges go to the
-// workspace as (reference m, sum l, unnormalised O) in fp32 and are joined by a second kernel:
+// short, each row into parts of its own. A CTA works through its range row by row; a row that lies in one range is
+// finished there, the parts of a row cut between ranges go to the workspace as (reference m, sum l, unnormalised O) in
+// fp32 and are joined by a second kernel:
 //   M = max_i m_i;  O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.
 // No atomics and a fixed order of the sums: the same inputs give the same bits.
 //
 // One CTA of 22 warps an SM, over units of 64 tokens and a tile of 64 heads:
 //   gather (4 warps): a whole unit of a page as TMA tiles (4 chunks [64 tokens x 128 B] and the rope keys), a row's last
 //       units and selected tokens by cp.async row by row, what is not there zero-filled; five units in flight;
-//   scores (1 warp issues): S [128 query parts x 64 tokens] = Q K^T, tcgen05 kind::f8f6f4. bf16 queries enter exactly, as
-//       two e4m3 parts (64 high rows, 64 low ones): the half of the tensor core that 64 heads alone would leave idle.
+//   scores (1 warp issues): S [128 query parts x 64 tokens] = Q K^T, tcgen05 kind::f8f6f4. bf16 queries enter as two
+//       e4m3 parts (64 high rows, 64 low ones; `stage_q`): the half of the tensor core that 64 heads alone would leave idle.
 //       Q stands in TMEM, which has room for all but 96 bytes a row;
 //   softmax (2 sets of 8 warps, every second unit each; 16 tokens of one head a thread): the high and low parts of a head
 //       are 16 lanes apart and change places by shuffles. Weights 2^(s - E), E one exponent for a head's 32 tokens, again
@@ -25,16 +26,18 @@
 //       rows read the other way round.
 // TMEM: O^T 256 columns, S of two units 128, Q 120, block scales 8. Shared memory: five units' rows 5 x 36 KB (the high
 // parts of P take the place of the rope keys, which only the scores need), the low parts of P 2 x 4 KB, the end of Q 12 KB.
-// Bounds: 576 bytes a token from HBM against 128 x 576 + 2 x 64 x 512 products of 8 bits: 1,350 cycles a unit at the
-// measured copy rate, and as many for the two products (18 instructions of 32 cycles, 16 of 48, which read shared memory at
-// its full rate). A unit takes about 1,700 cycles. Measured, bf16 queries, 64 heads: 64 rows x 32,768 tokens in 300 to 320 us
-// (4.1 TB/s of cache), where the card is at its power limit (the clock falls to 1.4 GHz and the time to 378 us when the call is
-// repeated for seconds); 32 rows of 128 to 32,768 tokens 80 us; 1 x 131,072 tokens 41 us; 1 x 1,000 tokens 18 us, of which
-// the plan is 1.3, the query's staging 5.5, the unit and its products 4.5, the parts' stores 2.3 and the join 4.
-// Measured against it: units of 128 tokens in two slots with a token and 16 heads a thread, whose block maxima need warp
-// reductions, 380 us at 64 x 32,768; one warp issuing both products 356 (its waits for scores and for weights then
-// follow one another); S of one unit 312. The roles' loops are kept small because they share 28 KB of instruction cache:
-// unrolled in full they took 511 us where rolled ones took 485.
+// Bounds: 576 bytes a token from HBM against 128 x 576 + 2 x 64 x 512 products of 8 bits. A unit's bytes take 0.83 us of
+// an SM's share of the measured copy rate (1,640 cycles at 1.965 GHz, 1,130 at 1.36), its products 1,340 cycles (18
+// instructions of 32, 16 of 48, which read shared memory at its full rate). It takes more than either: 2,000 cycles where
+// one row has the card (1 x 131,072), 2,250 under sustained load at 64 rows x 32,768 tokens (386 us a call at 990 W, where
+// the power limit holds the clock at 1.36 GHz), 2,700 in single calls at 1.965 GHz (322 us from cold caches, 307 and less
+// in short bursts). Which role holds the rest is not shown. 32 rows of 128 to 32,768 tokens 81 us in a burst, 92 sustained;
+// 1 x 131,072 tokens 42 us; 1 x 1,000 tokens 18 us, of which the plan is 1.3, the query's staging 5.5, the unit and its
+// products 4.5, the parts' stores 2.3 and the join 4.
+// Measured against it (bursts): units of 128 tokens in two slots with a token and 16 heads a thread, whose block maxima
+// need warp reductions, 380 us at 64 x 32,768; one warp issuing both products 356 (its waits for scores and for weights
+// then follow one another); S of one unit 312. The roles' loops are kept small because they share 28 KB of instruction
+// cache: unrolled in full they took 511 us where rolled ones took 485.
 #include <cuda_fp16.h>
 
 #include "common.cuh"
