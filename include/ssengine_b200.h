@@ -197,7 +197,8 @@ int ssb_kda_prefill_ws(const ssb_kda_layer* layer, const void* x, int64_t ldx, c
  * prefill form rounds the conv outputs to bf16). No workspace; one launch. x, g, conv state 4-byte aligned with even
  * pitches (with one row, T = 1, its pitches are not used), recurrent state 16-byte aligned (block stride % 4 == 0).
  * Sequences that reach outside [0, T) or name a negative block are skipped with status 1, sequences without rows leave
- * their blocks as they are; the blocks named by one call must be distinct. */
+ * their blocks as they are; the blocks named by one call must be distinct and lie in the state pools, whose size the
+ * call is not told. */
 int ssb_kda_decode(const ssb_kda_layer* layer, const void* x, int64_t ldx, const void* g, int64_t ldg,
                    const void* beta, int64_t ldb, int64_t T, const int32_t* seqs, int64_t R, void* out, int64_t ldo,
                    int32_t* status, void* stream);
