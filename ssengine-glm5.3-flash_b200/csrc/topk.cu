@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kTopkThreads)
   __shared__ uint32_t cand_key[kCand];
   uint32_t* cand_col = sm_keys + cache_keys;  // dynamic shared memory after the row cache: [kCand] then [kMaxK]
   uint32_t* sel = cand_col + kCand;
-  __shared__ uint32_t s_bin, s_need, s_ncand, s_nsel, s_ntie;
+  __shared__ uint32_t s_bin, s_need, s_ncand, s_nsel, s_ntie, s_at;
   __shared__ uint32_t w_above[kTopkWarps], w_tie[kTopkWarps];
   const int tid = threadIdx.x;
   const int lane = tid & 31;
@@ -161,6 +161,7 @@ __global__ void __launch_bounds__(kTopkThreads)
         s_ncand = 0;
         s_nsel = 0;
         s_ntie = 0;
+        s_at = 0;
       }
       __syncthreads();
       for_keys(row, n, tid, [&](int, uint32_t key) { atomicAdd(&hist[key >> 21], 1u); });
@@ -211,10 +212,9 @@ __global__ void __launch_bounds__(kTopkThreads)
           __syncthreads();
           goto streaming;
         }
-        if (tid == 0) s_ntie = 0;
-        __syncthreads();
+        // hist is free: the tie columns. They have a counter of their own: s_ntie, which every warp has yet to read, stays
         for (int i = tid; i < static_cast<int>(nc); i += kTopkThreads)
-          if (cand_key[i] == prefix) hist[atomicAdd(&s_ntie, 1u)] = cand_col[i];   // hist is free: the tie columns
+          if (cand_key[i] == prefix) hist[atomicAdd(&s_at, 1u)] = cand_col[i];
         __syncthreads();
         if (nt > need) {                                                   // lowest columns first
           int np2 = 1;
@@ -236,7 +236,8 @@ __global__ void __launch_bounds__(kTopkThreads)
         __syncthreads();                                                   // the next row reuses the buffers
         continue;
       }
-      // more candidates than the list holds: the streaming passes below
+      // more candidates than the list holds: the streaming passes below, once every warp has read s_ncand
+      __syncthreads();
     }
   streaming:
 
