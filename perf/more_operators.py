@@ -306,6 +306,8 @@ def prepare(case, seed):
             s["beam"] = beam
             n = beam.workspace_bytes(*s["scores"].shape, s["x"].shape[1], s["k"])
             s["workspace"] = torch.empty(n, dtype=torch.uint8, **dev)
+            shape = (s["scores"].shape[0], s["k"])
+            s["picked"] = tuple(torch.empty(shape, dtype=t, **dev) for t in (torch.float32, torch.int32, torch.int64))
     return s
 
 
@@ -323,14 +325,15 @@ def _run_own(s):
                                     reqs=s["reqs"], workspace=s["workspace"], status=s["status"])
     if op == "kda_tree":
         return s["layer"].decode_tree(s["proj"], s["gate"], s["beta"], s["out"], s["seq_table"], s["parents"],
-                                      s["conv"], s["rec"], status=s["status"])
+                                      s["conv"], s["rec"], max_nodes=max(len(t) for t in s["trees"]),
+                                      status=s["status"])
     if op == "advance":
         s["layer"].advance(s["proj"], s["gate"], s["beta"], s["rows"], s["seq_table"], s["conv"], s["rec"],
                            status=s["status"])
         return dict(conv_state=s["conv"], rec_state=s["rec"])
     if op == "beams":
         scores, parents, tokens = s["beam"].select(s["x"], s["scores"], s["k"], finished=s["finished"], pad=s["pad"],
-                                                   workspace=s["workspace"])
+                                                   out=s["picked"], workspace=s["workspace"])
         return dict(scores=scores, parents=parents, tokens=tokens)
     s["mover"](s["src_table"], s["dst_table"], status=s["status"])
     return s["views"]
