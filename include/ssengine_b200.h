@@ -203,6 +203,24 @@ int ssb_kda_decode(const ssb_kda_layer* layer, const void* x, int64_t ldx, const
                    const void* beta, int64_t ldb, int64_t T, const int32_t* seqs, int64_t R, void* out, int64_t ldo,
                    int32_t* status, void* stream);
 
+/* The same steps along trees of drafted tokens: the rows of a sequence are the nodes of one tree, at most max_nodes (1..64)
+ * of them, parents first; node i continues the state of node parents[first row + i] (int32 [T], smaller than i; -1: the
+ * request's state block, or zeros where the sequence has none), its conv taps the rows on its path and behind them the
+ * block's conv rows. Every node's output to its row of out; the state blocks are read and left as they are. Arguments
+ * otherwise as ssb_kda_decode; several sequences may read one block. A sequence that reaches outside [0, T), has more than
+ * max_nodes rows or a parent that is not before its child, or names a negative block, is skipped with status 1. */
+int ssb_kda_decode_tree(const ssb_kda_layer* layer, const void* x, int64_t ldx, const void* g, int64_t ldg,
+                        const void* beta, int64_t ldb, int64_t T, const int32_t* parents, const int32_t* seqs, int64_t R,
+                        int32_t max_nodes, void* out, int64_t ldo, int32_t* status, void* stream);
+
+/* The state blocks moved on along rows of an earlier step (the accepted path of a tree): what ssb_kda_decode leaves in them
+ * for the input rows rows[first .. end - 1] (int32 [n_rows]; the sequences' first and end rows are places in it), without
+ * the outputs. A sequence that reaches outside [0, n_rows), lists a row outside [0, T) or names a negative block is
+ * skipped with status 1. */
+int ssb_kda_advance(const ssb_kda_layer* layer, const void* x, int64_t ldx, const void* g, int64_t ldg,
+                    const void* beta, int64_t ldb, int64_t T, const int32_t* rows, int64_t n_rows, const int32_t* seqs,
+                    int64_t R, int32_t* status, void* stream);
+
 /* The short conv alone: q, k, v bf16 [T, H * 128] each (contiguous) and the conv state blocks updated; rows outside
  * every sequence are written as 0. Replaces `kda_conv.conv_qkv` (ssengine/model/kda_conv.py:146-164). */
 int ssb_kda_conv(const ssb_kda_layer* layer, const void* x, int64_t ldx, int64_t T, const int32_t* seqs, int64_t R,
@@ -295,6 +313,51 @@ int ssb_mla_decode(const void* q, int32_t q_e4m3, int64_t ldq, int64_t head_stri
 
 /* Device bytes of the workspace of ssb_mla_decode; -1 on bad arguments. */
 int64_t ssb_mla_decode_workspace_bytes(int64_t T, int32_t heads);
+
+/* The same attention for the nodes of trees of drafted tokens: a request's nodes lie in its cache behind its seq_lens
+ * context tokens, at most 64 of them, and query row t sees positions 0 .. seq_lens[t] - 1 and seq_lens[t] + j for every bit
+ * j set in ancestors[t] (int64 [T], 8-byte aligned: the nodes on the row's path, itself among them; any set is taken). A
+ * negative seq_lens[t], or neither context nor bits: no token. The other arguments, the workspace and what is refused as
+ * ssb_mla_decode. */
+int ssb_mla_decode_tree(const void* q, int32_t q_e4m3, int64_t ldq, int64_t head_stride, int64_t T, int32_t heads,
+                        const void* kv_cache, int64_t cache_rows, const int32_t* page_table, int64_t R, int64_t width,
+                        const int32_t* reqs, const int32_t* seq_lens, const int64_t* ancestors, float bmm1_scale,
+                        float bmm2_scale, void* out, float* lse, void* workspace, int64_t ws_bytes, int32_t* status,
+                        void* stream);
+
+/* Rows of cache views moved by lists on the device: for every view v and group g < groups, with l = v.list, row
+ * dst[l][g][i] of the view takes what its row src[l][g][i] held before the call, i < n (src, dst int32 [lists, groups, n]
+ * on the device, n <= 64). Within a group any rows may be both read and written (a permutation in place, one source for
+ * several rows); an entry with a negative id, or whose ids are equal, moves nothing, and of entries with one destination
+ * the first counts. A row that one group writes must not occur in another group of its list, nor two views overlap in rows
+ * moved: what such a call leaves there is undefined. An id past a view's rows: the entry moves nothing there, status 1.
+ * Beams' states and pages reordered (src = the parents' rows), pages forked (src = the shared page), accepted tokens of a
+ * tree brought to its front. */
+typedef struct ssb_move_view {
+  void* base;                  /* device memory, 16-byte aligned: row r is the nbytes at base + r * stride */
+  int64_t stride;              /* % 16 == 0, nbytes or more (not used with one row) */
+  int64_t nbytes;              /* % 16 == 0 */
+  int64_t rows;
+  int64_t list;                /* which list of ids the view goes by */
+} ssb_move_view;
+/* views: n_views <= 80 of them in host memory, read before the call returns. */
+int ssb_move_rows(const ssb_move_view* views, int32_t n_views, const int32_t* src, const int32_t* dst, int64_t lists,
+                  int64_t groups, int32_t n, int32_t* status, void* stream);
+
+/* A beam search's selection for G requests of `beams` (1..64) beams: of the candidates (b, v) with score scores[g, b] +
+ * x[g, b, v] - log sum_v exp x[g, b, v] the k (1..64) best in order, equal scores by the lower b * V + v: their scores
+ * (fp32), beams and tokens to out_scores, out_parents, out_tokens [G, k]. logits [G * beams, ld] fp32 or bf16 (bf16 = 1),
+ * read once; sums in 64 bits across threads, scores compared in 64 bits (log sums are right to about 2^-23). A beam
+ * with finished[g, b] != 0 (uint8 [G, beams] or NULL) has one candidate, token `pad` at scores[g, b], and its logits are
+ * not read. A logit of -inf is no candidate, nor is any of a beam whose score or log sum is infinite or NaN; places
+ * without a candidate get -inf, -1, -1. workspace: 256-byte aligned, ssb_beam_workspace_bytes or more (returns 3 when
+ * smaller), its contents need not be kept. */
+int ssb_beam_select(const void* logits, int32_t bf16, int64_t ld, int64_t G, int32_t beams, int64_t V, const float* scores,
+                    const uint8_t* finished, int64_t pad, int32_t k, float* out_scores, int32_t* out_parents,
+                    int64_t* out_tokens, void* workspace, int64_t ws_bytes, void* stream);
+
+/* Device bytes of the workspace of ssb_beam_select; -1 on bad arguments. */
+int64_t ssb_beam_workspace_bytes(int64_t G, int32_t beams, int64_t V, int32_t k);
 
 /* MLA cache append: row t of src bf16 [T, 576] (row pitch lds elements, % 8 == 0) into kv_cache row slots[t] (int64,
  * skipped when < 0) as e4m3(x / k_scale), round to nearest even, saturating to +-448 (576 bytes a row). Replaces the

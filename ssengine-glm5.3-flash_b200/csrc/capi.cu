@@ -319,6 +319,40 @@ int ssb_kda_decode(const ssb_kda_layer* layer, const void* x, int64_t ldx, const
   return ssb::launch_kda_decode(a, static_cast<cudaStream_t>(stream));
 }
 
+int ssb_kda_advance(const ssb_kda_layer* layer, const void* x, int64_t ldx, const void* g, int64_t ldg,
+                    const void* beta, int64_t ldb, int64_t T, const int32_t* rows, int64_t n_rows, const int32_t* seqs,
+                    int64_t R, int32_t* status, void* stream) {
+  ssb::KdaArgs a;
+  if (T < 0 || !kda_args(layer, x, ldx, seqs, R, a)) return kErrArgs;
+  a.g = static_cast<const __nv_bfloat16*>(g);
+  a.ldg = ldg;
+  a.beta = static_cast<const __nv_bfloat16*>(beta);
+  a.ldb = ldb;
+  a.status = status;
+  a.T = T;
+  a.rows = rows;
+  a.n_rows = n_rows;
+  return ssb::launch_kda_advance(a, static_cast<cudaStream_t>(stream));
+}
+
+int ssb_kda_decode_tree(const ssb_kda_layer* layer, const void* x, int64_t ldx, const void* g, int64_t ldg,
+                        const void* beta, int64_t ldb, int64_t T, const int32_t* parents, const int32_t* seqs, int64_t R,
+                        int32_t max_nodes, void* out, int64_t ldo, int32_t* status, void* stream) {
+  ssb::KdaArgs a;
+  if (T < 0 || !kda_args(layer, x, ldx, seqs, R, a)) return kErrArgs;
+  a.g = static_cast<const __nv_bfloat16*>(g);
+  a.ldg = ldg;
+  a.beta = static_cast<const __nv_bfloat16*>(beta);
+  a.ldb = ldb;
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.ldo = ldo;
+  a.status = status;
+  a.T = T;
+  a.parents = parents;
+  a.max_nodes = max_nodes;
+  return ssb::launch_kda_tree(a, static_cast<cudaStream_t>(stream));
+}
+
 int64_t ssb_kda_workspace_bytes(int32_t heads, int64_t T, int64_t R) {
   if (heads <= 0 || T < 0 || R < 0 || R > (1 << 30)) return -1;
   return ssb::kda_workspace_bytes(heads, T, static_cast<int>(R));
@@ -404,11 +438,11 @@ int64_t ssb_mla_decode_workspace_bytes(int64_t T, int32_t heads) {
   return ssb::mla_decode_workspace_bytes(T, heads);
 }
 
-int ssb_mla_decode(const void* q, int32_t q_e4m3, int64_t ldq, int64_t head_stride, int64_t T, int32_t heads,
-                   const void* kv_cache, int64_t cache_rows, const int32_t* page_table, int64_t R, int64_t width,
-                   const int32_t* reqs, const int32_t* seq_lens, const int32_t* indices, int64_t ld_idx,
-                   int32_t n_idx, float bmm1_scale, float bmm2_scale, void* out, float* lse, void* workspace,
-                   int64_t ws_bytes, int32_t* status, void* stream) {
+static int mla_decode_args(const void* q, int32_t q_e4m3, int64_t ldq, int64_t head_stride, int64_t T, int32_t heads,
+                           const void* kv_cache, int64_t cache_rows, const int32_t* page_table, int64_t R, int64_t width,
+                           const int32_t* reqs, const int32_t* seq_lens, const int32_t* indices, int64_t ld_idx,
+                           int32_t n_idx, const void* ancestors, float bmm1_scale, float bmm2_scale, void* out, float* lse,
+                           void* workspace, int64_t ws_bytes, int32_t* status, void* stream) {
   if (width < 0 || width > (1 << 24) || R < 0 || R > (1 << 28) || (q_e4m3 != 0 && q_e4m3 != 1)) return kErrArgs;
   ssb::MlaDecodeArgs a;
   a.q = q;
@@ -427,12 +461,80 @@ int ssb_mla_decode(const void* q, int32_t q_e4m3, int64_t ldq, int64_t head_stri
   a.indices = indices;
   a.ld_idx = ld_idx;
   a.n_idx = n_idx;
+  a.ancestors = static_cast<const uint64_t*>(ancestors);
   a.bmm1 = bmm1_scale;
   a.bmm2 = bmm2_scale;
   a.out = static_cast<__nv_bfloat16*>(out);
   a.lse = lse;
   a.status = status;
   return ssb::launch_mla_decode(a, workspace, ws_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int ssb_mla_decode(const void* q, int32_t q_e4m3, int64_t ldq, int64_t head_stride, int64_t T, int32_t heads,
+                   const void* kv_cache, int64_t cache_rows, const int32_t* page_table, int64_t R, int64_t width,
+                   const int32_t* reqs, const int32_t* seq_lens, const int32_t* indices, int64_t ld_idx,
+                   int32_t n_idx, float bmm1_scale, float bmm2_scale, void* out, float* lse, void* workspace,
+                   int64_t ws_bytes, int32_t* status, void* stream) {
+  return mla_decode_args(q, q_e4m3, ldq, head_stride, T, heads, kv_cache, cache_rows, page_table, R, width, reqs, seq_lens,
+                         indices, ld_idx, n_idx, nullptr, bmm1_scale, bmm2_scale, out, lse, workspace, ws_bytes, status,
+                         stream);
+}
+
+int ssb_mla_decode_tree(const void* q, int32_t q_e4m3, int64_t ldq, int64_t head_stride, int64_t T, int32_t heads,
+                        const void* kv_cache, int64_t cache_rows, const int32_t* page_table, int64_t R, int64_t width,
+                        const int32_t* reqs, const int32_t* seq_lens, const int64_t* ancestors, float bmm1_scale,
+                        float bmm2_scale, void* out, float* lse, void* workspace, int64_t ws_bytes, int32_t* status,
+                        void* stream) {
+  if (T > 0 && ancestors == nullptr) return kErrArgs;
+  return mla_decode_args(q, q_e4m3, ldq, head_stride, T, heads, kv_cache, cache_rows, page_table, R, width, reqs, seq_lens,
+                         nullptr, 0, 0, ancestors, bmm1_scale, bmm2_scale, out, lse, workspace, ws_bytes, status, stream);
+}
+
+int ssb_move_rows(const ssb_move_view* views, int32_t n_views, const int32_t* src, const int32_t* dst, int64_t lists,
+                  int64_t groups, int32_t n, int32_t* status, void* stream) {
+  if (n_views < 0 || n_views > ssb::kMoveViews || (n_views > 0 && views == nullptr)) return kErrArgs;
+  ssb::MoveView v[ssb::kMoveViews];
+  for (int i = 0; i < n_views; ++i) {
+    v[i].base = static_cast<uint8_t*>(views[i].base);
+    v[i].stride = views[i].stride;
+    v[i].nbytes = views[i].nbytes;
+    v[i].rows = views[i].rows;
+    v[i].list = views[i].list;
+  }
+  ssb::MoveArgs a;
+  a.views = n_views;
+  a.n = n;
+  a.src = src;
+  a.dst = dst;
+  a.lists = lists;
+  a.groups = groups;
+  a.status = status;
+  return ssb::launch_move_rows(v, a, static_cast<cudaStream_t>(stream));
+}
+
+int64_t ssb_beam_workspace_bytes(int64_t G, int32_t beams, int64_t V, int32_t k) {
+  return ssb::beam_workspace_bytes(G, beams, V, k);
+}
+
+int ssb_beam_select(const void* logits, int32_t bf16, int64_t ld, int64_t G, int32_t beams, int64_t V, const float* scores,
+                    const uint8_t* finished, int64_t pad, int32_t k, float* out_scores, int32_t* out_parents,
+                    int64_t* out_tokens, void* workspace, int64_t ws_bytes, void* stream) {
+  if (bf16 != 0 && bf16 != 1) return kErrArgs;
+  ssb::BeamArgs a;
+  a.x = logits;
+  a.bf16 = bf16;
+  a.ldx = ld;
+  a.G = G;
+  a.B = beams;
+  a.V = V;
+  a.k = k;
+  a.scores = scores;
+  a.finished = finished;
+  a.pad = pad;
+  a.out_scores = out_scores;
+  a.out_parents = out_parents;
+  a.out_tokens = out_tokens;
+  return ssb::launch_beam_select(a, workspace, ws_bytes, static_cast<cudaStream_t>(stream));
 }
 
 int ssb_mla_cache_append(const void* src, int64_t lds, const int64_t* slots, int64_t T, void* cache, float k_scale,

@@ -20,6 +20,7 @@
 // every other one (614 us). Runs: each further token costs its arithmetic, little of it beside other CTAs' copies: 24
 // requests x 64 heads 39 us with one token each, 45, 60 and 96 with 2, 4 and 8.
 #include "common.cuh"
+#include "kda_math.cuh"
 #include "ops.h"
 
 namespace ssb {
@@ -29,21 +30,6 @@ constexpr int kDim = 128;
 constexpr int kDecThreads = 256;
 constexpr int kRowsW = 16;             // value rows a warp
 
-// e^x as 2^(x log2 e) with the product's rounding error carried to first order: ex2.approx's own error (2^-22) remains.
-// x above 88 counts as 88 (e^x must stay finite, or its correction is inf - inf): as a divisor e^88 makes the quotients
-// below 0, as they are there to 2^-126. NaN stays NaN.
-SSB_DEVICE float exp_fast(float x) {
-  x = x > 88.0f ? 88.0f : x;
-  constexpr float kHi = 1.44269502162933349609375f, kLo = 1.925963033500928e-8f;        // log2 e in two parts
-  const float t = x * kHi;
-  const float r = fmaf(x, kLo, fmaf(x, kHi, -t));
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t));
-  return fmaf(y, fminf(fmaxf(r, -1.0f), 1.0f) * 0.6931471805599453f, y);
-}
-SSB_DEVICE float sigmoid_fast(float z) { return __fdividef(1.0f, 1.0f + exp_fast(-z)); }
-SSB_DEVICE float silu_fast(float y) { return __fdividef(y, 1.0f + exp_fast(-y)); }
-SSB_DEVICE float2 bf2(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
 // The state is not read again by this call: its stores leave the caches first.
 SSB_DEVICE void store_stream(float* p, ulonglong2 v) {
   float4 f;
@@ -71,17 +57,43 @@ SSB_DEVICE float warp_sum_transposed(float (&v)[32], int lane) {
   return v[0];
 }
 
+// The same of 16 values a lane: lanes l and l + 16 receive the total of value l (16 shuffles).
+SSB_DEVICE float warp_sum_transposed16(float (&v)[16], int lane) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const float keep = up ? v[i + o] : v[i], send = up ? v[i] : v[i + o];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+    }
+  }
+  return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 16);
+}
+
+// kAdvance: the steps go along a list of rows (a sequence's rows are places in it) and leave the state alone, no outputs:
+// the queries' conv rows move on, their products are left out.
+template <bool kAdvance>
 __global__ void __launch_bounds__(kDecThreads, 2) kda_decode_kernel(const __grid_constant__ KdaArgs a) {
   __shared__ __align__(16) float sy[2][4][kDim];       // q | k | v | decay of a token, double-buffered
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int r = blockIdx.x / a.H, h = blockIdx.x - r * a.H;
   const int4 sq = __ldg(reinterpret_cast<const int4*>(a.seqs) + r);   // {first row, end row, state block, has state}
   const int s = sq.x, e = sq.y;
-  if (s < 0 || e < s || e > a.T || sq.z < 0) {
+  if (s < 0 || e < s || e > (kAdvance ? a.n_rows : a.T) || sq.z < 0) {
     if (tid == 0 && h == 0) raise_status(a.status, kErrArgs);
     return;
   }
   if (e == s) return;
+  if (kAdvance) {                                      // a row that is none leaves its whole sequence as it was
+    bool bad = false;
+    for (int i = s + tid; i < e; i += kDecThreads) bad |= static_cast<uint32_t>(a.rows[i]) >= static_cast<uint32_t>(a.T);
+    if (__syncthreads_or(bad)) {
+      if (tid == 0 && h == 0) raise_status(a.status, kErrArgs);
+      return;
+    }
+  }
+  const auto row_of = [&](int i) -> int64_t { return kAdvance ? __ldg(a.rows + i) : i; };
   const bool init = sq.w != 0;
   float* S = a.rec_state + (int64_t)sq.z * a.rs_stride + ((int64_t)h * kDim + kRowsW * warp) * kDim + 4 * lane;
   ulonglong2 st[kRowsW];                               // row i of the warp: columns 4 lane .. 4 lane + 3
@@ -102,13 +114,15 @@ __global__ void __launch_bounds__(kDecThreads, 2) kda_decode_kernel(const __grid
     raw1 = *reinterpret_cast<const uint32_t*>(cs + 3 * a.P);
     raw2 = *reinterpret_cast<const uint32_t*>(cs + 6 * a.P);
   }
-  uint32_t raw = __ldg(in + s * pitch);
-  float beta = __bfloat162float(a.beta[(int64_t)s * a.ldb + h]);
+  uint32_t raw = __ldg(in + row_of(s) * pitch);
+  float beta = __bfloat162float(a.beta[row_of(s) * a.ldb + h]);
 #pragma unroll 1
   for (int t = s; t < e; ++t) {
     float* y = &sy[(t - s) & 1][0][0];
-    float2 o;
-    if (conv) {
+    float2 o = make_float2(0.0f, 0.0f);
+    if (kAdvance && part == 0) {
+      raw0 = raw1, raw1 = raw2, raw2 = raw;
+    } else if (conv) {
       const uint4 wv = __ldg(reinterpret_cast<const uint4*>(a.conv_w + col * 4));   // 2 channels x 4 taps
       const float2 x0 = bf2(raw0), x1 = bf2(raw1), x2 = bf2(raw2), x3 = bf2(raw);
       const float2 p0 = bf2(wv.x), p1 = bf2(wv.y), p2 = bf2(wv.z), p3 = bf2(wv.w);
@@ -124,8 +138,8 @@ __global__ void __launch_bounds__(kDecThreads, 2) kda_decode_kernel(const __grid
     *reinterpret_cast<float2*>(y + part * kDim + 2 * pair) = o;
     const float b = sigmoid_fast(beta);
     if (t + 1 < e) {                                     // the next token's inputs, behind this one's arithmetic
-      raw = __ldg(in + (t + 1) * pitch);
-      beta = __bfloat162float(a.beta[(int64_t)(t + 1) * a.ldb + h]);
+      raw = __ldg(in + row_of(t + 1) * pitch);
+      beta = __bfloat162float(a.beta[row_of(t + 1) * a.ldb + h]);
     }
     __syncthreads();
     const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(y + 4 * lane);
@@ -140,20 +154,24 @@ __global__ void __launch_bounds__(kDecThreads, 2) kda_decode_kernel(const __grid
       nd += __shfl_xor_sync(0xffffffffu, nd, o2);
     }
     const float rq = a.scale * rsqrtf(nq + 1e-6f), rk = rsqrtf(nk + 1e-6f);
-    float d[2 * kRowsW];                                 // of row i: S k at i, S q at 16 + i (k, q not yet normalised)
+    float d[kAdvance ? kRowsW : 2 * kRowsW];             // of row i: S k at i, S q at 16 + i (k, q not yet normalised)
 #pragma unroll
     for (int i = 0; i < kRowsW; ++i) {
       ulonglong2& m = st[i];
       m.x = mul2(m.x, dec.x);
       m.y = mul2(m.y, dec.y);
       d[i] = sum2(fma2(m.y, k.y, mul2(m.x, k.x)));
-      d[kRowsW + i] = sum2(fma2(m.y, q.y, mul2(m.x, q.x)));
+      if constexpr (!kAdvance) d[kRowsW + i] = sum2(fma2(m.y, q.y, mul2(m.x, q.x)));
     }
-    const float tot = warp_sum_transposed(d, lane);
-    const float sqv = __shfl_xor_sync(0xffffffffu, tot, kRowsW);       // lanes 0-15: S q of their row
+    float tot;
+    if constexpr (kAdvance) tot = warp_sum_transposed16(d, lane);
+    else tot = warp_sum_transposed(d, lane);
     const int row = kRowsW * warp + (lane & 15);
     const float u = b * (y[2 * kDim + row] - tot * rk);                // lanes 0-15: u of their row
-    if (lane < kRowsW) a.out[(int64_t)t * a.ldo + h * kDim + row] = __float2bfloat16(sqv * rq + u * (nd * rq * rk));
+    if constexpr (!kAdvance) {
+      const float sqv = __shfl_xor_sync(0xffffffffu, tot, kRowsW);     // lanes 0-15: S q of their row
+      if (lane < kRowsW) a.out[(int64_t)t * a.ldo + h * kDim + row] = __float2bfloat16(sqv * rq + u * (nd * rq * rk));
+    }
     const float ur = u * rk;
 #pragma unroll
     for (int i = 0; i < kRowsW; ++i) {
@@ -172,26 +190,24 @@ __global__ void __launch_bounds__(kDecThreads, 2) kda_decode_kernel(const __grid
   }
 }
 
-bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
-
 }  // namespace
 
 int launch_kda_decode(const KdaArgs& a, cudaStream_t stream) {
-  // empty tensors (no rows, no sequences) have no address
-  if ((a.T > 0 && (a.x == nullptr || a.g == nullptr || a.beta == nullptr || a.out == nullptr)) ||
-      (a.R > 0 && a.seqs == nullptr) || a.a_log == nullptr || a.dt_bias == nullptr || a.conv_w == nullptr ||
-      a.conv_state == nullptr || a.rec_state == nullptr || a.T < 0 || a.T > 0x7fffffff || (a.cs_stride % 2) ||
-      (a.rs_stride % 4) || a.cs_stride < 9 * (int64_t)a.P || a.rs_stride < (int64_t)a.H * kDim * kDim ||
-      !aligned(a.x, 4) || !aligned(a.g, 4) || !aligned(a.conv_w, 16) || !aligned(a.dt_bias, 8) ||
-      !aligned(a.conv_state, 4) || !aligned(a.rec_state, 16) || !aligned(a.seqs, 16) || !aligned(a.beta, 2) ||
-      !aligned(a.out, 2))
-    return kErrArgs;
-  // one row has no pitch: what the caller's tensors state there is not used
-  if (a.T > 1 && ((a.ldx % 2) || (a.ldg % 2) || a.ldx < 3 * (int64_t)a.P || a.ldg < a.P || a.ldb < a.H || a.ldo < a.P))
+  if (!kda_step_args(a) || (a.T > 0 && a.out == nullptr) || !kda_aligned(a.out, 2) || (a.T > 1 && a.ldo < a.P))
     return kErrArgs;
   if (a.R == 0) return kOk;
   if ((int64_t)a.R * a.H > 0x7fffffff) return kErrArgs;
-  kda_decode_kernel<<<(unsigned)(a.R * a.H), kDecThreads, 0, stream>>>(a);
+  kda_decode_kernel<false><<<(unsigned)(a.R * a.H), kDecThreads, 0, stream>>>(a);
+  return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
+}
+
+int launch_kda_advance(const KdaArgs& a, cudaStream_t stream) {
+  if (!kda_step_args(a) || a.n_rows < 0 || a.n_rows > 0x7fffffff || (a.n_rows > 0 && a.rows == nullptr) ||
+      !kda_aligned(a.rows, 4))
+    return kErrArgs;
+  if (a.R == 0) return kOk;
+  if ((int64_t)a.R * a.H > 0x7fffffff) return kErrArgs;
+  kda_decode_kernel<true><<<(unsigned)(a.R * a.H), kDecThreads, 0, stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
 }
 

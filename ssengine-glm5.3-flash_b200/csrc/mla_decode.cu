@@ -264,10 +264,20 @@ SSB_DEVICE void mbar_arrive_n(uint32_t bar, uint32_t n) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n) : "memory");
 }
 
+// Tree form: the positions before the end of row t's visible ones: the context's and those up to the last node on its path
+// (0: a reqs entry outside the table, or a negative length). Positions past 2^31 - 2^7 are past any table.
+SSB_DEVICE int row_tokens(const MlaDecodeArgs& a, int t) {
+  const int len = a.seq_lens[t];
+  if (len < 0 || (a.reqs != nullptr && static_cast<uint32_t>(a.reqs[t]) >= static_cast<uint32_t>(a.R))) return 0;
+  return min(len, 0x7fffff00) + 64 - __clzll(static_cast<long long>(a.ancestors[t]));
+}
+
 // ---- the plan -----------------------------------------------------------------------------------------------------
 // Tokens and units of row t. How many tokens a row's list names is not known before it is read: its share is planned
 // by the list's width or, where that is smaller, the tokens it can name.
+template <bool kTree>
 SSB_DEVICE int row_units(const MlaDecodeArgs& a, int t) {
+  if constexpr (kTree) return row_tokens(a, t) <= 0 ? 0 : min((row_tokens(a, t) + kUnit - 1) / kUnit, kPage / kUnit * a.width);
   int n = a.indices != nullptr ? a.n_idx : 0x7fffff00;
   if (a.seq_lens != nullptr) n = min(n, a.seq_lens[t]);
   if (a.reqs != nullptr && static_cast<uint32_t>(a.reqs[t]) >= static_cast<uint32_t>(a.R)) n = 0;
@@ -285,6 +295,7 @@ struct Segment {
 struct Walk {
   int t, nb, first, lo, hi, cost;               // next row, its units, the units and costs before it, the range, the cost
 };
+template <bool kTree>
 __device__ __noinline__ bool walk_next(const MlaDecodeArgs& a, Walk& w, Segment& s) {
   bool found = false;
   while (!found && w.first < w.hi) {
@@ -295,7 +306,7 @@ __device__ __noinline__ bool walk_next(const MlaDecodeArgs& a, Walk& w, Segment&
     if (++w.t >= a.T) {
       w.first = w.hi;
     } else {
-      w.nb = row_units(a, w.t);
+      w.nb = row_units<kTree>(a, w.t);
     }
   }
   return found;
@@ -309,12 +320,13 @@ constexpr int kRowCost = 10, kCostFrom = 24;      // units; ranges of so many un
 // worst; it is taken where `per` exceeds the equal share by less than those beginnings cost. 34 rows x 1,853 tokens: 38 us
 // in equal ranges, 28 in parts; 62 rows of 2,051 selected tokens: 39 and 35; on the other side 41 rows (median 6,427
 // tokens, 32 heads): 69 and 77; 48 rows (median 4,096, 16 heads): 50 and 59.
+template <bool kTree>
 SSB_DEVICE bool find_range(const MlaDecodeArgs& a, int cta, int ctas, int32_t* sh, Walk& w) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int units = 0, rows = 0;
 #pragma unroll 1
   for (int t = tid; t < a.T; t += kThreads) {
-    const int n = row_units(a, t);
+    const int n = row_units<kTree>(a, t);
     units += n;
     rows += n > 0;
   }
@@ -342,7 +354,7 @@ SSB_DEVICE bool find_range(const MlaDecodeArgs& a, int cta, int ctas, int32_t* s
     int base = 0;
 #pragma unroll 1
     for (int c = 0; c < a.T; c += 32) {
-      const int t = c + lane, nb = t < a.T ? row_units(a, t) : 0, v = nb == 0 ? 0 : parts ? (nb + per - 1) / per : nb + w.cost;
+      const int t = c + lane, nb = t < a.T ? row_units<kTree>(a, t) : 0, v = nb == 0 ? 0 : parts ? (nb + per - 1) / per : nb + w.cost;
       int end = v;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -367,10 +379,11 @@ SSB_DEVICE bool find_range(const MlaDecodeArgs& a, int cta, int ctas, int32_t* s
 }
 
 // Rows without a token: zeros. One warp.
+template <bool kTree>
 __device__ __noinline__ void zero_rows(const MlaDecodeArgs& a, int cta, int h0, int nh, int lane) {
 #pragma unroll 1
   for (int t = cta; t < a.T; t += gridDim.x) {
-    if (row_units(a, t) != 0) continue;
+    if (row_units<kTree>(a, t) != 0) continue;
     if (lane == 0 && a.reqs != nullptr && static_cast<uint32_t>(a.reqs[t]) >= static_cast<uint32_t>(a.R))
       raise_status(a.status, kErrArgs);
     uint4* o = reinterpret_cast<uint4*>(a.out + ((int64_t)t * a.H + h0) * kDv);
@@ -532,7 +545,8 @@ __device__ __noinline__ int stage_q(const MlaDecodeArgs& a, uint8_t* smem, uint3
   return k;
 }
 
-template <bool Q8>
+// kTree: a row sees its first seq_len tokens and, of the 64 after them, those that its word names (the nodes on its path).
+template <bool Q8, bool kTree>
 __global__ void __launch_bounds__(kThreads, 1)
     mla_decode_kernel(const __grid_constant__ CUtensorMap mlat, const __grid_constant__ CUtensorMap mrope,
                       const __grid_constant__ MlaDecodeArgs a) {
@@ -570,9 +584,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc_fence_before();
   Walk walk;
-  if (!find_range(a, cta, gridDim.x, reinterpret_cast<int32_t*>(smem + kOffPlan), walk)) {
+  if (!find_range<kTree>(a, cta, gridDim.x, reinterpret_cast<int32_t*>(smem + kOffPlan), walk)) {
     if (warp == kValueWarp) {
-      zero_rows(a, cta, h0, nh, lane);
+      zero_rows<kTree>(a, cta, h0, nh, lane);
       tmem_dealloc(0, 512);
     }
     return;
@@ -592,9 +606,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     int slot = 0, round = 0;                             // unit u's slot u % kSlots, and u / kSlots
     Segment s;
     bool ok = true;
-    while (ok && walk_next(a, walk, s)) {
+    while (ok && walk_next<kTree>(a, walk, s)) {
       const int32_t* pages = a.table + (int64_t)(a.reqs != nullptr ? a.reqs[s.t] : s.t) * a.width;
-      const int len = a.seq_lens != nullptr ? a.seq_lens[s.t] : 0x7fffffff;
+      const int len = kTree ? row_tokens(a, s.t) : a.seq_lens != nullptr ? a.seq_lens[s.t] : 0x7fffffff;
+      // the tokens all seen; those from there on by the row's word
+      const int plain = kTree ? min(a.seq_lens[s.t], 0x7fffff00) : len;
+      const uint64_t word = kTree ? a.ancestors[s.t] : 0;
       const int32_t* idx = a.indices != nullptr ? a.indices + (int64_t)s.t * a.ld_idx : nullptr;
       int c0 = s.b0, c1 = s.b1;
       if (idx != nullptr) {                              // the row's planned share as units of list columns
@@ -613,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         p = -1;
         if (idx == nullptr) {
           if (c < c1) p = c * kUnit + 32 * half + lane;
-          if (p >= len) p = -1;
+          if (p >= len || (kTree && p >= plain && !(word >> (p - plain) & 1))) p = -1;
           return min(c, c1);
         }
         while (c < c1) {
@@ -649,7 +666,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // row by row: rows that are not there have to be zeros (whatever the cache holds there, NaN too, would meet weight 0
         // in the value product).
         const int64_t y = (int64_t)page * kPage + ((c * kUnit) & (kPage - 1));
-        const bool whole = idx == nullptr && (c + 1) * kUnit <= len && page >= 0 && y + kUnit <= a.cache_rows;
+        const bool whole = idx == nullptr && (c + 1) * kUnit <= plain && page >= 0 && y + kUnit <= a.cache_rows;
         if (whole) {
           if (lane == 0) {
             mbar_arrive_expect_tx(full, w == 3 ? kChunk + kRope : kChunk);
@@ -676,9 +693,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           cp_async_arrive_noinc(full);                   // fires when this thread's copies have landed
         }
         if (lane == 0) {
-          int32_t* word = reinterpret_cast<int32_t*>(slots + slot);
-          if (pair == 0) word[half] = static_cast<int32_t>(present);
-          if (w == 0) word[2] = cn >= c1 ? kLast : kMore;
+          int32_t* told = reinterpret_cast<int32_t*>(slots + slot);
+          if (pair == 0) told[half] = static_cast<int32_t>(present);
+          if (w == 0) told[2] = cn >= c1 ? kLast : kMore;
           mbar_arrive_n(full, whole ? 32 : 1);           // of a whole unit also for the lanes that copied nothing
         }
         if (++slot == kSlots) slot = 0, ++round;
@@ -692,13 +709,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok) drain_tiles(B.full, slot, round);
   } else if (warp == kValueWarp) {
     // ---------------------------------------------------------------- value products
-    zero_rows(a, cta, h0, nh, lane);
+    zero_rows<kTree>(a, cta, h0, nh, lane);
     __syncwarp();
     const bool leader = elect_lane();
     int u = 0, slot = 0, seg = 0;
     Segment s;
     bool ok = true;
-    while (ok && walk_next(a, walk, s)) {
+    while (ok && walk_next<kTree>(a, walk, s)) {
       bool last = false, fresh = true;
       if (seg > 0) ok = mbar_nap(B.o_free, (seg - 1) & 1, abort_flag, a.status);      // the row before has been read
       while (!last) {
@@ -723,7 +740,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int u = 0, slot = 0, round = 0, seg = 0;
     Segment s;
     bool ok = true;
-    while (ok && walk_next(a, walk, s)) {
+    while (ok && walk_next<kTree>(a, walk, s)) {
       bool last = false;
       const int first = u;
       while (!last) {
@@ -772,7 +789,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp < 4) tmem_st_x4(tq + kColV, 0x7478u);
     int u0 = 0, seg = 0, events = 0;                     // the row's first unit
     Segment s;
-    bool more = walk_next(a, walk, s), ok = true;
+    bool more = walk_next<kTree>(a, walk, s), ok = true;
     if (teller) refs[mine] = mine < nh ? kNone : 0.0f;
     int k = stage_q<Q8>(a, smem, tmem, s.t, h0, nh);     // exponent of head mine's query scale
     tc_fence_before();
@@ -932,7 +949,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         refs[mine] = mine < nh ? kNone : 0.0f;
       }
       const Segment done = s;
-      more = walk_next(a, walk, s);
+      more = walk_next<kTree>(a, walk, s);
       if (more) {
         if (!Q8) named_bar(5, kSoftmax);                 // the sums are read: their place takes the query's maxima
         k = stage_q<Q8>(a, smem, tmem, s.t, h0, nh);
@@ -1006,13 +1023,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 // number of CTAs, below). Rows that one CTA finished, or that have no token, are left alone, and those without a valid
 // record: the status tells of them.
 constexpr int kJoinWarps = 16;
+template <bool kTree>
 __global__ void __launch_bounds__(32 * kJoinWarps) mla_join_kernel(const __grid_constant__ MlaDecodeArgs a) {
   __shared__ float4 so[kJoinWarps][32];
   __shared__ float sl[kJoinWarps];
   const int64_t t = blockIdx.x;
   const int h = blockIdx.y, tile = h / kTileH, hh = h - tile * kTileH;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int units = row_units(a, static_cast<int>(t));     // of the inputs alone
+  const int units = row_units<kTree>(a, static_cast<int>(t));     // of the inputs alone
   asm volatile("griddepcontrol.wait;" ::: "memory");       // the parts are written
   if (units == 0) return;
   const MlaRowParts rp = a.rows[t];
@@ -1077,14 +1095,14 @@ int launch_mla_decode(const MlaDecodeArgs& a_in, void* ws, int64_t ws_bytes, cud
   if (a.T < 0 || a.T > 0x7fffffff || a.H <= 0 || a.H > 128) return kErrArgs;
   if (a.T == 0) return kOk;                              // empty tensors have no address: the others are not looked at
   if (a.R <= 0 || a.width <= 0 || a.cache_rows <= 0 || a.cache_rows > 0x7fffffff ||
-      (a.indices == nullptr && a.seq_lens == nullptr) ||
+      (a.indices == nullptr && a.seq_lens == nullptr) || (a.ancestors != nullptr && a.indices != nullptr) ||
       (a.indices != nullptr && (a.n_idx < 0 || (a.T > 1 && a.ld_idx < a.n_idx))) || (a.reqs == nullptr && a.T > a.R))
     return kErrArgs;
   const int64_t most =                                   // units of a row
       a.indices != nullptr ? (a.n_idx + kUnit - 1) / kUnit : (int64_t)(kPage / kUnit) * a.width;
   if (a.T * (most + kRowCost) > 0x7fffffff) return kErrArgs;
   if (a.q == nullptr || a.kv == nullptr || a.table == nullptr || a.out == nullptr || ws == nullptr ||
-      !aligned(a.q, 16) || !aligned(a.kv, 16) || !aligned(a.out, 16) || !aligned(ws, 256))
+      !aligned(a.q, 16) || !aligned(a.kv, 16) || !aligned(a.out, 16) || !aligned(ws, 256) || !aligned(a.ancestors, 8))
     return kErrArgs;
   // one row has no row stride, one head no head stride: what the caller's tensor states there is not used
   if (a.T > 1 && ((a.ldq * eb) % 16 != 0 || a.ldq < kDq)) return kErrArgs;
@@ -1097,13 +1115,15 @@ int launch_mla_decode(const MlaDecodeArgs& a_in, void* ws, int64_t ws_bytes, cud
   a.part_ml = reinterpret_cast<float2*>(p);
   p += up256(slots * kTileH * 8);
   a.part_o = reinterpret_cast<float*>(p);
-  auto* kernel = a.q_e4m3 ? mla_decode_kernel<true> : mla_decode_kernel<false>;
-  static OncePerDevice attr[2];
+  const bool tree = a.ancestors != nullptr;
+  auto* kernel = tree ? (a.q_e4m3 ? mla_decode_kernel<true, true> : mla_decode_kernel<false, true>)
+                      : (a.q_e4m3 ? mla_decode_kernel<true, false> : mla_decode_kernel<false, false>);
+  static OncePerDevice attr[4];
   int device = 0;
   const auto set = [&] {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) == cudaSuccess;
   };
-  if (cudaGetDevice(&device) != cudaSuccess || !attr[a.q_e4m3].done(device, set)) return kErrCuda;
+  if (cudaGetDevice(&device) != cudaSuccess || !attr[2 * tree + a.q_e4m3].done(device, set)) return kErrCuda;
   CUtensorMap mlat = {}, mrope = {};
   if (a.indices == nullptr) {                            // selected tokens are copied row by row
     const int u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
@@ -1126,7 +1146,7 @@ int launch_mla_decode(const MlaDecodeArgs& a_in, void* ws, int64_t ws_bytes, cud
   early.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, mla_join_kernel, a) == cudaSuccess ? kOk : kErrCuda;
+  return cudaLaunchKernelEx(&cfg, tree ? mla_join_kernel<true> : mla_join_kernel<false>, a) == cudaSuccess ? kOk : kErrCuda;
 }
 
 }  // namespace ssb

@@ -133,6 +133,10 @@ struct KdaArgs {
   int64_t ldo = 0;
   int32_t* status = nullptr;           // device status word (bounded copy waits)
   int64_t T = 0;                       // rows of x, g, beta, out
+  const int32_t* rows = nullptr;       // advance: [n_rows] input rows, a sequence's rows are places in it
+  int64_t n_rows = 0;
+  const int32_t* parents = nullptr;    // tree: [T] a row's parent as a node of its sequence, -1: the state block
+  int32_t max_nodes = 0;               // tree: the longest sequence's rows
   uint8_t* ws = nullptr;               // chunk workspace (kda_workspace_bytes); null: allocated on the stream
   int64_t ws_bytes = 0;
   int64_t ws_slots = 0;                // chunk slots the workspace holds (set by the launcher)
@@ -140,6 +144,8 @@ struct KdaArgs {
 int64_t kda_workspace_bytes(int H, int64_t T, int R);
 // The recurrent form over short runs of new tokens (csrc/kda_decode.cu); the workspace fields are not used.
 int launch_kda_decode(const KdaArgs& a, cudaStream_t stream);
+int launch_kda_advance(const KdaArgs& a, cudaStream_t stream);     // kda_decode.cu
+int launch_kda_tree(const KdaArgs& a, cudaStream_t stream);        // kda_tree.cu
 int launch_kda_prefill(const KdaArgs& a, cudaStream_t stream);
 
 // 2D tensor map (no swizzle) over [rows, width] elements of `dtype` (a CUtensorMapDataType) with row pitch ld_bytes;
@@ -253,6 +259,7 @@ struct MlaDecodeArgs {
   const int32_t* indices = nullptr;    // [T, ld_idx] selected positions, -1 = none (null: all visible tokens)
   int64_t ld_idx = 0;
   int32_t n_idx = 0;
+  const uint64_t* ancestors = nullptr; // tree form: bit j of row t: it sees position seq_lens[t] + j too (null: none)
   float bmm1 = 0.0f, bmm2 = 1.0f;
   __nv_bfloat16* out = nullptr;        // [T, H, 512]
   float* lse = nullptr;                // [T, H] or null
@@ -291,6 +298,50 @@ int launch_head_tiles(int heads, int64_t rows_pad, int32_t* tiles, int64_t tile_
                       cudaStream_t stream);
 int launch_concat_cols(const void* a, int64_t lda, int wa, const void* b, int64_t ldb, int wb, void* out, int64_t ldo,
                        int64_t rows, cudaStream_t stream);
+
+// Rows of cache views moved by lists (csrc/move.cu).
+constexpr int kMoveViews = 80;
+struct MoveView {
+  uint8_t* base = nullptr;             // row r: base + r * stride, nbytes of it
+  int64_t stride = 0, nbytes = 0;
+  int64_t rows = 0;
+  int64_t list = 0;
+  int64_t first = 0;                   // the view's first item (set by the launcher)
+};
+struct MoveArgs {
+  int32_t views = 0;
+  int32_t n = 0;                       // rows of a group
+  const int32_t* src = nullptr;        // [lists, groups, n]
+  const int32_t* dst = nullptr;
+  int64_t lists = 0, groups = 0;
+  int64_t slice = 0;                   // bytes of a row that a CTA moves (set by the launcher)
+  int32_t* status = nullptr;
+};
+int launch_move_rows(const MoveView* views, const MoveArgs& a, cudaStream_t stream);
+
+// A beam search's selection (csrc/beam.cu).
+struct BeamPart {                      // of one part of one row: the largest logit, sum of e^(x - m)
+  double sum;
+  float m, pad;
+};
+struct BeamArgs {
+  const void* x = nullptr;             // [G * B, ldx] fp32 or bf16 logits
+  int32_t bf16 = 0;
+  int64_t ldx = 0;
+  int64_t G = 0, V = 0;
+  int32_t B = 0, k = 0;
+  const float* scores = nullptr;       // [G * B]
+  const uint8_t* finished = nullptr;   // [G * B] or null
+  int64_t pad = 0;
+  float* out_scores = nullptr;         // [G, k]
+  int32_t* out_parents = nullptr;
+  int64_t* out_tokens = nullptr;
+  uint64_t* keys = nullptr;            // workspace (set by the launcher)
+  BeamPart* part = nullptr;
+  int32_t parts = 0;
+};
+int64_t beam_workspace_bytes(int64_t G, int64_t B, int64_t V, int64_t k);
+int launch_beam_select(const BeamArgs& a, void* ws, int64_t ws_bytes, cudaStream_t stream);
 
 int device_sm_count();
 

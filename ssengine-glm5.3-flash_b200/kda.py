@@ -18,6 +18,7 @@ import torch
 from . import lib
 
 HEAD_DIM = 128
+MAX_NODES = 64                 # nodes of a tree of drafted tokens
 
 def workspace_bytes(heads: int, T: int, R: int) -> int:
     """Device bytes of the chunk workspace of one prefill call (`ssb_kda_workspace_bytes`)."""
@@ -45,6 +46,16 @@ def _row_pitch(name: str, t: torch.Tensor, rows: int, cols: int) -> int:
             return pitch
     raise ValueError(f"{name}: bf16 [{rows}, >= {cols}] with unit column stride, got {t.dtype} {tuple(t.shape)} strides "
                      f"{t.stride()}")
+
+
+def _check_seqs(seqs: torch.Tensor) -> None:
+    if seqs.dtype is not torch.int32 or seqs.dim() != 2 or seqs.shape[1] != 4 or not seqs.is_contiguous():
+        raise ValueError(f"seqs: contiguous int32 [R, 4], got {seqs.dtype} {tuple(seqs.shape)}")
+
+
+def _check_list(name: str, t: torch.Tensor, n: int | None) -> None:
+    if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n):
+        raise ValueError(f"{name}: contiguous int32 [{'n' if n is None else n}], got {t.dtype} {tuple(t.shape)}")
 
 
 @dataclass
@@ -109,8 +120,7 @@ class KdaLayer:
         P = H * HEAD_DIM
         ldx, ldg = _row_pitch("qkv", qkv, T, 3 * P), _row_pitch("g", g, T, P)
         ldb, ldo = _row_pitch("beta", beta, T, H), _row_pitch("out", out, T, P)
-        if seqs.dtype is not torch.int32 or seqs.dim() != 2 or seqs.shape[1] != 4 or not seqs.is_contiguous():
-            raise ValueError(f"seqs: contiguous int32 [R, 4], got {seqs.dtype} {tuple(seqs.shape)}")
+        _check_seqs(seqs)
         lib.check_device((qkv, g, beta, out, seqs, conv_state, rec_state, self.conv_weight, self.a_log, self.dt_bias),
                          status, stream)
         L = self.c_struct(conv_state, rec_state)
@@ -119,6 +129,54 @@ class KdaLayer:
                                None if status is None else status.data_ptr(), lib.stream_ptr(stream))
         lib.check("ssb_kda_decode", rc)
         return out
+
+    def decode_tree(self, qkv: torch.Tensor, g: torch.Tensor, beta: torch.Tensor, out: torch.Tensor, seqs: torch.Tensor,
+                    parents: torch.Tensor, conv_state: torch.Tensor, rec_state: torch.Tensor, max_nodes: int = 64,
+                    stream=None, status: torch.Tensor | None = None) -> torch.Tensor:
+        """The recurrent form for trees of drafted tokens: the arguments of `decode`, the rows of a sequence the nodes of
+        one tree, node i continuing node parents[first row + i] of its sequence (int32 [T], smaller than i; -1: the
+        request's state). Every node's output is written, the state blocks stay as they are (`advance` moves them on by
+        the accepted path). max_nodes (1..64): the largest tree's nodes, if the caller knows it; smaller trees run
+        faster. `status` receives 1 if a sequence is no such tree, has more nodes, reaches outside the rows or names a
+        negative block (it is skipped). Returns `out`."""
+        so = lib.load()
+        H, T = self.a_log.numel(), qkv.shape[0]
+        P = H * HEAD_DIM
+        ldx, ldg = _row_pitch("qkv", qkv, T, 3 * P), _row_pitch("g", g, T, P)
+        ldb, ldo = _row_pitch("beta", beta, T, H), _row_pitch("out", out, T, P)
+        _check_seqs(seqs)
+        _check_list("parents", parents, T)
+        if not 1 <= max_nodes <= MAX_NODES:
+            raise ValueError(f"max_nodes {max_nodes} outside 1..{MAX_NODES}")
+        lib.check_device((qkv, g, beta, out, seqs, parents, conv_state, rec_state, self.conv_weight, self.a_log,
+                          self.dt_bias), status, stream)
+        L = self.c_struct(conv_state, rec_state)
+        rc = so.ssb_kda_decode_tree(ctypes.byref(L), qkv.data_ptr(), ldx, g.data_ptr(), ldg, beta.data_ptr(), ldb, T,
+                                    parents.data_ptr(), seqs.data_ptr(), seqs.shape[0], max_nodes, out.data_ptr(), ldo,
+                                    None if status is None else status.data_ptr(), lib.stream_ptr(stream))
+        lib.check("ssb_kda_decode_tree", rc)
+        return out
+
+    def advance(self, qkv: torch.Tensor, g: torch.Tensor, beta: torch.Tensor, rows: torch.Tensor, seqs: torch.Tensor,
+                conv_state: torch.Tensor, rec_state: torch.Tensor, stream=None,
+                status: torch.Tensor | None = None) -> None:
+        """Moves the state blocks on along rows of an earlier step, as `decode` of those rows would, without outputs: the
+        accepted path of a tree. rows int32 [n]: rows of qkv, g and beta; `seqs` as in `decode` with first and end row
+        places in `rows`. `status` receives 1 if a sequence reaches outside `rows`, lists a row that is none or names a
+        negative block (it is skipped)."""
+        so = lib.load()
+        H, T = self.a_log.numel(), qkv.shape[0]
+        P = H * HEAD_DIM
+        ldx, ldg, ldb = _row_pitch("qkv", qkv, T, 3 * P), _row_pitch("g", g, T, P), _row_pitch("beta", beta, T, H)
+        _check_seqs(seqs)
+        _check_list("rows", rows, None)
+        lib.check_device((qkv, g, beta, rows, seqs, conv_state, rec_state, self.conv_weight, self.a_log, self.dt_bias),
+                         status, stream)
+        L = self.c_struct(conv_state, rec_state)
+        rc = so.ssb_kda_advance(ctypes.byref(L), qkv.data_ptr(), ldx, g.data_ptr(), ldg, beta.data_ptr(), ldb, T,
+                                rows.data_ptr(), rows.shape[0], seqs.data_ptr(), seqs.shape[0],
+                                None if status is None else status.data_ptr(), lib.stream_ptr(stream))
+        lib.check("ssb_kda_advance", rc)
 
     def conv_qkv(self, qkv: torch.Tensor, seqs: torch.Tensor, conv_state: torch.Tensor, rec_state: torch.Tensor,
                  stream=None):

@@ -29,6 +29,8 @@ from dataclasses import dataclass
 
 import torch
 
+from . import lib
+
 BLOCK_TOKENS = 8576
 PAGE_TOKENS = 128
 PAGES_PER_BLOCK = BLOCK_TOKENS // PAGE_TOKENS          # 67
@@ -82,6 +84,54 @@ def block_bytes(layers, is_dsa, kda_heads: int, pool_fp8: bool = False) -> int:
     return pages + len(dsa) * (PAGES_PER_BLOCK * pool + 2 * 4 * POOL_ROW * 2)
 
 
+MOVE_VIEWS, MOVE_ROWS = 80, 64
+
+
+class RowMover:
+    """Moves rows of cache views by lists on the device (`ssb_move_rows`): beams' states and pages reordered in place, pages
+    forked, accepted tokens compacted, all views in one launch. `views`: tensors on one GPU whose first dimension counts
+    rows, each row contiguous, 16-byte aligned and a multiple of 16 bytes (rows may lie apart, not over one another); at
+    most 80. `lists[i]`: the list of ids that view i goes by (default: all by list 0). The views' addresses are kept."""
+
+    def __init__(self, views, lists=None):
+        self.views = list(views)
+        lists = [0] * len(self.views) if lists is None else [int(v) for v in lists]
+        if not 1 <= len(self.views) <= MOVE_VIEWS or len(lists) != len(self.views) or min(lists) < 0:
+            raise ValueError(f"{len(self.views)} views (1..{MOVE_VIEWS}) with lists {lists}")
+        self.lists = max(lists) + 1
+        self._c = (lib.MoveViewC * len(self.views))()
+        for i, t in enumerate(self.views):
+            size = t.element_size()
+            if t.dim() < 1 or t.shape[0] < 1 or not t[0].is_contiguous():
+                raise ValueError(f"view {i}: rows contiguous in themselves, got {tuple(t.shape)} strides {t.stride()}")
+            nbytes, stride = t[0].numel() * size, t.stride(0) * size
+            if nbytes == 0 or nbytes % 16 or t.data_ptr() % 16 or \
+                    (t.shape[0] > 1 and (stride % 16 or stride < nbytes)):
+                raise ValueError(f"view {i}: rows of {nbytes} bytes, {stride} apart, at {t.data_ptr() % 16} past a 16-byte "
+                                 "boundary (all of them multiples of 16, no overlap)")
+            self._c[i] = lib.MoveViewC(t.data_ptr(), stride, nbytes, t.shape[0], lists[i])
+
+    def __call__(self, src: torch.Tensor, dst: torch.Tensor, stream=None, status: torch.Tensor | None = None) -> None:
+        """Row dst[l, g, i] of every view of list l takes what its row src[l, g, i] held before the call (int32 [lists, G,
+        n] on the device, n <= 64; with one list [G, n] too). The rows of a group g may be permuted in place and one source
+        may go to several rows; an entry with a negative id or equal ids moves nothing, of entries with one destination
+        the first counts. A row that one group writes must not occur in another group of its list. `status` (int32 [1] on
+        the device) receives 1 for an id past a view's rows (nothing is moved for it there)."""
+        so = lib.load()
+        for name, t in (("src", src), ("dst", dst)):
+            if t.dtype is not torch.int32 or not t.is_contiguous() or t.shape != src.shape or \
+                    not (t.dim() == 3 and t.shape[0] >= self.lists or t.dim() == 2 and self.lists == 1) or \
+                    t.shape[-1] > MOVE_ROWS:
+                raise ValueError(f"{name}: contiguous int32 [{self.lists}, groups, <= {MOVE_ROWS}] like the other, got "
+                                 f"{t.dtype} {tuple(t.shape)}")
+        lib.check_device((src, dst, *self.views), status, stream)
+        n = src.shape[-1]
+        rc = so.ssb_move_rows(self._c, len(self.views), src.data_ptr(), dst.data_ptr(),
+                              1 if src.dim() == 2 else src.shape[0], src.shape[-2], n,
+                              None if status is None else status.data_ptr(), lib.stream_ptr(stream))
+        lib.check("ssb_move_rows", rc)
+
+
 class StageKv:
     """The pages of one stage's layers `layers` (model layer ids; `is_dsa(i)` for the kind) over `num_blocks` blocks.
 
@@ -96,6 +146,7 @@ class StageKv:
         self.device = dev
         self.num_blocks = num_blocks
         self.kda_heads = kda_heads
+        self._movers = {}
         self.layers, self.is_dsa = list(layers), is_dsa
         mem = dict(pin_memory=True) if pin else {}       # a host-memory copy of the views (the DRAM tier)
         self.conv_bytes, self.rec_off, state_page = kda_state_bytes(kda_heads)
@@ -155,6 +206,54 @@ class StageKv:
         """(device pointer, bytes) of every tensor (the capacity tiers' view ranges)."""
         ts = self.pages + self.pool + self.tail
         return [(t.data_ptr(), t.numel() * t.element_size()) for t in ts]
+
+    # ------------------------------------------------------------------ several continuations of one request
+    def _mover(self, kind: str) -> RowMover | None:
+        """The movers of the stage's views, made on first use (None: the stage has no such view)."""
+        if kind not in self._movers:
+            n, tokens = self.num_blocks, self.num_blocks * BLOCK_TOKENS
+            latents = [self.pages[j] for j in range(len(self.dsa_layers))]
+            if kind == "states":
+                state = self.rec_off + self.kda_heads * 128 * 128 * 4
+                views = [self.pages[self.slot[i]][:, :state] for i in self.kda_layers] + self.tail
+                lists = [self.group[i] for i in self.kda_layers] + [TAIL_STATE] * len(self.tail)
+            elif kind == "pages":
+                views = [t.view(n * PAGES_PER_BLOCK, PAGE_TOKENS * LATENT_ROW) for t in latents] + \
+                        [t.view(n * PAGES_PER_BLOCK, -1) for t in self.pool]
+                lists = None
+            else:
+                views, lists = [t.view(tokens, LATENT_ROW) for t in latents], None
+            self._movers[kind] = RowMover(views, lists) if views else None
+        return self._movers[kind]
+
+    def move_states(self, src: torch.Tensor, dst: torch.Tensor, stream=None, status=None) -> None:
+        """State blocks by lists, every layer's at once: src, dst int32 [6, G, n] on the device, block ids by state group
+        (the KDA groups, then the tail ring, as a request's `state_blocks`). Beams reordered in place: dst the beams'
+        blocks, src their parents'; a request forked: src its blocks, dst the copy's. `RowMover.__call__`'s rules."""
+        if src.dim() != 3 or src.shape[0] != KDA_GROUPS + 1:
+            raise ValueError(f"src: int32 [{KDA_GROUPS + 1}, groups, n], got {tuple(src.shape)}")
+        mover = self._mover("states")
+        if mover is not None:
+            mover(src, dst, stream, status)
+
+    def move_pages(self, src: torch.Tensor, dst: torch.Tensor, stream=None, status=None) -> None:
+        """KV pages of 128 tokens by lists, every DSA layer's latent rows and pool keys: src, dst int32 [G, n] on the device,
+        page ids (as `kv_pages`)."""
+        if src.dim() != 2:
+            raise ValueError(f"src: int32 [groups, n], got {tuple(src.shape)}")
+        mover = self._mover("pages")
+        if mover is not None:
+            mover(src, dst, stream, status)
+
+    def move_tokens(self, src: torch.Tensor, dst: torch.Tensor, stream=None, status=None) -> None:
+        """Latent rows by lists, every DSA layer's: src, dst int32 [G, n] on the device, slots (page * 128 + position %
+        128). The accepted tokens of a tree brought to its front: src their slots in ascending order, dst the slots from
+        the context's end on. Pool keys are not moved (a pool's key is of four tokens in a row)."""
+        if src.dim() != 2:
+            raise ValueError(f"src: int32 [groups, n], got {tuple(src.shape)}")
+        mover = self._mover("tokens")
+        if mover is not None:
+            mover(src, dst, stream, status)
 
     def tier_ranges(self, stage: int) -> list["ViewRange"]:
         """Every byte range a context owns on this stage, as one block's row of one cache view (the reference's

@@ -26,7 +26,8 @@ EXPORTS = ("ssb_version", "ssb_sf_atom_cols", "ssb_nvfp4_quantize", "ssb_nvfp4_g
            "ssb_nvfp4_gemm_grouped", "ssb_rmsnorm_cols", "ssb_rope", "ssb_transpose_heads", "ssb_concat_cols",
            "ssb_head_tiles", "ssb_moe_route_sigmoid", "ssb_copy_runs", "ssb_indexer_logits_fp8",
            "ssb_indexer_q_quant", "ssb_kpool_insert_fp8", "ssb_kda_decode", "ssb_mla_decode",
-           "ssb_mla_decode_workspace_bytes")
+           "ssb_mla_decode_workspace_bytes", "ssb_mla_decode_tree", "ssb_kda_decode_tree", "ssb_kda_advance",
+           "ssb_move_rows", "ssb_beam_select", "ssb_beam_workspace_bytes")
 
 EPI_F32, EPI_BF16, EPI_SWIGLU = 0, 1, 2
 ROUTE_SOFTMAX, ROUTE_SIGMOID_BIAS = 0, 1
@@ -65,6 +66,12 @@ class KdaLayerC(ctypes.Structure):
                 ("rec_state", ctypes.c_void_p), ("rec_state_stride", ctypes.c_int64)]
 
 
+class MoveViewC(ctypes.Structure):
+    """Mirror of `ssb_move_view`."""
+    _fields_ = [("base", ctypes.c_void_p), ("stride", ctypes.c_int64), ("nbytes", ctypes.c_int64),
+                ("rows", ctypes.c_int64), ("list", ctypes.c_int64)]
+
+
 class MhcParamsC(ctypes.Structure):
     """Mirror of `ssb_mhc_params`."""
     _fields_ = [("hidden", ctypes.c_int32), ("hc_mult", ctypes.c_int32), ("fn", ctypes.c_void_p),
@@ -79,7 +86,8 @@ _LIB = None
 # Kernels each entry point launches (1 unless listed), for the count of this library's launches in a timed region
 KERNELS_PER_CALL = {"ssb_moe_forward": 10, "ssb_moe_forward_profiled": 10, "ssb_mhc_ws": 2,
                     "ssb_kda_prefill": 2, "ssb_kda_prefill_ws": 2, "ssb_kpool_insert": 2, "ssb_kpool_insert_fp8": 2,
-                    "ssb_stage_metadata": 2, "ssb_mla_decode": 2}
+                    "ssb_stage_metadata": 2, "ssb_mla_decode": 2, "ssb_mla_decode_tree": 2,
+                    "ssb_beam_select": 2}
 
 
 class _Counting:
@@ -144,6 +152,15 @@ _SIGS = {
     "ssb_mla_decode": ([_P, _I32, _I64, _I64, _I64, _I32, _P, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _I32, _F, _F, _P,
                         _P, _P, _I64, _P, _P], ctypes.c_int),
     "ssb_mla_decode_workspace_bytes": ([_I64, _I32], ctypes.c_int64),
+    "ssb_mla_decode_tree": ([_P, _I32, _I64, _I64, _I64, _I32, _P, _I64, _P, _I64, _I64, _P, _P, _P, _F, _F, _P, _P, _P,
+                             _I64, _P, _P], ctypes.c_int),
+    "ssb_kda_decode_tree": ([ctypes.POINTER(KdaLayerC), _P, _I64, _P, _I64, _P, _I64, _I64, _P, _P, _I64, _I32, _P, _I64,
+                             _P, _P], ctypes.c_int),
+    "ssb_kda_advance": ([ctypes.POINTER(KdaLayerC), _P, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _P, _P],
+                        ctypes.c_int),
+    "ssb_move_rows": ([ctypes.POINTER(MoveViewC), _I32, _P, _P, _I64, _I64, _I32, _P, _P], ctypes.c_int),
+    "ssb_beam_select": ([_P, _I32, _I64, _I64, _I32, _I64, _P, _P, _I64, _I32, _P, _P, _P, _P, _I64, _P], ctypes.c_int),
+    "ssb_beam_workspace_bytes": ([_I64, _I32, _I64, _I32], ctypes.c_int64),
     "ssb_ipc_export": ([_P, _P, ctypes.POINTER(ctypes.c_int64)], ctypes.c_int),
     "ssb_ipc_open": ([_P, ctypes.POINTER(ctypes.c_void_p)], ctypes.c_int),
     "ssb_ipc_close": ([_P], ctypes.c_int),

@@ -1,5 +1,5 @@
 """Sparse MLA prefill, the attention of new tokens, the FP8 latent-cache append and the FP8 query pack of one DSA layer
-through the C ABI (`ssb_sparse_mla`, `ssb_mla_decode`, `ssb_mla_cache_append`, `ssb_mla_q_pack`).
+through the C ABI (`ssb_sparse_mla`, `ssb_mla_decode`, `ssb_mla_decode_tree`, `ssb_mla_cache_append`, `ssb_mla_q_pack`).
 
 Mirrors the reference's calls: the TRTLLM sparse MLA with FP8 query and cache (`trtllm_batch_decode_with_kv_cache_mla`
 with the indexer's top-k token lists and bmm1 = scale * q_scale * k_scale, bmm2 = k_scale; split at 32,768 rows:
@@ -78,7 +78,38 @@ def decode_selected(q: torch.Tensor, kv_cache: torch.Tensor, indices: torch.Tens
     return _decode(q, kv_cache, indices, page_table, seq_lens, bmm1, out, bmm2, n, reqs, lse, workspace, stream, status)
 
 
-def _decode(q, kv_cache, indices, page_table, seq_lens, bmm1, out, bmm2, n_idx, reqs, lse, workspace, stream, status):
+def decode_tree(q: torch.Tensor, kv_cache: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
+                ancestors: torch.Tensor, bmm1: float, out: torch.Tensor, bmm2: float = 1.0,
+                reqs: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+                workspace: torch.Tensor | None = None, stream=None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """`decode` for the nodes of trees of drafted tokens, a request's nodes in its cache behind its context (at most 64):
+    row t sees positions 0 .. seq_lens[t] - 1 and seq_lens[t] + j for every bit j of ancestors[t] (int64 [T]: the nodes on
+    the row's path, itself among them, as `tree_masks` makes them; any set is taken). A row without either gets zeros."""
+    if ancestors.dtype is not torch.int64 or ancestors.shape != q.shape[:1] or not ancestors.is_contiguous():
+        raise ValueError(f"ancestors: contiguous int64 [{q.shape[0]}], got {ancestors.dtype} {tuple(ancestors.shape)}")
+    if seq_lens is None:
+        raise ValueError("seq_lens: int32 [T], the context before each row's tree")
+    return _decode(q, kv_cache, None, page_table, seq_lens, bmm1, out, bmm2, None, reqs, lse, workspace, stream, status,
+                   ancestors)
+
+
+def tree_masks(parents) -> tuple[torch.Tensor, torch.Tensor]:
+    """One tree's parents (a parent before its children, -1 for a root; at most 64 nodes) -> (ancestors int64 [n]: bit j set
+    where node j is on the node's path, itself among them; depths int64 [n]: nodes above it, so that a node's position is
+    the context's length + its depth), on the host. ValueError if it is no such tree."""
+    masks, depths = [], []
+    for i, p in enumerate(parents):
+        p = int(p)
+        if not -1 <= p < i or i > 63:
+            raise ValueError(f"node {i} with parent {p}: parents come first, at most 64 nodes")
+        masks.append((masks[p] if p >= 0 else 0) | 1 << i)
+        depths.append(depths[p] + 1 if p >= 0 else 0)
+    signed = [m - (1 << 64) if m >> 63 else m for m in masks]
+    return torch.tensor(signed, dtype=torch.int64), torch.tensor(depths, dtype=torch.int64)
+
+
+def _decode(q, kv_cache, indices, page_table, seq_lens, bmm1, out, bmm2, n_idx, reqs, lse, workspace, stream, status,
+            ancestors=None):
     so = lib.load()
     e4m3 = q.dtype is torch.uint8
     if not (e4m3 or q.dtype is torch.bfloat16) or q.dim() != 3 or q.shape[2] != DQ or q.stride(2) != 1:
@@ -105,13 +136,21 @@ def _decode(q, kv_cache, indices, page_table, seq_lens, bmm1, out, bmm2, n_idx, 
     if workspace is not None and (workspace.dtype != torch.uint8 or not workspace.is_contiguous() or
                                   workspace.numel() < need):
         raise ValueError(f"workspace: contiguous uint8 of {need} bytes or more")
-    lib.check_device((q, kv_cache, page_table, out, seq_lens, indices, reqs, lse, workspace), status, stream)
+    lib.check_device((q, kv_cache, page_table, out, seq_lens, indices, reqs, lse, workspace, ancestors), status,
+                     stream)
     if workspace is None:
         workspace = lib.stream_scratch(q.device, need, stream)
     ptr = lambda t: None if t is None else t.data_ptr()
     ldq, head_stride, _ = q.stride()
     # a selection without columns has no address of its own (NULL means every visible token): any other one, never read
     listed = None if indices is None else indices.data_ptr() or page_table.data_ptr()
+    if ancestors is not None:
+        rc = so.ssb_mla_decode_tree(q.data_ptr(), int(e4m3), ldq, head_stride, T, H, kv_cache.data_ptr(),
+                                    kv_cache.shape[0], page_table.data_ptr(), rows, width, ptr(reqs), ptr(seq_lens),
+                                    ptr(ancestors), bmm1, bmm2, out.data_ptr(), ptr(lse), workspace.data_ptr(),
+                                    workspace.numel(), ptr(status), lib.stream_ptr(stream))
+        lib.check("ssb_mla_decode_tree", rc)
+        return out
     rc = so.ssb_mla_decode(q.data_ptr(), int(e4m3), ldq, head_stride, T, H, kv_cache.data_ptr(),
                            kv_cache.shape[0], page_table.data_ptr(), rows, width, ptr(reqs), ptr(seq_lens),
                            listed, 0 if indices is None else indices.stride(0), n_idx or 0, bmm1, bmm2,
