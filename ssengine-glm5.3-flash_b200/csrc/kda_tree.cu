@@ -4,11 +4,23 @@
 // Per head, with the conv, norms and gates of kda_decode.cu along each node's path (the taps before a root come from the
 // block's conv rows): S_i = S_parent diag(a_i) + u_i k_i^T, u_i = b_i (v_i - S_parent diag(a_i) k_i), o_i = D^-1/2 S_i q_i.
 // Written out along the path, with A_i the product of the decays on it and A_ij that of the decays below j,
-//   u_i = b_i (v_i - S (A_i k_i) - sum_{j above i} u_j M_ij),   M_ij = (A_ij k_j) . k_i
-//   o_i = D^-1/2 (S (A_i q_i) + sum_{j on the path} u_j N_ij),  N_ij = (A_ij k_j) . q_i
-// so the state S [value, key] is read once, whatever the nodes, and no node's own state is ever formed: two products of S
-// with the nodes' vectors, scalars for the pairs of a node and one above it, and a substitution down the tree for each
-// value row. The decays multiply down the path (each is at most 1; quotients of cumulated ones would overflow).
+//   u_i = b_i (w_i - sum_{j above i} u_j M_ij),   w_i = v_i - S (A_i k_i),   M_ij = (A_ij k_j) . k_i
+//   o_i = S (A_i q_i) + sum_{j on the path} u_j N_ij,                        N_ij = (A_ij k_j) . q_i   (q with D^-1/2)
+// and, since the u are linear in the w with scalars of the path alone, o_i = S (A_i q_i) + sum_{j on the path} P_ij w_j with
+// P_i (1 + b M) = N_i b: a substitution up each node's path, on scalars. So the state S [value, key] is read once, whatever
+// the nodes, no node's own state is formed, and nothing but the scalars goes node after node. A_ij = 2^(G_i - G_j), G the sum
+// of the log2 of the decays down the path: differences along a path are never positive, where quotients of products would
+// overflow.
+//
+// One CTA a (request, head), 256 threads, two CTAs an SM:
+//   conv and gates: a thread a pair of channels of q, k or g, in shared memory in place (a node's row is overwritten when
+//       the nodes below it are done: from the last node to the first);
+//   pairs: a warp a node and those above it, 4 channels a lane;
+//   products: [S (A k) | S (A q)] on the tensor cores, M = 128 value rows, N = 2 nodes, K = 128 keys, tcgen05 kind::f16: S in
+//       TMEM and the vectors in shared memory, both as two bf16 parts, three of the four products (what is left out is below
+//       2^-16 of a product; the output has 8 bits). S comes straight from global memory, a value row a lane;
+//   outputs: a value row a thread, as the products lie in TMEM.
+// The exponentials are the short ones (error about 2^-20 here): nothing computed here is kept but the bf16 outputs.
 #include "common.cuh"
 #include "kda_math.cuh"
 #include "ops.h"
@@ -17,174 +29,446 @@ namespace ssb {
 namespace {
 
 constexpr int kDim = 128;
-constexpr int kTreeThreads = 256;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxNodes = 64;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr uint32_t kColS = 0, kColD = 128, kCols = 256;    // TMEM: S as 64 columns of high and 64 of low parts; the products
 
 template <int N>
 struct TreeSmem {
-  float k[N][kDim];            // keys, normalised; once the pairs are done, S (A q)
-  float dec[N][kDim];          // decays
-  float aq[N][kDim];           // queries, then A q
-  float ak[N][kDim];           // A k
-  float u[N][kDim];            // values, then u
-  float m[N][N], n[N][N];      // the pairs
+  union {
+    struct {
+      float k[N][kDim];                    // keys, normalised
+      float q[N][kDim];                    // queries, normalised and scaled
+    };
+    uint8_t op[2][2][2 * N][128];          // A k, A q: high and low parts, 2 chunks of 64 keys [rows x 128 B], swizzled
+    float w[N][kDim];                      // values, then w
+  };
+  float g[N][kDim];                        // log2 of the decays, summed down the path
+  float pn[N * (N + 1) / 2];               // N_ij, then P_ij: of node i from off[i] on, by distance
+  float pm[N * (N - 1) / 2];               // M_ij: of node i from off[i] - i on, by distance - 1
+  uint64_t mask[N];                        // a node's path, itself among it
   float beta[N];
-  int32_t parent[N];
-  int32_t tap[N][3];           // the conv's rows before a node's own, newest first: a node, or -1 - j: the j-th newest kept row
+  uint16_t off[N];
+  uint64_t bar;
+  uint32_t tmem;
+  int32_t abort;
 };
 
+SSB_DEVICE float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+SSB_DEVICE float sigmoid_short(float x) { return __fdividef(1.0f, 1.0f + ex2(-kLog2e * x)); }
+SSB_DEVICE float silu_short(float x) { return __fdividef(x, 1.0f + ex2(-kLog2e * x)); }
+// Two values as bf16 pairs: the high parts, and what they leave.
+SSB_DEVICE void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  const __nv_bfloat162 l = __floats2bfloat162_rn(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xFFFF0000u));
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+// The last node of a path and the path above it.
+SSB_DEVICE int pop(uint64_t& path) {
+  const int i = 63 - __clzll(static_cast<long long>(path));
+  path ^= 1ull << i;
+  return i;
+}
+SSB_DEVICE void ld8(const float* p, float* v) {              // 32 bytes
+  asm volatile("ld.global.nc.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+               : "l"(p));
+}
+SSB_DEVICE void tmem_ld_x8(uint32_t taddr, float (&v)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+               : "r"(taddr));
+}
+// D[tmem] (+)= A B with bf16 A in TMEM (a row a lane, 2 values a column) and B in shared memory.
+SSB_DEVICE void mma_f16_ta(uint32_t d, uint32_t a, uint64_t bd, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(bd), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+// A node's conv taps of a channel pair: its own row's value x0, then those of the three rows before it on its path, the
+// block's kept rows behind a root (held[0] the newest). row(j): node j's value.
+template <class Row>
+SSB_DEVICE float2 conv4(const float2 (&p)[4], uint32_t x0, uint64_t above, const uint32_t (&held)[3], Row row) {
+  uint32_t x[4] = {0, 0, 0, x0};
+  if (__popcll(above) >= 3) {
+    x[2] = row(pop(above)), x[1] = row(pop(above)), x[0] = row(pop(above));
+  } else if (above == 0) {
+    x[2] = held[0], x[1] = held[1], x[0] = held[2];
+  } else {
+    x[2] = row(pop(above));
+    if (above == 0) {
+      x[1] = held[0], x[0] = held[1];
+    } else {
+      x[1] = row(pop(above)), x[0] = held[0];
+    }
+  }
+  const float2 x1 = bf2(x[0]), x2 = bf2(x[1]), x3 = bf2(x[2]), x4 = bf2(x[3]);
+  float2 o;
+  o.x = silu_short(fmaf(p[1].y, x4.x, fmaf(p[1].x, x3.x, fmaf(p[0].y, x2.x, p[0].x * x1.x))));
+  o.y = silu_short(fmaf(p[3].y, x4.y, fmaf(p[3].x, x3.y, fmaf(p[2].y, x2.y, p[2].x * x1.y))));
+  return o;
+}
+
 template <int N>
-__global__ void __launch_bounds__(kTreeThreads) kda_tree_kernel(const __grid_constant__ KdaArgs a) {
-  extern __shared__ __align__(16) uint8_t raw_smem[];
+__global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_constant__ KdaArgs a) {
+  extern __shared__ __align__(1024) uint8_t raw_smem[];
   TreeSmem<N>& sm = *reinterpret_cast<TreeSmem<N>*>(raw_smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int r = blockIdx.x / a.H, h = blockIdx.x - r * a.H;
   const int4 sq = __ldg(reinterpret_cast<const int4*>(a.seqs) + r);   // {first row, end row, state block, has state}
   const int s = sq.x, n = sq.y - sq.x;
-  bool bad = s < 0 || sq.y < s || sq.y > a.T || n > N || sq.z < 0;
-  if (!bad && tid < n) {
-    const int p = a.parents[s + tid];
-    sm.parent[tid] = p;
-    bad = p < -1 || p >= tid;
+  if (s < 0 || sq.y < s || sq.y > a.T || n > N || sq.z < 0 || (smem_u32(raw_smem) & 1023)) {
+    if (tid == 0 && h == 0) raise_status(a.status, kErrArgs);
+    return;
+  }
+  if (n == 0) return;
+  const bool init = sq.w != 0;
+
+  // ---- the state's loads: a value row a lane, half of its keys a thread
+  const int quarter = warp & 3, half = warp >> 2, v = 32 * quarter + lane;
+  float st[64];
+  {
+    const float* S = a.rec_state + (int64_t)sq.z * a.rs_stride + ((int64_t)h * kDim + v) * kDim + 64 * half;
+    const bool wide = (reinterpret_cast<uintptr_t>(S) & 31) == 0;
+#pragma unroll
+    for (int c = 0; c < 64; c += 8) {
+      if (init && wide) {
+        ld8(S + c, st + c);
+      } else if (init) {
+        const float4 x = __ldg(reinterpret_cast<const float4*>(S + c)), y = __ldg(reinterpret_cast<const float4*>(S + c + 4));
+        st[c] = x.x, st[c + 1] = x.y, st[c + 2] = x.z, st[c + 3] = x.w;
+        st[c + 4] = y.x, st[c + 5] = y.y, st[c + 6] = y.z, st[c + 7] = y.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) st[c + j] = 0.0f;
+      }
+    }
+  }
+  // ---- the inputs of q, k and g into their places (threads 0-191: a pair of channels each); the tree (threads 192-255)
+  const int pair = tid & 63, part = tid >> 6;
+  const bool in_q = part == 0, in_k = part == 1, in_g = part == 2;
+  float* column = in_q ? &sm.q[0][2 * pair] : in_k ? &sm.k[0][2 * pair] : &sm.g[0][2 * pair];
+  bool bad = false;
+  if (part < 3) {
+    const uint32_t* in = reinterpret_cast<const uint32_t*>(in_g ? a.g + h * kDim + 2 * pair
+                                                                : a.x + (int64_t)part * a.P + h * kDim + 2 * pair);
+    const int64_t pitch = (in_g ? a.ldg : a.ldx) / 2;
+    in += s * pitch;
+#pragma unroll 1
+    for (int i = 0; i < n; i += 8) {
+      uint32_t x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = __ldg(in + min(i + j, n - 1) * pitch);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (i + j < n) column[(i + j) * kDim] = __uint_as_float(x[j]);
+    }
+  } else {
+    // thread 192 + i: node i. The parents go through the places of the paths
+    const int i = tid - 192;
+    int p = -1;
+    if (i < n) {
+      p = a.parents[s + i];
+      bad = p < -1 || p >= i;
+      sm.beta[i] = sigmoid_short(__bfloat162float(a.beta[(int64_t)(s + i) * a.ldb + h]));
+      sm.mask[i] = static_cast<uint64_t>(static_cast<int64_t>(p));
+    }
+    bad = named_bar_or(1, 64, bad);
+    uint64_t path = 0;
+    if (i < n && !bad) {
+      path = 1ull << i;
+      while (p >= 0) {
+        path |= 1ull << p;
+        p = static_cast<int>(static_cast<int64_t>(sm.mask[p]));
+      }
+    }
+    named_bar(1, 64);
+    if (i < n) sm.mask[i] = path;
+    // offsets: the sum of the path lengths before the node, a warp each, the second one's behind the first's
+    const int len = __popcll(path);
+    int end = len;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, end, o);
+      if (lane >= o) end += x;
+    }
+    if (i == 31) sm.abort = end;
+    named_bar(1, 64);
+    if (i >= 32) end += sm.abort;
+    if (i < n) sm.off[i] = static_cast<uint16_t>(end - len);
   }
   if (__syncthreads_or(bad)) {
     if (tid == 0 && h == 0) raise_status(a.status, kErrArgs);
     return;
   }
-  if (n <= 0) return;
-  if (tid < n) {
-    int p = tid, kept = 0;
-    for (int j = 0; j < 3; ++j) {
-      p = p >= 0 ? sm.parent[p] : -1;
-      sm.tap[tid][j] = p >= 0 ? p : -1 - kept++;
-    }
-    sm.beta[tid] = sigmoid_fast(__bfloat162float(a.beta[(int64_t)(s + tid) * a.ldb + h]));
+  if (tid == 0) {
+    sm.abort = 0;
+    mbar_init(smem_u32(&sm.bar), 1);
+    fence_barrier_init();
   }
-  __syncthreads();
-  const bool init = sq.w != 0;
+  if (warp == 0) {
+    tmem_alloc(smem_u32(&sm.tmem), kCols);
+    tmem_relinquish();
+  }
 
-  // ---- conv, gates: a pair of channels a thread, node after node
-  const bool conv = tid < 192;
-  const int pair = tid & 63, part = tid >> 6;
-  const int64_t col = (int64_t)part * a.P + h * kDim + 2 * pair;
-  if (conv) {
-    const uint32_t* x = reinterpret_cast<const uint32_t*>(a.x + col);
-    const int64_t pitch = a.ldx / 2;
-    const __nv_bfloat16* cs = a.conv_state + (int64_t)sq.z * a.cs_stride + col;
-    uint32_t held[3] = {0, 0, 0};                      // newest first
+  // ---- conv and gates in place
+  const __nv_bfloat16* cs = a.conv_state + (int64_t)sq.z * a.cs_stride + h * kDim + 2 * pair;   // of q; k, v: + P, + 2 P
+  if (part < 2) {
+    uint32_t held[3] = {0, 0, 0};
     if (init)
-      for (int j = 0; j < 3; ++j) held[j] = *reinterpret_cast<const uint32_t*>(cs + (int64_t)(2 - j) * 3 * a.P);
-    const uint4 wv = __ldg(reinterpret_cast<const uint4*>(a.conv_w + col * 4));     // 2 channels x 4 taps
-    const float2 p0 = bf2(wv.x), p1 = bf2(wv.y), p2 = bf2(wv.z), p3 = bf2(wv.w);
-    float* to = part == 0 ? &sm.aq[0][0] : part == 1 ? &sm.k[0][0] : &sm.u[0][0];
-    for (int i = 0; i < n; ++i) {
-      float2 xs[4];
-      xs[3] = bf2(__ldg(x + (s + i) * pitch));
-      for (int j = 0; j < 3; ++j) {
-        const int t = sm.tap[i][j];
-        xs[2 - j] = bf2(t >= 0 ? __ldg(x + (s + t) * pitch) : t == -1 ? held[0] : t == -2 ? held[1] : held[2]);
-      }
-      float2 o;
-      o.x = silu_fast(fmaf(p1.y, xs[3].x, fmaf(p1.x, xs[2].x, fmaf(p0.y, xs[1].x, p0.x * xs[0].x))));
-      o.y = silu_fast(fmaf(p3.y, xs[3].y, fmaf(p3.x, xs[2].y, fmaf(p2.y, xs[1].y, p2.x * xs[0].y))));
-      *reinterpret_cast<float2*>(to + i * kDim + 2 * pair) = o;
+      for (int j = 0; j < 3; ++j) held[j] = *reinterpret_cast<const uint32_t*>(cs + ((int64_t)(2 - j) * 3 + part) * a.P);
+    const uint4* wp = reinterpret_cast<const uint4*>(a.conv_w + ((int64_t)part * a.P + h * kDim + 2 * pair) * 4);
+    const uint4 wv = __ldg(wp);                              // 2 channels x 4 taps
+    const float2 p[4] = {bf2(wv.x), bf2(wv.y), bf2(wv.z), bf2(wv.w)};
+    const auto row = [&](int j) { return __float_as_uint(column[j * kDim]); };
+#pragma unroll 1
+    for (int i = n - 1; i >= 0; i -= 4) {                    // 4 nodes read before the first is written
+      float2 o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i - j >= 0) o[j] = conv4(p, row(i - j), sm.mask[i - j] ^ (1ull << (i - j)), held, row);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i - j >= 0) *reinterpret_cast<float2*>(column + (i - j) * kDim) = o[j];
     }
-  } else {
-    const uint32_t* g = reinterpret_cast<const uint32_t*>(a.g + h * kDim + 2 * pair);
+  } else if (in_g) {
     const float2 dt = __ldg(reinterpret_cast<const float2*>(a.dt_bias + h * kDim) + pair);
-    const float rate = exp_fast(__ldg(a.a_log + h));
-    for (int i = 0; i < n; ++i) {
-      const float2 v = bf2(__ldg(g + (s + i) * (a.ldg / 2)));
-      float2 o;
-      o.x = exp_fast(a.lower_bound * sigmoid_fast(rate * (v.x + dt.x)));
-      o.y = exp_fast(a.lower_bound * sigmoid_fast(rate * (v.y + dt.y)));
-      *reinterpret_cast<float2*>(&sm.dec[i][2 * pair]) = o;
+    const float rate = exp_fast(__ldg(a.a_log + h)), lb = a.lower_bound * kLog2e;
+#pragma unroll 1
+    for (int i = 0; i < n; i += 4) {
+      float2 o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (i + j >= n) continue;
+        const float2 x = bf2(__float_as_uint(column[(i + j) * kDim]));
+        o[j].x = lb * sigmoid_short(rate * (x.x + dt.x));
+        o[j].y = lb * sigmoid_short(rate * (x.y + dt.y));
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (i + j >= n) continue;
+        uint64_t above = sm.mask[i + j] ^ (1ull << (i + j));
+        if (above != 0) {
+          const float2 up = *reinterpret_cast<float2*>(column + pop(above) * kDim);
+          o[j].x += up.x, o[j].y += up.y;
+        }
+        *reinterpret_cast<float2*>(column + (i + j) * kDim) = o[j];
+      }
     }
   }
+  tc_fence_before();
   __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem;
+  // ---- the state's parts to TMEM
+  {
+    const uint32_t at = tmem + (static_cast<uint32_t>(32 * quarter) << 16) + kColS + 32 * half;
+    float hi[32], lo[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      uint32_t x, y;
+      split2(st[2 * j], st[2 * j + 1], x, y);
+      hi[j] = __uint_as_float(x), lo[j] = __uint_as_float(y);
+    }
+    tmem_st_32x32b_x32(at, hi);
+    tmem_st_32x32b_x32(at + 64, lo);
+    tmem_st_wait();
+  }
 
   // ---- norms: a warp a node, 4 channels a lane
-  for (int i = warp; i < n; i += kTreeThreads / 32) {
-    float4 q = *reinterpret_cast<float4*>(&sm.aq[i][4 * lane]), k = *reinterpret_cast<float4*>(&sm.k[i][4 * lane]);
-    float nq = q.x * q.x + q.y * q.y + q.z * q.z + q.w * q.w, nk = k.x * k.x + k.y * k.y + k.z * k.z + k.w * k.w;
-    for (int o = 16; o > 0; o >>= 1) {
-      nq += __shfl_xor_sync(0xffffffffu, nq, o);
-      nk += __shfl_xor_sync(0xffffffffu, nk, o);
-    }
-    const float rq = a.scale * rsqrtf(nq + 1e-6f), rk = rsqrtf(nk + 1e-6f);
-    *reinterpret_cast<float4*>(&sm.aq[i][4 * lane]) = make_float4(q.x * rq, q.y * rq, q.z * rq, q.w * rq);
-    *reinterpret_cast<float4*>(&sm.k[i][4 * lane]) = make_float4(k.x * rk, k.y * rk, k.z * rk, k.w * rk);
+#pragma unroll 1
+  for (int i = warp; i < n; i += kWarps) {
+    float4* kp = reinterpret_cast<float4*>(&sm.k[i][4 * lane]);
+    float4* qp = reinterpret_cast<float4*>(&sm.q[i][4 * lane]);
+    float4 q = *qp, k = *kp;
+    const float nk = k.x * k.x + k.y * k.y + k.z * k.z + k.w * k.w, nq = q.x * q.x + q.y * q.y + q.z * q.z + q.w * q.w;
+    float t = (lane < 16 ? nk : nq) + __shfl_xor_sync(0xffffffffu, lane < 16 ? nq : nk, 16);   // lanes 0-15: k's, 16-31: q's
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    t = rsqrtf(t + 1e-6f);
+    const float rk = __shfl_sync(0xffffffffu, t, 0), rq = a.scale * __shfl_sync(0xffffffffu, t, 16);
+    *kp = make_float4(k.x * rk, k.y * rk, k.z * rk, k.w * rk);
+    *qp = make_float4(q.x * rq, q.y * rq, q.z * rq, q.w * rq);
   }
   __syncthreads();
-
-  // ---- the pairs of a node and those above it, the decays multiplied up the path
-  for (int i = warp; i < n; i += kTreeThreads / 32) {
-    const float4 q = *reinterpret_cast<float4*>(&sm.aq[i][4 * lane]), k = *reinterpret_cast<float4*>(&sm.k[i][4 * lane]);
-    float4 f = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-    for (int j = i; j >= 0; j = sm.parent[j]) {
-      const float4 kj = *reinterpret_cast<float4*>(&sm.k[j][4 * lane]), dj = *reinterpret_cast<float4*>(&sm.dec[j][4 * lane]);
-      const float4 t = make_float4(f.x * kj.x, f.y * kj.y, f.z * kj.z, f.w * kj.w);
-      float m = t.x * k.x + t.y * k.y + t.z * k.z + t.w * k.w, nn = t.x * q.x + t.y * q.y + t.z * q.z + t.w * q.w;
-      for (int o = 16; o > 0; o >>= 1) {
-        m += __shfl_xor_sync(0xffffffffu, m, o);
-        nn += __shfl_xor_sync(0xffffffffu, nn, o);
-      }
-      if (lane == 0) sm.m[i][j] = m, sm.n[i][j] = nn;
-      f = make_float4(f.x * dj.x, f.y * dj.y, f.z * dj.z, f.w * dj.w);
+  // ---- the pairs of a node and those above it
+#pragma unroll 1
+  for (int i = warp; i < n; i += kWarps) {
+    const float4 k = *reinterpret_cast<float4*>(&sm.k[i][4 * lane]), q = *reinterpret_cast<float4*>(&sm.q[i][4 * lane]);
+    const float4 g = *reinterpret_cast<float4*>(&sm.g[i][4 * lane]);
+    uint64_t path = sm.mask[i];
+    int at = sm.off[i];
+    for (int d = 0; path != 0; ++d) {
+      const int j = pop(path);
+      const float4 kj = *reinterpret_cast<float4*>(&sm.k[j][4 * lane]), gj = *reinterpret_cast<float4*>(&sm.g[j][4 * lane]);
+      const float x = kj.x * ex2(g.x - gj.x), y = kj.y * ex2(g.y - gj.y);
+      const float z = kj.z * ex2(g.z - gj.z), w = kj.w * ex2(g.w - gj.w);
+      const float m = x * k.x + y * k.y + z * k.z + w * k.w, nn = x * q.x + y * q.y + z * q.z + w * q.w;
+      float t = (lane < 16 ? m : nn) + __shfl_xor_sync(0xffffffffu, lane < 16 ? nn : m, 16);
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+      if (lane == 0 && d > 0) sm.pm[at - i + d - 1] = t;
+      if (lane == 16) sm.pn[at + d] = t;
     }
-    *reinterpret_cast<float4*>(&sm.ak[i][4 * lane]) = make_float4(k.x * f.x, k.y * f.y, k.z * f.z, k.w * f.w);
-    *reinterpret_cast<float4*>(&sm.aq[i][4 * lane]) = make_float4(q.x * f.x, q.y * f.y, q.z * f.z, q.w * f.w);
   }
-  __syncthreads();
-
-  // ---- S (A k) and the substitution (threads 0-127), S (A q) (threads 128-255): a value row a thread
-  const int v = tid & 127;
-  const bool first = tid < 128;
-  float row[kDim];
+  // ---- A k and A q as the products' second operand, in the place of k and q
   {
-    const float* S = a.rec_state + (int64_t)sq.z * a.rs_stride + ((int64_t)h * kDim + v) * kDim;
+    uint32_t hi[N / kWarps][4], lo[N / kWarps][4];
 #pragma unroll
-    for (int c = 0; c < kDim; c += 4) {
-      const float4 w = init ? __ldg(reinterpret_cast<const float4*>(S + c)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      row[c] = w.x, row[c + 1] = w.y, row[c + 2] = w.z, row[c + 3] = w.w;
+    for (int t = 0; t < N / kWarps; ++t) {
+      const int i = warp + kWarps * t;
+      if (i >= n) continue;
+      const float4 k = *reinterpret_cast<float4*>(&sm.k[i][4 * lane]), q = *reinterpret_cast<float4*>(&sm.q[i][4 * lane]);
+      const float4 g = *reinterpret_cast<float4*>(&sm.g[i][4 * lane]);
+      const float x = ex2(g.x), y = ex2(g.y), z = ex2(g.z), w = ex2(g.w);
+      split2(k.x * x, k.y * y, hi[t][0], lo[t][0]);
+      split2(k.z * z, k.w * w, hi[t][1], lo[t][1]);
+      split2(q.x * x, q.y * y, hi[t][2], lo[t][2]);
+      split2(q.z * z, q.w * w, hi[t][3], lo[t][3]);
+    }
+    __syncthreads();
+    const int chunk = lane >> 4, granule = (lane & 15) >> 1, within = (lane & 1) * 8;
+#pragma unroll
+    for (int t = 0; t < N / kWarps; ++t) {
+      const int i = warp + kWarps * t;
+      if (i >= n) continue;
+      const int at = ((granule ^ (i & 7)) << 4) + within;      // rows i and N + i swizzle alike
+      *reinterpret_cast<uint2*>(&sm.op[0][chunk][i][at]) = make_uint2(hi[t][0], hi[t][1]);
+      *reinterpret_cast<uint2*>(&sm.op[1][chunk][i][at]) = make_uint2(lo[t][0], lo[t][1]);
+      *reinterpret_cast<uint2*>(&sm.op[0][chunk][N + i][at]) = make_uint2(hi[t][2], hi[t][3]);
+      *reinterpret_cast<uint2*>(&sm.op[1][chunk][N + i][at]) = make_uint2(lo[t][2], lo[t][3]);
     }
   }
-  for (int i = 0; i < n; ++i) {
-    const float4* w = reinterpret_cast<const float4*>(first ? sm.ak[i] : sm.aq[i]);
-    float d0 = 0.0f, d1 = 0.0f;
-#pragma unroll
-    for (int c = 0; c < kDim; c += 8) {
-      const float4 w0 = w[c / 4], w1 = w[c / 4 + 1];
-      d0 = fmaf(row[c], w0.x, fmaf(row[c + 1], w0.y, fmaf(row[c + 2], w0.z, fmaf(row[c + 3], w0.w, d0))));
-      d1 = fmaf(row[c + 4], w1.x, fmaf(row[c + 5], w1.y, fmaf(row[c + 6], w1.z, fmaf(row[c + 7], w1.w, d1))));
-    }
-    const float d = d0 + d1;
-    if (first) {
-      float t = sm.u[i][v] - d;
-      for (int j = sm.parent[i]; j >= 0; j = sm.parent[j]) t = fmaf(-sm.m[i][j], sm.u[j][v], t);
-      sm.u[i][v] = sm.beta[i] * t;
-    } else {
-      sm.k[i][v] = d;
-    }
-  }
+  fence_proxy_async_smem();
+  tc_fence_before();
   __syncthreads();
-  for (int i = first ? 0 : 1; i < n; i += 2) {
-    float t = sm.k[i][v];
-    for (int j = i; j >= 0; j = sm.parent[j]) t = fmaf(sm.n[i][j], sm.u[j][v], t);
-    a.out[(int64_t)(s + i) * a.ldo + h * kDim + v] = __float2bfloat16(t);
+  const uint32_t bar = smem_u32(&sm.bar);
+  if (tid == 0) {
+    tc_fence_after();
+    constexpr uint32_t idesc = idesc_bf16(128, 2 * N);
+    uint32_t acc = 0;
+#pragma unroll 1
+    for (int t = 0; t < 3; ++t) {                              // high x high, high x low, low x high
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const uint64_t bd = smem_desc(smem_u32(&sm.op[t == 1][c][0][0]), 0, 1024, 2);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          mma_f16_ta(tmem + kColD, tmem + kColS + (t == 2 ? 64 : 0) + 32 * c + 8 * ks, bd + 2 * ks, idesc, acc);
+          acc = 1;
+        }
+      }
+    }
+    tc_commit(bar);
   }
+  // ---- meanwhile the values (64 pairs of channels x 4 nodes at a time), and the scalars (threads 192 + i: node i's)
+  float2 val[N / 4];
+  {
+    uint32_t held[3] = {0, 0, 0};
+    if (init)
+      for (int j = 0; j < 3; ++j) held[j] = *reinterpret_cast<const uint32_t*>(cs + ((int64_t)(2 - j) * 3 + 2) * a.P);
+    const uint4 wv = __ldg(reinterpret_cast<const uint4*>(a.conv_w + (2 * (int64_t)a.P + h * kDim + 2 * pair) * 4));
+    const float2 p[4] = {bf2(wv.x), bf2(wv.y), bf2(wv.z), bf2(wv.w)};
+    const int64_t pitch = a.ldx / 2;
+    const uint32_t* in = reinterpret_cast<const uint32_t*>(a.x + 2 * (int64_t)a.P + h * kDim + 2 * pair) + s * pitch;
+    const auto row = [&](int j) { return __ldg(in + j * pitch); };
+#pragma unroll
+    for (int t = 0; t < N / 4; ++t) {
+      const int i = part + 4 * t;
+      if (i < n) val[t] = conv4(p, row(i), sm.mask[i] ^ (1ull << i), held, row);
+    }
+  }
+  if (tid >= 192 && tid - 192 < n) {
+    const int i = tid - 192;
+    uint64_t path = sm.mask[i];
+    const int len = __popcll(path);
+    float* pn = sm.pn + sm.off[i];
+    for (int c = 0; c < len; ++c) {
+      const int m = pop(path);
+      const float y = pn[c] * sm.beta[m];
+      pn[c] = y;
+      const float* pm = sm.pm + (sm.off[m] - m);
+#pragma unroll 4
+      for (int e = c + 1; e < len; ++e) pn[e] = fmaf(-y, pm[e - c - 1], pn[e]);
+    }
+  }
+  const bool ok = mbar_wait(bar, 0, &sm.abort, a.status);
+#pragma unroll
+  for (int t = 0; t < N / 4; ++t) {
+    const int i = part + 4 * t;
+    if (i < n) *reinterpret_cast<float2*>(&sm.w[i][2 * pair]) = val[t];
+  }
+  const bool done = !__syncthreads_or(!ok);
+  tc_fence_after();
+  if (done) {
+    const uint32_t d = tmem + (static_cast<uint32_t>(32 * quarter) << 16) + kColD;
+    constexpr int kHalf = N / 2;                               // a half of the nodes a thread of its value row
+#pragma unroll
+    for (int c = 0; c < kHalf; c += 8) {
+      float y[8];
+      tmem_ld_x8(d + kHalf * half + c, y);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (kHalf * half + c + j < n) sm.w[kHalf * half + c + j][v] -= y[j];
+    }
+    __syncthreads();
+    __nv_bfloat16* out = a.out + (int64_t)s * a.ldo + h * kDim + v;
+#pragma unroll 1
+    for (int c = 0; c < kHalf; c += 8) {
+      float z[8];
+      tmem_ld_x8(d + N + kHalf * half + c, z);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = kHalf * half + c + j;
+        if (i >= n) continue;
+        uint64_t path = sm.mask[i];
+        const float* pn = sm.pn + sm.off[i];
+        float o = z[j];
+        while (path != 0) o = fmaf(*pn++, sm.w[pop(path)][v], o);
+        out[i * a.ldo] = __float2bfloat16(o);
+      }
+    }
+  } else {
+    const unsigned long long t0 = globaltimer();               // the products may still be on their way
+    while (!mbar_try_wait(bar, 0) && globaltimer() - t0 <= 2 * kWaitNs) {}
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kCols);
+  }
+}
+
+// TMEM holds two CTAs' columns: shared memory of which three do not fit an SM keeps a third from waiting for them.
+template <int N>
+constexpr int smem_bytes() {
+  static_assert(sizeof(TreeSmem<N>) <= 115712, "two CTAs an SM");
+  return sizeof(TreeSmem<N>) > 80 * 1024 ? sizeof(TreeSmem<N>) : 80 * 1024;
 }
 
 template <int N>
 int launch_nodes(const KdaArgs& a, cudaStream_t stream) {
   static OncePerDevice attr;
   int device = 0;
-  const auto set = [&] {
-    return cudaFuncSetAttribute(kda_tree_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(TreeSmem<N>)) ==
+  const auto set = [] {
+    return cudaFuncSetAttribute(kda_tree_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<N>()) ==
            cudaSuccess;
   };
   if (cudaGetDevice(&device) != cudaSuccess || !attr.done(device, set)) return kErrCuda;
-  kda_tree_kernel<N><<<(unsigned)(a.R * a.H), kTreeThreads, sizeof(TreeSmem<N>), stream>>>(a);
+  kda_tree_kernel<N><<<(unsigned)(a.R * a.H), kThreads, smem_bytes<N>(), stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
 }
 
