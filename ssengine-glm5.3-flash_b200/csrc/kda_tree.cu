@@ -42,14 +42,22 @@ struct TreeSmem {
       float q[N][kDim];                    // queries, normalised and scaled
     };
     uint8_t op[2][2][2 * N][128];          // A k, A q: high and low parts, 2 chunks of 64 keys [rows x 128 B], swizzled
-    float w[N][kDim];                      // values, then w
+    float w[N][kDim];                      // v - S (A k)
   };
-  float g[N][kDim];                        // log2 of the decays, summed down the path
-  float pn[N * (N + 1) / 2];               // N_ij, then P_ij: of node i from off[i] on, by distance
+  union {
+    float g[N][kDim];                      // log2 of the decays, summed down the path
+    struct {                               // once A k and A q are made
+      uint32_t v[N][kDim / 2];             // inputs of the values
+      uint8_t up[N * (N + 1) / 2];         // the paths: of node i from off[i] on, from itself up
+    };
+  };
+  float pn[N * (N + 1) / 2];               // N_ij, then P_ij: of node i from off[i] on, by distance. Before, bytes: node i's
+                                           // path, in the last bytes of its place (overwritten behind their use)
   float pm[N * (N - 1) / 2];               // M_ij: of node i from off[i] - i on, by distance - 1
-  uint64_t mask[N];                        // a node's path, itself among it
   float beta[N];
-  uint16_t off[N];
+  uint32_t tap[N];                         // bytes: the rows before the node's in the conv, kMaxNodes + j: the j-th newest kept row
+  uint16_t off[N + 2];
+  int8_t parent[N];
   uint64_t bar;
   uint32_t tmem;
   int32_t abort;
@@ -68,12 +76,6 @@ SSB_DEVICE void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
   hi = *reinterpret_cast<const uint32_t*>(&h);
   const __nv_bfloat162 l = __floats2bfloat162_rn(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xFFFF0000u));
   lo = *reinterpret_cast<const uint32_t*>(&l);
-}
-// The last node of a path and the path above it.
-SSB_DEVICE int pop(uint64_t& path) {
-  const int i = 63 - __clzll(static_cast<long long>(path));
-  path ^= 1ull << i;
-  return i;
 }
 SSB_DEVICE void ld8(const float* p, float* v) {              // 32 bytes
   asm volatile("ld.global.nc.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
@@ -95,28 +97,17 @@ SSB_DEVICE void mma_f16_ta(uint32_t d, uint32_t a, uint64_t bd, uint32_t idesc, 
       : "memory");
 }
 
-// A node's conv taps of a channel pair: its own row's value x0, then those of the three rows before it on its path, the
-// block's kept rows behind a root (held[0] the newest). row(j): node j's value.
-template <class Row>
-SSB_DEVICE float2 conv4(const float2 (&p)[4], uint32_t x0, uint64_t above, const uint32_t (&held)[3], Row row) {
-  uint32_t x[4] = {0, 0, 0, x0};
-  if (__popcll(above) >= 3) {
-    x[2] = row(pop(above)), x[1] = row(pop(above)), x[0] = row(pop(above));
-  } else if (above == 0) {
-    x[2] = held[0], x[1] = held[1], x[0] = held[2];
-  } else {
-    x[2] = row(pop(above));
-    if (above == 0) {
-      x[1] = held[0], x[0] = held[1];
-    } else {
-      x[1] = row(pop(above)), x[0] = held[0];
-    }
-  }
-  const float2 x1 = bf2(x[0]), x2 = bf2(x[1]), x3 = bf2(x[2]), x4 = bf2(x[3]);
-  float2 o;
-  o.x = silu_short(fmaf(p[1].y, x4.x, fmaf(p[1].x, x3.x, fmaf(p[0].y, x2.x, p[0].x * x1.x))));
-  o.y = silu_short(fmaf(p[3].y, x4.y, fmaf(p[3].x, x3.y, fmaf(p[2].y, x2.y, p[2].x * x1.y))));
-  return o;
+SSB_DEVICE void cp_async4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+SSB_DEVICE void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// The value of tap j (0: the newest) of a node: row(node), or one of the block's kept rows behind a root.
+template <class T, class Row>
+SSB_DEVICE T tap_of(uint32_t taps, int j, const T (&held)[3], Row row) {
+  const uint32_t t = (taps >> (8 * j)) & 0xFF;
+  const T x = row(static_cast<int>(t & (kMaxNodes - 1)));
+  return t < kMaxNodes ? x : t == kMaxNodes ? held[0] : t == kMaxNodes + 1 ? held[1] : held[2];
 }
 
 template <int N>
@@ -164,39 +155,37 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
                                                                 : a.x + (int64_t)part * a.P + h * kDim + 2 * pair);
     const int64_t pitch = (in_g ? a.ldg : a.ldx) / 2;
     in += s * pitch;
-#pragma unroll 1
-    for (int i = 0; i < n; i += 8) {
-      uint32_t x[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = __ldg(in + min(i + j, n - 1) * pitch);
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (i + j < n) column[(i + j) * kDim] = __uint_as_float(x[j]);
-    }
+#pragma unroll 4
+    for (int i = 0; i < n; ++i, in += pitch) cp_async4(column + i * kDim, in);
   } else {
-    // thread 192 + i: node i. The parents go through the places of the paths
+    // thread 192 + i: node i, its path walked twice: its length, then its nodes
     const int i = tid - 192;
+    const bool node = i < n;
     int p = -1;
-    if (i < n) {
+    if (node) {
       p = a.parents[s + i];
       bad = p < -1 || p >= i;
       sm.beta[i] = sigmoid_short(__bfloat162float(a.beta[(int64_t)(s + i) * a.ldb + h]));
-      sm.mask[i] = static_cast<uint64_t>(static_cast<int64_t>(p));
+      sm.parent[i] = static_cast<int8_t>(p);
+      // the values' rows are wanted late: on their way to L2
+      const __nv_bfloat16* x = a.x + (s + i) * a.ldx + 2 * (int64_t)a.P + h * kDim;
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(x));
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(x + kDim / 2));
     }
     bad = named_bar_or(1, 64, bad);
-    uint64_t path = 0;
-    if (i < n && !bad) {
-      path = 1ull << i;
-      while (p >= 0) {
-        path |= 1ull << p;
-        p = static_cast<int>(static_cast<int64_t>(sm.mask[p]));
+    int len = 0;
+    uint32_t taps = 0;
+    if (node && !bad) {
+      int at = p;
+      for (int j = 0, kept = kMaxNodes; j < 3; ++j) {
+        taps |= static_cast<uint32_t>(at >= 0 ? at : kept++) << (8 * j);
+        if (at >= 0) at = sm.parent[at], ++len;
       }
+      for (; at >= 0; at = sm.parent[at]) ++len;
+      sm.tap[i] = taps;
+      ++len;
     }
-    named_bar(1, 64);
-    if (i < n) sm.mask[i] = path;
-    // offsets: the sum of the path lengths before the node, a warp each, the second one's behind the first's
-    const int len = __popcll(path);
-    int end = len;
+    int end = len;                                           // the sum of the lengths: a warp each, the second behind the first
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int x = __shfl_up_sync(0xffffffffu, end, o);
@@ -205,8 +194,18 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
     if (i == 31) sm.abort = end;
     named_bar(1, 64);
     if (i >= 32) end += sm.abort;
-    if (i < n) sm.off[i] = static_cast<uint16_t>(end - len);
+    if (node && !bad) {
+      sm.off[i] = static_cast<uint16_t>(end - len);
+      if (i == n - 1) sm.off[n] = static_cast<uint16_t>(end);
+      uint8_t* path = reinterpret_cast<uint8_t*>(sm.pn + (end - len)) + 3 * len;
+      int at = i;
+      for (int d = 0; d < len; ++d) {
+        path[d] = static_cast<uint8_t>(at);
+        at = sm.parent[at];
+      }
+    }
   }
+  cp_async_wait();
   if (__syncthreads_or(bad)) {
     if (tid == 0 && h == 0) raise_status(a.status, kErrArgs);
     return;
@@ -222,24 +221,34 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
   }
 
   // ---- conv and gates in place
-  const __nv_bfloat16* cs = a.conv_state + (int64_t)sq.z * a.cs_stride + h * kDim + 2 * pair;   // of q; k, v: + P, + 2 P
+  const __nv_bfloat16* cs = a.conv_state + (int64_t)sq.z * a.cs_stride + h * kDim;              // of q; k, v: + P, + 2 P
   if (part < 2) {
     uint32_t held[3] = {0, 0, 0};
     if (init)
-      for (int j = 0; j < 3; ++j) held[j] = *reinterpret_cast<const uint32_t*>(cs + ((int64_t)(2 - j) * 3 + part) * a.P);
-    const uint4* wp = reinterpret_cast<const uint4*>(a.conv_w + ((int64_t)part * a.P + h * kDim + 2 * pair) * 4);
-    const uint4 wv = __ldg(wp);                              // 2 channels x 4 taps
-    const float2 p[4] = {bf2(wv.x), bf2(wv.y), bf2(wv.z), bf2(wv.w)};
+      for (int j = 0; j < 3; ++j)
+        held[j] = *reinterpret_cast<const uint32_t*>(cs + ((int64_t)(2 - j) * 3 + part) * a.P + 2 * pair);
+    const uint4 wv = __ldg(reinterpret_cast<const uint4*>(a.conv_w + ((int64_t)part * a.P + h * kDim + 2 * pair) * 4));
+    const float2 p0 = bf2(wv.x), p1 = bf2(wv.y), p2 = bf2(wv.z), p3 = bf2(wv.w);               // 2 channels x 4 taps
     const auto row = [&](int j) { return __float_as_uint(column[j * kDim]); };
 #pragma unroll 1
     for (int i = n - 1; i >= 0; i -= 4) {                    // 4 nodes read before the first is written
-      float2 o[4];
+      uint32_t x[4][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (i - j >= 0) o[j] = conv4(p, row(i - j), sm.mask[i - j] ^ (1ull << (i - j)), held, row);
+      for (int j = 0; j < 4; ++j) {
+        const int m = max(i - j, 0);
+        const uint32_t taps = sm.tap[m];
+        x[j][3] = row(m);
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (i - j >= 0) *reinterpret_cast<float2*>(column + (i - j) * kDim) = o[j];
+        for (int e = 0; e < 3; ++e) x[j][2 - e] = tap_of(taps, e, held, row);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 x0 = bf2(x[j][0]), x1 = bf2(x[j][1]), x2 = bf2(x[j][2]), x3 = bf2(x[j][3]);
+        float2 o;
+        o.x = silu_short(fmaf(p1.y, x3.x, fmaf(p1.x, x2.x, fmaf(p0.y, x1.x, p0.x * x0.x))));
+        o.y = silu_short(fmaf(p3.y, x3.y, fmaf(p3.x, x2.y, fmaf(p2.y, x1.y, p2.x * x0.y))));
+        if (i - j >= 0) *reinterpret_cast<float2*>(column + (i - j) * kDim) = o;
+      }
     }
   } else if (in_g) {
     const float2 dt = __ldg(reinterpret_cast<const float2*>(a.dt_bias + h * kDim) + pair);
@@ -247,21 +256,20 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
 #pragma unroll 1
     for (int i = 0; i < n; i += 4) {
       float2 o[4];
+      int up[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (i + j >= n) continue;
-        const float2 x = bf2(__float_as_uint(column[(i + j) * kDim]));
+        const int m = min(i + j, n - 1);
+        up[j] = sm.parent[m];
+        const float2 x = bf2(__float_as_uint(column[m * kDim]));
         o[j].x = lb * sigmoid_short(rate * (x.x + dt.x));
         o[j].y = lb * sigmoid_short(rate * (x.y + dt.y));
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if (i + j >= n) continue;
-        uint64_t above = sm.mask[i + j] ^ (1ull << (i + j));
-        if (above != 0) {
-          const float2 up = *reinterpret_cast<float2*>(column + pop(above) * kDim);
-          o[j].x += up.x, o[j].y += up.y;
-        }
+        const float2 g = *reinterpret_cast<float2*>(column + max(up[j], 0) * kDim);
+        if (up[j] >= 0) o[j].x += g.x, o[j].y += g.y;
         *reinterpret_cast<float2*>(column + (i + j) * kDim) = o[j];
       }
     }
@@ -301,24 +309,45 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
     *qp = make_float4(q.x * rq, q.y * rq, q.z * rq, q.w * rq);
   }
   __syncthreads();
-  // ---- the pairs of a node and those above it
+  // ---- the pairs of a node and those above it, 4 at a time
 #pragma unroll 1
   for (int i = warp; i < n; i += kWarps) {
     const float4 k = *reinterpret_cast<float4*>(&sm.k[i][4 * lane]), q = *reinterpret_cast<float4*>(&sm.q[i][4 * lane]);
     const float4 g = *reinterpret_cast<float4*>(&sm.g[i][4 * lane]);
-    uint64_t path = sm.mask[i];
-    int at = sm.off[i];
-    for (int d = 0; path != 0; ++d) {
-      const int j = pop(path);
-      const float4 kj = *reinterpret_cast<float4*>(&sm.k[j][4 * lane]), gj = *reinterpret_cast<float4*>(&sm.g[j][4 * lane]);
-      const float x = kj.x * ex2(g.x - gj.x), y = kj.y * ex2(g.y - gj.y);
-      const float z = kj.z * ex2(g.z - gj.z), w = kj.w * ex2(g.w - gj.w);
-      const float m = x * k.x + y * k.y + z * k.z + w * k.w, nn = x * q.x + y * q.y + z * q.z + w * q.w;
-      float t = (lane < 16 ? m : nn) + __shfl_xor_sync(0xffffffffu, lane < 16 ? nn : m, 16);
+    const int at = sm.off[i], len = sm.off[i + 1] - at;
+    const uint8_t* path = reinterpret_cast<const uint8_t*>(sm.pn + at) + 3 * len;
+#pragma unroll 1
+    for (int d = 0; d < len; d += 4) {
+      int js[4];
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-      if (lane == 0 && d > 0) sm.pm[at - i + d - 1] = t;
-      if (lane == 16) sm.pn[at + d] = t;
+      for (int e = 0; e < 4; ++e) js[e] = path[min(d + e, len - 1)];
+      float t[8];                                              // M of 4 pairs, N of 4 pairs
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float4 kj = *reinterpret_cast<float4*>(&sm.k[js[e]][4 * lane]);
+        const float4 gj = *reinterpret_cast<float4*>(&sm.g[js[e]][4 * lane]);
+        const float x = kj.x * ex2(g.x - gj.x), y = kj.y * ex2(g.y - gj.y);
+        const float z = kj.z * ex2(g.z - gj.z), w = kj.w * ex2(g.w - gj.w);
+        t[e] = fmaf(x, k.x, fmaf(y, k.y, fmaf(z, k.z, w * k.w)));
+        t[4 + e] = fmaf(x, q.x, fmaf(y, q.y, fmaf(z, q.z, w * q.w)));
+      }
+#pragma unroll
+      for (int o = 16, m = 4; o >= 4; o >>= 1, m >>= 1) {      // lanes 4 x .. + 3 receive value x
+        const bool up = lane & o;
+#pragma unroll
+        for (int e = 0; e < m; ++e) {
+          const float keep = up ? t[e + m] : t[e], send = up ? t[e] : t[e + m];
+          t[e] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+        }
+      }
+      t[0] += __shfl_xor_sync(0xffffffffu, t[0], 2);
+      t[0] += __shfl_xor_sync(0xffffffffu, t[0], 1);
+      __syncwarp();                                            // the path's bytes are read
+      const int e = d + ((lane >> 2) & 3);
+      if ((lane & 3) == 0 && e < len) {
+        if (lane >= 16) sm.pn[at + e] = t[0];
+        else if (e > 0) sm.pm[at - i + e - 1] = t[0];
+      }
     }
   }
   // ---- A k and A q as the products' second operand, in the place of k and q
@@ -371,30 +400,25 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
     }
     tc_commit(bar);
   }
-  // ---- meanwhile the values (64 pairs of channels x 4 nodes at a time), and the scalars (threads 192 + i: node i's)
-  float2 val[N / 4];
+  // ---- meanwhile the values' inputs, and the scalars (threads 192 + i: node i's)
   {
-    uint32_t held[3] = {0, 0, 0};
-    if (init)
-      for (int j = 0; j < 3; ++j) held[j] = *reinterpret_cast<const uint32_t*>(cs + ((int64_t)(2 - j) * 3 + 2) * a.P);
-    const uint4 wv = __ldg(reinterpret_cast<const uint4*>(a.conv_w + (2 * (int64_t)a.P + h * kDim + 2 * pair) * 4));
-    const float2 p[4] = {bf2(wv.x), bf2(wv.y), bf2(wv.z), bf2(wv.w)};
+    const uint32_t* in = reinterpret_cast<const uint32_t*>(a.x + 2 * (int64_t)a.P + h * kDim + 2 * pair);
     const int64_t pitch = a.ldx / 2;
-    const uint32_t* in = reinterpret_cast<const uint32_t*>(a.x + 2 * (int64_t)a.P + h * kDim + 2 * pair) + s * pitch;
-    const auto row = [&](int j) { return __ldg(in + j * pitch); };
-#pragma unroll
-    for (int t = 0; t < N / 4; ++t) {
-      const int i = part + 4 * t;
-      if (i < n) val[t] = conv4(p, row(i), sm.mask[i] ^ (1ull << i), held, row);
-    }
+#pragma unroll 4
+    for (int i = part; i < n; i += 4) cp_async4(&sm.v[i][pair], in + (s + i) * pitch);
   }
-  if (tid >= 192 && tid - 192 < n) {
+  if (part == 3) {
     const int i = tid - 192;
-    uint64_t path = sm.mask[i];
-    const int len = __popcll(path);
-    float* pn = sm.pn + sm.off[i];
+    const int at = i < n ? sm.off[i] : 0, len = i < n ? sm.off[i + 1] - at : 0;
+    int m = i;
     for (int c = 0; c < len; ++c) {
-      const int m = pop(path);
+      sm.up[at + c] = static_cast<uint8_t>(m);
+      m = sm.parent[m];
+    }
+    float* pn = sm.pn + at;
+#pragma unroll 1
+    for (int c = 0; c < len; ++c) {
+      m = sm.up[at + c];
       const float y = pn[c] * sm.beta[m];
       pn[c] = y;
       const float* pm = sm.pm + (sm.off[m] - m);
@@ -402,41 +426,50 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
       for (int e = c + 1; e < len; ++e) pn[e] = fmaf(-y, pm[e - c - 1], pn[e]);
     }
   }
+  cp_async_wait();
   const bool ok = mbar_wait(bar, 0, &sm.abort, a.status);
-#pragma unroll
-  for (int t = 0; t < N / 4; ++t) {
-    const int i = part + 4 * t;
-    if (i < n) *reinterpret_cast<float2*>(&sm.w[i][2 * pair]) = val[t];
-  }
   const bool done = !__syncthreads_or(!ok);
   tc_fence_after();
   if (done) {
     const uint32_t d = tmem + (static_cast<uint32_t>(32 * quarter) << 16) + kColD;
     constexpr int kHalf = N / 2;                               // a half of the nodes a thread of its value row
+    {
+      float held[3] = {0.0f, 0.0f, 0.0f};
+      if (init)
+        for (int j = 0; j < 3; ++j) held[j] = __bfloat162float(cs[((int64_t)(2 - j) * 3 + 2) * a.P + v]);
+      const uint2 wv = __ldg(reinterpret_cast<const uint2*>(a.conv_w + (2 * (int64_t)a.P + h * kDim + v) * 4));
+      const float2 p0 = bf2(wv.x), p1 = bf2(wv.y);
+      const auto row = [&](int j) { return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(sm.v[j])[v]); };
+#pragma unroll 1
+      for (int c = kHalf * half; c < min(kHalf * (half + 1), n); c += 8) {
+        float y[8];
+        tmem_ld_x8(d + c, y);
+        tmem_ld_wait();
 #pragma unroll
-    for (int c = 0; c < kHalf; c += 8) {
-      float y[8];
-      tmem_ld_x8(d + kHalf * half + c, y);
-      tmem_ld_wait();
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (kHalf * half + c + j < n) sm.w[kHalf * half + c + j][v] -= y[j];
+        for (int j = 0; j < 8; ++j) {
+          const int i = min(c + j, n - 1);
+          const uint32_t taps = sm.tap[i];
+          const float x = fmaf(p1.y, row(i), fmaf(p1.x, tap_of(taps, 0, held, row),
+                                                  fmaf(p0.y, tap_of(taps, 1, held, row), p0.x * tap_of(taps, 2, held, row))));
+          if (c + j < n) sm.w[i][v] = silu_short(x) - y[j];
+        }
+      }
     }
     __syncthreads();
     __nv_bfloat16* out = a.out + (int64_t)s * a.ldo + h * kDim + v;
 #pragma unroll 1
-    for (int c = 0; c < kHalf; c += 8) {
+    for (int c = kHalf * half; c < min(kHalf * (half + 1), n); c += 8) {
       float z[8];
-      tmem_ld_x8(d + N + kHalf * half + c, z);
+      tmem_ld_x8(d + N + c, z);
       tmem_ld_wait();
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int i = kHalf * half + c + j;
+        const int i = c + j;
         if (i >= n) continue;
-        uint64_t path = sm.mask[i];
-        const float* pn = sm.pn + sm.off[i];
+        const int at = sm.off[i], end = sm.off[i + 1];
         float o = z[j];
-        while (path != 0) o = fmaf(*pn++, sm.w[pop(path)][v], o);
+#pragma unroll 4
+        for (int e = at; e < end; ++e) o = fmaf(sm.pn[e], sm.w[sm.up[e]][v], o);
         out[i * a.ldo] = __float2bfloat16(o);
       }
     }
