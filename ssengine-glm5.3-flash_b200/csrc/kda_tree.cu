@@ -8,18 +8,17 @@
 //   o_i = S (A_i q_i) + sum_{j on the path} u_j N_ij,                        N_ij = (A_ij k_j) . q_i   (q with D^-1/2)
 // and, since the u are linear in the w with scalars of the path alone, o_i = S (A_i q_i) + sum_{j on the path} P_ij w_j with
 // P_i (1 + b M) = N_i b: a substitution up each node's path, on scalars. So the state S [value, key] is read once, whatever
-// the nodes, no node's own state is formed, and nothing but the scalars goes node after node. A_ij = 2^(G_i - G_j), G the sum
-// of the log2 of the decays down the path: differences along a path are never positive, where quotients of products would
-// overflow.
+// the nodes, no node's own state is formed, and nothing but the scalars goes node after node. The decays multiply up the
+// path (each is at most 1; quotients of cumulated ones would overflow).
 //
 // One CTA a (request, head), 256 threads, two CTAs an SM:
-//   conv and gates: a thread a pair of channels of q, k or g, in shared memory in place (a node's row is overwritten when
-//       the nodes below it are done: from the last node to the first);
-//   pairs: a warp a node and those above it, 4 channels a lane;
+//   conv and gates: a thread a pair of channels of q or k for every second node, of g for every fourth;
+//   pairs: a warp a node and those above it, 4 at a time, 4 channels a lane;
 //   products: [S (A k) | S (A q)] on the tensor cores, M = 128 value rows, N = 2 nodes, K = 128 keys, tcgen05 kind::f16: S in
 //       TMEM and the vectors in shared memory, both as two bf16 parts, three of the four products (what is left out is below
 //       2^-16 of a product; the output has 8 bits). S comes straight from global memory, a value row a lane;
-//   outputs: a value row a thread, as the products lie in TMEM.
+//   outputs: w by value rows, as the products lie in TMEM, back there as bf16 parts, and W^T P^T onto S (A q) by the tensor
+//       cores, K = nodes.
 // The exponentials are the short ones (error about 2^-20 here): nothing computed here is kept but the bf16 outputs.
 #include "common.cuh"
 #include "kda_math.cuh"
@@ -32,7 +31,8 @@ constexpr int kDim = 128;
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxNodes = 64;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr uint32_t kColS = 0, kColD = 128, kCols = 256;    // TMEM: S as 64 columns of high and 64 of low parts; the products
+// TMEM: S as 64 columns of high and 64 of low parts, later W^T in the same places; the products
+constexpr uint32_t kColS = 0, kColLo = 64, kColD = 128, kCols = 256;
 
 template <int N>
 struct TreeSmem {
@@ -42,34 +42,45 @@ struct TreeSmem {
       float q[N][kDim];                    // queries, normalised and scaled
     };
     uint8_t op[2][2][2 * N][128];          // A k, A q: high and low parts, 2 chunks of 64 keys [rows x 128 B], swizzled
-    float w[N][kDim];                      // v - S (A k)
   };
   union {
-    float g[N][kDim];                      // log2 of the decays, summed down the path
+    uint32_t in[2][N][kDim / 2];           // inputs of q and k
+    float dec[N][kDim];                    // then the decays
     struct {                               // once A k and A q are made
+      uint8_t p[2][N][128];                // P: high and low parts [nodes x nodes], swizzled
       uint32_t v[N][kDim / 2];             // inputs of the values
-      uint8_t up[N * (N + 1) / 2];         // the paths: of node i from off[i] on, from itself up
     };
   };
-  float pn[N * (N + 1) / 2];               // N_ij, then P_ij: of node i from off[i] on, by distance. Before, bytes: node i's
-                                           // path, in the last bytes of its place (overwritten behind their use)
+  float pn[N * (N + 1) / 2];               // N_ij: of node i from off[i] on, by distance. Before, bytes: node i's path, in the
+                                           // last bytes of its place (overwritten behind their use)
   float pm[N * (N - 1) / 2];               // M_ij: of node i from off[i] - i on, by distance - 1
   float beta[N];
   uint32_t tap[N];                         // bytes: the rows before the node's in the conv, kMaxNodes + j: the j-th newest kept row
   uint16_t off[N + 2];
   int8_t parent[N];
-  uint64_t bar;
+  uint64_t bar[2];
   uint32_t tmem;
   int32_t abort;
 };
+static_assert(sizeof(uint8_t[2][64][128]) + sizeof(uint32_t[64][64]) == sizeof(float[64][kDim]), "one place");
 
 SSB_DEVICE float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-SSB_DEVICE float sigmoid_short(float x) { return __fdividef(1.0f, 1.0f + ex2(-kLog2e * x)); }
-SSB_DEVICE float silu_short(float x) { return __fdividef(x, 1.0f + ex2(-kLog2e * x)); }
+SSB_DEVICE float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+SSB_DEVICE float sigmoid_short(float x) { return rcp(1.0f + ex2(-kLog2e * x)); }
+SSB_DEVICE float silu_short(float x) { return x * rcp(1.0f + ex2(-kLog2e * x)); }
+SSB_DEVICE float sum2(uint64_t v) {
+  float x, y;
+  f2unpack(v, x, y);
+  return x + y;
+}
 // Two values as bf16 pairs: the high parts, and what they leave.
 SSB_DEVICE void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
@@ -87,6 +98,11 @@ SSB_DEVICE void tmem_ld_x8(uint32_t taddr, float (&v)[8]) {
                : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
                : "r"(taddr));
 }
+SSB_DEVICE void tmem_st_x4(uint32_t taddr, const uint32_t (&v)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3])
+               : "memory");
+}
 // D[tmem] (+)= A B with bf16 A in TMEM (a row a lane, 2 values a column) and B in shared memory.
 SSB_DEVICE void mma_f16_ta(uint32_t d, uint32_t a, uint64_t bd, uint32_t idesc, uint32_t acc) {
   asm volatile(
@@ -102,12 +118,20 @@ SSB_DEVICE void cp_async4(void* dst, const void* src) {
 }
 SSB_DEVICE void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// The value of tap j (0: the newest) of a node: row(node), or one of the block's kept rows behind a root.
+// Four conv taps (0: the oldest) of a node: x[3] its own row's value, the others by `taps`, of which those behind a root are
+// the block's kept rows (held[0] the newest).
 template <class T, class Row>
-SSB_DEVICE T tap_of(uint32_t taps, int j, const T (&held)[3], Row row) {
-  const uint32_t t = (taps >> (8 * j)) & 0xFF;
-  const T x = row(static_cast<int>(t & (kMaxNodes - 1)));
-  return t < kMaxNodes ? x : t == kMaxNodes ? held[0] : t == kMaxNodes + 1 ? held[1] : held[2];
+SSB_DEVICE void load_taps(T (&x)[4], int i, uint32_t taps, const T (&held)[3], Row row) {
+  x[3] = row(i);
+#pragma unroll
+  for (int e = 0; e < 3; ++e) x[2 - e] = row(static_cast<int>((taps >> (8 * e)) & (kMaxNodes - 1)));
+  if (taps & 0x404040u) {
+#pragma unroll
+    for (int e = 0; e < 3; ++e) {
+      const uint32_t t = (taps >> (8 * e)) & 0xFF;
+      if (t >= kMaxNodes) x[2 - e] = t == kMaxNodes ? held[0] : t == kMaxNodes + 1 ? held[1] : held[2];
+    }
+  }
 }
 
 template <int N>
@@ -124,6 +148,15 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
   }
   if (n == 0) return;
   const bool init = sq.w != 0;
+  if (warp == 0) {
+    tmem_alloc(smem_u32(&sm.tmem), kCols);
+    tmem_relinquish();
+    if (lane == 0) {
+      mbar_init(smem_u32(&sm.bar[0]), 1);
+      mbar_init(smem_u32(&sm.bar[1]), 1);
+      fence_barrier_init();
+    }
+  }
 
   // ---- the state's loads: a value row a lane, half of its keys a thread
   const int quarter = warp & 3, half = warp >> 2, v = 32 * quarter + lane;
@@ -145,18 +178,14 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
       }
     }
   }
-  // ---- the inputs of q, k and g into their places (threads 0-191: a pair of channels each); the tree (threads 192-255)
+  // ---- the inputs of q and k into shared memory (threads 0-191); the tree (threads 192-255)
   const int pair = tid & 63, part = tid >> 6;
-  const bool in_q = part == 0, in_k = part == 1, in_g = part == 2;
-  float* column = in_q ? &sm.q[0][2 * pair] : in_k ? &sm.k[0][2 * pair] : &sm.g[0][2 * pair];
   bool bad = false;
   if (part < 3) {
-    const uint32_t* in = reinterpret_cast<const uint32_t*>(in_g ? a.g + h * kDim + 2 * pair
-                                                                : a.x + (int64_t)part * a.P + h * kDim + 2 * pair);
-    const int64_t pitch = (in_g ? a.ldg : a.ldx) / 2;
-    in += s * pitch;
+    const uint32_t* in = reinterpret_cast<const uint32_t*>(a.x + h * kDim + 2 * pair) + s * (a.ldx / 2);
 #pragma unroll 4
-    for (int i = 0; i < n; ++i, in += pitch) cp_async4(column + i * kDim, in);
+    for (int i = part; i < 2 * n; i += 3)
+      cp_async4(&sm.in[i & 1][i >> 1][pair], in + (i >> 1) * (a.ldx / 2) + (i & 1) * (a.P / 2));
   } else {
     // thread 192 + i: node i, its path walked twice: its length, then its nodes
     const int i = tid - 192;
@@ -205,77 +234,21 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
       }
     }
   }
+  // the gates' inputs: a pair of channels of every fourth node a thread
+  uint32_t gin[N / 4];
+  {
+    const uint32_t* in = reinterpret_cast<const uint32_t*>(a.g + h * kDim + 2 * pair) + s * (a.ldg / 2);
+#pragma unroll
+    for (int t = 0; t < N / 4; ++t) gin[t] = __ldg(in + min(part + 4 * t, n - 1) * (a.ldg / 2));
+  }
   cp_async_wait();
+  tc_fence_before();
   if (__syncthreads_or(bad)) {
     if (tid == 0 && h == 0) raise_status(a.status, kErrArgs);
+    if (warp == 0) tmem_dealloc(sm.tmem, kCols);
     return;
   }
-  if (tid == 0) {
-    sm.abort = 0;
-    mbar_init(smem_u32(&sm.bar), 1);
-    fence_barrier_init();
-  }
-  if (warp == 0) {
-    tmem_alloc(smem_u32(&sm.tmem), kCols);
-    tmem_relinquish();
-  }
-
-  // ---- conv and gates in place
-  const __nv_bfloat16* cs = a.conv_state + (int64_t)sq.z * a.cs_stride + h * kDim;              // of q; k, v: + P, + 2 P
-  if (part < 2) {
-    uint32_t held[3] = {0, 0, 0};
-    if (init)
-      for (int j = 0; j < 3; ++j)
-        held[j] = *reinterpret_cast<const uint32_t*>(cs + ((int64_t)(2 - j) * 3 + part) * a.P + 2 * pair);
-    const uint4 wv = __ldg(reinterpret_cast<const uint4*>(a.conv_w + ((int64_t)part * a.P + h * kDim + 2 * pair) * 4));
-    const float2 p0 = bf2(wv.x), p1 = bf2(wv.y), p2 = bf2(wv.z), p3 = bf2(wv.w);               // 2 channels x 4 taps
-    const auto row = [&](int j) { return __float_as_uint(column[j * kDim]); };
-#pragma unroll 1
-    for (int i = n - 1; i >= 0; i -= 4) {                    // 4 nodes read before the first is written
-      uint32_t x[4][4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int m = max(i - j, 0);
-        const uint32_t taps = sm.tap[m];
-        x[j][3] = row(m);
-#pragma unroll
-        for (int e = 0; e < 3; ++e) x[j][2 - e] = tap_of(taps, e, held, row);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 x0 = bf2(x[j][0]), x1 = bf2(x[j][1]), x2 = bf2(x[j][2]), x3 = bf2(x[j][3]);
-        float2 o;
-        o.x = silu_short(fmaf(p1.y, x3.x, fmaf(p1.x, x2.x, fmaf(p0.y, x1.x, p0.x * x0.x))));
-        o.y = silu_short(fmaf(p3.y, x3.y, fmaf(p3.x, x2.y, fmaf(p2.y, x1.y, p2.x * x0.y))));
-        if (i - j >= 0) *reinterpret_cast<float2*>(column + (i - j) * kDim) = o;
-      }
-    }
-  } else if (in_g) {
-    const float2 dt = __ldg(reinterpret_cast<const float2*>(a.dt_bias + h * kDim) + pair);
-    const float rate = exp_fast(__ldg(a.a_log + h)), lb = a.lower_bound * kLog2e;
-#pragma unroll 1
-    for (int i = 0; i < n; i += 4) {
-      float2 o[4];
-      int up[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int m = min(i + j, n - 1);
-        up[j] = sm.parent[m];
-        const float2 x = bf2(__float_as_uint(column[m * kDim]));
-        o[j].x = lb * sigmoid_short(rate * (x.x + dt.x));
-        o[j].y = lb * sigmoid_short(rate * (x.y + dt.y));
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (i + j >= n) continue;
-        const float2 g = *reinterpret_cast<float2*>(column + max(up[j], 0) * kDim);
-        if (up[j] >= 0) o[j].x += g.x, o[j].y += g.y;
-        *reinterpret_cast<float2*>(column + (i + j) * kDim) = o[j];
-      }
-    }
-  }
-  tc_fence_before();
-  __syncthreads();
+  if (tid == 0) sm.abort = 0;                                // its place was in use
   tc_fence_after();
   const uint32_t tmem = sm.tmem;
   // ---- the state's parts to TMEM
@@ -289,8 +262,54 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
       hi[j] = __uint_as_float(x), lo[j] = __uint_as_float(y);
     }
     tmem_st_32x32b_x32(at, hi);
-    tmem_st_32x32b_x32(at + 64, lo);
+    tmem_st_32x32b_x32(at + kColLo, lo);
     tmem_st_wait();
+  }
+
+  // ---- the conv of q and k: 4 nodes at a time, every second one
+  const __nv_bfloat16* cs = a.conv_state + (int64_t)sq.z * a.cs_stride + h * kDim;              // of q; k, v: + P, + 2 P
+  {
+    const int which = part & 1;                              // q, k
+    uint32_t held[3] = {0, 0, 0};
+    if (init)
+      for (int j = 0; j < 3; ++j)
+        held[j] = *reinterpret_cast<const uint32_t*>(cs + ((int64_t)(2 - j) * 3 + which) * a.P + 2 * pair);
+    const uint4 wv = __ldg(reinterpret_cast<const uint4*>(a.conv_w + ((int64_t)which * a.P + h * kDim + 2 * pair) * 4));
+    const float2 a0 = bf2(wv.x), a1 = bf2(wv.y), b0 = bf2(wv.z), b1 = bf2(wv.w);               // 2 channels x 4 taps
+    const uint64_t p0 = f2pack(a0.x, b0.x), p1 = f2pack(a0.y, b0.y), p2 = f2pack(a1.x, b1.x), p3 = f2pack(a1.y, b1.y);
+    const auto row = [&](int j) { return sm.in[which][j][pair]; };
+    float* to = (which ? &sm.k[0][0] : &sm.q[0][0]) + 2 * pair;
+#pragma unroll 1
+    for (int i = half; i < n; i += 8) {
+      uint32_t x[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int m = min(i + 2 * j, n - 1);
+        load_taps(x[j], m, sm.tap[m], held, row);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint64_t o = fma2(p3, bf2_f2(x[j][3]), fma2(p2, bf2_f2(x[j][2]), fma2(p1, bf2_f2(x[j][1]), mul2(p0, bf2_f2(x[j][0])))));
+        float2 y;
+        f2unpack(o, y.x, y.y);
+        y.x = silu_short(y.x), y.y = silu_short(y.y);
+        if (i + 2 * j < n) *reinterpret_cast<float2*>(to + (i + 2 * j) * kDim) = y;
+      }
+    }
+  }
+  __syncthreads();
+  // ---- the decays, in the place of the inputs
+  {
+    const float2 dt = __ldg(reinterpret_cast<const float2*>(a.dt_bias + h * kDim) + pair);
+    const float rate = -kLog2e * exp_fast(__ldg(a.a_log + h)), lb = a.lower_bound * kLog2e;
+#pragma unroll
+    for (int t = 0; t < N / 4; ++t) {
+      const float2 x = bf2(gin[t]);
+      float2 o;
+      o.x = ex2(lb * rcp(1.0f + ex2(rate * (x.x + dt.x))));
+      o.y = ex2(lb * rcp(1.0f + ex2(rate * (x.y + dt.y))));
+      if (part + 4 * t < n) *reinterpret_cast<float2*>(&sm.dec[part + 4 * t][2 * pair]) = o;
+    }
   }
 
   // ---- norms: a warp a node, 4 channels a lane
@@ -312,10 +331,10 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
   // ---- the pairs of a node and those above it, 4 at a time
 #pragma unroll 1
   for (int i = warp; i < n; i += kWarps) {
-    const float4 k = *reinterpret_cast<float4*>(&sm.k[i][4 * lane]), q = *reinterpret_cast<float4*>(&sm.q[i][4 * lane]);
-    const float4 g = *reinterpret_cast<float4*>(&sm.g[i][4 * lane]);
+    const ulonglong2 k = *reinterpret_cast<ulonglong2*>(&sm.k[i][4 * lane]), q = *reinterpret_cast<ulonglong2*>(&sm.q[i][4 * lane]);
     const int at = sm.off[i], len = sm.off[i + 1] - at;
     const uint8_t* path = reinterpret_cast<const uint8_t*>(sm.pn + at) + 3 * len;
+    ulonglong2 f = make_ulonglong2(f2pack(1.0f, 1.0f), f2pack(1.0f, 1.0f));                    // the decays below
 #pragma unroll 1
     for (int d = 0; d < len; d += 4) {
       int js[4];
@@ -324,12 +343,12 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
       float t[8];                                              // M of 4 pairs, N of 4 pairs
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float4 kj = *reinterpret_cast<float4*>(&sm.k[js[e]][4 * lane]);
-        const float4 gj = *reinterpret_cast<float4*>(&sm.g[js[e]][4 * lane]);
-        const float x = kj.x * ex2(g.x - gj.x), y = kj.y * ex2(g.y - gj.y);
-        const float z = kj.z * ex2(g.z - gj.z), w = kj.w * ex2(g.w - gj.w);
-        t[e] = fmaf(x, k.x, fmaf(y, k.y, fmaf(z, k.z, w * k.w)));
-        t[4 + e] = fmaf(x, q.x, fmaf(y, q.y, fmaf(z, q.z, w * q.w)));
+        const ulonglong2 kj = *reinterpret_cast<ulonglong2*>(&sm.k[js[e]][4 * lane]);
+        const ulonglong2 dj = *reinterpret_cast<ulonglong2*>(&sm.dec[js[e]][4 * lane]);
+        const uint64_t x = mul2(f.x, kj.x), y = mul2(f.y, kj.y);
+        t[e] = sum2(fma2(x, k.x, mul2(y, k.y)));
+        t[4 + e] = sum2(fma2(x, q.x, mul2(y, q.y)));
+        f.x = mul2(f.x, dj.x), f.y = mul2(f.y, dj.y);
       }
 #pragma unroll
       for (int o = 16, m = 4; o >= 4; o >>= 1, m >>= 1) {      // lanes 4 x .. + 3 receive value x
@@ -350,20 +369,42 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
       }
     }
   }
-  // ---- A k and A q as the products' second operand, in the place of k and q
+  // ---- A k and A q as the products' second operand, in the place of k and q; all the warp's paths walked at once
   {
     uint32_t hi[N / kWarps][4], lo[N / kWarps][4];
+    {
+      ulonglong2 f[N / kWarps];
+      int at[N / kWarps];
+      bool more = true;
 #pragma unroll
-    for (int t = 0; t < N / kWarps; ++t) {
-      const int i = warp + kWarps * t;
-      if (i >= n) continue;
-      const float4 k = *reinterpret_cast<float4*>(&sm.k[i][4 * lane]), q = *reinterpret_cast<float4*>(&sm.q[i][4 * lane]);
-      const float4 g = *reinterpret_cast<float4*>(&sm.g[i][4 * lane]);
-      const float x = ex2(g.x), y = ex2(g.y), z = ex2(g.z), w = ex2(g.w);
-      split2(k.x * x, k.y * y, hi[t][0], lo[t][0]);
-      split2(k.z * z, k.w * w, hi[t][1], lo[t][1]);
-      split2(q.x * x, q.y * y, hi[t][2], lo[t][2]);
-      split2(q.z * z, q.w * w, hi[t][3], lo[t][3]);
+      for (int t = 0; t < N / kWarps; ++t) {
+        f[t] = make_ulonglong2(f2pack(1.0f, 1.0f), f2pack(1.0f, 1.0f));
+        at[t] = warp + kWarps * t < n ? warp + kWarps * t : -1;
+      }
+#pragma unroll 1
+      while (more) {
+        more = false;
+#pragma unroll
+        for (int t = 0; t < N / kWarps; ++t) {
+          if (at[t] < 0) continue;
+          const ulonglong2 d = *reinterpret_cast<ulonglong2*>(&sm.dec[at[t]][4 * lane]);
+          f[t].x = mul2(f[t].x, d.x), f[t].y = mul2(f[t].y, d.y);
+          at[t] = sm.parent[at[t]];
+          more = true;
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < N / kWarps; ++t) {
+        const int i = min(warp + kWarps * t, n - 1);
+        const ulonglong2 k = *reinterpret_cast<ulonglong2*>(&sm.k[i][4 * lane]), q = *reinterpret_cast<ulonglong2*>(&sm.q[i][4 * lane]);
+        const uint64_t y[4] = {mul2(f[t].x, k.x), mul2(f[t].y, k.y), mul2(f[t].x, q.x), mul2(f[t].y, q.y)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float y0, y1;
+          f2unpack(y[e], y0, y1);
+          split2(y0, y1, hi[t][e], lo[t][e]);
+        }
+      }
     }
     __syncthreads();
     const int chunk = lane >> 4, granule = (lane & 15) >> 1, within = (lane & 1) * 8;
@@ -381,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
   fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
-  const uint32_t bar = smem_u32(&sm.bar);
+  const uint32_t bar = smem_u32(&sm.bar[0]);
   if (tid == 0) {
     tc_fence_after();
     constexpr uint32_t idesc = idesc_bf16(128, 2 * N);
@@ -393,89 +434,112 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
         const uint64_t bd = smem_desc(smem_u32(&sm.op[t == 1][c][0][0]), 0, 1024, 2);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
-          mma_f16_ta(tmem + kColD, tmem + kColS + (t == 2 ? 64 : 0) + 32 * c + 8 * ks, bd + 2 * ks, idesc, acc);
+          mma_f16_ta(tmem + kColD, tmem + kColS + (t == 2 ? kColLo : 0) + 32 * c + 8 * ks, bd + 2 * ks, idesc, acc);
           acc = 1;
         }
       }
     }
     tc_commit(bar);
   }
-  // ---- meanwhile the values' inputs, and the scalars (threads 192 + i: node i's)
+  // ---- meanwhile the values' inputs, and the scalars (threads 192 + i: node i's row of P)
   {
     const uint32_t* in = reinterpret_cast<const uint32_t*>(a.x + 2 * (int64_t)a.P + h * kDim + 2 * pair);
     const int64_t pitch = a.ldx / 2;
 #pragma unroll 4
     for (int i = part; i < n; i += 4) cp_async4(&sm.v[i][pair], in + (s + i) * pitch);
   }
-  if (part == 3) {
+  if (part == 3 && tid - 192 < N) {
     const int i = tid - 192;
+#pragma unroll
+    for (int c = 0; c < 128; c += 16)
+      *reinterpret_cast<uint4*>(&sm.p[0][i][c]) = *reinterpret_cast<uint4*>(&sm.p[1][i][c]) = make_uint4(0, 0, 0, 0);
     const int at = i < n ? sm.off[i] : 0, len = i < n ? sm.off[i + 1] - at : 0;
-    int m = i;
-    for (int c = 0; c < len; ++c) {
-      sm.up[at + c] = static_cast<uint8_t>(m);
-      m = sm.parent[m];
-    }
     float* pn = sm.pn + at;
+    int m = i;
 #pragma unroll 1
     for (int c = 0; c < len; ++c) {
-      m = sm.up[at + c];
       const float y = pn[c] * sm.beta[m];
-      pn[c] = y;
       const float* pm = sm.pm + (sm.off[m] - m);
 #pragma unroll 4
       for (int e = c + 1; e < len; ++e) pn[e] = fmaf(-y, pm[e - c - 1], pn[e]);
+      const __nv_bfloat16 y_hi = __float2bfloat16(y);
+      const int to = (((m >> 3) ^ (i & 7)) << 4) + 2 * (m & 7);
+      *reinterpret_cast<__nv_bfloat16*>(&sm.p[0][i][to]) = y_hi;
+      *reinterpret_cast<__nv_bfloat16*>(&sm.p[1][i][to]) = __float2bfloat16(y - __bfloat162float(y_hi));
+      m = sm.parent[m];
     }
   }
   cp_async_wait();
-  const bool ok = mbar_wait(bar, 0, &sm.abort, a.status);
-  const bool done = !__syncthreads_or(!ok);
+  bool ok = mbar_wait(bar, 0, &sm.abort, a.status);
+  fence_proxy_async_smem();
+  ok = !__syncthreads_or(!ok);
   tc_fence_after();
-  if (done) {
-    const uint32_t d = tmem + (static_cast<uint32_t>(32 * quarter) << 16) + kColD;
-    constexpr int kHalf = N / 2;                               // a half of the nodes a thread of its value row
-    {
-      float held[3] = {0.0f, 0.0f, 0.0f};
-      if (init)
-        for (int j = 0; j < 3; ++j) held[j] = __bfloat162float(cs[((int64_t)(2 - j) * 3 + 2) * a.P + v]);
-      const uint2 wv = __ldg(reinterpret_cast<const uint2*>(a.conv_w + (2 * (int64_t)a.P + h * kDim + v) * 4));
-      const float2 p0 = bf2(wv.x), p1 = bf2(wv.y);
-      const auto row = [&](int j) { return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(sm.v[j])[v]); };
+  const uint32_t rows = static_cast<uint32_t>(32 * quarter) << 16;
+  constexpr int kHalf = N / 2;                                 // a half of the nodes a thread of its value row
+  // ---- w = v - S (A k), as bf16 parts in the place of S; zeros past the nodes, whose columns of P are zeros too
+  if (ok) {
+    float held[3] = {0.0f, 0.0f, 0.0f};
+    if (init)
+      for (int j = 0; j < 3; ++j) held[j] = __bfloat162float(cs[((int64_t)(2 - j) * 3 + 2) * a.P + v]);
+    const uint2 wv = __ldg(reinterpret_cast<const uint2*>(a.conv_w + (2 * (int64_t)a.P + h * kDim + v) * 4));
+    const float2 p0 = bf2(wv.x), p1 = bf2(wv.y);
+    const auto row = [&](int j) { return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(sm.v[j])[v]); };
 #pragma unroll 1
-      for (int c = kHalf * half; c < min(kHalf * (half + 1), n); c += 8) {
-        float y[8];
-        tmem_ld_x8(d + c, y);
-        tmem_ld_wait();
+    for (int c = kHalf * half; c < kHalf * (half + 1); c += 8) {
+      float y[8], w[8];
+      tmem_ld_x8(tmem + rows + kColD + c, y);
+      float x[8][4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int i = min(c + j, n - 1);
-          const uint32_t taps = sm.tap[i];
-          const float x = fmaf(p1.y, row(i), fmaf(p1.x, tap_of(taps, 0, held, row),
-                                                  fmaf(p0.y, tap_of(taps, 1, held, row), p0.x * tap_of(taps, 2, held, row))));
-          if (c + j < n) sm.w[i][v] = silu_short(x) - y[j];
-        }
+      for (int j = 0; j < 8; ++j) {
+        const int i = min(c + j, n - 1);
+        load_taps(x[j], i, sm.tap[i], held, row);
       }
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float t = silu_short(fmaf(p1.y, x[j][3], fmaf(p1.x, x[j][2], fmaf(p0.y, x[j][1], p0.x * x[j][0]))));
+        w[j] = c + j < n ? t - y[j] : 0.0f;
+      }
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) split2(w[2 * j], w[2 * j + 1], hi[j], lo[j]);
+      tmem_st_x4(tmem + rows + kColS + c / 2, hi);
+      tmem_st_x4(tmem + rows + kColS + kColLo + c / 2, lo);
     }
-    __syncthreads();
+    tmem_st_wait();
+  }
+  tc_fence_before();
+  __syncthreads();
+  const uint32_t bar2 = smem_u32(&sm.bar[1]);
+  if (ok && tid == 0) {
+    tc_fence_after();
+    constexpr uint32_t idesc = idesc_bf16(128, N);
+#pragma unroll 1
+    for (int t = 0; t < 3; ++t) {                              // onto S (A q)
+      const uint64_t bd = smem_desc(smem_u32(&sm.p[t == 1][0][0]), 0, 1024, 2);
+#pragma unroll
+      for (int ks = 0; ks < N / 16; ++ks)
+        mma_f16_ta(tmem + kColD + N, tmem + kColS + (t == 2 ? kColLo : 0) + 8 * ks, bd + 2 * ks, idesc, 1u);
+    }
+    tc_commit(bar2);
+  }
+  if (ok) ok = mbar_wait(bar2, 0, &sm.abort, a.status);
+  if (!__syncthreads_or(!ok)) {
+    tc_fence_after();
     __nv_bfloat16* out = a.out + (int64_t)s * a.ldo + h * kDim + v;
 #pragma unroll 1
     for (int c = kHalf * half; c < min(kHalf * (half + 1), n); c += 8) {
       float z[8];
-      tmem_ld_x8(d + N + c, z);
+      tmem_ld_x8(tmem + rows + kColD + N + c, z);
       tmem_ld_wait();
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int i = c + j;
-        if (i >= n) continue;
-        const int at = sm.off[i], end = sm.off[i + 1];
-        float o = z[j];
-#pragma unroll 4
-        for (int e = at; e < end; ++e) o = fmaf(sm.pn[e], sm.w[sm.up[e]][v], o);
-        out[i * a.ldo] = __float2bfloat16(o);
-      }
+      for (int j = 0; j < 8; ++j)
+        if (c + j < n) out[(c + j) * a.ldo] = __float2bfloat16(z[j]);
     }
   } else {
-    const unsigned long long t0 = globaltimer();               // the products may still be on their way
-    while (!mbar_try_wait(bar, 0) && globaltimer() - t0 <= 2 * kWaitNs) {}
+    // products may still be on their way
+    const unsigned long long t0 = globaltimer();
+    while (!(mbar_try_wait(bar, 0) && mbar_try_wait(bar2, 0)) && globaltimer() - t0 <= 2 * kWaitNs) {}
   }
   tc_fence_before();
   __syncthreads();
