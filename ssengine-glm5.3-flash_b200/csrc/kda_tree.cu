@@ -12,8 +12,9 @@
 // path (each is at most 1; quotients of cumulated ones would overflow).
 //
 // One CTA a (request, head), 256 threads, two CTAs an SM:
-//   conv and gates: a thread a pair of channels of q or k for every second node, of g for every fourth;
-//   pairs: a warp a node and those above it, 4 at a time, 4 channels a lane;
+//   conv and gates: a thread a pair of channels of q and k (they share the taps' addresses) for every fourth node, then of g,
+//       late of v;
+//   norms, pairs, A k and A q: half a warp a node (8 channels a lane), its pairs 4 at a time;
 //   products: [S (A k) | S (A q)] on the tensor cores, M = 128 value rows, N = 2 nodes, K = 128 keys, tcgen05 kind::f16: S in
 //       TMEM and the vectors in shared memory, both as two bf16 parts, three of the four products (what is left out is below
 //       2^-16 of a product; the output has 8 bits). S comes straight from global memory, a value row a lane;
@@ -42,20 +43,25 @@ struct TreeSmem {
       float q[N][kDim];                    // queries, normalised and scaled
     };
     uint8_t op[2][2][2 * N][128];          // A k, A q: high and low parts, 2 chunks of 64 keys [rows x 128 B], swizzled
+    float v[N][kDim];                      // then the values
   };
   union {
-    uint32_t in[2][N][kDim / 2];           // inputs of q and k
-    float dec[N][kDim];                    // then the decays
-    struct {                               // once A k and A q are made
-      uint8_t p[2][N][128];                // P: high and low parts [nodes x nodes], swizzled
-      uint32_t v[N][kDim / 2];             // inputs of the values
+    uint32_t in[N + 3][2][kDim / 2];       // inputs of q and k, behind them the block's kept rows (N the newest)
+    struct {
+      union {
+        float dec[N][kDim];                // the decays
+        struct {                           // once A k and A q are made
+          uint8_t p[2][N][128];            // P: high and low parts [nodes x nodes], swizzled
+          uint32_t vin[N][kDim / 2];       // inputs of the values
+        };
+      };
+      float pm[N * (N - 1) / 2];           // M_ij: of node i from off[i] - i on, by distance - 1
     };
   };
   float pn[N * (N + 1) / 2];               // N_ij: of node i from off[i] on, by distance. Before, bytes: node i's path, in the
                                            // last bytes of its place (overwritten behind their use)
-  float pm[N * (N - 1) / 2];               // M_ij: of node i from off[i] - i on, by distance - 1
   float beta[N];
-  uint32_t tap[N];                         // bytes: the rows before the node's in the conv, kMaxNodes + j: the j-th newest kept row
+  uint32_t tap[N];                         // bytes: the rows before the node's in the conv, N + j: the j-th newest kept row
   uint16_t off[N + 2];
   int8_t parent[N];
   uint64_t bar[2];
@@ -118,20 +124,17 @@ SSB_DEVICE void cp_async4(void* dst, const void* src) {
 }
 SSB_DEVICE void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// Four conv taps (0: the oldest) of a node: x[3] its own row's value, the others by `taps`, of which those behind a root are
-// the block's kept rows (held[0] the newest).
-template <class T, class Row>
-SSB_DEVICE void load_taps(T (&x)[4], int i, uint32_t taps, const T (&held)[3], Row row) {
-  x[3] = row(i);
-#pragma unroll
-  for (int e = 0; e < 3; ++e) x[2 - e] = row(static_cast<int>((taps >> (8 * e)) & (kMaxNodes - 1)));
-  if (taps & 0x404040u) {
-#pragma unroll
-    for (int e = 0; e < 3; ++e) {
-      const uint32_t t = (taps >> (8 * e)) & 0xFF;
-      if (t >= kMaxNodes) x[2 - e] = t == kMaxNodes ? held[0] : t == kMaxNodes + 1 ? held[1] : held[2];
-    }
-  }
+// A pair of channels through the conv (packed weights, the oldest tap's first) and SiLU.
+SSB_DEVICE float2 conv_silu(const uint64_t (&p)[4], const uint32_t (&x)[4]) {
+  const uint64_t o = fma2(p[3], bf2_f2(x[3]), fma2(p[2], bf2_f2(x[2]), fma2(p[1], bf2_f2(x[1]), mul2(p[0], bf2_f2(x[0])))));
+  float2 y;
+  f2unpack(o, y.x, y.y);
+  return make_float2(silu_short(y.x), silu_short(y.y));
+}
+SSB_DEVICE void conv_weights(uint64_t (&p)[4], const __nv_bfloat16* w) {             // 2 channels x 4 taps
+  const uint4 wv = __ldg(reinterpret_cast<const uint4*>(w));
+  const float2 a0 = bf2(wv.x), a1 = bf2(wv.y), b0 = bf2(wv.z), b1 = bf2(wv.w);
+  p[0] = f2pack(a0.x, b0.x), p[1] = f2pack(a0.y, b0.y), p[2] = f2pack(a1.x, b1.x), p[3] = f2pack(a1.y, b1.y);
 }
 
 template <int N>
@@ -180,12 +183,20 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
   }
   // ---- the inputs of q and k into shared memory (threads 0-191); the tree (threads 192-255)
   const int pair = tid & 63, part = tid >> 6;
+  const __nv_bfloat16* cs = a.conv_state + (int64_t)sq.z * a.cs_stride + h * kDim;            // of q; k, v: + P, + 2 P
   bool bad = false;
   if (part < 3) {
     const uint32_t* in = reinterpret_cast<const uint32_t*>(a.x + h * kDim + 2 * pair) + s * (a.ldx / 2);
-#pragma unroll 4
-    for (int i = part; i < 2 * n; i += 3)
-      cp_async4(&sm.in[i & 1][i >> 1][pair], in + (i >> 1) * (a.ldx / 2) + (i & 1) * (a.P / 2));
+#pragma unroll 2
+    for (int i = part; i < n; i += 3) {
+      const uint32_t* x = in + i * (a.ldx / 2);
+      cp_async4(&sm.in[i][0][pair], x);
+      cp_async4(&sm.in[i][1][pair], x + a.P / 2);
+    }
+    // kept row part (0: the oldest)
+    const uint32_t* kept = reinterpret_cast<const uint32_t*>(cs + (int64_t)part * 3 * a.P + 2 * pair);
+    sm.in[N + 2 - part][0][pair] = init ? __ldg(kept) : 0;
+    sm.in[N + 2 - part][1][pair] = init ? __ldg(kept + a.P / 2) : 0;
   } else {
     // thread 192 + i: node i, its path walked twice: its length, then its nodes
     const int i = tid - 192;
@@ -206,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
     uint32_t taps = 0;
     if (node && !bad) {
       int at = p;
-      for (int j = 0, kept = kMaxNodes; j < 3; ++j) {
+      for (int j = 0, kept = N; j < 3; ++j) {
         taps |= static_cast<uint32_t>(at >= 0 ? at : kept++) << (8 * j);
         if (at >= 0) at = sm.parent[at], ++len;
       }
@@ -239,7 +250,8 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
   {
     const uint32_t* in = reinterpret_cast<const uint32_t*>(a.g + h * kDim + 2 * pair) + s * (a.ldg / 2);
 #pragma unroll
-    for (int t = 0; t < N / 4; ++t) gin[t] = __ldg(in + min(part + 4 * t, n - 1) * (a.ldg / 2));
+    for (int t = 0; t < N / 4; ++t)
+      if (part + 4 * t < n) gin[t] = __ldg(in + (part + 4 * t) * (a.ldg / 2));
   }
   cp_async_wait();
   tc_fence_before();
@@ -266,34 +278,32 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
     tmem_st_wait();
   }
 
-  // ---- the conv of q and k: 4 nodes at a time, every second one
-  const __nv_bfloat16* cs = a.conv_state + (int64_t)sq.z * a.cs_stride + h * kDim;              // of q; k, v: + P, + 2 P
+  // ---- the conv of q and k: every fourth node, 2 at a time
   {
-    const int which = part & 1;                              // q, k
-    uint32_t held[3] = {0, 0, 0};
-    if (init)
-      for (int j = 0; j < 3; ++j)
-        held[j] = *reinterpret_cast<const uint32_t*>(cs + ((int64_t)(2 - j) * 3 + which) * a.P + 2 * pair);
-    const uint4 wv = __ldg(reinterpret_cast<const uint4*>(a.conv_w + ((int64_t)which * a.P + h * kDim + 2 * pair) * 4));
-    const float2 a0 = bf2(wv.x), a1 = bf2(wv.y), b0 = bf2(wv.z), b1 = bf2(wv.w);               // 2 channels x 4 taps
-    const uint64_t p0 = f2pack(a0.x, b0.x), p1 = f2pack(a0.y, b0.y), p2 = f2pack(a1.x, b1.x), p3 = f2pack(a1.y, b1.y);
-    const auto row = [&](int j) { return sm.in[which][j][pair]; };
-    float* to = (which ? &sm.k[0][0] : &sm.q[0][0]) + 2 * pair;
+    uint64_t pq[4], pk[4];
+    conv_weights(pq, a.conv_w + ((int64_t)h * kDim + 2 * pair) * 4);
+    conv_weights(pk, a.conv_w + ((int64_t)a.P + h * kDim + 2 * pair) * 4);
 #pragma unroll 1
-    for (int i = half; i < n; i += 8) {
-      uint32_t x[4][4];
+    for (int i = part; i < n; i += 8) {
+      uint32_t xq[2][4], xk[2][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int m = min(i + 2 * j, n - 1);
-        load_taps(x[j], m, sm.tap[m], held, row);
+      for (int j = 0; j < 2; ++j) {
+        const int m = min(i + 4 * j, n - 1);
+        const uint32_t taps = sm.tap[m];
+        xq[j][3] = sm.in[m][0][pair], xk[j][3] = sm.in[m][1][pair];
+#pragma unroll
+        for (int e = 0; e < 3; ++e) {
+          const uint32_t* row = &sm.in[(taps >> (8 * e)) & 0xFF][0][pair];
+          xq[j][2 - e] = row[0], xk[j][2 - e] = row[kDim / 2];
+        }
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint64_t o = fma2(p3, bf2_f2(x[j][3]), fma2(p2, bf2_f2(x[j][2]), fma2(p1, bf2_f2(x[j][1]), mul2(p0, bf2_f2(x[j][0])))));
-        float2 y;
-        f2unpack(o, y.x, y.y);
-        y.x = silu_short(y.x), y.y = silu_short(y.y);
-        if (i + 2 * j < n) *reinterpret_cast<float2*>(to + (i + 2 * j) * kDim) = y;
+      for (int j = 0; j < 2; ++j) {
+        const float2 q = conv_silu(pq, xq[j]), k = conv_silu(pk, xk[j]);
+        if (i + 4 * j < n) {
+          *reinterpret_cast<float2*>(&sm.q[i + 4 * j][2 * pair]) = q;
+          *reinterpret_cast<float2*>(&sm.k[i + 4 * j][2 * pair]) = k;
+        }
       }
     }
   }
@@ -304,119 +314,159 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
     const float rate = -kLog2e * exp_fast(__ldg(a.a_log + h)), lb = a.lower_bound * kLog2e;
 #pragma unroll
     for (int t = 0; t < N / 4; ++t) {
+      if (part + 4 * t >= n) continue;
       const float2 x = bf2(gin[t]);
       float2 o;
       o.x = ex2(lb * rcp(1.0f + ex2(rate * (x.x + dt.x))));
       o.y = ex2(lb * rcp(1.0f + ex2(rate * (x.y + dt.y))));
-      if (part + 4 * t < n) *reinterpret_cast<float2*>(&sm.dec[part + 4 * t][2 * pair]) = o;
+      *reinterpret_cast<float2*>(&sm.dec[part + 4 * t][2 * pair]) = o;
     }
   }
 
-  // ---- norms: a warp a node, 4 channels a lane
+  // ---- norms: half a warp a node, channels 4 l .. + 3 and 64 + 4 l .. + 3 a lane
+  const int l = lane & 15, first = 2 * warp + (lane >> 4);    // node first + 16 t
+  const auto load8 = [&](const float* row, ulonglong2 (&x)[2]) {
+    x[0] = *reinterpret_cast<const ulonglong2*>(row + 4 * l);
+    x[1] = *reinterpret_cast<const ulonglong2*>(row + 64 + 4 * l);
+  };
+  const auto dot8 = [](const ulonglong2 (&x)[2], const ulonglong2 (&y)[2]) {
+    return sum2(fma2(x[0].x, y[0].x, fma2(x[0].y, y[0].y, fma2(x[1].x, y[1].x, mul2(x[1].y, y[1].y)))));
+  };
+  const auto scale8 = [](ulonglong2 (&x)[2], uint64_t f) {
+    x[0].x = mul2(x[0].x, f), x[0].y = mul2(x[0].y, f), x[1].x = mul2(x[1].x, f), x[1].y = mul2(x[1].y, f);
+  };
+  const auto mul8 = [](ulonglong2 (&x)[2], const ulonglong2 (&y)[2]) {
+    x[0].x = mul2(x[0].x, y[0].x), x[0].y = mul2(x[0].y, y[0].y), x[1].x = mul2(x[1].x, y[1].x), x[1].y = mul2(x[1].y, y[1].y);
+  };
+  const ulonglong2 ones = make_ulonglong2(f2pack(1.0f, 1.0f), f2pack(1.0f, 1.0f));
 #pragma unroll 1
-  for (int i = warp; i < n; i += kWarps) {
-    float4* kp = reinterpret_cast<float4*>(&sm.k[i][4 * lane]);
-    float4* qp = reinterpret_cast<float4*>(&sm.q[i][4 * lane]);
-    float4 q = *qp, k = *kp;
-    const float nk = k.x * k.x + k.y * k.y + k.z * k.z + k.w * k.w, nq = q.x * q.x + q.y * q.y + q.z * q.z + q.w * q.w;
-    float t = (lane < 16 ? nk : nq) + __shfl_xor_sync(0xffffffffu, lane < 16 ? nq : nk, 16);   // lanes 0-15: k's, 16-31: q's
+  for (int i0 = 2 * warp; i0 < n; i0 += 2 * kWarps) {
+    const int i = min(i0 + (lane >> 4), n - 1);
+    ulonglong2 q[2], k[2];
+    load8(sm.q[i], q);
+    load8(sm.k[i], k);
+    const float nk = dot8(k, k), nq = dot8(q, q);
+    float t = (l < 8 ? nk : nq) + __shfl_xor_sync(0xffffffffu, l < 8 ? nq : nk, 8);            // l < 8: k's, from 8 on: q's
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    for (int o = 4; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
     t = rsqrtf(t + 1e-6f);
-    const float rk = __shfl_sync(0xffffffffu, t, 0), rq = a.scale * __shfl_sync(0xffffffffu, t, 16);
-    *kp = make_float4(k.x * rk, k.y * rk, k.z * rk, k.w * rk);
-    *qp = make_float4(q.x * rq, q.y * rq, q.z * rq, q.w * rq);
+    const float other = __shfl_xor_sync(0xffffffffu, t, 8);
+    const float rk = l < 8 ? t : other, rq = a.scale * (l < 8 ? other : t);
+    scale8(q, f2pack(rq, rq));
+    scale8(k, f2pack(rk, rk));
+    __syncwarp();                                              // the last node may be read by both halves
+    if (i == i0 + (lane >> 4)) {
+      *reinterpret_cast<ulonglong2*>(&sm.q[i][4 * l]) = q[0], *reinterpret_cast<ulonglong2*>(&sm.q[i][64 + 4 * l]) = q[1];
+      *reinterpret_cast<ulonglong2*>(&sm.k[i][4 * l]) = k[0], *reinterpret_cast<ulonglong2*>(&sm.k[i][64 + 4 * l]) = k[1];
+    }
   }
   __syncthreads();
   // ---- the pairs of a node and those above it, 4 at a time
 #pragma unroll 1
-  for (int i = warp; i < n; i += kWarps) {
-    const ulonglong2 k = *reinterpret_cast<ulonglong2*>(&sm.k[i][4 * lane]), q = *reinterpret_cast<ulonglong2*>(&sm.q[i][4 * lane]);
-    const int at = sm.off[i], len = sm.off[i + 1] - at;
+  for (int i0 = 2 * warp; i0 < n; i0 += 2 * kWarps) {
+    const int i = i0 + (lane >> 4);
+    ulonglong2 q[2], k[2], f[2] = {ones, ones};                // f: the decays below
+    const int im = min(i, n - 1);
+    load8(sm.q[im], q);
+    load8(sm.k[im], k);
+    const int at = sm.off[im], len = sm.off[im + 1] - at;
+    const int most = max(len, __shfl_xor_sync(0xffffffffu, len, 16));
     const uint8_t* path = reinterpret_cast<const uint8_t*>(sm.pn + at) + 3 * len;
-    ulonglong2 f = make_ulonglong2(f2pack(1.0f, 1.0f), f2pack(1.0f, 1.0f));                    // the decays below
 #pragma unroll 1
-    for (int d = 0; d < len; d += 4) {
+    for (int d = 0; d < most; d += 4) {
       int js[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) js[e] = path[min(d + e, len - 1)];
       float t[8];                                              // M of 4 pairs, N of 4 pairs
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const ulonglong2 kj = *reinterpret_cast<ulonglong2*>(&sm.k[js[e]][4 * lane]);
-        const ulonglong2 dj = *reinterpret_cast<ulonglong2*>(&sm.dec[js[e]][4 * lane]);
-        const uint64_t x = mul2(f.x, kj.x), y = mul2(f.y, kj.y);
-        t[e] = sum2(fma2(x, k.x, mul2(y, k.y)));
-        t[4 + e] = sum2(fma2(x, q.x, mul2(y, q.y)));
-        f.x = mul2(f.x, dj.x), f.y = mul2(f.y, dj.y);
+        ulonglong2 x[2], dj[2];
+        load8(sm.k[js[e] & (N - 1)], x);
+        load8(sm.dec[js[e] & (N - 1)], dj);
+        mul8(x, f);
+        t[e] = dot8(x, k);
+        t[4 + e] = dot8(x, q);
+        mul8(f, dj);
       }
 #pragma unroll
-      for (int o = 16, m = 4; o >= 4; o >>= 1, m >>= 1) {      // lanes 4 x .. + 3 receive value x
-        const bool up = lane & o;
+      for (int o = 8, m = 4; m > 0; o >>= 1, m >>= 1) {        // lanes l = 2 x, 2 x + 1 receive value x
+        const bool up = l & o;
 #pragma unroll
         for (int e = 0; e < m; ++e) {
           const float keep = up ? t[e + m] : t[e], send = up ? t[e] : t[e + m];
           t[e] = keep + __shfl_xor_sync(0xffffffffu, send, o);
         }
       }
-      t[0] += __shfl_xor_sync(0xffffffffu, t[0], 2);
       t[0] += __shfl_xor_sync(0xffffffffu, t[0], 1);
       __syncwarp();                                            // the path's bytes are read
-      const int e = d + ((lane >> 2) & 3);
-      if ((lane & 3) == 0 && e < len) {
-        if (lane >= 16) sm.pn[at + e] = t[0];
+      const int e = d + ((l >> 1) & 3);
+      if ((l & 1) == 0 && e < len && i < n) {
+        if (l >= 8) sm.pn[at + e] = t[0];
         else if (e > 0) sm.pm[at - i + e - 1] = t[0];
       }
+      __syncwarp();
     }
   }
   // ---- A k and A q as the products' second operand, in the place of k and q; all the warp's paths walked at once
   {
-    uint32_t hi[N / kWarps][4], lo[N / kWarps][4];
+    constexpr int kOwn = N / (2 * kWarps);
+    uint32_t hi[kOwn][8], lo[kOwn][8];                         // k, then q
     {
-      ulonglong2 f[N / kWarps];
-      int at[N / kWarps];
-      bool more = true;
+      ulonglong2 f[kOwn][2];
+      int at[kOwn];
 #pragma unroll
-      for (int t = 0; t < N / kWarps; ++t) {
-        f[t] = make_ulonglong2(f2pack(1.0f, 1.0f), f2pack(1.0f, 1.0f));
-        at[t] = warp + kWarps * t < n ? warp + kWarps * t : -1;
+      for (int t = 0; t < kOwn; ++t) {
+        f[t][0] = f[t][1] = ones;
+        at[t] = first + 16 * t < n ? first + 16 * t : -1;
       }
 #pragma unroll 1
-      while (more) {
-        more = false;
+      while (true) {
+        bool more = false;
 #pragma unroll
-        for (int t = 0; t < N / kWarps; ++t) {
+        for (int t = 0; t < kOwn; ++t) {
           if (at[t] < 0) continue;
-          const ulonglong2 d = *reinterpret_cast<ulonglong2*>(&sm.dec[at[t]][4 * lane]);
-          f[t].x = mul2(f[t].x, d.x), f[t].y = mul2(f[t].y, d.y);
+          ulonglong2 d[2];
+          load8(sm.dec[at[t]], d);
+          mul8(f[t], d);
           at[t] = sm.parent[at[t]];
           more = true;
         }
+        if (!__any_sync(0xffffffffu, more)) break;
       }
 #pragma unroll
-      for (int t = 0; t < N / kWarps; ++t) {
-        const int i = min(warp + kWarps * t, n - 1);
-        const ulonglong2 k = *reinterpret_cast<ulonglong2*>(&sm.k[i][4 * lane]), q = *reinterpret_cast<ulonglong2*>(&sm.q[i][4 * lane]);
-        const uint64_t y[4] = {mul2(f[t].x, k.x), mul2(f[t].y, k.y), mul2(f[t].x, q.x), mul2(f[t].y, q.y)};
+      for (int t = 0; t < kOwn; ++t) {
+        if (2 * warp + 16 * t >= n) continue;
+        const int i = min(first + 16 * t, n - 1);
+        ulonglong2 x[2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float y0, y1;
-          f2unpack(y[e], y0, y1);
-          split2(y0, y1, hi[t][e], lo[t][e]);
+        for (int e = 0; e < 2; ++e) {
+          load8(e ? sm.q[i] : sm.k[i], x);
+          mul8(x, f[t]);
+          const uint64_t y[4] = {x[0].x, x[0].y, x[1].x, x[1].y};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            float y0, y1;
+            f2unpack(y[c], y0, y1);
+            split2(y0, y1, hi[t][4 * e + c], lo[t][4 * e + c]);
+          }
         }
       }
     }
     __syncthreads();
-    const int chunk = lane >> 4, granule = (lane & 15) >> 1, within = (lane & 1) * 8;
+    const int granule = l >> 1, within = (l & 1) * 8;
 #pragma unroll
-    for (int t = 0; t < N / kWarps; ++t) {
-      const int i = warp + kWarps * t;
+    for (int t = 0; t < kOwn; ++t) {
+      const int i = first + 16 * t;
       if (i >= n) continue;
       const int at = ((granule ^ (i & 7)) << 4) + within;      // rows i and N + i swizzle alike
-      *reinterpret_cast<uint2*>(&sm.op[0][chunk][i][at]) = make_uint2(hi[t][0], hi[t][1]);
-      *reinterpret_cast<uint2*>(&sm.op[1][chunk][i][at]) = make_uint2(lo[t][0], lo[t][1]);
-      *reinterpret_cast<uint2*>(&sm.op[0][chunk][N + i][at]) = make_uint2(hi[t][2], hi[t][3]);
-      *reinterpret_cast<uint2*>(&sm.op[1][chunk][N + i][at]) = make_uint2(lo[t][2], lo[t][3]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {                            // A k, A q
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {                          // channels 4 l, 64 + 4 l
+          *reinterpret_cast<uint2*>(&sm.op[0][c][N * e + i][at]) = make_uint2(hi[t][4 * e + 2 * c], hi[t][4 * e + 2 * c + 1]);
+          *reinterpret_cast<uint2*>(&sm.op[1][c][N * e + i][at]) = make_uint2(lo[t][4 * e + 2 * c], lo[t][4 * e + 2 * c + 1]);
+        }
+      }
     }
   }
   fence_proxy_async_smem();
@@ -446,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
     const uint32_t* in = reinterpret_cast<const uint32_t*>(a.x + 2 * (int64_t)a.P + h * kDim + 2 * pair);
     const int64_t pitch = a.ldx / 2;
 #pragma unroll 4
-    for (int i = part; i < n; i += 4) cp_async4(&sm.v[i][pair], in + (s + i) * pitch);
+    for (int i = part; i < n; i += 4) cp_async4(&sm.vin[i][pair], in + (s + i) * pitch);
   }
   if (part == 3 && tid - 192 < N) {
     const int i = tid - 192;
@@ -476,30 +526,51 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
   tc_fence_after();
   const uint32_t rows = static_cast<uint32_t>(32 * quarter) << 16;
   constexpr int kHalf = N / 2;                                 // a half of the nodes a thread of its value row
+  // ---- the values, in the place of the products' second operand: a pair of channels of every fourth node a thread
+  {
+    uint64_t p[4];
+    conv_weights(p, a.conv_w + (2 * (int64_t)a.P + h * kDim + 2 * pair) * 4);
+    uint32_t held[3] = {0, 0, 0};
+    if (init)
+      for (int j = 0; j < 3; ++j)
+        held[j] = __ldg(reinterpret_cast<const uint32_t*>(cs + ((int64_t)(2 - j) * 3 + 2) * a.P + 2 * pair));
+#pragma unroll 1
+    for (int i = part; i < n; i += 16) {                       // 4 nodes at a time
+      uint32_t x[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int m = min(i + 4 * j, n - 1);
+        const uint32_t taps = sm.tap[m];
+        x[j][3] = sm.vin[m][pair];
+#pragma unroll
+        for (int e = 0; e < 3; ++e) x[j][2 - e] = sm.vin[(taps >> (8 * e)) & (N - 1)][pair];
+        if (taps & (N * 0x010101u)) {                          // some are kept rows
+#pragma unroll
+          for (int e = 0; e < 3; ++e) {
+            const uint32_t t = (taps >> (8 * e)) & 0xFF;
+            if (t >= N) x[j][2 - e] = t == N ? held[0] : t == N + 1 ? held[1] : held[2];
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 y = conv_silu(p, x[j]);
+        if (i + 4 * j < n) *reinterpret_cast<float2*>(&sm.v[i + 4 * j][2 * pair]) = y;
+      }
+    }
+  }
+  __syncthreads();
   // ---- w = v - S (A k), as bf16 parts in the place of S; zeros past the nodes, whose columns of P are zeros too
   if (ok) {
-    float held[3] = {0.0f, 0.0f, 0.0f};
-    if (init)
-      for (int j = 0; j < 3; ++j) held[j] = __bfloat162float(cs[((int64_t)(2 - j) * 3 + 2) * a.P + v]);
-    const uint2 wv = __ldg(reinterpret_cast<const uint2*>(a.conv_w + (2 * (int64_t)a.P + h * kDim + v) * 4));
-    const float2 p0 = bf2(wv.x), p1 = bf2(wv.y);
-    const auto row = [&](int j) { return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(sm.v[j])[v]); };
 #pragma unroll 1
     for (int c = kHalf * half; c < kHalf * (half + 1); c += 8) {
       float y[8], w[8];
       tmem_ld_x8(tmem + rows + kColD + c, y);
-      float x[8][4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int i = min(c + j, n - 1);
-        load_taps(x[j], i, sm.tap[i], held, row);
-      }
+      for (int j = 0; j < 8; ++j) w[j] = sm.v[c + j][v];
       tmem_ld_wait();
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float t = silu_short(fmaf(p1.y, x[j][3], fmaf(p1.x, x[j][2], fmaf(p0.y, x[j][1], p0.x * x[j][0]))));
-        w[j] = c + j < n ? t - y[j] : 0.0f;
-      }
+      for (int j = 0; j < 8; ++j) w[j] = c + j < n ? w[j] - y[j] : 0.0f;
       uint32_t hi[4], lo[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) split2(w[2 * j], w[2 * j + 1], hi[j], lo[j]);
