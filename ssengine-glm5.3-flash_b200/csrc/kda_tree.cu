@@ -11,8 +11,8 @@
 // the nodes, no node's own state is formed, and nothing but the scalars goes node after node. The decays multiply up the
 // path (each is at most 1; quotients of cumulated ones would overflow).
 //
-// One CTA a (request, head), 256 threads, two CTAs an SM:
-//   conv and gates: a thread a pair of channels of q and k (they share the taps' addresses) for every fourth node, then of g,
+// One CTA a (request, head), 512 threads, two CTAs an SM:
+//   conv and gates: a thread a pair of channels of q and k (they share the taps' addresses) for every eighth node, then of g,
 //       late of v;
 //   norms, pairs, A k and A q: half a warp a node (8 channels a lane), its pairs 4 at a time;
 //   products: [S (A k) | S (A q)] on the tensor cores, M = 128 value rows, N = 2 nodes, K = 128 keys, tcgen05 kind::f16: S in
@@ -29,7 +29,8 @@ namespace ssb {
 namespace {
 
 constexpr int kDim = 128;
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kGroups = kThreads / 64;       // of 64 threads, one a pair of channels; the last one also looks after the tree
 constexpr int kMaxNodes = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 // TMEM: S as 64 columns of high and 64 of low parts, later W^T in the same places; the products
@@ -161,14 +162,14 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
     }
   }
 
-  // ---- the state's loads: a value row a lane, half of its keys a thread
-  const int quarter = warp & 3, half = warp >> 2, v = 32 * quarter + lane;
-  float st[64];
+  // ---- the state's loads: a value row a lane, a fourth of its keys a thread
+  const int quarter = warp & 3, fourth = warp >> 2, v = 32 * quarter + lane;
+  float st[32];
   {
-    const float* S = a.rec_state + (int64_t)sq.z * a.rs_stride + ((int64_t)h * kDim + v) * kDim + 64 * half;
+    const float* S = a.rec_state + (int64_t)sq.z * a.rs_stride + ((int64_t)h * kDim + v) * kDim + 32 * fourth;
     const bool wide = (reinterpret_cast<uintptr_t>(S) & 31) == 0;
 #pragma unroll
-    for (int c = 0; c < 64; c += 8) {
+    for (int c = 0; c < 32; c += 8) {
       if (init && wide) {
         ld8(S + c, st + c);
       } else if (init) {
@@ -181,25 +182,27 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
       }
     }
   }
-  // ---- the inputs of q and k into shared memory (threads 0-191); the tree (threads 192-255)
+  // ---- the inputs of q and k into shared memory; the tree (the last 64 threads)
   const int pair = tid & 63, part = tid >> 6;
   const __nv_bfloat16* cs = a.conv_state + (int64_t)sq.z * a.cs_stride + h * kDim;            // of q; k, v: + P, + 2 P
   bool bad = false;
-  if (part < 3) {
+  if (part < kGroups - 1) {
     const uint32_t* in = reinterpret_cast<const uint32_t*>(a.x + h * kDim + 2 * pair) + s * (a.ldx / 2);
 #pragma unroll 2
-    for (int i = part; i < n; i += 3) {
+    for (int i = part; i < n; i += kGroups - 1) {
       const uint32_t* x = in + i * (a.ldx / 2);
       cp_async4(&sm.in[i][0][pair], x);
       cp_async4(&sm.in[i][1][pair], x + a.P / 2);
     }
     // kept row part (0: the oldest)
-    const uint32_t* kept = reinterpret_cast<const uint32_t*>(cs + (int64_t)part * 3 * a.P + 2 * pair);
-    sm.in[N + 2 - part][0][pair] = init ? __ldg(kept) : 0;
-    sm.in[N + 2 - part][1][pair] = init ? __ldg(kept + a.P / 2) : 0;
+    if (part < 3) {
+      const uint32_t* kept = reinterpret_cast<const uint32_t*>(cs + (int64_t)part * 3 * a.P + 2 * pair);
+      sm.in[N + 2 - part][0][pair] = init ? __ldg(kept) : 0;
+      sm.in[N + 2 - part][1][pair] = init ? __ldg(kept + a.P / 2) : 0;
+    }
   } else {
-    // thread 192 + i: node i, its path walked twice: its length, then its nodes
-    const int i = tid - 192;
+    // node i a thread, its path walked twice: its length, then its nodes
+    const int i = tid - 64 * (kGroups - 1);
     const bool node = i < n;
     int p = -1;
     if (node) {
@@ -245,13 +248,13 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
       }
     }
   }
-  // the gates' inputs: a pair of channels of every fourth node a thread
-  uint32_t gin[N / 4];
+  // the gates' inputs: a pair of channels of every eighth node a thread
+  uint32_t gin[N / kGroups];
   {
     const uint32_t* in = reinterpret_cast<const uint32_t*>(a.g + h * kDim + 2 * pair) + s * (a.ldg / 2);
 #pragma unroll
-    for (int t = 0; t < N / 4; ++t)
-      if (part + 4 * t < n) gin[t] = __ldg(in + (part + 4 * t) * (a.ldg / 2));
+    for (int t = 0; t < N / kGroups; ++t)
+      if (part + kGroups * t < n) gin[t] = __ldg(in + (part + kGroups * t) * (a.ldg / 2));
   }
   cp_async_wait();
   tc_fence_before();
@@ -265,30 +268,29 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
   const uint32_t tmem = sm.tmem;
   // ---- the state's parts to TMEM
   {
-    const uint32_t at = tmem + (static_cast<uint32_t>(32 * quarter) << 16) + kColS + 32 * half;
-    float hi[32], lo[32];
+    const uint32_t at = tmem + (static_cast<uint32_t>(32 * quarter) << 16) + kColS + 16 * fourth;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      uint32_t x, y;
-      split2(st[2 * j], st[2 * j + 1], x, y);
-      hi[j] = __uint_as_float(x), lo[j] = __uint_as_float(y);
+    for (int j = 0; j < 4; ++j) {
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) split2(st[8 * j + 2 * e], st[8 * j + 2 * e + 1], hi[e], lo[e]);
+      tmem_st_x4(at + 4 * j, hi);
+      tmem_st_x4(at + kColLo + 4 * j, lo);
     }
-    tmem_st_32x32b_x32(at, hi);
-    tmem_st_32x32b_x32(at + kColLo, lo);
     tmem_st_wait();
   }
 
-  // ---- the conv of q and k: every fourth node, 2 at a time
+  // ---- the conv of q and k: every eighth node, 2 at a time
   {
     uint64_t pq[4], pk[4];
     conv_weights(pq, a.conv_w + ((int64_t)h * kDim + 2 * pair) * 4);
     conv_weights(pk, a.conv_w + ((int64_t)a.P + h * kDim + 2 * pair) * 4);
 #pragma unroll 1
-    for (int i = part; i < n; i += 8) {
+    for (int i = part; i < n; i += 2 * kGroups) {
       uint32_t xq[2][4], xk[2][4];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int m = min(i + 4 * j, n - 1);
+        const int m = min(i + kGroups * j, n - 1);
         const uint32_t taps = sm.tap[m];
         xq[j][3] = sm.in[m][0][pair], xk[j][3] = sm.in[m][1][pair];
 #pragma unroll
@@ -300,9 +302,9 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const float2 q = conv_silu(pq, xq[j]), k = conv_silu(pk, xk[j]);
-        if (i + 4 * j < n) {
-          *reinterpret_cast<float2*>(&sm.q[i + 4 * j][2 * pair]) = q;
-          *reinterpret_cast<float2*>(&sm.k[i + 4 * j][2 * pair]) = k;
+        if (i + kGroups * j < n) {
+          *reinterpret_cast<float2*>(&sm.q[i + kGroups * j][2 * pair]) = q;
+          *reinterpret_cast<float2*>(&sm.k[i + kGroups * j][2 * pair]) = k;
         }
       }
     }
@@ -313,18 +315,18 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
     const float2 dt = __ldg(reinterpret_cast<const float2*>(a.dt_bias + h * kDim) + pair);
     const float rate = -kLog2e * exp_fast(__ldg(a.a_log + h)), lb = a.lower_bound * kLog2e;
 #pragma unroll
-    for (int t = 0; t < N / 4; ++t) {
-      if (part + 4 * t >= n) continue;
+    for (int t = 0; t < N / kGroups; ++t) {
+      if (part + kGroups * t >= n) continue;
       const float2 x = bf2(gin[t]);
       float2 o;
       o.x = ex2(lb * rcp(1.0f + ex2(rate * (x.x + dt.x))));
       o.y = ex2(lb * rcp(1.0f + ex2(rate * (x.y + dt.y))));
-      *reinterpret_cast<float2*>(&sm.dec[part + 4 * t][2 * pair]) = o;
+      *reinterpret_cast<float2*>(&sm.dec[part + kGroups * t][2 * pair]) = o;
     }
   }
 
   // ---- norms: half a warp a node, channels 4 l .. + 3 and 64 + 4 l .. + 3 a lane
-  const int l = lane & 15, first = 2 * warp + (lane >> 4);    // node first + 16 t
+  const int l = lane & 15, first = 2 * warp + (lane >> 4);    // node first + 2 kWarps t
   const auto load8 = [&](const float* row, ulonglong2 (&x)[2]) {
     x[0] = *reinterpret_cast<const ulonglong2*>(row + 4 * l);
     x[1] = *reinterpret_cast<const ulonglong2*>(row + 64 + 4 * l);
@@ -409,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
   }
   // ---- A k and A q as the products' second operand, in the place of k and q; all the warp's paths walked at once
   {
-    constexpr int kOwn = N / (2 * kWarps);
+    constexpr int kOwn = N > 2 * kWarps ? N / (2 * kWarps) : 1;
     uint32_t hi[kOwn][8], lo[kOwn][8];                         // k, then q
     {
       ulonglong2 f[kOwn][2];
@@ -417,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
 #pragma unroll
       for (int t = 0; t < kOwn; ++t) {
         f[t][0] = f[t][1] = ones;
-        at[t] = first + 16 * t < n ? first + 16 * t : -1;
+        at[t] = first + 2 * kWarps * t < n ? first + 2 * kWarps * t : -1;
       }
 #pragma unroll 1
       while (true) {
@@ -435,8 +437,8 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
       }
 #pragma unroll
       for (int t = 0; t < kOwn; ++t) {
-        if (2 * warp + 16 * t >= n) continue;
-        const int i = min(first + 16 * t, n - 1);
+        if (2 * warp + 2 * kWarps * t >= n) continue;
+        const int i = min(first + 2 * kWarps * t, n - 1);
         ulonglong2 x[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -456,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
     const int granule = l >> 1, within = (l & 1) * 8;
 #pragma unroll
     for (int t = 0; t < kOwn; ++t) {
-      const int i = first + 16 * t;
+      const int i = first + 2 * kWarps * t;
       if (i >= n) continue;
       const int at = ((granule ^ (i & 7)) << 4) + within;      // rows i and N + i swizzle alike
 #pragma unroll
@@ -491,15 +493,15 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
     }
     tc_commit(bar);
   }
-  // ---- meanwhile the values' inputs, and the scalars (threads 192 + i: node i's row of P)
+  // ---- meanwhile the values' inputs, and the scalars (node i's row of P by the i-th of the last 64 threads)
   {
     const uint32_t* in = reinterpret_cast<const uint32_t*>(a.x + 2 * (int64_t)a.P + h * kDim + 2 * pair);
     const int64_t pitch = a.ldx / 2;
 #pragma unroll 4
-    for (int i = part; i < n; i += 4) cp_async4(&sm.vin[i][pair], in + (s + i) * pitch);
+    for (int i = part; i < n; i += kGroups) cp_async4(&sm.vin[i][pair], in + (s + i) * pitch);
   }
-  if (part == 3 && tid - 192 < N) {
-    const int i = tid - 192;
+  if (part == kGroups - 1 && pair < N) {
+    const int i = pair;
 #pragma unroll
     for (int c = 0; c < 128; c += 16)
       *reinterpret_cast<uint4*>(&sm.p[0][i][c]) = *reinterpret_cast<uint4*>(&sm.p[1][i][c]) = make_uint4(0, 0, 0, 0);
@@ -525,8 +527,8 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
   ok = !__syncthreads_or(!ok);
   tc_fence_after();
   const uint32_t rows = static_cast<uint32_t>(32 * quarter) << 16;
-  constexpr int kHalf = N / 2;                                 // a half of the nodes a thread of its value row
-  // ---- the values, in the place of the products' second operand: a pair of channels of every fourth node a thread
+  constexpr int kShare = N < 32 ? 8 : N / 4;                   // nodes of its value row that a thread has
+  // ---- the values, in the place of the products' second operand: a pair of channels of every eighth node a thread
   {
     uint64_t p[4];
     conv_weights(p, a.conv_w + (2 * (int64_t)a.P + h * kDim + 2 * pair) * 4);
@@ -535,11 +537,11 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
       for (int j = 0; j < 3; ++j)
         held[j] = __ldg(reinterpret_cast<const uint32_t*>(cs + ((int64_t)(2 - j) * 3 + 2) * a.P + 2 * pair));
 #pragma unroll 1
-    for (int i = part; i < n; i += 16) {                       // 4 nodes at a time
-      uint32_t x[4][4];
+    for (int i = part; i < n; i += 2 * kGroups) {              // 2 nodes at a time
+      uint32_t x[2][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int m = min(i + 4 * j, n - 1);
+      for (int j = 0; j < 2; ++j) {
+        const int m = min(i + kGroups * j, n - 1);
         const uint32_t taps = sm.tap[m];
         x[j][3] = sm.vin[m][pair];
 #pragma unroll
@@ -553,9 +555,9 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
         }
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 2; ++j) {
         const float2 y = conv_silu(p, x[j]);
-        if (i + 4 * j < n) *reinterpret_cast<float2*>(&sm.v[i + 4 * j][2 * pair]) = y;
+        if (i + kGroups * j < n) *reinterpret_cast<float2*>(&sm.v[i + kGroups * j][2 * pair]) = y;
       }
     }
   }
@@ -563,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
   // ---- w = v - S (A k), as bf16 parts in the place of S; zeros past the nodes, whose columns of P are zeros too
   if (ok) {
 #pragma unroll 1
-    for (int c = kHalf * half; c < kHalf * (half + 1); c += 8) {
+    for (int c = kShare * fourth; c < min(kShare * (fourth + 1), N); c += 8) {
       float y[8], w[8];
       tmem_ld_x8(tmem + rows + kColD + c, y);
 #pragma unroll
@@ -599,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
     tc_fence_after();
     __nv_bfloat16* out = a.out + (int64_t)s * a.ldo + h * kDim + v;
 #pragma unroll 1
-    for (int c = kHalf * half; c < min(kHalf * (half + 1), n); c += 8) {
+    for (int c = kShare * fourth; c < min(kShare * (fourth + 1), n); c += 8) {
       float z[8];
       tmem_ld_x8(tmem + rows + kColD + N + c, z);
       tmem_ld_wait();
