@@ -11,8 +11,8 @@
 // the nodes, no node's own state is formed, and nothing but the scalars goes node after node. The decays multiply up the
 // path (each is at most 1; quotients of cumulated ones would overflow).
 //
-// One CTA a (request, head), 512 threads, two CTAs an SM:
-//   conv and gates: a thread a pair of channels of q and k (they share the taps' addresses) for every eighth node, then of g,
+// One CTA a (request, head), two or four an SM:
+//   conv and gates: a thread a pair of channels of q and k (they share the taps' addresses) for every fourth (eighth) node, then of g,
 //       late of v;
 //   norms, pairs, A k and A q: half a warp a node (8 channels a lane), its pairs 4 at a time;
 //   products: [S (A k) | S (A q)] on the tensor cores, M = 128 value rows, N = 2 nodes, K = 128 keys, tcgen05 kind::f16: S in
@@ -29,12 +29,23 @@ namespace ssb {
 namespace {
 
 constexpr int kDim = 128;
-constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kGroups = kThreads / 64;       // of 64 threads, one a pair of channels; the last one also looks after the tree
 constexpr int kMaxNodes = 64;
 constexpr float kLog2e = 1.4426950408889634f;
-// TMEM: S as 64 columns of high and 64 of low parts, later W^T in the same places; the products
-constexpr uint32_t kColS = 0, kColLo = 64, kColD = 128, kCols = 256;
+
+// How a CTA is made for trees of up to N nodes. Its phases are short and wait on one another (barriers, chains down the
+// tree, tensor core and memory latencies), so other CTAs have to fill the SM: up to 32 nodes four of 256 threads, which have
+// TMEM for half of the keys at a time; above, where shared memory holds two, 512 threads each.
+template <int N>
+struct Shape {
+  static constexpr int kThreads = N > 32 ? 512 : 256, kWarps = kThreads / 32, kBlocks = N > 32 ? 2 : 4;
+  static constexpr int kGroups = kThreads / 64;        // of 64 threads, one a pair of channels; the last looks after the tree
+  static constexpr int kParts = kThreads / 128;        // threads of a value row, 32 keys of S each
+  static constexpr int kPasses = 4 / kParts;           // over the keys
+  // TMEM: S of a pass, high and low parts, later W^T in the same places; [S (A k) | S (A q)]
+  static constexpr uint32_t kColS = 0, kColLo = 16 * kParts, kColD = 2 * kColLo, kCols = N > 32 ? 256 : 128;
+  static constexpr int kOwn = N > 2 * kWarps ? N / (2 * kWarps) : 1;                   // nodes of half a warp
+  static constexpr int kShare = N < 8 * kParts ? 8 : N / kParts;                       // nodes of a thread of a value row
+};
 
 template <int N>
 struct TreeSmem {
@@ -65,7 +76,7 @@ struct TreeSmem {
   uint32_t tap[N];                         // bytes: the rows before the node's in the conv, N + j: the j-th newest kept row
   uint16_t off[N + 2];
   int8_t parent[N];
-  uint64_t bar[2];
+  uint64_t bar[3];
   uint32_t tmem;
   int32_t abort;
 };
@@ -132,14 +143,16 @@ SSB_DEVICE float2 conv_silu(const uint64_t (&p)[4], const uint32_t (&x)[4]) {
   f2unpack(o, y.x, y.y);
   return make_float2(silu_short(y.x), silu_short(y.y));
 }
-SSB_DEVICE void conv_weights(uint64_t (&p)[4], const __nv_bfloat16* w) {             // 2 channels x 4 taps
-  const uint4 wv = __ldg(reinterpret_cast<const uint4*>(w));
+SSB_DEVICE void conv_weights(uint64_t (&p)[4], uint4 wv) {                           // 2 channels x 4 taps
   const float2 a0 = bf2(wv.x), a1 = bf2(wv.y), b0 = bf2(wv.z), b1 = bf2(wv.w);
   p[0] = f2pack(a0.x, b0.x), p[1] = f2pack(a0.y, b0.y), p[2] = f2pack(a1.x, b1.x), p[3] = f2pack(a1.y, b1.y);
 }
 
 template <int N>
-__global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_constant__ KdaArgs a) {
+__global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tree_kernel(const __grid_constant__ KdaArgs a) {
+  using C = Shape<N>;
+  constexpr int kWarps = C::kWarps, kGroups = C::kGroups, kParts = C::kParts, kOwn = C::kOwn, kShare = C::kShare;
+  constexpr uint32_t kColS = C::kColS, kColLo = C::kColLo, kColD = C::kColD, kCols = C::kCols;
   extern __shared__ __align__(1024) uint8_t raw_smem[];
   TreeSmem<N>& sm = *reinterpret_cast<TreeSmem<N>*>(raw_smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -156,24 +169,24 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
     tmem_alloc(smem_u32(&sm.tmem), kCols);
     tmem_relinquish();
     if (lane == 0) {
-      mbar_init(smem_u32(&sm.bar[0]), 1);
-      mbar_init(smem_u32(&sm.bar[1]), 1);
+      for (int j = 0; j < 3; ++j) mbar_init(smem_u32(&sm.bar[j]), 1);
       fence_barrier_init();
     }
   }
 
-  // ---- the state's loads: a value row a lane, a fourth of its keys a thread
+  // ---- the state's loads: a value row a lane, 32 keys of a pass a thread
   const int quarter = warp & 3, fourth = warp >> 2, v = 32 * quarter + lane;
+  const float* S = a.rec_state + (int64_t)sq.z * a.rs_stride + ((int64_t)h * kDim + v) * kDim + 32 * fourth;
   float st[32];
-  {
-    const float* S = a.rec_state + (int64_t)sq.z * a.rs_stride + ((int64_t)h * kDim + v) * kDim + 32 * fourth;
-    const bool wide = (reinterpret_cast<uintptr_t>(S) & 31) == 0;
+  const auto load_state = [&](int pass) {
+    const float* from = S + 32 * kParts * pass;
+    const bool wide = (reinterpret_cast<uintptr_t>(from) & 31) == 0;
 #pragma unroll
     for (int c = 0; c < 32; c += 8) {
       if (init && wide) {
-        ld8(S + c, st + c);
+        ld8(from + c, st + c);
       } else if (init) {
-        const float4 x = __ldg(reinterpret_cast<const float4*>(S + c)), y = __ldg(reinterpret_cast<const float4*>(S + c + 4));
+        const float4 x = __ldg(reinterpret_cast<const float4*>(from + c)), y = __ldg(reinterpret_cast<const float4*>(from + c + 4));
         st[c] = x.x, st[c + 1] = x.y, st[c + 2] = x.z, st[c + 3] = x.w;
         st[c + 4] = y.x, st[c + 5] = y.y, st[c + 6] = y.z, st[c + 7] = y.w;
       } else {
@@ -181,7 +194,9 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
         for (int j = 0; j < 8; ++j) st[c + j] = 0.0f;
       }
     }
-  }
+  };
+  load_state(0);
+  if (C::kPasses > 1 && init) asm volatile("prefetch.global.L2 [%0];" ::"l"(S + 32 * kParts));
   // ---- the inputs of q and k into shared memory; the tree (the last 64 threads)
   const int pair = tid & 63, part = tid >> 6;
   const __nv_bfloat16* cs = a.conv_state + (int64_t)sq.z * a.cs_stride + h * kDim;            // of q; k, v: + P, + 2 P
@@ -248,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
       }
     }
   }
-  // the gates' inputs: a pair of channels of every eighth node a thread
+  // the gates' inputs: a pair of channels of every kGroups-th node a thread
   uint32_t gin[N / kGroups];
   {
     const uint32_t* in = reinterpret_cast<const uint32_t*>(a.g + h * kDim + 2 * pair) + s * (a.ldg / 2);
@@ -256,6 +271,11 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
     for (int t = 0; t < N / kGroups; ++t)
       if (part + kGroups * t < n) gin[t] = __ldg(in + (part + kGroups * t) * (a.ldg / 2));
   }
+  // the conv's weights of q and k and the gates' parameters
+  const uint4 wq = __ldg(reinterpret_cast<const uint4*>(a.conv_w + ((int64_t)h * kDim + 2 * pair) * 4));
+  const uint4 wk = __ldg(reinterpret_cast<const uint4*>(a.conv_w + ((int64_t)a.P + h * kDim + 2 * pair) * 4));
+  const float2 dt = __ldg(reinterpret_cast<const float2*>(a.dt_bias + h * kDim) + pair);
+  const float a_log = __ldg(a.a_log + h);
   cp_async_wait();
   tc_fence_before();
   if (__syncthreads_or(bad)) {
@@ -267,24 +287,25 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
   tc_fence_after();
   const uint32_t tmem = sm.tmem;
   // ---- the state's parts to TMEM
-  {
-    const uint32_t at = tmem + (static_cast<uint32_t>(32 * quarter) << 16) + kColS + 16 * fourth;
+  const uint32_t rows = static_cast<uint32_t>(32 * quarter) << 16;
+  const auto store_state = [&] {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       uint32_t hi[4], lo[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) split2(st[8 * j + 2 * e], st[8 * j + 2 * e + 1], hi[e], lo[e]);
-      tmem_st_x4(at + 4 * j, hi);
-      tmem_st_x4(at + kColLo + 4 * j, lo);
+      tmem_st_x4(tmem + rows + kColS + 16 * fourth + 4 * j, hi);
+      tmem_st_x4(tmem + rows + kColS + kColLo + 16 * fourth + 4 * j, lo);
     }
     tmem_st_wait();
-  }
+  };
+  store_state();
 
-  // ---- the conv of q and k: every eighth node, 2 at a time
+  // ---- the conv of q and k: every kGroups-th node, 2 at a time
   {
     uint64_t pq[4], pk[4];
-    conv_weights(pq, a.conv_w + ((int64_t)h * kDim + 2 * pair) * 4);
-    conv_weights(pk, a.conv_w + ((int64_t)a.P + h * kDim + 2 * pair) * 4);
+    conv_weights(pq, wq);
+    conv_weights(pk, wk);
 #pragma unroll 1
     for (int i = part; i < n; i += 2 * kGroups) {
       uint32_t xq[2][4], xk[2][4];
@@ -312,8 +333,7 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
   __syncthreads();
   // ---- the decays, in the place of the inputs
   {
-    const float2 dt = __ldg(reinterpret_cast<const float2*>(a.dt_bias + h * kDim) + pair);
-    const float rate = -kLog2e * exp_fast(__ldg(a.a_log + h)), lb = a.lower_bound * kLog2e;
+    const float rate = -kLog2e * exp_fast(a_log), lb = a.lower_bound * kLog2e;
 #pragma unroll
     for (int t = 0; t < N / kGroups; ++t) {
       if (part + kGroups * t >= n) continue;
@@ -411,7 +431,6 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
   }
   // ---- A k and A q as the products' second operand, in the place of k and q; all the warp's paths walked at once
   {
-    constexpr int kOwn = N > 2 * kWarps ? N / (2 * kWarps) : 1;
     uint32_t hi[kOwn][8], lo[kOwn][8];                         // k, then q
     {
       ulonglong2 f[kOwn][2];
@@ -474,16 +493,16 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
   fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
-  const uint32_t bar = smem_u32(&sm.bar[0]);
-  if (tid == 0) {
+  const auto bar = [&](int i) { return smem_u32(&sm.bar[i]); };
+  const auto products = [&](int pass) {                        // of a pass's keys, by one thread
     tc_fence_after();
     constexpr uint32_t idesc = idesc_bf16(128, 2 * N);
-    uint32_t acc = 0;
+    uint32_t acc = pass;
 #pragma unroll 1
     for (int t = 0; t < 3; ++t) {                              // high x high, high x low, low x high
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint64_t bd = smem_desc(smem_u32(&sm.op[t == 1][c][0][0]), 0, 1024, 2);
+      for (int c = 0; c < kParts / 2; ++c) {                   // chunks of 64 keys
+        const uint64_t bd = smem_desc(smem_u32(&sm.op[t == 1][kParts / 2 * pass + c][0][0]), 0, 1024, 2);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
           mma_f16_ta(tmem + kColD, tmem + kColS + (t == 2 ? kColLo : 0) + 32 * c + 8 * ks, bd + 2 * ks, idesc, acc);
@@ -491,8 +510,9 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
         }
       }
     }
-    tc_commit(bar);
-  }
+    tc_commit(bar(pass));
+  };
+  if (tid == 0) products(0);
   // ---- meanwhile the values' inputs, and the scalars (node i's row of P by the i-th of the last 64 threads)
   {
     const uint32_t* in = reinterpret_cast<const uint32_t*>(a.x + 2 * (int64_t)a.P + h * kDim + 2 * pair);
@@ -500,6 +520,12 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
 #pragma unroll 4
     for (int i = part; i < n; i += kGroups) cp_async4(&sm.vin[i][pair], in + (s + i) * pitch);
   }
+  if (C::kPasses > 1) load_state(1);
+  const uint4 wv = __ldg(reinterpret_cast<const uint4*>(a.conv_w + (2 * (int64_t)a.P + h * kDim + 2 * pair) * 4));
+  uint32_t held[3] = {0, 0, 0};                                // the values' kept rows, the newest first
+  if (init)
+    for (int j = 0; j < 3; ++j)
+      held[j] = __ldg(reinterpret_cast<const uint32_t*>(cs + ((int64_t)(2 - j) * 3 + 2) * a.P + 2 * pair));
   if (part == kGroups - 1 && pair < N) {
     const int i = pair;
 #pragma unroll
@@ -522,20 +548,23 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
     }
   }
   cp_async_wait();
-  bool ok = mbar_wait(bar, 0, &sm.abort, a.status);
+  bool ok = mbar_wait(bar(0), 0, &sm.abort, a.status);
+  if (C::kPasses > 1) {                                        // the other half of the keys
+    ok = !__syncthreads_or(!ok);
+    tc_fence_after();
+    if (ok) store_state();
+    tc_fence_before();
+    __syncthreads();
+    if (ok && tid == 0) products(1);
+    if (ok) ok = mbar_wait(bar(1), 0, &sm.abort, a.status);
+  }
   fence_proxy_async_smem();
   ok = !__syncthreads_or(!ok);
   tc_fence_after();
-  const uint32_t rows = static_cast<uint32_t>(32 * quarter) << 16;
-  constexpr int kShare = N < 32 ? 8 : N / 4;                   // nodes of its value row that a thread has
-  // ---- the values, in the place of the products' second operand: a pair of channels of every eighth node a thread
+  // ---- the values, in the place of the products' second operand: a pair of channels of every kGroups-th node a thread
   {
     uint64_t p[4];
-    conv_weights(p, a.conv_w + (2 * (int64_t)a.P + h * kDim + 2 * pair) * 4);
-    uint32_t held[3] = {0, 0, 0};
-    if (init)
-      for (int j = 0; j < 3; ++j)
-        held[j] = __ldg(reinterpret_cast<const uint32_t*>(cs + ((int64_t)(2 - j) * 3 + 2) * a.P + 2 * pair));
+    conv_weights(p, wv);
 #pragma unroll 1
     for (int i = part; i < n; i += 2 * kGroups) {              // 2 nodes at a time
       uint32_t x[2][4];
@@ -583,7 +612,6 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
   }
   tc_fence_before();
   __syncthreads();
-  const uint32_t bar2 = smem_u32(&sm.bar[1]);
   if (ok && tid == 0) {
     tc_fence_after();
     constexpr uint32_t idesc = idesc_bf16(128, N);
@@ -594,9 +622,9 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
       for (int ks = 0; ks < N / 16; ++ks)
         mma_f16_ta(tmem + kColD + N, tmem + kColS + (t == 2 ? kColLo : 0) + 8 * ks, bd + 2 * ks, idesc, 1u);
     }
-    tc_commit(bar2);
+    tc_commit(bar(2));
   }
-  if (ok) ok = mbar_wait(bar2, 0, &sm.abort, a.status);
+  if (ok) ok = mbar_wait(bar(2), 0, &sm.abort, a.status);
   if (!__syncthreads_or(!ok)) {
     tc_fence_after();
     __nv_bfloat16* out = a.out + (int64_t)s * a.ldo + h * kDim + v;
@@ -612,7 +640,8 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
   } else {
     // products may still be on their way
     const unsigned long long t0 = globaltimer();
-    while (!(mbar_try_wait(bar, 0) && mbar_try_wait(bar2, 0)) && globaltimer() - t0 <= 2 * kWaitNs) {}
+    while (!(mbar_try_wait(bar(0), 0) && (C::kPasses == 1 || mbar_try_wait(bar(1), 0)) && mbar_try_wait(bar(2), 0)) &&
+           globaltimer() - t0 <= 2 * kWaitNs) {}
   }
   tc_fence_before();
   __syncthreads();
@@ -622,11 +651,13 @@ __global__ void __launch_bounds__(kThreads, 2) kda_tree_kernel(const __grid_cons
   }
 }
 
-// TMEM holds two CTAs' columns: shared memory of which three do not fit an SM keeps a third from waiting for them.
+// TMEM has columns for Shape<N>::kBlocks CTAs: shared memory of which one more does not fit an SM (228 KB, 1 KB of it for
+// each) keeps it from waiting for them.
 template <int N>
 constexpr int smem_bytes() {
-  static_assert(sizeof(TreeSmem<N>) <= 115712, "two CTAs an SM");
-  return sizeof(TreeSmem<N>) > 80 * 1024 ? sizeof(TreeSmem<N>) : 80 * 1024;
+  constexpr int most = 228 * 1024 / Shape<N>::kBlocks - 1024, least = 228 * 1024 / (Shape<N>::kBlocks + 1);
+  static_assert(sizeof(TreeSmem<N>) <= most, "shared memory");
+  return sizeof(TreeSmem<N>) > least ? sizeof(TreeSmem<N>) : least;
 }
 
 template <int N>
@@ -638,7 +669,7 @@ int launch_nodes(const KdaArgs& a, cudaStream_t stream) {
            cudaSuccess;
   };
   if (cudaGetDevice(&device) != cudaSuccess || !attr.done(device, set)) return kErrCuda;
-  kda_tree_kernel<N><<<(unsigned)(a.R * a.H), kThreads, smem_bytes<N>(), stream>>>(a);
+  kda_tree_kernel<N><<<(unsigned)(a.R * a.H), Shape<N>::kThreads, smem_bytes<N>(), stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
 }
 
