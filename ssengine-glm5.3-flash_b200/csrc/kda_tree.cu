@@ -14,7 +14,7 @@
 // One CTA a (request, head), two or four an SM:
 //   conv and gates: a thread a pair of channels of q and k (they share the taps' addresses) for every fourth (eighth) node, then of g,
 //       late of v;
-//   norms, pairs, A k and A q: half a warp a node (8 channels a lane), its pairs 4 at a time;
+//   norms, pairs, A k and A q: half a warp a node (8 channels a lane), its pairs 2 at a time;
 //   products: [S (A k) | S (A q)] on the tensor cores, M = 128 value rows, N = 2 nodes, K = 128 keys, tcgen05 kind::f16: S in
 //       TMEM and the vectors in shared memory, both as two bf16 parts, three of the four products (what is left out is below
 //       2^-16 of a product; the output has 8 bits). S comes straight from global memory, a value row a lane;
@@ -383,97 +383,88 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
     }
   }
   __syncthreads();
-  // ---- the pairs of a node and those above it, 4 at a time
-#pragma unroll 1
-  for (int i0 = 2 * warp; i0 < n; i0 += 2 * kWarps) {
-    const int i = i0 + (lane >> 4);
-    ulonglong2 q[2], k[2], f[2] = {ones, ones};                // f: the decays below
+  // ---- the pairs of a node and those above it, 2 at a time; A q in the place of q
+  ulonglong2 f[kOwn][2];                                       // the decays below, at the end of the path A
+  uint32_t nodes[kOwn];                                        // the path: distances l + 16 c in byte c
+#pragma unroll
+  for (int t = 0; t < kOwn; ++t) {
+    nodes[t] = 0;
+    if (2 * warp + 2 * kWarps * t >= n) continue;
+    const int i = first + 2 * kWarps * t;
+    ulonglong2 q[2], k[2];
+    f[t][0] = f[t][1] = ones;
     const int im = min(i, n - 1);
     load8(sm.q[im], q);
     load8(sm.k[im], k);
     const int at = sm.off[im], len = sm.off[im + 1] - at;
     const int most = max(len, __shfl_xor_sync(0xffffffffu, len, 16));
     const uint8_t* path = reinterpret_cast<const uint8_t*>(sm.pn + at) + 3 * len;
+    for (int c = 0; 16 * c < most; ++c) nodes[t] |= static_cast<uint32_t>(path[min(16 * c + l, len - 1)] & (N - 1)) << (8 * c);
+    __syncwarp();                                              // the path's bytes are read
 #pragma unroll 1
-    for (int d = 0; d < most; d += 4) {
-      int js[4];
+    for (int d = 0; d < most; d += 2) {
+      float x[4];                                              // M of 2 pairs, N of 2 pairs
+      const uint32_t word = nodes[t] >> (8 * (d >> 4));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) js[e] = path[min(d + e, len - 1)];
-      float t[8];                                              // M of 4 pairs, N of 4 pairs
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        ulonglong2 x[2], dj[2];
-        load8(sm.k[js[e] & (N - 1)], x);
-        load8(sm.dec[js[e] & (N - 1)], dj);
-        mul8(x, f);
-        t[e] = dot8(x, k);
-        t[4 + e] = dot8(x, q);
-        mul8(f, dj);
+      for (int e = 0; e < 2; ++e) {
+        const int j = __shfl_sync(0xffffffffu, word, (d + e) & 15, 16) & 0xFF;
+        ulonglong2 kj[2], dj[2];
+        load8(sm.k[j], kj);
+        load8(sm.dec[j], dj);
+        mul8(kj, f[t]);
+        x[e] = dot8(kj, k);
+        x[2 + e] = dot8(kj, q);
+        if (d + e < len) mul8(f[t], dj);
       }
 #pragma unroll
-      for (int o = 8, m = 4; m > 0; o >>= 1, m >>= 1) {        // lanes l = 2 x, 2 x + 1 receive value x
+      for (int o = 8, m = 2; m > 0; o >>= 1, m >>= 1) {        // lanes l = 4 c .. + 3 receive value c
         const bool up = l & o;
 #pragma unroll
         for (int e = 0; e < m; ++e) {
-          const float keep = up ? t[e + m] : t[e], send = up ? t[e] : t[e + m];
-          t[e] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+          const float keep = up ? x[e + m] : x[e], send = up ? x[e] : x[e + m];
+          x[e] = keep + __shfl_xor_sync(0xffffffffu, send, o);
         }
       }
-      t[0] += __shfl_xor_sync(0xffffffffu, t[0], 1);
-      __syncwarp();                                            // the path's bytes are read
-      const int e = d + ((l >> 1) & 3);
-      if ((l & 1) == 0 && e < len && i < n) {
-        if (l >= 8) sm.pn[at + e] = t[0];
-        else if (e > 0) sm.pm[at - i + e - 1] = t[0];
+      x[0] += __shfl_xor_sync(0xffffffffu, x[0], 2);
+      x[0] += __shfl_xor_sync(0xffffffffu, x[0], 1);
+      const int e = d + ((l >> 2) & 1);
+      if ((l & 3) == 0 && e < len && i < n) {
+        if (l >= 8) sm.pn[at + e] = x[0];
+        else if (e > 0) sm.pm[at - i + e - 1] = x[0];
       }
-      __syncwarp();
+    }
+    if (i < n) {
+      mul8(q, f[t]);
+      *reinterpret_cast<ulonglong2*>(&sm.q[i][4 * l]) = q[0], *reinterpret_cast<ulonglong2*>(&sm.q[i][64 + 4 * l]) = q[1];
     }
   }
-  // ---- A k and A q as the products' second operand, in the place of k and q; all the warp's paths walked at once
+  // ---- A k and A q as the products' second operand, in the place of k and q
   {
     uint32_t hi[kOwn][8], lo[kOwn][8];                         // k, then q
-    {
-      ulonglong2 f[kOwn][2];
-      int at[kOwn];
 #pragma unroll
-      for (int t = 0; t < kOwn; ++t) {
-        f[t][0] = f[t][1] = ones;
-        at[t] = first + 2 * kWarps * t < n ? first + 2 * kWarps * t : -1;
-      }
-#pragma unroll 1
-      while (true) {
-        bool more = false;
+    for (int t = 0; t < kOwn; ++t) {
+      if (2 * warp + 2 * kWarps * t >= n) continue;
+      const int i = min(first + 2 * kWarps * t, n - 1);
+      ulonglong2 x[2];
 #pragma unroll
-        for (int t = 0; t < kOwn; ++t) {
-          if (at[t] < 0) continue;
-          ulonglong2 d[2];
-          load8(sm.dec[at[t]], d);
-          mul8(f[t], d);
-          at[t] = sm.parent[at[t]];
-          more = true;
-        }
-        if (!__any_sync(0xffffffffu, more)) break;
-      }
+      for (int e = 0; e < 2; ++e) {
+        load8(e ? sm.q[i] : sm.k[i], x);
+        if (e == 0) mul8(x, f[t]);
+        const uint64_t y[4] = {x[0].x, x[0].y, x[1].x, x[1].y};
 #pragma unroll
-      for (int t = 0; t < kOwn; ++t) {
-        if (2 * warp + 2 * kWarps * t >= n) continue;
-        const int i = min(first + 2 * kWarps * t, n - 1);
-        ulonglong2 x[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          load8(e ? sm.q[i] : sm.k[i], x);
-          mul8(x, f[t]);
-          const uint64_t y[4] = {x[0].x, x[0].y, x[1].x, x[1].y};
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            float y0, y1;
-            f2unpack(y[c], y0, y1);
-            split2(y0, y1, hi[t][4 * e + c], lo[t][4 * e + c]);
-          }
+        for (int c = 0; c < 4; ++c) {
+          float y0, y1;
+          f2unpack(y[c], y0, y1);
+          split2(y0, y1, hi[t][4 * e + c], lo[t][4 * e + c]);
         }
       }
     }
     __syncthreads();
+    // the decays' place is free: P's zeros, the values' inputs
+    for (int c = tid; c < 2 * N * 128 / 16; c += C::kThreads) reinterpret_cast<uint4*>(sm.p)[c] = make_uint4(0, 0, 0, 0);
+    const uint32_t* in = reinterpret_cast<const uint32_t*>(a.x + 2 * (int64_t)a.P + h * kDim + 2 * pair) + s * (a.ldx / 2);
+#pragma unroll 4
+    for (int i = part; i < n; i += kGroups) cp_async4(&sm.vin[i][pair], in + i * (a.ldx / 2));
     const int granule = l >> 1, within = (l & 1) * 8;
 #pragma unroll
     for (int t = 0; t < kOwn; ++t) {
@@ -513,38 +504,53 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
     tc_commit(bar(pass));
   };
   if (tid == 0) products(0);
-  // ---- meanwhile the values' inputs, and the scalars (node i's row of P by the i-th of the last 64 threads)
-  {
-    const uint32_t* in = reinterpret_cast<const uint32_t*>(a.x + 2 * (int64_t)a.P + h * kDim + 2 * pair);
-    const int64_t pitch = a.ldx / 2;
-#pragma unroll 4
-    for (int i = part; i < n; i += kGroups) cp_async4(&sm.vin[i][pair], in + (s + i) * pitch);
-  }
+  // ---- meanwhile the rest of the inputs, and the scalars
   if (C::kPasses > 1) load_state(1);
   const uint4 wv = __ldg(reinterpret_cast<const uint4*>(a.conv_w + (2 * (int64_t)a.P + h * kDim + 2 * pair) * 4));
   uint32_t held[3] = {0, 0, 0};                                // the values' kept rows, the newest first
   if (init)
     for (int j = 0; j < 3; ++j)
       held[j] = __ldg(reinterpret_cast<const uint32_t*>(cs + ((int64_t)(2 - j) * 3 + 2) * a.P + 2 * pair));
-  if (part == kGroups - 1 && pair < N) {
-    const int i = pair;
+  // P_i of half a warp's node: lanes hold the distances l + 16 c; the nodes on the path from i up subtract their share from
+  // those above them
 #pragma unroll
-    for (int c = 0; c < 128; c += 16)
-      *reinterpret_cast<uint4*>(&sm.p[0][i][c]) = *reinterpret_cast<uint4*>(&sm.p[1][i][c]) = make_uint4(0, 0, 0, 0);
-    const int at = i < n ? sm.off[i] : 0, len = i < n ? sm.off[i + 1] - at : 0;
-    float* pn = sm.pn + at;
-    int m = i;
-#pragma unroll 1
-    for (int c = 0; c < len; ++c) {
-      const float y = pn[c] * sm.beta[m];
-      const float* pm = sm.pm + (sm.off[m] - m);
-#pragma unroll 4
-      for (int e = c + 1; e < len; ++e) pn[e] = fmaf(-y, pm[e - c - 1], pn[e]);
+  for (int t = 0; t < kOwn; ++t) {
+    if (2 * warp + 2 * kWarps * t >= n) continue;
+    const int i = first + 2 * kWarps * t, im = min(i, n - 1);
+    const int at = sm.off[im], len = i < n ? sm.off[im + 1] - at : 0;
+    const int most = max(len, __shfl_xor_sync(0xffffffffu, len, 16));
+    constexpr int kWords = N / 16;
+    float x[kWords], b[kWords];
+    int base[kWords];                                          // of the node's M
+#pragma unroll
+    for (int c = 0; c < kWords; ++c) {
+      const int m = (nodes[t] >> (8 * c)) & 0xFF;
+      const bool have = 16 * c + l < len;
+      x[c] = have ? sm.pn[at + 16 * c + l] : 0.0f;
+      b[c] = have ? sm.beta[m] : 0.0f;
+      base[c] = sm.off[m] - m;
+    }
+#pragma unroll
+    for (int c = 0; c < kWords; ++c) {
+      if (16 * c >= most) break;
+#pragma unroll 2
+      for (int d = 0; d < min(most - 16 * c, 16); ++d) {
+        const float y = __shfl_sync(0xffffffffu, x[c] * b[c], d, 16);
+        const float* pm = sm.pm + __shfl_sync(0xffffffffu, base[c], d, 16) + l - d - 1;
+#pragma unroll
+        for (int e = c; e < kWords; ++e)
+          if (16 * e + l > 16 * c + d && 16 * e + l < len) x[e] = fmaf(-y, pm[16 * (e - c)], x[e]);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < kWords; ++c) {
+      if (16 * c + l >= len) break;
+      const int m = (nodes[t] >> (8 * c)) & 0xFF;
+      const float y = x[c] * b[c];
       const __nv_bfloat16 y_hi = __float2bfloat16(y);
       const int to = (((m >> 3) ^ (i & 7)) << 4) + 2 * (m & 7);
       *reinterpret_cast<__nv_bfloat16*>(&sm.p[0][i][to]) = y_hi;
       *reinterpret_cast<__nv_bfloat16*>(&sm.p[1][i][to]) = __float2bfloat16(y - __bfloat162float(y_hi));
-      m = sm.parent[m];
     }
   }
   cp_async_wait();
