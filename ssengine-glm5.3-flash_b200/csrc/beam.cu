@@ -2,13 +2,15 @@
 //   score[b] + x[b, v] - log sum_v exp x[b, v]
 // in order, equal ones by the lower b V + v. One pass over the logits.
 //
-// scan: a CTA has one part of one beam's row; each warp keeps the running maximum and sum of exponentials and the k largest
-//   (logit, token) it has seen, as 64-bit keys whose order is that of the candidates (equal logits: the lower token is
-//   larger). A logit below the warp's k-th key costs one comparison; those above it go to the warp's list in shared memory,
-//   which is cut back to its k largest when it is full. The CTA leaves k keys, the maximum and the sum.
-// join: a CTA a request: the rows' log sums in 64 bits, then every candidate's score in 64 bits (a beam's own candidates
-//   keep the order of their logits, those of different beams are compared at the sums' accuracy). The candidates at or above
-//   the best part's k-th go to shared memory and each finds its place by counting those before it.
+// scan: a CTA has one part of one beam's row, 16 bytes a load. Each warp keeps a sum of exponentials against a reference (a
+//   logit it has seen; it moves only when one exceeds it by 40, where a running maximum would be rescaled all the time) and
+//   the k largest (logit, token) as 64-bit keys whose order is that of the candidates (equal logits: the lower token is
+//   larger). The largest logit of a load is compared with the warp's k-th; what is above goes to the warp's list in shared
+//   memory, which is cut back to its k largest when it is full. The first k-th is that of the lanes' maxima over their first
+//   loads. The CTA leaves k keys, the reference and the sum.
+// join: a CTA a request: the rows' log sums, then every candidate's score in 64 bits (a beam's own candidates keep the order
+//   of their logits, those of different beams are compared at the sums' accuracy). The candidates at or above the best
+//   part's k-th go to shared memory and each finds its place by counting those before it.
 // Bound: HBM, a read of the logits.
 #include "common.cuh"
 #include "ops.h"
@@ -17,8 +19,10 @@ namespace ssb {
 namespace {
 
 constexpr int kScanWarps = 8, kScanThreads = 32 * kScanWarps;
-constexpr int kList = 512;                       // keys a warp holds between cuts
-constexpr int kJoinThreads = 1024;
+constexpr int kList = 256;                       // keys a warp holds between cuts
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRise = 40.0f;                   // above the reference before it moves: e^40 times 2^31 terms stay finite
+constexpr int kJoinThreads = 512;
 constexpr int kMaxK = 64, kMaxBeams = 64;
 constexpr int kMaxCandidates = 8192;             // of a request, all parts together
 constexpr int kMinPart = 2048;                   // logits a part has at least
@@ -35,57 +39,61 @@ SSB_DEVICE float key_logit(uint64_t key) {
 }
 SSB_DEVICE uint32_t key_token(uint64_t key) { return 0xFFFFFFFFu - static_cast<uint32_t>(key); }
 
+// The largest of the lanes' keys.
 SSB_DEVICE uint64_t warp_max(uint64_t v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const uint64_t w = __shfl_xor_sync(0xffffffffu, v, o);
-    v = w > v ? w : v;
-  }
-  return v;
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(v >> 32));
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(v >> 32) == hi ? static_cast<uint32_t>(v) : 0u);
+  return static_cast<uint64_t>(hi) << 32 | lo;
 }
-
+SSB_DEVICE float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+SSB_DEVICE uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 // e^d, d <= 0: 2^(d log2 e) with the product's rounding error carried to first order (ex2.approx's 2^-22 remains).
 SSB_DEVICE float exp_neg(float d) {
   constexpr float kHi = 1.44269502162933349609375f, kLo = 1.925963033500928e-8f;        // log2 e in two parts
   const float t = d * kHi;
   const float r = fmaf(d, kLo, fmaf(d, kHi, -t));
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t));
+  const float y = ex2(t);
   return fmaf(y, fminf(fmaxf(r, -1.0f), 1.0f) * 0.6931471805599453f, y);
 }
 
-// The k largest of `count` keys of a list to its front, in order (one warp; keys are distinct). Returns how many.
-SSB_DEVICE int cut_list(uint64_t* list, int count, int k, int lane) {
-  uint64_t mine[kList / 32];
-#pragma unroll
-  for (int j = 0; j < kList / 32; ++j) mine[j] = 32 * j + lane < count ? list[32 * j + lane] : 0;
-  __syncwarp();
-  const int keep = min(k, count);
-  for (int i = 0; i < keep; ++i) {
+// The k largest of the keys that the lanes hold (R each, 0: none; distinct) to out, in order; how many there are.
+template <int R>
+SSB_DEVICE int take_largest(uint64_t (&mine)[R], uint64_t* out, int k, int lane) {
+  int n = 0;
+  for (; n < k; ++n) {
     uint64_t top = 0;
 #pragma unroll
-    for (int j = 0; j < kList / 32; ++j) top = mine[j] > top ? mine[j] : top;
+    for (int j = 0; j < R; ++j) top = mine[j] > top ? mine[j] : top;
     top = warp_max(top);
+    if (top == 0) break;
 #pragma unroll
-    for (int j = 0; j < kList / 32; ++j)
+    for (int j = 0; j < R; ++j)
       if (mine[j] == top) mine[j] = 0;
-    if (lane == 0) list[i] = top;
+    if (lane == 0) out[n] = top;
   }
   __syncwarp();
-  return keep;
+  return n;
 }
 
-// Adds the lanes' keys that are above `least` (k-th of the list, 0 while it is short) to the list.
+// A warp's candidates.
 struct WarpList {
   uint64_t* list;
   int count, k;
-  uint64_t least;
-  float bar;                                     // a logit below it is below `least`
+  uint64_t least;                                // the k-th largest, 0 while it is not known
+  float bar;                                     // a logit below it is not among the k largest
   SSB_DEVICE void add(float x, uint32_t token, int lane) {
-    const bool maybe = x >= bar;                 // false for NaN
-    if (!__any_sync(0xffffffffu, maybe)) return;
-    const uint64_t key = maybe && x > -INFINITY ? make_key(x, token) : 0;
-    const bool in = key > least;
+    bool in = x >= bar && x > -INFINITY;         // false for NaN
+    if (!__any_sync(0xffffffffu, in)) return;
+    const uint64_t key = make_key(x, token);
+    in = in && key > least;
     const uint32_t mask = __ballot_sync(0xffffffffu, in);
     if (mask == 0) return;
     if (count + 32 > kList) cut(lane);
@@ -94,7 +102,19 @@ struct WarpList {
     __syncwarp();
   }
   SSB_DEVICE void cut(int lane) {
-    count = cut_list(list, count, k, lane);
+    if (count <= 64) {
+      uint64_t mine[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) mine[j] = 32 * j + lane < count ? list[32 * j + lane] : 0;
+      __syncwarp();
+      count = take_largest(mine, list, k, lane);
+    } else {
+      uint64_t mine[kList / 32];
+#pragma unroll
+      for (int j = 0; j < kList / 32; ++j) mine[j] = 32 * j + lane < count ? list[32 * j + lane] : 0;
+      __syncwarp();
+      count = take_largest(mine, list, k, lane);
+    }
     if (count == k) {
       least = list[k - 1];
       bar = key_logit(least);
@@ -103,11 +123,15 @@ struct WarpList {
   }
 };
 
-template <bool kBf16>
-__global__ void __launch_bounds__(kScanThreads) beam_scan_kernel(const __grid_constant__ BeamArgs a) {
+// kSkewed: rows may begin anywhere in a 16-byte piece of memory. A lane's values are the same ones of a row then too, put
+// together from two pieces: equal rows get the same sums wherever they lie, and equal candidates stay equal.
+template <bool kBf16, bool kSkewed>
+__global__ void __launch_bounds__(kScanThreads, 5) beam_scan_kernel(const __grid_constant__ BeamArgs a) {
+  constexpr int kVec = kBf16 ? 8 : 4, kBytes = 16 / kVec;
+  constexpr int kLoads = kSkewed ? 2 : 4;                    // 16-byte loads a lane has on their way
   __shared__ uint64_t lists[kScanWarps][kList];
   __shared__ float wm[kScanWarps];
-  __shared__ double ws[kScanWarps];
+  __shared__ float ws[kScanWarps];
   __shared__ int32_t wn[kScanWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t row = blockIdx.x / a.parts;
@@ -115,59 +139,144 @@ __global__ void __launch_bounds__(kScanThreads) beam_scan_kernel(const __grid_co
   asm volatile("griddepcontrol.launch_dependents;");
   const float score = a.scores[row];
   if (!(fabsf(score) < INFINITY) || (a.finished != nullptr && a.finished[row])) return;
-  const int64_t begin = a.V * part / a.parts, end = a.V * (part + 1) / a.parts;
-  const float* xf = static_cast<const float*>(a.x) + (kBf16 ? 0 : row * a.ldx);
-  const __nv_bfloat16* xb = static_cast<const __nv_bfloat16*>(a.x) + (kBf16 ? row * a.ldx : 0);
-  WarpList L = {lists[warp], 0, a.k, 0, -INFINITY};
-  float m = -INFINITY, s = 0.0f;
-  for (int64_t i0 = begin + 32 * warp; i0 < end; i0 += kScanThreads) {
-    const int64_t i = i0 + lane;
-    float x = -INFINITY;
-    if (i < end) x = kBf16 ? __bfloat162float(xb[i]) : xf[i];
-    if (x > m) {
-      s *= m > -INFINITY ? exp_neg(m - x) : 0.0f;
-      m = x;
+  // the row in vectors of 16 bytes
+  const char* p = static_cast<const char*>(a.x) + row * a.ldx * kBytes;
+  const int64_t vectors = (a.V + kVec - 1) / kVec;
+  const int64_t begin = vectors * part / a.parts, end = vectors * (part + 1) / a.parts;
+  const int skew = kSkewed ? static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15) : 0;      // bytes
+  const uint4* pieces = reinterpret_cast<const uint4*>(p - skew);
+  const int64_t whole0 = skew > 0, whole1 = kSkewed ? (a.V * kBytes + skew) / 16 - 1 : a.V / kVec;   // whose pieces are the row's
+  const auto load = [&](int64_t i) {                         // -inf where it is not the row's
+    if (i >= whole0 && i < whole1 && i < end) {
+      if (!kSkewed) return __ldcs(pieces + i);
+      const uint4 q0 = __ldg(pieces + i), q1 = __ldg(pieces + i + 1);
+      uint32_t w[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
+#pragma unroll
+      for (int j = 0; j < 6; ++j) w[j] = skew & 8 ? w[j + 2] : w[j];
+#pragma unroll
+      for (int j = 0; j < 5; ++j) w[j] = skew & 4 ? w[j + 1] : w[j];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = __funnelshift_r(w[j], w[j + 1], 8 * (skew & 2));
+      return make_uint4(w[0], w[1], w[2], w[3]);
     }
-    if (x > -INFINITY || x != x) s += exp_neg(x - m);   // a NaN, or an infinite maximum, makes the sum NaN
-    L.add(x, static_cast<uint32_t>(i), lane);
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      const int64_t e = i * kVec + j;
+      const bool in = i < end && e < a.V;
+      if (kBf16) {
+        const uint32_t v = in ? reinterpret_cast<const uint16_t*>(p)[e] : 0xFF80u;
+        w[j / 2] = j % 2 ? w[j / 2] | v << 16 : v;
+      } else {
+        w[j] = in ? reinterpret_cast<const uint32_t*>(p)[e] : 0xFF800000u;
+      }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  };
+  const auto values = [](uint4 q, float (&x)[kVec]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (kBf16) x[2 * j] = __uint_as_float(w[j] << 16), x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+      else x[j] = __uint_as_float(w[j]);
+    }
+  };
+  const auto largest = [](uint4 q) {                         // NaN is passed over (unless all are)
+    if (!kBf16)
+      return fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)), fmaxf(__uint_as_float(q.z), __uint_as_float(q.w)));
+    const auto b2 = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+    const __nv_bfloat162 m = __hmax2(__hmax2(b2(q.x), b2(q.y)), __hmax2(b2(q.z), b2(q.w)));
+    return fmaxf(__low2float(m), __high2float(m));
+  };
+  WarpList L = {lists[warp], 0, a.k, 0, -INFINITY};
+  float ref = -INFINITY;                                     // the same in all lanes
+  uint64_t neg = 0, sum = 0;                                 // -ref (0 while there is none) and the sum, as pairs
+  bool first = true;
+#pragma unroll 1
+  for (int64_t i0 = begin + 32 * warp; i0 < end; i0 += kLoads * kScanThreads) {
+    uint4 q[kLoads];
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) q[u] = load(i0 + u * kScanThreads + lane);
+    if (first) {                                             // at least k logits are as large as the k-th lane's maximum
+      first = false;
+      float most = largest(q[0]);
+#pragma unroll
+      for (int u = 1; u < kLoads; ++u) most = fmaxf(most, largest(q[u]));
+      uint64_t mine[1] = {most > -INFINITY ? make_key(most, lane) : 0};
+      const int n = take_largest(mine, L.list, min(a.k, 32), lane);
+      if (n > 0) ref = key_logit(L.list[0]), neg = f2pack(-ref, -ref);
+      if (n == a.k) L.bar = key_logit(L.list[n - 1]);
+      __syncwarp();
+    }
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      float x[kVec];
+      values(q[u], x);
+      const float top = largest(q[u]);
+      if (__any_sync(0xffffffffu, top >= L.bar)) {
+        if (__any_sync(0xffffffffu, top > ref + kRise || ref == -INFINITY)) {
+          float now = top == top ? top : -INFINITY;
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
+          if (now > ref) {
+            const float f = ref > -INFINITY ? ex2((ref - now) * kLog2e) : 0.0f;
+            sum = mul2(sum, f2pack(f, f));
+            ref = now;
+            neg = f2pack(-ref, -ref);
+          }
+        }
+        const int64_t at = (i0 + u * kScanThreads + lane) * kVec;
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) L.add(x[j], static_cast<uint32_t>(at + j), lane);
+      }
+      const uint64_t scale = f2pack(kLog2e, kLog2e);
+#pragma unroll
+      for (int j = 0; j < kVec; j += 2) {
+        float t0, t1;
+        f2unpack(mul2(add2(f2pack(x[j], x[j + 1]), neg), scale), t0, t1);
+        sum = add2(sum, f2pack(ex2(t0), ex2(t1)));           // NaN for a NaN, or an infinite reference
+      }
+    }
   }
   L.cut(lane);
-  // the CTA's maximum and sum, then its k largest
-  float top = m;
+  // the CTA's reference and sum, then its k largest
+  float s0, s1;
+  f2unpack(sum, s0, s1);
+  s0 += s1;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  double sum = m > -INFINITY || s != s ? static_cast<double>(s) * exp(static_cast<double>(m) - top) : 0.0;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) wm[warp] = top, ws[warp] = sum, wn[warp] = L.count;
+  for (int o = 16; o > 0; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+  if (lane == 0) wm[warp] = ref, ws[warp] = s0, wn[warp] = L.count;
   __syncthreads();
   if (warp != 0) return;
-  if (lane == 0) {
-    float t = -INFINITY;
-    for (int w = 0; w < kScanWarps; ++w) t = fmaxf(t, wm[w]);
-    double z = 0.0;
-    for (int w = 0; w < kScanWarps; ++w)
-      if (wm[w] > -INFINITY || ws[w] != ws[w]) z += ws[w] * exp(static_cast<double>(wm[w]) - t);
-    BeamPart& p = a.part[row * a.parts + part];
-    p.m = t, p.sum = z;
-  }
-  uint64_t mine[kScanWarps * kMaxK / 32];
+  const float m = lane < kScanWarps ? wm[lane] : -INFINITY;
+  float t = m;
 #pragma unroll
-  for (int j = 0; j < kScanWarps * kMaxK / 32; ++j) {
-    const int i = 32 * j + lane, w = i / kMaxK, e = i % kMaxK;
-    mine[j] = e < wn[w] ? lists[w][e] : 0;
-  }
+  for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+  const float z = lane < kScanWarps ? ws[lane] : 0.0f;
+  float part_sum = m > -INFINITY ? z * exp_neg(m - t) : z;   // without a reference the sum is 0, or NaN
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) part_sum += __shfl_xor_sync(0xffffffffu, part_sum, o);
+  if (lane == 0) a.part[row * a.parts + part] = {part_sum, t};
   uint64_t* out = a.keys + (row * a.parts + part) * a.k;
-  for (int i = 0; i < a.k; ++i) {
-    uint64_t best = 0;
+  int n = 0;
+  if (a.k <= 8) {
+    uint64_t mine[kScanWarps * 8 / 32];
 #pragma unroll
-    for (int j = 0; j < kScanWarps * kMaxK / 32; ++j) best = mine[j] > best ? mine[j] : best;
-    best = warp_max(best);
+    for (int j = 0; j < kScanWarps * 8 / 32; ++j) {
+      const int i = 32 * j + lane, w = i / 8, e = i % 8;
+      mine[j] = e < wn[w] ? lists[w][e] : 0;
+    }
+    n = take_largest(mine, out, a.k, lane);
+  } else {
+    uint64_t mine[kScanWarps * kMaxK / 32];
 #pragma unroll
-    for (int j = 0; j < kScanWarps * kMaxK / 32; ++j)
-      if (mine[j] == best) mine[j] = 0;
-    if (lane == 0) out[i] = best;
+    for (int j = 0; j < kScanWarps * kMaxK / 32; ++j) {
+      const int i = 32 * j + lane, w = i / kMaxK, e = i % kMaxK;
+      mine[j] = e < wn[w] ? lists[w][e] : 0;
+    }
+    n = take_largest(mine, out, a.k, lane);
   }
+  for (int i = n + lane; i < a.k; i += 32) out[i] = 0;
 }
 
 struct Candidate {
@@ -201,7 +310,7 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
       double z = 0.0;
       for (int p = lane; p < a.parts; p += 32) {
         const BeamPart q = a.part[row * a.parts + p];
-        if (q.m > -INFINITY || q.sum != q.sum) z += q.sum * exp(static_cast<double>(q.m) - m);
+        if (q.m > -INFINITY || q.sum != q.sum) z += static_cast<double>(q.sum) * exp_neg(q.m - m);
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
@@ -308,7 +417,10 @@ int launch_beam_select(const BeamArgs& a_in, void* ws, int64_t ws_bytes, cudaStr
                                 (kMaxCandidates + kMaxBeams) * static_cast<int>(sizeof(Candidate))) == cudaSuccess;
   };
   if (cudaGetDevice(&device) != cudaSuccess || !attr.done(device, set)) return kErrCuda;
-  (a.bf16 ? beam_scan_kernel<true> : beam_scan_kernel<false>)<<<static_cast<unsigned>(n), kScanThreads, 0, stream>>>(a);
+  const int64_t bytes = a.bf16 ? 2 : 4;
+  const bool skewed = off(a.x, 16) || (rows > 1 && a.ldx * bytes % 16 != 0);
+  (a.bf16 ? (skewed ? beam_scan_kernel<true, true> : beam_scan_kernel<true, false>)
+          : (skewed ? beam_scan_kernel<false, true> : beam_scan_kernel<false, false>))<<<static_cast<unsigned>(n), kScanThreads, 0, stream>>>(a);
   if (cudaGetLastError() != cudaSuccess) return kErrCuda;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.G));

@@ -320,9 +320,8 @@ struct MoveArgs {
 int launch_move_rows(const MoveView* views, const MoveArgs& a, cudaStream_t stream);
 
 // A beam search's selection (csrc/beam.cu).
-struct BeamPart {                      // of one part of one row: the largest logit, sum of e^(x - m)
-  double sum;
-  float m, pad;
+struct BeamPart {                      // of one part of one row: sum of e^(x - m), the reference m
+  float sum, m;
 };
 struct BeamArgs {
   const void* x = nullptr;             // [G * B, ldx] fp32 or bf16 logits
