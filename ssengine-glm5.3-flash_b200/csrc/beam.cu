@@ -5,9 +5,10 @@
 // scan: a CTA has one part of one beam's row, 16 bytes a load. Each warp keeps a sum of exponentials against a reference (a
 //   logit it has seen; it moves only when one exceeds it by 40, where a running maximum would be rescaled all the time) and
 //   the k largest (logit, token) as 64-bit keys whose order is that of the candidates (equal logits: the lower token is
-//   larger). The largest logit of a load is compared with the warp's k-th; what is above goes to the warp's list in shared
-//   memory, which is cut back to its k largest when it is full. The first k-th is that of the lanes' maxima over their first
-//   loads. The CTA leaves k keys, the reference and the sum.
+//   larger). A load's largest logit is compared with a bound of the CTA's k-th largest: the least of its 8 warps' ceil(k / 8)-th
+//   largest, at first of the lanes' maxima over their first loads, then of the lists. What is not below goes to the warp's
+//   list in shared memory, cut back to its k largest when it is full or the logits seen are four times as many. The CTA
+//   leaves k keys, the reference and the sum.
 // join: a CTA a request: the rows' log sums, then every candidate's score in 64 bits (a beam's own candidates keep the order
 //   of their logits, those of different beams are compared at the sums' accuracy). The candidates at or above the best
 //   part's k-th go to shared memory and each finds its place by counting those before it.
@@ -83,56 +84,61 @@ SSB_DEVICE int take_largest(uint64_t (&mine)[R], uint64_t* out, int k, int lane)
   return n;
 }
 
-// A warp's candidates.
+// A warp's candidates in shared memory. top: a logit of which the warp has seen ceil(k / 8) as large or larger, so that the
+// least `top` of the CTA's 8 warps bounds the CTA's k-th largest from below.
 struct WarpList {
-  uint64_t* list;
-  int count, k;
-  uint64_t least;                                // the k-th largest, 0 while it is not known
-  float bar;                                     // a logit below it is not among the k largest
-  SSB_DEVICE void add(float x, uint32_t token, int lane) {
-    bool in = x >= bar && x > -INFINITY;         // false for NaN
-    if (!__any_sync(0xffffffffu, in)) return;
-    const uint64_t key = make_key(x, token);
-    in = in && key > least;
-    const uint32_t mask = __ballot_sync(0xffffffffu, in);
-    if (mask == 0) return;
-    if (count + 32 > kList) cut(lane);
-    if (in) list[count + __popc(mask & ((1u << lane) - 1))] = key;
-    count += __popc(mask);
-    __syncwarp();
-  }
-  SSB_DEVICE void cut(int lane) {
-    if (count <= 64) {
-      uint64_t mine[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) mine[j] = 32 * j + lane < count ? list[32 * j + lane] : 0;
-      __syncwarp();
-      count = take_largest(mine, list, k, lane);
-    } else {
-      uint64_t mine[kList / 32];
-#pragma unroll
-      for (int j = 0; j < kList / 32; ++j) mine[j] = 32 * j + lane < count ? list[32 * j + lane] : 0;
-      __syncwarp();
-      count = take_largest(mine, list, k, lane);
-    }
-    if (count == k) {
-      least = list[k - 1];
-      bar = key_logit(least);
-    }
-    __syncwarp();
-  }
+  uint64_t key[kList];
+  uint64_t least;                                // the warp's k-th largest key, 0 while it is not known
+  float top;
+  int32_t count;
 };
+__device__ __noinline__ void cut_list(WarpList& L, int k, int lane) {
+  const int count = L.count;
+  int n;
+  if (count <= 64) {
+    uint64_t mine[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) mine[j] = 32 * j + lane < count ? L.key[32 * j + lane] : 0;
+    __syncwarp();
+    n = take_largest(mine, L.key, k, lane);
+  } else {
+    uint64_t mine[kList / 32];
+#pragma unroll
+    for (int j = 0; j < kList / 32; ++j) mine[j] = 32 * j + lane < count ? L.key[32 * j + lane] : 0;
+    __syncwarp();
+    n = take_largest(mine, L.key, k, lane);
+  }
+  const int share = (k + kScanWarps - 1) / kScanWarps;
+  if (lane == 0) {
+    L.count = n;
+    if (n == k) L.least = L.key[k - 1];
+    if (n >= share) L.top = fmaxf(L.top, key_logit(L.key[share - 1]));
+  }
+  __syncwarp();
+}
+// Adds the lanes' logits x that are not below bar and above the list's k-th.
+__device__ __noinline__ void offer(WarpList& L, int k, float x, uint32_t token, float bar, int lane) {
+  const uint64_t key = make_key(x, token);
+  const bool in = x >= bar && x > -INFINITY && key > L.least;          // false for NaN
+  const uint32_t mask = __ballot_sync(0xffffffffu, in);
+  if (mask == 0) return;
+  if (L.count + 32 > kList) cut_list(L, k, lane);
+  const int count = L.count;
+  if (in) L.key[count + __popc(mask & ((1u << lane) - 1))] = key;
+  __syncwarp();
+  if (lane == 0) L.count = count + __popc(mask);
+  __syncwarp();
+}
 
 // kSkewed: rows may begin anywhere in a 16-byte piece of memory. A lane's values are the same ones of a row then too, put
 // together from two pieces: equal rows get the same sums wherever they lie, and equal candidates stay equal.
 template <bool kBf16, bool kSkewed>
-__global__ void __launch_bounds__(kScanThreads, 5) beam_scan_kernel(const __grid_constant__ BeamArgs a) {
+__global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid_constant__ BeamArgs a) {
   constexpr int kVec = kBf16 ? 8 : 4, kBytes = 16 / kVec;
   constexpr int kLoads = kSkewed ? 2 : 4;                    // 16-byte loads a lane has on their way
-  __shared__ uint64_t lists[kScanWarps][kList];
+  __shared__ WarpList lists[kScanWarps];
   __shared__ float wm[kScanWarps];
   __shared__ float ws[kScanWarps];
-  __shared__ int32_t wn[kScanWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t row = blockIdx.x / a.parts;
   const int part = static_cast<int>(blockIdx.x - row * a.parts);
@@ -141,13 +147,16 @@ __global__ void __launch_bounds__(kScanThreads, 5) beam_scan_kernel(const __grid
   if (!(fabsf(score) < INFINITY) || (a.finished != nullptr && a.finished[row])) return;
   // the row in vectors of 16 bytes
   const char* p = static_cast<const char*>(a.x) + row * a.ldx * kBytes;
-  const int64_t vectors = (a.V + kVec - 1) / kVec;
-  const int64_t begin = vectors * part / a.parts, end = vectors * (part + 1) / a.parts;
+  const int32_t V = static_cast<int32_t>(a.V), vectors = (V - 1) / kVec + 1;
+  const int32_t begin = static_cast<int32_t>(static_cast<int64_t>(vectors) * part / a.parts);
+  const int32_t end = static_cast<int32_t>(static_cast<int64_t>(vectors) * (part + 1) / a.parts);
   const int skew = kSkewed ? static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15) : 0;      // bytes
   const uint4* pieces = reinterpret_cast<const uint4*>(p - skew);
-  const int64_t whole0 = skew > 0, whole1 = kSkewed ? (a.V * kBytes + skew) / 16 - 1 : a.V / kVec;   // whose pieces are the row's
-  const auto load = [&](int64_t i) {                         // -inf where it is not the row's
-    if (i >= whole0 && i < whole1 && i < end) {
+  // vectors all of whose pieces are the row's
+  const int32_t lo = max(begin, kSkewed && skew > 0 ? 1 : 0);
+  const int32_t hi = min(end, kSkewed ? static_cast<int32_t>((a.V * kBytes + skew) / 16) - 1 : V / kVec);
+  const auto load = [&](int32_t i) {                         // -inf where it is not the part's
+    if (i >= lo && i < hi) {
       if (!kSkewed) return __ldcs(pieces + i);
       const uint4 q0 = __ldg(pieces + i), q1 = __ldg(pieces + i + 1);
       uint32_t w[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
@@ -162,7 +171,7 @@ __global__ void __launch_bounds__(kScanThreads, 5) beam_scan_kernel(const __grid
     uint32_t w[4];
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
-      const int64_t e = i * kVec + j;
+      const int64_t e = static_cast<int64_t>(i) * kVec + j;
       const bool in = i < end && e < a.V;
       if (kBf16) {
         const uint32_t v = in ? reinterpret_cast<const uint16_t*>(p)[e] : 0xFF80u;
@@ -188,32 +197,51 @@ __global__ void __launch_bounds__(kScanThreads, 5) beam_scan_kernel(const __grid
     const __nv_bfloat162 m = __hmax2(__hmax2(b2(q.x), b2(q.y)), __hmax2(b2(q.z), b2(q.w)));
     return fmaxf(__low2float(m), __high2float(m));
   };
-  WarpList L = {lists[warp], 0, a.k, 0, -INFINITY};
-  float ref = -INFINITY;                                     // the same in all lanes
+  WarpList& L = lists[warp];
+  if (lane == 0) L.least = 0, L.top = -INFINITY, L.count = 0;
+  __syncthreads();
+  float ref = -INFINITY, bar = -INFINITY;                    // the same in all lanes; a logit below bar is no candidate
   uint64_t neg = 0, sum = 0;                                 // -ref (0 while there is none) and the sum, as pairs
-  bool first = true;
+  int32_t seen = 0, look = 1;                                // iterations, when to cut the list next
+  uint4 q[kLoads];
+  const int32_t i1 = begin + 32 * warp;
+#pragma unroll
+  for (int u = 0; u < kLoads; ++u) q[u] = load(i1 + u * kScanThreads + lane);
+  {                                                          // at least k logits are as large as the k-th lane's maximum
+    float most = largest(q[0]);
+#pragma unroll
+    for (int u = 1; u < kLoads; ++u) most = fmaxf(most, largest(q[u]));
+    uint64_t mine[1] = {most > -INFINITY ? make_key(most, lane) : 0};
+    const int n = take_largest(mine, L.key, min(a.k, 32), lane), share = (a.k + kScanWarps - 1) / kScanWarps;
+    if (n > 0) ref = key_logit(L.key[0]), neg = f2pack(-ref, -ref);
+    if (n == a.k) bar = key_logit(L.key[n - 1]);
+    if (lane == 0 && n >= share) L.top = key_logit(L.key[share - 1]);
+  }
+  __syncthreads();
 #pragma unroll 1
-  for (int64_t i0 = begin + 32 * warp; i0 < end; i0 += kLoads * kScanThreads) {
-    uint4 q[kLoads];
+  for (int32_t i0 = i1; i0 < end; i0 += kLoads * kScanThreads) {
+    if (seen > 0) {
 #pragma unroll
-    for (int u = 0; u < kLoads; ++u) q[u] = load(i0 + u * kScanThreads + lane);
-    if (first) {                                             // at least k logits are as large as the k-th lane's maximum
-      first = false;
-      float most = largest(q[0]);
-#pragma unroll
-      for (int u = 1; u < kLoads; ++u) most = fmaxf(most, largest(q[u]));
-      uint64_t mine[1] = {most > -INFINITY ? make_key(most, lane) : 0};
-      const int n = take_largest(mine, L.list, min(a.k, 32), lane);
-      if (n > 0) ref = key_logit(L.list[0]), neg = f2pack(-ref, -ref);
-      if (n == a.k) L.bar = key_logit(L.list[n - 1]);
-      __syncwarp();
+      for (int u = 0; u < kLoads; ++u) q[u] = load(i0 + u * kScanThreads + lane);
     }
+    if (seen == look) {                                      // the list's cut costs as much as an iteration or two
+      look *= 4;
+      cut_list(L, a.k, lane);
+    }
+    ++seen;
+    {
+      // other warps' tops may be read old: they only rise
+      float t = lane < kScanWarps ? *static_cast<volatile float*>(&lists[lane].top) : INFINITY;
+#pragma unroll
+      for (int o = kScanWarps / 2; o > 0; o >>= 1) t = fminf(t, __shfl_xor_sync(0xffffffffu, t, o));
+      bar = fmaxf(bar, __shfl_sync(0xffffffffu, t, 0));
+      if (L.least != 0) bar = fmaxf(bar, key_logit(L.least));
+    }
+    float limit = fminf(bar, ref + kRise);                   // of the loads to look at
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) {
-      float x[kVec];
-      values(q[u], x);
       const float top = largest(q[u]);
-      if (__any_sync(0xffffffffu, top >= L.bar)) {
+      if (__any_sync(0xffffffffu, top >= limit)) {
         if (__any_sync(0xffffffffu, top > ref + kRise || ref == -INFINITY)) {
           float now = top == top ? top : -INFINITY;
 #pragma unroll
@@ -223,12 +251,18 @@ __global__ void __launch_bounds__(kScanThreads, 5) beam_scan_kernel(const __grid
             sum = mul2(sum, f2pack(f, f));
             ref = now;
             neg = f2pack(-ref, -ref);
+            limit = fminf(bar, ref + kRise);
           }
         }
-        const int64_t at = (i0 + u * kScanThreads + lane) * kVec;
+        float x[kVec];
+        values(q[u], x);
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) L.add(x[j], static_cast<uint32_t>(at + j), lane);
+        for (int j = 0; j < kVec; ++j)
+          if (__any_sync(0xffffffffu, x[j] >= bar))
+            offer(L, a.k, x[j], static_cast<uint32_t>(i0 + u * kScanThreads + lane) * kVec + j, bar, lane);
       }
+      float x[kVec];
+      values(q[u], x);
       const uint64_t scale = f2pack(kLog2e, kLog2e);
 #pragma unroll
       for (int j = 0; j < kVec; j += 2) {
@@ -238,14 +272,14 @@ __global__ void __launch_bounds__(kScanThreads, 5) beam_scan_kernel(const __grid
       }
     }
   }
-  L.cut(lane);
+  cut_list(L, a.k, lane);
   // the CTA's reference and sum, then its k largest
   float s0, s1;
   f2unpack(sum, s0, s1);
   s0 += s1;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
-  if (lane == 0) wm[warp] = ref, ws[warp] = s0, wn[warp] = L.count;
+  if (lane == 0) wm[warp] = ref, ws[warp] = s0;
   __syncthreads();
   if (warp != 0) return;
   const float m = lane < kScanWarps ? wm[lane] : -INFINITY;
@@ -264,7 +298,7 @@ __global__ void __launch_bounds__(kScanThreads, 5) beam_scan_kernel(const __grid
 #pragma unroll
     for (int j = 0; j < kScanWarps * 8 / 32; ++j) {
       const int i = 32 * j + lane, w = i / 8, e = i % 8;
-      mine[j] = e < wn[w] ? lists[w][e] : 0;
+      mine[j] = e < lists[w].count ? lists[w].key[e] : 0;
     }
     n = take_largest(mine, out, a.k, lane);
   } else {
@@ -272,7 +306,7 @@ __global__ void __launch_bounds__(kScanThreads, 5) beam_scan_kernel(const __grid
 #pragma unroll
     for (int j = 0; j < kScanWarps * kMaxK / 32; ++j) {
       const int i = 32 * j + lane, w = i / kMaxK, e = i % kMaxK;
-      mine[j] = e < wn[w] ? lists[w][e] : 0;
+      mine[j] = e < lists[w].count ? lists[w].key[e] : 0;
     }
     n = take_largest(mine, out, a.k, lane);
   }
@@ -375,10 +409,11 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
   }
 }
 
-// Parts a row is cut into: CTAs for every SM several times over, none short, the candidates of a request within bounds.
+// Parts a row is cut into: what fills the SMs once, 4 CTAs each (64 x 8 beams: one part 66 us, five 107, whose first lists
+// cost more than the tail they save), none short, the candidates of a request within bounds.
 int beam_parts(int64_t G, int64_t B, int64_t V, int64_t k) {
   const int64_t rows = G * B;
-  int64_t parts = rows > 0 ? (148 * 8 + rows - 1) / rows : 1;
+  int64_t parts = rows > 0 ? 148 * 4 / rows : 1;
   parts = parts < V / kMinPart ? parts : V / kMinPart;
   parts = parts < kMaxCandidates / (B * k) ? parts : kMaxCandidates / (B * k);
   return static_cast<int>(parts > 1 ? parts : 1);
