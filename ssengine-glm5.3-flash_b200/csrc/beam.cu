@@ -19,8 +19,9 @@
 namespace ssb {
 namespace {
 
-constexpr int kScanWarps = 8, kScanThreads = 32 * kScanWarps;
+constexpr int kScanWarps = 8, kScanThreads = 32 * kScanWarps, kScanBlocks = 3;
 constexpr int kList = 256;                       // keys a warp holds between cuts
+constexpr int kGroups = 3;                        // groups of loads on their way to shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRise = 40.0f;                   // above the reference before it moves: e^40 times 2^31 terms stay finite
 constexpr int kJoinThreads = 512;
@@ -133,7 +134,7 @@ __device__ __noinline__ void offer(WarpList& L, int k, float x, uint32_t token, 
 // kSkewed: rows may begin anywhere in a 16-byte piece of memory. A lane's values are the same ones of a row then too, put
 // together from two pieces: equal rows get the same sums wherever they lie, and equal candidates stay equal.
 template <bool kBf16, bool kSkewed>
-__global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid_constant__ BeamArgs a) {
+__global__ void __launch_bounds__(kScanThreads, kScanBlocks) beam_scan_kernel(const __grid_constant__ BeamArgs a) {
   constexpr int kVec = kBf16 ? 8 : 4, kBytes = 16 / kVec;
   constexpr int kLoads = kSkewed ? 2 : 4;                    // 16-byte loads a lane has on their way
   __shared__ WarpList lists[kScanWarps];
@@ -182,6 +183,21 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   };
+  // Whole rows come by asynchronous copies, a lane's own places: a group of kLoads vectors is read while the next one is on its
+  // way, without registers held for it (64 x 8 beams: 76 us with loads alone, 68 with the next ones in registers).
+  extern __shared__ __align__(16) uint4 ring[];
+  const auto place = [&](int group, int u) { return ring + ((group % kGroups) * kLoads + u) * kScanThreads + tid; };
+  const auto ask = [&](int32_t i0, int group) {
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const int32_t i = i0 + u * kScanThreads + lane;
+      if (i >= lo && i < hi)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(place(group, u))), "l"(pieces + i) : "memory");
+      else
+        *place(group, u) = load(i);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
   const auto values = [](uint4 q, float (&x)[kVec]) {
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
@@ -204,26 +220,46 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
   uint64_t neg = 0, sum = 0;                                 // -ref (0 while there is none) and the sum, as pairs
   int32_t seen = 0, look = 1;                                // iterations, when to cut the list next
   uint4 q[kLoads];
-  const int32_t i1 = begin + 32 * warp;
+  const int32_t i1 = begin + 32 * warp, step = kLoads * kScanThreads;
+  const auto fetch = [&](int32_t i0, int group) {
+    if (kSkewed) {
 #pragma unroll
-  for (int u = 0; u < kLoads; ++u) q[u] = load(i1 + u * kScanThreads + lane);
+      for (int u = 0; u < kLoads; ++u) q[u] = load(i0 + u * kScanThreads + lane);
+    } else {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kGroups - 1) : "memory");
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) q[u] = *place(group, u);
+    }
+  };
+  if (!kSkewed) {
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) ask(i1 + g * step, g);
+  }
+  fetch(i1, 0);
   {                                                          // at least k logits are as large as the k-th lane's maximum
     float most = largest(q[0]);
 #pragma unroll
     for (int u = 1; u < kLoads; ++u) most = fmaxf(most, largest(q[u]));
-    uint64_t mine[1] = {most > -INFINITY ? make_key(most, lane) : 0};
-    const int n = take_largest(mine, L.key, min(a.k, 32), lane), share = (a.k + kScanWarps - 1) / kScanWarps;
-    if (n > 0) ref = key_logit(L.key[0]), neg = f2pack(-ref, -ref);
-    if (n == a.k) bar = key_logit(L.key[n - 1]);
-    if (lane == 0 && n >= share) L.top = key_logit(L.key[share - 1]);
+    uint32_t mine = most > -INFINITY ? static_cast<uint32_t>(make_key(most, 0) >> 32) : 0;
+    const int share = (a.k + kScanWarps - 1) / kScanWarps;
+    for (int n = 0; n < min(a.k, 32); ++n) {
+      const uint32_t best = __reduce_max_sync(0xffffffffu, mine);
+      if (best == 0) break;
+      if (lane == __ffs(__ballot_sync(0xffffffffu, mine == best)) - 1) mine = 0;
+      const float x = key_logit(static_cast<uint64_t>(best) << 32);
+      if (n == 0) ref = x, neg = f2pack(-ref, -ref);
+      if (n == share - 1 && lane == 0) L.top = x;
+      if (n == a.k - 1) bar = x;
+    }
   }
   __syncthreads();
 #pragma unroll 1
-  for (int32_t i0 = i1; i0 < end; i0 += kLoads * kScanThreads) {
-    if (seen > 0) {
+  for (int32_t i0 = i1; i0 < end; i0 += step) {
+    if (seen > 0) fetch(i0, seen);
+    float tops[kLoads];
 #pragma unroll
-      for (int u = 0; u < kLoads; ++u) q[u] = load(i0 + u * kScanThreads + lane);
-    }
+    for (int u = 0; u < kLoads; ++u) tops[u] = largest(q[u]);
+    if (!kSkewed) ask(i0 + kGroups * step, seen);            // into the places just read
     if (seen == look) {                                      // the list's cut costs as much as an iteration or two
       look *= 4;
       cut_list(L, a.k, lane);
@@ -240,7 +276,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
     float limit = fminf(bar, ref + kRise);                   // of the loads to look at
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) {
-      const float top = largest(q[u]);
+      const float top = tops[u];
       if (__any_sync(0xffffffffu, top >= limit)) {
         if (__any_sync(0xffffffffu, top > ref + kRise || ref == -INFINITY)) {
           float now = top == top ? top : -INFINITY;
@@ -418,6 +454,7 @@ int beam_parts(int64_t G, int64_t B, int64_t V, int64_t k) {
   parts = parts < kMaxCandidates / (B * k) ? parts : kMaxCandidates / (B * k);
   return static_cast<int>(parts > 1 ? parts : 1);
 }
+constexpr int kRing = kGroups * 4 * kScanThreads * 16;
 int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
 }  // namespace
@@ -448,14 +485,18 @@ int launch_beam_select(const BeamArgs& a_in, void* ws, int64_t ws_bytes, cudaStr
   static OncePerDevice attr;
   int device = 0;
   const auto set = [] {
-    return cudaFuncSetAttribute(beam_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (kMaxCandidates + kMaxBeams) * static_cast<int>(sizeof(Candidate))) == cudaSuccess;
+    const auto most = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    return cudaFuncSetAttribute(beam_join_kernel, most,
+                                (kMaxCandidates + kMaxBeams) * static_cast<int>(sizeof(Candidate))) == cudaSuccess &&
+           cudaFuncSetAttribute(beam_scan_kernel<false, false>, most, kRing) == cudaSuccess &&
+           cudaFuncSetAttribute(beam_scan_kernel<true, false>, most, kRing) == cudaSuccess;
   };
   if (cudaGetDevice(&device) != cudaSuccess || !attr.done(device, set)) return kErrCuda;
   const int64_t bytes = a.bf16 ? 2 : 4;
   const bool skewed = off(a.x, 16) || (rows > 1 && a.ldx * bytes % 16 != 0);
   (a.bf16 ? (skewed ? beam_scan_kernel<true, true> : beam_scan_kernel<true, false>)
-          : (skewed ? beam_scan_kernel<false, true> : beam_scan_kernel<false, false>))<<<static_cast<unsigned>(n), kScanThreads, 0, stream>>>(a);
+          : (skewed ? beam_scan_kernel<false, true> : beam_scan_kernel<false, false>))
+      <<<static_cast<unsigned>(n), kScanThreads, skewed ? 0 : kRing, stream>>>(a);
   if (cudaGetLastError() != cudaSuccess) return kErrCuda;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.G));
