@@ -351,57 +351,66 @@ __global__ void __launch_bounds__(kScanThreads, kScanBlocks) beam_scan_kernel(co
 
 struct Candidate {
   double score;
-  int64_t place;                                 // b V + v
+  uint64_t place;                                // beam, token: in the order of b V + v
 };
 // a before b in the result
 SSB_DEVICE bool before(const Candidate& a, const Candidate& b) {
   return a.score > b.score || (a.score == b.score && a.place < b.place);
 }
 
+// Shared memory: the parts' keys, then room for every candidate.
 __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_constant__ BeamArgs a) {
-  extern __shared__ __align__(16) Candidate cand[];
-  __shared__ double base[kMaxBeams];             // the rows' log sums, NaN: the beam has no candidate of its logits
+  extern __shared__ __align__(16) uint64_t keys[];
+  __shared__ double lse[kMaxBeams];              // the rows' log sums, NaN: the beam has no candidate of its logits
+  __shared__ double given[kMaxBeams];            // the beams' scores
   __shared__ Candidate bound[kJoinThreads / 32];
   __shared__ int32_t count;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t g = blockIdx.x;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int per = a.parts * a.k, total = a.B * per;
+  Candidate* cand = reinterpret_cast<Candidate*>(keys + (total + 1) / 2 * 2);
   if (tid == 0) count = 0;
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int i = tid; i < total; i += kJoinThreads) keys[i] = a.keys[g * total + i];     // anything of a beam left out
   for (int b = warp; b < a.B; b += kJoinThreads / 32) {
-    const int64_t row = g * a.B + b;
-    const float score = a.scores[row];
-    const bool done = a.finished != nullptr && a.finished[row];
-    double lse = nan("");
-    if (fabsf(score) < INFINITY && !done) {
+    const float score = a.scores[g * a.B + b];
+    const bool finite = fabsf(score) < INFINITY, done = a.finished != nullptr && a.finished[g * a.B + b];
+    double l = nan("");
+    if (finite && !done) {
+      const BeamPart* part = a.part + (g * a.B + b) * a.parts;
       float m = -INFINITY;
-      for (int p = lane; p < a.parts; p += 32) m = fmaxf(m, a.part[row * a.parts + p].m);
+      for (int p = lane; p < a.parts; p += 32) m = fmaxf(m, part[p].m);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       double z = 0.0;
       for (int p = lane; p < a.parts; p += 32) {
-        const BeamPart q = a.part[row * a.parts + p];
+        const BeamPart q = part[p];
         if (q.m > -INFINITY || q.sum != q.sum) z += static_cast<double>(q.sum) * exp_neg(q.m - m);
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-      lse = log(z) + m;
+      l = log(z) + m;
     }
-    if (lane == 0) base[b] = fabs(lse) < INFINITY ? lse : nan("");
+    if (lane == 0) {
+      given[b] = score;
+      lse[b] = fabs(l) < INFINITY ? l : nan("");
+      if (finite && done) cand[atomicAdd(&count, 1)] = {score, static_cast<uint64_t>(b) << 32 | static_cast<uint64_t>(a.pad)};
+    }
   }
   __syncthreads();
-  const int per = a.parts * a.k, total = a.B * per;
-  const auto get = [&](int i) {
+  const auto get = [&](int i) {                  // candidate i, whose score is -inf where there is none
     const int b = i / per;
-    const uint64_t key = base[b] == base[b] ? a.keys[g * total + i] : 0;
-    Candidate c = {-INFINITY, int64_t{0x7fffffffffffffff}};
-    if (key != 0) {
-      c.score = static_cast<double>(a.scores[g * a.B + b]) + (static_cast<double>(key_logit(key)) - base[b]);
-      c.place = b * a.V + key_token(key);
+    const uint64_t key = keys[i];
+    Candidate c = {-INFINITY, ~uint64_t{0}};
+    if (lse[b] == lse[b] && key != 0) {
+      c.score = given[b] + (static_cast<double>(key_logit(key)) - lse[b]);
+      c.place = static_cast<uint64_t>(b) << 32 | key_token(key);
     }
     return c;
   };
   // the best k-th candidate of a part: none after it is among the k best
-  Candidate bar = {-INFINITY, int64_t{0x7fffffffffffffff}};
+  Candidate bar = {-INFINITY, ~uint64_t{0}};
   for (int i = tid * a.k + a.k - 1; i < total; i += kJoinThreads * a.k) {
     const Candidate c = get(i);
     if (before(c, bar)) bar = c;
@@ -413,17 +422,11 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
   }
   if (lane == 0) bound[warp] = bar;
   __syncthreads();
+#pragma unroll
   for (int w = 0; w < kJoinThreads / 32; ++w)
     if (before(bound[w], bar)) bar = bound[w];
-  for (int i = tid; i < total + a.B; i += kJoinThreads) {
-    Candidate c = {-INFINITY, 0};
-    if (i < total) {
-      c = get(i);
-    } else if (a.finished != nullptr && a.finished[g * a.B + i - total]) {
-      c.score = a.scores[g * a.B + i - total];
-      c.place = (i - total) * a.V + a.pad;
-      if (!(fabs(c.score) < INFINITY)) c.score = -INFINITY;
-    }
+  for (int i = tid; i < total; i += kJoinThreads) {
+    const Candidate c = get(i);
     if (c.score > -INFINITY && !before(bar, c)) cand[atomicAdd(&count, 1)] = c;
   }
   __syncthreads();
@@ -431,11 +434,12 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
   for (int i = tid; i < n; i += kJoinThreads) {
     const Candidate c = cand[i];
     int rank = 0;
+#pragma unroll 4
     for (int j = 0; j < n; ++j) rank += before(cand[j], c);
     if (rank < a.k) {
       a.out_scores[g * a.k + rank] = static_cast<float>(c.score);
-      a.out_parents[g * a.k + rank] = static_cast<int32_t>(c.place / a.V);
-      a.out_tokens[g * a.k + rank] = c.place % a.V;
+      a.out_parents[g * a.k + rank] = static_cast<int32_t>(c.place >> 32);
+      a.out_tokens[g * a.k + rank] = static_cast<int64_t>(c.place & 0xFFFFFFFFu);
     }
   }
   for (int i = n + tid; i < a.k; i += kJoinThreads) {
@@ -445,8 +449,9 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
   }
 }
 
-// Parts a row is cut into: what fills the SMs once, 4 CTAs each (64 x 8 beams: one part 66 us, five 107, whose first lists
-// cost more than the tail they save), none short, the candidates of a request within bounds.
+// Parts a row is cut into, the same for every row (equal rows get equal sums): about what fills the SMs once (64 x 8 beams:
+// one part 76 us, five 107 with loads alone, since every part begins and ends with its lists), none short, the candidates of
+// a request within bounds.
 int beam_parts(int64_t G, int64_t B, int64_t V, int64_t k) {
   const int64_t rows = G * B;
   int64_t parts = rows > 0 ? 148 * 4 / rows : 1;
@@ -454,6 +459,10 @@ int beam_parts(int64_t G, int64_t B, int64_t V, int64_t k) {
   parts = parts < kMaxCandidates / (B * k) ? parts : kMaxCandidates / (B * k);
   return static_cast<int>(parts > 1 ? parts : 1);
 }
+constexpr int join_bytes(int candidates, int beams) {
+  return (candidates + 1) / 2 * 16 + (candidates + beams) * static_cast<int>(sizeof(Candidate));
+}
+static_assert(join_bytes(kMaxCandidates, kMaxBeams) + 4096 <= 232448, "shared memory");
 constexpr int kRing = kGroups * 4 * kScanThreads * 16;
 int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
@@ -481,13 +490,12 @@ int launch_beam_select(const BeamArgs& a_in, void* ws, int64_t ws_bytes, cudaStr
   a.keys = static_cast<uint64_t*>(ws);
   a.part = reinterpret_cast<BeamPart*>(static_cast<uint8_t*>(ws) + up256(n * a.k * 8));
   if (n > 0x7fffffff) return kErrArgs;
-  const int smem = (a.B * a.parts * a.k + a.B) * static_cast<int>(sizeof(Candidate));
+  const int smem = join_bytes(a.B * a.parts * a.k, a.B);
   static OncePerDevice attr;
   int device = 0;
   const auto set = [] {
     const auto most = cudaFuncAttributeMaxDynamicSharedMemorySize;
-    return cudaFuncSetAttribute(beam_join_kernel, most,
-                                (kMaxCandidates + kMaxBeams) * static_cast<int>(sizeof(Candidate))) == cudaSuccess &&
+    return cudaFuncSetAttribute(beam_join_kernel, most, join_bytes(kMaxCandidates, kMaxBeams)) == cudaSuccess &&
            cudaFuncSetAttribute(beam_scan_kernel<false, false>, most, kRing) == cudaSuccess &&
            cudaFuncSetAttribute(beam_scan_kernel<true, false>, most, kRing) == cudaSuccess;
   };
