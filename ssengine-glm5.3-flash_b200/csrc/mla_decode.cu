@@ -264,12 +264,33 @@ SSB_DEVICE void mbar_arrive_n(uint32_t bar, uint32_t n) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n) : "memory");
 }
 
-// Tree form: the positions before the end of row t's visible ones: the context's and those up to the last node on its path
+// Tree form. Where a row's heads fill half of a tile or less, up to a.group = 64 / H neighbouring rows share one, and with it
+// every unit they read: rows of one request with one context length, cut at multiples of the group. The first of them, which
+// leads, stands for all in the plan; head h of the tile is head h % H of row h / H behind it.
+SSB_DEVICE bool leads(const MlaDecodeArgs& a, int t) {
+  return t % a.group == 0 || a.reqs == nullptr || a.reqs[t] != a.reqs[t - 1] || a.seq_lens[t] != a.seq_lens[t - 1];
+}
+SSB_DEVICE int leader_of(const MlaDecodeArgs& a, int t) {
+  while (!leads(a, t)) --t;
+  return t;
+}
+SSB_DEVICE int rows_led(const MlaDecodeArgs& a, int t) {
+  int n = 1;
+  while (n < a.group && t + n < a.T && !leads(a, t + n)) ++n;
+  return n;
+}
+// The nodes that any of the rows sees that t leads.
+SSB_DEVICE uint64_t nodes_seen(const MlaDecodeArgs& a, int t) {
+  uint64_t w = a.ancestors[t];
+  for (int i = 1; i < a.group && t + i < a.T && !leads(a, t + i); ++i) w |= a.ancestors[t + i];
+  return w;
+}
+// The positions before the end of the visible ones of the rows that t leads: the context's and those up to the last node seen
 // (0: a reqs entry outside the table, or a negative length). Positions past 2^31 - 2^7 are past any table.
 SSB_DEVICE int row_tokens(const MlaDecodeArgs& a, int t) {
   const int len = a.seq_lens[t];
   if (len < 0 || (a.reqs != nullptr && static_cast<uint32_t>(a.reqs[t]) >= static_cast<uint32_t>(a.R))) return 0;
-  return min(len, 0x7fffff00) + 64 - __clzll(static_cast<long long>(a.ancestors[t]));
+  return min(len, 0x7fffff00) + 64 - __clzll(static_cast<long long>(nodes_seen(a, t)));
 }
 
 // ---- the plan -----------------------------------------------------------------------------------------------------
@@ -277,7 +298,7 @@ SSB_DEVICE int row_tokens(const MlaDecodeArgs& a, int t) {
 // by the list's width or, where that is smaller, the tokens it can name.
 template <bool kTree>
 SSB_DEVICE int row_units(const MlaDecodeArgs& a, int t) {
-  if constexpr (kTree) return row_tokens(a, t) <= 0 ? 0 : min((row_tokens(a, t) + kUnit - 1) / kUnit, kPage / kUnit * a.width);
+  if constexpr (kTree) return leads(a, t) ? min((row_tokens(a, t) + kUnit - 1) / kUnit, kPage / kUnit * a.width) : 0;
   int n = a.indices != nullptr ? a.n_idx : 0x7fffff00;
   if (a.seq_lens != nullptr) n = min(n, a.seq_lens[t]);
   if (a.reqs != nullptr && static_cast<uint32_t>(a.reqs[t]) >= static_cast<uint32_t>(a.R)) n = 0;
@@ -383,7 +404,7 @@ template <bool kTree>
 __device__ __noinline__ void zero_rows(const MlaDecodeArgs& a, int cta, int h0, int nh, int lane) {
 #pragma unroll 1
   for (int t = cta; t < a.T; t += gridDim.x) {
-    if (row_units<kTree>(a, t) != 0) continue;
+    if (row_units<kTree>(a, kTree ? leader_of(a, t) : t) != 0) continue;
     if (lane == 0 && a.reqs != nullptr && static_cast<uint32_t>(a.reqs[t]) >= static_cast<uint32_t>(a.R))
       raise_status(a.status, kErrArgs);
     uint4* o = reinterpret_cast<uint4*>(a.out + ((int64_t)t * a.H + h0) * kDv);
@@ -471,13 +492,18 @@ SSB_DEVICE void keep_q(uint8_t* smem, uint32_t to, const uint32_t (&w)[4], int p
 // unless it is below 2^-13 of the head's largest (then to 2^-21 of that). First the largest values, 8 threads a head (whole
 // lines); then a thread has half of its lane's head's quarter of the row (lanes l and l + 16 share a head), loaded four
 // ahead: lane l keeps the high parts, lane l + 16 the low ones, and they exchange the others. e4m3 queries have no low part.
-template <bool Q8>
+template <bool Q8, bool kTree>
 __device__ __noinline__ int stage_q(const MlaDecodeArgs& a, uint8_t* smem, uint32_t tmem, int t, int h0, int nh) {
   int32_t* tops = reinterpret_cast<int32_t*>(smem + kOffRow);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int h = 16 * (warp & 3) + (lane & 15), part = warp >> 2;      // 144 values
   const bool high = lane < 16, have = h < nh;
-  const int64_t off = (int64_t)t * a.ldq + (int64_t)(h0 + min(h, nh - 1)) * a.hsq + 144 * part;
+  const auto at_head = [&](int x) {                                   // of the tile, as an offset
+    if constexpr (kTree)
+      if (a.group > 1) return (int64_t)(t + x / a.H) * a.ldq + (int64_t)(x % a.H) * a.hsq;
+    return (int64_t)t * a.ldq + (int64_t)(h0 + x) * a.hsq;
+  };
+  const int64_t off = at_head(min(h, nh - 1)) + 144 * part;
   uint32_t to = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + kColQ + 36 * part;
   int k = 0;
   if (Q8) {
@@ -490,10 +516,10 @@ __device__ __noinline__ int stage_q(const MlaDecodeArgs& a, uint8_t* smem, uint3
       keep_q(smem, to, w, part, j);
     }
   } else {
-    const __nv_bfloat16* base = static_cast<const __nv_bfloat16*>(a.q) + (int64_t)t * a.ldq + (int64_t)h0 * a.hsq;
+    const __nv_bfloat16* base = static_cast<const __nv_bfloat16*>(a.q);
     {
       const int th = threadIdx.x >> 3, sub = threadIdx.x & 7;
-      const uint4* q = reinterpret_cast<const uint4*>(base + (int64_t)min(th, nh - 1) * a.hsq) + sub;
+      const uint4* q = reinterpret_cast<const uint4*>(base + at_head(min(th, nh - 1))) + sub;
       uint4 v[9];
 #pragma unroll
       for (int j = 0; j < 9; ++j) v[j] = __ldg(q + 8 * j);            // 8 values
@@ -510,7 +536,7 @@ __device__ __noinline__ int stage_q(const MlaDecodeArgs& a, uint8_t* smem, uint3
       for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
       if (sub == 0) tops[th] = top;
     }
-    const uint4* q = reinterpret_cast<const uint4*>(base + (int64_t)min(h, nh - 1) * a.hsq + 144 * part) + (high ? 0 : 1);
+    const uint4* q = reinterpret_cast<const uint4*>(base + off) + (high ? 0 : 1);
     uint4 next[4] = {__ldg(q), __ldg(q + 2), __ldg(q + 4), __ldg(q + 6)};
     named_bar(5, kSoftmax);
     const int top = tops[h];
@@ -554,6 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = blockIdx.x, tile = blockIdx.y;
   const int h0 = tile * kTileH, nh = min(kTileH, a.H - h0);
+  const auto heads_of = [&](int t) { return kTree && a.group > 1 ? rows_led(a, t) * a.H : nh; };    // heads of its tile
   const uint32_t sbase = smem_u32(smem), bar = sbase + kOffBar;
   const Bars B = {bar,       bar + 40,  bar + 80,  bar + 88,  bar + 104, bar + 120, bar + 136,
                   bar + 152, bar + 160, bar + 168, bar + 176, bar + 192, bar + 208};
@@ -611,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int len = kTree ? row_tokens(a, s.t) : a.seq_lens != nullptr ? a.seq_lens[s.t] : 0x7fffffff;
       // the tokens all seen; those from there on by the row's word
       const int plain = kTree ? min(a.seq_lens[s.t], 0x7fffff00) : len;
-      const uint64_t word = kTree ? a.ancestors[s.t] : 0;
+      const uint64_t word = kTree ? nodes_seen(a, s.t) : 0;
       const int32_t* idx = a.indices != nullptr ? a.indices + (int64_t)s.t * a.ld_idx : nullptr;
       int c0 = s.b0, c1 = s.b1;
       if (idx != nullptr) {                              // the row's planned share as units of list columns
@@ -696,6 +723,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           int32_t* told = reinterpret_cast<int32_t*>(slots + slot);
           if (pair == 0) told[half] = static_cast<int32_t>(present);
           if (w == 0) told[2] = cn >= c1 ? kLast : kMore;
+          if (kTree && w == 0) told[3] = c;
           mbar_arrive_n(full, whole ? 32 : 1);           // of a whole unit also for the lanes that copied nothing
         }
         if (++slot == kSlots) slot = 0, ++round;
@@ -717,6 +745,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     while (ok && walk_next<kTree>(a, walk, s)) {
       bool last = false, fresh = true;
+      const int heads = (heads_of(s.t) + 15) & ~15;
       if (seg > 0) ok = mbar_nap(B.o_free, (seg - 1) & 1, abort_flag, a.status);      // the row before has been read
       while (!last) {
         const int set = u & 1;
@@ -725,7 +754,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         last = ring[u & 7].z != kMore;
         tc_fence_after();
-        issue_values(B, sbase, slot, set, (nh + 15) & ~15, fresh, leader);
+        issue_values(B, sbase, slot, set, heads, fresh, leader);
         fresh = false;
         ++u;
         if (++slot == kSlots) slot = 0;
@@ -790,16 +819,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     int u0 = 0, seg = 0, events = 0;                     // the row's first unit
     Segment s;
     bool more = walk_next<kTree>(a, walk, s), ok = true;
-    if (teller) refs[mine] = mine < nh ? kNone : 0.0f;
-    int k = stage_q<Q8>(a, smem, tmem, s.t, h0, nh);     // exponent of head mine's query scale
+    int heads = heads_of(s.t);
+    if (teller) refs[mine] = mine < heads ? kNone : 0.0f;
+    int k = stage_q<Q8, kTree>(a, smem, tmem, s.t, h0, heads);     // exponent of head mine's query scale
     tc_fence_before();
     warp_arrive(B.q_full, lane);
     named_bar(5, kSoftmax);                              // every head's reference is written
     while (more) {
-      const float c = mine < nh ? a.bmm1 * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + k) << 23) : 0.0f;
+      const float c = mine < heads ? a.bmm1 * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + k) << 23) : 0.0f;
       const float c_own = part ? 0.0625f * c : c, c_got = part ? c : 0.0625f * c;
-      float l = 0.0f, ref = mine < nh ? kNone : 0.0f;    // the sum of the thread's weights, the reference it stands against
+      float l = 0.0f, ref = mine < heads ? kNone : 0.0f; // the sum of the thread's weights, the reference it stands against
       int u = u0 + ((set ^ u0) & 1);
+      // in a shared tile, the nodes that this head's row sees, behind `plain` tokens
+      const bool shared_tile = kTree && a.group > 1;
+      const uint64_t nodes = shared_tile && mine < heads ? a.ancestors[s.t + mine / a.H] : 0;
+      const int plain = shared_tile ? min(a.seq_lens[s.t], 0x7fffff00) : 0;
       while (true) {
         ok = mbar_nap(B.s_full + own, events & 1, abort_flag, a.status);
         ++events;
@@ -825,7 +859,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             v[i] = fmaf(part ? x[16 + i] : x[i], c_own, got * c_got);
           }
         }
-        const uint32_t present = static_cast<uint32_t>(half ? word.y : word.x);
+        uint32_t present = static_cast<uint32_t>(half ? word.y : word.x);
+        if (shared_tile && kUnit * word.w + kUnit > plain) {
+          const int from = kUnit * word.w + 32 * half - plain;         // the node of the thread's first token (< 0: context)
+          const uint64_t seen = from >= 64 ? 0 : from >= 0 ? nodes >> from : from <= -32 ? ~uint64_t{0}
+                                                                          : nodes << -from | ((uint64_t{1} << -from) - 1);
+          present &= static_cast<uint32_t>(seen);
+          // a token that some rows of the tile see and others do not: whatever its latent values are, the others must not meet
+          // NaN times weight 0. Its scores have been formed (NaN for the rows that see it): zeros in the value product do
+          uint4* rows16 = reinterpret_cast<uint4*>(smem + kOffKv + (u % kSlots) * kLat);
+#pragma unroll 1
+          for (int i = 32 * (warp & 7) + lane; i < kLat / 16; i += 32 * kSetWarps) {
+            uint4 b = rows16[i];
+            const uint32_t n0 = __vcmpeq4(b.x & 0x7F7F7F7Fu, 0x7F7F7F7Fu), n1 = __vcmpeq4(b.y & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+            const uint32_t n2 = __vcmpeq4(b.z & 0x7F7F7F7Fu, 0x7F7F7F7Fu), n3 = __vcmpeq4(b.w & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+            if (n0 | n1 | n2 | n3) rows16[i] = make_uint4(b.x & ~n0, b.y & ~n1, b.z & ~n2, b.w & ~n3);
+          }
+        }
         if (present != 0xffffffffu) {
 #pragma unroll
           for (int i = 0; i < 16; ++i)
@@ -944,15 +994,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       named_bar(5, kSoftmax);
       float total = rows[mine] + rows[64 + mine] + rows[128 + mine] + rows[192 + mine];
       if (ref == kNone && total == total) total = 0.0f;                              // no token
+      const Segment done = s;
+      const int done_heads = heads;
+      more = walk_next<kTree>(a, walk, s);
+      if (more) heads = heads_of(s.t);
       if (teller) {
         sums[mine] = total == 0.0f ? 0.0f : a.bmm2 / total;                          // a NaN sum stays one
-        refs[mine] = mine < nh ? kNone : 0.0f;
+        refs[mine] = mine < heads ? kNone : 0.0f;
       }
-      const Segment done = s;
-      more = walk_next<kTree>(a, walk, s);
       if (more) {
         if (!Q8) named_bar(5, kSoftmax);                 // the sums are read: their place takes the query's maxima
-        k = stage_q<Q8>(a, smem, tmem, s.t, h0, nh);
+        k = stage_q<Q8, kTree>(a, smem, tmem, s.t, h0, heads);
         tc_fence_before();
         warp_arrive(B.q_full, lane);
       }
@@ -963,7 +1015,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int slot = 2 * cta + (seg == 0 ? 0 : 1);
       if (teller) {
         if (!whole) part_ml(a, tile, slot)[mine] = make_float2(ref, total);
-        else if (a.lse != nullptr && mine < nh)
+        else if (a.lse != nullptr && mine < done_heads)
           a.lse[(int64_t)done.t * a.H + h0 + mine] =
               total == 0.0f ? kNone : ((ref == kNone ? 0.0f : ref) + log2f(total)) * kLn2;
         if (mine == 0 && tile == 0) {
@@ -975,7 +1027,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!whole) {                                      // a lane has one dim of 16 heads: 128 bytes a warp and head
         float* po = part_o(a, tile, slot) + hb * kDv + 32 * quarter + lane;
 #pragma unroll 1
-        for (int d = 0; d < 4 && hb < nh; ++d, po += 128) {
+        for (int d = 0; d < 4 && hb < done_heads; ++d, po += 128) {
           float o[16];
           tmem_ld_x16(tq + kColO + 64 * d + hb, o);
           tmem_ld_wait();
@@ -987,13 +1039,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int e = lane & 3, dim = 32 * quarter + (lane & 28);
       __nv_bfloat16* out = a.out + ((int64_t)done.t * a.H + h0 + hb + e) * kDv + dim;
 #pragma unroll 1
-      for (int i = 0; i < 16 && hb + i < nh && whole; i += 4) {      // 4 heads x 4 tiles of 128 dims
+      for (int i = 0; i < 16 && hb + i < done_heads && whole; i += 4) {      // 4 heads x 4 tiles of 128 dims
         float o[4][4];
 #pragma unroll
         for (int d = 0; d < 4; ++d) tmem_ld_x4(tq + kColO + 64 * d + hb + i, o[d]);
         tmem_ld_wait();
         const float inv = sums[hb + i + e];
-        const bool have = hb + i + e < nh;
+        const bool have = hb + i + e < done_heads;
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
           cross4(o[d], lane);
@@ -1028,12 +1080,14 @@ __global__ void __launch_bounds__(32 * kJoinWarps) mla_join_kernel(const __grid_
   __shared__ float4 so[kJoinWarps][32];
   __shared__ float sl[kJoinWarps];
   const int64_t t = blockIdx.x;
-  const int h = blockIdx.y, tile = h / kTileH, hh = h - tile * kTileH;
+  const int h = blockIdx.y, tile = h / kTileH;
+  const int64_t t0 = kTree ? leader_of(a, static_cast<int>(t)) : t;                       // the row whose tile this one shares
+  const int hh = static_cast<int>((t - t0) * a.H) + h - tile * kTileH;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int units = row_units<kTree>(a, static_cast<int>(t));     // of the inputs alone
+  const int units = row_units<kTree>(a, static_cast<int>(t0));     // of the inputs alone
   asm volatile("griddepcontrol.wait;" ::: "memory");       // the parts are written
   if (units == 0) return;
-  const MlaRowParts rp = a.rows[t];
+  const MlaRowParts rp = a.rows[t0];
   if (!rp.valid()) {
     if (threadIdx.x == 0) raise_status(a.status, kErrTimeout);
     return;
@@ -1116,6 +1170,7 @@ int launch_mla_decode(const MlaDecodeArgs& a_in, void* ws, int64_t ws_bytes, cud
   p += up256(slots * kTileH * 8);
   a.part_o = reinterpret_cast<float*>(p);
   const bool tree = a.ancestors != nullptr;
+  a.group = tree && a.H <= kTileH / 2 ? kTileH / a.H : 1;
   auto* kernel = tree ? (a.q_e4m3 ? mla_decode_kernel<true, true> : mla_decode_kernel<false, true>)
                       : (a.q_e4m3 ? mla_decode_kernel<true, false> : mla_decode_kernel<false, false>);
   static OncePerDevice attr[4];

@@ -260,6 +260,7 @@ struct MlaDecodeArgs {
   int64_t ld_idx = 0;
   int32_t n_idx = 0;
   const uint64_t* ancestors = nullptr; // tree form: bit j of row t: it sees position seq_lens[t] + j too (null: none)
+  int32_t group = 1;                   // tree form: rows that may share a tile (set by the launcher)
   float bmm1 = 0.0f, bmm2 = 1.0f;
   __nv_bfloat16* out = nullptr;        // [T, H, 512]
   float* lse = nullptr;                // [T, H] or null

@@ -115,6 +115,71 @@ def test_unseen_nodes_may_hold_nan(cuda):
         check(out[0], lse[0], *attention64(q64[0], cache.kv[0][np.r_[0:300, 300 + np.array(p)]], BMM1, 1.0))
 
 
+@pytest.mark.parametrize("heads", [1, 3, 16, 21, 32, 33, 64])
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_a_nan_node_reaches_its_descendants_alone(cuda, heads, kind):
+    """Nodes of one call, two of them with NaN in their cache rows: their descendants' outputs are NaN, no other node's."""
+    rng = np.random.default_rng(heads)
+    for n in (5, 64, 100, 250):
+        tree = wild(rng, 30)
+        cache = Cache(rng, [n + 30])
+        bad = [4, 17]
+        cache.bytes[cache.slots(0, n + np.array(bad)), [100, 511]] = 0x7F
+        cache.bytes[cache.slots(0, n + np.array(bad)), [7, 300]] = 0xFF
+        seq, masks, reqs, seen = tree_rows([tree], [n])
+        q, q64 = queries(rng, 30, heads, kind)
+        out, lse, status = call_tree(cuda, q, cache, seq, masks, np.array(reqs, np.int32))
+        assert status == 0
+        for i in range(30):
+            if set(path(tree, i)) & set(bad):
+                assert np.isnan(out[i]).all() and np.isnan(lse[i]).all(), (n, i)
+            else:
+                check(out[i], lse[i], *attention64(q64[i], cache.kv[0][seen[i]], BMM1, 1.0))
+
+
+@pytest.mark.parametrize("heads", [1, 2, 7, 16, 22, 32])
+def test_rows_that_share_a_tile(cuda, heads):
+    """Few heads: neighbouring rows of a request share a tile. Rows of one request with several context lengths, requests
+    that take turns, rows without a node or without any token among them, empty and bad requests; with and without lse."""
+    rng = np.random.default_rng(50 + heads)
+    lens = [300, 0, 129, 5]
+    cache = Cache(rng, [n + 64 for n in lens])
+    rows = []
+    for r in (0, 0, 0, 1, 1, 2, 2, 2, 2, 2, 0, 3, 3, 9, 9, 2, 2, 1, 0):
+        for _ in range(int(rng.integers(1, 9))):
+            n = lens[r] if r < 4 else 10
+            n = n if rng.random() < 0.8 else max(n - int(rng.integers(0, 3)), 0)
+            w = 0 if rng.random() < 0.15 else int(rng.integers(0, 2 ** 63)) * 2 + 1
+            rows.append((r, n, w - 2 ** 64 if w >= 2 ** 63 else w))
+    reqs, seq, masks = (np.array([x[i] for x in rows]) for i in range(3))
+    q, q64 = queries(rng, len(rows), heads, "bf16")
+    for lse in (True, False):
+        out, ls, status = call_tree(cuda, q, cache, seq, masks, reqs.astype(np.int32), lse=lse)
+        assert status == 1
+        for t, (r, n, w) in enumerate(rows):
+            pos = [] if r > 3 else list(range(n)) + [n + j for j in range(64) if (w >> j) & 1]
+            kv = cache.kv[min(r, 3)][np.array(pos, np.int64)]
+            check(out[t], ls[t] if lse else None, *attention64(q64[t], kv, BMM1, 1.0))
+
+
+def test_shared_tiles_over_a_long_context(cuda):
+    """Shared tiles cut into parts and joined, rows in ranges of several requests, a caller's workspace full of ones."""
+    from ssengine_b200 import mla
+
+    rng = np.random.default_rng(60)
+    lens = [9001, 700, 20000]
+    trees = [wild(rng, 20), wild(rng, 33), wild(rng, 9)]
+    cache = Cache(rng, [n + len(t) for n, t in zip(lens, trees)])
+    seq, masks, reqs, seen = tree_rows(trees, lens)
+    for heads in (16, 30):
+        q, q64 = queries(rng, len(seq), heads, "e4m3")
+        ws = torch.full((mla.decode_workspace_bytes(len(seq), heads),), 0xFF, dtype=torch.uint8, device=cuda)
+        out, lse, status = call_tree(cuda, q, cache, seq, masks, np.array(reqs, np.int32), workspace=ws)
+        assert status == 0
+        for t in range(0, len(seq), 3):
+            check(out[t], lse[t], *attention64(q64[t], cache.kv[reqs[t]][seen[t]], BMM1, 1.0))
+
+
 def test_chain_equals_decode(cuda):
     """A chain's nodes are the draft rows of `mla.decode`, bit for bit: the same units of the same tokens."""
     from ssengine_b200 import mla
