@@ -55,9 +55,9 @@ def select(logits: torch.Tensor, scores: torch.Tensor, k: int, finished: torch.T
         out = (torch.empty(G, k, dtype=torch.float32, **dev), torch.empty(G, k, dtype=torch.int32, **dev),
                torch.empty(G, k, dtype=torch.int64, **dev))
     else:
-        for name, t, dtype in zip(("scores", "parents", "tokens"), out, (torch.float32, torch.int32, torch.int64)):
+        for t, dtype in zip(out, (torch.float32, torch.int32, torch.int64)):
             if t.dtype is not dtype or t.shape != (G, k) or not t.is_contiguous():
-                raise ValueError(f"out {name}: contiguous {dtype} {(G, k)}, got {t.dtype} {tuple(t.shape)}")
+                raise ValueError(f"out: contiguous {dtype} {(G, k)}, got {t.dtype} {tuple(t.shape)}")
     if workspace is not None and (workspace.dtype != torch.uint8 or not workspace.is_contiguous() or
                                   workspace.numel() < need):
         raise ValueError(f"workspace: contiguous uint8 of {need} bytes or more")

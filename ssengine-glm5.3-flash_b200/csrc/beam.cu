@@ -24,7 +24,7 @@ constexpr int kList = 256;                       // keys a warp holds between cu
 constexpr int kGroups = 3;                        // groups of loads on their way to shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRise = 40.0f;                   // above the reference before it moves: e^40 times 2^31 terms stay finite
-constexpr int kJoinThreads = 512;
+constexpr int kJoinThreads = 512, kRanked = 64;
 constexpr int kMaxK = 64, kMaxBeams = 64;
 constexpr int kMaxCandidates = 8192;             // of a request, all parts together
 constexpr int kMinPart = 2048;                   // logits a part has at least
@@ -350,9 +350,16 @@ __global__ void __launch_bounds__(kScanThreads, kScanBlocks) beam_scan_kernel(co
 }
 
 struct Candidate {
-  double score;
+  uint64_t score;                                // a double's bits in an order of its own: larger is better, 0 is none
   uint64_t place;                                // beam, token: in the order of b V + v
 };
+SSB_DEVICE uint64_t order_of(double x) {
+  const uint64_t b = static_cast<uint64_t>(__double_as_longlong(x + 0.0));              // -0 counts as 0
+  return b >> 63 ? ~b : b | 1ull << 63;
+}
+SSB_DEVICE double score_of(uint64_t o) {
+  return __longlong_as_double(static_cast<int64_t>(o >> 63 ? o & ~(1ull << 63) : ~o));
+}
 // a before b in the result
 SSB_DEVICE bool before(const Candidate& a, const Candidate& b) {
   return a.score > b.score || (a.score == b.score && a.place < b.place);
@@ -364,6 +371,8 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
   __shared__ double lse[kMaxBeams];              // the rows' log sums, NaN: the beam has no candidate of its logits
   __shared__ double given[kMaxBeams];            // the beams' scores
   __shared__ Candidate bound[kJoinThreads / 32];
+  __shared__ uint64_t group[kJoinThreads / 32];
+  __shared__ int32_t rank[kRanked];
   __shared__ int32_t count;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t g = blockIdx.x;
@@ -379,15 +388,22 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
     double l = nan("");
     if (finite && !done) {
       const BeamPart* part = a.part + (g * a.B + b) * a.parts;
+      BeamPart q[4];                             // the first 128 parts, loaded once
       float m = -INFINITY;
-      for (int p = lane; p < a.parts; p += 32) m = fmaxf(m, part[p].m);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) q[j] = lane + 32 * j < a.parts ? part[lane + 32 * j] : BeamPart{0.0f, -INFINITY};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) m = fmaxf(m, q[j].m);
+      for (int p = lane + 128; p < a.parts; p += 32) m = fmaxf(m, part[p].m);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const auto term = [&](const BeamPart& p) {
+        return p.m > -INFINITY || p.sum != p.sum ? static_cast<double>(p.sum) * exp_neg(p.m - m) : 0.0;
+      };
       double z = 0.0;
-      for (int p = lane; p < a.parts; p += 32) {
-        const BeamPart q = part[p];
-        if (q.m > -INFINITY || q.sum != q.sum) z += static_cast<double>(q.sum) * exp_neg(q.m - m);
-      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) z += term(q[j]);
+      for (int p = lane + 128; p < a.parts; p += 32) z += term(part[p]);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
       l = log(z) + m;
@@ -395,52 +411,73 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
     if (lane == 0) {
       given[b] = score;
       lse[b] = fabs(l) < INFINITY ? l : nan("");
-      if (finite && done) cand[atomicAdd(&count, 1)] = {score, static_cast<uint64_t>(b) << 32 | static_cast<uint64_t>(a.pad)};
+      if (finite && done) cand[atomicAdd(&count, 1)] = {order_of(score), static_cast<uint64_t>(b) << 32 | static_cast<uint64_t>(a.pad)};
     }
   }
   __syncthreads();
-  const auto get = [&](int i) {                  // candidate i, whose score is -inf where there is none
+  const auto get = [&](int i) {                  // candidate i, of score 0 where there is none
     const int b = i / per;
     const uint64_t key = keys[i];
-    Candidate c = {-INFINITY, ~uint64_t{0}};
+    Candidate c = {0, ~uint64_t{0}};
     if (lse[b] == lse[b] && key != 0) {
-      c.score = given[b] + (static_cast<double>(key_logit(key)) - lse[b]);
+      c.score = order_of(given[b] + (static_cast<double>(key_logit(key)) - lse[b]));
       c.place = static_cast<uint64_t>(b) << 32 | key_token(key);
     }
     return c;
   };
-  // the best k-th candidate of a part: none after it is among the k best
-  Candidate bar = {-INFINITY, ~uint64_t{0}};
-  for (int i = tid * a.k + a.k - 1; i < total; i += kJoinThreads * a.k) {
-    const Candidate c = get(i);
+  // Two bounds of the k-th best: the best k-th candidate of a part, and the least of k groups' best firsts (parts i, i + k,
+  // ...). The first is tight where one part has most of the best, the second where they are spread.
+  const int lists = a.B * a.parts;
+  Candidate bar = {0, ~uint64_t{0}};
+  for (int i = tid; i < lists; i += kJoinThreads) {
+    const Candidate c = get(i * a.k + a.k - 1);
     if (before(c, bar)) bar = c;
+  }
+  uint64_t least = ~uint64_t{0};                 // of this warp's groups
+  for (int j = warp; j < a.k; j += kJoinThreads / 32) {
+    uint64_t best = 0;
+    for (int i = j + a.k * lane; i < lists; i += 32 * a.k) best = max(best, get(i * a.k).score);
+    least = min(least, warp_max(best));
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const Candidate c = {__shfl_xor_sync(0xffffffffu, bar.score, o), __shfl_xor_sync(0xffffffffu, bar.place, o)};
     if (before(c, bar)) bar = c;
   }
-  if (lane == 0) bound[warp] = bar;
+  if (lane == 0) bound[warp] = bar, group[warp] = least;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kJoinThreads / 32; ++w)
+  for (int w = 0; w < kJoinThreads / 32; ++w) {
     if (before(bound[w], bar)) bar = bound[w];
+    least = min(least, group[w]);
+  }
   for (int i = tid; i < total; i += kJoinThreads) {
     const Candidate c = get(i);
-    if (c.score > -INFINITY && !before(bar, c)) cand[atomicAdd(&count, 1)] = c;
+    if (c.score != 0 && c.score >= least && !before(bar, c)) cand[atomicAdd(&count, 1)] = c;
   }
   __syncthreads();
-  const int n = count;
-  for (int i = tid; i < n; i += kJoinThreads) {
-    const Candidate c = cand[i];
-    int rank = 0;
+  // a candidate's place: those before it, counted by kJoinThreads / kRanked threads
+  const int n = count, sharer = tid / kRanked;
+  for (int i0 = 0; i0 < n; i0 += kRanked) {
+    const int i = i0 + tid % kRanked;
+    if (tid < kRanked) rank[tid] = 0;
+    __syncthreads();
+    if (i < n) {
+      const Candidate c = cand[i];
+      int r = 0;
 #pragma unroll 4
-    for (int j = 0; j < n; ++j) rank += before(cand[j], c);
-    if (rank < a.k) {
-      a.out_scores[g * a.k + rank] = static_cast<float>(c.score);
-      a.out_parents[g * a.k + rank] = static_cast<int32_t>(c.place >> 32);
-      a.out_tokens[g * a.k + rank] = static_cast<int64_t>(c.place & 0xFFFFFFFFu);
+      for (int j = sharer; j < n; j += kJoinThreads / kRanked) r += before(cand[j], c);
+      if (r > 0) atomicAdd(&rank[tid % kRanked], r);
     }
+    __syncthreads();
+    if (tid < kRanked && i < n && rank[tid] < a.k) {
+      const Candidate c = cand[i];
+      const int64_t at = g * a.k + rank[tid];
+      a.out_scores[at] = static_cast<float>(score_of(c.score));
+      a.out_parents[at] = static_cast<int32_t>(c.place >> 32);
+      a.out_tokens[at] = static_cast<int64_t>(c.place & 0xFFFFFFFFu);
+    }
+    __syncthreads();
   }
   for (int i = n + tid; i < a.k; i += kJoinThreads) {
     a.out_scores[g * a.k + i] = -INFINITY;

@@ -16,11 +16,14 @@ constexpr int kMoveThreads = 256;
 constexpr int kMovePieces = 8;                         // 16-byte pieces a thread
 constexpr int kMoveRows = 64;                          // rows of a group
 
+// Kernel parameters are copied at every launch: few views come in a small table.
+template <int V>
 struct MoveTable {
-  MoveView v[kMoveViews];
+  MoveView v[V];
 };
 
-__global__ void __launch_bounds__(kMoveThreads) move_rows_kernel(const __grid_constant__ MoveTable table,
+template <int V>
+__global__ void __launch_bounds__(kMoveThreads) move_rows_kernel(const __grid_constant__ MoveTable<V> table,
                                                                  const __grid_constant__ MoveArgs a) {
   __shared__ int32_t ids[2][kMoveRows];
   __shared__ int32_t moved;
@@ -93,7 +96,7 @@ int launch_move_rows(const MoveView* views, const MoveArgs& a_in, cudaStream_t s
   int rows = 1;
   while (rows < a.n) rows *= 2;
   a.slice = kMoveThreads * kMovePieces * 16 / rows;
-  MoveTable t = {};
+  MoveTable<kMoveViews> t;
   int64_t items = 0;
   for (int i = 0; i < a.views; ++i) {
     const MoveView& v = views[i];
@@ -108,7 +111,14 @@ int launch_move_rows(const MoveView* views, const MoveArgs& a_in, cudaStream_t s
     items += slices * a.groups;
     if (items > 0x7fffffff) return kErrArgs;
   }
-  move_rows_kernel<<<static_cast<unsigned>(items), kMoveThreads, 0, stream>>>(t, a);
+  constexpr int kFew = 8;
+  if (a.views <= kFew) {
+    MoveTable<kFew> few;
+    for (int i = 0; i < a.views; ++i) few.v[i] = t.v[i];
+    move_rows_kernel<<<static_cast<unsigned>(items), kMoveThreads, 0, stream>>>(few, a);
+  } else {
+    move_rows_kernel<<<static_cast<unsigned>(items), kMoveThreads, 0, stream>>>(t, a);
+  }
   return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
 }
 

@@ -99,6 +99,9 @@ class RowMover:
         if not 1 <= len(self.views) <= MOVE_VIEWS or len(lists) != len(self.views) or min(lists) < 0:
             raise ValueError(f"{len(self.views)} views (1..{MOVE_VIEWS}) with lists {lists}")
         self.lists = max(lists) + 1
+        self._move = lib.load().ssb_move_rows
+        if any(t.get_device() != self.views[0].get_device() for t in self.views):
+            raise ValueError("the views must be on one device")
         self._c = (lib.MoveViewC * len(self.views))()
         for i, t in enumerate(self.views):
             size = t.element_size()
@@ -117,18 +120,15 @@ class RowMover:
         may go to several rows; an entry with a negative id or equal ids moves nothing, of entries with one destination
         the first counts. A row that one group writes must not occur in another group of its list. `status` (int32 [1] on
         the device) receives 1 for an id past a view's rows (nothing is moved for it there)."""
-        so = lib.load()
-        for name, t in (("src", src), ("dst", dst)):
-            if t.dtype is not torch.int32 or not t.is_contiguous() or t.shape != src.shape or \
-                    not (t.dim() == 3 and t.shape[0] >= self.lists or t.dim() == 2 and self.lists == 1) or \
-                    t.shape[-1] > MOVE_ROWS:
-                raise ValueError(f"{name}: contiguous int32 [{self.lists}, groups, <= {MOVE_ROWS}] like the other, got "
-                                 f"{t.dtype} {tuple(t.shape)}")
-        lib.check_device((src, dst, *self.views), status, stream)
-        n = src.shape[-1]
-        rc = so.ssb_move_rows(self._c, len(self.views), src.data_ptr(), dst.data_ptr(),
-                              1 if src.dim() == 2 else src.shape[0], src.shape[-2], n,
-                              None if status is None else status.data_ptr(), lib.stream_ptr(stream))
+        shape = src.shape
+        lists, groups, n = shape if len(shape) == 3 else (1, *shape) if len(shape) == 2 else (0, 0, 0)
+        if lists < self.lists or n > MOVE_ROWS or src.dtype is not torch.int32 or dst.dtype is not torch.int32 or \
+                dst.shape != shape or not src.is_contiguous() or not dst.is_contiguous():
+            raise ValueError(f"src, dst: contiguous int32 [{self.lists}, groups, <= {MOVE_ROWS}], got {src.dtype} "
+                             f"{tuple(shape)} and {dst.dtype} {tuple(dst.shape)}")
+        lib.check_device((src, dst, self.views[0]), status, stream)
+        rc = self._move(self._c, len(self.views), src.data_ptr(), dst.data_ptr(), lists, groups, n,
+                        None if status is None else status.data_ptr(), lib.stream_ptr(stream))
         lib.check("ssb_move_rows", rc)
 
 

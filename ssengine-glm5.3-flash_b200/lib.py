@@ -11,6 +11,8 @@ import contextlib
 import ctypes
 from pathlib import Path
 
+import torch
+
 PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "libssengine_b200.so"
 
@@ -259,17 +261,20 @@ def stream_scratch(device, nbytes: int, stream=None):
 def check_device(tensors, status=None, stream=None) -> None:
     """ValueError unless the tensors of one call (None: absent), its status word (int32 on the device) and its stream are
     all on one GPU, the current one: a launch takes their addresses as they are."""
-    import torch
-
     dev = tensors[0].get_device()
-    if status is not None and (status.dtype is not torch.int32 or status.numel() < 1):
-        raise ValueError(f"status: int32 [1] on the device, got {status.dtype} {tuple(status.shape)}")
-    for t in (*tensors, status):
+    for t in tensors:
         if t is not None and t.get_device() != dev:
+            raise ValueError("the tensors of one call must be on one device")
+    if status is not None:
+        if status.dtype is not torch.int32 or status.numel() < 1:
+            raise ValueError(f"status: int32 [1] on the device, got {status.dtype} {tuple(status.shape)}")
+        if status.get_device() != dev:
             raise ValueError("the tensors of one call must be on one device")
     if dev < 0:
         raise ValueError(f"the tensors are on {tensors[0].device}, not on a GPU")
     current = torch.cuda.current_device()
+    if stream is None and dev == current:
+        return
     stream_dev = dev if stream is None else getattr(stream, "device_index", dev)
     if dev != current or stream_dev != dev:
         raise ValueError(f"the tensors are on cuda:{dev}, the current device is cuda:{current}" +
@@ -282,8 +287,6 @@ def check(name: str, rc: int) -> None:
 
 
 def stream_ptr(stream=None) -> int:
-    import torch
-
     if stream is None:
         # the current stream's handle itself: building the Stream object costs 4 us a call
         return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
