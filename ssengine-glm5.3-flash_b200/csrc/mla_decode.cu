@@ -78,8 +78,8 @@ constexpr int kOffRing = kOffSlot + 128;        // int4 [8]: the same by unit, a
 constexpr int kOffRef = kOffRing + 128;         // float [64]: the heads' references
 constexpr int kOffRow = kOffRef + 256;          // float [4][64]: maxima and rescale factors, the sums, or maxima of the query
 constexpr int kOffSum = kOffRow + 1024;         // float [64]: bmm2 / l
-constexpr int kOffPlan = kOffSum + 256;         // int32 [52]: the plan's sums and first row
-constexpr int kSmem = kOffPlan + 208;
+constexpr int kOffPlan = kOffSum + 256;         // int32 [76]: the plan's sums, first row and maxima
+constexpr int kSmem = kOffPlan + 304;
 static_assert(kOffSlot % 16 == 0 && kOffRow % 16 == 0 && kOffSf % 128 == 0 && kSmem <= 232448, "shared memory");
 // TMEM columns: O^T as 4 tiles of 128 dims x 64 heads; S of two units, 64 tokens each; the first 480 bytes of the query
 // parts; block scales of V (byte 0, 2^-7, against the high parts of P, byte 1, 2^-11, against the low ones) and of P (2
@@ -344,12 +344,17 @@ constexpr int kRowCost = 10, kCostFrom = 24;      // units; ranges of so many un
 template <bool kTree>
 SSB_DEVICE bool find_range(const MlaDecodeArgs& a, int cta, int ctas, int32_t* sh, Walk& w) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  int units = 0, rows = 0;
+  int units = 0, rows = 0, most = 0;
 #pragma unroll 1
   for (int t = tid; t < a.T; t += kThreads) {
     const int n = row_units<kTree>(a, t);
     units += n;
     rows += n > 0;
+    if (kTree) most = max(most, n);
+  }
+  if (kTree) {
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) sh[52 + warp] = most;
   }
   units = __reduce_add_sync(0xffffffffu, units);
   rows = __reduce_add_sync(0xffffffffu, rows);
@@ -358,7 +363,14 @@ SSB_DEVICE bool find_range(const MlaDecodeArgs& a, int cta, int ctas, int32_t* s
   __syncthreads();
   units = __reduce_add_sync(0xffffffffu, lane < kThreads / 32 ? sh[lane] : 0);
   rows = __reduce_add_sync(0xffffffffu, lane < kThreads / 32 ? sh[24 + lane] : 0);
-  const int spare = max(ctas - rows, 1), per = max((units + spare - 1) / spare, 2);
+  const int spare = max(ctas - rows, 1);
+  int per = max((units + spare - 1) / spare, 2);
+  if (kTree && 0 < rows && rows <= ctas) {
+    // a tree's rows are of one length: floor(ctas / rows) parts of each suffice too (24 rows of 63 units: 11 and not 13)
+    const int each = ctas / rows;
+    most = __reduce_max_sync(0xffffffffu, lane < kThreads / 32 ? sh[52 + lane] : 0);
+    per = max(min(per, (most + each - 1) / each), 2);
+  }
   const bool parts = rows < ctas && per <= units / ctas + kRowCost + kRowCost * rows / ctas;
   w.cost = units < kCostFrom * ctas ? 0 : kRowCost;
   if (parts) {
