@@ -169,11 +169,13 @@ class KdaAttention:
 
     def forward(self, y: torch.Tensor, seqs: torch.Tensor, conv_state: torch.Tensor, rec_state: torch.Tensor,
                 status: torch.Tensor, out: torch.Tensor | None = None, stream=None, keep: bool = False,
-                decode: bool = False) -> torch.Tensor:
+                decode: bool = False, tree: tuple | None = None) -> torch.Tensor:
         """y bf16 [T, H] (the layer input after the boundary's RMSNorm) -> attention output bf16 [T, H]; the KDA state
         blocks of `seqs` (int32 [R, 4] on the device) are updated in place. keep: the intermediates stay in
         `self.parts` (for checks). decode: the recurrence token by token (`KdaLayer.decode`), for a step's few new
-        rows a request, in place of the chunked scan."""
+        rows a request, in place of the chunked scan. tree (parents int32 [T], the largest tree's nodes): the rows are
+        trees of drafted tokens (`KdaLayer.decode_tree`); the state blocks stay as they are, and `self.step` keeps what
+        `accept` needs."""
         T, P, dev = y.shape[0], self.P, self.device
         s = lib.stream_ptr(stream)
         proj = torch.empty(T, self.in_proj.N_pad, dtype=torch.bfloat16, device=dev)
@@ -186,8 +188,13 @@ class KdaAttention:
         ogate = torch.empty(T, P, dtype=torch.bfloat16, device=dev)
         self.g_b(g_a, ogate, status, stream)
         o = torch.empty(T, P, dtype=torch.bfloat16, device=dev)
-        scan = self.kda.decode if decode else self.kda.prefill
-        scan(proj, gate, beta, o, seqs, conv_state, rec_state, stream=stream, status=status)
+        if tree is not None:
+            self.kda.decode_tree(proj, gate, beta, o, seqs, tree[0], conv_state, rec_state, max_nodes=tree[1],
+                                 stream=stream, status=status)
+            self.step = (proj, gate, beta)
+        else:
+            scan = self.kda.decode if decode else self.kda.prefill
+            scan(proj, gate, beta, o, seqs, conv_state, rec_state, stream=stream, status=status)
         if keep:
             self.parts = dict(proj=proj, gate=gate, ogate=ogate, o=o.clone())
         if out is None:
@@ -208,6 +215,11 @@ class KdaAttention:
                                                         sf.data_ptr(), T, self.heads, s))
             self.o_proj.gemm(codes, sf, T, out, status, stream)
         return out
+
+    def accept(self, rows, seqs, conv_state, rec_state, status, stream=None) -> None:
+        """Moves the states on along the accepted rows (int32 [n], `seqs` over places in them) of the last tree."""
+        self.kda.advance(*self.step, rows, seqs, conv_state, rec_state, stream=stream, status=status)
+        self.step = None
 
 
 class MhcBoundary:
@@ -268,9 +280,9 @@ class KdaDecoderLayer:
         self.device = dev
 
     def forward(self, res, x_prev, post_prev, comb_prev, seqs, conv_state, rec_state, status, stream=None,
-                decode: bool = False):
+                decode: bool = False, tree: tuple | None = None):
         """res bf16 [T, 4, H]; x_prev bf16 [T, H] with post_prev fp32 [T, 4] / comb_prev [T, 4, 4] (x_prev None: the
-        first layer of the stage, pre only); decode: `KdaAttention.forward`'s. Returns (res after attention, MoE
+        first layer of the stage, pre only); decode, tree: `KdaAttention.forward`'s. Returns (res after attention, MoE
         rows, post, comb) for the next boundary."""
         T, H, dev = res.shape[0], self.H, self.device
         f32 = dict(dtype=torch.float32, device=dev)
@@ -279,7 +291,7 @@ class KdaDecoderLayer:
         y = torch.empty(T, H, dtype=torch.bfloat16, device=dev)
         self.bound_a(x_prev, res, post_prev, comb_prev, res_a if x_prev is not None else None, post_a, comb_a, y,
                      stream, status=status)
-        x_a = self.attn.forward(y, seqs, conv_state, rec_state, status, stream=stream, decode=decode)
+        x_a = self.attn.forward(y, seqs, conv_state, rec_state, status, stream=stream, decode=decode, tree=tree)
         res_b = torch.empty_like(res)
         post_b, comb_b = torch.empty(T, 4, **f32), torch.empty(T, 4, 4, **f32)
         self.bound_b(x_a, res_a, post_a, comb_a, res_b, post_b, comb_b, y, stream, status=status)
@@ -468,13 +480,15 @@ class DsaAttention:
         decode (form, reqs int32 [T], seq_lens int32 [T]): the attention of a step's few new rows a request (row t's
         request and the tokens that it sees, positions[t] + 1), split over the cache: form "selected" over the
         indexer's tokens as in the prefill (`mla.decode_selected`), "dense" over the whole context (`mla.decode`;
-        the pool keys are inserted, the logits and the top-k are left out)."""
+        the pool keys are inserted, the logits and the top-k are left out). Form "tree" (with a fourth entry, ancestors
+        int64 [T]): trees of drafted tokens behind contexts of seq_lens tokens (`mla.decode_tree`), dense; the pool keys
+        are left alone until `accept`, for which `self.step` keeps their projections."""
         from . import indexer, mla
 
-        form, reqs, seq_lens = decode if decode is not None else (None, None, None)
-        if form not in (None, "selected", "dense"):
+        form, reqs, seq_lens, *words = decode if decode is not None else (None, None, None)
+        if form not in (None, "selected", "dense", "tree"):
             raise ValueError(f"decode form {form!r}")
-        select = form != "dense"
+        select = form not in ("dense", "tree")
         T, dev, s = y.shape[0], self.device, lib.stream_ptr(stream)
         so, QL, L, RP, NH = self._lib, self.q_lora, self.LATENT, self.ROPE, self.HEADS
         bf = dict(dtype=torch.bfloat16, device=dev)
@@ -530,9 +544,11 @@ class DsaAttention:
         if select:
             self.wq_idx.gemm(*qa_q, T, q_idx, status, side)
         self.idx_proj.gemm(*y_q, T, idx, status, side)
-        k_idx, gate = idx[:, :self.IDX_DIM], idx[:, self.IDX_DIM + self.IDX_HEADS:2 * self.IDX_DIM + self.IDX_HEADS]
+        k_idx, gate = self._pool_inputs(idx)
         w = idx[:, self.IDX_DIM:self.IDX_DIM + self.IDX_HEADS]          # bf16 head weights, read in place
-        if self.indexer_fp8:
+        if form == "tree":
+            self.step = idx
+        elif self.indexer_fp8:
             # the logits' common factor (softmax scale x heads^-1/2 = 2^-6) is left out: a power of two, it changes
             # neither the top-k set nor its ties
             if select:
@@ -570,7 +586,9 @@ class DsaAttention:
             if ws is not None and ws.numel() < mla.decode_workspace_bytes(T, NH):
                 ws = None
             common = dict(bmm2=self.k_scale, reqs=reqs, workspace=ws, stream=stream, status=status)
-            if select:
+            if form == "tree":
+                mla.decode_tree(q8, kv_cache, page_table, seq_lens, words[0], bmm1, o_lat, **common)
+            elif select:
                 mla.decode_selected(q8, kv_cache, tok, page_table, bmm1, o_lat, n_idx=4 * self.TOPK + 3,
                                     seq_lens=seq_lens, **common)
             else:
@@ -586,6 +604,20 @@ class DsaAttention:
             self.parts = dict(a=a, qa=qa, kvn=kvn, kv_rows=kv_rows, q=q, q_lat=q_lat, q8=q8, q_idx=q_idx,
                               idx=idx, w=w, logits=logits, ids=ids, tok=tok, o_lat=o_lat, v=v, o_in=o_in)
         return out
+
+
+    def _pool_inputs(self, idx):
+        """The keys and gates of the indexer's pools in the rows of its projection."""
+        return idx[:, :self.IDX_DIM], idx[:, self.IDX_DIM + self.IDX_HEADS:2 * self.IDX_DIM + self.IDX_HEADS]
+
+    def accept(self, rows, kpool_reqs, max_rows, page_table, pool_cache, tail_ring, stream=None) -> None:
+        """Inserts the accepted rows (int64 [n]) of the last tree into the pool keys: kpool_reqs int32 [R, 4] {first place,
+        places, start position, tail block} over the places in `rows`."""
+        from . import indexer
+
+        idx, self.step = self.step[rows], None
+        insert = indexer.kpool_insert_fp8 if self.indexer_fp8 else indexer.kpool_insert
+        insert(*self._pool_inputs(idx), self.ape, kpool_reqs, max_rows, page_table, pool_cache, tail_ring, stream)
 
 
 class DsaDecoderLayer:

@@ -13,7 +13,9 @@ Mirrors ssengine/model/stage.py:216-762 of the reference and its contract in sse
   chunk order; enqueues GPU work only, a fresh output per call;
 - `forward(plan, hidden_in) = run(prepare(plan), hidden_in)`; `tier_ranges()`;
 - `decode(plan, hidden_in)`: the same forward for a step of few new tokens a request (one, or a draft of several),
-  through the layers' decode forms: the KDA recurrence token by token, the DSA attention split over the cache.
+  through the layers' decode forms: the KDA recurrence token by token, the DSA attention split over the cache;
+- `verify(plan, trees, hidden_in)` and `accept(paths)`: a step of trees of drafted tokens, checked at once, and the
+  requests' continuation by a path of each.
 
 Layer kinds (`StageConfig.layer_kind`):
 - "hybrid": the Glm5Next split, decoder layers on the 4-stream mHC residual, DSA + MoE at layers 3, 7, ..., KDA + MoE
@@ -151,6 +153,74 @@ class Batch:
     tier_ops: list = field(default_factory=list)   # the plan's DRAM tier copies, applied before its forward
 
 
+class Trees:
+    """The trees of one `StageModel.verify`: a plan's chunks with their parents, checked on the host, and the device tensors
+    of its rows (chunk by chunk in the plan's order: all are decode-class)."""
+
+    def __init__(self, chunks, trees, batch: Batch, device):
+        from . import mla
+
+        if len(trees) != len(chunks):
+            raise ValueError(f"{len(trees)} trees for {len(chunks)} chunks")
+        self.chunks, self.device = list(chunks), device
+        self.trees = [[int(p) for p in t] for t in trees]
+        masks, depths = [], []
+        for c, t in zip(self.chunks, self.trees):
+            if len(t) != c.num_tokens:
+                raise ValueError(f"chunk {c.req_id}: a tree of {len(t)} nodes for {c.num_tokens} tokens")
+            m, d = mla.tree_masks(t)
+            masks.append(m)
+            depths.append(d + c.start)
+        self.first = np.cumsum([0] + [len(t) for t in self.trees])
+        self.most = max([len(t) for t in self.trees] + [1])
+        n = int(self.first[-1])
+        assert batch.order == list(range(len(self.chunks)))
+        ids = np.repeat(np.arange(len(self.chunks)), [len(t) for t in self.trees])
+        host = np.stack([np.fromiter((p for t in self.trees for p in t), np.int64, n), ids,
+                         np.array([c.start for c in self.chunks], np.int64)[ids]]).astype(np.int32)
+        dev = self._up(torch.from_numpy(host))
+        self.parents, self.reqs, self.context = dev[0], dev[1], dev[2]
+        # a node's place in the cache is its number behind the context, its position its depth
+        both = self._up(torch.cat([torch.cat(masks), torch.cat(depths)]) if masks else torch.zeros(0, dtype=torch.int64))
+        self.ancestors = both[:n]
+        if batch.dsa is not None:
+            batch.dsa["positions"] = both[n:]
+        batch.last_rows = torch.arange(n, dtype=torch.int64, device=device)
+        self.page_table = None if batch.dsa is None else batch.dsa["page_table"]
+
+    def _up(self, t: torch.Tensor) -> torch.Tensor:
+        return t.pin_memory().to(self.device, non_blocking=True) if self.device.type == "cuda" else t
+
+    def accepted(self, paths) -> dict | None:
+        """The device tensors of `StageModel.accept` for a path of each tree (None: nothing accepted). ValueError if one is
+        not a path from a root down."""
+        paths = [[int(v) for v in p] for p in paths]
+        if len(paths) != len(self.trees):
+            raise ValueError(f"{len(paths)} paths for {len(self.trees)} trees")
+        for c, t, p in zip(self.chunks, self.trees, paths):
+            for above, node in zip([-1] + p, p):
+                if not 0 <= node < len(t) or t[node] != above:
+                    raise ValueError(f"chunk {c.req_id}: {p} is not a path of its tree")
+        most = max([len(p) for p in paths] + [0])
+        if most == 0:
+            return None
+        ends = np.cumsum([0] + [len(p) for p in paths])
+        rows = np.concatenate([self.first[r] + np.array(p, np.int64) for r, p in enumerate(paths)])
+        seqs = np.empty((5, len(paths), 4), np.int32)
+        kpool = np.empty((len(paths), 4), np.int32)
+        src, dst = (np.full((len(paths), most), -1, np.int32) for _ in range(2))
+        for r, (c, p) in enumerate(zip(self.chunks, paths)):
+            seqs[:, r] = [(ends[r], ends[r + 1], b, int(c.start > 0)) for b in c.state_blocks[:5]]
+            kpool[r] = (ends[r], len(p), c.start, c.state_blocks[5])
+            pages = np.asarray(c.kv_pages, np.int64)
+            slot = lambda pos: pages[pos // PAGE_TOKENS] * PAGE_TOKENS + pos % PAGE_TOKENS
+            src[r, :len(p)] = slot(c.start + np.array(p, np.int64))
+            dst[r, :len(p)] = slot(c.start + np.arange(len(p)))
+        up = lambda a: self._up(torch.from_numpy(np.ascontiguousarray(a)))
+        return dict(rows=up(rows.astype(np.int32)), rows64=up(rows), seqs=up(seqs), kpool=up(kpool), most=most, src=up(src),
+                    dst=up(dst))
+
+
 class _Pack:
     """Arrays of one microbatch in one pinned host buffer, copied to the device with one stream-ordered copy."""
 
@@ -250,6 +320,7 @@ class StageModel:
         self.cuda_graphs = cfg.cuda_graphs if cuda_graphs is None else cuda_graphs
         self.ipc_kv = ipc_kv
         self.layer_hook = None          # optional callable(layer, res, x_prev, post, comb) after each layer (checks)
+        self.trees = None               # the trees of the last `verify`, until `accept`
         self.moe_profile = None         # optional list: each MoE layer's forward records per-step CUDA events into it
         self._lib = lib.load()
         H, F, E = cfg.hidden, cfg.inter, cfg.experts
@@ -439,16 +510,16 @@ class StageModel:
                      tier_ops=list(getattr(plan, "tier_ops", None) or []))
 
     def run(self, batch: Batch, hidden_in: torch.Tensor | None, edge_out=None,
-            decode: str | None = None) -> torch.Tensor | None:
+            decode: str | None = None, tree: "Trees | None" = None) -> torch.Tensor | None:
         """edge_out: a device address, or a callable returning one when called right before the last kernel (the
         next stage's receive slot, a peer pointer), into which a non-last hybrid stage's final boundary kernel stores
         its [T, 4H] rows directly (the fused stage edge); the call then returns None. Without it the rows come back as
         a fresh tensor (the reference's contract). decode: None, or the layers' decode form ("selected" or "dense",
-        `decode` below)."""
+        `decode` below); tree: the step's trees (`verify` below)."""
         if decode not in (None, "selected", "dense"):
             raise ValueError(f"decode form {decode!r}")
         if self.kda:
-            return self._run_kda(batch, hidden_in, edge_out, decode)
+            return self._run_kda(batch, hidden_in, edge_out, decode, tree)
         T, H = batch.num_tokens, self.hidden_width
         s = lib.stream_ptr()
         if self.first:
@@ -465,7 +536,8 @@ class StageModel:
             return x
         return self._head(x, batch.last_rows)
 
-    def _run_kda(self, batch: Batch, hidden_in: torch.Tensor | None, edge_out=None, decode: str | None = None):
+    def _run_kda(self, batch: Batch, hidden_in: torch.Tensor | None, edge_out=None, decode: str | None = None,
+                 tree: "Trees | None" = None):
         """KDA + MoE decoder layers on the 4-stream residual: stage 0 expands its embeddings (hc_expand), a later stage
         starts from the received residual with a pre-only boundary (edge_recv); a stage that is not the last ends with
         a post-only boundary into the [T, 4H] rows it sends (edge_send, ssengine/model/pp_patch.py:156-163); the last
@@ -489,6 +561,8 @@ class StageModel:
             rows = torch.arange(T, dtype=torch.int32, device=self.device)
             reqs = torch.searchsorted(batch.dsa["qsl"], rows, right=True, out_int32=True) - 1
             step = (decode, reqs, (batch.dsa["positions"] + 1).to(torch.int32))
+        if tree is not None and batch.dsa is not None:
+            step = ("tree", tree.reqs, tree.context, tree.ancestors)
         for layer in self.layers:
             layer.moe_profile = self.moe_profile
         for layer, state, dsa, grp in zip(self.layers, self.kda_states, self.is_dsa, self.kda_group):
@@ -497,7 +571,8 @@ class StageModel:
                                                         decode=step)
             else:
                 res, x_prev, post, comb = layer.forward(res, x_prev, post, comb, batch.kda_seqs[grp], *state,
-                                                        self.status, decode=decode is not None)
+                                                        self.status, decode=decode is not None,
+                                                        tree=None if tree is None else (tree.parents, tree.most))
             if self.layer_hook is not None:
                 self.layer_hook(layer, res, x_prev, post, comb)
         if edge_out is not None and not self.last and x_prev is not None:
@@ -535,6 +610,39 @@ class StageModel:
         (attention "selected") or `mla.decode` over the whole context ("dense", the indexer's pool keys kept up to
         date). Chunks of any length are right; the chunked forms of `forward` are faster for long ones."""
         return self.run(self.prepare(plan), hidden_in, decode=attention)
+
+    def verify(self, plan, trees, hidden_in: torch.Tensor | None = None, edge_out=None) -> torch.Tensor | None:
+        """One step of trees of drafted tokens, checked at once: a plan whose chunks hold a tree each (token_ids its nodes'
+        tokens, num_tokens its nodes, at most 64, kv_pages for all of them behind the context) and `trees`, each chunk's
+        parents (a parent before its children, -1: the context's last token). Every node is computed as if its path followed
+        the context: `KdaLayer.decode_tree` in the KDA layers, `mla.decode_tree` (over the whole context) in the DSA layers.
+        Returns what `forward` returns, the last stage the greedy token after every node, in the plan's order (`last_logits`
+        its logits). The requests' states and pool keys stay as they are until `accept`, which comes before the stage's
+        next step of these requests; a second `verify` in its place checks other trees."""
+        if not self.kda:
+            raise ValueError('layer_kind "moe" has no requests to continue')
+        batch = self.prepare(plan)
+        self.trees = Trees(plan.chunks, trees, batch, self.device)
+        return self.run(batch, hidden_in, edge_out, tree=self.trees)
+
+    def accept(self, paths) -> None:
+        """Continues the requests of the last `verify` by a path of each tree (the nodes from a root down, () for none): the
+        KDA states advance along it (`KdaLayer.advance`), its latent rows move up to the context's end
+        (`StageKv.move_tokens`), its pool keys are inserted. Every stage of a pipeline takes the same paths."""
+        t = self.trees
+        if t is None:
+            raise ValueError("no trees to accept a path of")
+        acc = t.accepted(paths)
+        self.trees = None
+        if acc is None:
+            return
+        for layer, state, dsa, grp in zip(self.layers, self.kda_states, self.is_dsa, self.kda_group):
+            if dsa:
+                layer.attn.accept(acc["rows64"], acc["kpool"], acc["most"], t.page_table, state[1], state[2])
+            else:
+                layer.attn.accept(acc["rows"], acc["seqs"][grp], *state, self.status)
+        if any(self.is_dsa):
+            self.kv.move_tokens(acc["src"], acc["dst"], status=self.status)
 
     def tier_ranges(self) -> list:
         """Byte ranges (device pointer, bytes) of the stage's KV and state tensors for the capacity tiers: every

@@ -1,0 +1,70 @@
+"""`stage.Trees` on the host: the checks of a plan's trees and of the accepted paths, and the tables made of them."""
+
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+
+def trees_of(parents, starts=(5, 130), device="cpu", dsa=True):
+    from ssengine_b200.messages import Chunk
+    from ssengine_b200.stage import Trees
+
+    chunks = [Chunk(f"r{i}", s, len(p), [70 + 10 * i, 71 + 10 * i], [10 * i + g for g in range(1, 7)], True, [0] * len(p))
+              for i, (s, p) in enumerate(zip(starts, parents))]
+    batch = SimpleNamespace(order=list(range(len(chunks))), last_rows=None,
+                            dsa=dict(positions=None, page_table=torch.zeros(2, 2, dtype=torch.int32)) if dsa else None)
+    return Trees(chunks, parents, batch, torch.device(device)), batch
+
+
+def test_rows_of_the_trees():
+    t, batch = trees_of([[-1, 0, 0, 2], [-1, -1, 1]])
+    assert t.parents.tolist() == [-1, 0, 0, 2, -1, -1, 1] and t.reqs.tolist() == [0, 0, 0, 0, 1, 1, 1]
+    assert t.context.tolist() == [5] * 4 + [130] * 3 and t.ancestors.tolist() == [1, 3, 5, 13, 1, 2, 6]
+    assert batch.dsa["positions"].tolist() == [5, 6, 6, 7, 130, 130, 131] and batch.last_rows.tolist() == list(range(7))
+    assert t.most == 4 and t.parents.dtype == torch.int32 and t.ancestors.dtype == torch.int64
+
+
+def test_accepted_tables():
+    t, _ = trees_of([[-1, 0, 0, 2], [-1, -1, 1]], starts=(126, 0))
+    a = t.accepted([[0, 2, 3], [1]])
+    assert a["rows"].tolist() == [0, 2, 3, 5] and a["rows64"].tolist() == [0, 2, 3, 5] and a["most"] == 3
+    assert a["kpool"].tolist() == [[0, 3, 126, 6], [3, 1, 0, 16]]
+    for g in range(5):
+        assert a["seqs"][g].tolist() == [[0, 3, 1 + g, 1], [3, 4, 11 + g, 0]]
+    assert a["src"].tolist() == [[70 * 128 + 126, 71 * 128 + 0, 71 * 128 + 1], [80 * 128 + 1, -1, -1]]
+    assert a["dst"].tolist() == [[70 * 128 + 126, 70 * 128 + 127, 71 * 128], [80 * 128, -1, -1]]
+    assert t.accepted([[], []]) is None
+    assert t.accepted([(), (0,)])["rows"].tolist() == [4]
+
+
+@pytest.mark.parametrize("paths", [
+    [[0]], [[0], [0], []], [[1], []], [[0, 3], []], [[0, 2, 2], []], [[4], []], [[-1], []], [[0], [0, 2]],
+])
+def test_what_is_no_path_is_refused(paths):
+    t, _ = trees_of([[-1, 0, 0, 2], [-1, -1, 1]])
+    with pytest.raises(ValueError):
+        t.accepted(paths)
+
+
+@pytest.mark.parametrize("parents", [[[-1, 1], [-1]], [[0], [-1]], [[-1], list(range(-1, 64))]])
+def test_what_is_no_tree_is_refused(parents):
+    with pytest.raises(ValueError):
+        trees_of(parents)
+
+
+def test_a_tree_of_another_length_and_nothing_to_accept_are_refused():
+    from ssengine_b200.messages import Chunk
+    from ssengine_b200.stage import StageModel, Trees
+
+    batch = SimpleNamespace(order=[0], last_rows=None, dsa=None)
+    with pytest.raises(ValueError):
+        Trees([Chunk("a", 0, 3, [1], [0] * 6, True, None)], [[-1, 0]], batch, torch.device("cpu"))
+    with pytest.raises(ValueError):
+        Trees([Chunk("a", 0, 1, [1], [0] * 6, True, None)], [[-1], [-1]], batch, torch.device("cpu"))
+    st = object.__new__(StageModel)
+    st.trees, st.kda = None, False
+    with pytest.raises(ValueError):
+        st.accept([[0]])
+    with pytest.raises(ValueError):
+        st.verify(None, [])
