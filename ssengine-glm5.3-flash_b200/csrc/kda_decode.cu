@@ -135,23 +135,23 @@ __global__ void __launch_bounds__(kDecThreads, 2) kda_decode_kernel(const __grid
       o.x = exp_fast(a.lower_bound * sigmoid_fast(rate * (g.x + dt.x)));
       o.y = exp_fast(a.lower_bound * sigmoid_fast(rate * (g.y + dt.y)));
     }
-    *reinterpret_cast<float2*>(y + part * kDim + 2 * pair) = o;
+    if (!kAdvance || part > 0) *reinterpret_cast<float2*>(y + part * kDim + 2 * pair) = o;
     const float b = sigmoid_fast(beta);
     if (t + 1 < e) {                                     // the next token's inputs, behind this one's arithmetic
       raw = __ldg(in + row_of(t + 1) * pitch);
       beta = __bfloat162float(a.beta[row_of(t + 1) * a.ldb + h]);
     }
     __syncthreads();
-    const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(y + 4 * lane);
+    const ulonglong2 q = kAdvance ? make_ulonglong2(0, 0) : *reinterpret_cast<const ulonglong2*>(y + 4 * lane);
     const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(y + kDim + 4 * lane);
     const ulonglong2 dec = *reinterpret_cast<const ulonglong2*>(y + 3 * kDim + 4 * lane);
     float nq = sum2(fma2(q.y, q.y, mul2(q.x, q.x))), nk = sum2(fma2(k.y, k.y, mul2(k.x, k.x)));
     float nd = sum2(fma2(q.y, k.y, mul2(q.x, k.x)));
 #pragma unroll
     for (int o2 = 16; o2 > 0; o2 >>= 1) {
-      nq += __shfl_xor_sync(0xffffffffu, nq, o2);
+      if constexpr (!kAdvance) nq += __shfl_xor_sync(0xffffffffu, nq, o2);
       nk += __shfl_xor_sync(0xffffffffu, nk, o2);
-      nd += __shfl_xor_sync(0xffffffffu, nd, o2);
+      if constexpr (!kAdvance) nd += __shfl_xor_sync(0xffffffffu, nd, o2);
     }
     const float rq = a.scale * rsqrtf(nq + 1e-6f), rk = rsqrtf(nk + 1e-6f);
     float d[kAdvance ? kRowsW : 2 * kRowsW];             // of row i: S k at i, S q at 16 + i (k, q not yet normalised)
