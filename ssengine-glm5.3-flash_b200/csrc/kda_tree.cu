@@ -524,6 +524,7 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
     int base[kWords];                                          // of the node's M
 #pragma unroll
     for (int c = 0; c < kWords; ++c) {
+      if (c > 0 && 16 * c >= most) break;
       const int m = (nodes[t] >> (8 * c)) & 0xFF;
       const bool have = 16 * c + l < len;
       x[c] = have ? sm.pn[at + 16 * c + l] : 0.0f;
@@ -538,8 +539,10 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
         const float y = __shfl_sync(0xffffffffu, x[c] * b[c], d, 16);
         const float* pm = sm.pm + __shfl_sync(0xffffffffu, base[c], d, 16) + l - d - 1;
 #pragma unroll
-        for (int e = c; e < kWords; ++e)
+        for (int e = c; e < kWords; ++e) {
+          if (16 * e >= most) break;
           if (16 * e + l > 16 * c + d && 16 * e + l < len) x[e] = fmaf(-y, pm[16 * (e - c)], x[e]);
+        }
       }
     }
 #pragma unroll
