@@ -131,8 +131,8 @@ SSB_DEVICE void mma_f16_ta(uint32_t d, uint32_t a, uint64_t bd, uint32_t idesc, 
       : "memory");
 }
 
-SSB_DEVICE void cp_async4(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+SSB_DEVICE void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 SSB_DEVICE void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
@@ -202,12 +202,14 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
   const __nv_bfloat16* cs = a.conv_state + (int64_t)sq.z * a.cs_stride + h * kDim;            // of q; k, v: + P, + 2 P
   bool bad = false;
   if (part < kGroups - 1) {
-    const uint32_t* in = reinterpret_cast<const uint32_t*>(a.x + h * kDim + 2 * pair) + s * (a.ldx / 2);
+    const uint32_t* q = reinterpret_cast<const uint32_t*>(a.x + h * kDim + 2 * pair) + (s + part) * (a.ldx / 2);
+    const uint32_t* k = q + a.P / 2;
+    const int64_t step = (kGroups - 1) * (a.ldx / 2);
+    uint32_t to = smem_u32(&sm.in[part][0][pair]);
 #pragma unroll 2
-    for (int i = part; i < n; i += kGroups - 1) {
-      const uint32_t* x = in + i * (a.ldx / 2);
-      cp_async4(&sm.in[i][0][pair], x);
-      cp_async4(&sm.in[i][1][pair], x + a.P / 2);
+    for (int i = part; i < n; i += kGroups - 1, q += step, k += step, to += (kGroups - 1) * 2 * kDim * 2) {
+      cp_async4(to, q);
+      cp_async4(to + kDim * 2, k);
     }
     // kept row part (0: the oldest)
     if (part < 3) {
@@ -266,10 +268,11 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
   // the gates' inputs: a pair of channels of every kGroups-th node a thread
   uint32_t gin[N / kGroups];
   {
-    const uint32_t* in = reinterpret_cast<const uint32_t*>(a.g + h * kDim + 2 * pair) + s * (a.ldg / 2);
+    const uint32_t* in = reinterpret_cast<const uint32_t*>(a.g + h * kDim + 2 * pair) + (s + part) * (a.ldg / 2);
+    const int64_t step = kGroups * (a.ldg / 2);
 #pragma unroll
-    for (int t = 0; t < N / kGroups; ++t)
-      if (part + kGroups * t < n) gin[t] = __ldg(in + (part + kGroups * t) * (a.ldg / 2));
+    for (int t = 0; t < N / kGroups; ++t, in += step)
+      if (part + kGroups * t < n) gin[t] = __ldg(in);
   }
   // the conv's weights of q and k and the gates' parameters
   const uint4 wq = __ldg(reinterpret_cast<const uint4*>(a.conv_w + ((int64_t)h * kDim + 2 * pair) * 4));
@@ -462,9 +465,12 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
     __syncthreads();
     // the decays' place is free: P's zeros, the values' inputs
     for (int c = tid; c < 2 * N * 128 / 16; c += C::kThreads) reinterpret_cast<uint4*>(sm.p)[c] = make_uint4(0, 0, 0, 0);
-    const uint32_t* in = reinterpret_cast<const uint32_t*>(a.x + 2 * (int64_t)a.P + h * kDim + 2 * pair) + s * (a.ldx / 2);
-#pragma unroll 4
-    for (int i = part; i < n; i += kGroups) cp_async4(&sm.vin[i][pair], in + i * (a.ldx / 2));
+    const uint32_t* in =
+        reinterpret_cast<const uint32_t*>(a.x + 2 * (int64_t)a.P + h * kDim + 2 * pair) + (s + part) * (a.ldx / 2);
+    const int64_t step = kGroups * (a.ldx / 2);
+    uint32_t to = smem_u32(&sm.vin[part][pair]);
+#pragma unroll 2
+    for (int i = part; i < n; i += kGroups, in += step, to += kGroups * kDim * 2) cp_async4(to, in);
     const int granule = l >> 1, within = (l & 1) * 8;
 #pragma unroll
     for (int t = 0; t < kOwn; ++t) {
@@ -636,15 +642,15 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
   if (ok) ok = mbar_wait(bar(2), 0, &sm.abort, a.status);
   if (!__syncthreads_or(!ok)) {
     tc_fence_after();
-    __nv_bfloat16* out = a.out + (int64_t)s * a.ldo + h * kDim + v;
+    __nv_bfloat16* out = a.out + (int64_t)(s + kShare * fourth) * a.ldo + h * kDim + v;
 #pragma unroll 1
     for (int c = kShare * fourth; c < min(kShare * (fourth + 1), n); c += 8) {
       float z[8];
       tmem_ld_x8(tmem + rows + kColD + N + c, z);
       tmem_ld_wait();
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (c + j < n) out[(c + j) * a.ldo] = __float2bfloat16(z[j]);
+      for (int j = 0; j < 8; ++j, out += a.ldo)
+        if (c + j < n) *out = __float2bfloat16(z[j]);
     }
   } else {
     // products may still be on their way
