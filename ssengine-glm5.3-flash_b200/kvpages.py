@@ -104,10 +104,15 @@ class RowMover:
             raise ValueError("the views must be on one device")
         self._c = (lib.MoveViewC * len(self.views))()
         for i, t in enumerate(self.views):
-            size = t.element_size()
-            if t.dim() < 1 or t.shape[0] < 1 or not t[0].is_contiguous():
-                raise ValueError(f"view {i}: rows contiguous in themselves, got {tuple(t.shape)} strides {t.stride()}")
-            nbytes, stride = t[0].numel() * size, t.stride(0) * size
+            shape, strides, row = tuple(t.shape), t.stride(), 1
+            for n, step in zip(shape[:0:-1], strides[:0:-1]):
+                if step != row and n > 1:
+                    row = -1
+                    break
+                row *= n
+            if not shape or shape[0] < 1 or row < 0:
+                raise ValueError(f"view {i}: rows contiguous in themselves, got {shape} strides {strides}")
+            nbytes, stride = row * t.element_size(), strides[0] * t.element_size()
             if nbytes == 0 or nbytes % 16 or t.data_ptr() % 16 or \
                     (t.shape[0] > 1 and (stride % 16 or stride < nbytes)):
                 raise ValueError(f"view {i}: rows of {nbytes} bytes, {stride} apart, at {t.data_ptr() % 16} past a 16-byte "
