@@ -267,30 +267,57 @@ SSB_DEVICE void mbar_arrive_n(uint32_t bar, uint32_t n) {
 // Tree form. Where a row's heads fill half of a tile or less, up to a.group = 64 / H neighbouring rows share one, and with it
 // every unit they read: rows of one request with one context length, cut at multiples of the group. The first of them, which
 // leads, stands for all in the plan; head h of the tile is head h % H of row h / H behind it.
-SSB_DEVICE bool leads(const MlaDecodeArgs& a, int t) {
-  return t % a.group == 0 || a.reqs == nullptr || a.reqs[t] != a.reqs[t - 1] || a.seq_lens[t] != a.seq_lens[t - 1];
-}
+struct TreeRows {                                // where the rows' requests (null: every row its own), contexts and nodes are
+  const int32_t *req, *len;
+  const uint64_t* nodes;
+  SSB_DEVICE TreeRows(const int32_t* r, const int32_t* l, const uint64_t* n) : req(r), len(l), nodes(n) {}
+  SSB_DEVICE explicit TreeRows(const MlaDecodeArgs& a) : req(a.reqs), len(a.seq_lens), nodes(a.ancestors) {}
+  SSB_DEVICE bool leads(const MlaDecodeArgs& a, int t) const {
+    return t % a.group == 0 || req == nullptr || req[t] != req[t - 1] || len[t] != len[t - 1];
+  }
+  // Units up to the end of what the rows see that t leads (0: it leads none, a reqs entry outside the table, or a negative
+  // length). Positions past 2^31 - 2^7 are past any table.
+  SSB_DEVICE int units(const MlaDecodeArgs& a, int t, uint64_t seen) const {
+    if (len[t] < 0 || (req != nullptr && static_cast<uint32_t>(req[t]) >= static_cast<uint32_t>(a.R))) return 0;
+    const int tokens = min(len[t], 0x7fffff00) + 64 - __clzll(static_cast<long long>(seen));
+    return min((tokens + kUnit - 1) / kUnit, kPage / kUnit * a.width);
+  }
+  // By one thread.
+  SSB_DEVICE int units_of(const MlaDecodeArgs& a, int t) const {
+    if (!leads(a, t)) return 0;
+    uint64_t w = nodes[t];
+    for (int i = 1; i < a.group && t + i < a.T && !leads(a, t + i); ++i) w |= nodes[t + i];
+    return units(a, t, w);
+  }
+};
+// By a whole warp, whose lanes look at the neighbouring rows at once: the row that leads t, the rows that t leads, the nodes
+// that any of those sees, and their units.
 SSB_DEVICE int leader_of(const MlaDecodeArgs& a, int t) {
-  while (!leads(a, t)) --t;
-  return t;
+  const TreeRows R(a);
+  const int lane = threadIdx.x & 31;
+  for (int i = t; true; i -= 32) {
+    const uint32_t m = __ballot_sync(0xffffffffu, i - lane < 0 || R.leads(a, max(i - lane, 0)));
+    if (m != 0) return i - (__ffs(m) - 1);
+  }
 }
 SSB_DEVICE int rows_led(const MlaDecodeArgs& a, int t) {
-  int n = 1;
-  while (n < a.group && t + n < a.T && !leads(a, t + n)) ++n;
-  return n;
+  const TreeRows R(a);
+  const int lane = threadIdx.x & 31;
+  for (int i = 1; true; i += 32) {
+    const int j = i + lane;
+    const uint32_t m = __ballot_sync(0xffffffffu, j >= a.group || t + j >= a.T || R.leads(a, t + j));
+    if (m != 0) return i + __ffs(m) - 1;
+  }
 }
-// The nodes that any of the rows sees that t leads.
 SSB_DEVICE uint64_t nodes_seen(const MlaDecodeArgs& a, int t) {
-  uint64_t w = a.ancestors[t];
-  for (int i = 1; i < a.group && t + i < a.T && !leads(a, t + i); ++i) w |= a.ancestors[t + i];
-  return w;
+  const int lane = threadIdx.x & 31, n = rows_led(a, t);
+  const uint64_t w = (lane < n ? a.ancestors[t + lane] : 0) | (lane + 32 < n ? a.ancestors[t + lane + 32] : 0);
+  return static_cast<uint64_t>(__reduce_or_sync(0xffffffffu, static_cast<uint32_t>(w >> 32))) << 32 |
+         __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(w));
 }
-// The positions before the end of the visible ones of the rows that t leads: the context's and those up to the last node seen
-// (0: a reqs entry outside the table, or a negative length). Positions past 2^31 - 2^7 are past any table.
-SSB_DEVICE int row_tokens(const MlaDecodeArgs& a, int t) {
-  const int len = a.seq_lens[t];
-  if (len < 0 || (a.reqs != nullptr && static_cast<uint32_t>(a.reqs[t]) >= static_cast<uint32_t>(a.R))) return 0;
-  return min(len, 0x7fffff00) + 64 - __clzll(static_cast<long long>(nodes_seen(a, t)));
+SSB_DEVICE int tree_units(const MlaDecodeArgs& a, int t) {
+  const TreeRows R(a);
+  return R.leads(a, t) ? R.units(a, t, nodes_seen(a, t)) : 0;
 }
 
 // ---- the plan -----------------------------------------------------------------------------------------------------
@@ -298,7 +325,7 @@ SSB_DEVICE int row_tokens(const MlaDecodeArgs& a, int t) {
 // by the list's width or, where that is smaller, the tokens it can name.
 template <bool kTree>
 SSB_DEVICE int row_units(const MlaDecodeArgs& a, int t) {
-  if constexpr (kTree) return leads(a, t) ? min((row_tokens(a, t) + kUnit - 1) / kUnit, kPage / kUnit * a.width) : 0;
+  if constexpr (kTree) return tree_units(a, t);            // by a whole warp
   int n = a.indices != nullptr ? a.n_idx : 0x7fffff00;
   if (a.seq_lens != nullptr) n = min(n, a.seq_lens[t]);
   if (a.reqs != nullptr && static_cast<uint32_t>(a.reqs[t]) >= static_cast<uint32_t>(a.R)) n = 0;
@@ -326,7 +353,7 @@ __device__ __noinline__ bool walk_next(const MlaDecodeArgs& a, Walk& w, Segment&
     if (w.nb > 0) w.first += w.nb + w.cost;
     if (++w.t >= a.T) {
       w.first = w.hi;
-    } else {
+    } else if (w.first < w.hi) {                           // looked up where the range goes on
       w.nb = row_units<kTree>(a, w.t);
     }
   }
@@ -341,13 +368,37 @@ constexpr int kRowCost = 10, kCostFrom = 24;      // units; ranges of so many un
 // worst; it is taken where `per` exceeds the equal share by less than those beginnings cost. 34 rows x 1,853 tokens: 38 us
 // in equal ranges, 28 in parts; 62 rows of 2,051 selected tokens: 39 and 35; on the other side 41 rows (median 6,427
 // tokens, 32 heads): 69 and 77; 48 rows (median 4,096, 16 heads): 50 and 59.
+// The tree form's rows are looked at by their neighbours too, one load behind another: up to kPlanRows of them are kept in
+// `room` (shared memory that the units take later) with their units (20 x 12 rows of 16 heads: 71 us without, 63 with).
+constexpr int kPlanRows = 4096;
 template <bool kTree>
-SSB_DEVICE bool find_range(const MlaDecodeArgs& a, int cta, int ctas, int32_t* sh, Walk& w) {
+SSB_DEVICE bool find_range(const MlaDecodeArgs& a, int cta, int ctas, int32_t* sh, uint8_t* room, Walk& w) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int units = 0, rows = 0, most = 0;
+  const bool kept = kTree && a.T <= kPlanRows;
+  uint64_t* nodes = reinterpret_cast<uint64_t*>(room);
+  int32_t* of = reinterpret_cast<int32_t*>(nodes + kPlanRows);           // units, requests, contexts
+  if (kTree && kept) {
+#pragma unroll 1
+    for (int t = tid; t < a.T; t += kThreads) {
+      nodes[t] = a.ancestors[t];
+      of[kPlanRows + t] = a.reqs != nullptr ? a.reqs[t] : t;
+      of[2 * kPlanRows + t] = a.seq_lens[t];
+    }
+    __syncthreads();
+  }
+  const auto units_at = [&](int t) {
+    if constexpr (kTree) {
+      if (kept) return TreeRows(of + kPlanRows, of + 2 * kPlanRows, nodes).units_of(a, t);
+      return TreeRows(a).units_of(a, t);
+    } else {
+      return row_units<false>(a, t);
+    }
+  };
 #pragma unroll 1
   for (int t = tid; t < a.T; t += kThreads) {
-    const int n = row_units<kTree>(a, t);
+    const int n = units_at(t);
+    if (kTree && kept) of[t] = n;
     units += n;
     rows += n > 0;
     if (kTree) most = max(most, n);
@@ -387,7 +438,8 @@ SSB_DEVICE bool find_range(const MlaDecodeArgs& a, int cta, int ctas, int32_t* s
     int base = 0;
 #pragma unroll 1
     for (int c = 0; c < a.T; c += 32) {
-      const int t = c + lane, nb = t < a.T ? row_units<kTree>(a, t) : 0, v = nb == 0 ? 0 : parts ? (nb + per - 1) / per : nb + w.cost;
+      const int t = c + lane, nb = t >= a.T ? 0 : kept ? of[t] : units_at(t);
+      const int v = nb == 0 ? 0 : parts ? (nb + per - 1) / per : nb + w.cost;
       int end = v;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -401,6 +453,7 @@ SSB_DEVICE bool find_range(const MlaDecodeArgs& a, int cta, int ctas, int32_t* s
       if (__any_sync(0xffffffffu, hit)) break;
     }
   }
+  if (kTree) fence_proxy_async_smem();           // the room's next writes may be tiles
   __syncthreads();
   w.t = sh[48], w.nb = sh[49], w.first = sh[50];
   if (w.t < 0) return false;
@@ -521,10 +574,12 @@ __device__ __noinline__ int stage_q(const MlaDecodeArgs& a, uint8_t* smem, uint3
   if (Q8) {
     const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.q) + off);
     const bool keep = have && high;
-#pragma unroll 3
-    for (int j = 0; j < 9; ++j, to += 4) {                            // 16 values
-      const uint4 g = __ldg(q + j);
-      const uint32_t w[4] = {keep ? g.x : 0, keep ? g.y : 0, keep ? g.z : 0, keep ? g.w : 0};
+    uint4 v[9];
+#pragma unroll
+    for (int j = 0; j < 9; ++j) v[j] = __ldg(q + j);                  // 16 values
+#pragma unroll
+    for (int j = 0; j < 9; ++j, to += 4) {
+      const uint32_t w[4] = {keep ? v[j].x : 0, keep ? v[j].y : 0, keep ? v[j].z : 0, keep ? v[j].w : 0};
       keep_q(smem, to, w, part, j);
     }
   } else {
@@ -623,7 +678,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc_fence_before();
   Walk walk;
-  if (!find_range<kTree>(a, cta, gridDim.x, reinterpret_cast<int32_t*>(smem + kOffPlan), walk)) {
+  if (!find_range<kTree>(a, cta, gridDim.x, reinterpret_cast<int32_t*>(smem + kOffPlan), smem + kOffKv, walk)) {
     if (warp == kValueWarp) {
       zero_rows<kTree>(a, cta, h0, nh, lane);
       tmem_dealloc(0, 512);
@@ -647,9 +702,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     while (ok && walk_next<kTree>(a, walk, s)) {
       const int32_t* pages = a.table + (int64_t)(a.reqs != nullptr ? a.reqs[s.t] : s.t) * a.width;
-      const int len = kTree ? row_tokens(a, s.t) : a.seq_lens != nullptr ? a.seq_lens[s.t] : 0x7fffffff;
-      // the tokens all seen; those from there on by the row's word
-      const int plain = kTree ? min(a.seq_lens[s.t], 0x7fffff00) : len;
+      const int len = a.seq_lens != nullptr ? a.seq_lens[s.t] : 0x7fffffff;
+      // the tokens all seen; those from there on by the rows' words
+      const int plain = kTree ? min(len, 0x7fffff00) : len;
       const uint64_t word = kTree ? nodes_seen(a, s.t) : 0;
       const int32_t* idx = a.indices != nullptr ? a.indices + (int64_t)s.t * a.ld_idx : nullptr;
       int c0 = s.b0, c1 = s.b1;
@@ -669,7 +724,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         p = -1;
         if (idx == nullptr) {
           if (c < c1) p = c * kUnit + 32 * half + lane;
-          if (p >= len || (kTree && p >= plain && !(word >> (p - plain) & 1))) p = -1;
+          if (p >= plain && (!kTree || p - plain >= 64 || !(word >> (p - plain) & 1))) p = -1;
           return min(c, c1);
         }
         while (c < c1) {
