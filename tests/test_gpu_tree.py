@@ -206,6 +206,24 @@ def test_long_context_is_split(cuda):
         check(out[t], lse[t], *attention64(q64[t], cache.kv[0][np.r_[0:40001, 40001 + np.array(p)]], BMM1, 1.0))
 
 
+@pytest.mark.parametrize("heads", [2, 16, 64])
+def test_thousands_of_rows(cuda, heads):
+    """More rows than the plan keeps close by (4,096), and one that fills that place to the last row."""
+    rng = np.random.default_rng(heads)
+    lens = [int(n) for n in rng.integers(0, 150, 72)]
+    trees = [wild(rng, 57) for _ in lens]
+    lens[3] = -1                                         # a request whose rows hold nothing
+    cache = Cache(rng, [max(n, 0) + 57 for n in lens])
+    seq, masks, reqs, seen = tree_rows(trees, lens)
+    q, q64 = queries(rng, len(seq), heads, "bf16")
+    for T in (4096, 4104):
+        out, lse, status = call_tree(cuda, q[:T], cache, seq[:T], masks[:T], np.array(reqs[:T], np.int32))
+        assert status == 0 and np.isfinite(out).all()
+        for t in [0, 3 * 57, 4 * 57 - 1, 4095, T - 1] + [int(t) for t in rng.integers(0, T, 40)]:
+            some = seen[t] if lens[reqs[t]] >= 0 else np.zeros(0, np.int64)
+            check(out[t], lse[t], *attention64(q64[t], cache.kv[reqs[t]][some], BMM1, 1.0))
+
+
 def test_missing_pages_and_bad_requests(cuda):
     """A missing page in the tree or past the table leaves its tokens out; a bad request gives zeros and status 1."""
     rng = np.random.default_rng(7)
