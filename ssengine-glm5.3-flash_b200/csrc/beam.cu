@@ -12,7 +12,9 @@
 // join: a CTA a request: the rows' log sums, then every candidate's score in 64 bits (a beam's own candidates keep the order
 //   of their logits, those of different beams are compared at the sums' accuracy). The candidates at or above the best
 //   part's k-th go to shared memory and each finds its place by counting those before it.
-// Bound: HBM, a read of the logits.
+// Bound: HBM, a read of the logits. 64 requests x 8 beams over 151,552 fp32 logits, a fifth of the beams finished: 64 us, 0.75
+// of the copy rate; a row is one part there, and its list work and the rows' uneven ends are not behind other CTAs' loads.
+// One request of 4 beams: 14 us, two launches and a row's parts over the card.
 #include "common.cuh"
 #include "ops.h"
 

@@ -19,6 +19,13 @@
 // row sums (357 us, then against 347); the states through three 64 KB buffers by bulk copies with two groups of warps on
 // every other one (614 us). Runs: each further token costs its arithmetic, little of it beside other CTAs' copies: 24
 // requests x 64 heads 39 us with one token each, 45, 60 and 96 with 2, 4 and 8.
+//
+// The advance (kAdvance) is the same walk for the state alone: 64 requests x 64 heads 94 us with one row each, 101, 124 and
+// 192 with 2, 4 and 8 (decode: 92, 105, 148 and 242), 125 with 1 to 6, 0.70 of the copy rate. What the rows add is the
+// latency of a token's chain (vectors, barrier, row sums, update) with 16 warps an SM, which registers allow: issue slots
+// 34 % in use. Measured against it at 1 to 6 rows: two tokens a step 138 us; 512 threads 152; 8 lanes a row 126; the inputs of
+// 8 tokens ahead in shared memory 123; both, with all vectors before the walk and no barrier in it, 127; CTAs that go from
+// head to head with the next state on its way as a bulk copy 126.
 #include "common.cuh"
 #include "kda_math.cuh"
 #include "ops.h"

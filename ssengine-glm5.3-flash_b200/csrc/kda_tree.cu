@@ -21,6 +21,15 @@
 //   outputs: w by value rows, as the products lie in TMEM, back there as bf16 parts, and W^T P^T onto S (A q) by the tensor
 //       cores, K = nodes.
 // The exponentials are the short ones (error about 2^-20 here): nothing computed here is kept but the bf16 outputs.
+//
+// Bound: not HBM (a head's state is read once, 64 KB, whatever the nodes) but the vectors' arithmetic and the pairs, which
+// are on no tensor core: the decays between two nodes cannot be split into a factor of each without overflow. 48 trees of 32
+// to 64 nodes x 64 heads: 304 us (61 us of bytes), 55,000 warp instructions a CTA (pairs 11,000, conv of q and k 9,000, of v
+// 7,000, decays and norms 9,000, the rest tree, state, scalars and outputs), issue slots 54 % in use, the rest waits for
+// barriers, shared memory and the state. 16 trees of 16 to 32 nodes 66 us (15), one tree of 24 nodes, 32 heads 16 us
+// (latency). Each node's state formed from its parent's, a CTA a head and node after node, took 1,477 us for the first of
+// these; the products on the tensor cores with two CTAs an SM 631; paths as lists 512; outputs as a second product 470; four
+// CTAs an SM up to 32 nodes and 512 threads above 352; a node's scalars by half a warp 317.
 #include "common.cuh"
 #include "kda_math.cuh"
 #include "ops.h"
