@@ -615,7 +615,10 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
     }
   }
   __syncthreads();
-  // ---- w = v - S (A k), as bf16 parts in the place of S; zeros past the nodes, whose columns of P are zeros too
+  // ---- w = v - S (A k), as bf16 parts in the place of S; zeros past the nodes, whose columns of P are zeros too. A w that is
+  // not finite concerns the nodes below its own alone, not those whose weight of it is 0: zero in the product, `lost` (bit j:
+  // the thread's node j's) makes their outputs NaN
+  uint32_t lost = 0;
   if (ok) {
 #pragma unroll 1
     for (int c = kShare * fourth; c < min(kShare * (fourth + 1), N); c += 8) {
@@ -626,6 +629,14 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
       tmem_ld_wait();
 #pragma unroll
       for (int j = 0; j < 8; ++j) w[j] = c + j < n ? w[j] - y[j] : 0.0f;
+      uint64_t odd = 0;                          // 0 but for values that the parts cannot hold
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) odd = fma2(mul2(f2pack(w[j], w[j + 1]), f2pack(1.01f, 1.01f)), 0, odd);
+      if (sum2(odd) != 0.0f) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (!(fabsf(w[j]) < 3.36e38f)) lost |= 1u << (c - kShare * fourth + j), w[j] = 0.0f;
+      }
       uint32_t hi[4], lo[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) split2(w[2 * j], w[2 * j + 1], hi[j], lo[j]);
@@ -635,7 +646,9 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
     tmem_st_wait();
   }
   tc_fence_before();
-  __syncthreads();
+  const bool any_lost = __syncthreads_or(lost != 0);
+  uint32_t* shared_lost = &sm.vin[0][0];                      // [part][value row]
+  if (any_lost) shared_lost[kDim * fourth + v] = lost;
   if (ok && tid == 0) {
     tc_fence_after();
     constexpr uint32_t idesc = idesc_bf16(128, N);
@@ -657,6 +670,12 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
       float z[8];
       tmem_ld_x8(tmem + rows + kColD + N + c, z);
       tmem_ld_wait();
+      if (any_lost) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          for (int at = c + j < n ? c + j : -1; at >= 0; at = sm.parent[at])
+            if (shared_lost[kDim * (at / kShare) + v] >> (at % kShare) & 1) z[j] = NAN;
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j, out += a.ldo)
         if (c + j < n) *out = __float2bfloat16(z[j]);

@@ -400,6 +400,39 @@ def test_extreme_gates(cuda):
     check_rows(out, tree64(d, seqs, trees, H), H)
 
 
+@pytest.mark.parametrize("n", [12, 30, 50])
+@pytest.mark.parametrize("where", ["v", "k", "q", "gate", "beta"])
+def test_what_is_not_finite_reaches_its_descendants_alone(cuda, n, where):
+    """One node's input NaN or infinite: what the recurrence makes NaN is (of a value one channel, of a key, a gate or a beta
+    the head, of a query the node and those whose conv has it), every other output is as if it were not there."""
+    rng = np.random.default_rng(n)
+    H, P = 2, 2 * D
+    trees = [wild(rng, n), STAR(n)]
+    d = kda_make(rng, 2 * n, H, 2)
+    d = {k: (torch.from_numpy(np.ascontiguousarray(v)).to(torch.bfloat16).float().numpy() if k in ("g", "beta", "x") else v)
+         for k, v in d.items()}
+    seqs = [(0, n, 0, 1), (n, 2 * n, 1, 1)]
+    for bad in (np.nan, np.inf):
+        if bad == np.inf and where in ("gate", "beta"):
+            continue                                      # finite there: a decay of e^-5 or 1, a beta of 0 or 1
+        e = {k: np.array(v) for k, v in d.items()}
+        for row in (n // 3, n + 4):
+            if where == "beta":
+                e["beta"][row, 1] = bad
+            elif where == "gate":
+                e["g"][row, D + 17] = bad
+            else:
+                e["x"][row, {"q": 0, "k": 1, "v": 2}[where] * P + D + 17] = bad
+        with np.errstate(all="ignore"):
+            want = tree64(e, seqs, trees, H).reshape(-1, H, D)
+        out, status = run_tree(cuda, e, H, seqs, sum(trees, []))
+        out = out.reshape(-1, H, D)
+        gone = ~np.isfinite(want)
+        assert status == 0 and gone.any() and not gone[:, 0].any() and (~np.isfinite(out) == gone).all()
+        bar = 2.0 ** -8 * np.abs(want) + 1e-3 * np.where(gone, 0, np.abs(want)).max(axis=2, keepdims=True)
+        assert (np.abs(out - want) <= bar)[~gone].all()
+
+
 def test_strided_rows_streams_and_repeats(cuda):
     """Rows cut from wider ones, another stream, the same bits every time and for every max_nodes' form."""
     rng = np.random.default_rng(14)
