@@ -621,9 +621,12 @@ class StageModel:
         next step of these requests; a second `verify` in its place checks other trees."""
         if not self.kda:
             raise ValueError('layer_kind "moe" has no requests to continue')
+        self.trees = None                # a step that fails leaves nothing to accept
         batch = self.prepare(plan)
-        self.trees = Trees(plan.chunks, trees, batch, self.device)
-        return self.run(batch, hidden_in, edge_out, tree=self.trees)
+        step = Trees(plan.chunks, trees, batch, self.device)
+        out = self.run(batch, hidden_in, edge_out, tree=step)
+        self.trees = step
+        return out
 
     def accept(self, paths) -> None:
         """Continues the requests of the last `verify` by a path of each tree (the nodes from a root down, () for none): the

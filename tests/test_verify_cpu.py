@@ -68,3 +68,28 @@ def test_a_tree_of_another_length_and_nothing_to_accept_are_refused():
         st.accept([[0]])
     with pytest.raises(ValueError):
         st.verify(None, [])
+
+
+def test_a_step_that_fails_leaves_nothing_to_accept(monkeypatch):
+    from ssengine_b200.messages import Chunk, Plan
+    from ssengine_b200.stage import StageModel
+
+    st = object.__new__(StageModel)
+    st.trees, st.kda, st.device = None, True, torch.device("cpu")
+    monkeypatch.setattr(st, "prepare", lambda plan: SimpleNamespace(order=[0], last_rows=None, dsa=None), raising=False)
+    monkeypatch.setattr(st, "run", lambda *a, **kw: "rows", raising=False)
+    plan = Plan(0, [Chunk("a", 3, 2, [1], [0] * 6, True, [4, 5])])
+    assert st.verify(plan, [[-1, 0]]) == "rows" and st.trees.trees == [[-1, 0]]
+
+    def failing(*a, **kw):
+        raise RuntimeError("out of memory")
+
+    monkeypatch.setattr(st, "run", failing, raising=False)
+    with pytest.raises(RuntimeError):
+        st.verify(plan, [[-1, -1]])
+    with pytest.raises(ValueError):
+        st.accept([[0]])
+    st.trees = "left over"
+    with pytest.raises(ValueError):
+        st.verify(plan, [[-1, 1]])
+    assert st.trees is None
