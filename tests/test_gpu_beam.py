@@ -203,6 +203,26 @@ def test_captured_selection_follows_its_inputs(cuda):
         check((out[0].double().cpu().numpy(), out[1].long().cpu().numpy(), out[2].cpu().numpy()), select64(hx, hs, k, hf, 0))
 
 
+def test_scores_in_place(cuda):
+    """A search's loop keeps its scores in one tensor: the new ones take the place of those read."""
+    from ssengine_b200 import beam
+
+    rng = np.random.default_rng(31)
+    G, B, V = 150, 8, 4100
+    scores = -rng.random((G, B)).astype(np.float32) * 6
+    finished = rng.random((G, B)) < 0.2
+    x = [rng.standard_normal((G * B, V)).astype(np.float32) * 3 for _ in range(3)]
+    kept = torch.from_numpy(scores).to(cuda)
+    f = torch.from_numpy(finished).to(cuda)
+    out = (kept, torch.empty(G, B, dtype=torch.int32, device=cuda), torch.empty(G, B, dtype=torch.int64, device=cuda))
+    for step in x:
+        before = kept.cpu().numpy()
+        got = beam.select(torch.from_numpy(step).to(cuda), kept, B, finished=f, out=out)
+        torch.cuda.synchronize()
+        assert got[0] is kept
+        check(tuple(t.cpu().numpy() for t in got), select64(step, before, B, finished))
+
+
 def test_no_requests(cuda):
     from ssengine_b200 import beam
 

@@ -35,6 +35,11 @@ def path(parents, i):
     return out[::-1]
 
 
+def wild_tree(n, seed):
+    rng = np.random.default_rng(seed)
+    return [-1] + [int(rng.integers(max(-1, i - 4), i)) for i in range(1, n)]
+
+
 TREES = [[-1, 0, 0, 2, 1, -1, 5, 3], [-1, -1, 0, 1, 3]]
 PROMPTS = [126, 61]
 
@@ -142,3 +147,41 @@ def test_two_stages_verify_as_one(cuda):
         na, nb = na + 1, nb + 1
     for st in (whole, s0, s1):
         assert int(st.status[0]) == 0
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_an_accepted_path_leaves_the_pages_of_its_decode(cuda, fp8):
+    """A stage that begins with its attention layer, given the rows of the layers before it: the path's latent rows, pool keys
+    and tail are those of the same rows decoded one after another, bit for bit."""
+    from ssengine_b200.messages import Chunk, Plan
+    from ssengine_b200.stage import StageModel
+
+    base = dict(layer_split=(3, 1), hidden=512, inter=256, experts=16, top_k=4, num_blocks=14, seed=8, indexer_fp8=fp8)
+    st, ref = (StageModel(cfg(**base), 1, cuda) for _ in range(2))
+    gen = torch.Generator(cuda).manual_seed(3)
+    rows = lambda n: torch.randn(n, st.hidden_width, generator=gen, device=cuda).to(torch.bfloat16)
+    a, b = ([67, 68], [2, 3, 4, 5, 6, 7]), ([69, 70], [8, 9, 10, 11, 12, 13])
+    at = [121, 6]
+    first, x = Plan(0, [Chunk("a", 0, at[0], *a, True, None), Chunk("b", 0, at[1], *b, True, None)]), rows(sum(at))
+    for s in (st, ref):
+        s.forward(first, x)
+    for k, (trees, paths) in enumerate([([wild_tree(20, 1), [-1, -1, 1]], [None, [1, 2]]),
+                                        ([[-1], wild_tree(64, 2)], [[0], None]),
+                                        ([wild_tree(5, 3), [-1, -1]], [[], [1]])]):
+        paths = [path(t, len(t) - 1) if p is None else p for t, p in zip(trees, paths)]
+        x = rows(sum(map(len, trees)))
+        st.verify(Plan(1 + k, [Chunk(n, s, len(t), *r, True, None) for n, s, t, r in zip("ab", at, trees, (a, b))]), trees, x)
+        st.accept(paths)
+        off = len(trees[0])
+        taken = torch.cat([x[paths[0]], x[[off + i for i in paths[1]]]])
+        ref.decode(Plan(1 + k, [Chunk(n, s, len(p), *r, True, None) for n, s, p, r in zip("ab", at, paths, (a, b)) if p]), taken,
+                   attention="dense")
+        at = [s + len(p) for s, p in zip(at, paths)]
+        torch.cuda.synchronize()
+        same = lambda u, v: torch.equal(u.contiguous().view(torch.uint8), v.contiguous().view(torch.uint8))
+        (lat, pool, tail), (lat_r, pool_r, tail_r) = st.kda_states[0], ref.kda_states[0]
+        assert same(pool, pool_r) and same(tail, tail_r)
+        for n, r in zip(at, (a, b)):
+            pages = lambda t: t.view(torch.uint8).view(-1, 128, 576)[r[0]].view(-1, 576)[:n]
+            assert torch.equal(pages(lat), pages(lat_r))
+    assert int(st.status.item()) == 0
