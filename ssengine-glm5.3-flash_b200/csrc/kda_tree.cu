@@ -26,7 +26,7 @@
 // are on no tensor core: the decays between two nodes cannot be split into a factor of each without overflow. 48 trees of 32
 // to 64 nodes x 64 heads: 304 us (61 us of bytes), 55,000 warp instructions a CTA (pairs 11,000, conv of q and k 9,000, of v
 // 7,000, decays and norms 9,000, the rest tree, state, scalars and outputs), issue slots 54 % in use, the rest waits for
-// barriers, shared memory and the state. 16 trees of 16 to 32 nodes 66 us (15), one tree of 24 nodes, 32 heads 16 us
+// barriers, shared memory and the state. 16 trees of 16 to 32 nodes 66 us (15), one tree of 24 nodes, 32 heads 14 us
 // (latency). Each node's state formed from its parent's, a CTA a head and node after node, took 1,477 us for the first of
 // these; the products on the tensor cores with two CTAs an SM 631; paths as lists 512; outputs as a second product 470; four
 // CTAs an SM up to 32 nodes and 512 threads above 352; a node's scalars by half a warp 317.
@@ -725,7 +725,9 @@ int launch_kda_tree(const KdaArgs& a, cudaStream_t stream) {
   if (a.R == 0) return kOk;
   if ((int64_t)a.R * a.H > 0x7fffffff) return kErrArgs;
   if (a.max_nodes <= 16) return launch_nodes<16>(a, stream);
-  if (a.max_nodes <= 32) return launch_nodes<32>(a, stream);
+  // up to 32 nodes four smaller CTAs an SM, unless the larger ones all run at once: 1 x 24 nodes, 32 heads 15.6 and 13.9 us,
+  // 4 x 24, 64 heads 19.7 and 19.1, 6 x 24, 64 heads 24.2 and 29.8
+  if (a.max_nodes <= 32 && a.R * (int64_t)a.H > Shape<64>::kBlocks * (int64_t)device_sm_count()) return launch_nodes<32>(a, stream);
   return launch_nodes<64>(a, stream);
 }
 

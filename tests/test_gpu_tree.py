@@ -400,6 +400,24 @@ def test_extreme_gates(cuda):
     check_rows(out, tree64(d, seqs, trees, H), H)
 
 
+def test_batches_of_trees(cuda):
+    """More requests and heads than run at once, trees of 1 to 32 nodes, one node's value NaN."""
+    rng = np.random.default_rng(21)
+    H, R = 5, 67
+    trees = [wild(rng, int(n)) for n in rng.integers(1, 33, R)]
+    trees[5], trees[6], trees[7] = CHAIN(32), STAR(31), BINARY(32)
+    ends = np.cumsum([0] + [len(t) for t in trees])
+    d = kda_make(rng, int(ends[-1]), H, R)
+    d["x"][ends[7] + 2, 2 * H * D + 3 * D + 11] = np.nan
+    seqs = [(int(ends[r]), int(ends[r + 1]), R - 1 - r, int(r % 5 != 2)) for r in range(R)]
+    want = tree64(d, seqs, trees, H)
+    out, status = run_tree(cuda, d, H, seqs, sum(trees, []), max_nodes=32)
+    assert status == 0
+    gone = np.isnan(want)
+    assert gone.any() and (gone.sum(axis=0) > 0).sum() == 1 and (np.isnan(out) == gone).all()
+    check_rows(np.where(gone, 0, out), np.where(gone, 0, want), H)
+
+
 @pytest.mark.parametrize("n", [12, 30, 50])
 @pytest.mark.parametrize("where", ["v", "k", "q", "gate", "beta"])
 def test_what_is_not_finite_reaches_its_descendants_alone(cuda, n, where):
