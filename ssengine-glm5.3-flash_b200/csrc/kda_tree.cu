@@ -12,8 +12,8 @@
 // path (each is at most 1; quotients of cumulated ones would overflow).
 //
 // One CTA a (request, head), two or four an SM:
-//   conv and gates: a thread a pair of channels of q and k (they share the taps' addresses) for every fourth (eighth) node, then of g,
-//       late of v;
+//   conv and gates: a thread a pair of channels of q and k (they share the taps' addresses) for every fourth (eighth) node,
+//       then of g, late of v;
 //   norms, pairs, A k and A q: half a warp a node (8 channels a lane), its pairs 2 at a time;
 //   products: [S (A k) | S (A q)] on the tensor cores, M = 128 value rows, N = 2 nodes, K = 128 keys, tcgen05 kind::f16: S in
 //       TMEM and the vectors in shared memory, both as two bf16 parts, three of the four products (what is left out is below
@@ -727,7 +727,8 @@ int launch_kda_tree(const KdaArgs& a, cudaStream_t stream) {
   if (a.max_nodes <= 16) return launch_nodes<16>(a, stream);
   // up to 32 nodes four smaller CTAs an SM, unless the larger ones all run at once: 1 x 24 nodes, 32 heads 15.6 and 13.9 us,
   // 4 x 24, 64 heads 19.7 and 19.1, 6 x 24, 64 heads 24.2 and 29.8
-  if (a.max_nodes <= 32 && a.R * (int64_t)a.H > Shape<64>::kBlocks * (int64_t)device_sm_count()) return launch_nodes<32>(a, stream);
+  const bool at_once = a.R * (int64_t)a.H <= Shape<64>::kBlocks * (int64_t)device_sm_count();
+  if (a.max_nodes <= 32 && !at_once) return launch_nodes<32>(a, stream);
   return launch_nodes<64>(a, stream);
 }
 
