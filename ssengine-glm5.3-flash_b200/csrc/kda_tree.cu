@@ -12,8 +12,8 @@
 // path (each is at most 1; quotients of cumulated ones would overflow).
 //
 // One CTA a (request, head), two or four an SM:
-//   conv and gates: a thread a pair of channels of q and k (they share the taps' addresses) for every fourth (eighth) node,
-//       then of g, late of v;
+//   conv: a warp a node, 4 channels a lane, of q or k, late of v; gates: a thread a pair of channels of every fourth (eighth)
+//       node;
 //   norms, pairs, A k and A q: half a warp a node (8 channels a lane), its pairs 2 at a time;
 //   products: [S (A k) | S (A q)] on the tensor cores, M = 128 value rows, N = 2 nodes, K = 128 keys, tcgen05 kind::f16: S in
 //       TMEM and the vectors in shared memory, both as two bf16 parts, three of the four products (what is left out is below
@@ -24,12 +24,12 @@
 //
 // Bound: not HBM (a head's state is read once, 64 KB, whatever the nodes) but the vectors' arithmetic and the pairs, which
 // are on no tensor core: the decays between two nodes cannot be split into a factor of each without overflow. 48 trees of 32
-// to 64 nodes x 64 heads: 304 us (61 us of bytes), 55,000 warp instructions a CTA (pairs 11,000, conv of q and k 9,000, of v
-// 7,000, decays and norms 9,000, the rest tree, state, scalars and outputs), issue slots 54 % in use, the rest waits for
-// barriers, shared memory and the state. 16 trees of 16 to 32 nodes 66 us (15), one tree of 24 nodes, 32 heads 14 us
+// to 64 nodes x 64 heads: 300 us (61 us of bytes), 52,000 warp instructions a CTA (pairs 11,000, conv 14,000, decays and norms 9,000, the rest tree, state, scalars and outputs), issue slots 54 % in use, the rest waits for
+// barriers, shared memory and the state. 16 trees of 16 to 32 nodes 65 us (15), one tree of 24 nodes, 32 heads 14 us
 // (latency). Each node's state formed from its parent's, a CTA a head and node after node, took 1,477 us for the first of
 // these; the products on the tensor cores with two CTAs an SM 631; paths as lists 512; outputs as a second product 470; four
-// CTAs an SM up to 32 nodes and 512 threads above 352; a node's scalars by half a warp 317.
+// CTAs an SM up to 32 nodes and 512 threads above 352; a node's scalars by half a warp 317; a thread a pair of
+// channels of q and k, or of v, in the conv 305.
 #include "common.cuh"
 #include "kda_math.cuh"
 #include "ops.h"
@@ -155,6 +155,13 @@ SSB_DEVICE float2 conv_silu(const uint64_t (&p)[4], const uint32_t (&x)[4]) {
 SSB_DEVICE void conv_weights(uint64_t (&p)[4], uint4 wv) {                           // 2 channels x 4 taps
   const float2 a0 = bf2(wv.x), a1 = bf2(wv.y), b0 = bf2(wv.z), b1 = bf2(wv.w);
   p[0] = f2pack(a0.x, b0.x), p[1] = f2pack(a0.y, b0.y), p[2] = f2pack(a1.x, b1.x), p[3] = f2pack(a1.y, b1.y);
+}
+
+// Two pairs: 4 channels.
+SSB_DEVICE float4 conv_silu4(const uint64_t (&p)[2][4], const uint2 (&x)[4]) {
+  const uint32_t xa[4] = {x[0].x, x[1].x, x[2].x, x[3].x}, xb[4] = {x[0].y, x[1].y, x[2].y, x[3].y};
+  const float2 y = conv_silu(p[0], xa), z = conv_silu(p[1], xb);
+  return make_float4(y.x, y.y, z.x, z.y);
 }
 
 template <int N>
@@ -283,9 +290,14 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
     for (int t = 0; t < N / kGroups; ++t, in += step)
       if (part + kGroups * t < n) gin[t] = __ldg(in);
   }
-  // the conv's weights of q and k and the gates' parameters
-  const uint4 wq = __ldg(reinterpret_cast<const uint4*>(a.conv_w + ((int64_t)h * kDim + 2 * pair) * 4));
-  const uint4 wk = __ldg(reinterpret_cast<const uint4*>(a.conv_w + ((int64_t)a.P + h * kDim + 2 * pair) * 4));
+  // the conv's weights of q or k and the gates' parameters
+  const auto conv_weight = [&](int kind, int j) {              // channels 4 lane + 2 j, + 1
+    return __ldg(reinterpret_cast<const uint4*>(a.conv_w + ((int64_t)kind * a.P + h * kDim + 4 * lane + 2 * j) * 4));
+  };
+  const int kind = warp & 1;                                   // q, k
+  uint4 w[2];                                                  // 2 channels x 4 taps each
+#pragma unroll
+  for (int j = 0; j < 2; ++j) w[j] = conv_weight(kind, j);
   const float2 dt = __ldg(reinterpret_cast<const float2*>(a.dt_bias + h * kDim) + pair);
   const float a_log = __ldg(a.a_log + h);
   cp_async_wait();
@@ -313,33 +325,20 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
   };
   store_state();
 
-  // ---- the conv of q and k: every kGroups-th node, 2 at a time
+  // ---- the conv: of q by the even warps, of k by the odd ones, a warp a node, 4 channels a lane
   {
-    uint64_t pq[4], pk[4];
-    conv_weights(pq, wq);
-    conv_weights(pk, wk);
-#pragma unroll 1
-    for (int i = part; i < n; i += 2 * kGroups) {
-      uint32_t xq[2][4], xk[2][4];
+    float* to = &(kind ? sm.k : sm.q)[0][4 * lane];
+    uint64_t p[2][4];
+    conv_weights(p[0], w[0]);
+    conv_weights(p[1], w[1]);
+#pragma unroll 2
+    for (int i = warp >> 1; i < n; i += kWarps / 2) {
+      const uint32_t taps = sm.tap[i];
+      uint2 x[4];
+      x[3] = *reinterpret_cast<const uint2*>(&sm.in[i][kind][2 * lane]);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int m = min(i + kGroups * j, n - 1);
-        const uint32_t taps = sm.tap[m];
-        xq[j][3] = sm.in[m][0][pair], xk[j][3] = sm.in[m][1][pair];
-#pragma unroll
-        for (int e = 0; e < 3; ++e) {
-          const uint32_t* row = &sm.in[(taps >> (8 * e)) & 0xFF][0][pair];
-          xq[j][2 - e] = row[0], xk[j][2 - e] = row[kDim / 2];
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float2 q = conv_silu(pq, xq[j]), k = conv_silu(pk, xk[j]);
-        if (i + kGroups * j < n) {
-          *reinterpret_cast<float2*>(&sm.q[i + kGroups * j][2 * pair]) = q;
-          *reinterpret_cast<float2*>(&sm.k[i + kGroups * j][2 * pair]) = k;
-        }
-      }
+      for (int e = 0; e < 3; ++e) x[2 - e] = *reinterpret_cast<const uint2*>(&sm.in[(taps >> (8 * e)) & 0xFF][kind][2 * lane]);
+      *reinterpret_cast<float4*>(to + i * kDim) = conv_silu4(p, x);
     }
   }
   __syncthreads();
@@ -521,11 +520,6 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
   if (tid == 0) products(0);
   // ---- meanwhile the rest of the inputs, and the scalars
   if (C::kPasses > 1) load_state(1);
-  const uint4 wv = __ldg(reinterpret_cast<const uint4*>(a.conv_w + (2 * (int64_t)a.P + h * kDim + 2 * pair) * 4));
-  uint32_t held[3] = {0, 0, 0};                                // the values' kept rows, the newest first
-  if (init)
-    for (int j = 0; j < 3; ++j)
-      held[j] = __ldg(reinterpret_cast<const uint32_t*>(cs + ((int64_t)(2 - j) * 3 + 2) * a.P + 2 * pair));
   // P_i of half a warp's node: lanes hold the distances l + 16 c; the nodes on the path from i up subtract their share from
   // those above them
 #pragma unroll
@@ -582,36 +576,38 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
     if (ok && tid == 0) products(1);
     if (ok) ok = mbar_wait(bar(1), 0, &sm.abort, a.status);
   }
+  uint4 wv[2];                                                 // 2 channels x 4 taps each
+#pragma unroll
+  for (int j = 0; j < 2; ++j) wv[j] = conv_weight(2, j);
+  uint2 held[3] = {};                                          // the values' kept rows, the newest first
+  if (init)
+    for (int j = 0; j < 3; ++j) {
+      const uint32_t* kept = reinterpret_cast<const uint32_t*>(cs + ((int64_t)(2 - j) * 3 + 2) * a.P + 4 * lane);
+      held[j] = make_uint2(__ldg(kept), __ldg(kept + 1));
+    }
   fence_proxy_async_smem();
   ok = !__syncthreads_or(!ok);
   tc_fence_after();
-  // ---- the values, in the place of the products' second operand: a pair of channels of every kGroups-th node a thread
+  // ---- the values, in the place of the products' second operand: a warp a node, 4 channels a lane
   {
-    uint64_t p[4];
-    conv_weights(p, wv);
+    uint64_t p[2][4];
+    conv_weights(p[0], wv[0]);
+    conv_weights(p[1], wv[1]);
 #pragma unroll 1
-    for (int i = part; i < n; i += 2 * kGroups) {              // 2 nodes at a time
-      uint32_t x[2][4];
+    for (int i = warp; i < n; i += kWarps) {
+      const uint32_t taps = sm.tap[i];
+      uint2 x[4];
+      x[3] = *reinterpret_cast<const uint2*>(&sm.vin[i][2 * lane]);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int m = min(i + kGroups * j, n - 1);
-        const uint32_t taps = sm.tap[m];
-        x[j][3] = sm.vin[m][pair];
+      for (int e = 0; e < 3; ++e) x[2 - e] = *reinterpret_cast<const uint2*>(&sm.vin[(taps >> (8 * e)) & (N - 1)][2 * lane]);
+      if (taps & (N * 0x010101u)) {                            // some are kept rows
 #pragma unroll
-        for (int e = 0; e < 3; ++e) x[j][2 - e] = sm.vin[(taps >> (8 * e)) & (N - 1)][pair];
-        if (taps & (N * 0x010101u)) {                          // some are kept rows
-#pragma unroll
-          for (int e = 0; e < 3; ++e) {
-            const uint32_t t = (taps >> (8 * e)) & 0xFF;
-            if (t >= N) x[j][2 - e] = t == N ? held[0] : t == N + 1 ? held[1] : held[2];
-          }
+        for (int e = 0; e < 3; ++e) {
+          const uint32_t t = (taps >> (8 * e)) & 0xFF;
+          if (t >= N) x[2 - e] = t == N ? held[0] : t == N + 1 ? held[1] : held[2];
         }
       }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float2 y = conv_silu(p, x[j]);
-        if (i + kGroups * j < n) *reinterpret_cast<float2*>(&sm.v[i + kGroups * j][2 * pair]) = y;
-      }
+      *reinterpret_cast<float4*>(&sm.v[i][4 * lane]) = conv_silu4(p, x);
     }
   }
   __syncthreads();
