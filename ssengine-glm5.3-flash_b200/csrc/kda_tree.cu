@@ -181,14 +181,6 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
   }
   if (n == 0) return;
   const bool init = sq.w != 0;
-  if (warp == 0) {
-    tmem_alloc(smem_u32(&sm.tmem), kCols);
-    tmem_relinquish();
-    if (lane == 0) {
-      for (int j = 0; j < 3; ++j) mbar_init(smem_u32(&sm.bar[j]), 1);
-      fence_barrier_init();
-    }
-  }
 
   // ---- the state's loads: a value row a lane, 32 keys of a pass a thread
   const int quarter = warp & 3, fourth = warp >> 2, v = 32 * quarter + lane;
@@ -230,8 +222,13 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
     // kept row part (0: the oldest)
     if (part < 3) {
       const uint32_t* kept = reinterpret_cast<const uint32_t*>(cs + (int64_t)part * 3 * a.P + 2 * pair);
-      sm.in[N + 2 - part][0][pair] = init ? __ldg(kept) : 0;
-      sm.in[N + 2 - part][1][pair] = init ? __ldg(kept + a.P / 2) : 0;
+      uint32_t(&at)[2][kDim / 2] = sm.in[N + 2 - part];
+      if (init) {
+        cp_async4(smem_u32(&at[0][pair]), kept);
+        cp_async4(smem_u32(&at[1][pair]), kept + a.P / 2);
+      } else {
+        at[0][pair] = at[1][pair] = 0;
+      }
     }
   } else {
     // node i a thread, its path walked twice: its length, then its nodes
@@ -300,6 +297,14 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
   for (int j = 0; j < 2; ++j) w[j] = conv_weight(kind, j);
   const float2 dt = __ldg(reinterpret_cast<const float2*>(a.dt_bias + h * kDim) + pair);
   const float a_log = __ldg(a.a_log + h);
+  if (warp == 0) {                                           // with the loads on their way
+    tmem_alloc(smem_u32(&sm.tmem), kCols);
+    tmem_relinquish();
+    if (lane == 0) {
+      for (int j = 0; j < 3; ++j) mbar_init(smem_u32(&sm.bar[j]), 1);
+      fence_barrier_init();
+    }
+  }
   cp_async_wait();
   tc_fence_before();
   if (__syncthreads_or(bad)) {
@@ -499,8 +504,12 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
   tc_fence_before();
   __syncthreads();
   const auto bar = [&](int i) { return smem_u32(&sm.bar[i]); };
-  const auto products = [&](int pass) {                        // of a pass's keys, by one thread
+  // the products are issued by one lane of the last warp, which has the fewest nodes; the whole warp goes along, so that the
+  // addresses stay in uniform registers
+  const bool issuer = warp == kWarps - 1;
+  const auto products = [&](int pass) {                        // of a pass's keys
     tc_fence_after();
+    const bool leader = elect_lane();
     constexpr uint32_t idesc = idesc_bf16(128, 2 * N);
     uint32_t acc = pass;
 #pragma unroll 1
@@ -510,14 +519,15 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
         const uint64_t bd = smem_desc(smem_u32(&sm.op[t == 1][kParts / 2 * pass + c][0][0]), 0, 1024, 2);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
-          mma_f16_ta(tmem + kColD, tmem + kColS + (t == 2 ? kColLo : 0) + 32 * c + 8 * ks, bd + 2 * ks, idesc, acc);
+          if (leader) mma_f16_ta(tmem + kColD, tmem + kColS + (t == 2 ? kColLo : 0) + 32 * c + 8 * ks, bd + 2 * ks, idesc, acc);
           acc = 1;
         }
       }
     }
-    tc_commit(bar(pass));
+    if (leader) tc_commit(bar(pass));
+    __syncwarp();
   };
-  if (tid == 0) products(0);
+  if (issuer) products(0);
   // ---- meanwhile the rest of the inputs, and the scalars
   if (C::kPasses > 1) load_state(1);
   // P_i of half a warp's node: lanes hold the distances l + 16 c; the nodes on the path from i up subtract their share from
@@ -573,7 +583,7 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
     if (ok) store_state();
     tc_fence_before();
     __syncthreads();
-    if (ok && tid == 0) products(1);
+    if (ok && issuer) products(1);
     if (ok) ok = mbar_wait(bar(1), 0, &sm.abort, a.status);
   }
   uint4 wv[2];                                                 // 2 channels x 4 taps each
@@ -645,17 +655,19 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
   const bool any_lost = __syncthreads_or(lost != 0);
   uint32_t* shared_lost = &sm.vin[0][0];                      // [part][value row]
   if (any_lost) shared_lost[kDim * fourth + v] = lost;
-  if (ok && tid == 0) {
+  if (ok && issuer) {
     tc_fence_after();
+    const bool leader = elect_lane();
     constexpr uint32_t idesc = idesc_bf16(128, N);
 #pragma unroll 1
     for (int t = 0; t < 3; ++t) {                              // onto S (A q)
       const uint64_t bd = smem_desc(smem_u32(&sm.p[t == 1][0][0]), 0, 1024, 2);
 #pragma unroll
       for (int ks = 0; ks < N / 16; ++ks)
-        mma_f16_ta(tmem + kColD + N, tmem + kColS + (t == 2 ? kColLo : 0) + 8 * ks, bd + 2 * ks, idesc, 1u);
+        if (leader) mma_f16_ta(tmem + kColD + N, tmem + kColS + (t == 2 ? kColLo : 0) + 8 * ks, bd + 2 * ks, idesc, 1u);
     }
-    tc_commit(bar(2));
+    if (leader) tc_commit(bar(2));
+    __syncwarp();
   }
   if (ok) ok = mbar_wait(bar(2), 0, &sm.abort, a.status);
   if (!__syncthreads_or(!ok)) {

@@ -154,15 +154,6 @@ SSB_DEVICE void tmem_st_4(uint32_t taddr, const uint32_t (&v)[4]) {
                "r"(v[2]), "r"(v[3])
                : "memory");
 }
-SSB_DEVICE bool elect_lane() {                   // true in one lane of a converged warp
-  uint32_t p;
-  asm volatile(
-      "{\n\t.reg .pred e;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "selp.u32 %0, 1, 0, e;\n\t}"
-      : "=r"(p));
-  return p != 0;
-}
 
 SSB_DEVICE void cp_async16(uint32_t dst, const void* src, bool valid) {
   const int n = valid ? 16 : 0;
