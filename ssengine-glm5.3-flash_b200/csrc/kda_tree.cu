@@ -130,6 +130,13 @@ SSB_DEVICE void tmem_st_x4(uint32_t taddr, const uint32_t (&v)[4]) {
                "r"(v[2]), "r"(v[3])
                : "memory");
 }
+// 16 rows x 16 columns: a lane has of rows lane / 4 and + 8 the columns 2 (lane % 4), + 1 (two registers each), then those of
+// the next 8 columns.
+SSB_DEVICE void tmem_st_16x256(uint32_t taddr, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.16x256b.x2.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 // D[tmem] (+)= A B with bf16 A in TMEM (a row a lane, 2 values a column) and B in shared memory.
 SSB_DEVICE void mma_f16_ta(uint32_t d, uint32_t a, uint64_t bd, uint32_t idesc, uint32_t acc) {
   asm volatile(
@@ -182,19 +189,21 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
   if (n == 0) return;
   const bool init = sq.w != 0;
 
-  // ---- the state's loads: a value row a lane, 32 keys of a pass a thread
+  // ---- the state's loads, 32 keys of a pass a thread: 8 keys 8 (lane % 4) .. + 7 of each of the value rows lane / 4 + 8 i,
+  // which are 128 bytes of a row for 4 lanes (a row a lane, as TMEM stands, is 4 times the lines a load: 297 us for 48 trees
+  // of up to 64 nodes)
   const int quarter = warp & 3, fourth = warp >> 2, v = 32 * quarter + lane;
-  const float* S = a.rec_state + (int64_t)sq.z * a.rs_stride + ((int64_t)h * kDim + v) * kDim + 32 * fourth;
+  const float* S = a.rec_state + (int64_t)sq.z * a.rs_stride + ((int64_t)h * kDim + 32 * quarter) * kDim + 32 * fourth;
   float st[32];
   const auto load_state = [&](int pass) {
-    const float* from = S + 32 * kParts * pass;
+    const float* from = S + 32 * kParts * pass + (lane >> 2) * kDim + 8 * (lane & 3);
     const bool wide = (reinterpret_cast<uintptr_t>(from) & 31) == 0;
 #pragma unroll
-    for (int c = 0; c < 32; c += 8) {
+    for (int c = 0; c < 32; c += 8, from += 8 * kDim) {
       if (init && wide) {
-        ld8(from + c, st + c);
+        ld8(from, st + c);
       } else if (init) {
-        const float4 x = __ldg(reinterpret_cast<const float4*>(from + c)), y = __ldg(reinterpret_cast<const float4*>(from + c + 4));
+        const float4 x = __ldg(reinterpret_cast<const float4*>(from)), y = __ldg(reinterpret_cast<const float4*>(from + 4));
         st[c] = x.x, st[c + 1] = x.y, st[c + 2] = x.z, st[c + 3] = x.w;
         st[c + 4] = y.x, st[c + 5] = y.y, st[c + 6] = y.z, st[c + 7] = y.w;
       } else {
@@ -204,7 +213,7 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
     }
   };
   load_state(0);
-  if (C::kPasses > 1 && init) asm volatile("prefetch.global.L2 [%0];" ::"l"(S + 32 * kParts));
+  if (C::kPasses > 1 && init) asm volatile("prefetch.global.L2 [%0];" ::"l"(S + 32 * kParts + lane * kDim));
   // ---- the inputs of q and k into shared memory; the tree (the last 64 threads)
   const int pair = tid & 63, part = tid >> 6;
   const __nv_bfloat16* cs = a.conv_state + (int64_t)sq.z * a.cs_stride + h * kDim;            // of q; k, v: + P, + 2 P
@@ -315,16 +324,21 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
   if (tid == 0) sm.abort = 0;                                // its place was in use
   tc_fence_after();
   const uint32_t tmem = sm.tmem;
-  // ---- the state's parts to TMEM
+  // ---- the state's parts to TMEM, by 16 rows: of 32 keys, in 16 columns of pairs, first the pairs 4 c and 4 c + 1 of all c,
+  // then 4 c + 2 and 4 c + 3. The products' other operand has them in the same order
   const uint32_t rows = static_cast<uint32_t>(32 * quarter) << 16;
   const auto store_state = [&] {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t hi[4], lo[4];
+    for (int half = 0; half < 2; ++half) {
+      uint32_t hi[8], lo[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) split2(st[8 * j + 2 * e], st[8 * j + 2 * e + 1], hi[e], lo[e]);
-      tmem_st_x4(tmem + rows + kColS + 16 * fourth + 4 * j, hi);
-      tmem_st_x4(tmem + rows + kColS + kColLo + 16 * fourth + 4 * j, lo);
+      for (int e = 0; e < 8; ++e) {                            // pair (e & 1) + 2 (e >> 2) of row 16 half + 8 (e >> 1 & 1)
+        const float* x = st + 16 * half + 8 * (e >> 1 & 1) + 2 * (e & 1) + 4 * (e >> 2);
+        split2(x[0], x[1], hi[e], lo[e]);
+      }
+      const uint32_t to = tmem + rows + (static_cast<uint32_t>(16 * half) << 16) + kColS + 16 * fourth;
+      tmem_st_16x256(to, hi);
+      tmem_st_16x256(to + kColLo, lo);
     }
     tmem_st_wait();
   };
@@ -484,7 +498,8 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
     uint32_t to = smem_u32(&sm.vin[part][pair]);
 #pragma unroll 2
     for (int i = part; i < n; i += kGroups, in += step, to += kGroups * kDim * 2) cp_async4(to, in);
-    const int granule = l >> 1, within = (l & 1) * 8;
+    // channels 4 l .. + 3 of 64, in the state's order of pairs
+    const int granule = 4 * (l >> 3) + 2 * (l & 1) + ((l >> 2) & 1), within = (l & 2) * 4;
 #pragma unroll
     for (int t = 0; t < kOwn; ++t) {
       const int i = first + 2 * kWarps * t;
