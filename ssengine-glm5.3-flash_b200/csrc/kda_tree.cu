@@ -175,6 +175,7 @@ template <int N>
 __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tree_kernel(const __grid_constant__ KdaArgs a) {
   using C = Shape<N>;
   constexpr int kWarps = C::kWarps, kGroups = C::kGroups, kParts = C::kParts, kOwn = C::kOwn, kShare = C::kShare;
+  constexpr int kConvWarps = kWarps - 2;                     // the last two make the lists of the paths meanwhile
   constexpr uint32_t kColS = C::kColS, kColLo = C::kColLo, kColD = C::kColD, kCols = C::kCols;
   extern __shared__ __align__(1024) uint8_t raw_smem[];
   TreeSmem<N>& sm = *reinterpret_cast<TreeSmem<N>*>(raw_smem);
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
       }
     }
   } else {
-    // node i a thread, its path walked twice: its length, then its nodes
+    // node i a thread
     const int i = tid - 64 * (kGroups - 1);
     const bool node = i < n;
     int p = -1;
@@ -255,36 +256,13 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
       asm volatile("prefetch.global.L2 [%0];" ::"l"(x + kDim / 2));
     }
     bad = named_bar_or(1, 64, bad);
-    int len = 0;
-    uint32_t taps = 0;
     if (node && !bad) {
-      int at = p;
-      for (int j = 0, kept = N; j < 3; ++j) {
+      uint32_t taps = 0;
+      for (int j = 0, kept = N, at = p; j < 3; ++j) {
         taps |= static_cast<uint32_t>(at >= 0 ? at : kept++) << (8 * j);
-        if (at >= 0) at = sm.parent[at], ++len;
+        if (at >= 0) at = sm.parent[at];
       }
-      for (; at >= 0; at = sm.parent[at]) ++len;
       sm.tap[i] = taps;
-      ++len;
-    }
-    int end = len;                                           // the sum of the lengths: a warp each, the second behind the first
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, end, o);
-      if (lane >= o) end += x;
-    }
-    if (i == 31) sm.abort = end;
-    named_bar(1, 64);
-    if (i >= 32) end += sm.abort;
-    if (node && !bad) {
-      sm.off[i] = static_cast<uint16_t>(end - len);
-      if (i == n - 1) sm.off[n] = static_cast<uint16_t>(end);
-      uint8_t* path = reinterpret_cast<uint8_t*>(sm.pn + (end - len)) + 3 * len;
-      int at = i;
-      for (int d = 0; d < len; ++d) {
-        path[d] = static_cast<uint8_t>(at);
-        at = sm.parent[at];
-      }
     }
   }
   // the gates' inputs: a pair of channels of every kGroups-th node a thread
@@ -310,6 +288,7 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
     tmem_alloc(smem_u32(&sm.tmem), kCols);
     tmem_relinquish();
     if (lane == 0) {
+      sm.abort = 0;
       for (int j = 0; j < 3; ++j) mbar_init(smem_u32(&sm.bar[j]), 1);
       fence_barrier_init();
     }
@@ -321,7 +300,6 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
     if (warp == 0) tmem_dealloc(sm.tmem, kCols);
     return;
   }
-  if (tid == 0) sm.abort = 0;                                // its place was in use
   tc_fence_after();
   const uint32_t tmem = sm.tmem;
   // ---- the state's parts to TMEM, by 16 rows: of 32 keys, in 16 columns of pairs, first the pairs 4 c and 4 c + 1 of all c,
@@ -345,13 +323,37 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
   store_state();
 
   // ---- the conv: of q by the even warps, of k by the odd ones, a warp a node, 4 channels a lane
-  {
+  if (warp >= kConvWarps) {
+    // a node's path, a node a thread, walked twice: its length, then its nodes
+    const int i = tid - 32 * kConvWarps;
+    int len = 0;
+    for (int at = i < n ? i : -1; at >= 0; at = sm.parent[at]) ++len;
+    int end = len;                                           // the sum of the lengths: a warp each, the second behind the first
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, end, o);
+      if (lane >= o) end += x;
+    }
+    if (i == 31) sm.off[N + 1] = static_cast<uint16_t>(end);
+    named_bar(1, 64);
+    if (i >= 32) end += sm.off[N + 1];
+    if (i < n) {
+      sm.off[i] = static_cast<uint16_t>(end - len);
+      if (i == n - 1) sm.off[n] = static_cast<uint16_t>(end);
+      uint8_t* path = reinterpret_cast<uint8_t*>(sm.pn + (end - len)) + 3 * len;
+      int at = i;
+      for (int d = 0; d < len; ++d) {
+        path[d] = static_cast<uint8_t>(at);
+        at = sm.parent[at];
+      }
+    }
+  } else {
     float* to = &(kind ? sm.k : sm.q)[0][4 * lane];
     uint64_t p[2][4];
     conv_weights(p[0], w[0]);
     conv_weights(p[1], w[1]);
 #pragma unroll 2
-    for (int i = warp >> 1; i < n; i += kWarps / 2) {
+    for (int i = warp >> 1; i < n; i += kConvWarps / 2) {
       const uint32_t taps = sm.tap[i];
       uint2 x[4];
       x[3] = *reinterpret_cast<const uint2*>(&sm.in[i][kind][2 * lane]);
