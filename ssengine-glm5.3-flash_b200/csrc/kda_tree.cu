@@ -17,19 +17,20 @@
 //   norms, pairs, A k and A q: half a warp a node (8 channels a lane), its pairs 2 at a time;
 //   products: [S (A k) | S (A q)] on the tensor cores, M = 128 value rows, N = 2 nodes, K = 128 keys, tcgen05 kind::f16: S in
 //       TMEM and the vectors in shared memory, both as two bf16 parts, three of the four products (what is left out is below
-//       2^-16 of a product; the output has 8 bits). S comes straight from global memory, a value row a lane;
+//       2^-16 of a product; the output has 8 bits). S comes straight from global memory;
 //   outputs: w by value rows, as the products lie in TMEM, back there as bf16 parts, and W^T P^T onto S (A q) by the tensor
 //       cores, K = nodes.
 // The exponentials are the short ones (error about 2^-20 here): nothing computed here is kept but the bf16 outputs.
 //
 // Bound: not HBM (a head's state is read once, 64 KB, whatever the nodes) but the vectors' arithmetic and the pairs, which
 // are on no tensor core: the decays between two nodes cannot be split into a factor of each without overflow. 48 trees of 32
-// to 64 nodes x 64 heads: 300 us (61 us of bytes), 52,000 warp instructions a CTA (pairs 11,000, conv 14,000, decays and norms 9,000, the rest tree, state, scalars and outputs), issue slots 54 % in use, the rest waits for
-// barriers, shared memory and the state. 16 trees of 16 to 32 nodes 65 us (15), one tree of 24 nodes, 32 heads 14 us
-// (latency). Each node's state formed from its parent's, a CTA a head and node after node, took 1,477 us for the first of
-// these; the products on the tensor cores with two CTAs an SM 631; paths as lists 512; outputs as a second product 470; four
-// CTAs an SM up to 32 nodes and 512 threads above 352; a node's scalars by half a warp 317; a thread a pair of
-// channels of q and k, or of v, in the conv 305.
+// to 64 nodes x 64 heads: 262 to 264 us (61 us of bytes), 53,000 warp instructions a CTA (pairs 11,000, conv 14,000, decays
+// and norms 9,000, the rest tree, state, scalars and outputs), issue slots 60 % in use, the rest waits for barriers, shared
+// memory and the state. 16 trees of 16 to 32 nodes 57 us (15), one tree of 24 nodes, 32 heads 13 us (latency). Each node's
+// state formed from its parent's, a CTA a head and node after node, took 1,477 us for the first of these; the products on the
+// tensor cores with two CTAs an SM 631; paths as lists 512; outputs as a second product 470; four CTAs an SM up to 32 nodes
+// and 512 threads above 352; a node's scalars by half a warp 317; the conv by a warp a node, 4 channels a lane, 300; the
+// state by lines 264. Nodes dealt to the warps by the lengths of their paths: 270, the order costs more than it evens out.
 #include "common.cuh"
 #include "kda_math.cuh"
 #include "ops.h"
