@@ -184,7 +184,8 @@ __global__ void __launch_bounds__(Shape<N>::kThreads, Shape<N>::kBlocks) kda_tre
   const int r = blockIdx.x / a.H, h = blockIdx.x - r * a.H;
   const int4 sq = __ldg(reinterpret_cast<const int4*>(a.seqs) + r);   // {first row, end row, state block, has state}
   const int s = sq.x, n = sq.y - sq.x;
-  if (s < 0 || sq.y < s || sq.y > a.T || n > N || sq.z < 0 || (smem_u32(raw_smem) & 1023)) {
+  // the caller's bound, which is at most N, whatever N the call was dispatched to
+  if (s < 0 || sq.y < s || sq.y > a.T || n > a.max_nodes || sq.z < 0 || (smem_u32(raw_smem) & 1023)) {
     if (tid == 0 && h == 0) raise_status(a.status, kErrArgs);
     return;
   }
