@@ -329,8 +329,9 @@ int ssb_mla_decode_tree(const void* q, int32_t q_e4m3, int64_t ldq, int64_t head
  * dst[l][g][i] of the view takes what its row src[l][g][i] held before the call, i < n (src, dst int32 [lists, groups, n]
  * on the device, n <= 64). Within a group any rows may be both read and written (a permutation in place, one source for
  * several rows); an entry with a negative id, or whose ids are equal, moves nothing, and of entries with one destination
- * the first counts. A row that one group writes must not occur in another group of its list, nor two views overlap in rows
- * moved: what such a call leaves there is undefined. An id past a view's rows: the entry moves nothing there, status 1.
+ * the first counts (equal ids: the row stays). An id past a view's rows: the entry moves nothing there, takes no
+ * destination from a later one, and status 1. A row that one group writes must not occur in another group of its list, nor
+ * two views overlap in rows moved: what such a call leaves there is undefined.
  * Beams' states and pages reordered (src = the parents' rows), pages forked (src = the shared page), accepted tokens of a
  * tree brought to its front. */
 typedef struct ssb_move_view {

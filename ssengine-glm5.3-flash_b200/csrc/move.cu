@@ -41,7 +41,7 @@ __global__ void __launch_bounds__(kMoveThreads) move_rows_kernel(const __grid_co
   const int64_t g = (item - v.first) / slices, slice = item - v.first - g * slices;
   const int64_t at = (v.list * a.groups + g) * a.n;
 
-  // the rows to move: both ids given and different, and the first of its destination
+  // the rows to move: both ids given, within the rows and different, and the first such of its destination
   if (tid < 32) {
     int count = 0;
     for (int i0 = 0; i0 < a.n; i0 += 32) {
@@ -52,8 +52,8 @@ __global__ void __launch_bounds__(kMoveThreads) move_rows_kernel(const __grid_co
         go = false;
         raise_status(a.status, kErrArgs);
       }
-      for (int j = 0; go && j < i; ++j)
-        if (a.dst[at + j] == to && a.src[at + j] >= 0) go = false;
+      for (int j = 0; go && j < i; ++j)                // a source past the rows makes no entry
+        if (a.dst[at + j] == to && a.src[at + j] >= 0 && a.src[at + j] < v.rows) go = false;
       go = go && from != to;
       const uint32_t mask = __ballot_sync(0xffffffffu, go);
       if (go) {

@@ -124,7 +124,7 @@ class RowMover:
         n] on the device, n <= 64; with one list [G, n] too). The rows of a group g may be permuted in place and one source
         may go to several rows; an entry with a negative id or equal ids moves nothing, of entries with one destination
         the first counts. A row that one group writes must not occur in another group of its list. `status` (int32 [1] on
-        the device) receives 1 for an id past a view's rows (nothing is moved for it there)."""
+        the device) receives 1 for an id past a view's rows (its entry counts for nothing there)."""
         shape = src.shape
         lists, groups, n = shape if len(shape) == 3 else (1, *shape) if len(shape) == 2 else (0, 0, 0)
         if lists < self.lists or n > MOVE_ROWS or src.dtype is not torch.int32 or dst.dtype is not torch.int32 or \

@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 from test_gpu_decode import kda_make
+from test_gpu_move import run as move_run
 from test_gpu_tree import check_rows, run_tree, tree64, wild
 
 pytestmark = pytest.mark.gpu
@@ -34,3 +35,17 @@ def test_more_nodes_than_stated_are_skipped_whatever_the_batch(cuda, most, reque
         want = tree64(d, [seqs[r] for r in pick], [trees[r] for r in pick], H)
         for r in pick:
             check_rows(out[ends[r]:ends[r + 1]], want[ends[r]:ends[r + 1]], H)
+
+
+# ---- moves ----------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("n", [2, 40])
+def test_an_entry_past_the_view_does_not_take_a_destination(cuda, n):
+    """An entry that moves nothing because its source is past the rows is not the first of its destination."""
+    src = np.full((1, 1, n), -1, np.int32)
+    dst = np.full((1, 1, n), -1, np.int32)
+    src[0, 0, [0, n - 1]], dst[0, 0, [0, n - 1]] = [9, 1], [3, 3]
+    got, want, status, between = move_run(cuda, [(8, 64), (12, 4096)], [0, 0], src, dst, pitch=16)
+    assert status == 1 and between
+    assert all((g == w).all() for g, w in zip(got, want))
