@@ -348,11 +348,12 @@ int ssb_move_rows(const ssb_move_view* views, int32_t n_views, const int32_t* sr
 /* A beam search's selection for G requests of `beams` (1..64) beams: of the candidates (b, v) with score scores[g, b] +
  * x[g, b, v] - log sum_v exp x[g, b, v] the k (1..64) best in order, equal scores by the lower b * V + v: their scores
  * (fp32), beams and tokens to out_scores, out_parents, out_tokens [G, k]. logits [G * beams, ld] fp32 or bf16 (bf16 = 1),
- * read once; sums in 64 bits across threads, scores compared in 64 bits (log sums are right to about 2^-23). A beam
- * with finished[g, b] != 0 (uint8 [G, beams] or NULL) has one candidate, token `pad` at scores[g, b], and its logits are
- * not read. A logit of -inf is no candidate, nor is any of a beam whose score or log sum is infinite or NaN; places
- * without a candidate get -inf, -1, -1. With k = beams out_scores may be scores itself. workspace: 256-byte aligned, ssb_beam_workspace_bytes or more (returns 3 when
- * smaller), its contents need not be kept. */
+ * read once. Scores are compared in 64 bits and none is above its beam's. A log sum is right to 2^-18 at worst (rows of up to
+ * 2^23 logits, or whose mass lies within 16 of their largest), to about 2^-22 as the roundings fall. A beam with
+ * finished[g, b] != 0 (uint8 [G, beams] or NULL) has one candidate, token `pad` at scores[g, b], and its logits are not
+ * read. A logit of -inf is no candidate, nor is any of a beam whose score or log sum is infinite or NaN; places without a
+ * candidate get -inf, -1, -1. With k = beams out_scores may be scores itself. workspace: 256-byte aligned,
+ * ssb_beam_workspace_bytes or more (returns 3 when smaller), its contents need not be kept. */
 int ssb_beam_select(const void* logits, int32_t bf16, int64_t ld, int64_t G, int32_t beams, int64_t V, const float* scores,
                     const uint8_t* finished, int64_t pad, int32_t k, float* out_scores, int32_t* out_parents,
                     int64_t* out_tokens, void* workspace, int64_t ws_bytes, void* stream);

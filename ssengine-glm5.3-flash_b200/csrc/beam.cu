@@ -2,9 +2,10 @@
 //   score[b] + x[b, v] - log sum_v exp x[b, v]
 // in order, equal ones by the lower b V + v. One pass over the logits.
 //
-// scan: a CTA has one part of one beam's row, 16 bytes a load. Each warp keeps a sum of exponentials against a reference (a
-//   logit it has seen; it moves only when one exceeds it by 40, where a running maximum would be rescaled all the time) and
-//   the k largest (logit, token) as 64-bit keys whose order is that of the candidates (equal logits: the lower token is
+// scan: a CTA has one part of one beam's row, 16 bytes a load. Each warp keeps a sum of exponentials against the largest logit
+//   that it has seen, so that this one's term is exactly 1 and no term's exponent is large where the term is: in 32 bits over
+//   the terms of one iteration (at most 32 of a lane), in 64 beyond. A new largest logit, a handful a row, rescales the sum
+//   by an exponential in 64 bits. Beside it the k largest (logit, token) as 64-bit keys whose order is that of the candidates (equal logits: the lower token is
 //   larger). A load's largest logit is compared with a bound of the CTA's k-th largest: the least of its 8 warps' ceil(k / 8)-th
 //   largest, at first of the lanes' maxima over their first loads, then of the lists. What is not below goes to the warp's
 //   list in shared memory, cut back to its k largest when it is full or the logits seen are four times as many. The CTA
@@ -25,7 +26,6 @@ constexpr int kScanWarps = 8, kScanThreads = 32 * kScanWarps, kScanBlocks = 3;
 constexpr int kList = 256;                       // keys a warp holds between cuts
 constexpr int kGroups = 3;                        // groups of loads on their way to shared memory
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRise = 40.0f;                   // above the reference before it moves: e^40 times 2^31 terms stay finite
 constexpr int kJoinThreads = 512, kRanked = 64;
 constexpr int kMaxK = 64, kMaxBeams = 64;
 constexpr int kMaxCandidates = 8192;             // of a request, all parts together
@@ -133,6 +133,11 @@ __device__ __noinline__ void offer(WarpList& L, int k, float x, uint32_t token, 
   __syncwarp();
 }
 
+// What stood against `ref` against the larger `now`. Without a reference there is no sum yet: 0, or NaN.
+__device__ __noinline__ double rebase(double total, float ref, float now) {
+  return ref > -INFINITY ? total * exp(static_cast<double>(ref) - static_cast<double>(now)) : total;
+}
+
 // kSkewed: rows may begin anywhere in a 16-byte piece of memory. A lane's values are the same ones of a row then too, put
 // together from two pieces: equal rows get the same sums wherever they lie, and equal candidates stay equal.
 template <bool kBf16, bool kSkewed>
@@ -141,7 +146,7 @@ __global__ void __launch_bounds__(kScanThreads, kScanBlocks) beam_scan_kernel(co
   constexpr int kLoads = kSkewed ? 2 : 4;                    // 16-byte loads a lane has on their way
   __shared__ WarpList lists[kScanWarps];
   __shared__ float wm[kScanWarps];
-  __shared__ float ws[kScanWarps];
+  __shared__ double ws[kScanWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t row = blockIdx.x / a.parts;
   const int part = static_cast<int>(blockIdx.x - row * a.parts);
@@ -219,7 +224,8 @@ __global__ void __launch_bounds__(kScanThreads, kScanBlocks) beam_scan_kernel(co
   if (lane == 0) L.least = 0, L.top = -INFINITY, L.count = 0;
   __syncthreads();
   float ref = -INFINITY, bar = -INFINITY;                    // the same in all lanes; a logit below bar is no candidate
-  uint64_t neg = 0, sum = 0;                                 // -ref (0 while there is none) and the sum, as pairs
+  uint64_t neg = 0;                                          // -ref, 0 while there is none, as a pair
+  double total = 0.0;
   int32_t seen = 0, look = 1;                                // iterations, when to cut the list next
   uint4 q[kLoads];
   const int32_t i1 = begin + 32 * warp, step = kLoads * kScanThreads;
@@ -275,22 +281,25 @@ __global__ void __launch_bounds__(kScanThreads, kScanBlocks) beam_scan_kernel(co
       bar = fmaxf(bar, __shfl_sync(0xffffffffu, t, 0));
       if (L.least != 0) bar = fmaxf(bar, key_logit(L.least));
     }
-    float limit = fminf(bar, ref + kRise);                   // of the loads to look at
+    uint64_t sum = 0;                                        // of this iteration, as a pair
+    const auto flush = [&] {
+      float s0, s1;
+      f2unpack(sum, s0, s1);
+      total += static_cast<double>(s0 + s1);
+      sum = 0;
+    };
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) {
       const float top = tops[u];
-      if (__any_sync(0xffffffffu, top >= limit)) {
-        if (__any_sync(0xffffffffu, top > ref + kRise || ref == -INFINITY)) {
+      if (__any_sync(0xffffffffu, top >= bar || top > ref)) {
+        if (__any_sync(0xffffffffu, top > ref)) {
           float now = top == top ? top : -INFINITY;
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
-          if (now > ref) {
-            const float f = ref > -INFINITY ? ex2((ref - now) * kLog2e) : 0.0f;
-            sum = mul2(sum, f2pack(f, f));
-            ref = now;
-            neg = f2pack(-ref, -ref);
-            limit = fminf(bar, ref + kRise);
-          }
+          flush();
+          total = rebase(total, ref, now);
+          ref = now;
+          neg = f2pack(-ref, -ref);
         }
         float x[kVec];
         values(q[u], x);
@@ -309,23 +318,21 @@ __global__ void __launch_bounds__(kScanThreads, kScanBlocks) beam_scan_kernel(co
         sum = add2(sum, f2pack(ex2(t0), ex2(t1)));           // NaN for a NaN, or an infinite reference
       }
     }
+    flush();
   }
   cut_list(L, a.k, lane);
   // the CTA's reference and sum, then its k largest
-  float s0, s1;
-  f2unpack(sum, s0, s1);
-  s0 += s1;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
-  if (lane == 0) wm[warp] = ref, ws[warp] = s0;
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if (lane == 0) wm[warp] = ref, ws[warp] = total;
   __syncthreads();
   if (warp != 0) return;
   const float m = lane < kScanWarps ? wm[lane] : -INFINITY;
   float t = m;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
-  const float z = lane < kScanWarps ? ws[lane] : 0.0f;
-  float part_sum = m > -INFINITY ? z * exp_neg(m - t) : z;   // without a reference the sum is 0, or NaN
+  const double z = lane < kScanWarps ? ws[lane] : 0.0;
+  double part_sum = m > -INFINITY ? z * exp_neg(m - t) : z;  // without a reference the sum is 0, or NaN
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) part_sum += __shfl_xor_sync(0xffffffffu, part_sum, o);
   if (lane == 0) a.part[row * a.parts + part] = {part_sum, t};
@@ -393,14 +400,14 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
       BeamPart q[4];                             // the first 128 parts, loaded once
       float m = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) q[j] = lane + 32 * j < a.parts ? part[lane + 32 * j] : BeamPart{0.0f, -INFINITY};
+      for (int j = 0; j < 4; ++j) q[j] = lane + 32 * j < a.parts ? part[lane + 32 * j] : BeamPart{0.0, -INFINITY};
 #pragma unroll
       for (int j = 0; j < 4; ++j) m = fmaxf(m, q[j].m);
       for (int p = lane + 128; p < a.parts; p += 32) m = fmaxf(m, part[p].m);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       const auto term = [&](const BeamPart& p) {
-        return p.m > -INFINITY || p.sum != p.sum ? static_cast<double>(p.sum) * exp_neg(p.m - m) : 0.0;
+        return p.m > -INFINITY || p.sum != p.sum ? p.sum * exp_neg(p.m - m) : 0.0;
       };
       double z = 0.0;
 #pragma unroll

@@ -321,8 +321,9 @@ struct MoveArgs {
 int launch_move_rows(const MoveView* views, const MoveArgs& a, cudaStream_t stream);
 
 // A beam search's selection (csrc/beam.cu).
-struct BeamPart {                      // of one part of one row: sum of e^(x - m), the reference m
-  float sum, m;
+struct BeamPart {                      // of one part of one row: sum of e^(x - m), its largest logit m
+  double sum;
+  float m;
 };
 struct BeamArgs {
   const void* x = nullptr;             // [G * B, ldx] fp32 or bf16 logits

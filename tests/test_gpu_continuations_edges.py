@@ -3,7 +3,9 @@ not make. Tolerances, derived before the first run, stand at each test."""
 
 import numpy as np
 import pytest
+import torch
 
+from test_gpu_beam import run as beam_run
 from test_gpu_decode import kda_make
 from test_gpu_move import run as move_run
 from test_gpu_tree import check_rows, run_tree, tree64, wild
@@ -35,6 +37,62 @@ def test_more_nodes_than_stated_are_skipped_whatever_the_batch(cuda, most, reque
         want = tree64(d, [seqs[r] for r in pick], [trees[r] for r in pick], H)
         for r in pick:
             check_rows(out[ends[r]:ends[r + 1]], want[ends[r]:ends[r + 1]], H)
+
+
+# ---- beam selection -------------------------------------------------------------------------------------------------
+
+
+def lse_errors(cuda, x, bf16=False):
+    """Rows x as requests of one beam whose score makes the best candidate's about 0, where float32 is fine: the kernel's
+    log sums less the true ones, and the largest logits."""
+    t = torch.from_numpy(np.ascontiguousarray(x, np.float32)).to(torch.bfloat16 if bf16 else torch.float32)
+    x = t.double().numpy()
+    top = x.max(axis=1)
+    lse = top + np.log(np.exp(x - top[:, None]).sum(axis=1))
+    given = (lse - top).astype(np.float32)
+    s, p, v = beam_run(cuda, t, given[:, None], 1, bf16=bf16)
+    assert (v[:, 0] == x.argmax(axis=1)).all()
+    return (given.astype(np.float64) + top - lse) - s[:, 0], given, s[:, 0]
+
+
+@pytest.mark.parametrize("V", [700, 5003, 32768, 151552])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_log_sums_of_peaked_rows(cuda, V, bf16):
+    """One logit 20 to 40 above the rest, wherever it lies. Its term is the reference's own, 1; the others are at most
+    151,552 e^-16 = 2 % of it, each right to 2^-18: 1e-7, and 2^-24 of the score's own magnitude (below 2 %). No score is
+    above its beam's."""
+    rng = np.random.default_rng(V)
+    rows = 48
+    x = rng.uniform(-2, 2, (rows, V)).astype(np.float32)
+    at = rng.integers(0, V, rows)
+    at[:4] = [0, V - 1, V // 2, min(V - 1, 33)]
+    x[np.arange(rows), at] = (2 + rng.uniform(20, 40, rows)).astype(np.float32)
+    err, given, score = lse_errors(cuda, x, bf16)
+    assert np.abs(err).max() <= 1.2e-7, np.abs(err).max()
+    scores = -rng.random((6, 8)).astype(np.float32)
+    t = torch.from_numpy(x)
+    s, p, v = beam_run(cuda, t, scores, 8, bf16=bf16)
+    for g in range(6):
+        assert (s[g] <= scores[g][p[g]]).all()
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_log_sums_of_other_rows(cuda, bf16):
+    """Where the mass of a row lies within 16 of its largest logit a term's exponent is off by half a step of the difference
+    (below 16: 2^-21), half a step of its product with log2 e (below 23.1: 2^-20 ln 2), and log2 e's own 1.4e-8 of it: 1.4e-6;
+    the exponential by 2^-22, a thread's sums of at most 16 terms by 15 x 2^-24, the warps' and parts' weights by 2^-22 each:
+    3.1e-6 in all, below 2^-18 = 3.8e-6, if every rounding of the row falls to one side. One addition of 32 logits to 1 is the
+    lowest in the last two rows, so their mass is deep below the largest."""
+    rng = np.random.default_rng(9)
+    V = 151552
+    rows = [rng.standard_normal(V), rng.standard_normal(V) * 3, rng.uniform(-8, 0, V), np.linspace(-8, 8, V), np.linspace(8, -8, V),
+            np.linspace(0, 0.05, V), np.full(V, 2.7), rng.integers(-3, 3, V) * 1.1, np.repeat(rng.standard_normal(V // 32) * 2, 32)]
+    for depth in (5.3, 11.9):
+        row = np.full(V, -depth)
+        row[rng.integers(0, V)] = 0.0
+        rows.append(row + 0.77)
+    err, _, _ = lse_errors(cuda, np.stack(rows), bf16)
+    assert np.abs(err).max() <= 2.0 ** -18, err
 
 
 # ---- moves ----------------------------------------------------------------------------------------------------------
