@@ -173,9 +173,9 @@ class KdaAttention:
         """y bf16 [T, H] (the layer input after the boundary's RMSNorm) -> attention output bf16 [T, H]; the KDA state
         blocks of `seqs` (int32 [R, 4] on the device) are updated in place. keep: the intermediates stay in
         `self.parts` (for checks). decode: the recurrence token by token (`KdaLayer.decode`), for a step's few new
-        rows a request, in place of the chunked scan. tree (parents int32 [T], the largest tree's nodes): the rows are
-        trees of drafted tokens (`KdaLayer.decode_tree`); the state blocks stay as they are, and `self.step` keeps what
-        `accept` needs."""
+        rows a request, in place of the chunked scan. tree (parents int32 [T], the largest tree's nodes, a list): the
+        rows are trees of drafted tokens (`KdaLayer.decode_tree`); the state blocks stay as they are, and the list receives
+        what `accept` needs of them."""
         T, P, dev = y.shape[0], self.P, self.device
         s = lib.stream_ptr(stream)
         proj = torch.empty(T, self.in_proj.N_pad, dtype=torch.bfloat16, device=dev)
@@ -191,7 +191,7 @@ class KdaAttention:
         if tree is not None:
             self.kda.decode_tree(proj, gate, beta, o, seqs, tree[0], conv_state, rec_state, max_nodes=tree[1],
                                  stream=stream, status=status)
-            self.step = (proj, gate, beta)
+            tree[2].append((proj, gate, beta))
         else:
             scan = self.kda.decode if decode else self.kda.prefill
             scan(proj, gate, beta, o, seqs, conv_state, rec_state, stream=stream, status=status)
@@ -216,10 +216,9 @@ class KdaAttention:
             self.o_proj.gemm(codes, sf, T, out, status, stream)
         return out
 
-    def accept(self, rows, seqs, conv_state, rec_state, status, stream=None) -> None:
-        """Moves the states on along the accepted rows (int32 [n], `seqs` over places in them) of the last tree."""
-        self.kda.advance(*self.step, rows, seqs, conv_state, rec_state, stream=stream, status=status)
-        self.step = None
+    def accept(self, step, rows, seqs, conv_state, rec_state, status, stream=None) -> None:
+        """Moves the states on along the accepted rows (int32 [n], `seqs` over places in them) of the trees that left `step`."""
+        self.kda.advance(*step, rows, seqs, conv_state, rec_state, stream=stream, status=status)
 
 
 class MhcBoundary:
@@ -480,12 +479,12 @@ class DsaAttention:
         decode (form, reqs int32 [T], seq_lens int32 [T]): the attention of a step's few new rows a request (row t's
         request and the tokens that it sees, positions[t] + 1), split over the cache: form "selected" over the
         indexer's tokens as in the prefill (`mla.decode_selected`), "dense" over the whole context (`mla.decode`;
-        the pool keys are inserted, the logits and the top-k are left out). Form "tree" (with a fourth entry, ancestors
-        int64 [T]): trees of drafted tokens behind contexts of seq_lens tokens (`mla.decode_tree`), dense; the pool keys
-        are left alone until `accept`, for which `self.step` keeps their projections."""
+        the pool keys are inserted, the logits and the top-k are left out). Form "tree" (with two more entries, ancestors
+        int64 [T] and a list): trees of drafted tokens behind contexts of seq_lens tokens (`mla.decode_tree`), dense; the
+        pool keys are left alone until `accept`, for which the list receives their projections."""
         from . import indexer, mla
 
-        form, reqs, seq_lens, *words = decode if decode is not None else (None, None, None)
+        form, reqs, seq_lens, *tree = decode if decode is not None else (None, None, None)
         if form not in (None, "selected", "dense", "tree"):
             raise ValueError(f"decode form {form!r}")
         select = form not in ("dense", "tree")
@@ -547,7 +546,7 @@ class DsaAttention:
         k_idx, gate = self._pool_inputs(idx)
         w = idx[:, self.IDX_DIM:self.IDX_DIM + self.IDX_HEADS]          # bf16 head weights, read in place
         if form == "tree":
-            self.step = idx
+            tree[1].append(idx)
         elif self.indexer_fp8:
             # the logits' common factor (softmax scale x heads^-1/2 = 2^-6) is left out: a power of two, it changes
             # neither the top-k set nor its ties
@@ -587,7 +586,7 @@ class DsaAttention:
                 ws = None
             common = dict(bmm2=self.k_scale, reqs=reqs, workspace=ws, stream=stream, status=status)
             if form == "tree":
-                mla.decode_tree(q8, kv_cache, page_table, seq_lens, words[0], bmm1, o_lat, **common)
+                mla.decode_tree(q8, kv_cache, page_table, seq_lens, tree[0], bmm1, o_lat, **common)
             elif select:
                 mla.decode_selected(q8, kv_cache, tok, page_table, bmm1, o_lat, n_idx=4 * self.TOPK + 3,
                                     seq_lens=seq_lens, **common)
@@ -610,12 +609,12 @@ class DsaAttention:
         """The keys and gates of the indexer's pools in the rows of its projection."""
         return idx[:, :self.IDX_DIM], idx[:, self.IDX_DIM + self.IDX_HEADS:2 * self.IDX_DIM + self.IDX_HEADS]
 
-    def accept(self, rows, kpool_reqs, max_rows, page_table, pool_cache, tail_ring, stream=None) -> None:
-        """Inserts the accepted rows (int64 [n]) of the last tree into the pool keys: kpool_reqs int32 [R, 4] {first place,
-        places, start position, tail block} over the places in `rows`."""
+    def accept(self, step, rows, kpool_reqs, max_rows, page_table, pool_cache, tail_ring, stream=None) -> None:
+        """Inserts the accepted rows (int64 [n]) of the trees that left `step` into the pool keys: kpool_reqs int32 [R, 4]
+        {first place, places, start position, tail block} over the places in `rows`."""
         from . import indexer
 
-        idx, self.step = self.step[rows], None
+        idx = step[rows]
         insert = indexer.kpool_insert_fp8 if self.indexer_fp8 else indexer.kpool_insert
         insert(*self._pool_inputs(idx), self.ape, kpool_reqs, max_rows, page_table, pool_cache, tail_ring, stream)
 

@@ -154,15 +154,16 @@ class Batch:
 
 
 class Trees:
-    """The trees of one `StageModel.verify`: a plan's chunks with their parents, checked on the host, and the device tensors
-    of its rows (chunk by chunk in the plan's order: all are decode-class)."""
+    """The trees of one `StageModel.verify`: a plan's chunks with their parents, checked on the host, the device tensors of
+    its rows (chunk by chunk in the plan's order: all are decode-class), and what each layer keeps of them for `accept`
+    (`steps`, in layer order)."""
 
     def __init__(self, chunks, trees, batch: Batch, device):
         from . import mla
 
         if len(trees) != len(chunks):
             raise ValueError(f"{len(trees)} trees for {len(chunks)} chunks")
-        self.chunks, self.device = list(chunks), device
+        self.chunks, self.device, self.steps = list(chunks), device, []
         self.trees = [[int(p) for p in t] for t in trees]
         masks, depths = [], []
         for c, t in zip(self.chunks, self.trees):
@@ -562,7 +563,7 @@ class StageModel:
             reqs = torch.searchsorted(batch.dsa["qsl"], rows, right=True, out_int32=True) - 1
             step = (decode, reqs, (batch.dsa["positions"] + 1).to(torch.int32))
         if tree is not None and batch.dsa is not None:
-            step = ("tree", tree.reqs, tree.context, tree.ancestors)
+            step = ("tree", tree.reqs, tree.context, tree.ancestors, tree.steps)
         for layer in self.layers:
             layer.moe_profile = self.moe_profile
         for layer, state, dsa, grp in zip(self.layers, self.kda_states, self.is_dsa, self.kda_group):
@@ -570,9 +571,9 @@ class StageModel:
                 res, x_prev, post, comb = layer.forward(res, x_prev, post, comb, batch.dsa, state, self.status,
                                                         decode=step)
             else:
+                nodes = None if tree is None else (tree.parents, tree.most, tree.steps)
                 res, x_prev, post, comb = layer.forward(res, x_prev, post, comb, batch.kda_seqs[grp], *state,
-                                                        self.status, decode=decode is not None,
-                                                        tree=None if tree is None else (tree.parents, tree.most))
+                                                        self.status, decode=decode is not None, tree=nodes)
             if self.layer_hook is not None:
                 self.layer_hook(layer, res, x_prev, post, comb)
         if edge_out is not None and not self.last and x_prev is not None:
@@ -618,7 +619,8 @@ class StageModel:
         the context: `KdaLayer.decode_tree` in the KDA layers, `mla.decode_tree` (over the whole context) in the DSA layers.
         Returns what `forward` returns, the last stage the greedy token after every node, in the plan's order (`last_logits`
         its logits). The requests' states and pool keys stay as they are until `accept`, which comes before the stage's
-        next step of these requests; a second `verify` in its place checks other trees."""
+        next step of these requests; a second `verify` in its place checks other trees. Until then every layer's inputs of the
+        nodes are kept."""
         if not self.kda:
             raise ValueError('layer_kind "moe" has no requests to continue')
         self.trees = None                # a step that fails leaves nothing to accept
@@ -639,11 +641,11 @@ class StageModel:
         self.trees = None
         if acc is None:
             return
-        for layer, state, dsa, grp in zip(self.layers, self.kda_states, self.is_dsa, self.kda_group):
+        for layer, kept, state, dsa, grp in zip(self.layers, t.steps, self.kda_states, self.is_dsa, self.kda_group):
             if dsa:
-                layer.attn.accept(acc["rows64"], acc["kpool"], acc["most"], t.page_table, state[1], state[2])
+                layer.attn.accept(kept, acc["rows64"], acc["kpool"], acc["most"], t.page_table, state[1], state[2])
             else:
-                layer.attn.accept(acc["rows"], acc["seqs"][grp], *state, self.status)
+                layer.attn.accept(kept, acc["rows"], acc["seqs"][grp], *state, self.status)
         if any(self.is_dsa):
             self.kv.move_tokens(acc["src"], acc["dst"], status=self.status)
 

@@ -1,6 +1,8 @@
 """Calls of the operators for several continuations of a request that their documentation allows and the tests beside them do
 not make. Tolerances, derived before the first run, stand at each test."""
 
+import gc
+
 import numpy as np
 import pytest
 import torch
@@ -9,6 +11,7 @@ from test_gpu_beam import run as beam_run
 from test_gpu_decode import kda_make
 from test_gpu_move import run as move_run
 from test_gpu_tree import check_rows, run_tree, tree64, wild
+from test_gpu_verify_stage import cfg
 
 pytestmark = pytest.mark.gpu
 
@@ -107,3 +110,56 @@ def test_an_entry_past_the_view_does_not_take_a_destination(cuda, n):
     got, want, status, between = move_run(cuda, [(8, 64), (12, 4096)], [0, 0], src, dst, pitch=16)
     assert status == 1 and between
     assert all((g == w).all() for g, w in zip(got, want))
+
+
+# ---- a stage's trees ------------------------------------------------------------------------------------------------
+
+SMALL = dict(hidden=512, inter=256, experts=16, top_k=4, num_blocks=20, seed=6, routing="softmax")
+RES = {"a": ([67, 68], [2, 3, 4, 5, 6, 7]), "b": ([69, 70], [8, 9, 10, 11, 12, 13])}
+AT = {"a": 130, "b": 30}
+
+
+def started(cuda, rng, **over):
+    from ssengine_b200.messages import Chunk, Plan
+    from ssengine_b200.stage import StageModel
+
+    st = StageModel(cfg(**{**SMALL, **over}), 0, cuda)
+    st.forward(Plan(0, [Chunk(r, 0, AT[r], *RES[r], True, rng.integers(0, 1000, AT[r]).tolist()) for r in "ab"]))
+    return st
+
+
+def step(k, names, trees, tokens, at=AT):
+    from ssengine_b200.messages import Chunk, Plan
+
+    return Plan(k, [Chunk(r, at[r], len(t), *RES[r], True, tok) for r, t, tok in zip(names, trees, tokens)])
+
+
+def test_trees_given_up_leave_no_rows(cuda):
+    """An acceptance of nothing, and a verify that fails on its way, leave no memory behind."""
+    st = started(cuda, np.random.default_rng(1))
+    trees, tokens = [[-1, 0, 0, 2], [-1, -1, 1]], [[1, 2, 3, 4], [5, 6, 7]]
+
+    def held():
+        gc.collect()
+        torch.cuda.synchronize()
+        return torch.cuda.memory_allocated(cuda)
+
+    st.verify(step(1, "ab", trees, tokens), trees)
+    st.accept([[0, 2], [1]])
+    before = held()
+    at = {"a": 132, "b": 31}
+    st.verify(step(2, "ab", trees, tokens, at), trees)
+    st.accept([[], []])
+    assert held() == before
+
+    def failing(layer, *_):
+        if layer is st.layers[-1]:
+            raise RuntimeError("a check")
+
+    st.layer_hook = failing
+    with pytest.raises(RuntimeError):
+        st.verify(step(3, "ab", trees, tokens, at), trees)
+    st.layer_hook = None
+    assert st.trees is None and held() == before
+    with pytest.raises(ValueError):
+        st.accept([[0], [0]])

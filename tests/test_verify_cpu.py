@@ -93,3 +93,35 @@ def test_a_step_that_fails_leaves_nothing_to_accept(monkeypatch):
     with pytest.raises(ValueError):
         st.verify(plan, [[-1, 1]])
     assert st.trees is None
+
+
+def test_what_the_layers_keep_ends_with_its_trees(monkeypatch):
+    """An acceptance of nothing and a verify that fails on its way leave none of the layers' rows alive."""
+    import gc
+    import weakref
+
+    from ssengine_b200.messages import Chunk, Plan
+    from ssengine_b200.stage import StageModel
+
+    st = object.__new__(StageModel)
+    st.trees, st.kda, st.device, rows = None, True, torch.device("cpu"), []
+    monkeypatch.setattr(st, "prepare", lambda plan: SimpleNamespace(order=[0], last_rows=None, dsa=None), raising=False)
+
+    def run(batch, hidden, edge, tree, fails=False):
+        tree.steps.append(torch.zeros(3))
+        rows.append(weakref.ref(tree.steps[0]))
+        if fails:
+            raise RuntimeError("a check")
+
+    plan = Plan(0, [Chunk("a", 3, 2, [1], [0] * 6, True, [4, 5])])
+    monkeypatch.setattr(st, "run", run, raising=False)
+    st.verify(plan, [[-1, 0]])
+    assert rows[0]() is not None
+    st.accept([[]])
+    gc.collect()
+    assert rows[0]() is None
+    monkeypatch.setattr(st, "run", lambda *a, **kw: run(*a, **kw, fails=True), raising=False)
+    with pytest.raises(RuntimeError):
+        st.verify(plan, [[-1, 0]])
+    gc.collect()
+    assert rows[1]() is None and st.trees is None
