@@ -37,6 +37,7 @@ The last stage's head: the mean of the 4 streams ("kda"), RMSNorm of each reques
 from __future__ import annotations
 
 import ctypes
+import weakref
 from dataclasses import dataclass, field
 
 import numpy as np
@@ -156,7 +157,7 @@ class Batch:
 class Trees:
     """The trees of one `StageModel.verify`: a plan's chunks with their parents, checked on the host, the device tensors of
     its rows (chunk by chunk in the plan's order: all are decode-class), and what each layer keeps of them for `accept`
-    (`steps`, in layer order)."""
+    (`steps`, in layer order; None once they are accepted)."""
 
     def __init__(self, chunks, trees, batch: Batch, device):
         from . import mla
@@ -321,7 +322,7 @@ class StageModel:
         self.cuda_graphs = cfg.cuda_graphs if cuda_graphs is None else cuda_graphs
         self.ipc_kv = ipc_kv
         self.layer_hook = None          # optional callable(layer, res, x_prev, post, comb) after each layer (checks)
-        self.trees = None               # the trees of the last `verify`, until `accept`
+        self.trees = None               # the trees of the last `verify`, until their `accept`
         self.moe_profile = None         # optional list: each MoE layer's forward records per-step CUDA events into it
         self._lib = lib.load()
         H, F, E = cfg.hidden, cfg.inter, cfg.experts
@@ -620,28 +621,34 @@ class StageModel:
         Returns what `forward` returns, the last stage the greedy token after every node, in the plan's order (`last_logits`
         its logits). The requests' states and pool keys stay as they are until `accept`, which comes before the stage's
         next step of these requests; a second `verify` in its place checks other trees. Until then every layer's inputs of the
-        nodes are kept."""
+        nodes are kept. `self.trees` is the step for its `accept`."""
         if not self.kda:
             raise ValueError('layer_kind "moe" has no requests to continue')
         self.trees = None                # a step that fails leaves nothing to accept
         batch = self.prepare(plan)
         step = Trees(plan.chunks, trees, batch, self.device)
         out = self.run(batch, hidden_in, edge_out, tree=step)
-        self.trees = step
+        step.stage, self.trees = weakref.ref(self), step
         return out
 
-    def accept(self, paths) -> None:
-        """Continues the requests of the last `verify` by a path of each tree (the nodes from a root down, () for none): the
-        KDA states advance along it (`KdaLayer.advance`), its latent rows move up to the context's end
-        (`StageKv.move_tokens`), its pool keys are inserted. Every stage of a pipeline takes the same paths."""
-        t = self.trees
-        if t is None:
+    def accept(self, paths, trees: "Trees | None" = None) -> None:
+        """Continues the requests of a `verify` by a path of each tree (the nodes from a root down, () for none): the KDA states
+        advance along it (`KdaLayer.advance`), its latent rows move up to the context's end (`StageKv.move_tokens`), its pool
+        keys are inserted. Every stage of a pipeline takes the same paths. `trees`: which step's, what `self.trees` was after
+        its `verify` (default: the last one's); with several microbatches verified before the first is accepted each has to
+        name its own. A step is accepted once."""
+        t = self.trees if trees is None else trees
+        if t is None or t.steps is None:
             raise ValueError("no trees to accept a path of")
+        if t.stage() is not self:
+            raise ValueError("the trees of another stage's verify")
         acc = t.accepted(paths)
-        self.trees = None
+        steps, t.steps = t.steps, None
+        if t is self.trees:
+            self.trees = None
         if acc is None:
             return
-        for layer, kept, state, dsa, grp in zip(self.layers, t.steps, self.kda_states, self.is_dsa, self.kda_group):
+        for layer, kept, state, dsa, grp in zip(self.layers, steps, self.kda_states, self.is_dsa, self.kda_group):
             if dsa:
                 layer.attn.accept(kept, acc["rows64"], acc["kpool"], acc["most"], t.page_table, state[1], state[2])
             else:

@@ -163,3 +163,37 @@ def test_trees_given_up_leave_no_rows(cuda):
     assert st.trees is None and held() == before
     with pytest.raises(ValueError):
         st.accept([[0], [0]])
+
+
+def test_several_trees_in_flight(cuda):
+    """Two microbatches verified before either is accepted, accepted in the other order: what each alone leaves."""
+    rng = [np.random.default_rng(2) for _ in range(2)]
+    st, ref = (started(cuda, r) for r in rng)
+    trees = {"a": [-1, 0, 0, 2, 1], "b": [-1, 0, -1, 1]}
+    tokens = {"a": [9, 8, 7, 6, 5], "b": [4, 3, 2, 1]}
+    paths = {"a": [0, 2, 3], "b": [0, 1, 3]}                  # b's is a path of a's tree too, as far as it goes
+    got, open_ = {}, {}
+    for k, r in enumerate("ab"):
+        st.verify(step(1 + k, r, [trees[r]], [tokens[r]]), [trees[r]])
+        got[r], open_[r] = st.last_logits.clone(), st.trees
+    for r in "ab":
+        st.accept([paths[r]], trees=open_[r])
+    for r in "ab":
+        with pytest.raises(ValueError):                       # a step is accepted once
+            st.accept([paths[r]], trees=open_[r])
+    for k, r in enumerate("ab"):
+        ref.verify(step(1 + k, r, [trees[r]], [tokens[r]]), [trees[r]])
+        assert torch.equal(got[r], ref.last_logits)
+        ref.accept([paths[r]])
+    torch.cuda.synchronize()
+    same = lambda x, y: torch.equal(x.contiguous().view(torch.uint8), y.contiguous().view(torch.uint8))
+    for a, b, dsa in zip(st.kda_states, ref.kda_states, st.is_dsa):
+        if dsa:
+            assert same(a[1], b[1]) and same(a[2], b[2])
+        else:
+            blocks = RES["a"][1] + RES["b"][1]
+            assert all(same(u[blocks], v[blocks]) for u, v in zip(a, b))
+    at = {r: AT[r] + len(paths[r]) for r in "ab"}
+    more = step(5, "ab", [[-1], [-1]], [[11], [12]], at)
+    assert torch.equal(st.decode(more), ref.decode(more)) and torch.equal(st.last_logits, ref.last_logits)
+    assert int(st.status.item()) == 0 and int(ref.status.item()) == 0

@@ -125,3 +125,36 @@ def test_what_the_layers_keep_ends_with_its_trees(monkeypatch):
         st.verify(plan, [[-1, 0]])
     gc.collect()
     assert rows[1]() is None and st.trees is None
+
+
+def test_each_step_in_flight_is_accepted_by_name_and_once(monkeypatch):
+    from ssengine_b200.messages import Chunk, Plan
+    from ssengine_b200.stage import StageModel
+
+    st = object.__new__(StageModel)
+    st.trees, st.kda, st.device = None, True, torch.device("cpu")
+    st.status, st.kda_states, st.is_dsa, st.kda_group, took = None, [("conv", "rec")], [False], [0], []
+    attn = SimpleNamespace(accept=lambda kept, rows, seqs, *_: took.append((kept, rows.tolist(), seqs[0].tolist())))
+    st.layers = [SimpleNamespace(attn=attn)]
+    monkeypatch.setattr(st, "prepare", lambda plan: SimpleNamespace(order=[0], last_rows=None, dsa=None), raising=False)
+    monkeypatch.setattr(st, "run", lambda b, h, e, tree: tree.steps.append(tree.chunks[0].req_id), raising=False)
+    held = {}
+    for i, r in enumerate("abc"):
+        st.verify(Plan(i, [Chunk(r, 3 + i, 3, [1], [20 * i + g for g in range(6)], True, [4, 5, 6])]), [[-1, 0, 0]])
+        held[r] = st.trees
+    st.accept([[0, 1]], trees=held["a"])
+    assert st.trees is held["c"]
+    with pytest.raises(ValueError):
+        st.accept([[0]], trees=held["a"])
+    with pytest.raises(ValueError):
+        st.accept([[1]], trees=held["b"])                  # no path: the step stays open
+    other = object.__new__(StageModel)
+    other.trees, other.kda = None, True
+    with pytest.raises(ValueError):
+        other.accept([[0]], trees=held["b"])
+    st.accept([[0]], trees=held["b"])
+    st.accept([[0, 2]])
+    assert took == [("a", [0, 1], [0, 2, 0, 1]), ("b", [0], [0, 1, 20, 1]), ("c", [0, 2], [0, 2, 40, 1])]
+    assert st.trees is None
+    with pytest.raises(ValueError):
+        st.accept([[0, 2]], trees=held["c"])
