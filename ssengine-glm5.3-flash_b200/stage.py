@@ -51,6 +51,7 @@ BLOCK_TOKENS = 8576
 KERNEL_BLOCK = 64
 GRAPH_BUCKETS = (128,) + tuple(range(256, 8192 + 1, 256))
 PACK_ALIGN = 256
+SELECTED_TOKENS = 4 * 512 + 3          # what the DSA layers' indexer selects at most: 512 pools of 4 tokens and the tail
 
 
 def row_order(num_tokens: list[int]) -> list[int]:
@@ -173,6 +174,7 @@ class Trees:
             m, d = mla.tree_masks(t)
             masks.append(m)
             depths.append(d + c.start)
+        self.reach = max([int(d.max()) + 1 for d in depths if d.numel()], default=0)     # tokens that a node sees
         self.first = np.cumsum([0] + [len(t) for t in self.trees])
         self.most = max([len(t) for t in self.trees] + [1])
         n = int(self.first[-1])
@@ -613,11 +615,18 @@ class StageModel:
         date). Chunks of any length are right; the chunked forms of `forward` are faster for long ones."""
         return self.run(self.prepare(plan), hidden_in, decode=attention)
 
-    def verify(self, plan, trees, hidden_in: torch.Tensor | None = None, edge_out=None) -> torch.Tensor | None:
+    def verify(self, plan, trees, hidden_in: torch.Tensor | None = None, edge_out=None,
+               attention: str = "selected") -> torch.Tensor | None:
         """One step of trees of drafted tokens, checked at once: a plan whose chunks hold a tree each (token_ids its nodes'
         tokens, num_tokens its nodes, at most 64, kv_pages for all of them behind the context) and `trees`, each chunk's
         parents (a parent before its children, -1: the context's last token). Every node is computed as if its path followed
-        the context: `KdaLayer.decode_tree` in the KDA layers, `mla.decode_tree` (over the whole context) in the DSA layers.
+        the context: `KdaLayer.decode_tree` in the KDA layers, `mla.decode_tree` in the DSA layers.
+
+        That attention is over the whole context. `attention` is what the caller's other steps have: "selected" (`forward`, and
+        `decode` by default) is the same as long as the indexer's selection is all that a node sees, 2,051 tokens with the
+        node; a node that sees more is refused (ValueError), for its token would not be theirs. "dense" checks drafts of
+        any length against `decode(attention="dense")`.
+
         Returns what `forward` returns, the last stage the greedy token after every node, in the plan's order (`last_logits`
         its logits). The requests' states and pool keys stay as they are until `accept`, which comes before the stage's
         next step of these requests; a second `verify` in its place checks other trees. Until then every layer's inputs of the
@@ -625,8 +634,13 @@ class StageModel:
         if not self.kda:
             raise ValueError('layer_kind "moe" has no requests to continue')
         self.trees = None                # a step that fails leaves nothing to accept
+        if attention not in ("selected", "dense"):
+            raise ValueError(f"attention {attention!r}")
         batch = self.prepare(plan)
         step = Trees(plan.chunks, trees, batch, self.device)
+        if attention == "selected" and step.reach > SELECTED_TOKENS and self.cfg.layer_kind == "hybrid":
+            raise ValueError(f"a node that sees {step.reach} tokens, the indexer selects {SELECTED_TOKENS}: there is no tree "
+                             'form over selected tokens (attention="dense": over the whole context, as decode\'s)')
         out = self.run(batch, hidden_in, edge_out, tree=step)
         step.stage, self.trees = weakref.ref(self), step
         return out

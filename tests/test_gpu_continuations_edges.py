@@ -197,3 +197,33 @@ def test_several_trees_in_flight(cuda):
     more = step(5, "ab", [[-1], [-1]], [[11], [12]], at)
     assert torch.equal(st.decode(more), ref.decode(more)) and torch.equal(st.last_logits, ref.last_logits)
     assert int(st.status.item()) == 0 and int(ref.status.item()) == 0
+
+
+def test_a_node_past_the_selection_is_as_the_dense_decode(cuda):
+    """Behind a context that the indexer would choose from, `verify` takes the whole context only where it is told to; a chain
+    is then the dense decode of the same tokens, row by row (the attention is one operator's arithmetic, the recurrence's
+    closed form differs: the stage's chained bound, 6e-2)."""
+    from ssengine_b200.messages import Chunk, Plan
+    from ssengine_b200.stage import StageModel
+
+    rng = np.random.default_rng(4)
+    n, tree = 2049, [-1, 0, 1]
+    res = (list(range(67, 67 + 17)), [3, 4, 5, 6, 7, 8])
+    prompt, draft = rng.integers(0, 1000, n).tolist(), rng.integers(0, 1000, 3).tolist()
+    st, ref = (StageModel(cfg(**{**SMALL, "mb_tokens": 2176}), 0, cuda) for _ in range(2))
+    for s in (st, ref):
+        s.forward(Plan(0, [Chunk("a", 0, n, *res, True, prompt)]))
+    plan = Plan(1, [Chunk("a", n, 3, *res, True, draft)])
+    with pytest.raises(ValueError, match="selected"):
+        st.verify(plan, [tree])
+    assert st.trees is None
+    short = Plan(1, [Chunk("a", n, 2, *res, True, draft[:2])])
+    st.verify(short, [[-1, 0]])                               # 2,051 tokens: the selection is all of them
+    st.verify(plan, [tree], attention="dense")
+    logits = st.last_logits.clone()
+    for i in range(3):
+        ref.decode(Plan(2 + i, [Chunk("a", n + i, 1, *res, True, draft[i:i + 1])]), attention="dense")
+        got, want = logits[i].double(), ref.last_logits[0].double()
+        assert float((got - want).norm() / want.norm()) < 6e-2, i
+    with pytest.raises(ValueError):
+        st.verify(plan, [tree], attention="sparse")

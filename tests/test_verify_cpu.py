@@ -158,3 +158,29 @@ def test_each_step_in_flight_is_accepted_by_name_and_once(monkeypatch):
     assert st.trees is None
     with pytest.raises(ValueError):
         st.accept([[0, 2]], trees=held["c"])
+
+
+@pytest.mark.parametrize("kind", ["hybrid", "kda"])
+def test_nodes_past_the_selection_are_refused_unless_dense(monkeypatch, kind):
+    from ssengine_b200.layers import DsaAttention
+    from ssengine_b200.messages import Chunk, Plan
+    from ssengine_b200.stage import SELECTED_TOKENS, StageModel
+
+    assert SELECTED_TOKENS == 4 * DsaAttention.TOPK + 3
+    st = object.__new__(StageModel)
+    st.trees, st.kda, st.device, st.cfg = None, True, torch.device("cpu"), SimpleNamespace(layer_kind=kind)
+    monkeypatch.setattr(st, "prepare", lambda plan: SimpleNamespace(order=[0, 1], last_rows=None, dsa=None), raising=False)
+    monkeypatch.setattr(st, "run", lambda *a, **kw: "rows", raising=False)
+    trees = [[-1, -1], [-1, 0, 0, 1]]                       # the second is three nodes deep
+    at = lambda start: Plan(0, [Chunk(r, n, len(t), [1], [0] * 6, True, [0] * len(t))
+                                for r, n, t in zip("ab", (5, start), trees)])
+    assert st.verify(at(2048), trees) == "rows"             # 2,051 tokens
+    if kind == "hybrid":
+        with pytest.raises(ValueError, match="2052"):
+            st.verify(at(2049), trees)
+        assert st.trees is None
+    else:
+        assert st.verify(at(2049), trees) == "rows"         # no attention that selects
+    assert st.verify(at(2049), trees, attention="dense") == "rows" and st.trees.reach == 2052
+    with pytest.raises(ValueError):
+        st.verify(at(5), trees, attention="none")
