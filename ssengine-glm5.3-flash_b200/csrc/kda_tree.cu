@@ -731,14 +731,12 @@ constexpr int smem_bytes() {
 }
 
 template <int N>
+bool set_smem() {
+  return cudaFuncSetAttribute(kda_tree_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<N>()) == cudaSuccess;
+}
+
+template <int N>
 int launch_nodes(const KdaArgs& a, cudaStream_t stream) {
-  static OncePerDevice attr;
-  int device = 0;
-  const auto set = [] {
-    return cudaFuncSetAttribute(kda_tree_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<N>()) ==
-           cudaSuccess;
-  };
-  if (cudaGetDevice(&device) != cudaSuccess || !attr.done(device, set)) return kErrCuda;
   kda_tree_kernel<N><<<(unsigned)(a.R * a.H), Shape<N>::kThreads, smem_bytes<N>(), stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
 }
@@ -751,6 +749,10 @@ int launch_kda_tree(const KdaArgs& a, cudaStream_t stream) {
     return kErrArgs;
   if (a.R == 0) return kOk;
   if ((int64_t)a.R * a.H > 0x7fffffff) return kErrArgs;
+  static OncePerDevice attr;                     // of all sizes at once: which one a later call takes depends on its trees
+  int device = 0;
+  const auto set = [] { return set_smem<16>() && set_smem<32>() && set_smem<64>(); };
+  if (cudaGetDevice(&device) != cudaSuccess || !attr.done(device, set)) return kErrCuda;
   if (a.max_nodes <= 16) return launch_nodes<16>(a, stream);
   // up to 32 nodes four smaller CTAs an SM, unless the larger ones all run at once: 1 x 24 nodes, 32 heads 15.6 and 13.9 us,
   // 4 x 24, 64 heads 19.7 and 19.1, 6 x 24, 64 heads 24.2 and 29.8

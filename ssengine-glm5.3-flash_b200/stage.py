@@ -393,9 +393,10 @@ class StageModel:
         forward stalls the host for up to tens of milliseconds while the GPU drains its queue): the indexer's logits
         rows at `max_context` and the decode forms' workspace for `mb_tokens` rows (buffers that the stage's DSA layers
         share; they run in order on one stream), the KDA / mHC chunk workspace for `reserve_reqs` requests, one forward
-        of a dummy request of a full microbatch and one step of a token in each decode form (written into the null
-        block's pages and state) that load every kernel and leave their temporaries in the caching allocator for the
-        next microbatches; then the MoE layers' shared workspace."""
+        of a dummy request of a full microbatch, one step of a token in each decode form, and one as a tree that is
+        accepted (written into the null block's pages and state), that load every kernel and leave their temporaries in the
+        caching allocator for the next microbatches; then the MoE layers' shared workspace. What a verify keeps until its
+        acceptance is not reserved: it grows with the trees' nodes."""
         from .messages import Chunk, Plan
 
         cfg = self.cfg
@@ -424,6 +425,8 @@ class StageModel:
             token = Plan(-1, [Chunk("warmup", n - 1, 1, pages, [0] * 6, True, [0] if self.first else None)])
             for form in ("selected", "dense") if any(self.is_dsa) else ("selected",):
                 self.decode(token, None if self.first else hidden[:1], form)
+            self.verify(token, [[-1]], None if self.first else hidden[:1], attention="dense")
+            self.accept([[0]])
         moes = [layer.moe if self.kda else layer for layer in self.layers]
         moes = [m for m in moes if isinstance(m, moe.MoELayer)]
         ws = max(m.workspace_bytes(self.cfg.mb_tokens) for m in moes) if moes else 0

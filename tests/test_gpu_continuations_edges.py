@@ -227,3 +227,36 @@ def test_a_node_past_the_selection_is_as_the_dense_decode(cuda):
         assert float((got - want).norm() / want.norm()) < 6e-2, i
     with pytest.raises(ValueError):
         st.verify(plan, [tree], attention="sparse")
+
+
+def test_a_stages_first_trees_use_what_its_build_reserved(cuda, monkeypatch):
+    """The first verify and accept ask for no workspace, map no memory and load no kernel that the build did not run."""
+    from ssengine_b200 import kvpages, lib
+
+    ran = []
+    real = lib.load()
+
+    class Recorded:
+        def __getattr__(self, name):
+            f = getattr(real, name)
+            if not name.startswith("ssb_"):
+                return f
+            return lambda *a: (ran.append(name), f(*a))[1]
+
+    monkeypatch.setattr(lib, "load", lambda path=None: Recorded())
+    st = started(cuda, np.random.default_rng(3))
+    built = set(ran)
+    assert {"ssb_kda_decode_tree", "ssb_kda_advance", "ssb_mla_decode_tree", "ssb_move_rows"} <= built
+
+    def none(*_):
+        raise AssertionError("a step asked for a workspace")
+
+    monkeypatch.setattr(lib, "stream_scratch", none)
+    torch.cuda.synchronize()
+    mapped = torch.cuda.memory_reserved(cuda)
+    trees = [[-1, 0, 0, 2], [-1, -1, 1]]
+    st.verify(step(1, "ab", trees, [[1, 2, 3, 4], [5, 6, 7]]), trees)
+    st.accept([[0, 2], [1]])
+    torch.cuda.synchronize()
+    assert set(ran) == built and torch.cuda.memory_reserved(cuda) == mapped
+    assert int(st.status.item()) == 0 and st.trees is None
