@@ -208,7 +208,9 @@ int ssb_kda_decode(const ssb_kda_layer* layer, const void* x, int64_t ldx, const
  * request's state block, or zeros where the sequence has none), its conv taps the rows on its path and behind them the
  * block's conv rows. Every node's output to its row of out; the state blocks are read and left as they are. Arguments
  * otherwise as ssb_kda_decode; several sequences may read one block. A sequence that reaches outside [0, T), has more than
- * max_nodes rows or a parent that is not before its child, or names a negative block, is skipped with status 1. */
+ * max_nodes rows or a parent that is not before its child, or names a negative block, is skipped with status 1. The state
+ * and the vectors enter their products with 16 bits each (ssb_kda_decode's have 24): beside its bf16 rounding an output is
+ * off by up to 2^-15 of the state row's norm / sqrt(128), which counts where a state is hundreds of times its outputs. */
 int ssb_kda_decode_tree(const ssb_kda_layer* layer, const void* x, int64_t ldx, const void* g, int64_t ldg,
                         const void* beta, int64_t ldb, int64_t T, const int32_t* parents, const int32_t* seqs, int64_t R,
                         int32_t max_nodes, void* out, int64_t ldo, int32_t* status, void* stream);

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from test_gpu_beam import run as beam_run
-from test_gpu_decode import kda_make
+from test_gpu_decode import D, kda_make
 from test_gpu_move import run as move_run
 from test_gpu_tree import check_rows, run_tree, tree64, wild
 from test_gpu_verify_stage import cfg
@@ -40,6 +40,37 @@ def test_more_nodes_than_stated_are_skipped_whatever_the_batch(cuda, most, reque
         want = tree64(d, [seqs[r] for r in pick], [trees[r] for r in pick], H)
         for r in pick:
             check_rows(out[ends[r]:ends[r + 1]], want[ends[r]:ends[r + 1]], H)
+
+
+@pytest.mark.parametrize("size", [3.0, 100.0])
+def test_states_far_larger_than_the_outputs(cuda, size):
+    """A node's value takes the place of what the state has for its key, and its query is that key: the output is the value's,
+    a small difference of products of the state. The state and the vectors enter their product as two bf16 parts (2^-9, and
+    2^-9 of that is what they leave), high x high, high x low and low x high: a product s x is off by 3 x 2^-18 |s x| at
+    most, and the tensor core's sums by another 2^-18 of the magnitudes: 2^-16. The two products (with k and with q, the
+    first's share weighted by k . q) make it twice that of the magnitudes' sum, beside the bf16 store's 2^-8 and the
+    tests' 1e-3 of the row's largest for the rest."""
+    rng = np.random.default_rng(int(size))
+    H, n = 2, 6
+    P = H * D
+    d = kda_make(rng, n, H, 1)
+    d["rst"] = (rng.standard_normal((1, H, D, D)) * size).astype(np.float32)
+    d["x"][:, :P] = d["x"][:, P:2 * P]                       # queries as keys, through the same conv
+    d["w"][:P] = d["w"][P:2 * P]
+    d["cst"][:, :, :P] = d["cst"][:, :, P:2 * P]
+    d["g"][:] = -30.0                                        # decays of 1
+    d["beta"][:] = 30.0                                      # the state's value for the key is replaced
+    d = {k: (torch.from_numpy(np.ascontiguousarray(v)).to(torch.bfloat16).float().numpy() if k in ("g", "beta", "x") else v)
+         for k, v in d.items()}
+    tree, seqs = [-1] * n, [(0, n, 0, 1)]
+    want = tree64(d, seqs, [tree], H).reshape(n, H, D)
+    out, status = run_tree(cuda, d, H, seqs, tree)
+    assert status == 0
+    out = out.reshape(n, H, D)
+    # the keys' magnitudes times the state's: at most the 2-norm of the state's row (the key's is 1)
+    mass = np.linalg.norm(d["rst"][0].astype(np.float64), axis=2) * D ** -0.5
+    bar = 2.0 ** -8 * np.abs(want) + 1e-3 * np.abs(want).max(axis=2, keepdims=True) + 2 * 2.0 ** -16 * mass
+    assert (np.abs(out - want) <= bar).all(), (np.abs(out - want) / bar).max()
 
 
 # ---- beam selection -------------------------------------------------------------------------------------------------
