@@ -495,12 +495,15 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
   }
 }
 
-// Parts a row is cut into, the same for every row (equal rows get equal sums): about what fills the SMs once (64 x 8 beams:
-// one part 76 us, five 107 with loads alone, since every part begins and ends with its lists), none short, the candidates of
-// a request within bounds.
+// Parts a row is cut into, the same for every row (equal rows get equal sums) and on every device: as many as run at once, none
+// short, the candidates of a request within bounds. Every part begins and ends with its lists, so a second wave costs more
+// than it evens out: cut for 592 CTAs instead of 444, 2 x 4 beams take 19.3 us instead of 14.2, 4 x 8 28.8 (22.6), 16 x 4
+// 34.0 (26.9); where rows alone fill the SMs, 64 x 8 beams, one part a row takes 91 us, two 96, four 114, and with a fifth
+// finished 61, 77 and 96 (rows that do not lie on 16 bytes: 240, 198 and 201).
+constexpr int kAtOnce = 148 * kScanBlocks;
 int beam_parts(int64_t G, int64_t B, int64_t V, int64_t k) {
   const int64_t rows = G * B;
-  int64_t parts = rows > 0 ? 148 * 4 / rows : 1;
+  int64_t parts = rows > 0 ? kAtOnce / rows : 1;
   parts = parts < V / kMinPart ? parts : V / kMinPart;
   parts = parts < kMaxCandidates / (B * k) ? parts : kMaxCandidates / (B * k);
   return static_cast<int>(parts > 1 ? parts : 1);

@@ -253,3 +253,12 @@ def test_beam_workspace_sizes():
     so = lib.load()
     for bad in ((-1, 4, 100, 4), (1, 0, 100, 4), (1, 4, 0, 4), (1, 4, 1 << 31, 4), (1, 4, 100, 65)):
         assert so.ssb_beam_workspace_bytes(*bad) == -1
+
+
+def test_beam_rows_are_cut_into_what_runs_at_once():
+    """A part's keys and its sum (16 bytes) for each CTA: no more than 3 on each of 148 SMs unless the rows alone are more."""
+    from ssengine_b200 import beam
+
+    for G, B, k in ((1, 4, 4), (2, 4, 4), (4, 8, 8), (16, 4, 4), (16, 8, 8), (37, 4, 1), (64, 8, 8), (148, 4, 16)):
+        most = max(148 * 3, G * B)
+        assert beam.workspace_bytes(G, B, 151552, k) <= most * (8 * k + 16) + 512, (G, B, k)
