@@ -51,7 +51,7 @@ BLOCK_TOKENS = 8576
 KERNEL_BLOCK = 64
 GRAPH_BUCKETS = (128,) + tuple(range(256, 8192 + 1, 256))
 PACK_ALIGN = 256
-SELECTED_TOKENS = 4 * 512 + 3          # what the DSA layers' indexer selects at most: 512 pools of 4 tokens and the tail
+SELECTED_TOKENS = 4 * 512 + 3          # what the indexer selects at most: 512 pools of 4 tokens and the tail
 
 
 def row_order(num_tokens: list[int]) -> list[int]:
@@ -156,9 +156,9 @@ class Batch:
 
 
 class Trees:
-    """The trees of one `StageModel.verify`: a plan's chunks with their parents, checked on the host, the device tensors of
-    its rows (chunk by chunk in the plan's order: all are decode-class), and what each layer keeps of them for `accept`
-    (`steps`, in layer order; None once they are accepted)."""
+    """The trees of one `StageModel.verify`: a plan's chunks with their parents, checked on the host, the device
+    tensors of its rows (chunk by chunk in the plan's order: all are decode-class), and what each layer keeps of
+    them for `accept` (`steps`, in layer order; None once they are accepted)."""
 
     def __init__(self, chunks, trees, batch: Batch, device):
         from . import mla
@@ -303,6 +303,8 @@ def bench_config(mb_tokens: int, checkpoint: str | None = None, cuda_graphs: boo
 
 
 class StageModel:
+    _open = ()                          # the steps verified and not accepted (weak: who accepts one holds it)
+
     def __init__(self, cfg, stage: int, device, *, num_blocks: int | None = None, warmup: bool = True,
                  cuda_graphs: bool | None = None, ipc_kv: bool = False, extra_blocks: int = 0):
         """cfg: a `StageConfig`, or the reference's run config (read by `stage_settings`)."""
@@ -390,13 +392,13 @@ class StageModel:
 
     def _warm(self) -> None:
         """Reserves the device memory a microbatch needs, so that no forward maps new memory (a cudaMalloc inside a
-        forward stalls the host for up to tens of milliseconds while the GPU drains its queue): the indexer's logits
-        rows at `max_context` and the decode forms' workspace for `mb_tokens` rows (buffers that the stage's DSA layers
-        share; they run in order on one stream), the KDA / mHC chunk workspace for `reserve_reqs` requests, one forward
-        of a dummy request of a full microbatch, one step of a token in each decode form, and one as a tree that is
-        accepted (written into the null block's pages and state), that load every kernel and leave their temporaries in the
-        caching allocator for the next microbatches; then the MoE layers' shared workspace. What a verify keeps until its
-        acceptance is not reserved: it grows with the trees' nodes."""
+        forward stalls the host for up to tens of milliseconds while the GPU drains its queue): the indexer's
+        logits rows at `max_context` and the decode forms' workspace for `mb_tokens` rows (buffers that the stage's
+        DSA layers share; they run in order on one stream), the KDA / mHC chunk workspace for `reserve_reqs`
+        requests, one forward of a dummy request of a full microbatch, one step of a token in each decode form, and
+        one as a tree that is accepted (written into the null block's pages and state), that load every kernel and
+        leave their temporaries in the caching allocator for the next microbatches; then the MoE layers' shared
+        workspace. What a verify keeps until its acceptance is not reserved: it grows with the trees' nodes."""
         from .messages import Chunk, Plan
 
         cfg = self.cfg
@@ -620,20 +622,22 @@ class StageModel:
 
     def verify(self, plan, trees, hidden_in: torch.Tensor | None = None, edge_out=None,
                attention: str = "selected") -> torch.Tensor | None:
-        """One step of trees of drafted tokens, checked at once: a plan whose chunks hold a tree each (token_ids its nodes'
-        tokens, num_tokens its nodes, at most 64, kv_pages for all of them behind the context) and `trees`, each chunk's
-        parents (a parent before its children, -1: the context's last token). Every node is computed as if its path followed
-        the context: `KdaLayer.decode_tree` in the KDA layers, `mla.decode_tree` in the DSA layers.
+        """One step of trees of drafted tokens, checked at once: a plan whose chunks hold a tree each (token_ids its
+        nodes' tokens, num_tokens its nodes, at most 64, kv_pages for all of them behind the context) and `trees`,
+        each chunk's parents (a parent before its children, -1: the context's last token). Every node is computed
+        as if its path followed the context: `KdaLayer.decode_tree` in the KDA layers, `mla.decode_tree` in the DSA
+        layers.
 
-        That attention is over the whole context. `attention` is what the caller's other steps have: "selected" (`forward`, and
-        `decode` by default) is the same as long as the indexer's selection is all that a node sees, 2,051 tokens with the
-        node; a node that sees more is refused (ValueError), for its token would not be theirs. "dense" checks drafts of
-        any length against `decode(attention="dense")`.
+        That attention is over the whole context. `attention` is what the caller's other steps have: "selected"
+        (`forward`, and `decode` by default) is the same as long as the indexer's selection is all that a node sees,
+        2,051 tokens with the node; a node that sees more is refused (ValueError), for its token need not be theirs.
+        "dense" checks drafts of any length against `decode(attention="dense")`.
 
-        Returns what `forward` returns, the last stage the greedy token after every node, in the plan's order (`last_logits`
-        its logits). The requests' states and pool keys stay as they are until `accept`, which comes before the stage's
-        next step of these requests; a second `verify` in its place checks other trees. Until then every layer's inputs of the
-        nodes are kept. `self.trees` is the step for its `accept`."""
+        Returns what `forward` returns, the last stage the greedy token after every node, in the plan's order
+        (`last_logits` its logits). The requests' states and pool keys stay as they are until `accept`, which comes
+        before the stage's next step of these requests; a second `verify` of one of them in its place checks other
+        trees (the first step cannot be accepted any more). Until then every layer's inputs of the nodes are kept.
+        `self.trees` is the step for its `accept`."""
         if not self.kda:
             raise ValueError('layer_kind "moe" has no requests to continue')
         self.trees = None                # a step that fails leaves nothing to accept
@@ -642,23 +646,34 @@ class StageModel:
         batch = self.prepare(plan)
         step = Trees(plan.chunks, trees, batch, self.device)
         if attention == "selected" and step.reach > SELECTED_TOKENS and self.cfg.layer_kind == "hybrid":
-            raise ValueError(f"a node that sees {step.reach} tokens, the indexer selects {SELECTED_TOKENS}: there is no tree "
-                             'form over selected tokens (attention="dense": over the whole context, as decode\'s)')
+            raise ValueError(f"a node that sees {step.reach} tokens, the indexer selects {SELECTED_TOKENS}: there is no "
+                             'tree form over selected tokens (attention="dense": over the whole context, as decode\'s)')
+        # an open step with one of these requests ends: its nodes' cache rows are this step's from here on
+        names = {c.req_id for c in step.chunks}
+        for t in self._open_steps():
+            if not names.isdisjoint(c.req_id for c in t.chunks):
+                t.steps = None
         out = self.run(batch, hidden_in, edge_out, tree=step)
         step.stage, self.trees = weakref.ref(self), step
+        self._open = [*map(weakref.ref, self._open_steps()), weakref.ref(step)]
         return out
 
+    def _open_steps(self) -> list:
+        return [t for t in (ref() for ref in self._open) if t is not None and t.steps is not None]
+
     def accept(self, paths, trees: "Trees | None" = None) -> None:
-        """Continues the requests of a `verify` by a path of each tree (the nodes from a root down, () for none): the KDA states
-        advance along it (`KdaLayer.advance`), its latent rows move up to the context's end (`StageKv.move_tokens`), its pool
-        keys are inserted. Every stage of a pipeline takes the same paths. `trees`: which step's, what `self.trees` was after
-        its `verify` (default: the last one's); with several microbatches verified before the first is accepted each has to
-        name its own. A step is accepted once."""
+        """Continues the requests of a `verify` by a path of each tree (the nodes from a root down, () for none): the
+        KDA states advance along it (`KdaLayer.advance`), its latent rows move up to the context's end
+        (`StageKv.move_tokens`), its pool keys are inserted. Every stage of a pipeline takes the same paths.
+        `trees`: which step's, what `self.trees` was after its `verify` (default: the last one's); with several
+        microbatches verified before the first is accepted each has to name its own. A step is accepted once."""
         t = self.trees if trees is None else trees
         if t is None or t.steps is None:
             raise ValueError("no trees to accept a path of")
         if t.stage() is not self:
             raise ValueError("the trees of another stage's verify")
+        if trees is None and len(self._open_steps()) > 1:
+            raise ValueError("several verified steps are held: accept takes the trees of one")
         acc = t.accepted(paths)
         steps, t.steps = t.steps, None
         if t is self.trees:

@@ -1,5 +1,5 @@
-"""Calls of the operators for several continuations of a request that their documentation allows and the tests beside them do
-not make. Tolerances, derived before the first run, stand at each test."""
+"""Calls of the operators for several continuations of a request that their documentation allows and the tests beside
+them do not make. Tolerances, derived before the first run, stand at each test."""
 
 import gc
 
@@ -22,8 +22,8 @@ pytestmark = pytest.mark.gpu
 @pytest.mark.parametrize("most", [1, 5, 16, 20, 24, 32, 40, 63])
 @pytest.mark.parametrize("requests", [2, 67])
 def test_more_nodes_than_stated_are_skipped_whatever_the_batch(cuda, most, requests):
-    """Trees of max_nodes nodes and of one and several more, in a batch that runs at once and in a larger one: the latter are
-    skipped with status 1 and their rows left."""
+    """Trees of max_nodes nodes and of one and several more, in a batch that runs at once and in a larger one: the
+    latter are skipped with status 1 and their rows left."""
     rng = np.random.default_rng(most)
     H = 5
     for over in (1, min(64, most + 16) - most):
@@ -44,12 +44,12 @@ def test_more_nodes_than_stated_are_skipped_whatever_the_batch(cuda, most, reque
 
 @pytest.mark.parametrize("size", [3.0, 100.0])
 def test_states_far_larger_than_the_outputs(cuda, size):
-    """A node's value takes the place of what the state has for its key, and its query is that key: the output is the value's,
-    a small difference of products of the state. The state and the vectors enter their product as two bf16 parts (2^-9, and
-    2^-9 of that is what they leave), high x high, high x low and low x high: a product s x is off by 3 x 2^-18 |s x| at
-    most, and the tensor core's sums by another 2^-18 of the magnitudes: 2^-16. The two products (with k and with q, the
-    first's share weighted by k . q) make it twice that of the magnitudes' sum, beside the bf16 store's 2^-8 and the
-    tests' 1e-3 of the row's largest for the rest."""
+    """A node's value takes the place of what the state has for its key, and its query is that key: the output is the
+    value's, a small difference of products of the state. The state and the vectors enter their product as two bf16
+    parts (2^-9, and 2^-9 of that is what they leave), high x high, high x low and low x high: a product s x is off
+    by 3 x 2^-18 |s x| at most, and the tensor core's sums by another 2^-18 of the magnitudes: 2^-16. The two
+    products (with k and with q, the first's share weighted by k . q) make it twice that of the magnitudes' sum,
+    beside the bf16 store's 2^-8 and the tests' 1e-3 of the row's largest for the rest."""
     rng = np.random.default_rng(int(size))
     H, n = 2, 6
     P = H * D
@@ -60,8 +60,8 @@ def test_states_far_larger_than_the_outputs(cuda, size):
     d["cst"][:, :, :P] = d["cst"][:, :, P:2 * P]
     d["g"][:] = -30.0                                        # decays of 1
     d["beta"][:] = 30.0                                      # the state's value for the key is replaced
-    d = {k: (torch.from_numpy(np.ascontiguousarray(v)).to(torch.bfloat16).float().numpy() if k in ("g", "beta", "x") else v)
-         for k, v in d.items()}
+    to_bf16 = lambda v: torch.from_numpy(np.ascontiguousarray(v)).to(torch.bfloat16).float().numpy()
+    d = {k: to_bf16(v) if k in ("g", "beta", "x") else v for k, v in d.items()}
     tree, seqs = [-1] * n, [(0, n, 0, 1)]
     want = tree64(d, seqs, [tree], H).reshape(n, H, D)
     out, status = run_tree(cuda, d, H, seqs, tree)
@@ -77,8 +77,8 @@ def test_states_far_larger_than_the_outputs(cuda, size):
 
 
 def lse_errors(cuda, x, bf16=False):
-    """Rows x as requests of one beam whose score makes the best candidate's about 0, where float32 is fine: the kernel's
-    log sums less the true ones, and the largest logits."""
+    """Rows x as requests of one beam whose score makes the best candidate's about 0, where float32 is fine: the
+    kernel's log sums less the true ones, and the largest logits."""
     t = torch.from_numpy(np.ascontiguousarray(x, np.float32)).to(torch.bfloat16 if bf16 else torch.float32)
     x = t.double().numpy()
     top = x.max(axis=1)
@@ -93,8 +93,8 @@ def lse_errors(cuda, x, bf16=False):
 @pytest.mark.parametrize("bf16", [False, True])
 def test_log_sums_of_peaked_rows(cuda, V, bf16):
     """One logit 20 to 40 above the rest, wherever it lies. Its term is the reference's own, 1; the others are at most
-    151,552 e^-16 = 2 % of it, each right to 2^-18: 1e-7, and 2^-24 of the score's own magnitude (below 2 %). No score is
-    above its beam's."""
+    151,552 e^-16 = 2 % of it, each right to 2^-18: 1e-7, and 2^-24 of the score's own magnitude (below 2 %). No
+    score is above its beam's."""
     rng = np.random.default_rng(V)
     rows = 48
     x = rng.uniform(-2, 2, (rows, V)).astype(np.float32)
@@ -112,15 +112,17 @@ def test_log_sums_of_peaked_rows(cuda, V, bf16):
 
 @pytest.mark.parametrize("bf16", [False, True])
 def test_log_sums_of_other_rows(cuda, bf16):
-    """Where the mass of a row lies within 16 of its largest logit a term's exponent is off by half a step of the difference
-    (below 16: 2^-21), half a step of its product with log2 e (below 23.1: 2^-20 ln 2), and log2 e's own 1.4e-8 of it: 1.4e-6;
-    the exponential by 2^-22, a thread's sums of at most 16 terms by 15 x 2^-24, the warps' and parts' weights by 2^-22 each:
-    3.1e-6 in all, below 2^-18 = 3.8e-6, if every rounding of the row falls to one side. One addition of 32 logits to 1 is the
-    lowest in the last two rows, so their mass is deep below the largest."""
+    """Where the mass of a row lies within 16 of its largest logit a term's exponent is off by half a step of the
+    difference (below 16: 2^-21), half a step of its product with log2 e (below 23.1: 2^-20 ln 2), and log2 e's own
+    1.4e-8 of it: 1.4e-6; the exponential by 2^-22, a thread's sums of at most 16 terms by 15 x 2^-24, the warps'
+    and parts' weights by 2^-22 each: 3.1e-6 in all, below 2^-18 = 3.8e-6, if every rounding of the row falls to
+    one side. In the last two rows nearly all of the mass lies equally deep below the one largest logit, where the
+    roundings do fall alike."""
     rng = np.random.default_rng(9)
     V = 151552
-    rows = [rng.standard_normal(V), rng.standard_normal(V) * 3, rng.uniform(-8, 0, V), np.linspace(-8, 8, V), np.linspace(8, -8, V),
-            np.linspace(0, 0.05, V), np.full(V, 2.7), rng.integers(-3, 3, V) * 1.1, np.repeat(rng.standard_normal(V // 32) * 2, 32)]
+    rows = [rng.standard_normal(V), rng.standard_normal(V) * 3, rng.uniform(-8, 0, V), np.linspace(-8, 8, V),
+            np.linspace(8, -8, V), np.linspace(0, 0.05, V), np.full(V, 2.7), rng.integers(-3, 3, V) * 1.1,
+            np.repeat(rng.standard_normal(V // 32) * 2, 32)]
     for depth in (5.3, 11.9):
         row = np.full(V, -depth)
         row[rng.integers(0, V)] = 0.0
@@ -231,9 +233,9 @@ def test_several_trees_in_flight(cuda):
 
 
 def test_a_node_past_the_selection_is_as_the_dense_decode(cuda):
-    """Behind a context that the indexer would choose from, `verify` takes the whole context only where it is told to; a chain
-    is then the dense decode of the same tokens, row by row (the attention is one operator's arithmetic, the recurrence's
-    closed form differs: the stage's chained bound, 6e-2)."""
+    """Behind a context that the indexer would choose from, `verify` takes the whole context only where it is told to;
+    a chain is then the dense decode of the same tokens, row by row (the attention is one operator's arithmetic,
+    the recurrence's closed form differs: the stage's chained bound, 6e-2)."""
     from ssengine_b200.messages import Chunk, Plan
     from ssengine_b200.stage import StageModel
 

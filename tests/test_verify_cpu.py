@@ -142,6 +142,8 @@ def test_each_step_in_flight_is_accepted_by_name_and_once(monkeypatch):
     for i, r in enumerate("abc"):
         st.verify(Plan(i, [Chunk(r, 3 + i, 3, [1], [20 * i + g for g in range(6)], True, [4, 5, 6])]), [[-1, 0, 0]])
         held[r] = st.trees
+    with pytest.raises(ValueError):
+        st.accept([[0, 1]])                                # three are open, and none is named
     st.accept([[0, 1]], trees=held["a"])
     assert st.trees is held["c"]
     with pytest.raises(ValueError):
@@ -169,7 +171,8 @@ def test_nodes_past_the_selection_are_refused_unless_dense(monkeypatch, kind):
     assert SELECTED_TOKENS == 4 * DsaAttention.TOPK + 3
     st = object.__new__(StageModel)
     st.trees, st.kda, st.device, st.cfg = None, True, torch.device("cpu"), SimpleNamespace(layer_kind=kind)
-    monkeypatch.setattr(st, "prepare", lambda plan: SimpleNamespace(order=[0, 1], last_rows=None, dsa=None), raising=False)
+    batch = lambda plan: SimpleNamespace(order=[0, 1], last_rows=None, dsa=None)
+    monkeypatch.setattr(st, "prepare", batch, raising=False)
     monkeypatch.setattr(st, "run", lambda *a, **kw: "rows", raising=False)
     trees = [[-1, -1], [-1, 0, 0, 1]]                       # the second is three nodes deep
     at = lambda start: Plan(0, [Chunk(r, n, len(t), [1], [0] * 6, True, [0] * len(t))
@@ -184,3 +187,28 @@ def test_nodes_past_the_selection_are_refused_unless_dense(monkeypatch, kind):
     assert st.verify(at(2049), trees, attention="dense") == "rows" and st.trees.reach == 2052
     with pytest.raises(ValueError):
         st.verify(at(5), trees, attention="none")
+
+
+def test_a_second_verify_of_a_request_ends_the_first(monkeypatch):
+    """Its nodes took the cache rows of the first one's."""
+    from ssengine_b200.messages import Chunk, Plan
+    from ssengine_b200.stage import StageModel
+
+    st = object.__new__(StageModel)
+    st.trees, st.kda, st.device = None, True, torch.device("cpu")
+    st.layers = st.is_dsa = st.kda_states = st.kda_group = []
+    batch = lambda plan: SimpleNamespace(order=list(range(len(plan.chunks))), last_rows=None, dsa=None)
+    monkeypatch.setattr(st, "prepare", batch, raising=False)
+    monkeypatch.setattr(st, "run", lambda *a, **kw: None, raising=False)
+
+    def verify(names):
+        st.verify(Plan(0, [Chunk(r, 3, 2, [1], [0] * 6, True, [4, 5]) for r in names]), [[-1, 0]] * len(names))
+        return st.trees
+
+    ab, c, b = verify("ab"), verify("c"), verify("b")
+    with pytest.raises(ValueError):
+        st.accept([[0], [0]], trees=ab)
+    st.accept([[0]], trees=c)
+    with pytest.raises(ValueError):                          # a step that is refused takes no rows
+        st.verify(Plan(0, [Chunk("b", 3, 2, [1], [0] * 6, True, [4, 5])]), [[-1, 5]])
+    st.accept([[0]], trees=b)
