@@ -17,7 +17,10 @@ MAX_BEAMS, MAX_K = 64, 64
 @functools.cache
 def workspace_bytes(requests: int, beams: int, vocab: int, k: int) -> int:
     """Device bytes of the workspace of one `select` call (`ssb_beam_workspace_bytes`)."""
-    n = lib.load().ssb_beam_workspace_bytes(requests, beams, vocab, k)
+    so = lib.load()
+    # what an int32 argument would cut off is refused here
+    fits = 1 <= beams <= MAX_BEAMS and 1 <= k <= MAX_K
+    n = so.ssb_beam_workspace_bytes(requests, beams, vocab, k) if fits else -1
     if n < 0:
         raise ValueError(f"bad beam workspace query: {requests} requests x {beams} beams (1..{MAX_BEAMS}), vocabulary "
                          f"{vocab}, k={k} (1..{MAX_K})")
@@ -56,6 +59,8 @@ def select(logits: torch.Tensor, scores: torch.Tensor, k: int, finished: torch.T
         out = (torch.empty(G, k, dtype=torch.float32, **dev), torch.empty(G, k, dtype=torch.int32, **dev),
                torch.empty(G, k, dtype=torch.int64, **dev))
     else:
+        if len(out) != 3:
+            raise ValueError(f"out: three tensors, got {len(out)}")
         for t, dtype in zip(out, (torch.float32, torch.int32, torch.int64)):
             if t.dtype is not dtype or t.shape != (G, k) or not t.is_contiguous():
                 raise ValueError(f"out: contiguous {dtype} {(G, k)}, got {t.dtype} {tuple(t.shape)}")

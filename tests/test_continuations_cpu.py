@@ -262,3 +262,17 @@ def test_beam_rows_are_cut_into_what_runs_at_once():
     for G, B, k in ((1, 4, 4), (2, 4, 4), (4, 8, 8), (16, 4, 4), (16, 8, 8), (37, 4, 1), (64, 8, 8), (148, 4, 16)):
         most = max(148 * 3, G * B)
         assert beam.workspace_bytes(G, B, 151552, k) <= most * (8 * k + 16) + 512, (G, B, k)
+
+
+@pytest.mark.parametrize("over", [
+    dict(k=(1 << 32) + 4), dict(k=-(1 << 32) + 4), dict(out=(torch.zeros(2, 4), torch.zeros(2, 4, **I32))),
+])
+def test_beam_refuses_what_its_arguments_cannot_hold(over):
+    """A k that 32 bits cut to a fair one, outputs that are not three."""
+    from ssengine_b200 import beam
+
+    with pytest.raises(ValueError):
+        beam.select(**beam_args(**over))
+    if "k" in over:
+        with pytest.raises(ValueError):
+            beam.workspace_bytes(2, 3, 50, over["k"])
