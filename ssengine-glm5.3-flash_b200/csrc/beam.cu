@@ -59,14 +59,6 @@ SSB_DEVICE uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-// e^d, d <= 0: 2^(d log2 e) with the product's rounding error carried to first order (ex2.approx's 2^-22 remains).
-SSB_DEVICE float exp_neg(float d) {
-  constexpr float kHi = 1.44269502162933349609375f, kLo = 1.925963033500928e-8f;        // log2 e in two parts
-  const float t = d * kHi;
-  const float r = fmaf(d, kLo, fmaf(d, kHi, -t));
-  const float y = ex2(t);
-  return fmaf(y, fminf(fmaxf(r, -1.0f), 1.0f) * 0.6931471805599453f, y);
-}
 
 // The k largest of the keys that the lanes hold (R each, 0: none; distinct) to out, in order; how many there are.
 template <int R>
@@ -332,7 +324,7 @@ __global__ void __launch_bounds__(kScanThreads, kScanBlocks) beam_scan_kernel(co
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
   const double z = lane < kScanWarps ? ws[lane] : 0.0;
-  double part_sum = m > -INFINITY ? z * exp_neg(m - t) : z;  // without a reference the sum is 0, or NaN
+  double part_sum = m > -INFINITY ? z * exp_fast(m - t) : z;  // without a reference the sum is 0, or NaN
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) part_sum += __shfl_xor_sync(0xffffffffu, part_sum, o);
   if (lane == 0) a.part[row * a.parts + part] = {part_sum, t};
@@ -407,7 +399,7 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       const auto term = [&](const BeamPart& p) {
-        return p.m > -INFINITY || p.sum != p.sum ? p.sum * exp_neg(p.m - m) : 0.0;
+        return p.m > -INFINITY || p.sum != p.sum ? p.sum * exp_fast(p.m - m) : 0.0;
       };
       double z = 0.0;
 #pragma unroll

@@ -44,6 +44,19 @@ SSB_DEVICE void raise_status(int32_t* status, int32_t code) {
 
 SSB_DEVICE uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
+// e^x as 2^(x log2 e) with the product's rounding error carried to first order: ex2.approx's own error (2^-22) remains.
+// x above 88 counts as 88 (e^x must stay finite, or its correction is inf - inf): as a divisor e^88 makes the quotients
+// below 0, as they are there to 2^-126. NaN stays NaN.
+SSB_DEVICE float exp_fast(float x) {
+  x = x > 88.0f ? 88.0f : x;
+  constexpr float kHi = 1.44269502162933349609375f, kLo = 1.925963033500928e-8f;        // log2 e in two parts
+  const float t = x * kHi;
+  const float r = fmaf(x, kLo, fmaf(x, kHi, -t));
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t));
+  return fmaf(y, fminf(fmaxf(r, -1.0f), 1.0f) * 0.6931471805599453f, y);
+}
+
 // ---- mbarrier ---------------------------------------------------------------------------------------------------
 SSB_DEVICE void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));

@@ -1,5 +1,5 @@
-// What the recurrent forms of the KDA layer share (kda_decode.cu, kda_tree.cu): short exponentials and the checks of a
-// call's arguments.
+// What the recurrent forms of the KDA layer share (kda_decode.cu, kda_tree.cu): short quotients and the checks of a call's
+// arguments.
 #pragma once
 
 #include "common.cuh"
@@ -7,18 +7,6 @@
 
 namespace ssb {
 
-// e^x as 2^(x log2 e) with the product's rounding error carried to first order: ex2.approx's own error (2^-22) remains.
-// x above 88 counts as 88 (e^x must stay finite, or its correction is inf - inf): as a divisor e^88 makes the quotients
-// below 0, as they are there to 2^-126. NaN stays NaN.
-SSB_DEVICE float exp_fast(float x) {
-  x = x > 88.0f ? 88.0f : x;
-  constexpr float kHi = 1.44269502162933349609375f, kLo = 1.925963033500928e-8f;        // log2 e in two parts
-  const float t = x * kHi;
-  const float r = fmaf(x, kLo, fmaf(x, kHi, -t));
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t));
-  return fmaf(y, fminf(fmaxf(r, -1.0f), 1.0f) * 0.6931471805599453f, y);
-}
 SSB_DEVICE float sigmoid_fast(float z) { return __fdividef(1.0f, 1.0f + exp_fast(-z)); }
 SSB_DEVICE float silu_fast(float y) { return __fdividef(y, 1.0f + exp_fast(-y)); }
 SSB_DEVICE float2 bf2(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
