@@ -2,20 +2,23 @@
 //   score[b] + x[b, v] - log sum_v exp x[b, v]
 // in order, equal ones by the lower b V + v. One pass over the logits.
 //
-// scan: a CTA has one part of one beam's row, 16 bytes a load. Each warp keeps a sum of exponentials against the largest logit
-//   that it has seen, so that this one's term is exactly 1 and no term's exponent is large where the term is: in 32 bits over
-//   the terms of one iteration (at most 32 of a lane), in 64 beyond. A new largest logit, a handful a row, rescales the sum
-//   by an exponential in 64 bits. Beside it the k largest (logit, token) as 64-bit keys whose order is that of the candidates (equal logits: the lower token is
-//   larger). A load's largest logit is compared with a bound of the CTA's k-th largest: the least of its 8 warps' ceil(k / 8)-th
-//   largest, at first of the lanes' maxima over their first loads, then of the lists. What is not below goes to the warp's
-//   list in shared memory, cut back to its k largest when it is full or the logits seen are four times as many. The CTA
-//   leaves k keys, the reference and the sum.
+// scan: a CTA has one part of one beam's row, 16 bytes a load. Each warp keeps a sum of exponentials against the
+//   largest logit that it has seen, so that this one's term is exactly 1 and no term's exponent is large where the term
+//   is: in 32 bits over the terms of one iteration (at most 32 of a lane), in 64 beyond. A new largest logit, a handful
+//   a row, rescales the sum by an exponential in 64 bits. Beside it the k largest (logit, token) as 64-bit keys whose
+//   order is that of the candidates (equal logits: the lower token is larger). A load's largest logit is compared with
+//   a bound of the CTA's k-th largest: the least of its 8 warps' ceil(k / 8)-th largest, at first of the lanes' maxima
+//   over their first loads, then of the lists. What is not below goes to the warp's list in shared memory, cut back to
+//   its k largest when it is full or the logits seen are four times as many. The CTA leaves k keys, the reference and
+//   the sum.
 // join: a CTA a request: the rows' log sums, then every candidate's score in 64 bits (a beam's own candidates keep the order
 //   of their logits, those of different beams are compared at the sums' accuracy). The candidates at or above the best
 //   part's k-th go to shared memory and each finds its place by counting those before it.
-// Bound: HBM, a read of the logits. 64 requests x 8 beams over 151,552 fp32 logits, a fifth of the beams finished: 64 us, 0.75
-// of the copy rate; a row is one part there, and its list work and the rows' uneven ends are not behind other CTAs' loads.
-// One request of 4 beams: 13 us, two launches and a row's parts over the card.
+// Bound: HBM, a read of the logits. 64 requests x 8 beams over 151,552 fp32 logits, a fifth of the beams finished
+// (their logits are not read): 64 us, 0.61 of the copy rate, 61 in a graph; a row is one part there, and its list work
+// and the rows' uneven ends are not behind other CTAs' loads. With none finished 91 us, 0.52: 512 rows on 444 places;
+// bf16 logits 83; k = 16 110; rows that do not lie on 16 bytes, which come by plain loads, 240 (bf16 144). One request
+// of 4 beams: 13 us, two launches and a row's parts over the card.
 #include "common.cuh"
 #include "ops.h"
 
@@ -330,7 +333,7 @@ __global__ void __launch_bounds__(kScanThreads, kScanBlocks) beam_scan_kernel(co
   if (lane == 0) a.part[row * a.parts + part] = {part_sum, t};
   uint64_t* out = a.keys + (row * a.parts + part) * a.k;
   int n = 0;
-  if (a.k <= 8) {
+  if (a.k <= 8) {                                            // 64 keys, not 512: 1 x 4 beams 13.1 us instead of 13.7
     uint64_t mine[kScanWarps * 8 / 32];
 #pragma unroll
     for (int j = 0; j < kScanWarps * 8 / 32; ++j) {
@@ -487,11 +490,11 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
   }
 }
 
-// Parts a row is cut into, the same for every row (equal rows get equal sums) and on every device: as many as run at once, none
-// short, the candidates of a request within bounds. Every part begins and ends with its lists, so a second wave costs more
-// than it evens out: cut for 592 CTAs instead of 444, 2 x 4 beams take 19.3 us instead of 14.2, 4 x 8 28.8 (22.6), 16 x 4
-// 34.0 (26.9); where rows alone fill the SMs, 64 x 8 beams, one part a row takes 91 us, two 96, four 114, and with a fifth
-// finished 61, 77 and 96 (rows that do not lie on 16 bytes: 240, 198 and 201).
+// Parts a row is cut into, the same for every row (equal rows get equal sums) and on every device: as many as run at
+// once, none short, the candidates of a request within bounds. Every part begins and ends with its lists, so a second
+// wave costs more than it evens out: cut for 592 CTAs instead of 444, 2 x 4 beams take 19.3 us instead of 14.2, 4 x 8
+// 28.8 (22.6), 16 x 4 34.0 (26.9); where rows alone fill the SMs, 64 x 8 beams, one part a row takes 91 us, two 96,
+// four 114, and with a fifth finished 61, 77 and 96 (rows that do not lie on 16 bytes: 240, 198 and 201).
 constexpr int kAtOnce = 148 * kScanBlocks;
 int beam_parts(int64_t G, int64_t B, int64_t V, int64_t k) {
   const int64_t rows = G * B;

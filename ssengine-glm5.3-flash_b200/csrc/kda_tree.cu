@@ -9,7 +9,7 @@
 // and, since the u are linear in the w with scalars of the path alone, o_i = S (A_i q_i) + sum_{j on the path} P_ij w_j with
 // P_i (1 + b M) = N_i b: a substitution up each node's path, on scalars. So the state S [value, key] is read once, whatever
 // the nodes, no node's own state is formed, and nothing but the scalars goes node after node. The decays multiply up the
-// path (each is at most 1; quotients of cumulated ones would overflow).
+// path: each is at most 1, so any depth is safe.
 //
 // One CTA a (request, head), two or four an SM:
 //   conv: a warp a node, 4 channels a lane, of q or k, late of v; gates: a thread a pair of channels of every fourth (eighth)
@@ -23,7 +23,9 @@
 // The exponentials are the short ones (error about 2^-20 here): nothing computed here is kept but the bf16 outputs.
 //
 // Bound: not HBM (a head's state is read once, 64 KB, whatever the nodes) but the vectors' arithmetic and the pairs, which
-// are on no tensor core: the decays between two nodes cannot be split into a factor of each without overflow. 48 trees of 32
+// are on no tensor core. They could be one product in shallow trees: with C the log decays summed along a path, the decays
+// between i and j are exp(C_i + c) exp(-(C_j + c)), factors that fp32 and bf16 hold while |lower_bound| times the depth stays
+// below about 170 (30 levels and more at -5); deeper ones need this walk. Not built. 48 trees of 32
 // to 64 nodes x 64 heads: 262 to 264 us (61 us of bytes), 53,000 warp instructions a CTA (pairs 11,000, conv 14,000, decays
 // and norms 9,000, the rest tree, state, scalars and outputs), issue slots 60 % in use, the rest waits for barriers, shared
 // memory and the state. 16 trees of 16 to 32 nodes 57 us (15), one tree of 24 nodes, 32 heads 13 us (latency). Each node's
@@ -754,8 +756,8 @@ int launch_kda_tree(const KdaArgs& a, cudaStream_t stream) {
   const auto set = [] { return set_smem<16>() && set_smem<32>() && set_smem<64>(); };
   if (cudaGetDevice(&device) != cudaSuccess || !attr.done(device, set)) return kErrCuda;
   if (a.max_nodes <= 16) return launch_nodes<16>(a, stream);
-  // up to 32 nodes four smaller CTAs an SM, unless the larger ones all run at once: 1 x 24 nodes, 32 heads 15.6 and 13.9 us,
-  // 4 x 24, 64 heads 19.7 and 19.1, 6 x 24, 64 heads 24.2 and 29.8
+  // up to 32 nodes four smaller CTAs an SM, unless the larger ones all run at once: 1 x 24 nodes, 32 heads 13.7 and 11.6 us,
+  // 4 x 24, 64 heads 22.3 and 21.2, 4 x 32 24.9 and 23.6, 6 x 24 27.3 and 30.3, 8 x 32 38.7 and 42.8
   const bool at_once = a.R * (int64_t)a.H <= Shape<64>::kBlocks * (int64_t)device_sm_count();
   if (a.max_nodes <= 32 && !at_once) return launch_nodes<32>(a, stream);
   return launch_nodes<64>(a, stream);

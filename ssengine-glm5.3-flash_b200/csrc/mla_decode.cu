@@ -34,12 +34,14 @@
 // in short bursts). Which role holds the rest is not shown. 32 rows of 128 to 32,768 tokens 81 us in a burst, 92 sustained;
 // 1 x 131,072 tokens 42 us; 1 x 1,000 tokens 18 us, of which the plan is 1.3, the query's staging 5.5, the unit and its
 // products 4.5, the parts' stores 2.3 and the join 4.
-// Tree form (kTree): a row is a drafted token; it sees its request's context and, of the 64 tokens behind, those of its word.
-// What bounds it is the unit's pace again: each row of 64 heads is a tile that reads the pages anew, from L2, at 1,940 cycles
-// a unit. 24 rows x 4,001 tokens 35 us (plan and first query a third of it), 8 x 16-32 rows (median 8,192 tokens) 437 us,
-// 0.56 of the bf16 rate. Rows of few heads share a tile and its units: 20 x 6-12 rows of 16 heads, e4m3 queries 64 us, 111
-// with a tile a row. An e4m3 tile leaves half of the score product empty: 128 heads a tile would fill it, but their
-// accumulators (512 columns) leave no room in TMEM.
+// Tree form (kTree): a row is a drafted token; it sees its request's context and, of the 64 tokens behind, those of its
+// word. What bounds it is the unit's pace again: each row of 64 heads is a tile that reads the pages anew, from L2, at
+// 1,940 cycles a unit. 24 rows x 4,001 tokens 35 us (plan and first query a third of it), 8 x 16-32 rows (median 8,192
+// tokens) 437 us, 0.56 of the bf16 rate; the e4m3 queries of 64 heads that a stage packs 30.4 us for 32.7 (in a graph)
+// and 404 to 434 for 369 to 415 (in turn, with the clock under the power limit falling from run to run). Rows of few
+// heads share a tile and its units: 20 x 6-12 rows of 16 heads, e4m3 queries 64 us, 111 with a tile a row. An e4m3 tile
+// leaves half of the score product empty: 128 heads a tile would fill it, but their accumulators (512 columns) leave no
+// room in TMEM.
 // Measured against it (bursts): units of 128 tokens in two slots with a token and 16 heads a thread, whose block maxima
 // need warp reductions, 380 us at 64 x 32,768; one warp issuing both products 356 (its waits for scores and for weights
 // then follow one another); S of one unit 312. The roles' loops are kept small because they share 28 KB of instruction
