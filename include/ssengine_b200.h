@@ -348,7 +348,8 @@ int ssb_move_rows(const ssb_move_view* views, int32_t n_views, const int32_t* sr
                   int64_t groups, int32_t n, int32_t* status, void* stream);
 
 /* A beam search's selection for G requests of `beams` (1..64) beams: of the candidates (b, v) with score scores[g, b] +
- * x[g, b, v] - log sum_v exp x[g, b, v] the k (1..64) best in order, equal scores by the lower b * V + v: their scores
+ * x[g, b, v] - log sum_v exp x[g, b, v] the k (1..64) best in order, equal scores by the lower b * V + v (a beam's own go by
+ * their logits, equal ones by the lower v, also where 64 bits of score do not tell two logits apart): their scores
  * (fp32), beams and tokens to out_scores, out_parents, out_tokens [G, k]. logits [G * beams, ld] fp32 or bf16 (bf16 = 1),
  * read once. Scores are compared in 64 bits and none is above its beam's. A log sum is right to 2^-18 at worst (rows of up to
  * 2^23 logits, or whose mass lies within 16 of their largest), to about 2^-22 as the roundings fall. A beam with

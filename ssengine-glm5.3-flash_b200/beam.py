@@ -30,14 +30,14 @@ def workspace_bytes(requests: int, beams: int, vocab: int, k: int) -> int:
 def select(logits: torch.Tensor, scores: torch.Tensor, k: int, finished: torch.Tensor | None = None, pad: int = 0,
            out: tuple | None = None, workspace: torch.Tensor | None = None, stream=None) -> tuple:
     """The k best continuations of each request's beams: of the candidates (b, v) with score scores[g, b] + logits[g *
-    B + b, v] - log sum exp of that row the k best in order, equal ones by the lower b * V + v. logits fp32 or bf16
-    [G * B, V] with unit column stride, scores fp32 [G, B] (the beams' log probabilities so far; B 1..64; -inf: a
-    beam that is not there), k 1..64 -> (scores fp32 [G, k], parents int32 [G, k]: the beam continued, tokens int64
-    [G, k]), new tensors or the three of `out` (with k == B the first may be `scores` itself). A beam with
-    finished[g, b] (bool or uint8 [G, B]) has one candidate: token `pad` at its own score, its logits not read. A
-    logit of -inf is no candidate; nor is any of a beam whose score or log sum is infinite or NaN. Places without a
-    candidate get -inf, -1, -1. `workspace`: uint8, `workspace_bytes(G, B, V, k)` (default: one kept per stream, or
-    in a capture one of the graph's own)."""
+    B + b, v] - log sum exp of that row the k best in order, equal ones by the lower b * V + v (a beam's own by
+    their logits). logits fp32 or bf16 [G * B, V] with unit column stride, scores fp32 [G, B] (the beams' log
+    probabilities so far; B 1..64; -inf: a beam that is not there), k 1..64 -> (scores fp32 [G, k], parents int32
+    [G, k]: the beam continued, tokens int64 [G, k]), new tensors or the three of `out` (with k == B the first may
+    be `scores` itself). A beam with finished[g, b] (bool or uint8 [G, B]) has one candidate: token `pad` at its
+    own score, its logits not read. A logit of -inf is no candidate; nor is any of a beam whose score or log sum is
+    infinite or NaN. Places without a candidate get -inf, -1, -1. `workspace`: uint8, `workspace_bytes(G, B, V, k)`
+    (default: one kept per stream, or in a capture one of the graph's own)."""
     so = lib.load()
     if scores.dtype is not torch.float32 or scores.dim() != 2 or not scores.is_contiguous():
         raise ValueError(f"scores: contiguous float32 [requests, beams], got {scores.dtype} {tuple(scores.shape)}")

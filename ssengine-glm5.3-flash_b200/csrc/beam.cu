@@ -11,14 +11,14 @@
 //   over their first loads, then of the lists. What is not below goes to the warp's list in shared memory, cut back to
 //   its k largest when it is full or the logits seen are four times as many. The CTA leaves k keys, the reference and
 //   the sum.
-// join: a CTA a request: the rows' log sums, then every candidate's score in 64 bits (a beam's own candidates keep the order
-//   of their logits, those of different beams are compared at the sums' accuracy). The candidates at or above the best
-//   part's k-th go to shared memory and each finds its place by counting those before it.
+// join: a CTA a request: the rows' log sums, then every candidate's score in 64 bits; a beam's own candidates keep the
+//   order of their logits, those of different beams are compared at the sums' accuracy. The candidates at or above the
+//   best part's k-th go to shared memory and each finds its place by counting those before it.
 // Bound: HBM, a read of the logits. 64 requests x 8 beams over 151,552 fp32 logits, a fifth of the beams finished
-// (their logits are not read): 64 us, 0.61 of the copy rate, 61 in a graph; a row is one part there, and its list work
-// and the rows' uneven ends are not behind other CTAs' loads. With none finished 91 us, 0.52: 512 rows on 444 places;
-// bf16 logits 83; k = 16 110; rows that do not lie on 16 bytes, which come by plain loads, 240 (bf16 144). One request
-// of 4 beams: 13 us, two launches and a row's parts over the card.
+// (their logits are not read): 62 us, 0.63 of the copy rate, 59 in a graph; a row is one part there, and its list work
+// and the rows' uneven ends are not behind other CTAs' loads. With none finished 89 us, 0.53: 512 rows on 444 places;
+// bf16 logits 81; k = 16 108; rows that do not lie on 16 bytes, which come by plain loads, 234 (bf16 140). One request
+// of 4 beams: 12 us, two launches and a row's parts over the card.
 #include "common.cuh"
 #include "ops.h"
 
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kScanThreads, kScanBlocks) beam_scan_kernel(co
   if (lane == 0) a.part[row * a.parts + part] = {part_sum, t};
   uint64_t* out = a.keys + (row * a.parts + part) * a.k;
   int n = 0;
-  if (a.k <= 8) {                                            // 64 keys, not 512: 1 x 4 beams 13.1 us instead of 13.7
+  if (a.k <= 8) {                                            // 64 keys, not 512: 1 x 4 beams 12.2 us instead of 12.8
     uint64_t mine[kScanWarps * 8 / 32];
 #pragma unroll
     for (int j = 0; j < kScanWarps * 8 / 32; ++j) {
@@ -355,8 +355,24 @@ __global__ void __launch_bounds__(kScanThreads, kScanBlocks) beam_scan_kernel(co
 
 struct Candidate {
   uint64_t score;                                // a double's bits in an order of its own: larger is better, 0 is none
-  uint64_t place;                                // beam, token: in the order of b V + v
+  uint32_t beam;
+  uint32_t at;                                   // its key's place in shared memory, kNoKey: a finished beam's
 };
+constexpr uint32_t kNoKey = 0xFFFFFFFFu;
+// The order of the result: scores, then beams, then a beam's keys. A beam's own candidates go by their logits and tokens also
+// where 64 bits of score do not tell them apart (logits near 0 beside the log sum), since its parts chose them so.
+struct Bound {
+  uint64_t score, key;
+  uint32_t beam;
+};
+// The best of the lanes' bounds.
+SSB_DEVICE Bound warp_best(const Bound& x) {
+  Bound r;
+  r.score = warp_max(x.score);
+  r.beam = __reduce_min_sync(0xffffffffu, x.score == r.score ? x.beam : kNoKey);
+  r.key = warp_max(x.score == r.score && x.beam == r.beam ? x.key : 0);
+  return r;
+}
 SSB_DEVICE uint64_t order_of(double x) {
   const uint64_t b = static_cast<uint64_t>(__double_as_longlong(x + 0.0));              // -0 counts as 0
   return b >> 63 ? ~b : b | 1ull << 63;
@@ -364,17 +380,12 @@ SSB_DEVICE uint64_t order_of(double x) {
 SSB_DEVICE double score_of(uint64_t o) {
   return __longlong_as_double(static_cast<int64_t>(o >> 63 ? o & ~(1ull << 63) : ~o));
 }
-// a before b in the result
-SSB_DEVICE bool before(const Candidate& a, const Candidate& b) {
-  return a.score > b.score || (a.score == b.score && a.place < b.place);
-}
-
 // Shared memory: the parts' keys, then room for every candidate.
 __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_constant__ BeamArgs a) {
   extern __shared__ __align__(16) uint64_t keys[];
   __shared__ double lse[kMaxBeams];              // the rows' log sums, NaN: the beam has no candidate of its logits
   __shared__ double given[kMaxBeams];            // the beams' scores
-  __shared__ Candidate bound[kJoinThreads / 32];
+  __shared__ Bound bound[kJoinThreads / 32];
   __shared__ uint64_t group[kJoinThreads / 32];
   __shared__ int32_t rank[kRanked];
   __shared__ int32_t count;
@@ -415,27 +426,24 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
     if (lane == 0) {
       given[b] = score;
       lse[b] = fabs(l) < INFINITY ? l : nan("");
-      if (finite && done) cand[atomicAdd(&count, 1)] = {order_of(score), static_cast<uint64_t>(b) << 32 | static_cast<uint64_t>(a.pad)};
+      if (finite && done) cand[atomicAdd(&count, 1)] = {order_of(score), static_cast<uint32_t>(b), kNoKey};
     }
   }
   __syncthreads();
   const auto get = [&](int i) {                  // candidate i, of score 0 where there is none
-    const int b = i / per;
+    const uint32_t b = i / per;
     const uint64_t key = keys[i];
-    Candidate c = {0, ~uint64_t{0}};
-    if (lse[b] == lse[b] && key != 0) {
-      c.score = order_of(given[b] + (static_cast<double>(key_logit(key)) - lse[b]));
-      c.place = static_cast<uint64_t>(b) << 32 | key_token(key);
-    }
+    Bound c = {0, 0, kNoKey};
+    if (lse[b] == lse[b] && key != 0) c = {order_of(given[b] + (static_cast<double>(key_logit(key)) - lse[b])), key, b};
     return c;
   };
   // Two bounds of the k-th best: the best k-th candidate of a part, and the least of k groups' best firsts (parts i, i + k,
   // ...). The first is tight where one part has most of the best, the second where they are spread.
   const int lists = a.B * a.parts;
-  Candidate bar = {0, ~uint64_t{0}};
+  Bound bar = {0, 0, kNoKey};
   for (int i = tid; i < lists; i += kJoinThreads) {
-    const Candidate c = get(i * a.k + a.k - 1);
-    if (before(c, bar)) bar = c;
+    const Bound c = get(i * a.k + a.k - 1);
+    if (c.score > bar.score || (c.score == bar.score && (c.beam < bar.beam || (c.beam == bar.beam && c.key > bar.key)))) bar = c;
   }
   uint64_t least = ~uint64_t{0};                 // of this warp's groups
   for (int j = warp; j < a.k; j += kJoinThreads / 32) {
@@ -443,21 +451,17 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
     for (int i = j + a.k * lane; i < lists; i += 32 * a.k) best = max(best, get(i * a.k).score);
     least = min(least, warp_max(best));
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const Candidate c = {__shfl_xor_sync(0xffffffffu, bar.score, o), __shfl_xor_sync(0xffffffffu, bar.place, o)};
-    if (before(c, bar)) bar = c;
-  }
+  bar = warp_best(bar);
   if (lane == 0) bound[warp] = bar, group[warp] = least;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kJoinThreads / 32; ++w) {
-    if (before(bound[w], bar)) bar = bound[w];
-    least = min(least, group[w]);
-  }
+  constexpr int kJoinWarps = kJoinThreads / 32;
+  bar = warp_best(bound[lane % kJoinWarps]);
+  least = ~warp_max(~group[lane % kJoinWarps]);
   for (int i = tid; i < total; i += kJoinThreads) {
-    const Candidate c = get(i);
-    if (c.score != 0 && c.score >= least && !before(bar, c)) cand[atomicAdd(&count, 1)] = c;
+    const Bound c = get(i);
+    if (c.score == 0 || c.score < least || c.score < bar.score) continue;
+    if (c.score == bar.score && (c.beam > bar.beam || (c.beam == bar.beam && c.key < bar.key))) continue;
+    cand[atomicAdd(&count, 1)] = {c.score, c.beam, static_cast<uint32_t>(i)};
   }
   __syncthreads();
   // a candidate's place: those before it, counted by kJoinThreads / kRanked threads
@@ -468,9 +472,20 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
     __syncthreads();
     if (i < n) {
       const Candidate c = cand[i];
-      int r = 0;
+      int r = 0, same = 0;
 #pragma unroll 4
-      for (int j = sharer; j < n; j += kJoinThreads / kRanked) r += before(cand[j], c);
+      for (int j = sharer; j < n; j += kJoinThreads / kRanked) {
+        const uint64_t x = cand[j].score;
+        r += x > c.score;
+        same += x == c.score;
+      }
+      if (same > (i % (kJoinThreads / kRanked) == sharer)) {           // others than itself
+        for (int j = sharer; j < n; j += kJoinThreads / kRanked) {
+          const Candidate x = cand[j];
+          if (x.score == c.score && x.beam != c.beam) r += x.beam < c.beam;
+          else if (x.score == c.score && x.at != c.at) r += keys[x.at] > keys[c.at];     // a finished beam has one candidate
+        }
+      }
       if (r > 0) atomicAdd(&rank[tid % kRanked], r);
     }
     __syncthreads();
@@ -478,8 +493,8 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
       const Candidate c = cand[i];
       const int64_t at = g * a.k + rank[tid];
       a.out_scores[at] = static_cast<float>(score_of(c.score));
-      a.out_parents[at] = static_cast<int32_t>(c.place >> 32);
-      a.out_tokens[at] = static_cast<int64_t>(c.place & 0xFFFFFFFFu);
+      a.out_parents[at] = static_cast<int32_t>(c.beam);
+      a.out_tokens[at] = c.at == kNoKey ? a.pad : static_cast<int64_t>(key_token(keys[c.at]));
     }
     __syncthreads();
   }
@@ -492,9 +507,9 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
 
 // Parts a row is cut into, the same for every row (equal rows get equal sums) and on every device: as many as run at
 // once, none short, the candidates of a request within bounds. Every part begins and ends with its lists, so a second
-// wave costs more than it evens out: cut for 592 CTAs instead of 444, 2 x 4 beams take 19.3 us instead of 14.2, 4 x 8
-// 28.8 (22.6), 16 x 4 34.0 (26.9); where rows alone fill the SMs, 64 x 8 beams, one part a row takes 91 us, two 96,
-// four 114, and with a fifth finished 61, 77 and 96 (rows that do not lie on 16 bytes: 240, 198 and 201).
+// wave costs more than it evens out: cut for 592 CTAs instead of 444, 2 x 4 beams take 18.3 us instead of 13.3, 4 x 8
+// 27.8 (21.7), 16 x 4 32.8 (25.4); where rows alone fill the SMs, 64 x 8 beams, one part a row takes 89 us, two 94,
+// four 113, and with a fifth finished 59, 75 and 94 (rows that do not lie on 16 bytes: 234, 193 and 197).
 constexpr int kAtOnce = 148 * kScanBlocks;
 int beam_parts(int64_t G, int64_t B, int64_t V, int64_t k) {
   const int64_t rows = G * B;

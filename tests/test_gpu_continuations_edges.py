@@ -131,6 +131,32 @@ def test_log_sums_of_other_rows(cuda, bf16):
     assert np.abs(err).max() <= 2.0 ** -18, err
 
 
+@pytest.mark.parametrize("scale", [1e-17, 1e-25, 1e-38])
+def test_a_beams_logits_that_its_scores_do_not_tell_apart(cuda, scale):
+    """Logits so small that score + logit - log sum is one number in 64 bits for all: the candidates are those of the
+    largest logits, in their order, equal ones by the lower token; of two beams the lower one's."""
+    rng = np.random.default_rng(3)
+    V, k = 6001, 12
+    x = (rng.integers(-4, 5, (2, V)) * scale).astype(np.float32)
+    x[0, rng.permutation(V)[:9]] = (rng.permutation(9) + 5) * np.float32(scale)
+    for rows, B in ((x, 2), (x[:1], 1)):
+        s, p, v = beam_run(cuda, rows, np.full((1, B), -1.0, np.float32), k)
+        want = np.lexsort((np.arange(V), -x[0].astype(np.float64)))[:k]
+        assert (p == 0).all() and (v[0] == want).all(), (v[0], want)
+        assert np.abs(s - (-1.0 - np.log(V))).max() <= 2.0 ** -18 + 2.0 ** -20
+
+
+def test_finished_beams_among_equal_scores(cuda):
+    """Rows of one candidate each, whose score is their beam's own: finished and live beams of one score in the order of
+    the beams."""
+    V = 4096
+    x = np.full((5, V), -np.inf, np.float32)
+    x[[0, 1, 2, 3, 4], [7, 4000, 0, 31, 5]] = [3.0, -2.0, 0.0, 1e4, 2.5]
+    s, p, v = beam_run(cuda, x, np.full((1, 5), -1.25, np.float32), 6, finished=np.array([[1, 0, 1, 0, 0]], np.uint8), pad=9)
+    assert p[0].tolist() == [0, 1, 2, 3, 4, -1] and v[0].tolist() == [9, 4000, 9, 31, 5, -1]
+    assert (s[0, :5] == -1.25).all() and s[0, 5] == -np.inf
+
+
 # ---- moves ----------------------------------------------------------------------------------------------------------
 
 
