@@ -217,7 +217,8 @@ class KdaAttention:
         return out
 
     def accept(self, step, rows, seqs, conv_state, rec_state, status, stream=None) -> None:
-        """Moves the states on along the accepted rows (int32 [n], `seqs` over places in them) of the trees that left `step`."""
+        """Moves the states on along the accepted rows (int32 [n], `seqs` over places in them) of the trees that left
+        `step`."""
         self.kda.advance(*step, rows, seqs, conv_state, rec_state, stream=stream, status=status)
 
 

@@ -160,6 +160,8 @@ class Trees:
     tensors of its rows (chunk by chunk in the plan's order: all are decode-class), and what each layer keeps of
     them for `accept` (`steps`, in layer order; None once they are accepted)."""
 
+    stage = staticmethod(lambda: None)  # a weak reference to the stage that verified them
+
     def __init__(self, chunks, trees, batch: Batch, device):
         from . import mla
 

@@ -154,6 +154,8 @@ def test_each_step_in_flight_is_accepted_by_name_and_once(monkeypatch):
     other.trees, other.kda = None, True
     with pytest.raises(ValueError):
         other.accept([[0]], trees=held["b"])
+    with pytest.raises(ValueError):
+        st.accept([[0], []], trees=trees_of([[-1, 0], [-1]])[0])          # no stage has verified these
     st.accept([[0]], trees=held["b"])
     st.accept([[0, 2]])
     assert took == [("a", [0, 1], [0, 2, 0, 1]), ("b", [0], [0, 1, 20, 1]), ("c", [0, 2], [0, 2, 40, 1])]
